@@ -36,6 +36,10 @@ extern "C" {
 #define LMOE_DTYPE_F16 1
 #define LMOE_DTYPE_F32 2
 
+/* Microscaled 4-bit formats (E2M1 values with one scale byte per block of columns). */
+#define LMOE_FP4_MX 0   /* blocks of 32, E8M0 (power-of-two) scales                  */
+#define LMOE_FP4_NV 1   /* blocks of 16, E4M3 scales under an fp32 tensor scale      */
+
 typedef struct CUstream_st* lmoe_stream_t; /* identical to cudaStream_t */
 
 /* Library version as 10000*major + 100*minor + patch. */
@@ -227,6 +231,72 @@ int lmoe_w4a16_grouped_gemm(const void* input, int64_t total_rows, int K, const 
                             int epilogue, const int32_t* dest_rows, const float* row_scale,
                             int64_t max_rows_per_expert, void* output, int64_t ldo,
                             void* workspace, size_t workspace_bytes, lmoe_stream_t stream);
+
+/* Gradients of lmoe_grouped_gemm, y[r, n] = sum_k input[r, k] * weights[e, n, k], for the rows
+ * [offsets[e], offsets[e + 1]) of expert e; dtype of all operands LMOE_DTYPE_* (bf16 and fp16 on
+ * tensor cores with fp32 accumulation, fp32 in fp32 on CUDA cores); any N, K >= 1.
+ *   dgrad: grad_input [total_rows, K] = grad_output [total_rows, N] * weights [E, N, K] of the
+ *          row's expert; rows outside every expert are zero
+ *   wgrad: grad_weights [E, N, K] (out_dtype: dtype or LMOE_DTYPE_F32), the sum over the
+ *          expert's rows of grad_output^T * input; experts without rows are zero
+ * 16-bit operands with row lengths that are multiples of 8 are read where they lie and must be
+ * 16-byte aligned; other row lengths are copied into the workspace first
+ * (lmoe_grouped_gemm_grad_workspace_bytes, 0 where no copy is made).
+ * error: a device word that the caller has zeroed, or NULL.  Offsets that decrease or leave
+ * [0, total_rows] set it, and every row then counts as outside every expert.
+ * The reference's backward is autograd through one mm_out per expert (csrc/grouped_gemm.cu:30-40,
+ * python/light_moe/ops/grouped_gemm.py:65-106). */
+size_t lmoe_grouped_gemm_grad_workspace_bytes(int weight_grad, int dtype, int64_t total_rows, int N, int K,
+                                              int num_experts);
+int lmoe_grouped_gemm_dgrad(const void* grad_output, int dtype, int64_t total_rows, int N, const void* weights, int K,
+                            const void* expert_offsets, int offsets_are_int64, int num_experts, void* grad_input,
+                            void* workspace, size_t workspace_bytes, uint32_t* error, lmoe_stream_t stream);
+int lmoe_grouped_gemm_wgrad(const void* grad_output, int dtype, int64_t total_rows, int N, const void* input, int K,
+                            const void* expert_offsets, int offsets_are_int64, int num_experts, int out_dtype,
+                            void* grad_weights, void* workspace, size_t workspace_bytes, uint32_t* error,
+                            lmoe_stream_t stream);
+
+/* ------------------------------------------------------------------------------------ */
+/* Microscaled 4-bit floating point.  A row of K values (K % 32 == 0) is K/2 bytes of E2M1   */
+/* codes (even column in the low nibble; code magnitudes 0, .5, 1, 1.5, 2, 3, 4, 6, sign in  */
+/* bit 3) and one scale byte per block; scale rows are lmoe_fp4_scale_pitch(K) bytes apart   */
+/* (K / block padded to a multiple of 32, the padding zero).                                 */
+/*   LMOE_FP4_MX: byte = clamp(floor(log2 max|x|) - 2, -127, 127) + 127, scale 2^(byte-127)   */
+/*   LMOE_FP4_NV: scale s * g, s = E4M3(max|x| / (6 g)) (at most 448), g the tensor scale     */
+/* code = x / scale to the nearest code, ties to even, at most 6 (0 where s is 0).            */
+/* A block with an infinity or a NaN (or a g that is not positive and finite) gets the NaN   */
+/* scale byte (255 / 127) and zero codes, so it reads as NaN.                                 */
+/* The reference has no 4-bit floating point.                                                 */
+/* ------------------------------------------------------------------------------------ */
+
+/* Bytes between scale rows, or LMOE_ERR_INVALID_ARG. */
+int lmoe_fp4_scale_pitch(int K, int format);
+
+/* x: [rows, K] of LMOE_DTYPE_*, rows ldx elements apart.  global_scale (LMOE_FP4_NV; NULL = 1):
+ * one fp32 value per rows_per_scale rows.  positions (optional): int32 [rows, copies], the output
+ * rows that row r is written to (entries outside [0, out_rows) are skipped); without it copies
+ * = 1 and out_rows = rows.  q [out_rows, K/2] 8-byte aligned; scales [out_rows, pitch]. */
+int lmoe_quantize_fp4(const void* x, int dtype, int64_t rows, int K, int64_t ldx, int format,
+                      const float* global_scale, int64_t rows_per_scale, const int32_t* positions, int copies,
+                      int64_t out_rows, uint8_t* q, uint8_t* scales, lmoe_stream_t stream);
+
+/* out: bf16 [rows, K], 16-byte aligned; scale rows scale_pitch bytes apart. */
+int lmoe_dequantize_fp4(const uint8_t* q, const uint8_t* scales, int64_t scale_pitch, int64_t rows, int K, int format,
+                        const float* global_scale, int64_t rows_per_scale, void* out, lmoe_stream_t stream);
+
+/* Grouped product of 4-bit operands: for the rows r of expert e
+ *   output[r, n] = alpha[e] * sum_k x[r, k] * w[e, n, k]                      (wq_up == NULL)
+ *   output[r, n] = silu(alpha[e] * x . w[e, n]) * (alpha_up[e] * x . up[e, n])   otherwise
+ * exact products, fp32 accumulation.  x: codes xq [total_rows, K/2], scales xs; w (and up): codes
+ * [E, N, K/2], scales [E, N, ws_pitch]; both operands of the same format, pitches multiples of 32
+ * and at least lmoe_fp4_scale_pitch, pointers 16-byte aligned.  alpha, alpha_up: fp32 [E] or NULL
+ * (1): the product of the two tensor scales.  output [total_rows, N] of out_dtype; rows outside
+ * every expert are zero.  error: as above. */
+int lmoe_fp4_grouped_gemm(const uint8_t* xq, const uint8_t* xs, int64_t xs_pitch, int64_t total_rows, int K,
+                          const uint8_t* wq, const uint8_t* ws, const uint8_t* wq_up, const uint8_t* ws_up,
+                          int64_t ws_pitch, int N, int format, const void* expert_offsets, int offsets_are_int64,
+                          int num_experts, const float* alpha, const float* alpha_up, int out_dtype, void* output,
+                          uint32_t* error, lmoe_stream_t stream);
 
 /* Weighted combine of per-slot expert rows back to tokens:
  *   y[t, :] = sum_j weights[t*top_k+j] * rows[positions[t*top_k+j], :]

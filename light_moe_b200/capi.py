@@ -23,6 +23,9 @@ LMOE_DTYPE_BF16 = 0
 LMOE_DTYPE_F16 = 1
 LMOE_DTYPE_F32 = 2
 
+LMOE_FP4_MX = 0
+LMOE_FP4_NV = 1
+
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _I64 = ctypes.c_int64
@@ -66,6 +69,14 @@ SIGNATURES = {
     "lmoe_grouped_gemm_bf16": (_I, [_P, _I64, _I, _P, _I, _P, _I, _I, _I, _P, _P, _SZ, _P]),
     "lmoe_w4a16_grouped_gemm": (_I, [_P, _I64, _I, _P, _I, _I, _P, _I, _I, _P, _I, _I, _P, _P, _I64, _P, _I64, _P,
                                      _SZ, _P]),
+    "lmoe_grouped_gemm_grad_workspace_bytes": (_SZ, [_I, _I, _I64, _I, _I, _I]),
+    "lmoe_grouped_gemm_dgrad": (_I, [_P, _I, _I64, _I, _P, _I, _P, _I, _I, _P, _P, _SZ, _P, _P]),
+    "lmoe_grouped_gemm_wgrad": (_I, [_P, _I, _I64, _I, _P, _I, _P, _I, _I, _I, _P, _P, _SZ, _P, _P]),
+    "lmoe_fp4_scale_pitch": (_I, [_I, _I]),
+    "lmoe_quantize_fp4": (_I, [_P, _I, _I64, _I, _I64, _I, _P, _I64, _P, _I, _I64, _P, _P, _P]),
+    "lmoe_dequantize_fp4": (_I, [_P, _P, _I64, _I64, _I, _I, _P, _I64, _P, _P]),
+    "lmoe_fp4_grouped_gemm": (_I, [_P, _P, _I64, _I64, _I, _P, _P, _P, _P, _I64, _I, _I, _P, _I, _I, _P, _P, _I, _P,
+                                   _P, _P]),
     "lmoe_combine_rows": (_I, [_P, _P, _P, _I64, _I, _I, _P, _I, _P, _P]),
     "lmoe_moe_layer_workspace_bytes": (_SZ, [_I64, _I, _I, _I, _I, _I]),
     "lmoe_moe_layer_w4a16": (_I, [_P, _I64, _I, _P, _P, _I, _I, _I, _P, _P, _I, _I, _P, _P, _P, _P, _SZ, _P]),

@@ -11,8 +11,11 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <optional>
+#include <string>
 #include <tuple>
+#include <vector>
 
 #include "lmoe_b200.h"
 
@@ -316,6 +319,284 @@ std::vector<torch::Tensor> moe_layer_w4a16(torch::Tensor x, torch::Tensor gate_w
   return {y, ids, wts};
 }
 
+// ---------------------------------------------------------------- gradients of grouped_gemm
+
+void check_same_device(const torch::Tensor& t, const torch::Tensor& like, const char* name) {
+  check_cuda(t, name);
+  TORCH_CHECK(t.device() == like.device(), name, " must be on ", like.device(), ", is on ", t.device());
+}
+
+// Row-contiguous and 16-byte aligned (a view may start anywhere).
+torch::Tensor contig16(const torch::Tensor& t) {
+  auto c = t.contiguous();
+  return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 == 0 ? c : c.clone();
+}
+
+torch::Tensor check_offsets(const torch::Tensor& offsets, const torch::Tensor& like, int64_t num_experts) {
+  check_same_device(offsets, like, "expert_offsets");
+  TORCH_CHECK(num_experts >= 1, "num_experts must be at least 1");
+  TORCH_CHECK(offsets.scalar_type() == torch::kInt64 || offsets.scalar_type() == torch::kInt32, "offsets int64/int32");
+  TORCH_CHECK(offsets.numel() >= num_experts + 1, "expert_offsets must have num_experts + 1 entries");
+  return offsets.contiguous();
+}
+
+void check_float(const torch::Tensor& t, const char* name) {
+  const auto st = t.scalar_type();
+  TORCH_CHECK(st == torch::kBFloat16 || st == torch::kFloat16 || st == torch::kFloat32, name,
+              " must be bf16, fp16 or fp32, is ", st);
+}
+
+torch::Tensor grouped_gemm_dgrad(torch::Tensor grad_output, torch::Tensor weights, torch::Tensor expert_offsets,
+                                 int64_t num_experts) {
+  check_cuda(grad_output, "grad_output");
+  check_same_device(weights, grad_output, "weights");
+  check_float(grad_output, "grad_output");
+  TORCH_CHECK(grad_output.dim() == 2 && weights.dim() == 3, "grad_output [T,N], weights [E,N,K]");
+  TORCH_CHECK(weights.size(0) >= num_experts && weights.size(1) == grad_output.size(1), "shape mismatch");
+  TORCH_CHECK(weights.scalar_type() == grad_output.scalar_type(), "grad_output and weights differ in dtype");
+  const c10::cuda::OptionalCUDAGuard guard(grad_output.device());
+  auto off = check_offsets(expert_offsets, grad_output, num_experts);
+  auto dy = contig16(grad_output);
+  auto w = contig16(weights);
+  const int64_t T = dy.size(0), N = w.size(1), K = w.size(2);
+  auto out = torch::empty({T, K}, dy.options());
+  const int dt = dtype_code(dy);
+  auto ws = workspace((int64_t)lmoe_grouped_gemm_grad_workspace_bytes(0, dt, T, (int)N, (int)K, (int)num_experts), dy);
+  check_status(lmoe_grouped_gemm_dgrad(dy.data_ptr(), dt, T, (int)N, w.data_ptr(), (int)K, off.data_ptr(),
+                                       off.scalar_type() == torch::kInt64, (int)num_experts, out.data_ptr(),
+                                       ws.data_ptr(), ws.numel(), nullptr, cur_stream()),
+               "grouped_gemm_dgrad");
+  return out;
+}
+
+torch::Tensor grouped_gemm_wgrad(torch::Tensor grad_output, torch::Tensor input, torch::Tensor expert_offsets,
+                                 int64_t num_experts, std::optional<torch::ScalarType> out_dtype) {
+  check_cuda(grad_output, "grad_output");
+  check_same_device(input, grad_output, "input");
+  check_float(grad_output, "grad_output");
+  TORCH_CHECK(grad_output.dim() == 2 && input.dim() == 2, "grad_output [T,N], input [T,K]");
+  TORCH_CHECK(grad_output.size(0) == input.size(0), "grad_output and input differ in rows");
+  TORCH_CHECK(input.scalar_type() == grad_output.scalar_type(), "grad_output and input differ in dtype");
+  const auto ot = out_dtype.value_or(grad_output.scalar_type());
+  TORCH_CHECK(ot == grad_output.scalar_type() || ot == torch::kFloat32, "out_dtype must be the operands' or float32");
+  const c10::cuda::OptionalCUDAGuard guard(grad_output.device());
+  auto off = check_offsets(expert_offsets, grad_output, num_experts);
+  auto dy = contig16(grad_output);
+  auto x = contig16(input);
+  const int64_t T = dy.size(0), N = dy.size(1), K = x.size(1);
+  auto out = torch::empty({num_experts, N, K}, dy.options().dtype(ot));
+  const int dt = dtype_code(dy);
+  auto ws = workspace((int64_t)lmoe_grouped_gemm_grad_workspace_bytes(1, dt, T, (int)N, (int)K, (int)num_experts), dy);
+  check_status(lmoe_grouped_gemm_wgrad(dy.data_ptr(), dt, T, (int)N, x.data_ptr(), (int)K, off.data_ptr(),
+                                       off.scalar_type() == torch::kInt64, (int)num_experts, dtype_code(out),
+                                       out.data_ptr(), ws.data_ptr(), ws.numel(), nullptr, cur_stream()),
+               "grouped_gemm_wgrad");
+  return out;
+}
+
+// ---------------------------------------------------------------- microscaled 4-bit operands
+
+int fp4_format(const std::string& format) {
+  TORCH_CHECK(format == "mxfp4" || format == "nvfp4", "format must be 'mxfp4' or 'nvfp4', is '", format, "'");
+  return format == "mxfp4" ? LMOE_FP4_MX : LMOE_FP4_NV;
+}
+int64_t fp4_block(int format) { return format == LMOE_FP4_MX ? 32 : 16; }
+
+// The tensor scale(s) of `x` [.., rows, K]: one value, or one per leading index of a 3-D tensor.
+// Returns the pointer and sets the rows that share a value.
+const float* fp4_global_scale(const std::optional<torch::Tensor>& g, const torch::Tensor& x, int64_t lead,
+                              int64_t rows, int format, int64_t* rows_per_scale) {
+  *rows_per_scale = 1;
+  if (!g.has_value() || !g->defined()) return nullptr;
+  TORCH_CHECK(format == LMOE_FP4_NV, "global_scale belongs to nvfp4");
+  check_same_device(*g, x, "global_scale");
+  TORCH_CHECK(g->scalar_type() == torch::kFloat32 && g->is_contiguous(), "global_scale must be contiguous fp32");
+  TORCH_CHECK(g->numel() == 1 || g->numel() == lead, "global_scale must have 1 or ", lead, " elements");
+  *rows_per_scale = std::max<int64_t>(1, g->numel() == 1 ? rows : rows / lead);
+  return g->data_ptr<float>();
+}
+
+std::tuple<torch::Tensor, torch::Tensor> quantize_fp4(torch::Tensor x, const std::string& format,
+                                                      std::optional<torch::Tensor> global_scale,
+                                                      std::optional<torch::Tensor> positions) {
+  check_cuda(x, "x");
+  check_float(x, "x");
+  const int fmt = fp4_format(format);
+  TORCH_CHECK(x.dim() >= 2, "x must be [..., rows, K]");
+  const int64_t K = x.size(-1);
+  TORCH_CHECK(K > 0 && K % 32 == 0 && K <= INT32_MAX, "K must be a positive multiple of 32");
+  const c10::cuda::OptionalCUDAGuard guard(x.device());
+  const bool strided = x.dim() == 2 && x.stride(1) == 1 && (x.size(0) <= 1 || x.stride(0) >= K);
+  auto xc = strided ? x : x.contiguous();
+  const int64_t rows = xc.numel() / K;
+  const int64_t ldx = strided && x.size(0) > 1 ? x.stride(0) : K;
+  int64_t rps = 1;
+  const float* g = fp4_global_scale(global_scale, x, x.dim() == 3 ? x.size(0) : 1, rows, fmt, &rps);
+  auto shape = x.sizes().vec();
+  torch::Tensor pos;
+  int64_t copies = 1, out_rows = rows;
+  if (positions.has_value() && positions->defined()) {
+    TORCH_CHECK(x.dim() == 2, "positions needs x [rows, K]");
+    check_same_device(*positions, x, "positions");
+    TORCH_CHECK(positions->scalar_type() == torch::kInt32, "positions must be int32");
+    TORCH_CHECK(rows == 0 ? positions->numel() == 0 : (positions->numel() % rows == 0 && positions->numel() > 0),
+                "positions must hold the same number of entries for each row");
+    pos = positions->contiguous();
+    copies = rows ? pos.numel() / rows : 1;
+    out_rows = pos.numel();
+    shape[0] = out_rows;
+  }
+  auto u8 = x.options().dtype(torch::kUInt8);
+  shape.back() = K / 2;
+  auto q = torch::empty(shape, u8);
+  shape.back() = lmoe_fp4_scale_pitch((int)K, fmt);
+  auto s = torch::empty(shape, u8);
+  if (rows > 0)
+    check_status(lmoe_quantize_fp4(xc.data_ptr(), dtype_code(xc), rows, (int)K, ldx, fmt, g, rps,
+                                   pos.defined() ? pos.data_ptr<int32_t>() : nullptr, (int)copies, out_rows,
+                                   q.data_ptr<uint8_t>(), s.data_ptr<uint8_t>(), cur_stream()),
+                 "quantize_fp4");
+  return {q, s.narrow(-1, 0, K / fp4_block(fmt))};
+}
+
+struct Fp4Operand {
+  torch::Tensor q, s;
+  int64_t pitch = 0;
+};
+
+// Codes contiguous and aligned; scale rows on a pitch of a multiple of 32 bytes with the whole
+// padded row inside the storage, copied to such rows if they are not.
+Fp4Operand fp4_operand(const torch::Tensor& q, const torch::Tensor& s, const torch::Tensor& like, int fmt, bool pad,
+                       const char* name) {
+  check_same_device(q, like, name);
+  check_same_device(s, like, name);
+  TORCH_CHECK(q.scalar_type() == torch::kUInt8 && s.scalar_type() == torch::kUInt8, name,
+              ": codes and scales must be uint8");
+  TORCH_CHECK(q.dim() >= 2 && q.dim() == s.dim(), name, ": codes [..., rows, K/2], scales [..., rows, K/block]");
+  const int64_t K = q.size(-1) * 2;
+  TORCH_CHECK(K > 0 && K % 32 == 0 && K <= INT32_MAX, name, ": K must be a positive multiple of 32");
+  for (int64_t i = 0; i + 1 < q.dim(); ++i) TORCH_CHECK(q.size(i) == s.size(i), name, ": scales shape mismatch");
+  TORCH_CHECK(s.size(-1) == K / fp4_block(fmt), name, ": scales shape mismatch");
+  Fp4Operand o;
+  o.q = contig16(q);
+  const int64_t padded = lmoe_fp4_scale_pitch((int)K, fmt);
+  const int64_t rows = q.numel() / (K / 2);
+  if (rows == 0) {
+    o.s = s;
+    o.pitch = padded;
+    return o;
+  }
+  // rows evenly spaced over all leading dimensions
+  bool even = s.size(-1) == 1 || s.stride(-1) == 1;
+  int64_t pitch = 0;   // of the innermost dimension with more than one row
+  int64_t span = 0;
+  for (int64_t i = s.dim() - 2; i >= 0 && even; --i) {
+    if (s.size(i) == 1) continue;
+    if (!pitch)
+      pitch = s.stride(i);
+    else
+      even = s.stride(i) == span;
+    span = s.stride(i) * s.size(i);
+  }
+  if (!pitch) pitch = padded;
+  const int64_t have = (int64_t)s.storage().nbytes() - s.storage_offset();
+  const bool fits = even && (reinterpret_cast<uintptr_t>(s.data_ptr()) % 16 == 0) &&
+                    (pad ? pitch % 32 == 0 && pitch >= padded && (rows - 1) * pitch + padded <= have
+                         : pitch >= s.size(-1));
+  if (fits) {
+    o.s = s;
+    o.pitch = pitch;
+  } else {
+    auto shape = s.sizes().vec();
+    shape.back() = padded;
+    o.s = torch::zeros(shape, s.options());
+    o.s.narrow(-1, 0, K / fp4_block(fmt)).copy_(s);
+    o.pitch = padded;
+  }
+  return o;
+}
+
+torch::Tensor dequantize_fp4(torch::Tensor q, torch::Tensor scales, const std::string& format,
+                             std::optional<torch::Tensor> global_scale) {
+  check_cuda(q, "q");
+  const int fmt = fp4_format(format);
+  const c10::cuda::OptionalCUDAGuard guard(q.device());
+  const Fp4Operand o = fp4_operand(q, scales, q, fmt, false, "q");
+  const int64_t K = q.size(-1) * 2, rows = q.numel() / (K / 2);
+  int64_t rps = 1;
+  const float* g = fp4_global_scale(global_scale, q, q.dim() == 3 ? q.size(0) : 1, rows, fmt, &rps);
+  auto shape = q.sizes().vec();
+  shape.back() = K;
+  auto out = torch::empty(shape, q.options().dtype(torch::kBFloat16));
+  if (rows > 0)
+    check_status(lmoe_dequantize_fp4(o.q.data_ptr<uint8_t>(), o.s.data_ptr<uint8_t>(), o.pitch, rows, (int)K, fmt, g,
+                                     rps, out.data_ptr(), cur_stream()),
+                 "dequantize_fp4");
+  return out;
+}
+
+const float* fp4_alpha(const std::optional<torch::Tensor>& alpha, const torch::Tensor& like, int64_t num_experts,
+                       const char* name) {
+  if (!alpha.has_value() || !alpha->defined()) return nullptr;
+  check_same_device(*alpha, like, name);
+  TORCH_CHECK(alpha->scalar_type() == torch::kFloat32 && alpha->is_contiguous() && alpha->numel() >= num_experts, name,
+              " must be contiguous fp32 with num_experts elements");
+  return alpha->data_ptr<float>();
+}
+
+torch::Tensor fp4_grouped_gemm(torch::Tensor input, torch::Tensor input_scales, torch::Tensor weights,
+                               torch::Tensor weight_scales, torch::Tensor expert_offsets, int64_t num_experts,
+                               const std::string& format, std::optional<torch::Tensor> alpha,
+                               std::optional<torch::Tensor> weights_up, std::optional<torch::Tensor> weight_scales_up,
+                               std::optional<torch::Tensor> alpha_up, std::optional<torch::ScalarType> out_dtype) {
+  check_cuda(input, "input");
+  const int fmt = fp4_format(format);
+  TORCH_CHECK(input.dim() == 2 && weights.dim() == 3, "input [T,K/2], weights [E,N,K/2]");
+  TORCH_CHECK(weights.size(0) >= num_experts && weights.size(2) == input.size(1), "shape mismatch");
+  const c10::cuda::OptionalCUDAGuard guard(input.device());
+  auto off = check_offsets(expert_offsets, input, num_experts);
+  const Fp4Operand x = fp4_operand(input, input_scales, input, fmt, true, "input");
+  const Fp4Operand w = fp4_operand(weights, weight_scales, input, fmt, true, "weights");
+  Fp4Operand u;
+  const bool swiglu = weights_up.has_value() && weights_up->defined();
+  TORCH_CHECK(swiglu == (weight_scales_up.has_value() && weight_scales_up->defined()),
+              "weights_up and weight_scales_up belong together");
+  TORCH_CHECK(swiglu || !(alpha_up.has_value() && alpha_up->defined()), "alpha_up needs weights_up");
+  Fp4Operand wp = w;
+  if (swiglu) {
+    TORCH_CHECK(weights_up->sizes() == weights.sizes(), "gate and up shapes differ");
+    u = fp4_operand(*weights_up, *weight_scales_up, input, fmt, true, "weights_up");
+    if (u.pitch != w.pitch) {   // one pitch for both: padded copies
+      const int64_t nb = weight_scales.size(-1), padded = lmoe_fp4_scale_pitch((int)(input.size(1) * 2), fmt);
+      for (Fp4Operand* o : {&wp, &u}) {
+        if (o->pitch == padded) continue;
+        auto shape = weight_scales.sizes().vec();
+        shape.back() = padded;
+        auto c = torch::zeros(shape, weight_scales.options());
+        c.narrow(-1, 0, nb).copy_(o == &wp ? weight_scales : *weight_scales_up);
+        o->s = c;
+        o->pitch = padded;
+      }
+    }
+  }
+  const int64_t T = input.size(0), K = input.size(1) * 2, N = weights.size(1);
+  const float* al = fp4_alpha(alpha, input, num_experts, "alpha");
+  const float* au = fp4_alpha(alpha_up, input, num_experts, "alpha_up");
+  const auto ot = out_dtype.value_or(torch::kBFloat16);
+  TORCH_CHECK(ot == torch::kBFloat16 || ot == torch::kFloat16 || ot == torch::kFloat32,
+              "out_dtype must be bf16, fp16 or fp32");
+  auto out = torch::empty({T, N}, input.options().dtype(ot));
+  if (T > 0 && N > 0)
+    check_status(lmoe_fp4_grouped_gemm(x.q.data_ptr<uint8_t>(), x.s.data_ptr<uint8_t>(), x.pitch, T, (int)K,
+                                       wp.q.data_ptr<uint8_t>(), wp.s.data_ptr<uint8_t>(),
+                                       swiglu ? u.q.data_ptr<uint8_t>() : nullptr,
+                                       swiglu ? u.s.data_ptr<uint8_t>() : nullptr, wp.pitch, (int)N, fmt,
+                                       off.data_ptr(), off.scalar_type() == torch::kInt64, (int)num_experts, al, au,
+                                       dtype_code(out), out.data_ptr(), nullptr, cur_stream()),
+                 "fp4_grouped_gemm");
+  return out;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -341,6 +622,19 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("group_size"), py::arg("epilogue") = 0, py::arg("dest_rows") = py::none(),
         py::arg("row_scale") = py::none(), py::arg("out_rows") = 0, py::arg("max_rows_per_expert") = 0,
         py::arg("segment_expert") = py::none());
+  m.def("grouped_gemm_dgrad", &grouped_gemm_dgrad, "Input gradient of grouped_gemm", py::arg("grad_output"),
+        py::arg("weights"), py::arg("expert_offsets"), py::arg("num_experts"));
+  m.def("grouped_gemm_wgrad", &grouped_gemm_wgrad, "Weight gradient of grouped_gemm", py::arg("grad_output"),
+        py::arg("input"), py::arg("expert_offsets"), py::arg("num_experts"), py::arg("out_dtype") = py::none());
+  m.def("quantize_fp4", &quantize_fp4, "Rows -> microscaled 4-bit floating point", py::arg("x"), py::arg("format"),
+        py::arg("global_scale") = py::none(), py::arg("positions") = py::none());
+  m.def("dequantize_fp4", &dequantize_fp4, "Microscaled 4-bit floating point -> bf16", py::arg("q"),
+        py::arg("scales"), py::arg("format"), py::arg("global_scale") = py::none());
+  m.def("fp4_grouped_gemm", &fp4_grouped_gemm, "Grouped GEMM of microscaled 4-bit operands", py::arg("input"),
+        py::arg("input_scales"), py::arg("weights"), py::arg("weight_scales"), py::arg("expert_offsets"),
+        py::arg("num_experts"), py::arg("format"), py::arg("alpha") = py::none(), py::arg("weights_up") = py::none(),
+        py::arg("weight_scales_up") = py::none(), py::arg("alpha_up") = py::none(),
+        py::arg("out_dtype") = py::none());
   m.def("combine_rows", &combine_rows, "Weighted combine of slot rows back to tokens", py::arg("rows"),
         py::arg("positions"), py::arg("weights"), py::arg("num_tokens"), py::arg("top_k"),
         py::arg("extra_rows") = py::none(), py::arg("num_extra") = 0);

@@ -1,0 +1,124 @@
+// fp4_format.cuh -- the microscaled 4-bit formats.
+//
+// Values are E2M1 codes (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign), two to a byte, the even
+// column in the low nibble.  Each block of consecutive columns of a row has one scale byte:
+//   LMOE_FP4_MX  blocks of 32, E8M0 scales 2^(byte - 127), byte 255 = NaN
+//                byte = clamp(floor(log2 max|x|) - 2, -127, 127) + 127
+//   LMOE_FP4_NV  blocks of 16, E4M3 scales under an fp32 tensor scale g
+//                s = E4M3(max|x| / (6 g)), at most 448
+// and a value is code(x / scale) * scale, rounded to the nearest code (ties to even), at most 6.
+// A block that holds an infinity or a NaN gets the NaN scale and zero codes.
+// Scale rows are padded to a multiple of 32 bytes, so that the product reads whole sectors.
+#pragma once
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include <cstdint>
+
+#include "lmoe_b200.h"
+
+namespace lmoe {
+
+__host__ __device__ constexpr int fp4_block(int format) { return format == LMOE_FP4_NV ? 16 : 32; }
+__host__ __device__ constexpr int fp4_scale_pitch(int K, int format) { return (K / fp4_block(format) + 31) / 32 * 32; }
+
+// Eight values -> eight codes (the first in the lowest nibble): round to nearest even, at most 6.
+__device__ __forceinline__ uint32_t fp4_pack8(const float* v) {
+  uint32_t r;
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
+      "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
+      : "=r"(r)
+      : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+  return r;
+}
+
+__device__ __forceinline__ float e8m0_value(uint32_t byte) {
+  return byte == 255u ? __uint_as_float(0x7fc00000u)
+                      : (byte == 0u ? __uint_as_float(0x00400000u) : __uint_as_float(byte << 23));
+}
+__device__ __forceinline__ float e4m3_value(uint32_t byte) {
+  return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)byte, __NV_E4M3)));
+}
+
+// Codes of 16 values of one row under one scale.  `a` holds the values; the block's largest
+// absolute value is `amax` (finite).  MX: the scale is a power of two, so x / scale is exact.
+// Returns the scale byte.
+__device__ __forceinline__ uint32_t fp4_encode_mx(const float (&a)[16], float amax, uint2& codes) {
+  const uint32_t bits = __float_as_uint(amax);
+  int e = (int)(bits >> 23) - 127 - 2;   // below the normal range: the clamp applies either way
+  e = e < -127 ? -127 : e;
+  const int up = -e;                     // multiply by 2^up, -125 <= up <= 127
+  const float m = __uint_as_float((uint32_t)(up + 127) << 23);
+  float t[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) t[i] = __fmul_rn(a[i], m);
+  codes.x = fp4_pack8(t);
+  codes.y = fp4_pack8(t + 8);
+  return (uint32_t)(e + 127);
+}
+
+// NV: s is the E4M3 value nearest to amax / (6 g).  The double quotient cannot land on the
+// wrong side of a midpoint: amax and midpoint * 6 g are integers of at most 31 bits in a common
+// unit, so they differ by more than 2^-32 relative or not at all.
+__device__ __forceinline__ float fp4_nv_scale(float amax, float g) {
+  const double t = (double)amax / (6.0 * (double)g);
+  if (t >= 448.0) return 448.0f;
+  const float tf = (float)t;
+  int e = (int)(__float_as_uint(tf) >> 23) - 127;
+  e = e < -6 ? -6 : e;
+  // a quotient just below a power of two may round up to it in fp32: the step is then twice the
+  // true one, but the nearest value is the power of two itself either way
+  const double step = (double)__uint_as_float((uint32_t)(e - 3 + 127) << 23);
+  const double inv = (double)__uint_as_float((uint32_t)(3 - e + 127) << 23);
+  return (float)(rint(t * inv) * step);
+}
+
+// Code of |x| by exact comparisons with the borders b * s * g between codes: b * s is exact in
+// fp32 and the fused multiply-add keeps the sign of (b * s) * g - |x|.
+__device__ __forceinline__ uint32_t fp4_exact_code(float x, float s, float g) {
+  const float ax = fabsf(x);
+  uint32_t c = 0;
+  c += __fmaf_rn(0.25f * s, g, -ax) < 0.0f;    // ties go to the even code: > or >= in turn
+  c += __fmaf_rn(0.75f * s, g, -ax) <= 0.0f;
+  c += __fmaf_rn(1.25f * s, g, -ax) < 0.0f;
+  c += __fmaf_rn(1.75f * s, g, -ax) <= 0.0f;
+  c += __fmaf_rn(2.5f * s, g, -ax) < 0.0f;
+  c += __fmaf_rn(3.5f * s, g, -ax) <= 0.0f;
+  c += __fmaf_rn(5.0f * s, g, -ax) < 0.0f;
+  return c | (__float_as_uint(x) >> 31 << 3);
+}
+
+// The codes come from the rounded product with the reciprocal (three roundings, below 2^-21
+// relative); where a border lies that near, they come from fp4_exact_code.
+__device__ __forceinline__ uint32_t fp4_encode_nv(const float (&a)[16], float amax, float g, uint2& codes) {
+  const float s = fp4_nv_scale(amax, g);
+  codes = make_uint2(0u, 0u);
+  if (s > 0.0f) {
+    const float d = __fmul_rn(s, g);
+    const bool plain = d > 1e-30f && d < 1e30f;
+    const float r = __frcp_rn(plain ? d : 1.0f);
+    float lo[16], hi[16];
+    const float down = 1.0f - 0x1p-20f, upf = 1.0f + 0x1p-20f;
+    const float rl = __fmul_rn(r, down), rh = __fmul_rn(r, upf);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      lo[i] = __fmul_rn(a[i], rl);
+      hi[i] = __fmul_rn(a[i], rh);
+    }
+    codes.x = fp4_pack8(lo);
+    codes.y = fp4_pack8(lo + 8);
+    if (!plain || codes.x != fp4_pack8(hi) || codes.y != fp4_pack8(hi + 8)) {
+      uint32_t w[2] = {0u, 0u};
+#pragma unroll
+      for (int i = 0; i < 16; ++i) w[i >> 3] |= fp4_exact_code(a[i], s, g) << (4 * (i & 7));
+      codes = make_uint2(w[0], w[1]);
+    }
+  }
+  return (uint32_t)__nv_cvt_float_to_fp8(s, __NV_SATFINITE, __NV_E4M3);
+}
+
+}  // namespace lmoe

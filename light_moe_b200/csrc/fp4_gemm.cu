@@ -1,0 +1,566 @@
+// fp4_gemm.cu -- grouped product of microscaled 4-bit operands on CTA pairs (sm_100a).
+//
+//   y[r, n] = alpha[e] * sum_k x[r, k] * w[e, n, k]      for the rows r of expert e
+//   y[r, f] = silu(gate[r, f]) * up[r, f]                with a gate and an up matrix
+//
+// Both operands are E2M1 with a scale byte per 32 (MX) or 16 (NV) values (fp4_format.cuh); the
+// block-scaled tcgen05.mma multiplies codes and scales exactly and accumulates in fp32, four
+// times the bf16 rate for a quarter of the bytes.  With few rows the weights' bytes bound it
+// (HBM), with many the tensor pipe.
+//
+// Tile: 256 rows (128 per CTA, TMEM lane = row) x 192 weight rows (96 per CTA in shared memory).
+// 192 columns because two accumulators (2 x 192) and two buffers of scales (2 x 48 columns) fit
+// the 512 TMEM columns, so the epilogue of a tile overlaps the next tile's MMAs; 256 columns
+// would leave room for one accumulator only.  The lane being the row, a thread holds a row's
+// gate and up values of the same features, and the SwiGLU needs no exchange: for gate / up the
+// leader's 96 columns are gate rows and the follower's 96 the same rows of up.
+//
+// Operands stay in the canonical layout of the quantiser (codes [rows, K/2], scales [rows,
+// pitch]): the codes arrive by TMA (128-byte swizzle, 256 values = 128 bytes a row and stage).
+// The scales of a stage (8 or 16 bytes a row) must lie in shared memory as 512-byte tiles of
+// 128 rows x 4 scales, row r at (r % 32) * 16 + (r / 32) * 4, from where tcgen05.cp copies them
+// to TMEM; three warps read them as whole 32-byte sectors (four or two stages at a time, one
+// step ahead) and write the tiles with one 16-byte store per lane.
+//
+// Warps: 0 TMA producer; 1 MMA issuer (leader CTA); 2 scales of the rows; 3, 4 scales of the
+// columns 0-127 and 128-191 (each CTA keeps all 192: the MMA reads them beside its own rows);
+// 5-16 epilogue, twelve warps of 32 rows x 64 columns.
+// A stage is ready when, in both CTAs, the codes landed and the three scale warps wrote.
+#include <cuda_bf16.h>
+
+#include "fp4_format.cuh"
+#include "fp4_gemm.h"
+#include "host_util.h"
+#include "pair_gemm.cuh"
+
+namespace lmoe {
+namespace {
+
+constexpr int kRowsCta = 128, kTM = 256, kTN = 192, kHalf = 96;
+constexpr int kSK = 256;          // values per stage: one 128-byte swizzle line of codes
+constexpr int kStages = 6, kAcc = 2;
+constexpr int kEpiWarp0 = 5, kEpiWarps = 12;
+constexpr int kThreads = (kEpiWarp0 + kEpiWarps) * 32;
+constexpr uint32_t kABytes = kRowsCta * 128, kBBytes = kHalf * 128;
+constexpr uint32_t kSite = 0x500u;
+constexpr int kTmemCols = 512;
+
+struct Fp4Args {
+  const uint8_t* xs;     // scales of the rows
+  int64_t xs_pitch;
+  const uint8_t* ws;     // scales of the weights (gate), and of up
+  const uint8_t* ws_up;
+  int64_t ws_pitch;
+  const void* offsets;
+  int offsets_i64;
+  int E, N, K;
+  int64_t R;
+  int NB, KS;            // column tiles, stages
+  const float* alpha;    // per expert, or NULL
+  const float* alpha_up;
+  void* out;
+  int out_dtype;
+  int vec_out;
+  uint32_t* err;
+};
+
+struct __align__(8) Bars {
+  uint64_t full[kStages];       // this CTA's codes landed
+  uint64_t empty[kStages];      // the stage's MMAs finished (both CTAs)
+  uint64_t ready[kStages];      // leader: codes and scales of both CTAs
+  uint64_t acc_full[kAcc];
+  uint64_t acc_empty[kAcc];     // leader: both CTAs' epilogue warps
+  uint64_t mma_done;
+  uint32_t tmem_base;
+  int abort;
+  SegTable seg;
+};
+
+struct Tile {
+  int e, m, n, row0, row_end;
+  bool zero;   // rows outside every expert
+};
+
+__device__ __forceinline__ Tile tile_at(const SegTable& t, int E, int NB, int tile, int& hint) {
+  int j = hint;
+  while (tile >= t.tile_start[j + 1]) ++j;
+  hint = j;
+  Tile r;
+  const int rows = t.row[j + 1] - t.row[j];
+  raster(tile - t.tile_start[j], (rows + kTM - 1) / kTM, NB, r.m, r.n);
+  r.e = j - 1;
+  r.zero = j == 0 || j == E + 1;
+  r.row0 = t.row[j] + r.m * kTM;
+  r.row_end = t.row[j + 1];
+  return r;
+}
+
+// Instruction descriptor of the block-scaled kinds: E2M1 operands, K-major, M = 256, N = 192.
+__host__ __device__ constexpr uint32_t idesc_fp4(bool ue8m0, uint32_t sf_id) {
+  return (sf_id << 4) | (1u << 7) | (1u << 10) | ((kTN >> 3) << 17) | ((ue8m0 ? 1u : 0u) << 23) |
+         ((uint32_t)(kTM >> 4) << 24) | (sf_id << 29);
+}
+
+// Unswizzled descriptor of a 512-byte scale tile (32 rows of 16 bytes).
+__device__ __forceinline__ uint64_t sdesc_scales(uint32_t smem_addr) {
+  return (uint64_t)((smem_addr >> 4) & 0x3fffu) | ((uint64_t)(128u >> 4) << 32) | ((uint64_t)1u << 46);
+}
+
+__device__ __forceinline__ void copy_scales_pair(uint32_t taddr, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+
+template <int FORMAT>
+__device__ __forceinline__ void mma_fp4_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa,
+                                             uint32_t sfb, uint32_t accumulate) {
+  if constexpr (FORMAT == LMOE_FP4_MX)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(
+            d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
+}
+
+template <int FORMAT>
+struct Cfg {
+  static constexpr int kWords = FORMAT == LMOE_FP4_MX ? 2 : 4;       // 4-scale words a row and stage
+  static constexpr int kStagesPerLoad = 8 / kWords;                   // stages in a 32-byte sector
+  static constexpr uint32_t kSfABytes = kWords * 512, kSfBBytes = kWords * 1024;
+  static constexpr uint32_t kStageBytes = kABytes + kBBytes + kSfABytes + kSfBBytes;
+  static constexpr uint32_t kSfCols = kWords * 12;                    // TMEM columns: A 4, B 8 a word
+  static constexpr uint32_t kSmem = 1024 + kStages * kStageBytes + sizeof(Bars);
+  static_assert(kStageBytes % 1024 == 0, "swizzle atoms");
+  static_assert(kSmem <= 232448, "shared memory budget");
+  static_assert(kAcc * kTN + 2 * kSfCols <= kTmemCols, "tensor memory budget");
+};
+
+__device__ __forceinline__ float silu(float g) { return __fdividef(g, 1.0f + __expf(-g)); }
+
+template <int FORMAT, bool SWIGLU>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    fp4_gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_x32,
+                    const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_up,
+                    const Fp4Args a) {
+  using C = Cfg<FORMAT>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  Bars* bars = reinterpret_cast<Bars*>(base + kStages * C::kStageBytes);
+  volatile int* abort_flag = &bars->abort;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = rank == 0;
+
+  if (tid == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&bars->full[s], 1);
+      mbar_init(&bars->empty[s], 1);
+      mbar_init(&bars->ready[s], 6);
+    }
+    for (int s = 0; s < kAcc; ++s) {
+      mbar_init(&bars->acc_full[s], 1);
+      mbar_init(&bars->acc_empty[s], 2 * kEpiWarps);
+    }
+    mbar_init(&bars->mma_done, 1);
+    bars->abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(&bars->tmem_base, kTmemCols);
+    tmem_relinquish_pair();
+  }
+  load_segments(&bars->seg, a.offsets, a.offsets_i64, a.E, a.R, tid, kThreads);
+  const int segs = a.E + 2;
+  if (warp == 0)
+    scan_tiles(&bars->seg, segs, lane, [&](int j) {
+      return (bars->seg.row[j + 1] - bars->seg.row[j] + kTM - 1) / kTM * a.NB;
+    });
+  if (tid == 0 && bars->seg.bad && blockIdx.x == 0) report_error(a.err, kErrBadArg, kSite + 1);
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem = bars->tmem_base;
+  const SegTable& seg = bars->seg;
+  const int total = seg.tile_start[segs];
+  const int KS = a.KS;
+  const int first = blockIdx.x >> 1, stride = gridDim.x >> 1;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------ TMA producer
+    if (lane == 0) {
+      uint32_t it = 0;
+      int hint = 0;
+      bool ok = true;
+      for (int tile = first; tile < total && ok; tile += stride) {
+        const Tile t = tile_at(seg, a.E, a.NB, tile, hint);
+        if (t.zero) continue;
+        const int r0 = t.row0 + (int)rank * kRowsCta;
+        int rows = t.row_end - r0;
+        rows = rows < 0 ? 0 : (rows > kRowsCta ? kRowsCta : rows);
+        const int boxes = (rows + 31) >> 5;   // only the boxes that hold this tile's rows
+        const CUtensorMap* wmap = SWIGLU && !leader ? &tm_up : &tm_w;
+        const int wrow = SWIGLU ? t.n * kHalf : t.n * kTN + (int)rank * kHalf;
+        for (int ks = 0; ks < KS; ++ks, ++it) {
+          const int s = it % kStages;
+          if (!mbar_wait(&bars->empty[s], ((it / kStages) & 1u) ^ 1u, a.err, abort_flag, kSite + 2)) {
+            ok = false;
+            break;
+          }
+          uint8_t* st = base + s * C::kStageBytes;
+          mbar_arrive_expect_tx(&bars->full[s], (uint32_t)boxes * 4096u + kBBytes);
+          if (boxes == 4) {
+            tma_load_2d(st, &tm_x, &bars->full[s], ks * 128, r0);
+          } else {
+            for (int b = 0; b < boxes; ++b)
+              tma_load_2d(st + b * 4096, &tm_x32, &bars->full[s], ks * 128, r0 + b * 32);
+          }
+          tma_load_3d(st + kABytes, wmap, &bars->full[s], ks * 128, wrow, t.e);
+        }
+      }
+      // no copy of this CTA may still be in flight when it exits
+      const uint32_t from = it > (uint32_t)kStages ? it - kStages : 0u;
+      for (uint32_t j = from; j < it; ++j)
+        mbar_wait(&bars->full[j % kStages], (j / kStages) & 1u, a.err, nullptr, kSite + 3);
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ MMA issuer
+    if (leader && lane == 0) {
+      uint32_t it = 0, lt = 0;
+      int hint = 0;
+      bool ok = true;
+      for (int tile = first; tile < total && ok; tile += stride) {
+        const Tile t = tile_at(seg, a.E, a.NB, tile, hint);
+        if (t.zero) continue;
+        const uint32_t acc = lt % kAcc;
+        if (!mbar_wait_cluster(&bars->acc_empty[acc], ((lt / kAcc) & 1u) ^ 1u, a.err, abort_flag, kSite + 4)) break;
+        const uint32_t d = tmem + acc * kTN;
+        for (int ks = 0; ks < KS; ++ks, ++it) {
+          const int s = it % kStages;
+          // the scale buffer of this stage was last read by the MMAs of the stage before last
+          if (it >= 2 && !mbar_wait(&bars->empty[(it - 2) % kStages], ((it - 2) / kStages) & 1u, a.err, abort_flag,
+                                    kSite + 5)) { ok = false; break; }
+          if (!mbar_wait_cluster(&bars->ready[s], (it / kStages) & 1u, a.err, abort_flag, kSite + 6)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t st = smem_u32(base + s * C::kStageBytes);
+          const uint32_t sfa = tmem + kAcc * kTN + (it & 1u) * C::kSfCols, sfb = sfa + C::kWords * 4;
+#pragma unroll
+          for (int w = 0; w < C::kWords; ++w) {
+            copy_scales_pair(sfa + w * 4, sdesc_scales(st + kABytes + kBBytes + w * 512));
+            copy_scales_pair(sfb + w * 8, sdesc_scales(st + kABytes + kBBytes + C::kSfABytes + w * 1024));
+            copy_scales_pair(sfb + w * 8 + 4, sdesc_scales(st + kABytes + kBBytes + C::kSfABytes + w * 1024 + 512));
+          }
+          const int left = a.K - ks * kSK;
+          const int nk = left >= kSK ? 4 : (left + 63) / 64;   // 64 values per MMA
+          for (int kk = 0; kk < nk; ++kk) {
+            const uint32_t accum = (ks | kk) != 0 ? 1u : 0u;
+            const uint64_t ad = sdesc_k_sw128(st + kk * 32), bd = sdesc_k_sw128(st + kABytes + kk * 32);
+            if (FORMAT == LMOE_FP4_MX)
+              // a word holds the scales of 128 values: of two MMAs (scale id 0 and 2)
+              mma_fp4_pair<FORMAT>(d, ad, bd, idesc_fp4(true, (kk & 1) * 2), sfa + (kk >> 1) * 4, sfb + (kk >> 1) * 8,
+                                   accum);
+            else
+              mma_fp4_pair<FORMAT>(d, ad, bd, idesc_fp4(false, 0), sfa + kk * 4, sfb + kk * 8, accum);
+          }
+          mma_commit_pair(&bars->empty[s]);
+        }
+        if (ok) mma_commit_pair(&bars->acc_full[acc]);
+        ++lt;
+      }
+      mma_commit_pair(&bars->mma_done);
+      mbar_wait(&bars->mma_done, 0, a.err, nullptr, kSite + 7);
+    }
+  } else if (warp < kEpiWarp0) {
+    // ------------------------------------------------------------------ scales
+    const int part = warp - 2;   // 0: rows, 1: columns 0-127, 2: columns 128-191
+    const int nb = a.K / fp4_block(FORMAT);
+    const uint32_t dst0 = kABytes + kBBytes + (part == 0 ? 0u : C::kSfABytes + (part - 1) * 512u);
+    const uint32_t dst_word = part == 0 ? 512u : 1024u;
+    const int steps = (KS + C::kStagesPerLoad - 1) / C::kStagesPerLoad;   // 32-byte loads a row
+    const uint32_t ready_addr = mapa_u32(&bars->ready[0], 0);
+    // the lane's four rows (r = lane + 32 i) of a tile, NULL where there is none
+    auto sources = [&](const Tile& t, const uint8_t* (&p)[4]) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = lane + 32 * i;
+        p[i] = nullptr;
+        if (part == 0) {
+          const int row = t.row0 + (int)rank * kRowsCta + r;
+          if (row < t.row_end) p[i] = a.xs + (int64_t)row * a.xs_pitch;
+        } else {
+          const int c = r + (part - 1) * 128;
+          const bool up = SWIGLU && c >= kHalf;
+          const int n = SWIGLU ? t.n * kHalf + (up ? c - kHalf : c) : t.n * kTN + c;
+          if (c < kTN && n < a.N) p[i] = (up ? a.ws_up : a.ws) + ((int64_t)t.e * a.N + n) * a.ws_pitch;
+        }
+      }
+    };
+    auto load = [&](const uint8_t* (&p)[4], int step, uint4 (&v)[4][2]) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          v[i][h] = p[i] ? __ldg(reinterpret_cast<const uint4*>(p[i] + step * 32) + h) : make_uint4(0, 0, 0, 0);
+      }
+    };
+    uint32_t it = 0;
+    int hint = 0;
+    // the next load: tile and step
+    int ltile = first;
+    const uint8_t* lp[4];
+    auto next_tile = [&](int tile) {   // first non-empty tile at or behind `tile`
+      for (; tile < total; tile += stride) {
+        const Tile t = tile_at(seg, a.E, a.NB, tile, hint);
+        if (!t.zero) {
+          sources(t, lp);
+          break;
+        }
+      }
+      return tile;
+    };
+    ltile = next_tile(ltile);
+    int lstep = 0;
+    uint4 nxt[4][2];
+    if (ltile < total) load(lp, 0, nxt);
+    bool ok = true;
+    while (ltile < total && ok) {
+      uint4 cur[4][2];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        cur[i][0] = nxt[i][0];
+        cur[i][1] = nxt[i][1];
+      }
+      const int step = lstep;
+      if (++lstep == steps) {
+        lstep = 0;
+        ltile = next_tile(ltile + stride);
+      }
+      if (ltile < total) load(lp, lstep, nxt);
+      if ((step + 1) * 32 > nb) {
+        // scale bytes behind the last block are padding: zero, whatever they hold
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t* w = reinterpret_cast<uint32_t*>(&cur[i][0]);
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+            const int valid = nb - (step * 32 + q * 4);
+            if (valid < 4) w[q] = valid <= 0 ? 0u : (w[q] & ((1u << (8 * valid)) - 1u));
+          }
+        }
+      }
+#pragma unroll
+      for (int g = 0; g < C::kStagesPerLoad; ++g) {
+        if (step * C::kStagesPerLoad + g < KS && ok) {
+          const int s = it % kStages;
+          if (!mbar_wait(&bars->empty[s], ((it / kStages) & 1u) ^ 1u, a.err, abort_flag, kSite + 8)) ok = false;
+          ok = __all_sync(0xffffffffu, ok);
+          if (ok) {
+            uint8_t* st = base + s * C::kStageBytes + dst0 + lane * 16;
+#pragma unroll
+            for (int w = 0; w < C::kWords; ++w) {
+              const int q = g * C::kWords + w;   // word of the sector
+              uint32_t o[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const uint4 v = cur[i][q >> 2];
+                o[i] = (q & 3) == 0 ? v.x : (q & 3) == 1 ? v.y : (q & 3) == 2 ? v.z : v.w;
+              }
+              *reinterpret_cast<uint4*>(st + w * dst_word) = make_uint4(o[0], o[1], o[2], o[3]);
+            }
+            fence_proxy_async_smem();
+            if (part == 0 && !mbar_wait(&bars->full[s], (it / kStages) & 1u, a.err, abort_flag, kSite + 9)) ok = false;
+            ok = __all_sync(0xffffffffu, ok);
+            if (ok && lane == 0) mbar_arrive_cluster(ready_addr + s * 8);
+          }
+          ++it;
+        }
+      }
+    }
+  } else {
+    // ------------------------------------------------------------------ epilogue
+    const int q = warp & 3, cg = (warp - kEpiWarp0) >> 2;
+    const uint32_t lane_base = (uint32_t)(q * 32) << 16;
+    const uint32_t empty_addr = mapa_u32(&bars->acc_empty[0], 0);
+    const int64_t esize = a.out_dtype == LMOE_DTYPE_F32 ? 4 : 2;
+    uint32_t lt = 0;
+    int hint = 0;
+    for (int tile = first; tile < total; tile += stride) {
+      const Tile t = tile_at(seg, a.E, a.NB, tile, hint);
+      const int row = t.row0 + (int)rank * kRowsCta + q * 32 + lane;
+      const bool ok = row < t.row_end;
+      uint8_t* out = static_cast<uint8_t*>(a.out) + (int64_t)row * a.N * esize;
+      if (t.zero) {
+        if (ok) {
+          float z[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) z[i] = 0.0f;
+          if (SWIGLU) {
+            store_row32(out, t.n * kHalf + cg * 32, a.N, z, a.out_dtype, a.vec_out != 0);
+          } else {
+            store_row32(out, t.n * kTN + cg * 64, a.N, z, a.out_dtype, a.vec_out != 0);
+            store_row32(out, t.n * kTN + cg * 64 + 32, a.N, z, a.out_dtype, a.vec_out != 0);
+          }
+        }
+        continue;
+      }
+      const uint32_t acc = lt % kAcc;
+      const bool full = mbar_wait(&bars->acc_full[acc], (lt / kAcc) & 1u, a.err, abort_flag, kSite + 10);
+      if (!__all_sync(0xffffffffu, full)) break;
+      ++lt;
+      tc_fence_after();
+      uint32_t u[32], v[32];
+      const uint32_t c0 = tmem + lane_base + acc * kTN + (SWIGLU ? cg * 32 : cg * 64);
+      tmem_ld32(c0, u);
+      tmem_ld32(c0 + (SWIGLU ? kHalf : 32), v);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(empty_addr + acc * 8);
+      if (!ok) continue;
+      const float al = a.alpha ? __ldg(a.alpha + t.e) : 1.0f;
+      float f[32];
+      if (SWIGLU) {
+        const float au = a.alpha_up ? __ldg(a.alpha_up + t.e) : 1.0f;
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          f[i] = silu(__fmul_rn(__uint_as_float(u[i]), al)) * __fmul_rn(__uint_as_float(v[i]), au);
+        store_row32(out, t.n * kHalf + cg * 32, a.N, f, a.out_dtype, a.vec_out != 0);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) f[i] = __fmul_rn(__uint_as_float(u[i]), al);
+        store_row32(out, t.n * kTN + cg * 64, a.N, f, a.out_dtype, a.vec_out != 0);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) f[i] = __fmul_rn(__uint_as_float(v[i]), al);
+        store_row32(out, t.n * kTN + cg * 64 + 32, a.N, f, a.out_dtype, a.vec_out != 0);
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();   // the other CTA's arrivals and the MMAs on this CTA's memory are done
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem, kTmemCols);
+  }
+}
+
+template <int FORMAT, bool SWIGLU>
+int launch(const CUtensorMap& x, const CUtensorMap& x32, const CUtensorMap& w, const CUtensorMap& up, const Fp4Args& a,
+           int grid, cudaStream_t stream) {
+  auto fn = fp4_gemm_kernel<FORMAT, SWIGLU>;
+  const int st = set_max_dynamic_smem(reinterpret_cast<const void*>(fn), Cfg<FORMAT>::kSmem);
+  if (st != LMOE_OK) return st;
+  fn<<<grid, kThreads, Cfg<FORMAT>::kSmem, stream>>>(x, x32, w, up, a);
+  return cuda_status(cudaGetLastError());
+}
+
+}  // namespace
+
+int run_fp4_gemm(const Fp4Problem& p, cudaStream_t stream) {
+  DeviceInfo dev;
+  int st = get_device_info(&dev);
+  if (st != LMOE_OK) return st;
+  if (dev.cc_major != 10) return LMOE_ERR_DEVICE;
+  const bool swiglu = p.wq_up != nullptr;
+  Fp4Args a = {};
+  a.xs = p.xs;
+  a.xs_pitch = p.xs_pitch;
+  a.ws = p.ws;
+  a.ws_up = p.ws_up;
+  a.ws_pitch = p.ws_pitch;
+  a.offsets = p.offsets;
+  a.offsets_i64 = p.offsets_i64;
+  a.E = p.num_experts;
+  a.N = p.N;
+  a.K = p.K;
+  a.R = p.total_rows;
+  a.NB = swiglu ? (p.N + kHalf - 1) / kHalf : (p.N + kTN - 1) / kTN;
+  a.KS = (p.K + kSK - 1) / kSK;
+  a.alpha = p.alpha;
+  a.alpha_up = p.alpha_up;
+  a.out = p.out;
+  a.out_dtype = p.out_dtype;
+  const int64_t esize = p.out_dtype == LMOE_DTYPE_F32 ? 4 : 2;
+  a.vec_out = ((int64_t)p.N * esize) % 32 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 31) == 0;
+  a.err = p.err;
+  CUtensorMap tx, tx32, tw, tu;
+  const uint64_t kb = (uint64_t)p.K / 2;
+  st = encode_tmap_2d(&tx, p.xq, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, (uint64_t)p.total_rows, kb, kb, kRowsCta, 128, true);
+  if (st != LMOE_OK) return st;
+  st = encode_tmap_2d(&tx32, p.xq, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, (uint64_t)p.total_rows, kb, kb, 32, 128, true);
+  if (st != LMOE_OK) return st;
+  const uint64_t dims[3] = {kb, (uint64_t)p.N, (uint64_t)p.num_experts};
+  const uint64_t strides[2] = {kb, kb * (uint64_t)p.N};
+  const uint32_t box[3] = {128, (uint32_t)kHalf, 1};
+  st = encode_tmap_3d(&tw, p.wq, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, dims, strides, box);
+  if (st != LMOE_OK) return st;
+  tu = tw;
+  if (swiglu) {
+    st = encode_tmap_3d(&tu, p.wq_up, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, dims, strides, box);
+    if (st != LMOE_OK) return st;
+  }
+  const int grid = gemm_grid(dev) < 2 ? 2 : gemm_grid(dev) & ~1;   // whole pairs
+  if (p.format == LMOE_FP4_MX)
+    return swiglu ? launch<LMOE_FP4_MX, true>(tx, tx32, tw, tu, a, grid, stream)
+                  : launch<LMOE_FP4_MX, false>(tx, tx32, tw, tu, a, grid, stream);
+  return swiglu ? launch<LMOE_FP4_NV, true>(tx, tx32, tw, tu, a, grid, stream)
+                : launch<LMOE_FP4_NV, false>(tx, tx32, tw, tu, a, grid, stream);
+}
+
+}  // namespace lmoe
+
+using namespace lmoe;
+
+extern "C" int lmoe_fp4_grouped_gemm(const uint8_t* xq, const uint8_t* xs, int64_t xs_pitch, int64_t total_rows, int K,
+                                     const uint8_t* wq, const uint8_t* ws, const uint8_t* wq_up, const uint8_t* ws_up,
+                                     int64_t ws_pitch, int N, int format, const void* expert_offsets,
+                                     int offsets_are_int64, int num_experts, const float* alpha, const float* alpha_up,
+                                     int out_dtype, void* output, uint32_t* error, lmoe_stream_t stream_) {
+  cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
+  LMOE_ARG_CHECK(format == LMOE_FP4_MX || format == LMOE_FP4_NV);
+  LMOE_ARG_CHECK(out_dtype == LMOE_DTYPE_BF16 || out_dtype == LMOE_DTYPE_F16 || out_dtype == LMOE_DTYPE_F32);
+  LMOE_ARG_CHECK(total_rows >= 0 && total_rows <= INT32_MAX - 1024 && N > 0 && K > 0 && K % 32 == 0);
+  LMOE_ARG_CHECK(num_experts >= 1);
+  if (num_experts > kMaxGemmExperts) return LMOE_ERR_UNSUPPORTED;
+  LMOE_ARG_CHECK((wq_up == nullptr) == (ws_up == nullptr));
+  LMOE_ARG_CHECK(xs_pitch % 32 == 0 && ws_pitch % 32 == 0);
+  LMOE_ARG_CHECK(xs_pitch >= fp4_scale_pitch(K, format) && ws_pitch >= fp4_scale_pitch(K, format));
+  if (total_rows == 0) return LMOE_OK;
+  LMOE_ARG_CHECK(xq && xs && wq && ws && expert_offsets && output);
+  LMOE_ARG_CHECK(aligned16(xq) && aligned16(xs) && aligned16(wq) && aligned16(ws) && aligned16(wq_up) &&
+                 aligned16(ws_up));
+  LMOE_ARG_CHECK(reinterpret_cast<uintptr_t>(output) % (out_dtype == LMOE_DTYPE_F32 ? 4 : 2) == 0);
+  Fp4Problem p;
+  p.xq = xq;
+  p.xs = xs;
+  p.xs_pitch = xs_pitch;
+  p.total_rows = total_rows;
+  p.K = K;
+  p.wq = wq;
+  p.ws = ws;
+  p.wq_up = wq_up;
+  p.ws_up = ws_up;
+  p.ws_pitch = ws_pitch;
+  p.N = N;
+  p.format = format;
+  p.offsets = expert_offsets;
+  p.offsets_i64 = offsets_are_int64;
+  p.num_experts = num_experts;
+  p.alpha = alpha;
+  p.alpha_up = alpha_up;
+  p.out_dtype = out_dtype;
+  p.out = output;
+  p.err = error;
+  return run_fp4_gemm(p, stream);
+}

@@ -1,0 +1,506 @@
+// grad_gemm.cu -- the two gradients of the grouped product y[r, n] = sum_k x[r, k] * w[e, n, k]
+// over ragged row segments, on CTA pairs (sm_100a).
+//
+//   input gradient   dx[r, k]    = sum_n dy[r, n] * w[e(r), n, k]        contraction over n
+//   weight gradient  dw[e, n, k] = sum_{r in e} dy[r, n] * x[r, k]       contraction over rows
+//
+// Neither needs a transposed copy: an operand whose contraction index is the slow one in memory
+// (w and both operands of dw) is loaded by TMA as it lies, in chunks of 64 columns x 64
+// contraction rows, and read by tcgen05.mma as an M- or N-major operand.
+//
+// Tile: 256 x 256 on a CTA pair (128 rows of A and 128 columns of B per CTA), two accumulators
+// of 256 columns fill the 512 TMEM columns, six stages of 64 contraction values (32 KB per CTA).
+// Bound by the tensor pipe for prompt-sized segments; with few rows per expert the input
+// gradient is bound by reading w and the weight gradient by writing dw (HBM).
+//
+// A segment's rows need not end at a stage: the rows of the next expert (or beyond) in the last
+// stage of a weight gradient are cleared in shared memory, in both operands, before its MMAs --
+// a product with a zero row would not do, since those rows may hold infinities or NaN.  Experts
+// without rows get a zero dw, rows outside every expert a zero dx.
+//
+// Warps: 0 TMA producer; 1 MMA issuer (leader CTA); 2 hands each landed stage to the leader
+// after clearing its tail; 4-11 epilogue, eight warps of 32 rows x 128 columns.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "grad_gemm.h"
+#include "host_util.h"
+#include "pair_gemm.cuh"
+
+namespace lmoe {
+namespace {
+
+constexpr int kTile = 256, kCta = 128;
+constexpr int kSK = 64;            // contraction values per stage
+constexpr int kStages = 6, kAcc = 2;
+constexpr int kEpiWarp0 = 4, kEpiWarps = 8;
+constexpr int kThreads = (kEpiWarp0 + kEpiWarps) * 32;
+constexpr uint32_t kChunk = 64 * 128;             // 64 contraction rows of 64 columns
+constexpr uint32_t kOperand = 2 * kChunk;         // 128 x 64 values of one operand
+constexpr uint32_t kStageBytes = 2 * kOperand;
+constexpr uint32_t kSite = 0x600u;
+
+enum Form { kInputGrad = 0, kWeightGrad = 1 };
+
+struct GradArgs {
+  const void* offsets;
+  int offsets_i64;
+  int E, N, K;
+  int64_t R;
+  int MT, NB;        // weight gradient: row tiles of N; both: column tiles of K
+  int KS;            // input gradient: stages of N
+  int f16;           // operands fp16 (else bf16)
+  void* out;
+  int out_dtype;
+  int vec_out;
+  uint32_t* err;
+};
+
+struct __align__(8) Bars {
+  uint64_t full[kStages];       // this CTA's operands landed
+  uint64_t empty[kStages];      // the stage's MMAs finished (both CTAs)
+  uint64_t ready[kStages];      // leader: both CTAs' operands
+  uint64_t acc_full[kAcc];
+  uint64_t acc_empty[kAcc];     // leader: both CTAs' epilogue warps
+  uint64_t mma_done;
+  uint32_t tmem_base;
+  int abort;
+  SegTable seg;
+};
+
+struct Tile {
+  int e, m, n;
+  int row0, row_end;   // input gradient: output rows; weight gradient: the expert's rows
+  int ks;              // stages; 0: the tile is zero
+};
+
+template <int FORM>
+__device__ __forceinline__ Tile tile_at(const SegTable& t, const GradArgs& a, int tile, int& hint) {
+  int j = hint;
+  while (tile >= t.tile_start[j + 1]) ++j;
+  hint = j;
+  Tile r;
+  const int rows = t.row[j + 1] - t.row[j];
+  raster(tile - t.tile_start[j], FORM == kInputGrad ? (rows + kTile - 1) / kTile : a.MT, a.NB, r.m, r.n);
+  r.e = j - 1;
+  r.row_end = t.row[j + 1];
+  if (FORM == kInputGrad) {
+    r.row0 = t.row[j] + r.m * kTile;
+    r.ks = (j == 0 || j == a.E + 1) ? 0 : a.KS;
+  } else {
+    r.row0 = t.row[j];
+    r.ks = (rows + kSK - 1) / kSK;
+  }
+  return r;
+}
+
+template <int FORM>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    grad_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_a32,
+                     const __grid_constant__ CUtensorMap tm_b, const GradArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  Bars* bars = reinterpret_cast<Bars*>(base + kStages * kStageBytes);
+  volatile int* abort_flag = &bars->abort;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = rank == 0;
+
+  if (tid == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&bars->full[s], 1);
+      mbar_init(&bars->empty[s], 1);
+      mbar_init(&bars->ready[s], 2);
+    }
+    for (int s = 0; s < kAcc; ++s) {
+      mbar_init(&bars->acc_full[s], 1);
+      mbar_init(&bars->acc_empty[s], 2 * kEpiWarps);
+    }
+    mbar_init(&bars->mma_done, 1);
+    bars->abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(&bars->tmem_base, 512);
+    tmem_relinquish_pair();
+  }
+  load_segments(&bars->seg, a.offsets, a.offsets_i64, a.E, a.R, tid, kThreads);
+  const int segs = a.E + 2;
+  if (warp == 0)
+    scan_tiles(&bars->seg, segs, lane, [&](int j) {
+      if (FORM == kInputGrad) return (bars->seg.row[j + 1] - bars->seg.row[j] + kTile - 1) / kTile * a.NB;
+      return j == 0 || j == a.E + 1 ? 0 : a.MT * a.NB;
+    });
+  if (tid == 0 && bars->seg.bad && blockIdx.x == 0) report_error(a.err, kErrBadArg, kSite + 1);
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem = bars->tmem_base;
+  const SegTable& seg = bars->seg;
+  const int total = seg.tile_start[segs];
+  const int first = blockIdx.x >> 1, stride = gridDim.x >> 1;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------ TMA producer
+    if (lane == 0) {
+      uint32_t it = 0;
+      int hint = 0;
+      bool ok = true;
+      for (int tile = first; tile < total && ok; tile += stride) {
+        const Tile t = tile_at<FORM>(seg, a, tile, hint);
+        const int c0 = t.n * kTile + (int)rank * kCta;   // first column of B
+        const int m0 = (FORM == kInputGrad ? t.row0 : t.m * kTile) + (int)rank * kCta;
+        int boxes = 4;   // input gradient: 32-row boxes of dy that hold this CTA's rows
+        if (FORM == kInputGrad) {
+          const int rows = t.row_end - m0;
+          boxes = rows <= 0 ? 0 : (rows >= kCta ? 4 : (rows + 31) >> 5);
+        }
+        for (int ks = 0; ks < t.ks; ++ks, ++it) {
+          const int s = it % kStages;
+          if (!mbar_wait(&bars->empty[s], ((it / kStages) & 1u) ^ 1u, a.err, abort_flag, kSite + 2)) {
+            ok = false;
+            break;
+          }
+          uint8_t* sa = base + s * kStageBytes;
+          uint8_t* sb = sa + kOperand;
+          uint64_t* bar = &bars->full[s];
+          mbar_arrive_expect_tx(bar, (uint32_t)boxes * 4096u + kOperand);
+          if (FORM == kInputGrad) {
+            if (boxes == 4) {
+              tma_load_2d(sa, &tm_a, bar, ks * kSK, m0);
+            } else {
+              for (int b = 0; b < boxes; ++b) tma_load_2d(sa + b * 4096, &tm_a32, bar, ks * kSK, m0 + b * 32);
+            }
+            tma_load_3d(sb, &tm_b, bar, c0, ks * kSK, t.e);
+            tma_load_3d(sb + kChunk, &tm_b, bar, c0 + 64, ks * kSK, t.e);
+          } else {
+            const int r = t.row0 + ks * kSK;
+            tma_load_2d(sa, &tm_a, bar, m0, r);
+            tma_load_2d(sa + kChunk, &tm_a, bar, m0 + 64, r);
+            tma_load_2d(sb, &tm_b, bar, c0, r);
+            tma_load_2d(sb + kChunk, &tm_b, bar, c0 + 64, r);
+          }
+        }
+      }
+      // no copy of this CTA may still be in flight when it exits
+      const uint32_t from = it > (uint32_t)kStages ? it - kStages : 0u;
+      for (uint32_t j = from; j < it; ++j)
+        mbar_wait(&bars->full[j % kStages], (j / kStages) & 1u, a.err, nullptr, kSite + 3);
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ MMA issuer
+    if (leader && lane == 0) {
+      const uint32_t idesc = idesc_f16kind_f32(kTile, kTile, a.f16) | kIdescBMajorMN |
+                             (FORM == kWeightGrad ? kIdescAMajorMN : 0u);
+      uint32_t it = 0, lt = 0;
+      int hint = 0;
+      bool ok = true;
+      for (int tile = first; tile < total && ok; tile += stride) {
+        const Tile t = tile_at<FORM>(seg, a, tile, hint);
+        if (t.ks == 0) continue;
+        const uint32_t acc = lt % kAcc;
+        if (!mbar_wait_cluster(&bars->acc_empty[acc], ((lt / kAcc) & 1u) ^ 1u, a.err, abort_flag, kSite + 4)) break;
+        const uint32_t d = tmem + acc * kTile;
+        const int depth = FORM == kInputGrad ? a.N : t.row_end - t.row0;
+        for (int ks = 0; ks < t.ks; ++ks, ++it) {
+          const int s = it % kStages;
+          if (!mbar_wait_cluster(&bars->ready[s], (it / kStages) & 1u, a.err, abort_flag, kSite + 6)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t sa = smem_u32(base + s * kStageBytes), sb = sa + kOperand;
+          const int left = depth - ks * kSK;
+          const int nk = left >= kSK ? 4 : (left + 15) / 16;
+          for (int kk = 0; kk < nk; ++kk) {
+            const uint64_t ad = FORM == kInputGrad ? sdesc_k_sw128(sa + kk * 32) : sdesc_mn_sw128(sa + kk * 2048, kChunk);
+            mma_ss_pair(d, ad, sdesc_mn_sw128(sb + kk * 2048, kChunk), idesc, (ks | kk) != 0 ? 1u : 0u);
+          }
+          mma_commit_pair(&bars->empty[s]);
+        }
+        if (ok) mma_commit_pair(&bars->acc_full[acc]);
+        ++lt;
+      }
+      mma_commit_pair(&bars->mma_done);
+      mbar_wait(&bars->mma_done, 0, a.err, nullptr, kSite + 7);
+    }
+  } else if (warp == 2) {
+    // ------------------------------------------------------------------ stage hand-over
+    uint32_t it = 0;
+    int hint = 0;
+    bool ok = true;
+    for (int tile = first; tile < total && ok; tile += stride) {
+      const Tile t = tile_at<FORM>(seg, a, tile, hint);
+      for (int ks = 0; ks < t.ks; ++ks, ++it) {
+        const int s = it % kStages;
+        ok = mbar_wait(&bars->full[s], (it / kStages) & 1u, a.err, abort_flag, kSite + 8);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (FORM == kWeightGrad) {
+          const int left = t.row_end - t.row0 - ks * kSK;
+          if (left < kSK && (left & 15) != 0) {
+            // contraction rows [left, next multiple of 16) of the four chunks; a row is one
+            // 128-byte line, which the swizzle only permutes
+            const int n = (16 - (left & 15)) * 8;
+            uint8_t* st = base + s * kStageBytes + left * 128;
+            for (int i = lane; i < 4 * n; i += 32) {
+              const int c = i / n;
+              *reinterpret_cast<uint4*>(st + c * kChunk + (i - c * n) * 16) = make_uint4(0, 0, 0, 0);
+            }
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(mapa_u32(&bars->ready[s], 0));
+      }
+    }
+  } else if (warp >= kEpiWarp0) {
+    // ------------------------------------------------------------------ epilogue
+    const int q = warp & 3, half = (warp - kEpiWarp0) >> 2;
+    const uint32_t lane_base = (uint32_t)(q * 32) << 16;
+    const uint32_t empty_addr = mapa_u32(&bars->acc_empty[0], 0);
+    const int64_t esize = a.out_dtype == LMOE_DTYPE_F32 ? 4 : 2;
+    uint32_t lt = 0;
+    int hint = 0;
+    for (int tile = first; tile < total; tile += stride) {
+      const Tile t = tile_at<FORM>(seg, a, tile, hint);
+      const int r = (int)rank * kCta + q * 32 + lane;
+      const int64_t row = FORM == kInputGrad ? (int64_t)t.row0 + r : (int64_t)t.e * a.N + t.m * kTile + r;
+      const bool ok = FORM == kInputGrad ? t.row0 + r < t.row_end : t.m * kTile + r < a.N;
+      void* out = static_cast<uint8_t*>(a.out) + row * a.K * esize;
+      const int c0 = t.n * kTile + half * kCta;
+      uint32_t acc = 0;
+      if (t.ks != 0) {
+        acc = lt % kAcc;
+        const bool full = mbar_wait(&bars->acc_full[acc], (lt / kAcc) & 1u, a.err, abort_flag, kSite + 9);
+        if (!__all_sync(0xffffffffu, full)) break;
+        ++lt;
+        tc_fence_after();
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float f[32];
+        if (t.ks != 0) {
+          uint32_t u[32];
+          tmem_ld32(tmem + lane_base + acc * kTile + half * kCta + j * 32, u);
+          if (j == 3) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(empty_addr + acc * 8);
+          }
+#pragma unroll
+          for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(u[i]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) f[i] = 0.0f;
+        }
+        if (ok) store_row32(out, c0 + j * 32, a.K, f, a.out_dtype, a.vec_out != 0);
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();   // the other CTA's arrivals and the MMAs on this CTA's memory are done
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem, 512);
+  }
+}
+
+// dst[r, 0 .. pitch) = src[r, 0 .. cols) and zeros: 16-bit rows whose length is not a multiple of
+// 16 bytes cannot be read by TMA where they lie.
+__global__ void __launch_bounds__(256) pad_rows_kernel(const uint16_t* __restrict__ src, int64_t rows, int cols,
+                                                       int pitch, uint4* __restrict__ dst) {
+  const int per = pitch / 8;
+  const int64_t total = rows * per;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t r = i / per;
+    const int c = (int)(i - r * per) * 8;
+    uint16_t v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = c + j < cols ? src[r * cols + c + j] : (uint16_t)0;
+    dst[i] = *reinterpret_cast<const uint4*>(v);
+  }
+}
+
+int pad_rows(const void* src, int64_t rows, int cols, int pitch, void* dst, const DeviceInfo& dev, cudaStream_t s) {
+  const int64_t blocks = (rows * (pitch / 8) + 255) / 256, most = (int64_t)dev.num_sms * 8;
+  pad_rows_kernel<<<(unsigned)(blocks < most ? blocks : most), 256, 0, s>>>(static_cast<const uint16_t*>(src), rows,
+                                                                          cols, pitch, static_cast<uint4*>(dst));
+  return cuda_status(cudaGetLastError());
+}
+
+template <int FORM>
+int launch(const CUtensorMap& ta, const CUtensorMap& ta32, const CUtensorMap& tb, const GradArgs& a, int grid,
+           cudaStream_t stream) {
+  constexpr size_t smem = 1024 + kStages * kStageBytes + sizeof(Bars);
+  static_assert(smem <= 232448, "shared memory budget");
+  auto fn = grad_gemm_kernel<FORM>;
+  const int st = set_max_dynamic_smem(reinterpret_cast<const void*>(fn), smem);
+  if (st != LMOE_OK) return st;
+  fn<<<grid, kThreads, smem, stream>>>(ta, ta32, tb, a);
+  return cuda_status(cudaGetLastError());
+}
+
+inline int64_t pitch8(int64_t cols) { return (cols + 7) / 8 * 8; }
+inline size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
+
+}  // namespace
+
+size_t grad_gemm_workspace(const GradProblem& p) {
+  if (p.dtype == LMOE_DTYPE_F32) return 0;
+  size_t b = 0;
+  if (p.N % 8) b += align256((size_t)p.total_rows * pitch8(p.N) * 2);
+  if (p.K % 8)
+    b += align256(p.weight_grad ? (size_t)p.total_rows * pitch8(p.K) * 2
+                                : (size_t)p.num_experts * p.N * pitch8(p.K) * 2);
+  return b;
+}
+
+int run_grad_gemm(const GradProblem& p, cudaStream_t stream) {
+  DeviceInfo dev;
+  int st = get_device_info(&dev);
+  if (st != LMOE_OK) return st;
+  if (dev.cc_major != 10) return LMOE_ERR_DEVICE;
+  const void* dy = p.dy;
+  const void* other = p.other;
+  const int64_t ldy = pitch8(p.N), ldo = pitch8(p.K);
+  uint8_t* ws = static_cast<uint8_t*>(p.workspace);
+  if (ldy != p.N) {
+    st = pad_rows(p.dy, p.total_rows, p.N, (int)ldy, ws, dev, stream);
+    if (st != LMOE_OK) return st;
+    dy = ws;
+    ws += align256((size_t)p.total_rows * ldy * 2);
+  }
+  if (ldo != p.K) {
+    st = pad_rows(p.other, p.weight_grad ? p.total_rows : (int64_t)p.num_experts * p.N, p.K, (int)ldo, ws, dev, stream);
+    if (st != LMOE_OK) return st;
+    other = ws;
+  }
+  GradArgs a = {};
+  a.offsets = p.offsets;
+  a.offsets_i64 = p.offsets_i64;
+  a.E = p.num_experts;
+  a.N = p.N;
+  a.K = p.K;
+  a.R = p.total_rows;
+  a.MT = (p.N + kTile - 1) / kTile;
+  a.NB = (p.K + kTile - 1) / kTile;
+  a.KS = (p.N + kSK - 1) / kSK;
+  a.f16 = p.dtype == LMOE_DTYPE_F16;
+  a.out = p.out;
+  a.out_dtype = p.out_dtype;
+  const int64_t esize = p.out_dtype == LMOE_DTYPE_F32 ? 4 : 2;
+  a.vec_out = ((int64_t)p.K * esize) % 32 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 31) == 0;
+  a.err = p.err;
+  const CUtensorMapDataType dt = a.f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  CUtensorMap ta, ta32, tb;
+  const int grid = gemm_grid(dev) < 2 ? 2 : gemm_grid(dev) & ~1;   // whole pairs
+  // the maps end at the true sizes, so that TMA fills what lies behind them with zeros
+  if (p.weight_grad) {
+    st = encode_tmap_2d(&ta, dy, dt, 2, (uint64_t)p.total_rows, (uint64_t)p.N, (uint64_t)ldy * 2, kSK, 64, true);
+    if (st != LMOE_OK) return st;
+    st = encode_tmap_2d(&tb, other, dt, 2, (uint64_t)p.total_rows, (uint64_t)p.K, (uint64_t)ldo * 2, kSK, 64, true);
+    if (st != LMOE_OK) return st;
+    return launch<kWeightGrad>(ta, ta, tb, a, grid, stream);
+  }
+  st = encode_tmap_2d(&ta, dy, dt, 2, (uint64_t)p.total_rows, (uint64_t)p.N, (uint64_t)ldy * 2, kCta, 64, true);
+  if (st != LMOE_OK) return st;
+  st = encode_tmap_2d(&ta32, dy, dt, 2, (uint64_t)p.total_rows, (uint64_t)p.N, (uint64_t)ldy * 2, 32, 64, true);
+  if (st != LMOE_OK) return st;
+  const uint64_t dims[3] = {(uint64_t)p.K, (uint64_t)p.N, (uint64_t)p.num_experts};
+  const uint64_t strides[2] = {(uint64_t)ldo * 2, (uint64_t)ldo * 2 * (uint64_t)p.N};
+  const uint32_t box[3] = {64, (uint32_t)kSK, 1};
+  st = encode_tmap_3d(&tb, other, dt, 2, dims, strides, box);
+  if (st != LMOE_OK) return st;
+  return launch<kInputGrad>(ta, ta32, tb, a, grid, stream);
+}
+
+}  // namespace lmoe
+
+using namespace lmoe;
+
+namespace {
+
+int grad_entry(GradProblem& p, const void* offsets, void* out, void* workspace, size_t workspace_bytes,
+               cudaStream_t stream) {
+  LMOE_ARG_CHECK(p.dtype == LMOE_DTYPE_BF16 || p.dtype == LMOE_DTYPE_F16 || p.dtype == LMOE_DTYPE_F32);
+  LMOE_ARG_CHECK(p.out_dtype == p.dtype || (p.weight_grad && p.out_dtype == LMOE_DTYPE_F32));
+  LMOE_ARG_CHECK(p.total_rows >= 0 && p.total_rows <= INT32_MAX - 1024 && p.N > 0 && p.K > 0 && p.num_experts >= 1);
+  if (p.num_experts > kMaxGemmExperts) return LMOE_ERR_UNSUPPORTED;
+  const int64_t esize = p.dtype == LMOE_DTYPE_F32 ? 4 : 2, osize = p.out_dtype == LMOE_DTYPE_F32 ? 4 : 2;
+  LMOE_ARG_CHECK(out && reinterpret_cast<uintptr_t>(out) % osize == 0);
+  if (p.total_rows == 0) {
+    if (!p.weight_grad) return LMOE_OK;
+    return cuda_status(cudaMemsetAsync(out, 0, (size_t)p.num_experts * p.N * p.K * osize, stream));
+  }
+  LMOE_ARG_CHECK(p.dy && p.other && offsets);
+  LMOE_ARG_CHECK(reinterpret_cast<uintptr_t>(p.dy) % esize == 0 && reinterpret_cast<uintptr_t>(p.other) % esize == 0);
+  if (p.dtype == LMOE_DTYPE_F32) return run_grad_f32(p, stream);
+  // rows that TMA reads where they lie start at multiples of 16 bytes
+  LMOE_ARG_CHECK((p.N % 8 || aligned16(p.dy)) && (p.K % 8 || aligned16(p.other)));
+  const size_t need = grad_gemm_workspace(p);
+  if (need && (!workspace || workspace_bytes < need || !aligned16(workspace))) return LMOE_ERR_WORKSPACE;
+  p.workspace = workspace;
+  return run_grad_gemm(p, stream);
+}
+
+}  // namespace
+
+extern "C" size_t lmoe_grouped_gemm_grad_workspace_bytes(int weight_grad, int dtype, int64_t total_rows, int N, int K,
+                                                         int num_experts) {
+  if (total_rows < 0 || N <= 0 || K <= 0 || num_experts <= 0) return 0;
+  GradProblem p;
+  p.weight_grad = weight_grad != 0;
+  p.dtype = dtype;
+  p.total_rows = total_rows;
+  p.N = N;
+  p.K = K;
+  p.num_experts = num_experts;
+  return grad_gemm_workspace(p);
+}
+
+extern "C" int lmoe_grouped_gemm_dgrad(const void* grad_output, int dtype, int64_t total_rows, int N,
+                                       const void* weights, int K, const void* expert_offsets, int offsets_are_int64,
+                                       int num_experts, void* grad_input, void* workspace, size_t workspace_bytes,
+                                       uint32_t* error, lmoe_stream_t stream) {
+  GradProblem p;
+  p.weight_grad = false;
+  p.dtype = p.out_dtype = dtype;
+  p.total_rows = total_rows;
+  p.N = N;
+  p.K = K;
+  p.num_experts = num_experts;
+  p.dy = grad_output;
+  p.other = weights;
+  p.offsets = expert_offsets;
+  p.offsets_i64 = offsets_are_int64;
+  p.out = grad_input;
+  p.err = error;
+  if (total_rows == 0 && !grad_input) return N > 0 && K > 0 && num_experts >= 1 ? LMOE_OK : LMOE_ERR_INVALID_ARG;
+  return grad_entry(p, expert_offsets, grad_input, workspace, workspace_bytes, reinterpret_cast<cudaStream_t>(stream));
+}
+
+extern "C" int lmoe_grouped_gemm_wgrad(const void* grad_output, int dtype, int64_t total_rows, int N,
+                                       const void* input, int K, const void* expert_offsets, int offsets_are_int64,
+                                       int num_experts, int out_dtype, void* grad_weights, void* workspace,
+                                       size_t workspace_bytes, uint32_t* error, lmoe_stream_t stream) {
+  GradProblem p;
+  p.weight_grad = true;
+  p.dtype = dtype;
+  p.out_dtype = out_dtype;
+  p.total_rows = total_rows;
+  p.N = N;
+  p.K = K;
+  p.num_experts = num_experts;
+  p.dy = grad_output;
+  p.other = input;
+  p.offsets = expert_offsets;
+  p.offsets_i64 = offsets_are_int64;
+  p.out = grad_weights;
+  p.err = error;
+  return grad_entry(p, expert_offsets, grad_weights, workspace, workspace_bytes,
+                    reinterpret_cast<cudaStream_t>(stream));
+}

@@ -1,0 +1,30 @@
+// grad_gemm.h -- internal interface of the grouped product's gradients (grad_gemm.cu for 16-bit
+// operands on tensor cores, grad_f32.cu for fp32 operands).
+#pragma once
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+namespace lmoe {
+
+struct GradProblem {
+  bool weight_grad = false;   // dw[e, n, k] from dy and x, else dx[r, k] from dy and w
+  int dtype = 0;              // operands
+  int out_dtype = 0;
+  int64_t total_rows = 0;
+  int N = 0, K = 0;
+  int num_experts = 0;
+  const void* dy = nullptr;      // [total_rows, N]
+  const void* other = nullptr;   // x [total_rows, K] or w [num_experts, N, K]
+  const void* offsets = nullptr;
+  int offsets_i64 = 0;
+  void* out = nullptr;
+  void* workspace = nullptr;     // padded copies of operands whose rows TMA cannot read
+  uint32_t* err = nullptr;
+};
+
+size_t grad_gemm_workspace(const GradProblem& p);
+int run_grad_gemm(const GradProblem& p, cudaStream_t stream);
+int run_grad_f32(const GradProblem& p, cudaStream_t stream);
+
+}  // namespace lmoe

@@ -64,6 +64,11 @@ int encode_tmap_kblocks(CUtensorMap* map, const void* base, CUtensorMapDataType 
                         uint64_t rows, uint64_t cols, uint64_t row_stride_bytes, uint32_t box_rows,
                         uint32_t box_blocks);
 
+// Encode a row-major 3-D tensor (dims and box from the innermost; strides in bytes of the two
+// outer dimensions), 128-byte swizzle: box[0] elements are 128 bytes.
+int encode_tmap_3d(CUtensorMap* map, const void* base, CUtensorMapDataType dtype, uint32_t elem_bytes,
+                   const uint64_t (&dims)[3], const uint64_t (&strides)[2], const uint32_t (&box)[3]);
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 }  // namespace lmoe

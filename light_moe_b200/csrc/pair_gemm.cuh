@@ -1,0 +1,260 @@
+// pair_gemm.cuh -- what the grouped GEMMs on CTA pairs share: the cta_group::2 forms of the
+// tcgen05 instructions, cluster barriers, the segment table that every CTA derives from the
+// expert offsets, and the row stores of the epilogues.
+//
+// A pair of CTAs (a cluster of two) computes one tile of 256 rows x BN columns: each CTA holds
+// 128 rows of A, half of B's columns in shared memory and 128 x BN accumulators in its tensor
+// memory.  One thread of the leader CTA (rank 0) issues the MMAs for both, so each operand
+// byte in shared memory feeds twice the work of a single-CTA tile: a 128 x 256 bf16 tile needs
+// 96 bytes of operands per SM and cycle from L2 at full tensor rate, a 256 x 256 pair 64.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "grouped_gemm.h"
+#include "lmoe_b200.h"
+#include "ptx.cuh"
+
+namespace lmoe {
+
+// ---------------------------------------------------------------------------------------
+// clusters
+// ---------------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t cluster_ctarank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Shared-cluster address of `p` (an address of this CTA) in CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t mapa_u32(const void* p, uint32_t rank) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+__device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// mbar_wait for a barrier that the other CTA arrives on (acquire at cluster scope).
+__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity, uint32_t* err, volatile int* abort,
+                                                  uint32_t site) {
+  if (mbar_try_wait_cluster(bar, parity)) return true;
+  const uint64_t t0 = globaltimer_ns();
+  uint32_t spins = 0;
+  while (true) {
+    if (mbar_try_wait_cluster(bar, parity)) return true;
+    if (((++spins) & 63u) == 0u) {
+      if (abort && *abort) return false;
+      if (globaltimer_ns() - t0 > kWaitBudgetNs) {
+        report_error(err, kErrTimeout, site);
+        if (abort) *abort = 1;
+        return false;
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// tcgen05 on a CTA pair
+// ---------------------------------------------------------------------------------------
+// One warp of each CTA of the pair executes these.
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t* dst_smem, uint32_t ncols) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst_smem)),
+               "r"(ncols)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_relinquish_pair() {
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+}
+
+__device__ __forceinline__ void mma_ss_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// Arrive once on *bar (the same offset in both CTAs) when all tcgen05 operations that this
+// thread issued before have finished.
+__device__ __forceinline__ void mma_commit_pair(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          smem_u32(bar)),
+      "h"((uint16_t)3)
+      : "memory");
+}
+
+// Shared-memory descriptor of an M- or N-major 16-bit operand in 128-byte-swizzled chunks of
+// 64 elements x rows: a contraction row is one 128-byte line, eight rows are 1024 bytes, and
+// the next 64 elements lie `chunk_bytes` further on.  Sixteen contraction rows advance the
+// start address by 2048 bytes.
+__device__ __forceinline__ uint64_t sdesc_mn_sw128(uint32_t smem_addr, uint32_t chunk_bytes) {
+  uint64_t d = 0;
+  d |= (uint64_t)((smem_addr >> 4) & 0x3fffu);
+  d |= (uint64_t)((chunk_bytes >> 4) & 0x3fffu) << 16;   // leading byte offset: the next 64 elements
+  d |= (uint64_t)(1024u >> 4) << 32;                     // stride byte offset: the next 8 rows
+  d |= (uint64_t)1u << 46;
+  d |= (uint64_t)2u << 61;
+  return d;
+}
+constexpr uint32_t kIdescAMajorMN = 1u << 15;
+constexpr uint32_t kIdescBMajorMN = 1u << 16;
+
+// Each thread of the warp reads 32 consecutive 32-bit columns of its own TMEM lane.
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+      "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+
+// ---------------------------------------------------------------------------------------
+// segments
+// ---------------------------------------------------------------------------------------
+// Row ranges from the expert offsets: segment 0 = rows before the first expert, segment
+// 1 + e = expert e, segment E + 1 = rows behind the last expert.  Offsets that decrease or
+// leave [0, R] make every expert empty (all rows fall into segment 0), and are reported.
+struct SegTable {
+  int row[kMaxGemmExperts + 3];          // segment j holds rows [row[j], row[j + 1])
+  int tile_start[kMaxGemmExperts + 3];   // first tile of segment j; [segments] = total
+  int bad;
+};
+
+// Called by all threads of the CTA; `threads` of them.
+__device__ __forceinline__ void load_segments(SegTable* t, const void* offsets, int offsets_i64, int E, int64_t R,
+                                              int tid, int threads) {
+  if (tid == 0) t->bad = 0;
+  __syncthreads();
+  for (int e = tid; e <= E; e += threads) {
+    const int64_t o = offsets_i64 ? static_cast<const int64_t*>(offsets)[e]
+                                  : (int64_t) static_cast<const int32_t*>(offsets)[e];
+    int64_t prev = 0;
+    if (e > 0)
+      prev = offsets_i64 ? static_cast<const int64_t*>(offsets)[e - 1]
+                         : (int64_t) static_cast<const int32_t*>(offsets)[e - 1];
+    if (o < prev || o < 0 || o > R) t->bad = 1;
+    t->row[e + 1] = (int)o;
+  }
+  if (tid == 0) {
+    t->row[0] = 0;
+    t->row[E + 2] = (int)R;
+  }
+  __syncthreads();
+  if (t->bad)
+    for (int e = tid; e <= E; e += threads) t->row[e + 1] = (int)R;
+  __syncthreads();
+}
+
+// Exclusive scan of the segments' tile counts (count(j) for segment j) by one warp.
+template <typename F>
+__device__ __forceinline__ void scan_tiles(SegTable* t, int segments, int lane, F count) {
+  int carry = 0;
+  for (int j0 = 0; j0 < segments; j0 += 32) {
+    const int j = j0 + lane;
+    int v = j < segments ? count(j) : 0;
+    int s = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += u;
+    }
+    if (j < segments) t->tile_start[j] = carry + s - v;
+    carry += __shfl_sync(0xffffffffu, s, 31);
+  }
+  if (lane == 0) t->tile_start[segments] = carry;
+}
+
+// Tile `local` of a segment of mt x nb tiles.  Tiles are walked in groups of eight row tiles,
+// column tile by column tile inside a group, so that the pairs working at the same time share
+// eight row panels and a few column panels through L2.
+__device__ __forceinline__ void raster(int local, int mt, int nb, int& m, int& n) {
+  const int per = 8 * nb;
+  const int g = local / per;
+  const int left = mt - g * 8;
+  const int gm = left < 8 ? left : 8;
+  const int in = local - g * per;
+  n = in / gm;
+  m = g * 8 + in - n * gm;
+}
+
+// ---------------------------------------------------------------------------------------
+// epilogue stores
+// ---------------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t pack16(float a, float b, int f16) {
+  if (f16) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+__device__ __forceinline__ void st_global_v8(void* p, const uint32_t (&v)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+
+// 32 consecutive values of one output row from column c0 (columns >= cols are not written).
+// vec: every row starts at a multiple of 32 bytes, so whole 32-byte sectors are stored.
+__device__ __forceinline__ void store_row32(void* row, int c0, int cols, const float (&v)[32], int dtype, bool vec) {
+  if (c0 >= cols) return;
+  if (vec && c0 + 32 <= cols) {
+    if (dtype == LMOE_DTYPE_F32) {
+      float* p = static_cast<float*>(row) + c0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t w[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(v[8 * j + i]);
+        st_global_v8(p + 8 * j, w);
+      }
+    } else {
+      uint16_t* p = static_cast<uint16_t*>(row) + c0;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        uint32_t w[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = pack16(v[16 * j + 2 * i], v[16 * j + 2 * i + 1], dtype == LMOE_DTYPE_F16);
+        st_global_v8(p + 16 * j, w);
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    if (c0 + i < cols) {
+      if (dtype == LMOE_DTYPE_F32)
+        static_cast<float*>(row)[c0 + i] = v[i];
+      else
+        static_cast<uint16_t*>(row)[c0 + i] = (uint16_t)(pack16(v[i], 0.0f, dtype == LMOE_DTYPE_F16) & 0xffffu);
+    }
+  }
+}
+
+}  // namespace lmoe

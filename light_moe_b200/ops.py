@@ -9,7 +9,9 @@ Same names, argument names and return types as the reference's ``light_moe._C``
         -> (permuted, ids, weights, offsets int64, sorted_idx int64)
 
 plus the new ops (``fused_gate_topk_ex``, ``quantize_w4``, ``dequantize_w4``, ``prepack_w4``,
-``w4a16_grouped_gemm``, ``moe_layer_w4a16``).  Every op runs the CUDA library; if the
+``w4a16_grouped_gemm``, ``moe_layer_w4a16``; the gradients ``grouped_gemm_dgrad`` and
+``grouped_gemm_wgrad``; the 4-bit floating point ``quantize_fp4``, ``dequantize_fp4`` and
+``fp4_grouped_gemm``).  Every op runs the CUDA library; if the
 ``_C`` extension has not been built, calling any op raises -- there is no fallback path.
 """
 from __future__ import annotations
@@ -77,6 +79,48 @@ def w4a16_grouped_gemm(input, packed, expert_offsets, num_experts, N, group_size
     return extension().w4a16_grouped_gemm(input, packed, expert_offsets, num_experts, N,
                                           group_size, epilogue, dest_rows, row_scale, out_rows,
                                           max_rows_per_expert, segment_expert)
+
+
+def grouped_gemm_dgrad(grad_output, weights, expert_offsets, num_experts):
+    """Input gradient of grouped_gemm: [T, N] x [E, N, K] -> [T, K] (rows outside every expert are
+    zero).  bf16 / fp16 on tensor cores, fp32 in fp32; any N, K; operands of one dtype."""
+    return extension().grouped_gemm_dgrad(grad_output, weights, expert_offsets, num_experts)
+
+
+def grouped_gemm_wgrad(grad_output, input, expert_offsets, num_experts, out_dtype=None):
+    """Weight gradient of grouped_gemm: sum over each expert's rows of grad_output^T input ->
+    [E, N, K] in the operands' dtype or, with ``out_dtype=torch.float32``, unrounded; experts
+    without rows are zero."""
+    return extension().grouped_gemm_wgrad(grad_output, input, expert_offsets, num_experts, out_dtype)
+
+
+def quantize_fp4(x, format, global_scale=None, positions=None):
+    """x [..., K] (bf16 / fp16 / fp32, K % 32 == 0) -> (codes uint8 [..., K/2], scales uint8
+    [..., K/block]): E2M1 values, two to a byte (even column low), under one scale byte per
+    block -- ``"mxfp4"`` E8M0 scales for blocks of 32, ``"nvfp4"`` E4M3 scales for blocks of 16
+    times ``global_scale`` (fp32, one value or one per leading index of a 3-D x; None = 1).
+    Round to nearest even, saturating; blocks with an infinity or NaN read back as NaN.
+
+    ``positions`` int32 [rows, copies] (a permutation of 0 .. rows * copies - 1, like the
+    router's inverse permutation): row r is written to rows positions[r, :], so a MoE layer's
+    permutation needs no pass of its own.  Scale rows lie on a pitch of a multiple of 32 bytes
+    (the returned tensor is a view); the product copies scales that do not."""
+    return extension().quantize_fp4(x, format, global_scale, positions)
+
+
+def dequantize_fp4(q, scales, format, global_scale=None):
+    """Codes and scales -> bf16 [..., K]: bf16_rn(code * scale * global_scale)."""
+    return extension().dequantize_fp4(q, scales, format, global_scale)
+
+
+def fp4_grouped_gemm(input, input_scales, weights, weight_scales, expert_offsets, num_experts, format,
+                     alpha=None, weights_up=None, weight_scales_up=None, alpha_up=None, out_dtype=None):
+    """Grouped product of 4-bit operands (codes and scales as quantize_fp4 returns them): rows
+    [T, K] x weights [E, N, K] -> [T, N] of ``out_dtype`` (bf16 by default), times ``alpha[e]``
+    (fp32 [E], the product of the operands' global scales).  With ``weights_up``:
+    silu(gate) * up.  Exact products, fp32 accumulation; rows outside every expert are zero."""
+    return extension().fp4_grouped_gemm(input, input_scales, weights, weight_scales, expert_offsets, num_experts,
+                                        format, alpha, weights_up, weight_scales_up, alpha_up, out_dtype)
 
 
 def combine_rows(rows, positions, weights, num_tokens, top_k, extra_rows=None, num_extra=0):

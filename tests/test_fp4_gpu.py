@@ -1,0 +1,383 @@
+"""GPU tests of the microscaled 4-bit operators against their definition in 64 bits.
+
+Quantising and dequantising are exact (codes, scale bytes and bf16 values equal the oracle's).
+The product's tolerance is derived from its arithmetic: the 4-bit products are exact, K of them
+are summed in fp32 (at most K * 2^-23 of the sum of absolute products, each addition off by at
+most one unit in the last place), one factor (2^-24) and one rounding to the output type
+(eps / 2).  SwiGLU adds the error of the fast exponential and division.
+"""
+import numpy as np
+import pytest
+import torch
+
+import fp4_reference as ref
+from light_moe_b200 import capi, ops
+
+pytestmark = pytest.mark.gpu
+DT = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+
+
+def _np(t):
+    return t.cpu().numpy()
+
+
+def _check_quantize(x, fmt, g=None, **kw):
+    q, s = ops.quantize_fp4(x, fmt, None if g is None else torch.tensor([g], device="cuda"), **kw)
+    c, b = ref.quantize(x.double().cpu().numpy(), fmt, 1.0 if g is None else float(np.float32(g)))
+    assert q.dtype == torch.uint8 and s.dtype == torch.uint8
+    assert (_np(s) != b).sum() == 0
+    assert (ref.unpack(_np(q)) != c).sum() == 0
+    return q, s
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("dt", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("rows,K", [(1, 32), (3, 96), (257, 2816), (5, 4096), (2, 8224)])
+def test_quantize_random(fmt, dt, rows, K):
+    gen = torch.Generator(device="cuda").manual_seed(rows + K)
+    x = (torch.randn(rows, K, generator=gen, device="cuda") * 3).to(DT[dt])
+    x[:, ::17] *= 20
+    q, s = _check_quantize(x, fmt)
+    v = ops.dequantize_fp4(q, s, fmt)
+    want = torch.from_numpy(ref.values(_np(q), _np(s), fmt)).to(torch.bfloat16)   # exact in both formats
+    assert torch.equal(v.cpu(), want)
+
+
+@pytest.mark.parametrize("g", [1.0, 0.5, 0.0123456, 3.7e-5, 1e-33, 1e35])
+def test_quantize_tensor_scale(g):
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    x = torch.randn(64, 512, generator=gen, device="cuda") * (g * 100)
+    q, s = _check_quantize(x, "nvfp4", g)
+    v = _np(ops.dequantize_fp4(q, s, "nvfp4", torch.tensor([g], device="cuda")).double())
+    want = ref.values(_np(q), _np(s), "nvfp4", float(np.float32(g)))
+    # fp32 product with g, then bf16: half a unit of each (and of the smallest normal fp32)
+    assert np.all(np.abs(v - want) <= (2.0 ** -8 + 2.0 ** -23) * np.abs(want) + 2.0 ** -133)
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("unit", [1.0, 2.0 ** -20, 1.125, 0.3])
+def test_quantize_ties_and_borders(fmt, unit):
+    """Every multiple of 1/8 up to 8 and its fp32 neighbours, in units of the scale."""
+    t = torch.arange(0, 65, dtype=torch.float64) / 8
+    f = (t * unit).float()
+    v = torch.cat([f, torch.nextafter(f, f * 0 - 1), torch.nextafter(f, f * 0 + 100)])
+    v = torch.cat([v, -v])
+    b = ref.BLOCK[fmt]
+    per = b - 1
+    n = (len(v) + per - 1) // per
+    v = torch.cat([v, torch.zeros(n * per - len(v))]).view(n, per)
+    top = torch.full((n, 1), 6.0 * unit)                     # nails the block's scale (MX: at most 8 -> 2 units)
+    x = torch.cat([top, v.clamp(-6.0 * unit, 6.0 * unit)], 1).view(1, -1)
+    x = torch.cat([x, torch.zeros(1, (-x.shape[1]) % 32)], 1)
+    x = x.cuda()
+    _check_quantize(x, fmt)
+    if fmt == "nvfp4":
+        for g in (0.75, 1 / 3, 0.01):
+            _check_quantize((x * g).contiguous(), fmt, g)
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+def test_quantize_extremes(fmt):
+    x = torch.zeros(8, 64, device="cuda")
+    x[0, 3] = 3.0e38
+    x[1] = 1e-45
+    x[2] = -1.17549435e-38
+    x[3, ::2] = 5e-39
+    x[4] = -0.0
+    x[5, 0], x[5, 1] = 448.0 * 6, 500.0 * 6
+    x[6] = 2.0 ** -9 * 6
+    x[7] = 2.0 ** -10 * 6
+    _check_quantize(x, fmt)
+    _check_quantize(x.to(torch.bfloat16), fmt)
+
+
+@pytest.mark.parametrize("fmt,nan_byte", [("mxfp4", 255), ("nvfp4", 127)])
+@pytest.mark.parametrize("dt", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+def test_quantize_blocks_that_are_not_finite(fmt, nan_byte, dt, bad):
+    x = torch.ones(3, 128, device="cuda", dtype=DT[dt])
+    x[1, 70] = bad
+    q, s = _check_quantize(x, fmt)
+    blk = 70 // ref.BLOCK[fmt]
+    assert s[1, blk].item() == nan_byte and (s == nan_byte).sum().item() == 1
+    v = ops.dequantize_fp4(q, s, fmt)
+    assert torch.isnan(v).sum().item() == ref.BLOCK[fmt]
+
+
+@pytest.mark.parametrize("g", [0.0, -1.0, float("nan"), float("inf")])
+def test_quantize_bad_tensor_scale_gives_nan(g):
+    x = torch.ones(2, 32, device="cuda")
+    q, s = ops.quantize_fp4(x, "nvfp4", torch.tensor([g], device="cuda"))
+    assert (s == 127).all() and (q == 0).all()
+
+
+def test_quantize_views_batches_and_scales_per_expert():
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    wide = torch.randn(40, 400, generator=gen, device="cuda").to(torch.bfloat16)
+    for v in (wide[:, 8:8 + 96], wide[:, 3:3 + 96], wide[::3, :64], wide[:, ::2][:, :96], wide.t()[:64, :32]):
+        _check_quantize(v, "mxfp4")
+        _check_quantize(v, "nvfp4")
+    w = torch.randn(3, 5, 64, generator=gen, device="cuda")
+    g = torch.tensor([0.5, 0.01, 2.0], device="cuda")
+    q, s = ops.quantize_fp4(w, "nvfp4", g)
+    assert q.shape == (3, 5, 32) and s.shape == (3, 5, 4)
+    v = ops.dequantize_fp4(q, s, "nvfp4", g)
+    for e in range(3):
+        c, b = ref.quantize(w[e].double().cpu().numpy(), "nvfp4", float(g[e]))
+        assert np.array_equal(ref.unpack(_np(q[e])), c) and np.array_equal(_np(s[e]), b)
+        assert torch.equal(v[e], ops.dequantize_fp4(q[e], s[e], "nvfp4", g[e:e + 1]))
+    q0, s0 = ops.quantize_fp4(torch.empty(0, 64, device="cuda"), "mxfp4")
+    assert q0.shape == (0, 32) and ops.dequantize_fp4(q0, s0, "mxfp4").shape == (0, 64)
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+def test_quantize_to_permuted_rows(fmt):
+    """Row r lands on every row of positions[r]; entries outside the output are skipped."""
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    T, k, K = 37, 3, 160
+    x = torch.randn(T, K, generator=gen, device="cuda").to(torch.bfloat16)
+    pos = torch.randperm(T * k, generator=torch.Generator().manual_seed(3)).to(torch.int32).view(T, k).cuda()
+    q1, s1 = ops.quantize_fp4(x, fmt)
+    q, s = ops.quantize_fp4(x, fmt, positions=pos)
+    assert q.shape == (T * k, K // 2)
+    for j in range(k):
+        assert torch.equal(q[pos[:, j].long()], q1) and torch.equal(s[pos[:, j].long()], s1)
+    # the caller's buffers behind the last row stay as they are
+    pitch = capi.lib().lmoe_fp4_scale_pitch(K, capi.LMOE_FP4_MX if fmt == "mxfp4" else capi.LMOE_FP4_NV)
+    qb = torch.full((T * k + 2, K // 2), 7, dtype=torch.uint8, device="cuda")
+    sb = torch.full((T * k + 2, pitch), 7, dtype=torch.uint8, device="cuda")
+    bad = pos.clone()
+    bad[0, 0], bad[1, 1] = -1, T * k
+    capi.call("lmoe_quantize_fp4", x.data_ptr(), 0, T, K, K, 0 if fmt == "mxfp4" else 1, None, 1, bad.data_ptr(), k,
+              T * k, qb.data_ptr(), sb.data_ptr(), capi.stream_handle())
+    assert (qb[T * k:] == 7).all() and (sb[T * k:] == 7).all()
+    hit = torch.ones(T * k, dtype=torch.bool)
+    hit[pos[0, 0].item()] = hit[pos[1, 1].item()] = False
+    assert torch.equal(qb[:T * k].cpu()[hit], q.cpu()[hit]) and (qb[:T * k].cpu()[~hit] == 7).all()
+    assert (sb[:T * k].cpu()[hit][:, K // ref.BLOCK[fmt]:] == 0).all()   # the padding of a scale row
+
+
+def test_refusals_on_the_device():
+    x = torch.ones(4, 64, device="cuda")
+    q, s = ops.quantize_fp4(x, "mxfp4")
+    off = torch.tensor([0, 4], dtype=torch.int32, device="cuda")
+    g1 = torch.ones(1, device="cuda")
+    for call in (
+        lambda: ops.quantize_fp4(x, "fp4"),
+        lambda: ops.quantize_fp4(x[:, :40], "mxfp4"),
+        lambda: ops.quantize_fp4(x.double(), "mxfp4"),
+        lambda: ops.quantize_fp4(x[0], "mxfp4"),
+        lambda: ops.quantize_fp4(x, "mxfp4", g1),
+        lambda: ops.quantize_fp4(x, "nvfp4", g1.double()),
+        lambda: ops.quantize_fp4(x, "nvfp4", torch.ones(4, device="cuda")),
+        lambda: ops.quantize_fp4(x, "nvfp4", torch.ones(1)),
+        lambda: ops.quantize_fp4(x, "mxfp4", positions=torch.arange(4, device="cuda")),
+        lambda: ops.quantize_fp4(x, "mxfp4", positions=torch.arange(5, dtype=torch.int32, device="cuda")),
+        lambda: ops.dequantize_fp4(q, s[:, :1], "mxfp4"),
+        lambda: ops.dequantize_fp4(q, s[:3], "mxfp4"),
+        lambda: ops.dequantize_fp4(q.int(), s, "mxfp4"),
+        lambda: ops.fp4_grouped_gemm(q, s, q[None, :, :16], s[None], off, 1, "mxfp4"),
+        lambda: ops.fp4_grouped_gemm(q, s, q[None], s[None], off, 2, "mxfp4"),
+        lambda: ops.fp4_grouped_gemm(q, s, q[None], s[None], off, 0, "mxfp4"),
+        lambda: ops.fp4_grouped_gemm(q, s, q[None], s[None], off.float(), 1, "mxfp4"),
+        lambda: ops.fp4_grouped_gemm(q, s, q[None], s[None], off.cpu(), 1, "mxfp4"),
+        lambda: ops.fp4_grouped_gemm(q, s, q[None], s[None], off, 1, "nvfp4"),
+        lambda: ops.fp4_grouped_gemm(q, s, q[None], s[None], off, 1, "mxfp4", weights_up=q[None]),
+        lambda: ops.fp4_grouped_gemm(q, s, q[None], s[None], off, 1, "mxfp4", alpha_up=g1),
+        lambda: ops.fp4_grouped_gemm(q, s, q[None], s[None], off, 1, "mxfp4", alpha=g1.double()),
+        lambda: ops.fp4_grouped_gemm(q, s, q[None], s[None], off, 1, "mxfp4", out_dtype=torch.float64),
+    ):
+        with pytest.raises(RuntimeError):
+            call()
+
+
+# ------------------------------------------------------------------------------------ product
+def _operand(shape, fmt, gen, std=1.0):
+    x = torch.randn(*shape, generator=gen, device="cuda") * std
+    return ops.quantize_fp4(x, fmt)
+
+
+def _product64(xq, xs, wq, ws, bounds, fmt, alpha=None):
+    """Sums and sums of absolute products, in 64 bits, zero outside the experts."""
+    x = torch.from_numpy(ref.values(_np(xq), _np(xs), fmt)).cuda()
+    w = torch.from_numpy(ref.values(_np(wq), _np(ws), fmt)).cuda()
+    y = torch.zeros(x.shape[0], w.shape[1], dtype=torch.float64, device="cuda")
+    m = torch.zeros_like(y)
+    for e in range(len(bounds) - 1):
+        a, b = bounds[e], bounds[e + 1]
+        f = 1.0 if alpha is None else float(alpha[e])
+        y[a:b] = x[a:b] @ w[e].T * f
+        m[a:b] = x[a:b].abs() @ w[e].abs().T * abs(f)
+    return y, m
+
+
+def _check_product(counts, N, K, fmt, swiglu=False, odt=torch.bfloat16, head=0, tail=0, i64=False, alpha=True, seed=0):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    E = len(counts)
+    bounds = [head]
+    for c in counts:
+        bounds.append(bounds[-1] + c)
+    R = bounds[-1] + tail
+    off = torch.tensor(bounds, dtype=torch.int64 if i64 else torch.int32, device="cuda")
+    xq, xs = _operand((R, K), fmt, gen)
+    wq, ws = _operand((E, N, K), fmt, gen, 0.1)
+    al = (torch.rand(E, generator=gen, device="cuda") + 0.5) if alpha else None
+    kw = {}
+    if swiglu:
+        uq, us = _operand((E, N, K), fmt, gen, 0.1)
+        au = (torch.rand(E, generator=gen, device="cuda") + 0.5) if alpha else None
+        kw = dict(weights_up=uq, weight_scales_up=us, alpha_up=au)
+    y = ops.fp4_grouped_gemm(xq, xs, wq, ws, off, E, fmt, alpha=al, out_dtype=odt, **kw)
+    assert y.dtype == odt and y.shape == (R, N)
+    half = torch.finfo(odt).eps / 2
+    acc = (K + 2) * 2.0 ** -23
+    g, mg = _product64(xq, xs, wq, ws, bounds, fmt, al)
+    if swiglu:
+        u, mu = _product64(xq, xs, uq, us, bounds, fmt, au)
+        dg, du = acc * mg, acc * mu
+        want = g * torch.sigmoid(g) * u
+        # |silu'| <= 1.1; exp off by 2 + 1.16 |g| units, the division by 2
+        fast = (6 + 1.16 * g.abs()) * 2.0 ** -23
+        off_by = 1.1 * dg * (u.abs() + du) + (g.abs() + dg) * du + fast * want.abs()
+    else:
+        want, off_by = g, acc * mg
+    tol = off_by * (1 + half) + half * want.abs() + torch.finfo(odt).tiny
+    bad = (y.double() - want).abs() > tol
+    assert not bad.any(), (bad.sum().item(), (y.double() - want).abs().max().item())
+    assert (y[:head] == 0).all() and (y[R - tail:] == 0).all()
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("swiglu", [False, True])
+@pytest.mark.parametrize("counts,N,K", [
+    ([1], 64, 64), ([1, 0, 3], 96, 128), ([128], 192, 256), ([256, 129, 0, 31], 200, 512), ([5, 300], 384, 1408),
+    ([17, 33, 65], 1000, 96), ([2, 2], 7, 32), ([700], 640, 2816),
+])
+def test_product(fmt, swiglu, counts, N, K):
+    _check_product(counts, N, K, fmt, swiglu)
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("odt", [torch.bfloat16, torch.float16, torch.float32])
+def test_product_output_types(fmt, odt):
+    _check_product([40, 200], 300, 320, fmt, odt=odt)
+    _check_product([40, 200], 160, 320, fmt, swiglu=True, odt=odt, alpha=False)
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("swiglu", [False, True])
+def test_product_rows_outside_experts_and_offsets_64(fmt, swiglu):
+    _check_product([60, 0, 300, 1], 250, 608, fmt, swiglu, head=3, tail=290, i64=True)
+    _check_product([0, 0], 192, 256, fmt, swiglu, head=0, tail=5)
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+def test_product_many_experts_and_long_sums(fmt):
+    _check_product([i % 7 for i in range(256)], 64, 64, fmt)
+    _check_product([9, 140], 256, 14336, fmt)
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+def test_nan_blocks_stay_in_their_rows(fmt):
+    """A NaN block reaches its own row (or its weight's column) only; rows of other experts that
+    share a tile, padding bytes of scale rows and rows outside the experts do not leak."""
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    R, N, K = 200, 130, 160
+    x = torch.randn(R, K, generator=gen, device="cuda")
+    w = torch.randn(2, N, K, generator=gen, device="cuda")
+    off = torch.tensor([10, 90, 180], dtype=torch.int32, device="cuda")
+    clean = ops.fp4_grouped_gemm(*ops.quantize_fp4(x, fmt), *ops.quantize_fp4(w, fmt), off, 2, fmt)
+    x[5], x[50, 33], x[185, 0] = float("nan"), float("inf"), float("nan")
+    w[1, 7, 100] = float("nan")
+    xq, xs = ops.quantize_fp4(x, fmt)
+    wq, ws = ops.quantize_fp4(w, fmt)
+    # padding bytes of both scale rows hold the NaN byte
+    fill = 255 if fmt == "mxfp4" else 127
+    xs.as_strided((R, 32), (xs.stride(0), 1))[:, K // ref.BLOCK[fmt]:] = fill
+    ws.as_strided((2, N, 32), (ws.stride(0), ws.stride(1), 1))[..., K // ref.BLOCK[fmt]:] = fill
+    y = ops.fp4_grouped_gemm(xq, xs, wq, ws, off, 2, fmt)
+    want = torch.zeros(R, N, dtype=torch.bool, device="cuda")
+    want[50] = True
+    want[90:180, 7] = True
+    assert torch.equal(torch.isnan(y), want)
+    assert torch.equal(y[~want], clean[~want])
+    assert (y[:10] == 0).all() and (y[180:] == 0).all()
+
+
+@pytest.mark.parametrize("offsets", [[0, 50, 40, 100], [-1, 20, 40, 100], [0, 20, 40, 101]])
+def test_bad_offsets_give_zeros_and_an_error_word(offsets):
+    R, N, K = 100, 64, 64
+    xq, xs = ops.quantize_fp4(torch.ones(R, K, device="cuda"), "mxfp4")
+    wq, ws = ops.quantize_fp4(torch.ones(3, N, K, device="cuda"), "mxfp4")
+    off = torch.tensor(offsets, dtype=torch.int32, device="cuda")
+    y = torch.full((R, N), 5.0, device="cuda", dtype=torch.bfloat16)
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    capi.call("lmoe_fp4_grouped_gemm", xq.data_ptr(), xs.data_ptr(), 32, R, K, wq.data_ptr(), ws.data_ptr(), None,
+              None, 32, N, 0, off.data_ptr(), 0, 3, None, None, 0, y.data_ptr(), err.data_ptr(), capi.stream_handle())
+    assert (y == 0).all() and err.item() != 0
+
+
+def test_scales_on_other_pitches_and_views_of_codes():
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    R, N, K, fmt = 70, 96, 320, "nvfp4"
+    off = torch.tensor([0, 30, 70], dtype=torch.int32, device="cuda")
+    xq, xs = _operand((R, K), fmt, gen)
+    wq, ws = _operand((2, N, K), fmt, gen)
+    uq, us = _operand((2, N, K), fmt, gen)
+    want = ops.fp4_grouped_gemm(xq, xs, wq, ws, off, 2, fmt)
+    both = ops.fp4_grouped_gemm(xq, xs, wq, ws, off, 2, fmt, weights_up=uq, weight_scales_up=us)
+    xsc, wsc = xs.contiguous(), ws.contiguous()                      # 20 bytes a row
+    assert torch.equal(ops.fp4_grouped_gemm(xq, xsc, wq, wsc, off, 2, fmt), want)
+    wide = torch.zeros(2, N, 64, dtype=torch.uint8, device="cuda")   # another pitch of 32s
+    wide[..., :20] = ws
+    assert torch.equal(ops.fp4_grouped_gemm(xq, xs, wq, wide[..., :20], off, 2, fmt), want)
+    assert torch.equal(ops.fp4_grouped_gemm(xq, xs, wq, wide[..., :20], off, 2, fmt, weights_up=uq,
+                                            weight_scales_up=us), both)
+    assert torch.equal(ops.fp4_grouped_gemm(xq, xs, wq, ws, off, 2, fmt, weights_up=uq,
+                                            weight_scales_up=us.contiguous()), both)
+    xw = torch.zeros(R, K // 2 + 3, dtype=torch.uint8, device="cuda")
+    xw[:, 3:] = xq
+    assert torch.equal(ops.fp4_grouped_gemm(xw[:, 3:], xs, wq, ws, off, 2, fmt), want)
+    exact = torch.zeros(R * 32 - 12, dtype=torch.uint8, device="cuda")   # storage ends with the last row's scales
+    last = exact.as_strided((R, 20), (32, 1))
+    last.copy_(xs)
+    assert torch.equal(ops.fp4_grouped_gemm(xq, last, wq, ws, off, 2, fmt), want)
+    more = ops.fp4_grouped_gemm(xq, xs, wq, ws, off[:2], 1, fmt)     # fewer experts than weights
+    assert torch.equal(more[:30], want[:30]) and (more[30:] == 0).all()
+
+
+def test_streams_graphs_and_the_sm_limit():
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    R, N, K, fmt = 300, 500, 640, "mxfp4"
+    off = torch.tensor([0, 130, 300], dtype=torch.int32, device="cuda")
+    x = torch.randn(R, K, generator=gen, device="cuda").to(torch.bfloat16)
+    wq, ws = _operand((2, N, K), fmt, gen)
+
+    def step():
+        xq, xs = ops.quantize_fp4(x, fmt)
+        return ops.fp4_grouped_gemm(xq, xs, wq, ws, off, 2, fmt)
+
+    want = step()
+    torch.cuda.synchronize()
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.cuda.stream(s1):
+        a = step()
+    with torch.cuda.stream(s2):
+        b = step()
+    torch.cuda.synchronize()
+    assert torch.equal(a, want) and torch.equal(b, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = step()
+    x.copy_(x.flip(0))
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, step())
+    lib = capi.lib()
+    before = lib.lmoe_get_gemm_sm_limit()
+    try:
+        for cap in (1, 3, 64):
+            lib.lmoe_set_gemm_sm_limit(cap)
+            assert torch.equal(step(), y)
+    finally:
+        lib.lmoe_set_gemm_sm_limit(before)

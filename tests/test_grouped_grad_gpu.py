@@ -1,0 +1,193 @@
+"""GPU tests of the grouped product's gradients against the formula in 64 bits.
+
+Tolerance, derived: 16-bit products are exact in fp32; L of them are summed in fp32, each addition
+off by at most one unit in the last place (L * 2^-23 of the sum of absolute products); fp32
+operands round each product once more inside the fused multiply-add (the same bound); the output
+type rounds by eps / 2.
+"""
+import pytest
+import torch
+
+from light_moe_b200 import capi, ops
+
+pytestmark = pytest.mark.gpu
+DT = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+
+
+def _bounds(counts, head=0):
+    b = [head]
+    for c in counts:
+        b.append(b[-1] + c)
+    return b
+
+
+def _inputs(counts, N, K, dt, head=0, tail=0, seed=0):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    b = _bounds(counts, head)
+    R, E = b[-1] + tail, len(counts)
+    dy = torch.randn(R, N, generator=gen, device="cuda").to(dt)
+    x = torch.randn(R, K, generator=gen, device="cuda").to(dt)
+    w = (torch.randn(E, N, K, generator=gen, device="cuda") * 0.1).to(dt)
+    return dy, x, w, b, torch.tensor(b, dtype=torch.int32, device="cuda")
+
+
+def _close(got, want, mass, depth, what):
+    half = torch.finfo(got.dtype).eps / 2
+    tol = (depth + 1) * 2.0 ** -23 * mass * (1 + half) + half * want.abs() + torch.finfo(got.dtype).tiny
+    bad = ~((got.double() - want).abs() <= tol)
+    assert not bad.any(), (what, bad.sum().item(), (got.double() - want).abs().max().item())
+
+
+def _check(dy, x, w, b, off, out_dtype=None):
+    E = len(b) - 1
+    dx = ops.grouped_gemm_dgrad(dy, w, off, E)
+    dw = ops.grouped_gemm_wgrad(dy, x, off, E, out_dtype)
+    assert dx.dtype == dy.dtype and dx.shape == x.shape
+    assert dw.dtype == (out_dtype or dy.dtype) and dw.shape == w.shape
+    assert (dx[:b[0]] == 0).all() and (dx[b[-1]:] == 0).all()
+    for e in range(E):
+        r = slice(b[e], b[e + 1])
+        g, xe, we = dy[r].double(), x[r].double(), w[e].double()
+        _close(dx[r], g @ we, g.abs() @ we.abs(), w.shape[1], f"dx {e}")
+        _close(dw[e], g.T @ xe, g.abs().T @ xe.abs(), max(b[e + 1] - b[e], 1), f"dw {e}")
+    return dx, dw
+
+
+SHAPES = [
+    ([1], 64, 64), ([1, 0, 3], 8, 16), ([256], 256, 256), ([64, 65, 15, 0, 17], 256, 512), ([130, 1, 300], 320, 264),
+    ([5, 700], 1408, 520), ([33, 31], 72, 2048), ([2, 500, 2], 1000, 8),
+]
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("counts,N,K", SHAPES)
+def test_gradients(dt, counts, N, K):
+    _check(*_inputs(counts, N, K, DT[dt], seed=N + K))
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("counts,N,K", [([3, 40], 1, 1), ([20, 0, 9], 33, 64), ([129, 60], 64, 129), ([70, 300], 257, 517),
+                                        ([1], 7, 3)])
+def test_gradients_of_odd_sizes(dt, counts, N, K):
+    _check(*_inputs(counts, N, K, DT[dt], seed=N))
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+@pytest.mark.parametrize("head,tail", [(0, 0), (7, 0), (0, 300), (290, 5)])
+def test_rows_outside_every_expert(dt, head, tail):
+    """Rows outside the experts hold NaN and infinities; neither gradient sees them."""
+    dy, x, w, b, off = _inputs([30, 0, 100, 45], 136, 200, DT[dt], head, tail)
+    for t in (dy, x):
+        t[:b[0]] = float("nan")
+        t[b[-1]:] = float("inf")
+    _check(dy, x, w, b, off.long())
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp16", "fp32"])
+def test_what_is_not_finite_stays_in_its_expert(dt):
+    dy, x, w, b, off = _inputs([21, 50, 9, 70], 136, 136, DT[dt])
+    dx0, dw0 = _check(dy, x, w, b, off)
+    dy[b[1]] = float("nan")        # the row right behind expert 0
+    x[b[2] - 1] = float("inf")     # the last row of expert 1
+    w[2] = float("nan")            # right behind expert 1's matrix
+    dx = ops.grouped_gemm_dgrad(dy, w, off, 4)
+    dw = ops.grouped_gemm_wgrad(dy, x, off, 4)
+    for e in (0, 3):
+        assert torch.equal(dx[b[e]:b[e + 1]], dx0[b[e]:b[e + 1]]) and torch.equal(dw[e], dw0[e])
+    assert torch.equal(dw[2], dw0[2])
+    assert torch.isnan(dx[b[1]]).all() and torch.equal(dx[b[1] + 1:b[2]], dx0[b[1] + 1:b[2]])
+    assert torch.isnan(dw[1]).all() and torch.isnan(dx[b[2]:b[3]]).all()
+
+
+def test_weight_gradient_in_fp32_and_no_rows():
+    for dt in (torch.bfloat16, torch.float16):
+        _check(*_inputs([100, 0, 37], 264, 130, dt), out_dtype=torch.float32)
+    dy, x, w, b, off = _inputs([0, 0], 64, 64, torch.bfloat16)
+    assert ops.grouped_gemm_dgrad(dy, w, off, 2).shape == (0, 64)
+    assert (ops.grouped_gemm_wgrad(dy, x, off, 2) == 0).all()
+    assert (ops.grouped_gemm_wgrad(dy.float(), x.float(), off, 2) == 0).all()
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+def test_many_experts(dt):
+    _check(*_inputs([i % 5 * 9 for i in range(256)], 72, 80, DT[dt]))
+
+
+def test_uneven_prompt():
+    """Many tiles per pair of CTAs, loads from none to most of the rows."""
+    _check(*_inputs([0, 3000, 41, 0, 640, 257, 1], 1408, 1024, torch.bfloat16))
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+@pytest.mark.parametrize("offsets", [[0, 50, 40, 100], [-1, 20, 40, 100], [0, 20, 40, 101], [120, 130, 140, 150]])
+def test_bad_offsets_give_zeros_and_an_error_word(dt, offsets):
+    R, N, K, t = 100, 64, 64, DT[dt]
+    code = capi.dtype_code(t)
+    dy, x, w = (torch.ones(*s, device="cuda", dtype=t) for s in ((R, N), (R, K), (3, N, K)))
+    off = torch.tensor(offsets, dtype=torch.int32, device="cuda")
+    dx, dw = torch.full((R, K), 5.0, device="cuda", dtype=t), torch.full((3, N, K), 5.0, device="cuda", dtype=t)
+    e1, e2 = (torch.zeros(1, dtype=torch.int32, device="cuda") for _ in range(2))
+    capi.call("lmoe_grouped_gemm_dgrad", dy.data_ptr(), code, R, N, w.data_ptr(), K, off.data_ptr(), 0, 3,
+              dx.data_ptr(), None, 0, e1.data_ptr(), capi.stream_handle())
+    capi.call("lmoe_grouped_gemm_wgrad", dy.data_ptr(), code, R, N, x.data_ptr(), K, off.data_ptr(), 0, 3, code,
+              dw.data_ptr(), None, 0, e2.data_ptr(), capi.stream_handle())
+    assert (dx == 0).all() and (dw == 0).all() and e1.item() != 0 and e2.item() != 0
+
+
+def test_views_strides_and_more_weights_than_experts():
+    dy, x, w, b, off = _inputs([40, 60], 64, 96, torch.bfloat16)
+    dx, dw = _check(dy, x, w, b, off)
+    wide = torch.zeros(100, 67, device="cuda", dtype=torch.bfloat16)
+    wide[:, 3:] = dy
+    assert torch.equal(ops.grouped_gemm_dgrad(wide[:, 3:], w, off, 2), dx)
+    flat = torch.zeros(100 * 96 + 1, device="cuda", dtype=torch.bfloat16)
+    flat[1:] = x.reshape(-1)
+    assert torch.equal(ops.grouped_gemm_wgrad(dy, flat[1:].view(100, 96), off, 2), dw)   # contiguous, not aligned
+    assert torch.equal(ops.grouped_gemm_wgrad(dy.t().contiguous().t(), x, off, 2), dw)
+    more = torch.cat([w, torch.full_like(w, float("nan"))])
+    assert torch.equal(ops.grouped_gemm_dgrad(dy, more, off, 2), dx)
+    row = torch.randn(1, 64, device="cuda", dtype=torch.bfloat16).expand(100, 64)        # a broadcast gradient
+    assert torch.equal(ops.grouped_gemm_dgrad(row, w, off, 2), ops.grouped_gemm_dgrad(row.contiguous(), w, off, 2))
+
+
+def test_refusals_on_the_device():
+    dy, x, w, b, off = _inputs([40, 60], 64, 96, torch.bfloat16)
+    for call in (
+        lambda: ops.grouped_gemm_dgrad(dy, w.float(), off, 2),
+        lambda: ops.grouped_gemm_dgrad(dy[0], w, off, 2),
+        lambda: ops.grouped_gemm_dgrad(dy[:, :32], w, off, 2),
+        lambda: ops.grouped_gemm_dgrad(dy, w, off, 3),
+        lambda: ops.grouped_gemm_dgrad(dy, w, off[:2], 2),
+        lambda: ops.grouped_gemm_dgrad(dy, w, off.float(), 2),
+        lambda: ops.grouped_gemm_dgrad(dy, w, off.cpu(), 2),
+        lambda: ops.grouped_gemm_dgrad(dy, w.cpu(), off, 2),
+        lambda: ops.grouped_gemm_dgrad(dy.double(), w.double(), off, 2),
+        lambda: ops.grouped_gemm_wgrad(dy, x[:50], off, 2),
+        lambda: ops.grouped_gemm_wgrad(dy, x.half(), off, 2),
+        lambda: ops.grouped_gemm_wgrad(dy, x, off, 2, torch.float16),
+        lambda: ops.grouped_gemm_wgrad(dy, x, off, 0),
+    ):
+        with pytest.raises(RuntimeError):
+            call()
+
+
+def test_streams_and_graphs():
+    dy, x, w, b, off = _inputs([140, 0, 161], 264, 200, torch.bfloat16)
+    dx, dw = _check(dy, x, w, b, off)
+    torch.cuda.synchronize()
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.cuda.stream(s1):
+        a = ops.grouped_gemm_dgrad(dy, w, off, 3)
+    with torch.cuda.stream(s2):
+        c = ops.grouped_gemm_wgrad(dy, x, off, 3)
+    torch.cuda.synchronize()
+    assert torch.equal(a, dx) and torch.equal(c, dw)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        gx, gw = ops.grouped_gemm_dgrad(dy, w, off, 3), ops.grouped_gemm_wgrad(dy, x, off, 3)
+    dy.copy_(dy.flip(0))
+    off.copy_(torch.tensor([0, 10, 200, 301], dtype=torch.int32))
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(gx, ops.grouped_gemm_dgrad(dy, w, off, 3))
+    assert torch.equal(gw, ops.grouped_gemm_wgrad(dy, x, off, 3))
