@@ -17,15 +17,16 @@
 //
 // Operands stay in the canonical layout of the quantiser (codes [rows, K/2], scales [rows,
 // pitch]): the codes arrive by TMA (128-byte swizzle, 256 values = 128 bytes a row and stage).
-// The scales of a stage (8 or 16 bytes a row) must lie in shared memory as 512-byte tiles of
-// 128 rows x 4 scales, row r at (r % 32) * 16 + (r / 32) * 4, from where tcgen05.cp copies them
-// to TMEM; three warps read them as whole 32-byte sectors (four or two stages at a time, one
-// step ahead) and write the tiles with one 16-byte store per lane.
+// The scales must lie in shared memory as 512-byte tiles of 128 rows x 4 scales, row r at
+// (r % 32) * 16 + (r / 32) * 4, from where tcgen05.cp copies them to TMEM.  Three warps read them
+// as whole 32-byte sectors a row (a step: the scales of four stages of MX, two of NV), one step
+// ahead, write the tiles with one 16-byte store per lane and word, and hand a step to the leader
+// in one go: an arrival at the other CTA's barrier that releases memory costs ~900 ns.
 //
-// Warps: 0 TMA producer; 1 MMA issuer (leader CTA); 2 scales of the rows; 3, 4 scales of the
-// columns 0-127 and 128-191 (each CTA keeps all 192: the MMA reads them beside its own rows);
-// 5-16 epilogue, twelve warps of 32 rows x 64 columns.
-// A stage is ready when, in both CTAs, the codes landed and the three scale warps wrote.
+// Warps: 0 TMA producer, whose copies complete on the leader's stage barrier; 1 MMA issuer
+// (leader CTA); 2 scales of the rows; 3, 4 scales of the columns 0-127 and 128-191 (each CTA
+// keeps all 192: the MMA reads them beside its own rows); 5-16 epilogue, twelve warps of 32 rows
+// x 64 columns.
 #include <cuda_bf16.h>
 
 #include "fp4_format.cuh"
@@ -39,6 +40,7 @@ namespace {
 constexpr int kRowsCta = 128, kTM = 256, kTN = 192, kHalf = 96;
 constexpr int kSK = 256;          // values per stage: one 128-byte swizzle line of codes
 constexpr int kStages = 6, kAcc = 2;
+constexpr int kSfSlots = 3;      // steps of scales in shared memory
 constexpr int kEpiWarp0 = 5, kEpiWarps = 12;
 constexpr int kThreads = (kEpiWarp0 + kEpiWarps) * 32;
 constexpr uint32_t kABytes = kRowsCta * 128, kBBytes = kHalf * 128;
@@ -65,9 +67,10 @@ struct Fp4Args {
 };
 
 struct __align__(8) Bars {
-  uint64_t full[kStages];       // this CTA's codes landed
+  uint64_t full[kStages];       // leader: both CTAs' codes landed (one arrival each)
   uint64_t empty[kStages];      // the stage's MMAs finished (both CTAs)
-  uint64_t ready[kStages];      // leader: codes and scales of both CTAs
+  uint64_t sf_full[kSfSlots];   // leader: both CTAs' scale warps wrote the step
+  uint64_t sf_empty[kSfSlots];  // the step's scales were copied (both CTAs)
   uint64_t acc_full[kAcc];
   uint64_t acc_empty[kAcc];     // leader: both CTAs' epilogue warps
   uint64_t mma_done;
@@ -133,15 +136,16 @@ __device__ __forceinline__ void mma_fp4_pair(uint32_t d, uint64_t a, uint64_t b,
 template <int FORMAT>
 struct Cfg {
   static constexpr int kWords = FORMAT == LMOE_FP4_MX ? 2 : 4;       // 4-scale words a row and stage
-  static constexpr int kStagesPerLoad = 8 / kWords;                   // stages in a 32-byte sector
-  static constexpr uint32_t kSfABytes = kWords * 512, kSfBBytes = kWords * 1024;
-  static constexpr uint32_t kStageBytes = kABytes + kBBytes + kSfABytes + kSfBBytes;
+  static constexpr int kStep = 8 / kWords;                            // stages of a step
   static constexpr uint32_t kSfCols = kWords * 12;                    // TMEM columns: A 4, B 8 a word
-  static constexpr uint32_t kSmem = 1024 + kStages * kStageBytes + sizeof(Bars);
-  static_assert(kStageBytes % 1024 == 0, "swizzle atoms");
-  static_assert(kSmem <= 232448, "shared memory budget");
-  static_assert(kAcc * kTN + 2 * kSfCols <= kTmemCols, "tensor memory budget");
+  static constexpr int kSfBufs = FORMAT == LMOE_FP4_MX ? 4 : 2;       // TMEM buffers of a stage's scales
+  static_assert(kAcc * kTN + kSfBufs * kSfCols <= kTmemCols, "tensor memory budget");
 };
+constexpr uint32_t kStageBytes = kABytes + kBBytes;
+constexpr uint32_t kSfABytes = 8 * 512, kSfBBytes = 8 * 1024, kSfSlotBytes = kSfABytes + kSfBBytes;
+constexpr uint32_t kSmem = 1024 + kStages * kStageBytes + kSfSlots * kSfSlotBytes + sizeof(Bars);
+static_assert(kStageBytes % 1024 == 0, "swizzle atoms");
+static_assert(kSmem <= 232448, "shared memory budget");
 
 __device__ __forceinline__ float silu(float g) { return __fdividef(g, 1.0f + __expf(-g)); }
 
@@ -153,7 +157,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   using C = Cfg<FORMAT>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  Bars* bars = reinterpret_cast<Bars*>(base + kStages * C::kStageBytes);
+  uint8_t* sf_base = base + kStages * kStageBytes;
+  Bars* bars = reinterpret_cast<Bars*>(sf_base + kSfSlots * kSfSlotBytes);
   volatile int* abort_flag = &bars->abort;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t rank = cluster_ctarank();
@@ -161,9 +166,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 
   if (tid == 0) {
     for (int s = 0; s < kStages; ++s) {
-      mbar_init(&bars->full[s], 1);
+      mbar_init(&bars->full[s], 2);
       mbar_init(&bars->empty[s], 1);
-      mbar_init(&bars->ready[s], 6);
+    }
+    for (int s = 0; s < kSfSlots; ++s) {
+      mbar_init(&bars->sf_full[s], 6);
+      mbar_init(&bars->sf_empty[s], 1);
     }
     for (int s = 0; s < kAcc; ++s) {
       mbar_init(&bars->acc_full[s], 1);
@@ -196,99 +204,109 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer
-    if (lane == 0) {
-      uint32_t it = 0;
-      int hint = 0;
-      bool ok = true;
-      for (int tile = first; tile < total && ok; tile += stride) {
-        const Tile t = tile_at(seg, a.E, a.NB, tile, hint);
-        if (t.zero) continue;
-        const int r0 = t.row0 + (int)rank * kRowsCta;
-        int rows = t.row_end - r0;
-        rows = rows < 0 ? 0 : (rows > kRowsCta ? kRowsCta : rows);
-        const int boxes = (rows + 31) >> 5;   // only the boxes that hold this tile's rows
-        const CUtensorMap* wmap = SWIGLU && !leader ? &tm_up : &tm_w;
-        const int wrow = SWIGLU ? t.n * kHalf : t.n * kTN + (int)rank * kHalf;
-        for (int ks = 0; ks < KS; ++ks, ++it) {
-          const int s = it % kStages;
-          if (!mbar_wait(&bars->empty[s], ((it / kStages) & 1u) ^ 1u, a.err, abort_flag, kSite + 2)) {
-            ok = false;
-            break;
-          }
-          uint8_t* st = base + s * C::kStageBytes;
-          mbar_arrive_expect_tx(&bars->full[s], (uint32_t)boxes * 4096u + kBBytes);
+    const uint32_t full_addr = mapa_u32(&bars->full[0], 0);
+    const CUtensorMap* wmap = SWIGLU && !leader ? &tm_up : &tm_w;
+    uint32_t it = 0;
+    int hint = 0;
+    bool ok = true;
+    for (int tile = first; tile < total && ok; tile += stride) {
+      const Tile t = tile_at(seg, a.E, a.NB, tile, hint);
+      if (t.zero) continue;
+      const int r0 = t.row0 + (int)rank * kRowsCta;
+      int rows = t.row_end - r0;
+      rows = rows < 0 ? 0 : (rows > kRowsCta ? kRowsCta : rows);
+      const int boxes = (rows + 31) >> 5;   // only the boxes that hold this tile's rows
+      const int wrow = SWIGLU ? t.n * kHalf : t.n * kTN + (int)rank * kHalf;
+      for (int ks = 0; ks < KS; ++ks, ++it) {
+        const int s = it % kStages;
+        ok = warp_wait(&bars->empty[s], ((it / kStages) & 1u) ^ 1u, a.err, abort_flag, kSite + 2);
+        if (!ok) break;
+        if (elect_one()) {
+          uint8_t* st = base + s * kStageBytes;
+          const uint32_t bar = full_addr + s * 8;
+          mbar_arrive_expect_tx_cluster(bar, (uint32_t)boxes * 4096u + kBBytes);
           if (boxes == 4) {
-            tma_load_2d(st, &tm_x, &bars->full[s], ks * 128, r0);
+            tma_load_2d_pair(st, &tm_x, bar, ks * 128, r0);
           } else {
-            for (int b = 0; b < boxes; ++b)
-              tma_load_2d(st + b * 4096, &tm_x32, &bars->full[s], ks * 128, r0 + b * 32);
+            for (int b = 0; b < boxes; ++b) tma_load_2d_pair(st + b * 4096, &tm_x32, bar, ks * 128, r0 + b * 32);
           }
-          tma_load_3d(st + kABytes, wmap, &bars->full[s], ks * 128, wrow, t.e);
+          tma_load_3d_pair(st + kABytes, wmap, bar, ks * 128, wrow, t.e);
         }
       }
-      // no copy of this CTA may still be in flight when it exits
-      const uint32_t from = it > (uint32_t)kStages ? it - kStages : 0u;
-      for (uint32_t j = from; j < it; ++j)
-        mbar_wait(&bars->full[j % kStages], (j / kStages) & 1u, a.err, nullptr, kSite + 3);
     }
+    // the copies of a finished tile have landed (its MMAs read them)
+    if (!ok) let_copies_land();
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer
-    if (leader && lane == 0) {
-      uint32_t it = 0, lt = 0;
+    if (leader) {
+      uint32_t it = 0, lt = 0, step = 0;
       int hint = 0;
       bool ok = true;
       for (int tile = first; tile < total && ok; tile += stride) {
         const Tile t = tile_at(seg, a.E, a.NB, tile, hint);
         if (t.zero) continue;
         const uint32_t acc = lt % kAcc;
-        if (!mbar_wait_cluster(&bars->acc_empty[acc], ((lt / kAcc) & 1u) ^ 1u, a.err, abort_flag, kSite + 4)) break;
+        ok = warp_wait_cluster(&bars->acc_empty[acc], ((lt / kAcc) & 1u) ^ 1u, a.err, abort_flag, kSite + 4);
+        if (!ok) break;
         const uint32_t d = tmem + acc * kTN;
         for (int ks = 0; ks < KS; ++ks, ++it) {
           const int s = it % kStages;
-          // the scale buffer of this stage was last read by the MMAs of the stage before last
-          if (it >= 2 && !mbar_wait(&bars->empty[(it - 2) % kStages], ((it - 2) / kStages) & 1u, a.err, abort_flag,
-                                    kSite + 5)) { ok = false; break; }
-          if (!mbar_wait_cluster(&bars->ready[s], (it / kStages) & 1u, a.err, abort_flag, kSite + 6)) {
-            ok = false;
-            break;
-          }
+          const int part = ks % C::kStep;   // stage within the step of scales
+          const uint32_t slot = step % kSfSlots;
+          const bool last = part == C::kStep - 1 || ks == KS - 1;
+          // the TMEM buffer of this stage's scales was last read by the MMAs of kSfBufs stages ago
+          if (it >= (uint32_t)C::kSfBufs)
+            ok = warp_wait(&bars->empty[(it - C::kSfBufs) % kStages], ((it - C::kSfBufs) / kStages) & 1u, a.err,
+                           abort_flag, kSite + 5);
+          if (ok && part == 0)
+            ok = warp_wait_cluster(&bars->sf_full[slot], (step / kSfSlots) & 1u, a.err, abort_flag, kSite + 9);
+          if (ok) ok = warp_wait(&bars->full[s], (it / kStages) & 1u, a.err, abort_flag, kSite + 6);
+          if (!ok) break;
           tc_fence_after();
-          const uint32_t st = smem_u32(base + s * C::kStageBytes);
-          const uint32_t sfa = tmem + kAcc * kTN + (it & 1u) * C::kSfCols, sfb = sfa + C::kWords * 4;
+          if (elect_one()) {
+            const uint32_t sfa = tmem + kAcc * kTN + (it % C::kSfBufs) * C::kSfCols, sfb = sfa + C::kWords * 4;
+            const uint32_t sf = smem_u32(sf_base + slot * kSfSlotBytes);
 #pragma unroll
-          for (int w = 0; w < C::kWords; ++w) {
-            copy_scales_pair(sfa + w * 4, sdesc_scales(st + kABytes + kBBytes + w * 512));
-            copy_scales_pair(sfb + w * 8, sdesc_scales(st + kABytes + kBBytes + C::kSfABytes + w * 1024));
-            copy_scales_pair(sfb + w * 8 + 4, sdesc_scales(st + kABytes + kBBytes + C::kSfABytes + w * 1024 + 512));
+            for (int w = 0; w < C::kWords; ++w) {
+              const uint32_t q = part * C::kWords + w;
+              copy_scales_pair(sfa + w * 4, sdesc_scales(sf + q * 512));
+              copy_scales_pair(sfb + w * 8, sdesc_scales(sf + kSfABytes + q * 1024));
+              copy_scales_pair(sfb + w * 8 + 4, sdesc_scales(sf + kSfABytes + q * 1024 + 512));
+            }
+            const uint32_t st = smem_u32(base + s * kStageBytes);
+            const int left = a.K - ks * kSK;
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk) {   // 64 values per MMA
+              if (kk * 64 >= left) break;
+              const uint32_t accum = (ks | kk) != 0 ? 1u : 0u;
+              const uint64_t ad = sdesc_k_sw128(st + kk * 32), bd = sdesc_k_sw128(st + kABytes + kk * 32);
+              if (FORMAT == LMOE_FP4_MX)
+                // a word holds the scales of 128 values: of two MMAs (scale id 0 and 2)
+                mma_fp4_pair<FORMAT>(d, ad, bd, idesc_fp4(true, (kk & 1) * 2), sfa + (kk >> 1) * 4,
+                                     sfb + (kk >> 1) * 8, accum);
+              else
+                mma_fp4_pair<FORMAT>(d, ad, bd, idesc_fp4(false, 0), sfa + kk * 4, sfb + kk * 8, accum);
+            }
+            mma_commit_pair(&bars->empty[s]);
+            if (last) mma_commit_pair(&bars->sf_empty[slot]);
+            if (ks == KS - 1) mma_commit_pair(&bars->acc_full[acc]);
           }
-          const int left = a.K - ks * kSK;
-          const int nk = left >= kSK ? 4 : (left + 63) / 64;   // 64 values per MMA
-          for (int kk = 0; kk < nk; ++kk) {
-            const uint32_t accum = (ks | kk) != 0 ? 1u : 0u;
-            const uint64_t ad = sdesc_k_sw128(st + kk * 32), bd = sdesc_k_sw128(st + kABytes + kk * 32);
-            if (FORMAT == LMOE_FP4_MX)
-              // a word holds the scales of 128 values: of two MMAs (scale id 0 and 2)
-              mma_fp4_pair<FORMAT>(d, ad, bd, idesc_fp4(true, (kk & 1) * 2), sfa + (kk >> 1) * 4, sfb + (kk >> 1) * 8,
-                                   accum);
-            else
-              mma_fp4_pair<FORMAT>(d, ad, bd, idesc_fp4(false, 0), sfa + kk * 4, sfb + kk * 8, accum);
-          }
-          mma_commit_pair(&bars->empty[s]);
+          __syncwarp();
+          step += last ? 1 : 0;
         }
-        if (ok) mma_commit_pair(&bars->acc_full[acc]);
         ++lt;
       }
-      mma_commit_pair(&bars->mma_done);
+      if (elect_one()) mma_commit_pair(&bars->mma_done);
       mbar_wait(&bars->mma_done, 0, a.err, nullptr, kSite + 7);
     }
   } else if (warp < kEpiWarp0) {
     // ------------------------------------------------------------------ scales
     const int part = warp - 2;   // 0: rows, 1: columns 0-127, 2: columns 128-191
     const int nb = a.K / fp4_block(FORMAT);
-    const uint32_t dst0 = kABytes + kBBytes + (part == 0 ? 0u : C::kSfABytes + (part - 1) * 512u);
+    uint8_t* dst = sf_base + (part == 0 ? 0u : kSfABytes + (part - 1) * 512u) + lane * 16;
     const uint32_t dst_word = part == 0 ? 512u : 1024u;
-    const int steps = (KS + C::kStagesPerLoad - 1) / C::kStagesPerLoad;   // 32-byte loads a row
-    const uint32_t ready_addr = mapa_u32(&bars->ready[0], 0);
+    const int steps = (KS + C::kStep - 1) / C::kStep;   // 32-byte loads a row
+    const uint32_t full_addr = mapa_u32(&bars->sf_full[0], 0);
     // the lane's four rows (r = lane + 32 i) of a tile, NULL where there is none
     auto sources = [&](const Tile& t, const uint8_t* (&p)[4]) {
 #pragma unroll
@@ -314,7 +332,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           v[i][h] = p[i] ? __ldg(reinterpret_cast<const uint4*>(p[i] + step * 32) + h) : make_uint4(0, 0, 0, 0);
       }
     };
-    uint32_t it = 0;
+    uint32_t done = 0;   // steps handed over
     int hint = 0;
     // the next load: tile and step
     int ltile = first;
@@ -359,33 +377,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           }
         }
       }
+      const uint32_t slot = done % kSfSlots;
+      ok = mbar_wait(&bars->sf_empty[slot], ((done / kSfSlots) & 1u) ^ 1u, a.err, abort_flag, kSite + 8);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
 #pragma unroll
-      for (int g = 0; g < C::kStagesPerLoad; ++g) {
-        if (step * C::kStagesPerLoad + g < KS && ok) {
-          const int s = it % kStages;
-          if (!mbar_wait(&bars->empty[s], ((it / kStages) & 1u) ^ 1u, a.err, abort_flag, kSite + 8)) ok = false;
-          ok = __all_sync(0xffffffffu, ok);
-          if (ok) {
-            uint8_t* st = base + s * C::kStageBytes + dst0 + lane * 16;
+      for (int q = 0; q < 8; ++q) {
+        uint32_t o[4];
 #pragma unroll
-            for (int w = 0; w < C::kWords; ++w) {
-              const int q = g * C::kWords + w;   // word of the sector
-              uint32_t o[4];
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const uint4 v = cur[i][q >> 2];
-                o[i] = (q & 3) == 0 ? v.x : (q & 3) == 1 ? v.y : (q & 3) == 2 ? v.z : v.w;
-              }
-              *reinterpret_cast<uint4*>(st + w * dst_word) = make_uint4(o[0], o[1], o[2], o[3]);
-            }
-            fence_proxy_async_smem();
-            if (part == 0 && !mbar_wait(&bars->full[s], (it / kStages) & 1u, a.err, abort_flag, kSite + 9)) ok = false;
-            ok = __all_sync(0xffffffffu, ok);
-            if (ok && lane == 0) mbar_arrive_cluster(ready_addr + s * 8);
-          }
-          ++it;
+        for (int i = 0; i < 4; ++i) {
+          const uint4 v = cur[i][q >> 2];
+          o[i] = (q & 3) == 0 ? v.x : (q & 3) == 1 ? v.y : (q & 3) == 2 ? v.z : v.w;
         }
+        *reinterpret_cast<uint4*>(dst + slot * kSfSlotBytes + q * dst_word) = make_uint4(o[0], o[1], o[2], o[3]);
       }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(full_addr + slot * 8);
+      ++done;
     }
   } else {
     // ------------------------------------------------------------------ epilogue
@@ -459,9 +468,9 @@ template <int FORMAT, bool SWIGLU>
 int launch(const CUtensorMap& x, const CUtensorMap& x32, const CUtensorMap& w, const CUtensorMap& up, const Fp4Args& a,
            int grid, cudaStream_t stream) {
   auto fn = fp4_gemm_kernel<FORMAT, SWIGLU>;
-  const int st = set_max_dynamic_smem(reinterpret_cast<const void*>(fn), Cfg<FORMAT>::kSmem);
+  const int st = set_max_dynamic_smem(reinterpret_cast<const void*>(fn), kSmem);
   if (st != LMOE_OK) return st;
-  fn<<<grid, kThreads, Cfg<FORMAT>::kSmem, stream>>>(x, x32, w, up, a);
+  fn<<<grid, kThreads, kSmem, stream>>>(x, x32, w, up, a);
   return cuda_status(cudaGetLastError());
 }
 

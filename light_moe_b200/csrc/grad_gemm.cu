@@ -18,8 +18,9 @@
 // a product with a zero row would not do, since those rows may hold infinities or NaN.  Experts
 // without rows get a zero dw, rows outside every expert a zero dx.
 //
-// Warps: 0 TMA producer; 1 MMA issuer (leader CTA); 2 hands each landed stage to the leader
-// after clearing its tail; 4-11 epilogue, eight warps of 32 rows x 128 columns.
+// Warps: 0 TMA producer, whose copies complete on the leader's stage barrier; 1 MMA issuer
+// (leader CTA); 2 clears the tail of a segment's last stage (whose copies complete on a barrier
+// of its own CTA) and hands it to the leader; 4-11 epilogue, eight warps of 32 rows x 128 columns.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -57,9 +58,9 @@ struct GradArgs {
 };
 
 struct __align__(8) Bars {
-  uint64_t full[kStages];       // this CTA's operands landed
+  uint64_t full[kStages];       // leader: both CTAs' operands landed (one arrival each)
   uint64_t empty[kStages];      // the stage's MMAs finished (both CTAs)
-  uint64_t ready[kStages];      // leader: both CTAs' operands
+  uint64_t tail[kStages];       // this CTA's operands of a stage with a tail to clear
   uint64_t acc_full[kAcc];
   uint64_t acc_empty[kAcc];     // leader: both CTAs' epilogue warps
   uint64_t mma_done;
@@ -94,6 +95,9 @@ __device__ __forceinline__ Tile tile_at(const SegTable& t, const GradArgs& a, in
   return r;
 }
 
+// Whether a stage with `left` rows of its segment ends inside the 16 rows of an MMA.
+__device__ __forceinline__ bool has_tail(int left) { return left < kSK && (left & 15) != 0; }
+
 template <int FORM>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     grad_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_a32,
@@ -108,9 +112,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 
   if (tid == 0) {
     for (int s = 0; s < kStages; ++s) {
-      mbar_init(&bars->full[s], 1);
+      mbar_init(&bars->full[s], 2);
       mbar_init(&bars->empty[s], 1);
-      mbar_init(&bars->ready[s], 2);
+      mbar_init(&bars->tail[s], 1);
     }
     for (int s = 0; s < kAcc; ++s) {
       mbar_init(&bars->acc_full[s], 1);
@@ -143,54 +147,61 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer
-    if (lane == 0) {
-      uint32_t it = 0;
-      int hint = 0;
-      bool ok = true;
-      for (int tile = first; tile < total && ok; tile += stride) {
-        const Tile t = tile_at<FORM>(seg, a, tile, hint);
-        const int c0 = t.n * kTile + (int)rank * kCta;   // first column of B
-        const int m0 = (FORM == kInputGrad ? t.row0 : t.m * kTile) + (int)rank * kCta;
-        int boxes = 4;   // input gradient: 32-row boxes of dy that hold this CTA's rows
-        if (FORM == kInputGrad) {
-          const int rows = t.row_end - m0;
-          boxes = rows <= 0 ? 0 : (rows >= kCta ? 4 : (rows + 31) >> 5);
-        }
-        for (int ks = 0; ks < t.ks; ++ks, ++it) {
-          const int s = it % kStages;
-          if (!mbar_wait(&bars->empty[s], ((it / kStages) & 1u) ^ 1u, a.err, abort_flag, kSite + 2)) {
-            ok = false;
-            break;
-          }
+    const uint32_t full_addr = mapa_u32(&bars->full[0], 0);
+    uint32_t it = 0;
+    int hint = 0;
+    bool ok = true;
+    for (int tile = first; tile < total && ok; tile += stride) {
+      const Tile t = tile_at<FORM>(seg, a, tile, hint);
+      const int c0 = t.n * kTile + (int)rank * kCta;   // first column of B
+      const int m0 = (FORM == kInputGrad ? t.row0 : t.m * kTile) + (int)rank * kCta;
+      int boxes = 4;   // input gradient: 32-row boxes of dy that hold this CTA's rows
+      if (FORM == kInputGrad) {
+        const int rows = t.row_end - m0;
+        boxes = rows <= 0 ? 0 : (rows >= kCta ? 4 : (rows + 31) >> 5);
+      }
+      for (int ks = 0; ks < t.ks; ++ks, ++it) {
+        const int s = it % kStages;
+        ok = warp_wait(&bars->empty[s], ((it / kStages) & 1u) ^ 1u, a.err, abort_flag, kSite + 2);
+        if (!ok) break;
+        if (elect_one()) {
           uint8_t* sa = base + s * kStageBytes;
           uint8_t* sb = sa + kOperand;
-          uint64_t* bar = &bars->full[s];
-          mbar_arrive_expect_tx(bar, (uint32_t)boxes * 4096u + kOperand);
+          const uint32_t bar = full_addr + s * 8;
           if (FORM == kInputGrad) {
+            mbar_arrive_expect_tx_cluster(bar, (uint32_t)boxes * 4096u + kOperand);
             if (boxes == 4) {
-              tma_load_2d(sa, &tm_a, bar, ks * kSK, m0);
+              tma_load_2d_pair(sa, &tm_a, bar, ks * kSK, m0);
             } else {
-              for (int b = 0; b < boxes; ++b) tma_load_2d(sa + b * 4096, &tm_a32, bar, ks * kSK, m0 + b * 32);
+              for (int b = 0; b < boxes; ++b) tma_load_2d_pair(sa + b * 4096, &tm_a32, bar, ks * kSK, m0 + b * 32);
             }
-            tma_load_3d(sb, &tm_b, bar, c0, ks * kSK, t.e);
-            tma_load_3d(sb + kChunk, &tm_b, bar, c0 + 64, ks * kSK, t.e);
+            tma_load_3d_pair(sb, &tm_b, bar, c0, ks * kSK, t.e);
+            tma_load_3d_pair(sb + kChunk, &tm_b, bar, c0 + 64, ks * kSK, t.e);
           } else {
             const int r = t.row0 + ks * kSK;
-            tma_load_2d(sa, &tm_a, bar, m0, r);
-            tma_load_2d(sa + kChunk, &tm_a, bar, m0 + 64, r);
-            tma_load_2d(sb, &tm_b, bar, c0, r);
-            tma_load_2d(sb + kChunk, &tm_b, bar, c0 + 64, r);
+            if (has_tail(t.row_end - r)) {
+              uint64_t* own = &bars->tail[s];
+              mbar_arrive_expect_tx(own, 2 * kOperand);
+              tma_load_2d(sa, &tm_a, own, m0, r);
+              tma_load_2d(sa + kChunk, &tm_a, own, m0 + 64, r);
+              tma_load_2d(sb, &tm_b, own, c0, r);
+              tma_load_2d(sb + kChunk, &tm_b, own, c0 + 64, r);
+            } else {
+              mbar_arrive_expect_tx_cluster(bar, 2 * kOperand);
+              tma_load_2d_pair(sa, &tm_a, bar, m0, r);
+              tma_load_2d_pair(sa + kChunk, &tm_a, bar, m0 + 64, r);
+              tma_load_2d_pair(sb, &tm_b, bar, c0, r);
+              tma_load_2d_pair(sb + kChunk, &tm_b, bar, c0 + 64, r);
+            }
           }
         }
       }
-      // no copy of this CTA may still be in flight when it exits
-      const uint32_t from = it > (uint32_t)kStages ? it - kStages : 0u;
-      for (uint32_t j = from; j < it; ++j)
-        mbar_wait(&bars->full[j % kStages], (j / kStages) & 1u, a.err, nullptr, kSite + 3);
     }
+    // the copies of a finished tile have landed (its MMAs read them)
+    if (!ok) let_copies_land();
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer
-    if (leader && lane == 0) {
+    if (leader) {
       const uint32_t idesc = idesc_f16kind_f32(kTile, kTile, a.f16) | kIdescBMajorMN |
                              (FORM == kWeightGrad ? kIdescAMajorMN : 0u);
       uint32_t it = 0, lt = 0;
@@ -200,59 +211,63 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const Tile t = tile_at<FORM>(seg, a, tile, hint);
         if (t.ks == 0) continue;
         const uint32_t acc = lt % kAcc;
-        if (!mbar_wait_cluster(&bars->acc_empty[acc], ((lt / kAcc) & 1u) ^ 1u, a.err, abort_flag, kSite + 4)) break;
+        ok = warp_wait_cluster(&bars->acc_empty[acc], ((lt / kAcc) & 1u) ^ 1u, a.err, abort_flag, kSite + 4);
+        if (!ok) break;
         const uint32_t d = tmem + acc * kTile;
         const int depth = FORM == kInputGrad ? a.N : t.row_end - t.row0;
         for (int ks = 0; ks < t.ks; ++ks, ++it) {
           const int s = it % kStages;
-          if (!mbar_wait_cluster(&bars->ready[s], (it / kStages) & 1u, a.err, abort_flag, kSite + 6)) {
-            ok = false;
-            break;
-          }
+          ok = warp_wait_cluster(&bars->full[s], (it / kStages) & 1u, a.err, abort_flag, kSite + 6);
+          if (!ok) break;
           tc_fence_after();
-          const uint32_t sa = smem_u32(base + s * kStageBytes), sb = sa + kOperand;
-          const int left = depth - ks * kSK;
-          const int nk = left >= kSK ? 4 : (left + 15) / 16;
-          for (int kk = 0; kk < nk; ++kk) {
-            const uint64_t ad = FORM == kInputGrad ? sdesc_k_sw128(sa + kk * 32) : sdesc_mn_sw128(sa + kk * 2048, kChunk);
-            mma_ss_pair(d, ad, sdesc_mn_sw128(sb + kk * 2048, kChunk), idesc, (ks | kk) != 0 ? 1u : 0u);
+          if (elect_one()) {
+            const uint32_t sa = smem_u32(base + s * kStageBytes), sb = sa + kOperand;
+            const int left = depth - ks * kSK;
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk) {
+              if (kk * 16 >= left) break;
+              const uint64_t ad =
+                  FORM == kInputGrad ? sdesc_k_sw128(sa + kk * 32) : sdesc_mn_sw128(sa + kk * 2048, kChunk);
+              mma_ss_pair(d, ad, sdesc_mn_sw128(sb + kk * 2048, kChunk), idesc, (ks | kk) != 0 ? 1u : 0u);
+            }
+            mma_commit_pair(&bars->empty[s]);
+            if (ks == t.ks - 1) mma_commit_pair(&bars->acc_full[acc]);
           }
-          mma_commit_pair(&bars->empty[s]);
+          __syncwarp();
         }
-        if (ok) mma_commit_pair(&bars->acc_full[acc]);
         ++lt;
       }
-      mma_commit_pair(&bars->mma_done);
+      if (elect_one()) mma_commit_pair(&bars->mma_done);
       mbar_wait(&bars->mma_done, 0, a.err, nullptr, kSite + 7);
     }
   } else if (warp == 2) {
-    // ------------------------------------------------------------------ stage hand-over
-    uint32_t it = 0;
-    int hint = 0;
-    bool ok = true;
-    for (int tile = first; tile < total && ok; tile += stride) {
-      const Tile t = tile_at<FORM>(seg, a, tile, hint);
-      for (int ks = 0; ks < t.ks; ++ks, ++it) {
-        const int s = it % kStages;
-        ok = mbar_wait(&bars->full[s], (it / kStages) & 1u, a.err, abort_flag, kSite + 8);
+    // ------------------------------------------------------------------ segment tails
+    if (FORM == kWeightGrad) {
+      uint32_t it = 0, tail_parity = 0;   // a bit per stage
+      int hint = 0;
+      bool ok = true;
+      for (int tile = first; tile < total && ok; tile += stride) {
+        const Tile t = tile_at<FORM>(seg, a, tile, hint);
+        if (t.ks == 0) continue;
+        it += t.ks;
+        const int left = t.row_end - t.row0 - (t.ks - 1) * kSK;
+        if (!has_tail(left)) continue;
+        const int s = (it - 1) % kStages;
+        ok = mbar_wait(&bars->tail[s], tail_parity >> s & 1u, a.err, abort_flag, kSite + 8);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        if (FORM == kWeightGrad) {
-          const int left = t.row_end - t.row0 - ks * kSK;
-          if (left < kSK && (left & 15) != 0) {
-            // contraction rows [left, next multiple of 16) of the four chunks; a row is one
-            // 128-byte line, which the swizzle only permutes
-            const int n = (16 - (left & 15)) * 8;
-            uint8_t* st = base + s * kStageBytes + left * 128;
-            for (int i = lane; i < 4 * n; i += 32) {
-              const int c = i / n;
-              *reinterpret_cast<uint4*>(st + c * kChunk + (i - c * n) * 16) = make_uint4(0, 0, 0, 0);
-            }
-          }
+        tail_parity ^= 1u << s;
+        // contraction rows [left, next multiple of 16) of the four chunks; a row is one 128-byte
+        // line, which the swizzle only permutes
+        const int n = (16 - (left & 15)) * 8;
+        uint8_t* st = base + s * kStageBytes + left * 128;
+        for (int i = lane; i < 4 * n; i += 32) {
+          const int c = i / n;
+          *reinterpret_cast<uint4*>(st + c * kChunk + (i - c * n) * 16) = make_uint4(0, 0, 0, 0);
         }
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(mapa_u32(&bars->ready[s], 0));
+        if (lane == 0) mbar_arrive_cluster(mapa_u32(&bars->full[s], 0));
       }
     }
   } else if (warp >= kEpiWarp0) {

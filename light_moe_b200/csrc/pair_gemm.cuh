@@ -37,6 +37,12 @@ __device__ __forceinline__ uint32_t mapa_u32(const void* p, uint32_t rank) {
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
+// One arrival that also expects `bytes` of copies; it orders no memory (the copies do that).
+__device__ __forceinline__ void mbar_arrive_expect_tx_cluster(uint32_t cluster_addr, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.relaxed.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(cluster_addr),
+               "r"(bytes)
+               : "memory");
+}
 __device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
@@ -65,6 +71,48 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity
       }
     }
   }
+}
+
+// Tiled loads into this CTA's shared memory that complete on a barrier of the leader CTA
+// (`bar`: its shared-cluster address).  A hand-over by a warp of each CTA would cost an arrival
+// with release at cluster scope per stage, which measured ~900 ns (the input gradient of 8192
+// rows, N = 14336, K = 4096: 1447 us with the hand-over).
+__device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, uint32_t bar, int32_t x, int32_t y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], "
+      "[%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_3d_pair(void* dst, const CUtensorMap* map, uint32_t bar, int32_t x, int32_t y,
+                                                 int32_t z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, "
+      "%5}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+
+// A producer that gives up leaves its copies a millisecond to land (they take microseconds)
+// before its CTA may exit.
+__device__ __forceinline__ void let_copies_land() {
+  const uint64_t t0 = globaltimer_ns();
+  while (globaltimer_ns() - t0 < 1000000ull) {
+  }
+}
+
+// The waits of a whole warp, with one answer for all its lanes.  The warps that issue copies and
+// MMAs run their loops with all lanes and issue under elect.sync: under `lane == 0` the compiler
+// cannot tell that the operands are uniform, and every tcgen05 instruction then costs the thread
+// ~60 cycles (measured: the 4-bit product of 16384 rows took 1838 us, 890 cycles of issuer time
+// per stage of 384 cycles of MMAs).
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, uint32_t* err, volatile int* abort,
+                                          uint32_t site) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, err, abort, site));
+}
+__device__ __forceinline__ bool warp_wait_cluster(uint64_t* bar, uint32_t parity, uint32_t* err, volatile int* abort,
+                                                  uint32_t site) {
+  return __all_sync(0xffffffffu, mbar_wait_cluster(bar, parity, err, abort, site));
 }
 
 // ---------------------------------------------------------------------------------------
