@@ -23,10 +23,15 @@
 // ahead, write the tiles with one 16-byte store per lane and word, and hand a step to the leader
 // in one go: an arrival at the other CTA's barrier that releases memory costs ~900 ns.
 //
+// The copies to TMEM and the MMAs are issued by two warps.  A unit of two 4-scale words a row
+// (256 values of MX, 128 of NV: 24 TMEM columns, six copies) is copied ahead into a ring of five,
+// and commits of the two warps hand the units back and forth; with one warp issuing both, its
+// waits and copies stood between the MMAs.
+//
 // Warps: 0 TMA producer, whose copies complete on the leader's stage barrier; 1 MMA issuer
 // (leader CTA); 2 scales of the rows; 3, 4 scales of the columns 0-127 and 128-191 (each CTA
-// keeps all 192: the MMA reads them beside its own rows); 5-16 epilogue, twelve warps of 32 rows
-// x 64 columns.
+// keeps all 192: the MMA reads them beside its own rows); 5 copies the scales to TMEM (leader
+// CTA); 6-17 epilogue, twelve warps of 32 rows x 64 columns.
 #include <cuda_bf16.h>
 
 #include "fp4_format.cuh"
@@ -41,7 +46,9 @@ constexpr int kRowsCta = 128, kTM = 256, kTN = 192, kHalf = 96;
 constexpr int kSK = 256;          // values per stage: one 128-byte swizzle line of codes
 constexpr int kStages = 6, kAcc = 2;
 constexpr int kSfSlots = 3;      // steps of scales in shared memory
-constexpr int kEpiWarp0 = 5, kEpiWarps = 12;
+constexpr int kCopyWarp = 5, kEpiWarp0 = 6, kEpiWarps = 12;
+constexpr int kUnits = 5;        // units of scales in TMEM
+constexpr uint32_t kUnitCols = 24;   // 2 words x (4 columns of the rows' scales, 8 of the columns')
 constexpr int kThreads = (kEpiWarp0 + kEpiWarps) * 32;
 constexpr uint32_t kABytes = kRowsCta * 128, kBBytes = kHalf * 128;
 constexpr uint32_t kSite = 0x500u;
@@ -71,9 +78,11 @@ struct __align__(8) Bars {
   uint64_t empty[kStages];      // the stage's MMAs finished (both CTAs)
   uint64_t sf_full[kSfSlots];   // leader: both CTAs' scale warps wrote the step
   uint64_t sf_empty[kSfSlots];  // the step's scales were copied (both CTAs)
+  uint64_t unit_full[kUnits];   // leader: the unit's scales are in TMEM
+  uint64_t unit_empty[kUnits];  // leader: the unit's MMAs finished
   uint64_t acc_full[kAcc];
   uint64_t acc_empty[kAcc];     // leader: both CTAs' epilogue warps
-  uint64_t mma_done;
+  uint64_t mma_done, copy_done;
   uint32_t tmem_base;
   int abort;
   SegTable seg;
@@ -135,12 +144,11 @@ __device__ __forceinline__ void mma_fp4_pair(uint32_t d, uint64_t a, uint64_t b,
 
 template <int FORMAT>
 struct Cfg {
-  static constexpr int kWords = FORMAT == LMOE_FP4_MX ? 2 : 4;       // 4-scale words a row and stage
-  static constexpr int kStep = 8 / kWords;                            // stages of a step
-  static constexpr uint32_t kSfCols = kWords * 12;                    // TMEM columns: A 4, B 8 a word
-  static constexpr int kSfBufs = FORMAT == LMOE_FP4_MX ? 4 : 2;       // TMEM buffers of a stage's scales
-  static_assert(kAcc * kTN + kSfBufs * kSfCols <= kTmemCols, "tensor memory budget");
+  static constexpr int kUnitK = FORMAT == LMOE_FP4_MX ? 256 : 128;   // values of a unit
+  static constexpr int kStageUnits = kSK / kUnitK;
+  static constexpr int kStepK = 4 * kUnitK;                          // values of a step (8 words)
 };
+static_assert(kAcc * kTN + kUnits * kUnitCols <= kTmemCols, "tensor memory budget");
 constexpr uint32_t kStageBytes = kABytes + kBBytes;
 constexpr uint32_t kSfABytes = 8 * 512, kSfBBytes = 8 * 1024, kSfSlotBytes = kSfABytes + kSfBBytes;
 constexpr uint32_t kSmem = 1024 + kStages * kStageBytes + kSfSlots * kSfSlotBytes + sizeof(Bars);
@@ -173,11 +181,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       mbar_init(&bars->sf_full[s], 6);
       mbar_init(&bars->sf_empty[s], 1);
     }
+    for (int s = 0; s < kUnits; ++s) {
+      mbar_init(&bars->unit_full[s], 1);
+      mbar_init(&bars->unit_empty[s], 1);
+    }
     for (int s = 0; s < kAcc; ++s) {
       mbar_init(&bars->acc_full[s], 1);
       mbar_init(&bars->acc_empty[s], 2 * kEpiWarps);
     }
     mbar_init(&bars->mma_done, 1);
+    mbar_init(&bars->copy_done, 1);
     bars->abort = 0;
     fence_mbar_init();
   }
@@ -206,7 +219,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     // ------------------------------------------------------------------ TMA producer
     const uint32_t full_addr = mapa_u32(&bars->full[0], 0);
     const CUtensorMap* wmap = SWIGLU && !leader ? &tm_up : &tm_w;
-    uint32_t it = 0;
+    Ring<kStages> st;
     int hint = 0;
     bool ok = true;
     for (int tile = first; tile < total && ok; tile += stride) {
@@ -217,20 +230,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       rows = rows < 0 ? 0 : (rows > kRowsCta ? kRowsCta : rows);
       const int boxes = (rows + 31) >> 5;   // only the boxes that hold this tile's rows
       const int wrow = SWIGLU ? t.n * kHalf : t.n * kTN + (int)rank * kHalf;
-      for (int ks = 0; ks < KS; ++ks, ++it) {
-        const int s = it % kStages;
-        ok = warp_wait(&bars->empty[s], ((it / kStages) & 1u) ^ 1u, a.err, abort_flag, kSite + 2);
+      for (int ks = 0; ks < KS; ++ks, st.next()) {
+        ok = warp_wait(&bars->empty[st.i], st.phase ^ 1u, a.err, abort_flag, kSite + 2);
         if (!ok) break;
         if (elect_one()) {
-          uint8_t* st = base + s * kStageBytes;
-          const uint32_t bar = full_addr + s * 8;
+          uint8_t* dst = base + st.i * kStageBytes;
+          const uint32_t bar = full_addr + st.i * 8;
           mbar_arrive_expect_tx_cluster(bar, (uint32_t)boxes * 4096u + kBBytes);
           if (boxes == 4) {
-            tma_load_2d_pair(st, &tm_x, bar, ks * 128, r0);
+            tma_load_2d_pair(dst, &tm_x, bar, ks * 128, r0);
           } else {
-            for (int b = 0; b < boxes; ++b) tma_load_2d_pair(st + b * 4096, &tm_x32, bar, ks * 128, r0 + b * 32);
+            for (int b = 0; b < boxes; ++b) tma_load_2d_pair(dst + b * 4096, &tm_x32, bar, ks * 128, r0 + b * 32);
           }
-          tma_load_3d_pair(st + kABytes, wmap, bar, ks * 128, wrow, t.e);
+          tma_load_3d_pair(dst + kABytes, wmap, bar, ks * 128, wrow, t.e);
         }
       }
     }
@@ -239,73 +251,114 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer
     if (leader) {
-      uint32_t it = 0, lt = 0, step = 0;
+      const uint64_t adesc0 = sdesc_k_sw128(smem_u32(base)), bdesc0 = sdesc_k_sw128(smem_u32(base) + kABytes);
+      Ring<kStages> st;
+      Ring<kUnits> un;
+      Ring<kAcc> ac;
       int hint = 0;
       bool ok = true;
       for (int tile = first; tile < total && ok; tile += stride) {
         const Tile t = tile_at(seg, a.E, a.NB, tile, hint);
         if (t.zero) continue;
-        const uint32_t acc = lt % kAcc;
-        ok = warp_wait_cluster(&bars->acc_empty[acc], ((lt / kAcc) & 1u) ^ 1u, a.err, abort_flag, kSite + 4);
+        ok = warp_wait(&bars->acc_empty[ac.i], ac.phase ^ 1u, a.err, abort_flag, kSite + 4);
         if (!ok) break;
-        const uint32_t d = tmem + acc * kTN;
-        for (int ks = 0; ks < KS; ++ks, ++it) {
-          const int s = it % kStages;
-          const int part = ks % C::kStep;   // stage within the step of scales
-          const uint32_t slot = step % kSfSlots;
-          const bool last = part == C::kStep - 1 || ks == KS - 1;
-          // the TMEM buffer of this stage's scales was last read by the MMAs of kSfBufs stages ago
-          if (it >= (uint32_t)C::kSfBufs)
-            ok = warp_wait(&bars->empty[(it - C::kSfBufs) % kStages], ((it - C::kSfBufs) / kStages) & 1u, a.err,
-                           abort_flag, kSite + 5);
-          if (ok && part == 0)
-            ok = warp_wait_cluster(&bars->sf_full[slot], (step / kSfSlots) & 1u, a.err, abort_flag, kSite + 9);
-          if (ok) ok = warp_wait(&bars->full[s], (it / kStages) & 1u, a.err, abort_flag, kSite + 6);
+        const uint32_t d = tmem + ac.i * kTN;
+        int left = a.K;
+        for (int ks = 0; ks < KS; ++ks, st.next()) {
+          ok = warp_wait(&bars->full[st.i], st.phase, a.err, abort_flag, kSite + 6);
           if (!ok) break;
-          tc_fence_after();
-          if (elect_one()) {
-            const uint32_t sfa = tmem + kAcc * kTN + (it % C::kSfBufs) * C::kSfCols, sfb = sfa + C::kWords * 4;
-            const uint32_t sf = smem_u32(sf_base + slot * kSfSlotBytes);
+          // descriptors count 16 bytes; a stage is kStageBytes, 64 values (an MMA) 32 bytes
+          const uint64_t ad = adesc0 + st.i * (kStageBytes >> 4), bd = bdesc0 + st.i * (kStageBytes >> 4);
 #pragma unroll
-            for (int w = 0; w < C::kWords; ++w) {
-              const uint32_t q = part * C::kWords + w;
-              copy_scales_pair(sfa + w * 4, sdesc_scales(sf + q * 512));
-              copy_scales_pair(sfb + w * 8, sdesc_scales(sf + kSfABytes + q * 1024));
-              copy_scales_pair(sfb + w * 8 + 4, sdesc_scales(sf + kSfABytes + q * 1024 + 512));
-            }
-            const uint32_t st = smem_u32(base + s * kStageBytes);
-            const int left = a.K - ks * kSK;
+          for (int h = 0; h < C::kStageUnits; ++h) {
+            if (h * C::kUnitK >= left) break;
+            ok = warp_wait(&bars->unit_full[un.i], un.phase, a.err, abort_flag, kSite + 5);
+            if (!ok) break;
+            tc_fence_after();
+            if (elect_one()) {
+              const uint32_t sfa = tmem + kAcc * kTN + un.i * kUnitCols, sfb = sfa + 8;
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk) {   // 64 values per MMA
-              if (kk * 64 >= left) break;
-              const uint32_t accum = (ks | kk) != 0 ? 1u : 0u;
-              const uint64_t ad = sdesc_k_sw128(st + kk * 32), bd = sdesc_k_sw128(st + kABytes + kk * 32);
-              if (FORMAT == LMOE_FP4_MX)
-                // a word holds the scales of 128 values: of two MMAs (scale id 0 and 2)
-                mma_fp4_pair<FORMAT>(d, ad, bd, idesc_fp4(true, (kk & 1) * 2), sfa + (kk >> 1) * 4,
-                                     sfb + (kk >> 1) * 8, accum);
-              else
-                mma_fp4_pair<FORMAT>(d, ad, bd, idesc_fp4(false, 0), sfa + kk * 4, sfb + kk * 8, accum);
+              for (int j = 0; j < C::kUnitK / 64; ++j) {
+                const int kk = h * (C::kUnitK / 64) + j;
+                if (kk * 64 < left) {
+                  const uint32_t accum = (ks | kk) != 0 ? 1u : 0u;
+                  if (FORMAT == LMOE_FP4_MX)
+                    // a word holds the scales of 128 values: of two MMAs (scale id 0 and 2)
+                    mma_fp4_pair<FORMAT>(d, ad + kk * 2, bd + kk * 2, idesc_fp4(true, (kk & 1) * 2),
+                                         sfa + (j >> 1) * 4, sfb + (j >> 1) * 8, accum);
+                  else
+                    mma_fp4_pair<FORMAT>(d, ad + kk * 2, bd + kk * 2, idesc_fp4(false, 0), sfa + j * 4, sfb + j * 8,
+                                         accum);
+                }
+              }
+              mma_commit_leader(&bars->unit_empty[un.i]);
+              if ((h + 1) * C::kUnitK >= (left < kSK ? left : kSK)) {
+                mma_commit_pair(&bars->empty[st.i]);
+                if (ks == KS - 1) mma_commit_pair(&bars->acc_full[ac.i]);
+              }
             }
-            mma_commit_pair(&bars->empty[s]);
-            if (last) mma_commit_pair(&bars->sf_empty[slot]);
-            if (ks == KS - 1) mma_commit_pair(&bars->acc_full[acc]);
+            __syncwarp();
+            un.next();
           }
-          __syncwarp();
-          step += last ? 1 : 0;
+          if (!ok) break;
+          left -= kSK;
         }
-        ++lt;
+        ac.next();
       }
-      if (elect_one()) mma_commit_pair(&bars->mma_done);
+      if (elect_one()) mma_commit_leader(&bars->mma_done);
       mbar_wait(&bars->mma_done, 0, a.err, nullptr, kSite + 7);
     }
-  } else if (warp < kEpiWarp0) {
+  } else if (warp == kCopyWarp) {
+    // ------------------------------------------------------------------ scales to TMEM
+    if (leader) {
+      const uint64_t sfa0 = sdesc_scales(smem_u32(sf_base)), sfb0 = sdesc_scales(smem_u32(sf_base) + kSfABytes);
+      const int units = (a.K + C::kUnitK - 1) / C::kUnitK;
+      Ring<kSfSlots> sl;
+      Ring<kUnits> un;
+      int hint = 0;
+      bool ok = true;
+      for (int tile = first; tile < total && ok; tile += stride) {
+        const Tile t = tile_at(seg, a.E, a.NB, tile, hint);
+        if (t.zero) continue;
+        for (int u = 0; u < units; u += 4) {
+          ok = warp_wait(&bars->sf_full[sl.i], sl.phase, a.err, abort_flag, kSite + 9);
+          if (!ok) break;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if (u + j >= units) break;
+            ok = warp_wait(&bars->unit_empty[un.i], un.phase ^ 1u, a.err, abort_flag, kSite + 11);
+            if (!ok) break;
+            tc_fence_after();
+            if (elect_one()) {
+              const uint32_t sfa = tmem + kAcc * kTN + un.i * kUnitCols, sfb = sfa + 8;
+              const uint64_t da = sfa0 + sl.i * (kSfSlotBytes >> 4), db = sfb0 + sl.i * (kSfSlotBytes >> 4);
+#pragma unroll
+              for (int w = 0; w < 2; ++w) {
+                const int q = 2 * j + w;   // word of the step
+                copy_scales_pair(sfa + w * 4, da + q * 32);
+                copy_scales_pair(sfb + w * 8, db + q * 64);
+                copy_scales_pair(sfb + w * 8 + 4, db + q * 64 + 32);
+              }
+              mma_commit_leader(&bars->unit_full[un.i]);
+              if (j == 3 || u + j == units - 1) mma_commit_pair(&bars->sf_empty[sl.i]);
+            }
+            __syncwarp();
+            un.next();
+          }
+          if (!ok) break;
+          sl.next();
+        }
+      }
+      if (elect_one()) mma_commit_leader(&bars->copy_done);
+      mbar_wait(&bars->copy_done, 0, a.err, nullptr, kSite + 12);
+    }
+  } else if (warp < kCopyWarp) {
     // ------------------------------------------------------------------ scales
     const int part = warp - 2;   // 0: rows, 1: columns 0-127, 2: columns 128-191
     const int nb = a.K / fp4_block(FORMAT);
     uint8_t* dst = sf_base + (part == 0 ? 0u : kSfABytes + (part - 1) * 512u) + lane * 16;
     const uint32_t dst_word = part == 0 ? 512u : 1024u;
-    const int steps = (KS + C::kStep - 1) / C::kStep;   // 32-byte loads a row
+    const int steps = (a.K + C::kStepK - 1) / C::kStepK;   // 32-byte loads a row
     const uint32_t full_addr = mapa_u32(&bars->sf_full[0], 0);
     // the lane's four rows (r = lane + 32 i) of a tile, NULL where there is none
     auto sources = [&](const Tile& t, const uint8_t* (&p)[4]) {
@@ -332,7 +385,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           v[i][h] = p[i] ? __ldg(reinterpret_cast<const uint4*>(p[i] + step * 32) + h) : make_uint4(0, 0, 0, 0);
       }
     };
-    uint32_t done = 0;   // steps handed over
+    Ring<kSfSlots> sl;
     int hint = 0;
     // the next load: tile and step
     int ltile = first;
@@ -377,9 +430,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           }
         }
       }
-      const uint32_t slot = done % kSfSlots;
-      ok = mbar_wait(&bars->sf_empty[slot], ((done / kSfSlots) & 1u) ^ 1u, a.err, abort_flag, kSite + 8);
-      ok = __all_sync(0xffffffffu, ok);
+      ok = warp_wait(&bars->sf_empty[sl.i], sl.phase ^ 1u, a.err, abort_flag, kSite + 8);
       if (!ok) break;
 #pragma unroll
       for (int q = 0; q < 8; ++q) {
@@ -389,12 +440,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           const uint4 v = cur[i][q >> 2];
           o[i] = (q & 3) == 0 ? v.x : (q & 3) == 1 ? v.y : (q & 3) == 2 ? v.z : v.w;
         }
-        *reinterpret_cast<uint4*>(dst + slot * kSfSlotBytes + q * dst_word) = make_uint4(o[0], o[1], o[2], o[3]);
+        *reinterpret_cast<uint4*>(dst + sl.i * kSfSlotBytes + q * dst_word) = make_uint4(o[0], o[1], o[2], o[3]);
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(full_addr + slot * 8);
-      ++done;
+      if (lane == 0) mbar_arrive_cluster(full_addr + sl.i * 8);
+      sl.next();
     }
   } else {
     // ------------------------------------------------------------------ epilogue
@@ -402,7 +453,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const uint32_t lane_base = (uint32_t)(q * 32) << 16;
     const uint32_t empty_addr = mapa_u32(&bars->acc_empty[0], 0);
     const int64_t esize = a.out_dtype == LMOE_DTYPE_F32 ? 4 : 2;
-    uint32_t lt = 0;
+    Ring<kAcc> ac;
     int hint = 0;
     for (int tile = first; tile < total; tile += stride) {
       const Tile t = tile_at(seg, a.E, a.NB, tile, hint);
@@ -423,18 +474,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         }
         continue;
       }
-      const uint32_t acc = lt % kAcc;
-      const bool full = mbar_wait(&bars->acc_full[acc], (lt / kAcc) & 1u, a.err, abort_flag, kSite + 10);
-      if (!__all_sync(0xffffffffu, full)) break;
-      ++lt;
+      if (!warp_wait(&bars->acc_full[ac.i], ac.phase, a.err, abort_flag, kSite + 10)) break;
       tc_fence_after();
       uint32_t u[32], v[32];
-      const uint32_t c0 = tmem + lane_base + acc * kTN + (SWIGLU ? cg * 32 : cg * 64);
+      const uint32_t c0 = tmem + lane_base + ac.i * kTN + (SWIGLU ? cg * 32 : cg * 64);
       tmem_ld32(c0, u);
       tmem_ld32(c0 + (SWIGLU ? kHalf : 32), v);
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(empty_addr + acc * 8);
+      if (lane == 0) mbar_arrive_cluster(empty_addr + ac.i * 8);
+      ac.next();
       if (!ok) continue;
       const float al = a.alpha ? __ldg(a.alpha + t.e) : 1.0f;
       float f[32];

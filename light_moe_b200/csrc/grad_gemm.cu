@@ -148,7 +148,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer
     const uint32_t full_addr = mapa_u32(&bars->full[0], 0);
-    uint32_t it = 0;
+    Ring<kStages> st;
     int hint = 0;
     bool ok = true;
     for (int tile = first; tile < total && ok; tile += stride) {
@@ -160,14 +160,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const int rows = t.row_end - m0;
         boxes = rows <= 0 ? 0 : (rows >= kCta ? 4 : (rows + 31) >> 5);
       }
-      for (int ks = 0; ks < t.ks; ++ks, ++it) {
-        const int s = it % kStages;
-        ok = warp_wait(&bars->empty[s], ((it / kStages) & 1u) ^ 1u, a.err, abort_flag, kSite + 2);
+      for (int ks = 0; ks < t.ks; ++ks, st.next()) {
+        ok = warp_wait(&bars->empty[st.i], st.phase ^ 1u, a.err, abort_flag, kSite + 2);
         if (!ok) break;
         if (elect_one()) {
-          uint8_t* sa = base + s * kStageBytes;
+          uint8_t* sa = base + st.i * kStageBytes;
           uint8_t* sb = sa + kOperand;
-          const uint32_t bar = full_addr + s * 8;
+          const uint32_t bar = full_addr + st.i * 8;
           if (FORM == kInputGrad) {
             mbar_arrive_expect_tx_cluster(bar, (uint32_t)boxes * 4096u + kOperand);
             if (boxes == 4) {
@@ -180,7 +179,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           } else {
             const int r = t.row0 + ks * kSK;
             if (has_tail(t.row_end - r)) {
-              uint64_t* own = &bars->tail[s];
+              uint64_t* own = &bars->tail[st.i];
               mbar_arrive_expect_tx(own, 2 * kOperand);
               tma_load_2d(sa, &tm_a, own, m0, r);
               tma_load_2d(sa + kChunk, &tm_a, own, m0 + 64, r);
@@ -204,40 +203,38 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     if (leader) {
       const uint32_t idesc = idesc_f16kind_f32(kTile, kTile, a.f16) | kIdescBMajorMN |
                              (FORM == kWeightGrad ? kIdescAMajorMN : 0u);
-      uint32_t it = 0, lt = 0;
+      // descriptors count 16 bytes
+      const uint64_t adesc0 = FORM == kInputGrad ? sdesc_k_sw128(smem_u32(base)) : sdesc_mn_sw128(smem_u32(base), kChunk);
+      const uint64_t bdesc0 = sdesc_mn_sw128(smem_u32(base) + kOperand, kChunk);
+      Ring<kStages> st;
+      Ring<kAcc> ac;
       int hint = 0;
       bool ok = true;
       for (int tile = first; tile < total && ok; tile += stride) {
         const Tile t = tile_at<FORM>(seg, a, tile, hint);
         if (t.ks == 0) continue;
-        const uint32_t acc = lt % kAcc;
-        ok = warp_wait_cluster(&bars->acc_empty[acc], ((lt / kAcc) & 1u) ^ 1u, a.err, abort_flag, kSite + 4);
+        ok = warp_wait(&bars->acc_empty[ac.i], ac.phase ^ 1u, a.err, abort_flag, kSite + 4);
         if (!ok) break;
-        const uint32_t d = tmem + acc * kTile;
-        const int depth = FORM == kInputGrad ? a.N : t.row_end - t.row0;
-        for (int ks = 0; ks < t.ks; ++ks, ++it) {
-          const int s = it % kStages;
-          ok = warp_wait_cluster(&bars->full[s], (it / kStages) & 1u, a.err, abort_flag, kSite + 6);
+        const uint32_t d = tmem + ac.i * kTile;
+        int left = FORM == kInputGrad ? a.N : t.row_end - t.row0;
+        for (int ks = 0; ks < t.ks; ++ks, st.next(), left -= kSK) {
+          ok = warp_wait(&bars->full[st.i], st.phase, a.err, abort_flag, kSite + 6);
           if (!ok) break;
           tc_fence_after();
           if (elect_one()) {
-            const uint32_t sa = smem_u32(base + s * kStageBytes), sb = sa + kOperand;
-            const int left = depth - ks * kSK;
+            const uint64_t ad = adesc0 + st.i * (kStageBytes >> 4), bd = bdesc0 + st.i * (kStageBytes >> 4);
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk) {
-              if (kk * 16 >= left) break;
-              const uint64_t ad =
-                  FORM == kInputGrad ? sdesc_k_sw128(sa + kk * 32) : sdesc_mn_sw128(sa + kk * 2048, kChunk);
-              mma_ss_pair(d, ad, sdesc_mn_sw128(sb + kk * 2048, kChunk), idesc, (ks | kk) != 0 ? 1u : 0u);
-            }
-            mma_commit_pair(&bars->empty[s]);
-            if (ks == t.ks - 1) mma_commit_pair(&bars->acc_full[acc]);
+            for (int kk = 0; kk < 4; ++kk)
+              if (kk * 16 < left)
+                mma_ss_pair(d, ad + kk * (FORM == kInputGrad ? 2 : 128), bd + kk * 128, idesc, (ks | kk) != 0 ? 1u : 0u);
+            mma_commit_pair(&bars->empty[st.i]);
+            if (ks == t.ks - 1) mma_commit_pair(&bars->acc_full[ac.i]);
           }
           __syncwarp();
         }
-        ++lt;
+        ac.next();
       }
-      if (elect_one()) mma_commit_pair(&bars->mma_done);
+      if (elect_one()) mma_commit_leader(&bars->mma_done);
       mbar_wait(&bars->mma_done, 0, a.err, nullptr, kSite + 7);
     }
   } else if (warp == 2) {
@@ -276,7 +273,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const uint32_t lane_base = (uint32_t)(q * 32) << 16;
     const uint32_t empty_addr = mapa_u32(&bars->acc_empty[0], 0);
     const int64_t esize = a.out_dtype == LMOE_DTYPE_F32 ? 4 : 2;
-    uint32_t lt = 0;
+    Ring<kAcc> ac;
     int hint = 0;
     for (int tile = first; tile < total; tile += stride) {
       const Tile t = tile_at<FORM>(seg, a, tile, hint);
@@ -285,12 +282,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const bool ok = FORM == kInputGrad ? t.row0 + r < t.row_end : t.m * kTile + r < a.N;
       void* out = static_cast<uint8_t*>(a.out) + row * a.K * esize;
       const int c0 = t.n * kTile + half * kCta;
-      uint32_t acc = 0;
       if (t.ks != 0) {
-        acc = lt % kAcc;
-        const bool full = mbar_wait(&bars->acc_full[acc], (lt / kAcc) & 1u, a.err, abort_flag, kSite + 9);
-        if (!__all_sync(0xffffffffu, full)) break;
-        ++lt;
+        if (!warp_wait(&bars->acc_full[ac.i], ac.phase, a.err, abort_flag, kSite + 9)) break;
         tc_fence_after();
       }
 #pragma unroll
@@ -298,11 +291,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         float f[32];
         if (t.ks != 0) {
           uint32_t u[32];
-          tmem_ld32(tmem + lane_base + acc * kTile + half * kCta + j * 32, u);
+          tmem_ld32(tmem + lane_base + ac.i * kTile + half * kCta + j * 32, u);
           if (j == 3) {
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(empty_addr + acc * 8);
+            if (lane == 0) mbar_arrive_cluster(empty_addr + ac.i * 8);
+            ac.next();
           }
 #pragma unroll
           for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(u[i]);

@@ -34,8 +34,13 @@ __device__ __forceinline__ uint32_t mapa_u32(const void* p, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
   return a;
 }
+// Arrival at a barrier of either CTA.  What it announces is shared or tensor memory of the arriving
+// CTA, which only that CTA's tensor core touches next; the caller's proxy fence or tcgen05 fence
+// has completed those accesses, so the arrival itself need not order other memory.  (With
+// .release.cluster it also waits for the thread's loads and writes to global memory, ~900 ns:
+// the 4-bit product of 128 rows took 145 us.)
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 // One arrival that also expects `bytes` of copies; it orders no memory (the copies do that).
 __device__ __forceinline__ void mbar_arrive_expect_tx_cluster(uint32_t cluster_addr, uint32_t bytes) {
@@ -101,6 +106,18 @@ __device__ __forceinline__ void let_copies_land() {
   }
 }
 
+// Position in a ring of N slots and the parity of its pass.
+template <int N>
+struct Ring {
+  uint32_t i = 0, phase = 0;
+  __device__ __forceinline__ void next() {
+    if (++i == N) {
+      i = 0;
+      phase ^= 1u;
+    }
+  }
+};
+
 // The waits of a whole warp, with one answer for all its lanes.  The warps that issue copies and
 // MMAs run their loops with all lanes and issue under elect.sync: under `lane == 0` the compiler
 // cannot tell that the operands are uniform, and every tcgen05 instruction then costs the thread
@@ -149,6 +166,12 @@ __device__ __forceinline__ void mma_commit_pair(uint64_t* bar) {
           smem_u32(bar)),
       "h"((uint16_t)3)
       : "memory");
+}
+
+// The same on a barrier of this CTA alone (the one that issues).
+__device__ __forceinline__ void mma_commit_leader(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+               : "memory");
 }
 
 // Shared-memory descriptor of an M- or N-major 16-bit operand in 128-byte-swizzled chunks of
