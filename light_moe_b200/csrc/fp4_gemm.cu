@@ -16,22 +16,23 @@
 // leader's 96 columns are gate rows and the follower's 96 the same rows of up.
 //
 // Operands stay in the canonical layout of the quantiser (codes [rows, K/2], scales [rows,
-// pitch]): the codes arrive by TMA (128-byte swizzle, 256 values = 128 bytes a row and stage).
+// pitch]): the codes arrive by TMA (128-byte swizzle, 256 values = 128 bytes a row), two such blocks a stage.
 // The scales must lie in shared memory as 512-byte tiles of 128 rows x 4 scales, row r at
-// (r % 32) * 16 + (r / 32) * 4, from where tcgen05.cp copies them to TMEM.  Three warps read them
-// as whole 32-byte sectors a row (a step: the scales of four stages of MX, two of NV), one step
-// ahead, write the tiles with one 16-byte store per lane and word, and hand a step to the leader
-// in one go: an arrival at the other CTA's barrier that releases memory costs ~900 ns.
+// (r % 32) * 16 + (r / 32) * 4, from where tcgen05.cp copies them to TMEM.  Five warps of 64 rows
+// each read them as whole 32-byte sectors a row (a step: the scales of two stages of MX, one of
+// NV), three steps ahead in registers, write the tiles and hand a step to the leader in one go.
 //
-// The copies to TMEM and the MMAs are issued by two warps.  A unit of two 4-scale words a row
-// (256 values of MX, 128 of NV: 24 TMEM columns, six copies) is copied ahead into a ring of five,
-// and commits of the two warps hand the units back and forth; with one warp issuing both, its
-// waits and copies stood between the MMAs.
+// One thread issues a unit of four 4-scale words a row (512 values of MX, 256 of NV: twelve copies
+// into one of two TMEM buffers of 48 columns) and its MMAs, in whose order the tensor pipe runs
+// them.  Its waits and issue slots are what a stage costs beside the MMAs: ~65 cycles a wait, ~25
+// an instruction, against 96 cycles an MMA; so a stage holds 512 values and the waits of a unit
+// start together.  (With 256 values and one wait after another: 650 cycles per 384 of MMAs, 0.88
+// ms for the gate / up product of 16384 rows; with the copies issued by a warp of their own they
+// queue behind the MMAs issued before, and the hand-over then stands in the pipe.)
 //
 // Warps: 0 TMA producer, whose copies complete on the leader's stage barrier; 1 MMA issuer
-// (leader CTA); 2 scales of the rows; 3, 4 scales of the columns 0-127 and 128-191 (each CTA
-// keeps all 192: the MMA reads them beside its own rows); 5 copies the scales to TMEM (leader
-// CTA); 6-17 epilogue, twelve warps of 32 rows x 64 columns.
+// (leader CTA); 2-3 scales of the rows, 4-6 scales of the 192 columns (each CTA keeps all: the MMA
+// reads them beside its own rows); 7-18 epilogue, twelve warps of 32 rows x 64 columns.
 #include <cuda_bf16.h>
 
 #include "fp4_format.cuh"
@@ -43,14 +44,17 @@ namespace lmoe {
 namespace {
 
 constexpr int kRowsCta = 128, kTM = 256, kTN = 192, kHalf = 96;
-constexpr int kSK = 256;          // values per stage: one 128-byte swizzle line of codes
-constexpr int kStages = 6, kAcc = 2;
-constexpr int kSfSlots = 3;      // steps of scales in shared memory
-constexpr int kCopyWarp = 5, kEpiWarp0 = 6, kEpiWarps = 12;
-constexpr int kUnits = 5;        // units of scales in TMEM
-constexpr uint32_t kUnitCols = 24;   // 2 words x (4 columns of the rows' scales, 8 of the columns')
+constexpr int kBK = 256;          // values of a 128-byte swizzle line of codes
+constexpr int kSK = 512;          // values per stage
+constexpr int kStages = 3, kAcc = 2;
+constexpr int kSfSlots = 3;       // steps of scales in shared memory
+constexpr int kSfAhead = 3;       // steps of scales in registers
+constexpr int kUnits = 2;         // units of scales in TMEM
+constexpr uint32_t kUnitCols = 48;   // 4 words x (4 columns of the rows' scales, 8 of the columns')
+constexpr int kSfWarp0 = 2, kSfWarps = 5, kEpiWarp0 = 7, kEpiWarps = 12;
 constexpr int kThreads = (kEpiWarp0 + kEpiWarps) * 32;
-constexpr uint32_t kABytes = kRowsCta * 128, kBBytes = kHalf * 128;
+constexpr uint32_t kABlock = kRowsCta * 128, kBBlock = kHalf * 128;
+constexpr uint32_t kABytes = 2 * kABlock, kBBytes = 2 * kBBlock;
 constexpr uint32_t kSite = 0x500u;
 constexpr int kTmemCols = 512;
 
@@ -78,11 +82,10 @@ struct __align__(8) Bars {
   uint64_t empty[kStages];      // the stage's MMAs finished (both CTAs)
   uint64_t sf_full[kSfSlots];   // leader: both CTAs' scale warps wrote the step
   uint64_t sf_empty[kSfSlots];  // the step's scales were copied (both CTAs)
-  uint64_t unit_full[kUnits];   // leader: the unit's scales are in TMEM
   uint64_t unit_empty[kUnits];  // leader: the unit's MMAs finished
   uint64_t acc_full[kAcc];
   uint64_t acc_empty[kAcc];     // leader: both CTAs' epilogue warps
-  uint64_t mma_done, copy_done;
+  uint64_t mma_done;
   uint32_t tmem_base;
   int abort;
   SegTable seg;
@@ -144,9 +147,9 @@ __device__ __forceinline__ void mma_fp4_pair(uint32_t d, uint64_t a, uint64_t b,
 
 template <int FORMAT>
 struct Cfg {
-  static constexpr int kUnitK = FORMAT == LMOE_FP4_MX ? 256 : 128;   // values of a unit
+  static constexpr int kUnitK = FORMAT == LMOE_FP4_MX ? 512 : 256;   // values of a unit (4 words)
   static constexpr int kStageUnits = kSK / kUnitK;
-  static constexpr int kStepK = 4 * kUnitK;                          // values of a step (8 words)
+  static constexpr int kStepK = 2 * kUnitK;                          // values of a step (8 words)
 };
 static_assert(kAcc * kTN + kUnits * kUnitCols <= kTmemCols, "tensor memory budget");
 constexpr uint32_t kStageBytes = kABytes + kBBytes;
@@ -178,19 +181,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       mbar_init(&bars->empty[s], 1);
     }
     for (int s = 0; s < kSfSlots; ++s) {
-      mbar_init(&bars->sf_full[s], 6);
+      mbar_init(&bars->sf_full[s], 2 * kSfWarps);
       mbar_init(&bars->sf_empty[s], 1);
     }
-    for (int s = 0; s < kUnits; ++s) {
-      mbar_init(&bars->unit_full[s], 1);
-      mbar_init(&bars->unit_empty[s], 1);
-    }
+    for (int s = 0; s < kUnits; ++s) mbar_init(&bars->unit_empty[s], 1);
     for (int s = 0; s < kAcc; ++s) {
       mbar_init(&bars->acc_full[s], 1);
       mbar_init(&bars->acc_empty[s], 2 * kEpiWarps);
     }
     mbar_init(&bars->mma_done, 1);
-    mbar_init(&bars->copy_done, 1);
     bars->abort = 0;
     fence_mbar_init();
   }
@@ -236,13 +235,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         if (elect_one()) {
           uint8_t* dst = base + st.i * kStageBytes;
           const uint32_t bar = full_addr + st.i * 8;
-          mbar_arrive_expect_tx_cluster(bar, (uint32_t)boxes * 4096u + kBBytes);
-          if (boxes == 4) {
-            tma_load_2d_pair(dst, &tm_x, bar, ks * 128, r0);
-          } else {
-            for (int b = 0; b < boxes; ++b) tma_load_2d_pair(dst + b * 4096, &tm_x32, bar, ks * 128, r0 + b * 32);
+          const int blocks = a.K - ks * kSK > kBK ? 2 : 1;
+          mbar_arrive_expect_tx_cluster(bar, (uint32_t)blocks * ((uint32_t)boxes * 4096u + kBBlock));
+          for (int h = 0; h < blocks; ++h) {
+            const int x = ks * (kSK / 2) + h * 128;
+            if (boxes == 4) {
+              tma_load_2d_pair(dst + h * kABlock, &tm_x, bar, x, r0);
+            } else {
+              for (int b = 0; b < boxes; ++b)
+                tma_load_2d_pair(dst + h * kABlock + b * 4096, &tm_x32, bar, x, r0 + b * 32);
+            }
+            tma_load_3d_pair(dst + kABytes + h * kBBlock, wmap, bar, x, wrow, t.e);
           }
-          tma_load_3d_pair(dst + kABytes, wmap, bar, ks * 128, wrow, t.e);
         }
       }
     }
@@ -252,7 +256,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     // ------------------------------------------------------------------ MMA issuer
     if (leader) {
       const uint64_t adesc0 = sdesc_k_sw128(smem_u32(base)), bdesc0 = sdesc_k_sw128(smem_u32(base) + kABytes);
+      const uint64_t sfa0 = sdesc_scales(smem_u32(sf_base)), sfb0 = sdesc_scales(smem_u32(sf_base) + kSfABytes);
       Ring<kStages> st;
+      Ring<kSfSlots> sl;
       Ring<kUnits> un;
       Ring<kAcc> ac;
       int hint = 0;
@@ -261,191 +267,162 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const Tile t = tile_at(seg, a.E, a.NB, tile, hint);
         if (t.zero) continue;
         ok = warp_wait(&bars->acc_empty[ac.i], ac.phase ^ 1u, a.err, abort_flag, kSite + 4);
-        if (!ok) break;
         const uint32_t d = tmem + ac.i * kTN;
-        int left = a.K;
-        for (int ks = 0; ks < KS; ++ks, st.next()) {
-          ok = warp_wait(&bars->full[st.i], st.phase, a.err, abort_flag, kSite + 6);
-          if (!ok) break;
-          // descriptors count 16 bytes; a stage is kStageBytes, 64 values (an MMA) 32 bytes
-          const uint64_t ad = adesc0 + st.i * (kStageBytes >> 4), bd = bdesc0 + st.i * (kStageBytes >> 4);
+        uint32_t accum = 0;
+        for (int left = a.K; left > 0 && ok; left -= C::kStepK) {
+          // a step: two units, or one at the end of a row
+          const uint64_t sa = sfa0 + sl.i * (kSfSlotBytes >> 4), sb = sfb0 + sl.i * (kSfSlotBytes >> 4);
 #pragma unroll
-          for (int h = 0; h < C::kStageUnits; ++h) {
-            if (h * C::kUnitK >= left) break;
-            ok = warp_wait(&bars->unit_full[un.i], un.phase, a.err, abort_flag, kSite + 5);
+          for (int j = 0; j < 2; ++j) {
+            constexpr int kU = C::kUnitK;
+            if (j * kU >= left) break;
+            const bool stage_start = j % C::kStageUnits == 0;
+            // the waits start together; what has not come yet is waited for below
+            const bool w0 = mbar_test(&bars->unit_empty[un.i], un.phase ^ 1u);
+            const bool w1 = j > 0 || mbar_test(&bars->sf_full[sl.i], sl.phase);
+            const bool w2 = !stage_start || mbar_test(&bars->full[st.i], st.phase);
+            if (!(w0 && w1 && w2)) {
+              ok = mbar_wait(&bars->unit_empty[un.i], un.phase ^ 1u, a.err, abort_flag, kSite + 5);
+              if (ok && j == 0) ok = mbar_wait(&bars->sf_full[sl.i], sl.phase, a.err, abort_flag, kSite + 9);
+              if (ok && stage_start) ok = mbar_wait(&bars->full[st.i], st.phase, a.err, abort_flag, kSite + 6);
+            }
+            ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             tc_fence_after();
+            const bool last = (j + 1) * kU >= left;   // of the row
+            const bool stage_end = (j + 1) % C::kStageUnits == 0 || last;
             if (elect_one()) {
-              const uint32_t sfa = tmem + kAcc * kTN + un.i * kUnitCols, sfb = sfa + 8;
+              const uint32_t sfa = tmem + kAcc * kTN + un.i * kUnitCols, sfb = sfa + 16;
 #pragma unroll
-              for (int j = 0; j < C::kUnitK / 64; ++j) {
-                const int kk = h * (C::kUnitK / 64) + j;
-                if (kk * 64 < left) {
-                  const uint32_t accum = (ks | kk) != 0 ? 1u : 0u;
+              for (int w = 0; w < 4; ++w) {
+                const int q = 4 * j + w;   // word of the step
+                copy_scales_pair(sfa + w * 4, sa + q * 32);
+                copy_scales_pair(sfb + w * 8, sb + q * 64);
+                copy_scales_pair(sfb + w * 8 + 4, sb + q * 64 + 32);
+              }
+              // descriptors count 16 bytes; 64 values (an MMA) are 32 bytes of a block's lines
+              const uint64_t ad = adesc0 + st.i * (kStageBytes >> 4), bd = bdesc0 + st.i * (kStageBytes >> 4);
+#pragma unroll
+              for (int m = 0; m < kU / 64; ++m) {
+                if (j * kU + m * 64 < left) {
+                  const int kk = (j % C::kStageUnits) * (kU / 64) + m;   // of the stage's eight
+                  const uint64_t am = ad + (kk >> 2) * (kABlock >> 4) + (kk & 3) * 2;
+                  const uint64_t bm = bd + (kk >> 2) * (kBBlock >> 4) + (kk & 3) * 2;
                   if (FORMAT == LMOE_FP4_MX)
                     // a word holds the scales of 128 values: of two MMAs (scale id 0 and 2)
-                    mma_fp4_pair<FORMAT>(d, ad + kk * 2, bd + kk * 2, idesc_fp4(true, (kk & 1) * 2),
-                                         sfa + (j >> 1) * 4, sfb + (j >> 1) * 8, accum);
+                    mma_fp4_pair<FORMAT>(d, am, bm, idesc_fp4(true, (m & 1) * 2), sfa + (m >> 1) * 4,
+                                         sfb + (m >> 1) * 8, accum | (uint32_t)(m > 0));
                   else
-                    mma_fp4_pair<FORMAT>(d, ad + kk * 2, bd + kk * 2, idesc_fp4(false, 0), sfa + j * 4, sfb + j * 8,
-                                         accum);
+                    mma_fp4_pair<FORMAT>(d, am, bm, idesc_fp4(false, 0), sfa + m * 4, sfb + m * 8,
+                                         accum | (uint32_t)(m > 0));
                 }
               }
               mma_commit_leader(&bars->unit_empty[un.i]);
-              if ((h + 1) * C::kUnitK >= (left < kSK ? left : kSK)) {
-                mma_commit_pair(&bars->empty[st.i]);
-                if (ks == KS - 1) mma_commit_pair(&bars->acc_full[ac.i]);
-              }
+              if (stage_end) mma_commit_pair(&bars->empty[st.i]);
+              if (j == 1 || last) mma_commit_pair(&bars->sf_empty[sl.i]);
+              if (last) mma_commit_pair(&bars->acc_full[ac.i]);
             }
             __syncwarp();
+            accum = 1;
             un.next();
+            if (stage_end) st.next();
           }
-          if (!ok) break;
-          left -= kSK;
+          sl.next();
         }
         ac.next();
       }
       if (elect_one()) mma_commit_leader(&bars->mma_done);
       mbar_wait(&bars->mma_done, 0, a.err, nullptr, kSite + 7);
     }
-  } else if (warp == kCopyWarp) {
-    // ------------------------------------------------------------------ scales to TMEM
-    if (leader) {
-      const uint64_t sfa0 = sdesc_scales(smem_u32(sf_base)), sfb0 = sdesc_scales(smem_u32(sf_base) + kSfABytes);
-      const int units = (a.K + C::kUnitK - 1) / C::kUnitK;
-      Ring<kSfSlots> sl;
-      Ring<kUnits> un;
-      int hint = 0;
-      bool ok = true;
-      for (int tile = first; tile < total && ok; tile += stride) {
-        const Tile t = tile_at(seg, a.E, a.NB, tile, hint);
-        if (t.zero) continue;
-        for (int u = 0; u < units; u += 4) {
-          ok = warp_wait(&bars->sf_full[sl.i], sl.phase, a.err, abort_flag, kSite + 9);
-          if (!ok) break;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if (u + j >= units) break;
-            ok = warp_wait(&bars->unit_empty[un.i], un.phase ^ 1u, a.err, abort_flag, kSite + 11);
-            if (!ok) break;
-            tc_fence_after();
-            if (elect_one()) {
-              const uint32_t sfa = tmem + kAcc * kTN + un.i * kUnitCols, sfb = sfa + 8;
-              const uint64_t da = sfa0 + sl.i * (kSfSlotBytes >> 4), db = sfb0 + sl.i * (kSfSlotBytes >> 4);
-#pragma unroll
-              for (int w = 0; w < 2; ++w) {
-                const int q = 2 * j + w;   // word of the step
-                copy_scales_pair(sfa + w * 4, da + q * 32);
-                copy_scales_pair(sfb + w * 8, db + q * 64);
-                copy_scales_pair(sfb + w * 8 + 4, db + q * 64 + 32);
-              }
-              mma_commit_leader(&bars->unit_full[un.i]);
-              if (j == 3 || u + j == units - 1) mma_commit_pair(&bars->sf_empty[sl.i]);
-            }
-            __syncwarp();
-            un.next();
-          }
-          if (!ok) break;
-          sl.next();
-        }
-      }
-      if (elect_one()) mma_commit_leader(&bars->copy_done);
-      mbar_wait(&bars->copy_done, 0, a.err, nullptr, kSite + 12);
-    }
-  } else if (warp < kCopyWarp) {
+  } else if (warp < kEpiWarp0) {
     // ------------------------------------------------------------------ scales
-    const int part = warp - 2;   // 0: rows, 1: columns 0-127, 2: columns 128-191
+    const int part = warp - kSfWarp0;   // 0, 1: rows 0-63, 64-127; 2, 3, 4: columns 0-63, 64-127, 128-191
     const int nb = a.K / fp4_block(FORMAT);
-    uint8_t* dst = sf_base + (part == 0 ? 0u : kSfABytes + (part - 1) * 512u) + lane * 16;
-    const uint32_t dst_word = part == 0 ? 512u : 1024u;
+    // rows lane, lane + 32 of the 64 are words 0, 1 or 2, 3 of the lane's 16 bytes in a tile
+    uint8_t* dst = sf_base + lane * 16 +
+                   (part < 2 ? part * 8u : kSfABytes + (part == 4 ? 512u : (uint32_t)(part - 2) * 8u));
+    const uint32_t dst_word = part < 2 ? 512u : 1024u;
     const int steps = (a.K + C::kStepK - 1) / C::kStepK;   // 32-byte loads a row
     const uint32_t full_addr = mapa_u32(&bars->sf_full[0], 0);
-    // the lane's four rows (r = lane + 32 i) of a tile, NULL where there is none
-    auto sources = [&](const Tile& t, const uint8_t* (&p)[4]) {
+    int hint = 0, ltile = first, lstep = 0;   // the next load: tile and step
+    const uint8_t* lp[2];                     // the lane's two rows of that tile, NULL where there is none
+    auto next_tile = [&]() {   // first tile at or behind ltile that has an expert
+      for (; ltile < total; ltile += stride) {
+        const Tile t = tile_at(seg, a.E, a.NB, ltile, hint);
+        if (t.zero) continue;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = lane + 32 * i;
-        p[i] = nullptr;
-        if (part == 0) {
-          const int row = t.row0 + (int)rank * kRowsCta + r;
-          if (row < t.row_end) p[i] = a.xs + (int64_t)row * a.xs_pitch;
-        } else {
-          const int c = r + (part - 1) * 128;
-          const bool up = SWIGLU && c >= kHalf;
-          const int n = SWIGLU ? t.n * kHalf + (up ? c - kHalf : c) : t.n * kTN + c;
-          if (c < kTN && n < a.N) p[i] = (up ? a.ws_up : a.ws) + ((int64_t)t.e * a.N + n) * a.ws_pitch;
-        }
-      }
-    };
-    auto load = [&](const uint8_t* (&p)[4], int step, uint4 (&v)[4][2]) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-          v[i][h] = p[i] ? __ldg(reinterpret_cast<const uint4*>(p[i] + step * 32) + h) : make_uint4(0, 0, 0, 0);
-      }
-    };
-    Ring<kSfSlots> sl;
-    int hint = 0;
-    // the next load: tile and step
-    int ltile = first;
-    const uint8_t* lp[4];
-    auto next_tile = [&](int tile) {   // first non-empty tile at or behind `tile`
-      for (; tile < total; tile += stride) {
-        const Tile t = tile_at(seg, a.E, a.NB, tile, hint);
-        if (!t.zero) {
-          sources(t, lp);
-          break;
-        }
-      }
-      return tile;
-    };
-    ltile = next_tile(ltile);
-    int lstep = 0;
-    uint4 nxt[4][2];
-    if (ltile < total) load(lp, 0, nxt);
-    bool ok = true;
-    while (ltile < total && ok) {
-      uint4 cur[4][2];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        cur[i][0] = nxt[i][0];
-        cur[i][1] = nxt[i][1];
-      }
-      const int step = lstep;
-      if (++lstep == steps) {
-        lstep = 0;
-        ltile = next_tile(ltile + stride);
-      }
-      if (ltile < total) load(lp, lstep, nxt);
-      if ((step + 1) * 32 > nb) {
-        // scale bytes behind the last block are padding: zero, whatever they hold
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint32_t* w = reinterpret_cast<uint32_t*>(&cur[i][0]);
-#pragma unroll
-          for (int q = 0; q < 8; ++q) {
-            const int valid = nb - (step * 32 + q * 4);
-            if (valid < 4) w[q] = valid <= 0 ? 0u : (w[q] & ((1u << (8 * valid)) - 1u));
+        for (int i = 0; i < 2; ++i) {
+          lp[i] = nullptr;
+          if (part < 2) {
+            const int row = t.row0 + (int)rank * kRowsCta + part * 64 + lane + 32 * i;
+            if (row < t.row_end) lp[i] = a.xs + (int64_t)row * a.xs_pitch;
+          } else {
+            const int c = (part - 2) * 64 + lane + 32 * i;
+            const bool up = SWIGLU && c >= kHalf;
+            const int n = SWIGLU ? t.n * kHalf + (up ? c - kHalf : c) : t.n * kTN + c;
+            if (n < a.N) lp[i] = (up ? a.ws_up : a.ws) + ((int64_t)t.e * a.N + n) * a.ws_pitch;
           }
         }
+        return;
       }
-      ok = warp_wait(&bars->sf_empty[sl.i], sl.phase ^ 1u, a.err, abort_flag, kSite + 8);
-      if (!ok) break;
+    };
+    uint4 v[kSfAhead][2][2];
+    int pending = 0;
+    auto load = [&](uint4 (&b)[2][2]) {
+      if (ltile >= total) return;
 #pragma unroll
-      for (int q = 0; q < 8; ++q) {
-        uint32_t o[4];
+      for (int i = 0; i < 2; ++i) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint4 v = cur[i][q >> 2];
-          o[i] = (q & 3) == 0 ? v.x : (q & 3) == 1 ? v.y : (q & 3) == 2 ? v.z : v.w;
+        for (int h = 0; h < 2; ++h)
+          b[i][h] = lp[i] ? __ldg(reinterpret_cast<const uint4*>(lp[i] + lstep * 32) + h) : make_uint4(0, 0, 0, 0);
+      }
+      ++pending;
+      if (++lstep == steps) {
+        lstep = 0;
+        ltile += stride;
+        next_tile();
+      }
+    };
+    next_tile();
+#pragma unroll
+    for (int j = 0; j < kSfAhead; ++j) load(v[j]);
+    Ring<kSfSlots> sl;
+    int step = 0;
+    bool ok = true;
+    while (ok && pending > 0) {
+#pragma unroll
+      for (int j = 0; j < kSfAhead; ++j) {
+        if (!ok || pending == 0) break;
+        --pending;
+        if ((step + 1) * 32 > nb) {
+          // scale bytes behind the last block are padding: zero, whatever they hold
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            uint32_t* w = reinterpret_cast<uint32_t*>(&v[j][i][0]);
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+              const int valid = nb - (step * 32 + q * 4);
+              if (valid < 4) w[q] = valid <= 0 ? 0u : (w[q] & ((1u << (8 * valid)) - 1u));
+            }
+          }
         }
-        *reinterpret_cast<uint4*>(dst + sl.i * kSfSlotBytes + q * dst_word) = make_uint4(o[0], o[1], o[2], o[3]);
+        step = step + 1 == steps ? 0 : step + 1;
+        ok = warp_wait(&bars->sf_empty[sl.i], sl.phase ^ 1u, a.err, abort_flag, kSite + 8);
+        if (!ok) break;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          const uint4 x = v[j][0][q >> 2], y = v[j][1][q >> 2];
+          const uint2 o = (q & 3) == 0 ? make_uint2(x.x, y.x)
+                                       : (q & 3) == 1 ? make_uint2(x.y, y.y)
+                                                      : (q & 3) == 2 ? make_uint2(x.z, y.z) : make_uint2(x.w, y.w);
+          *reinterpret_cast<uint2*>(dst + sl.i * kSfSlotBytes + q * dst_word) = o;
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(full_addr + sl.i * 8);
+        sl.next();
+        load(v[j]);
       }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(full_addr + sl.i * 8);
-      sl.next();
     }
   } else {
     // ------------------------------------------------------------------ epilogue

@@ -127,10 +127,6 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, uint32
                                           uint32_t site) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, err, abort, site));
 }
-__device__ __forceinline__ bool warp_wait_cluster(uint64_t* bar, uint32_t parity, uint32_t* err, volatile int* abort,
-                                                  uint32_t site) {
-  return __all_sync(0xffffffffu, mbar_wait_cluster(bar, parity, err, abort, site));
-}
 
 // ---------------------------------------------------------------------------------------
 // tcgen05 on a CTA pair
