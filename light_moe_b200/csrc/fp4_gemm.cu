@@ -68,7 +68,8 @@ struct Fp4Args {
   int offsets_i64;
   int E, N, K;
   int64_t R;
-  int NB, KS;            // column tiles, stages
+  Raster raster;         // of the column tiles
+  int KS;                // stages
   const float* alpha;    // per expert, or NULL
   const float* alpha_up;
   void* out;
@@ -96,13 +97,13 @@ struct Tile {
   bool zero;   // rows outside every expert
 };
 
-__device__ __forceinline__ Tile tile_at(const SegTable& t, int E, int NB, int tile, int& hint) {
+__device__ __forceinline__ Tile tile_at(const SegTable& t, int E, const Raster& ra, int tile, int& hint) {
   int j = hint;
   while (tile >= t.tile_start[j + 1]) ++j;
   hint = j;
   Tile r;
   const int rows = t.row[j + 1] - t.row[j];
-  raster(tile - t.tile_start[j], (rows + kTM - 1) / kTM, NB, r.m, r.n);
+  ra.at(tile - t.tile_start[j], (rows + kTM - 1) / kTM, r.m, r.n);
   r.e = j - 1;
   r.zero = j == 0 || j == E + 1;
   r.row0 = t.row[j] + r.m * kTM;
@@ -201,7 +202,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const int segs = a.E + 2;
   if (warp == 0)
     scan_tiles(&bars->seg, segs, lane, [&](int j) {
-      return (bars->seg.row[j + 1] - bars->seg.row[j] + kTM - 1) / kTM * a.NB;
+      return (bars->seg.row[j + 1] - bars->seg.row[j] + kTM - 1) / kTM * a.raster.nb;
     });
   if (tid == 0 && bars->seg.bad && blockIdx.x == 0) report_error(a.err, kErrBadArg, kSite + 1);
   tc_fence_before();
@@ -222,7 +223,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     int hint = 0;
     bool ok = true;
     for (int tile = first; tile < total && ok; tile += stride) {
-      const Tile t = tile_at(seg, a.E, a.NB, tile, hint);
+      const Tile t = tile_at(seg, a.E, a.raster, tile, hint);
       if (t.zero) continue;
       const int r0 = t.row0 + (int)rank * kRowsCta;
       int rows = t.row_end - r0;
@@ -264,7 +265,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       int hint = 0;
       bool ok = true;
       for (int tile = first; tile < total && ok; tile += stride) {
-        const Tile t = tile_at(seg, a.E, a.NB, tile, hint);
+        const Tile t = tile_at(seg, a.E, a.raster, tile, hint);
         if (t.zero) continue;
         ok = warp_wait(&bars->acc_empty[ac.i], ac.phase ^ 1u, a.err, abort_flag, kSite + 4);
         const uint32_t d = tmem + ac.i * kTN;
@@ -348,7 +349,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const uint8_t* lp[2];                     // the lane's two rows of that tile, NULL where there is none
     auto next_tile = [&]() {   // first tile at or behind ltile that has an expert
       for (; ltile < total; ltile += stride) {
-        const Tile t = tile_at(seg, a.E, a.NB, ltile, hint);
+        const Tile t = tile_at(seg, a.E, a.raster, ltile, hint);
         if (t.zero) continue;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -433,7 +434,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     Ring<kAcc> ac;
     int hint = 0;
     for (int tile = first; tile < total; tile += stride) {
-      const Tile t = tile_at(seg, a.E, a.NB, tile, hint);
+      const Tile t = tile_at(seg, a.E, a.raster, tile, hint);
       const int row = t.row0 + (int)rank * kRowsCta + q * 32 + lane;
       const bool ok = row < t.row_end;
       uint8_t* out = static_cast<uint8_t*>(a.out) + (int64_t)row * a.N * esize;
@@ -520,7 +521,7 @@ int run_fp4_gemm(const Fp4Problem& p, cudaStream_t stream) {
   a.N = p.N;
   a.K = p.K;
   a.R = p.total_rows;
-  a.NB = swiglu ? (p.N + kHalf - 1) / kHalf : (p.N + kTN - 1) / kTN;
+  a.raster = Raster(swiglu ? (p.N + kHalf - 1) / kHalf : (p.N + kTN - 1) / kTN);
   a.KS = (p.K + kSK - 1) / kSK;
   a.alpha = p.alpha;
   a.alpha_up = p.alpha_up;

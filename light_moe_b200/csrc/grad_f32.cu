@@ -26,7 +26,8 @@ struct F32Args {
   int offsets_i64;
   int E, N, K;
   int64_t R;
-  int MT, NB;
+  int MT;
+  Raster raster;
   float* out;
   uint32_t* err;
 };
@@ -53,8 +54,8 @@ __global__ void __launch_bounds__(kNT, 2) grad_f32_kernel(const F32Args a) {
   const int segs = a.E + 2;
   if (tid < 32)
     scan_tiles(&seg, segs, tid, [&](int j) {
-      if (!WGRAD) return (seg.row[j + 1] - seg.row[j] + kT - 1) / kT * a.NB;
-      return j == 0 || j == a.E + 1 ? 0 : a.MT * a.NB;
+      if (!WGRAD) return (seg.row[j + 1] - seg.row[j] + kT - 1) / kT * a.raster.nb;
+      return j == 0 || j == a.E + 1 ? 0 : a.MT * a.raster.nb;
     });
   if (tid == 0 && seg.bad && blockIdx.x == 0) report_error(a.err, kErrBadArg, kSite + 1);
   __syncthreads();
@@ -65,7 +66,7 @@ __global__ void __launch_bounds__(kNT, 2) grad_f32_kernel(const F32Args a) {
     while (tile >= seg.tile_start[j + 1]) ++j;
     const int rows = seg.row[j + 1] - seg.row[j];
     int m, n;
-    raster(tile - seg.tile_start[j], WGRAD ? a.MT : (rows + kT - 1) / kT, a.NB, m, n);
+    a.raster.at(tile - seg.tile_start[j], WGRAD ? a.MT : (rows + kT - 1) / kT, m, n);
     const int e = j - 1;
     const bool zero = j == 0 || j == a.E + 1;
     const int r0 = seg.row[j] + (WGRAD ? 0 : m * kT);
@@ -165,7 +166,7 @@ int run_grad_f32(const GradProblem& p, cudaStream_t stream) {
   a.K = p.K;
   a.R = p.total_rows;
   a.MT = (p.N + kT - 1) / kT;
-  a.NB = (p.K + kT - 1) / kT;
+  a.raster = Raster((p.K + kT - 1) / kT);
   a.out = static_cast<float*>(p.out);
   a.err = p.err;
   const bool vec = p.N % 4 == 0 && p.K % 4 == 0 && aligned16(p.dy) && aligned16(p.other) && aligned16(p.out);

@@ -48,7 +48,8 @@ struct GradArgs {
   int offsets_i64;
   int E, N, K;
   int64_t R;
-  int MT, NB;        // weight gradient: row tiles of N; both: column tiles of K
+  int MT;            // weight gradient: row tiles of N
+  Raster raster;     // of the column tiles of K
   int KS;            // input gradient: stages of N
   int f16;           // operands fp16 (else bf16)
   void* out;
@@ -82,7 +83,7 @@ __device__ __forceinline__ Tile tile_at(const SegTable& t, const GradArgs& a, in
   hint = j;
   Tile r;
   const int rows = t.row[j + 1] - t.row[j];
-  raster(tile - t.tile_start[j], FORM == kInputGrad ? (rows + kTile - 1) / kTile : a.MT, a.NB, r.m, r.n);
+  a.raster.at(tile - t.tile_start[j], FORM == kInputGrad ? (rows + kTile - 1) / kTile : a.MT, r.m, r.n);
   r.e = j - 1;
   r.row_end = t.row[j + 1];
   if (FORM == kInputGrad) {
@@ -132,8 +133,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const int segs = a.E + 2;
   if (warp == 0)
     scan_tiles(&bars->seg, segs, lane, [&](int j) {
-      if (FORM == kInputGrad) return (bars->seg.row[j + 1] - bars->seg.row[j] + kTile - 1) / kTile * a.NB;
-      return j == 0 || j == a.E + 1 ? 0 : a.MT * a.NB;
+      if (FORM == kInputGrad) return (bars->seg.row[j + 1] - bars->seg.row[j] + kTile - 1) / kTile * a.raster.nb;
+      return j == 0 || j == a.E + 1 ? 0 : a.MT * a.raster.nb;
     });
   if (tid == 0 && bars->seg.bad && blockIdx.x == 0) report_error(a.err, kErrBadArg, kSite + 1);
   tc_fence_before();
@@ -396,7 +397,7 @@ int run_grad_gemm(const GradProblem& p, cudaStream_t stream) {
   a.K = p.K;
   a.R = p.total_rows;
   a.MT = (p.N + kTile - 1) / kTile;
-  a.NB = (p.K + kTile - 1) / kTile;
+  a.raster = Raster((p.K + kTile - 1) / kTile);
   a.KS = (p.N + kSK - 1) / kSK;
   a.f16 = p.dtype == LMOE_DTYPE_F16;
   a.out = p.out;

@@ -258,16 +258,39 @@ __device__ __forceinline__ void scan_tiles(SegTable* t, int segments, int lane, 
 
 // Tile `local` of a segment of mt x nb tiles.  Tiles are walked in groups of eight row tiles,
 // column tile by column tile inside a group, so that the pairs working at the same time share
-// eight row panels and a few column panels through L2.
-__device__ __forceinline__ void raster(int local, int mt, int nb, int& m, int& n) {
-  const int per = 8 * nb;
-  const int g = local / per;
-  const int left = mt - g * 8;
-  const int gm = left < 8 ? left : 8;
-  const int in = local - g * per;
-  n = in / gm;
-  m = g * 8 + in - n * gm;
-}
+// eight row panels and a few column panels through L2.  Every role of the kernel walks the tiles
+// by itself, the MMA issuer between the MMAs of two tiles, so the two divisions are
+// multiplications (with them: ~1000 cycles a tile).
+struct Raster {
+  int nb, per;      // column tiles; tiles of a full group
+  uint32_t magic;   // floor(2^32 / per)
+  __host__ __device__ Raster(int nb_ = 1)
+      : nb(nb_), per(8 * nb_), magic((uint32_t)(0x100000000ull / (uint32_t)(8 * nb_))) {}
+  // ceil(2^32 / d) of 2 .. 7
+  static __device__ __forceinline__ uint32_t small_magic(int d) {
+    return d < 4 ? (d == 2 ? 0x80000000u : 0x55555556u)
+                 : (d < 6 ? (d == 4 ? 0x40000000u : 0x33333334u) : (d == 6 ? 0x2aaaaaabu : 0x24924925u));
+  }
+  __device__ __forceinline__ void at(int local, int mt, int& m, int& n) const {
+    // the product is below the quotient by less than one
+    int g = (int)__umulhi((uint32_t)local, magic);
+    int in = local - g * per;
+    if (in >= per) {
+      ++g;
+      in -= per;
+    }
+    const int gm = mt - g * 8;
+    if (gm >= 8) {
+      n = in >> 3;
+      m = g * 8 + (in & 7);
+    } else {
+      // ceil(2^32 / gm) is exact for in * gm < 2^32
+      const uint32_t q = gm == 1 ? (uint32_t)in : __umulhi((uint32_t)in, small_magic(gm));
+      n = (int)q;
+      m = g * 8 + in - (int)q * gm;
+    }
+  }
+};
 
 // ---------------------------------------------------------------------------------------
 // epilogue stores
