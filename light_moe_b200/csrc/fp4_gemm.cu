@@ -8,7 +8,8 @@
 // times the bf16 rate for a quarter of the bytes.  With few rows the weights' bytes bound it
 // (HBM), with many the tensor pipe.
 //
-// Tile: 256 rows (128 per CTA, TMEM lane = row) x 192 weight rows (96 per CTA in shared memory).
+// Tile: 256 rows (128 per CTA, TMEM lane = row) x 192 weight rows (96 per CTA in shared memory),
+// or fewer where the last round of tiles would leave pairs idle.
 // 192 columns because two accumulators (2 x 192) and two buffers of scales (2 x 48 columns) fit
 // the 512 TMEM columns, so the epilogue of a tile overlaps the next tile's MMAs; 256 columns
 // would leave room for one accumulator only.  The lane being the row, a thread holds a row's
@@ -70,11 +71,12 @@ struct Fp4Args {
   int64_t R;
   Raster raster;         // of the column tiles
   int KS;                // stages
+  int width, half;       // columns of a tile, of one CTA's half
   const float* alpha;    // per expert, or NULL
   const float* alpha_up;
   void* out;
   int out_dtype;
-  int vec_out;
+  int store;             // StoreMode
   uint32_t* err;
 };
 
@@ -111,9 +113,9 @@ __device__ __forceinline__ Tile tile_at(const SegTable& t, int E, const Raster& 
   return r;
 }
 
-// Instruction descriptor of the block-scaled kinds: E2M1 operands, K-major, M = 256, N = 192.
-__host__ __device__ constexpr uint32_t idesc_fp4(bool ue8m0, uint32_t sf_id) {
-  return (sf_id << 4) | (1u << 7) | (1u << 10) | ((kTN >> 3) << 17) | ((ue8m0 ? 1u : 0u) << 23) |
+// Instruction descriptor of the block-scaled kinds: E2M1 operands, K-major, M = 256, N = width.
+__host__ __device__ constexpr uint32_t idesc_fp4(bool ue8m0, uint32_t sf_id, uint32_t width) {
+  return (sf_id << 4) | (1u << 7) | (1u << 10) | ((width >> 3) << 17) | ((ue8m0 ? 1u : 0u) << 23) |
          ((uint32_t)(kTM >> 4) << 24) | (sf_id << 29);
 }
 
@@ -155,7 +157,8 @@ struct Cfg {
 static_assert(kAcc * kTN + kUnits * kUnitCols <= kTmemCols, "tensor memory budget");
 constexpr uint32_t kStageBytes = kABytes + kBBytes;
 constexpr uint32_t kSfABytes = 8 * 512, kSfBBytes = 8 * 1024, kSfSlotBytes = kSfABytes + kSfBBytes;
-constexpr uint32_t kSmem = 1024 + kStages * kStageBytes + kSfSlots * kSfSlotBytes + sizeof(Bars);
+constexpr uint32_t kSmem =
+    1024 + kStages * kStageBytes + kSfSlots * kSfSlotBytes + kEpiWarps * kStoreStageBytes + sizeof(Bars);
 static_assert(kStageBytes % 1024 == 0, "swizzle atoms");
 static_assert(kSmem <= 232448, "shared memory budget");
 
@@ -170,7 +173,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sf_base = base + kStages * kStageBytes;
-  Bars* bars = reinterpret_cast<Bars*>(sf_base + kSfSlots * kSfSlotBytes);
+  uint8_t* store_stage = sf_base + kSfSlots * kSfSlotBytes;
+  Bars* bars = reinterpret_cast<Bars*>(store_stage + kEpiWarps * kStoreStageBytes);
   volatile int* abort_flag = &bars->abort;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t rank = cluster_ctarank();
@@ -229,7 +233,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       int rows = t.row_end - r0;
       rows = rows < 0 ? 0 : (rows > kRowsCta ? kRowsCta : rows);
       const int boxes = (rows + 31) >> 5;   // only the boxes that hold this tile's rows
-      const int wrow = SWIGLU ? t.n * kHalf : t.n * kTN + (int)rank * kHalf;
+      const int wrow = SWIGLU ? t.n * a.half : t.n * a.width + (int)rank * a.half;
       for (int ks = 0; ks < KS; ++ks, st.next()) {
         ok = warp_wait(&bars->empty[st.i], st.phase ^ 1u, a.err, abort_flag, kSite + 2);
         if (!ok) break;
@@ -237,7 +241,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           uint8_t* dst = base + st.i * kStageBytes;
           const uint32_t bar = full_addr + st.i * 8;
           const int blocks = a.K - ks * kSK > kBK ? 2 : 1;
-          mbar_arrive_expect_tx_cluster(bar, (uint32_t)blocks * ((uint32_t)boxes * 4096u + kBBlock));
+          mbar_arrive_expect_tx_cluster(bar, (uint32_t)blocks * ((uint32_t)boxes * 4096u + (uint32_t)a.half * 128u));
           for (int h = 0; h < blocks; ++h) {
             const int x = ks * (kSK / 2) + h * 128;
             if (boxes == 4) {
@@ -311,10 +315,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                   const uint64_t bm = bd + (kk >> 2) * (kBBlock >> 4) + (kk & 3) * 2;
                   if (FORMAT == LMOE_FP4_MX)
                     // a word holds the scales of 128 values: of two MMAs (scale id 0 and 2)
-                    mma_fp4_pair<FORMAT>(d, am, bm, idesc_fp4(true, (m & 1) * 2), sfa + (m >> 1) * 4,
+                    mma_fp4_pair<FORMAT>(d, am, bm, idesc_fp4(true, (m & 1) * 2, a.width), sfa + (m >> 1) * 4,
                                          sfb + (m >> 1) * 8, accum | (uint32_t)(m > 0));
                   else
-                    mma_fp4_pair<FORMAT>(d, am, bm, idesc_fp4(false, 0), sfa + m * 4, sfb + m * 8,
+                    mma_fp4_pair<FORMAT>(d, am, bm, idesc_fp4(false, 0, a.width), sfa + m * 4, sfb + m * 8,
                                          accum | (uint32_t)(m > 0));
                 }
               }
@@ -359,9 +363,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             if (row < t.row_end) lp[i] = a.xs + (int64_t)row * a.xs_pitch;
           } else {
             const int c = (part - 2) * 64 + lane + 32 * i;
-            const bool up = SWIGLU && c >= kHalf;
-            const int n = SWIGLU ? t.n * kHalf + (up ? c - kHalf : c) : t.n * kTN + c;
-            if (n < a.N) lp[i] = (up ? a.ws_up : a.ws) + ((int64_t)t.e * a.N + n) * a.ws_pitch;
+            const bool up = SWIGLU && c >= a.half;
+            const int n = SWIGLU ? t.n * a.half + (up ? c - a.half : c) : t.n * a.width + c;
+            if (c < a.width && n < a.N) lp[i] = (up ? a.ws_up : a.ws) + ((int64_t)t.e * a.N + n) * a.ws_pitch;
           }
         }
         return;
@@ -430,54 +434,47 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const int q = warp & 3, cg = (warp - kEpiWarp0) >> 2;
     const uint32_t lane_base = (uint32_t)(q * 32) << 16;
     const uint32_t empty_addr = mapa_u32(&bars->acc_empty[0], 0);
-    const int64_t esize = a.out_dtype == LMOE_DTYPE_F32 ? 4 : 2;
+    const int64_t pitch = (int64_t)a.N * (a.out_dtype == LMOE_DTYPE_F32 ? 4 : 2);
+    uint8_t* stage = store_stage + (warp - kEpiWarp0) * kStoreStageBytes;
     Ring<kAcc> ac;
     int hint = 0;
     for (int tile = first; tile < total; tile += stride) {
       const Tile t = tile_at(seg, a.E, a.raster, tile, hint);
-      const int row = t.row0 + (int)rank * kRowsCta + q * 32 + lane;
-      const bool ok = row < t.row_end;
-      uint8_t* out = static_cast<uint8_t*>(a.out) + (int64_t)row * a.N * esize;
-      if (t.zero) {
-        if (ok) {
-          float z[32];
-#pragma unroll
-          for (int i = 0; i < 32; ++i) z[i] = 0.0f;
-          if (SWIGLU) {
-            store_row32(out, t.n * kHalf + cg * 32, a.N, z, a.out_dtype, a.vec_out != 0);
-          } else {
-            store_row32(out, t.n * kTN + cg * 64, a.N, z, a.out_dtype, a.vec_out != 0);
-            store_row32(out, t.n * kTN + cg * 64 + 32, a.N, z, a.out_dtype, a.vec_out != 0);
-          }
-        }
-        continue;
-      }
-      if (!warp_wait(&bars->acc_full[ac.i], ac.phase, a.err, abort_flag, kSite + 10)) break;
-      tc_fence_after();
+      const int row = t.row0 + (int)rank * kRowsCta + q * 32;   // the warp's first
+      const int rows = t.row_end - row < 32 ? t.row_end - row : 32;
+      uint8_t* out = static_cast<uint8_t*>(a.out) + (int64_t)row * pitch;
+      // output columns of the tile, and the warp's first
+      const int tile_cols = SWIGLU ? a.half : a.width;
+      const int end = (t.n + 1) * tile_cols < a.N ? (t.n + 1) * tile_cols : a.N;
+      const int c0 = t.n * tile_cols + cg * (SWIGLU ? 32 : 64);
       uint32_t u[32], v[32];
-      const uint32_t c0 = tmem + lane_base + ac.i * kTN + (SWIGLU ? cg * 32 : cg * 64);
-      tmem_ld32(c0, u);
-      tmem_ld32(c0 + (SWIGLU ? kHalf : 32), v);
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(empty_addr + ac.i * 8);
-      ac.next();
-      if (!ok) continue;
-      const float al = a.alpha ? __ldg(a.alpha + t.e) : 1.0f;
-      float f[32];
-      if (SWIGLU) {
-        const float au = a.alpha_up ? __ldg(a.alpha_up + t.e) : 1.0f;
-#pragma unroll
-        for (int i = 0; i < 32; ++i)
-          f[i] = silu(__fmul_rn(__uint_as_float(u[i]), al)) * __fmul_rn(__uint_as_float(v[i]), au);
-        store_row32(out, t.n * kHalf + cg * 32, a.N, f, a.out_dtype, a.vec_out != 0);
+      float al = 1.0f, au = 1.0f;
+      if (!t.zero) {
+        if (!warp_wait(&bars->acc_full[ac.i], ac.phase, a.err, abort_flag, kSite + 10)) break;
+        tc_fence_after();
+        const uint32_t col = tmem + lane_base + ac.i * kTN + cg * (SWIGLU ? 32 : 64);
+        tmem_ld32x2(col, col + (SWIGLU ? a.half : 32), u, v);   // inside the accumulators' columns
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(empty_addr + ac.i * 8);
+        ac.next();
+        if (a.alpha) al = __ldg(a.alpha + t.e);
+        if (SWIGLU && a.alpha_up) au = __ldg(a.alpha_up + t.e);
       } else {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) f[i] = __fmul_rn(__uint_as_float(u[i]), al);
-        store_row32(out, t.n * kTN + cg * 64, a.N, f, a.out_dtype, a.vec_out != 0);
+        for (int i = 0; i < 32; ++i) u[i] = v[i] = 0u;
+      }
+      float f[32];
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        f[i] = __fmul_rn(__uint_as_float(u[i]), al);
+        if (SWIGLU) f[i] = silu(f[i]) * __fmul_rn(__uint_as_float(v[i]), au);
+      }
+      store_rows32(out, pitch, rows, c0, end, f, a.out_dtype, a.store, stage, lane);
+      if (!SWIGLU) {
 #pragma unroll
         for (int i = 0; i < 32; ++i) f[i] = __fmul_rn(__uint_as_float(v[i]), al);
-        store_row32(out, t.n * kTN + cg * 64 + 32, a.N, f, a.out_dtype, a.vec_out != 0);
+        store_rows32(out, pitch, rows, c0 + 32, end, f, a.out_dtype, a.store, stage, lane);
       }
     }
   }
@@ -521,14 +518,20 @@ int run_fp4_gemm(const Fp4Problem& p, cudaStream_t stream) {
   a.N = p.N;
   a.K = p.K;
   a.R = p.total_rows;
-  a.raster = Raster(swiglu ? (p.N + kHalf - 1) / kHalf : (p.N + kTN - 1) / kTN);
+  const int grid = gemm_grid(dev) < 2 ? 2 : gemm_grid(dev) & ~1;   // whole pairs
+  // 160 columns instead of 192: 33.0 instead of 35.1 us for 2 rows x [2 x 14336, 4096]
+  const int64_t row_tiles = even_row_tiles(p.total_rows, p.num_experts, kTM);
+  const int widths[] = {192, 160, 128, 96};
+  auto col_tiles = [&](int w) { return swiglu ? (p.N + w / 2 - 1) / (w / 2) : (p.N + w - 1) / w; };
+  a.width = pick_width(widths, grid / 2, 112, 16, [&](int w) { return row_tiles * col_tiles(w); });
+  a.half = a.width / 2;
+  a.raster = Raster(col_tiles(a.width));
   a.KS = (p.K + kSK - 1) / kSK;
   a.alpha = p.alpha;
   a.alpha_up = p.alpha_up;
   a.out = p.out;
   a.out_dtype = p.out_dtype;
-  const int64_t esize = p.out_dtype == LMOE_DTYPE_F32 ? 4 : 2;
-  a.vec_out = ((int64_t)p.N * esize) % 32 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 31) == 0;
+  a.store = store_mode(p.out, p.N, p.out_dtype);
   a.err = p.err;
   CUtensorMap tx, tx32, tw, tu;
   const uint64_t kb = (uint64_t)p.K / 2;
@@ -538,7 +541,7 @@ int run_fp4_gemm(const Fp4Problem& p, cudaStream_t stream) {
   if (st != LMOE_OK) return st;
   const uint64_t dims[3] = {kb, (uint64_t)p.N, (uint64_t)p.num_experts};
   const uint64_t strides[2] = {kb, kb * (uint64_t)p.N};
-  const uint32_t box[3] = {128, (uint32_t)kHalf, 1};
+  const uint32_t box[3] = {128, (uint32_t)a.half, 1};
   st = encode_tmap_3d(&tw, p.wq, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, dims, strides, box);
   if (st != LMOE_OK) return st;
   tu = tw;
@@ -546,7 +549,6 @@ int run_fp4_gemm(const Fp4Problem& p, cudaStream_t stream) {
     st = encode_tmap_3d(&tu, p.wq_up, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, dims, strides, box);
     if (st != LMOE_OK) return st;
   }
-  const int grid = gemm_grid(dev) < 2 ? 2 : gemm_grid(dev) & ~1;   // whole pairs
   if (p.format == LMOE_FP4_MX)
     return swiglu ? launch<LMOE_FP4_MX, true>(tx, tx32, tw, tu, a, grid, stream)
                   : launch<LMOE_FP4_MX, false>(tx, tx32, tw, tu, a, grid, stream);

@@ -9,7 +9,8 @@
 // contraction rows, and read by tcgen05.mma as an M- or N-major operand.
 //
 // Tile: 256 x 256 on a CTA pair (128 rows of A and 128 columns of B per CTA), two accumulators
-// of 256 columns fill the 512 TMEM columns, six stages of 64 contraction values (32 KB per CTA).
+// of 256 columns fill the 512 TMEM columns, six stages of 64 contraction values (32 KB per CTA);
+// 256 x 128 where the last round of tiles would leave pairs idle.
 // Bound by the tensor pipe for prompt-sized segments; with few rows per expert the input
 // gradient is bound by reading w and the weight gradient by writing dw (HBM).
 //
@@ -54,7 +55,8 @@ struct GradArgs {
   int f16;           // operands fp16 (else bf16)
   void* out;
   int out_dtype;
-  int vec_out;
+  int width;         // columns of a tile: 256 or 128
+  int store;         // StoreMode
   uint32_t* err;
 };
 
@@ -105,7 +107,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                      const __grid_constant__ CUtensorMap tm_b, const GradArgs a) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  Bars* bars = reinterpret_cast<Bars*>(base + kStages * kStageBytes);
+  uint8_t* store_stage = base + kStages * kStageBytes;
+  Bars* bars = reinterpret_cast<Bars*>(store_stage + kEpiWarps * kStoreStageBytes);
   volatile int* abort_flag = &bars->abort;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t rank = cluster_ctarank();
@@ -154,13 +157,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     bool ok = true;
     for (int tile = first; tile < total && ok; tile += stride) {
       const Tile t = tile_at<FORM>(seg, a, tile, hint);
-      const int c0 = t.n * kTile + (int)rank * kCta;   // first column of B
+      const int c0 = t.n * a.width + (int)rank * (a.width / 2);   // first column of B
       const int m0 = (FORM == kInputGrad ? t.row0 : t.m * kTile) + (int)rank * kCta;
       int boxes = 4;   // input gradient: 32-row boxes of dy that hold this CTA's rows
       if (FORM == kInputGrad) {
         const int rows = t.row_end - m0;
         boxes = rows <= 0 ? 0 : (rows >= kCta ? 4 : (rows + 31) >> 5);
       }
+      const bool wide = a.width == kTile;
+      const uint32_t b_bytes = wide ? kOperand : kChunk;
       for (int ks = 0; ks < t.ks; ++ks, st.next()) {
         ok = warp_wait(&bars->empty[st.i], st.phase ^ 1u, a.err, abort_flag, kSite + 2);
         if (!ok) break;
@@ -169,29 +174,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           uint8_t* sb = sa + kOperand;
           const uint32_t bar = full_addr + st.i * 8;
           if (FORM == kInputGrad) {
-            mbar_arrive_expect_tx_cluster(bar, (uint32_t)boxes * 4096u + kOperand);
+            mbar_arrive_expect_tx_cluster(bar, (uint32_t)boxes * 4096u + b_bytes);
             if (boxes == 4) {
               tma_load_2d_pair(sa, &tm_a, bar, ks * kSK, m0);
             } else {
               for (int b = 0; b < boxes; ++b) tma_load_2d_pair(sa + b * 4096, &tm_a32, bar, ks * kSK, m0 + b * 32);
             }
             tma_load_3d_pair(sb, &tm_b, bar, c0, ks * kSK, t.e);
-            tma_load_3d_pair(sb + kChunk, &tm_b, bar, c0 + 64, ks * kSK, t.e);
+            if (wide) tma_load_3d_pair(sb + kChunk, &tm_b, bar, c0 + 64, ks * kSK, t.e);
           } else {
             const int r = t.row0 + ks * kSK;
             if (has_tail(t.row_end - r)) {
               uint64_t* own = &bars->tail[st.i];
-              mbar_arrive_expect_tx(own, 2 * kOperand);
+              mbar_arrive_expect_tx(own, kOperand + b_bytes);
               tma_load_2d(sa, &tm_a, own, m0, r);
               tma_load_2d(sa + kChunk, &tm_a, own, m0 + 64, r);
               tma_load_2d(sb, &tm_b, own, c0, r);
-              tma_load_2d(sb + kChunk, &tm_b, own, c0 + 64, r);
+              if (wide) tma_load_2d(sb + kChunk, &tm_b, own, c0 + 64, r);
             } else {
-              mbar_arrive_expect_tx_cluster(bar, 2 * kOperand);
+              mbar_arrive_expect_tx_cluster(bar, kOperand + b_bytes);
               tma_load_2d_pair(sa, &tm_a, bar, m0, r);
               tma_load_2d_pair(sa + kChunk, &tm_a, bar, m0 + 64, r);
               tma_load_2d_pair(sb, &tm_b, bar, c0, r);
-              tma_load_2d_pair(sb + kChunk, &tm_b, bar, c0 + 64, r);
+              if (wide) tma_load_2d_pair(sb + kChunk, &tm_b, bar, c0 + 64, r);
             }
           }
         }
@@ -202,7 +207,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer
     if (leader) {
-      const uint32_t idesc = idesc_f16kind_f32(kTile, kTile, a.f16) | kIdescBMajorMN |
+      const uint32_t idesc = idesc_f16kind_f32(kTile, a.width, a.f16) | kIdescBMajorMN |
                              (FORM == kWeightGrad ? kIdescAMajorMN : 0u);
       // descriptors count 16 bytes
       const uint64_t adesc0 = FORM == kInputGrad ? sdesc_k_sw128(smem_u32(base)) : sdesc_mn_sw128(smem_u32(base), kChunk);
@@ -273,27 +278,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const int q = warp & 3, half = (warp - kEpiWarp0) >> 2;
     const uint32_t lane_base = (uint32_t)(q * 32) << 16;
     const uint32_t empty_addr = mapa_u32(&bars->acc_empty[0], 0);
-    const int64_t esize = a.out_dtype == LMOE_DTYPE_F32 ? 4 : 2;
+    const int64_t pitch = (int64_t)a.K * (a.out_dtype == LMOE_DTYPE_F32 ? 4 : 2);
+    uint8_t* stage = store_stage + (warp - kEpiWarp0) * kStoreStageBytes;
     Ring<kAcc> ac;
     int hint = 0;
     for (int tile = first; tile < total; tile += stride) {
       const Tile t = tile_at<FORM>(seg, a, tile, hint);
-      const int r = (int)rank * kCta + q * 32 + lane;
+      // the warp's 32 rows, and the first of its half of the columns
+      const int r = (int)rank * kCta + q * 32;
+      const int left = FORM == kInputGrad ? t.row_end - t.row0 - r : a.N - t.m * kTile - r;
+      const int rows = left < 32 ? left : 32;
       const int64_t row = FORM == kInputGrad ? (int64_t)t.row0 + r : (int64_t)t.e * a.N + t.m * kTile + r;
-      const bool ok = FORM == kInputGrad ? t.row0 + r < t.row_end : t.m * kTile + r < a.N;
-      void* out = static_cast<uint8_t*>(a.out) + row * a.K * esize;
-      const int c0 = t.n * kTile + half * kCta;
+      uint8_t* out = static_cast<uint8_t*>(a.out) + row * pitch;
+      const int cols = a.width / 2;
+      const int c0 = t.n * a.width + half * cols;
       if (t.ks != 0) {
         if (!warp_wait(&bars->acc_full[ac.i], ac.phase, a.err, abort_flag, kSite + 9)) break;
         tc_fence_after();
       }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < cols; j += 32) {
         float f[32];
         if (t.ks != 0) {
           uint32_t u[32];
-          tmem_ld32(tmem + lane_base + ac.i * kTile + half * kCta + j * 32, u);
-          if (j == 3) {
+          tmem_ld32(tmem + lane_base + ac.i * kTile + half * cols + j, u);
+          if (j + 32 == cols) {
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster(empty_addr + ac.i * 8);
@@ -305,7 +313,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int i = 0; i < 32; ++i) f[i] = 0.0f;
         }
-        if (ok) store_row32(out, c0 + j * 32, a.K, f, a.out_dtype, a.vec_out != 0);
+        store_rows32(out, pitch, rows, c0 + j, a.K, f, a.out_dtype, a.store, stage, lane);
       }
     }
   }
@@ -345,7 +353,7 @@ int pad_rows(const void* src, int64_t rows, int cols, int pitch, void* dst, cons
 template <int FORM>
 int launch(const CUtensorMap& ta, const CUtensorMap& ta32, const CUtensorMap& tb, const GradArgs& a, int grid,
            cudaStream_t stream) {
-  constexpr size_t smem = 1024 + kStages * kStageBytes + sizeof(Bars);
+  constexpr size_t smem = 1024 + kStages * kStageBytes + kEpiWarps * kStoreStageBytes + sizeof(Bars);
   static_assert(smem <= 232448, "shared memory budget");
   auto fn = grad_gemm_kernel<FORM>;
   const int st = set_max_dynamic_smem(reinterpret_cast<const void*>(fn), smem);
@@ -397,17 +405,20 @@ int run_grad_gemm(const GradProblem& p, cudaStream_t stream) {
   a.K = p.K;
   a.R = p.total_rows;
   a.MT = (p.N + kTile - 1) / kTile;
-  a.raster = Raster((p.K + kTile - 1) / kTile);
   a.KS = (p.N + kSK - 1) / kSK;
   a.f16 = p.dtype == LMOE_DTYPE_F16;
   a.out = p.out;
   a.out_dtype = p.out_dtype;
-  const int64_t esize = p.out_dtype == LMOE_DTYPE_F32 ? 4 : 2;
-  a.vec_out = ((int64_t)p.K * esize) % 32 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 31) == 0;
+  a.store = store_mode(p.out, p.K, p.out_dtype);
   a.err = p.err;
   const CUtensorMapDataType dt = a.f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   CUtensorMap ta, ta32, tb;
   const int grid = gemm_grid(dev) < 2 ? 2 : gemm_grid(dev) & ~1;   // whole pairs
+  const int64_t row_tiles = p.weight_grad ? (int64_t)a.MT * p.num_experts
+                                          : even_row_tiles(p.total_rows, p.num_experts, kTile);
+  const int widths[] = {256, 128};
+  a.width = pick_width(widths, grid / 2, 0, 16, [&](int w) { return row_tiles * ((p.K + w - 1) / w); });
+  a.raster = Raster((p.K + a.width - 1) / a.width);
   // the maps end at the true sizes, so that TMA fills what lies behind them with zeros
   if (p.weight_grad) {
     st = encode_tmap_2d(&ta, dy, dt, 2, (uint64_t)p.total_rows, (uint64_t)p.N, (uint64_t)ldy * 2, kSK, 64, true);

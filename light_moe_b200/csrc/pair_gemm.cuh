@@ -200,6 +200,27 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
       : "memory");
 }
 
+// Two of them under one completion wait.
+__device__ __forceinline__ void tmem_ld32x2(uint32_t taddr0, uint32_t taddr1, uint32_t (&r)[32], uint32_t (&u)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%64];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
+      "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%65];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
+        "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),
+        "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]),
+        "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]),
+        "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]), "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]),
+        "=r"(u[13]), "=r"(u[14]), "=r"(u[15]), "=r"(u[16]), "=r"(u[17]), "=r"(u[18]), "=r"(u[19]),
+        "=r"(u[20]), "=r"(u[21]), "=r"(u[22]), "=r"(u[23]), "=r"(u[24]), "=r"(u[25]), "=r"(u[26]),
+        "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
+      : "r"(taddr0), "r"(taddr1)
+      : "memory");
+}
+
 // ---------------------------------------------------------------------------------------
 // segments
 // ---------------------------------------------------------------------------------------
@@ -310,41 +331,114 @@ __device__ __forceinline__ void st_global_v8(void* p, const uint32_t (&v)[8]) {
                : "memory");
 }
 
-// 32 consecutive values of one output row from column c0 (columns >= cols are not written).
-// vec: every row starts at a multiple of 32 bytes, so whole 32-byte sectors are stored.
-__device__ __forceinline__ void store_row32(void* row, int c0, int cols, const float (&v)[32], int dtype, bool vec) {
-  if (c0 >= cols) return;
-  if (vec && c0 + 32 <= cols) {
+// How rows of an output can be stored: whole 32-byte sectors, 16-byte vectors, or neither.
+enum StoreMode : int { kStoreStaged = 0, kStore16 = 16, kStore32 = 32 };
+inline int store_mode(const void* out, int64_t cols, int dtype) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(out) | (uintptr_t)(cols * (dtype == LMOE_DTYPE_F32 ? 4 : 2));
+  return a % 32 == 0 ? kStore32 : (a % 16 == 0 ? kStore16 : kStoreStaged);
+}
+constexpr uint32_t kStoreStageBytes = 1152;   // per warp
+
+// Called by a whole warp: lane l holds 32 values of row l (of `rows` valid ones) from column c0;
+// columns at or behind `cols` are not written.  Rows that start at odd addresses go through
+// `stage` (kStoreStageBytes of the warp's own), so that neighbouring lanes write neighbouring
+// columns: storing them value by value from the lanes that hold them touches 32 sectors per
+// instruction (the gradients of fp16 rows of odd lengths took 7.9 ms, of which ~7 ms stores).
+__device__ __forceinline__ void store_rows32(uint8_t* base, int64_t pitch, int rows, int c0, int cols,
+                                             const float (&v)[32], int dtype, int mode, uint8_t* stage, int lane) {
+  if (c0 >= cols || rows <= 0) return;
+  const bool f16 = dtype == LMOE_DTYPE_F16;
+  if (mode != kStoreStaged) {
+    if (lane >= rows) return;
+    uint8_t* row = base + lane * pitch;
     if (dtype == LMOE_DTYPE_F32) {
-      float* p = static_cast<float*>(row) + c0;
+      float* p = reinterpret_cast<float*>(row) + c0;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        uint32_t w[8];
+        if (mode == kStore32 && c0 + 8 * j < cols) {
+          uint32_t w[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(v[8 * j + i]);
-        st_global_v8(p + 8 * j, w);
+          for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(v[8 * j + i]);
+          st_global_v8(p + 8 * j, w);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            if (c0 + 8 * j + 4 * i < cols)
+              *reinterpret_cast<float4*>(p + 8 * j + 4 * i) =
+                  make_float4(v[8 * j + 4 * i], v[8 * j + 4 * i + 1], v[8 * j + 4 * i + 2], v[8 * j + 4 * i + 3]);
+        }
       }
     } else {
-      uint16_t* p = static_cast<uint16_t*>(row) + c0;
+      uint16_t* p = reinterpret_cast<uint16_t*>(row) + c0;
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         uint32_t w[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) w[i] = pack16(v[16 * j + 2 * i], v[16 * j + 2 * i + 1], dtype == LMOE_DTYPE_F16);
-        st_global_v8(p + 16 * j, w);
+        for (int i = 0; i < 8; ++i) w[i] = pack16(v[16 * j + 2 * i], v[16 * j + 2 * i + 1], f16);
+        if (mode == kStore32 && c0 + 16 * j < cols) {
+          st_global_v8(p + 16 * j, w);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            if (c0 + 16 * j + 8 * i < cols)
+              *reinterpret_cast<uint4*>(p + 16 * j + 8 * i) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+        }
       }
     }
     return;
   }
+  if (dtype == LMOE_DTYPE_F32) {
+    float* st = reinterpret_cast<float*>(stage);   // [32][9]
 #pragma unroll
-  for (int i = 0; i < 32; ++i) {
-    if (c0 + i < cols) {
-      if (dtype == LMOE_DTYPE_F32)
-        static_cast<float*>(row)[c0 + i] = v[i];
-      else
-        static_cast<uint16_t*>(row)[c0 + i] = (uint16_t)(pack16(v[i], 0.0f, dtype == LMOE_DTYPE_F16) & 0xffffu);
+    for (int ch = 0; ch < 4; ++ch) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) st[lane * 9 + i] = v[8 * ch + i];
+      __syncwarp();
+      const int c = c0 + 8 * ch + (lane & 7);
+      for (int r = lane >> 3; r < rows; r += 4)
+        if (c < cols) reinterpret_cast<float*>(base + r * pitch)[c] = st[r * 9 + (lane & 7)];
+      __syncwarp();
+    }
+  } else {
+#pragma unroll
+    for (int ch = 0; ch < 2; ++ch) {   // [32][18] 16-bit values
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        *reinterpret_cast<uint32_t*>(stage + lane * 36 + i * 4) = pack16(v[16 * ch + 2 * i], v[16 * ch + 2 * i + 1], f16);
+      __syncwarp();
+      const int c = c0 + 16 * ch + (lane & 15);
+      for (int r = lane >> 4; r < rows; r += 2)
+        if (c < cols)
+          reinterpret_cast<uint16_t*>(base + r * pitch)[c] =
+              *reinterpret_cast<const uint16_t*>(stage + r * 36 + (lane & 15) * 2);
+      __syncwarp();
     }
   }
+}
+
+// Width of the column tiles: the one with the shortest static schedule of `tiles(width)` tiles on
+// `pairs` pairs, a round taking as long as its columns and a constant (`floor_cols`: what a
+// round costs at least, `extra`: what a tile costs beside its columns).  With few rows a kernel
+// streams weights, and the last round of wide tiles leaves most pairs idle.
+template <int N, typename F>
+inline int pick_width(const int (&widths)[N], int pairs, int floor_cols, int extra, F tiles) {
+  int best = widths[0];
+  int64_t best_cost = INT64_MAX;
+  for (int w : widths) {
+    const int64_t rounds = (tiles(w) + pairs - 1) / pairs;
+    const int64_t cost = rounds * ((w > floor_cols ? w : floor_cols) + extra);
+    if (cost < best_cost) {
+      best_cost = cost;
+      best = w;
+    }
+  }
+  return best;
+}
+// Row tiles of `rows` rows spread evenly over `experts` experts (the counts are on the device).
+inline int64_t even_row_tiles(int64_t rows, int experts, int tile) {
+  if (rows <= experts) return rows;
+  const int64_t each = (rows + experts - 1) / experts;
+  return (each + tile - 1) / tile * experts;
 }
 
 }  // namespace lmoe
