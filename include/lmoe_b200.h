@@ -275,12 +275,12 @@ int lmoe_fp4_scale_pitch(int K, int format);
 /* x: [rows, K] of LMOE_DTYPE_*, rows ldx elements apart.  global_scale (LMOE_FP4_NV; NULL = 1):
  * one fp32 value per rows_per_scale rows.  positions (optional): int32 [rows, copies], the output
  * rows that row r is written to (entries outside [0, out_rows) are skipped); without it copies
- * = 1 and out_rows = rows.  q [out_rows, K/2] 8-byte aligned; scales [out_rows, pitch]. */
+ * = 1 and out_rows = rows.  q [out_rows, K/2] 16-byte aligned; scales [out_rows, pitch], 2-byte aligned. */
 int lmoe_quantize_fp4(const void* x, int dtype, int64_t rows, int K, int64_t ldx, int format,
                       const float* global_scale, int64_t rows_per_scale, const int32_t* positions, int copies,
                       int64_t out_rows, uint8_t* q, uint8_t* scales, lmoe_stream_t stream);
 
-/* out: bf16 [rows, K], 16-byte aligned; scale rows scale_pitch bytes apart. */
+/* q and out (bf16 [rows, K]) 16-byte aligned; scale rows scale_pitch bytes apart. */
 int lmoe_dequantize_fp4(const uint8_t* q, const uint8_t* scales, int64_t scale_pitch, int64_t rows, int K, int format,
                         const float* global_scale, int64_t rows_per_scale, void* out, lmoe_stream_t stream);
 

@@ -44,27 +44,27 @@ __device__ __forceinline__ float e4m3_value(uint32_t byte) {
   return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)byte, __NV_E4M3)));
 }
 
-// Codes of 16 values of one row under one scale.  `a` holds the values; the block's largest
-// absolute value is `amax` (finite).  MX: the scale is a power of two, so x / scale is exact.
-// Returns the scale byte.
-__device__ __forceinline__ uint32_t fp4_encode_mx(const float (&a)[16], float amax, uint2& codes) {
-  const uint32_t bits = __float_as_uint(amax);
-  int e = (int)(bits >> 23) - 127 - 2;   // below the normal range: the clamp applies either way
+// 1 / x, off by at most one unit in the last place (2^-23).
+__device__ __forceinline__ float rcp_approx(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// Scale byte of an MX block whose largest absolute value is amax (finite).  *mul = 1 / scale: a
+// power of two, so x / scale is exact.
+__device__ __forceinline__ uint32_t fp4_mx_scale(float amax, float* mul) {
+  int e = (int)(__float_as_uint(amax) >> 23) - 127 - 2;   // below the normal range: the clamp applies either way
   e = e < -127 ? -127 : e;
-  const int up = -e;                     // multiply by 2^up, -125 <= up <= 127
-  const float m = __uint_as_float((uint32_t)(up + 127) << 23);
-  float t[16];
-#pragma unroll
-  for (int i = 0; i < 16; ++i) t[i] = __fmul_rn(a[i], m);
-  codes.x = fp4_pack8(t);
-  codes.y = fp4_pack8(t + 8);
+  *mul = __uint_as_float((uint32_t)(127 - e) << 23);      // 2^-e, -125 <= -e <= 127
   return (uint32_t)(e + 127);
 }
 
-// NV: s is the E4M3 value nearest to amax / (6 g).  The double quotient cannot land on the
-// wrong side of a midpoint: amax and midpoint * 6 g are integers of at most 31 bits in a common
-// unit, so they differ by more than 2^-32 relative or not at all.
-__device__ __forceinline__ float fp4_nv_scale(float amax, float g) {
+// NV: s is the E4M3 value nearest to amax / (6 g), at most 448.
+// Exactly: the double quotient cannot land on the wrong side of a midpoint, since amax and
+// midpoint * 6 g are integers of at most 31 bits in a common unit and differ by more than 2^-32
+// relative or not at all.
+static __device__ __noinline__ float fp4_nv_scale_exact(float amax, float g) {
   const double t = (double)amax / (6.0 * (double)g);
   if (t >= 448.0) return 448.0f;
   const float tf = (float)t;
@@ -75,6 +75,17 @@ __device__ __forceinline__ float fp4_nv_scale(float amax, float g) {
   const double step = (double)__uint_as_float((uint32_t)(e - 3 + 127) << 23);
   const double inv = (double)__uint_as_float((uint32_t)(3 - e + 127) << 23);
   return (float)(rint(t * inv) * step);
+}
+// r6 = rcp_approx(6 g): the product with it is off by less than 2^-22 + 2^-24, below 2^-17 of a
+// step (a value has at most 16), so clear of a midpoint by 2^-16 its rounding is the exact one.
+__device__ __forceinline__ float fp4_nv_scale(float amax, float g, float r6) {
+  const float t = __fmul_rn(amax, r6);
+  int e = (int)(__float_as_uint(t) >> 23) - 127;
+  e = e < -6 ? -6 : e;
+  const float u = __fmul_rn(t, __uint_as_float((uint32_t)(3 - e + 127) << 23));   // exact, in steps
+  const float n = rintf(u);
+  if (!(t < 440.0f) || !(t > 1e-30f) || fabsf(fabsf(u - n) - 0.5f) < 0x1p-16f) return fp4_nv_scale_exact(amax, g);
+  return __fmul_rn(n, __uint_as_float((uint32_t)(e - 3 + 127) << 23));
 }
 
 // Code of |x| by exact comparisons with the borders b * s * g between codes: b * s is exact in
@@ -92,15 +103,15 @@ __device__ __forceinline__ uint32_t fp4_exact_code(float x, float s, float g) {
   return c | (__float_as_uint(x) >> 31 << 3);
 }
 
-// The codes come from the rounded product with the reciprocal (three roundings, below 2^-21
-// relative); where a border lies that near, they come from fp4_exact_code.
-__device__ __forceinline__ uint32_t fp4_encode_nv(const float (&a)[16], float amax, float g, uint2& codes) {
-  const float s = fp4_nv_scale(amax, g);
+// The codes come from the rounded product with the reciprocal (three roundings and the reciprocal's
+// unit, below 2^-21 relative); where a border lies that near, they come from fp4_exact_code.
+__device__ __forceinline__ uint32_t fp4_encode_nv(const float* a, float amax, float g, float r6, uint2& codes) {
+  const float s = fp4_nv_scale(amax, g, r6);
   codes = make_uint2(0u, 0u);
   if (s > 0.0f) {
     const float d = __fmul_rn(s, g);
     const bool plain = d > 1e-30f && d < 1e30f;
-    const float r = __frcp_rn(plain ? d : 1.0f);
+    const float r = rcp_approx(plain ? d : 1.0f);
     float lo[16], hi[16];
     const float down = 1.0f - 0x1p-20f, upf = 1.0f + 0x1p-20f;
     const float rl = __fmul_rn(r, down), rh = __fmul_rn(r, upf);

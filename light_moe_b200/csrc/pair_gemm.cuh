@@ -325,12 +325,6 @@ __device__ __forceinline__ uint32_t pack16(float a, float b, int f16) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-__device__ __forceinline__ void st_global_v8(void* p, const uint32_t (&v)[8]) {
-  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
-               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
-               : "memory");
-}
-
 // How rows of an output can be stored: whole 32-byte sectors, 16-byte vectors, or neither.
 enum StoreMode : int { kStoreStaged = 0, kStore16 = 16, kStore32 = 32 };
 inline int store_mode(const void* out, int64_t cols, int dtype) {
