@@ -234,14 +234,18 @@ int lmoe_w4a16_grouped_gemm(const void* input, int64_t total_rows, int K, const 
 
 /* Gradients of lmoe_grouped_gemm, y[r, n] = sum_k input[r, k] * weights[e, n, k], for the rows
  * [offsets[e], offsets[e + 1]) of expert e; dtype of all operands LMOE_DTYPE_* (bf16 and fp16 on
- * tensor cores with fp32 accumulation, fp32 in fp32 on CUDA cores); any N, K >= 1.
+ * tensor cores with fp32 accumulation; fp32 as sums of bf16 products of fp32 accuracy on tensor
+ * cores, or in fp32 on CUDA cores); any N, K >= 1.
  *   dgrad: grad_input [total_rows, K] = grad_output [total_rows, N] * weights [E, N, K] of the
  *          row's expert; rows outside every expert are zero
  *   wgrad: grad_weights [E, N, K] (out_dtype: dtype or LMOE_DTYPE_F32), the sum over the
  *          expert's rows of grad_output^T * input; experts without rows are zero
  * 16-bit operands with row lengths that are multiples of 8 are read where they lie and must be
- * 16-byte aligned; other row lengths are copied into the workspace first
- * (lmoe_grouped_gemm_grad_workspace_bytes, 0 where no copy is made).
+ * 16-byte aligned; other row lengths are copied into the workspace first.  fp32 operands of many
+ * rows per expert are written to the workspace as three bf16 planes each; without a workspace
+ * (NULL) they take the CUDA cores.  lmoe_grouped_gemm_grad_workspace_bytes: 0 where no copy is
+ * made.  Operands that are not finite give results that are not finite (fp32 on tensor cores: NaN
+ * where fp32 may give an infinity).
  * error: a device word that the caller has zeroed, or NULL.  Offsets that decrease or leave
  * [0, total_rows] set it, and every row then counts as outside every expert.
  * The reference's backward is autograd through one mm_out per expert (csrc/grouped_gemm.cu:30-40,

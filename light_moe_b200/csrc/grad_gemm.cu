@@ -19,6 +19,13 @@
 // a product with a zero row would not do, since those rows may hold infinities or NaN.  Experts
 // without rows get a zero dw, rows outside every expert a zero dx.
 //
+// fp32 operands (SPLIT) are first written as three bf16 planes each, x = high + middle + low to
+// 2^-26, and the tile sums the six products of planes down to 2^-18: (l, h), (h, l), (m, m),
+// (m, h), (h, m), (h, h), six times the bf16 work at ~16 times the FFMA rate.  The tensor pipe
+// truncates its sums (measured: 1024 bf16 products of mean 1 come out 8e-7 low, 8192 2.5e-5), so
+// a TMEM accumulator takes 128 contraction values only, small products first, and the epilogue
+// adds the accumulators in registers, rounding to nearest.
+//
 // Warps: 0 TMA producer, whose copies complete on the leader's stage barrier; 1 MMA issuer
 // (leader CTA); 2 clears the tail of a segment's last stage (whose copies complete on a barrier
 // of its own CTA) and hands it to the leader; 4-11 epilogue, eight warps of 32 rows x 128 columns.
@@ -41,6 +48,10 @@ constexpr uint32_t kChunk = 64 * 128;             // 64 contraction rows of 64 c
 constexpr uint32_t kOperand = 2 * kChunk;         // 128 x 64 values of one operand
 constexpr uint32_t kStageBytes = 2 * kOperand;
 constexpr uint32_t kSite = 0x600u;
+
+// fp32 operands are split from this many rows per expert on (below, the copies cost more than the
+// CUDA cores' products).
+constexpr int kSplitRowsX = 48, kSplitRowsW = 16;
 
 enum Form { kInputGrad = 0, kWeightGrad = 1 };
 
@@ -98,10 +109,32 @@ __device__ __forceinline__ Tile tile_at(const SegTable& t, const GradArgs& a, in
   return r;
 }
 
+// The stages of a tile: one after another into one accumulator, or (SPLIT) two at a time into an
+// accumulator of their own, once for each pair of planes, the small products first.
+template <bool SPLIT>
+struct Passes {
+  static constexpr int kStep = 2, kPairs = 6;
+  int step;
+  __device__ __forceinline__ explicit Passes(int ks) : step(SPLIT ? kStep : (ks > 0 ? ks : 1)) {}
+  __device__ __forceinline__ int stages(int ks0, int ks) const {
+    const int n = ks - ks0 < step ? ks - ks0 : step;
+    return SPLIT ? n * kPairs : n;
+  }
+  // Stage i of n: its offset in contraction stages, and the planes (0 high, 1 middle, 2 low).
+  __device__ __forceinline__ int at(int i, int n, int& pa, int& pb) const {
+    pa = pb = 0;
+    if (!SPLIT) return i;
+    const int pair = n == 2 * kPairs ? i >> 1 : i;
+    pa = (0x001102 >> (4 * pair)) & 15;   // l, h, m, m, h, h
+    pb = (0x010120 >> (4 * pair)) & 15;   // h, l, m, h, m, h
+    return n == 2 * kPairs ? i & 1 : 0;
+  }
+};
+
 // Whether a stage with `left` rows of its segment ends inside the 16 rows of an MMA.
 __device__ __forceinline__ bool has_tail(int left) { return left < kSK && (left & 15) != 0; }
 
-template <int FORM>
+template <int FORM, bool SPLIT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     grad_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_a32,
                      const __grid_constant__ CUtensorMap tm_b, const GradArgs a) {
@@ -166,37 +199,44 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       }
       const bool wide = a.width == kTile;
       const uint32_t b_bytes = wide ? kOperand : kChunk;
-      for (int ks = 0; ks < t.ks; ++ks, st.next()) {
-        ok = warp_wait(&bars->empty[st.i], st.phase ^ 1u, a.err, abort_flag, kSite + 2);
-        if (!ok) break;
-        if (elect_one()) {
-          uint8_t* sa = base + st.i * kStageBytes;
-          uint8_t* sb = sa + kOperand;
-          const uint32_t bar = full_addr + st.i * 8;
-          if (FORM == kInputGrad) {
-            mbar_arrive_expect_tx_cluster(bar, (uint32_t)boxes * 4096u + b_bytes);
-            if (boxes == 4) {
-              tma_load_2d_pair(sa, &tm_a, bar, ks * kSK, m0);
+      const Passes<SPLIT> ps(t.ks);
+      for (int ks0 = 0; ks0 < t.ks && ok; ks0 += ps.step) {
+        const int n = ps.stages(ks0, t.ks);
+        for (int i = 0; i < n; ++i, st.next()) {
+          ok = warp_wait(&bars->empty[st.i], st.phase ^ 1u, a.err, abort_flag, kSite + 2);
+          if (!ok) break;
+          int pa, pb;   // planes of the operands
+          const int ks = ks0 + ps.at(i, n, pa, pb);
+          if (elect_one()) {
+            uint8_t* sa = base + st.i * kStageBytes;
+            uint8_t* sb = sa + kOperand;
+            const uint32_t bar = full_addr + st.i * 8;
+            if (FORM == kInputGrad) {
+              const int y = m0 + pa * (int)a.R;
+              mbar_arrive_expect_tx_cluster(bar, (uint32_t)boxes * 4096u + b_bytes);
+              if (boxes == 4) {
+                tma_load_2d_pair(sa, &tm_a, bar, ks * kSK, y);
+              } else {
+                for (int b = 0; b < boxes; ++b) tma_load_2d_pair(sa + b * 4096, &tm_a32, bar, ks * kSK, y + b * 32);
+              }
+              tma_load_3d_pair(sb, &tm_b, bar, c0, ks * kSK, t.e + pb * a.E);
+              if (wide) tma_load_3d_pair(sb + kChunk, &tm_b, bar, c0 + 64, ks * kSK, t.e + pb * a.E);
             } else {
-              for (int b = 0; b < boxes; ++b) tma_load_2d_pair(sa + b * 4096, &tm_a32, bar, ks * kSK, m0 + b * 32);
-            }
-            tma_load_3d_pair(sb, &tm_b, bar, c0, ks * kSK, t.e);
-            if (wide) tma_load_3d_pair(sb + kChunk, &tm_b, bar, c0 + 64, ks * kSK, t.e);
-          } else {
-            const int r = t.row0 + ks * kSK;
-            if (has_tail(t.row_end - r)) {
-              uint64_t* own = &bars->tail[st.i];
-              mbar_arrive_expect_tx(own, kOperand + b_bytes);
-              tma_load_2d(sa, &tm_a, own, m0, r);
-              tma_load_2d(sa + kChunk, &tm_a, own, m0 + 64, r);
-              tma_load_2d(sb, &tm_b, own, c0, r);
-              if (wide) tma_load_2d(sb + kChunk, &tm_b, own, c0 + 64, r);
-            } else {
-              mbar_arrive_expect_tx_cluster(bar, kOperand + b_bytes);
-              tma_load_2d_pair(sa, &tm_a, bar, m0, r);
-              tma_load_2d_pair(sa + kChunk, &tm_a, bar, m0 + 64, r);
-              tma_load_2d_pair(sb, &tm_b, bar, c0, r);
-              if (wide) tma_load_2d_pair(sb + kChunk, &tm_b, bar, c0 + 64, r);
+              const int r = t.row0 + ks * kSK, ra = r + pa * (int)a.R, rb = r + pb * (int)a.R;
+              if (has_tail(t.row_end - r)) {
+                uint64_t* own = &bars->tail[st.i];
+                mbar_arrive_expect_tx(own, kOperand + b_bytes);
+                tma_load_2d(sa, &tm_a, own, m0, ra);
+                tma_load_2d(sa + kChunk, &tm_a, own, m0 + 64, ra);
+                tma_load_2d(sb, &tm_b, own, c0, rb);
+                if (wide) tma_load_2d(sb + kChunk, &tm_b, own, c0 + 64, rb);
+              } else {
+                mbar_arrive_expect_tx_cluster(bar, kOperand + b_bytes);
+                tma_load_2d_pair(sa, &tm_a, bar, m0, ra);
+                tma_load_2d_pair(sa + kChunk, &tm_a, bar, m0 + 64, ra);
+                tma_load_2d_pair(sb, &tm_b, bar, c0, rb);
+                if (wide) tma_load_2d_pair(sb + kChunk, &tm_b, bar, c0 + 64, rb);
+              }
             }
           }
         }
@@ -218,27 +258,32 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       bool ok = true;
       for (int tile = first; tile < total && ok; tile += stride) {
         const Tile t = tile_at<FORM>(seg, a, tile, hint);
-        if (t.ks == 0) continue;
-        ok = warp_wait(&bars->acc_empty[ac.i], ac.phase ^ 1u, a.err, abort_flag, kSite + 4);
-        if (!ok) break;
-        const uint32_t d = tmem + ac.i * kTile;
-        int left = FORM == kInputGrad ? a.N : t.row_end - t.row0;
-        for (int ks = 0; ks < t.ks; ++ks, st.next(), left -= kSK) {
-          ok = warp_wait(&bars->full[st.i], st.phase, a.err, abort_flag, kSite + 6);
+        const Passes<SPLIT> ps(t.ks);
+        const int depth = FORM == kInputGrad ? a.N : t.row_end - t.row0;
+        for (int ks0 = 0; ks0 < t.ks && ok; ks0 += ps.step) {
+          ok = warp_wait(&bars->acc_empty[ac.i], ac.phase ^ 1u, a.err, abort_flag, kSite + 4);
           if (!ok) break;
-          tc_fence_after();
-          if (elect_one()) {
-            const uint64_t ad = adesc0 + st.i * (kStageBytes >> 4), bd = bdesc0 + st.i * (kStageBytes >> 4);
+          const uint32_t d = tmem + ac.i * kTile;
+          const int n = ps.stages(ks0, t.ks);
+          for (int i = 0; i < n; ++i, st.next()) {
+            ok = warp_wait(&bars->full[st.i], st.phase, a.err, abort_flag, kSite + 6);
+            if (!ok) break;
+            tc_fence_after();
+            int pa, pb;
+            const int left = depth - (ks0 + ps.at(i, n, pa, pb)) * kSK;
+            if (elect_one()) {
+              const uint64_t ad = adesc0 + st.i * (kStageBytes >> 4), bd = bdesc0 + st.i * (kStageBytes >> 4);
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
-              if (kk * 16 < left)
-                mma_ss_pair(d, ad + kk * (FORM == kInputGrad ? 2 : 128), bd + kk * 128, idesc, (ks | kk) != 0 ? 1u : 0u);
-            mma_commit_pair(&bars->empty[st.i]);
-            if (ks == t.ks - 1) mma_commit_pair(&bars->acc_full[ac.i]);
+              for (int kk = 0; kk < 4; ++kk)
+                if (kk * 16 < left)
+                  mma_ss_pair(d, ad + kk * (FORM == kInputGrad ? 2 : 128), bd + kk * 128, idesc, (i | kk) != 0 ? 1u : 0u);
+              mma_commit_pair(&bars->empty[st.i]);
+              if (i == n - 1) mma_commit_pair(&bars->acc_full[ac.i]);
+            }
+            __syncwarp();
           }
-          __syncwarp();
+          ac.next();
         }
-        ac.next();
       }
       if (elect_one()) mma_commit_leader(&bars->mma_done);
       mbar_wait(&bars->mma_done, 0, a.err, nullptr, kSite + 7);
@@ -246,31 +291,35 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   } else if (warp == 2) {
     // ------------------------------------------------------------------ segment tails
     if (FORM == kWeightGrad) {
-      uint32_t it = 0, tail_parity = 0;   // a bit per stage
+      Ring<kStages> st;
+      uint32_t tail_parity = 0;   // a bit per stage
       int hint = 0;
       bool ok = true;
       for (int tile = first; tile < total && ok; tile += stride) {
         const Tile t = tile_at<FORM>(seg, a, tile, hint);
-        if (t.ks == 0) continue;
-        it += t.ks;
-        const int left = t.row_end - t.row0 - (t.ks - 1) * kSK;
-        if (!has_tail(left)) continue;
-        const int s = (it - 1) % kStages;
-        ok = mbar_wait(&bars->tail[s], tail_parity >> s & 1u, a.err, abort_flag, kSite + 8);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        tail_parity ^= 1u << s;
-        // contraction rows [left, next multiple of 16) of the four chunks; a row is one 128-byte
-        // line, which the swizzle only permutes
-        const int n = (16 - (left & 15)) * 8;
-        uint8_t* st = base + s * kStageBytes + left * 128;
-        for (int i = lane; i < 4 * n; i += 32) {
-          const int c = i / n;
-          *reinterpret_cast<uint4*>(st + c * kChunk + (i - c * n) * 16) = make_uint4(0, 0, 0, 0);
+        const Passes<SPLIT> ps(t.ks);
+        const int left = t.row_end - t.row0 - (t.ks - 1) * kSK;   // rows of the last stage
+        for (int ks0 = 0; ks0 < t.ks && ok; ks0 += ps.step) {
+          const int n = ps.stages(ks0, t.ks);
+          for (int i = 0; i < n && ok; ++i, st.next()) {
+            int pa, pb;
+            if (ks0 + ps.at(i, n, pa, pb) != t.ks - 1 || !has_tail(left)) continue;
+            ok = warp_wait(&bars->tail[st.i], tail_parity >> st.i & 1u, a.err, abort_flag, kSite + 8);
+            if (!ok) break;
+            tail_parity ^= 1u << st.i;
+            // contraction rows [left, next multiple of 16) of the four chunks; a row is one
+            // 128-byte line, which the swizzle only permutes
+            const int m = (16 - (left & 15)) * 8;
+            uint8_t* at = base + st.i * kStageBytes + left * 128;
+            for (int k = lane; k < 4 * m; k += 32) {
+              const int c = k / m;
+              *reinterpret_cast<uint4*>(at + c * kChunk + (k - c * m) * 16) = make_uint4(0, 0, 0, 0);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(mapa_u32(&bars->full[st.i], 0));
+          }
         }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(mapa_u32(&bars->full[s], 0));
       }
     }
   } else if (warp >= kEpiWarp0) {
@@ -282,6 +331,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     uint8_t* stage = store_stage + (warp - kEpiWarp0) * kStoreStageBytes;
     Ring<kAcc> ac;
     int hint = 0;
+    bool ok = true;
     for (int tile = first; tile < total; tile += stride) {
       const Tile t = tile_at<FORM>(seg, a, tile, hint);
       // the warp's 32 rows, and the first of its half of the columns
@@ -292,28 +342,62 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       uint8_t* out = static_cast<uint8_t*>(a.out) + row * pitch;
       const int cols = a.width / 2;
       const int c0 = t.n * a.width + half * cols;
-      if (t.ks != 0) {
-        if (!warp_wait(&bars->acc_full[ac.i], ac.phase, a.err, abort_flag, kSite + 9)) break;
-        tc_fence_after();
-      }
-      for (int j = 0; j < cols; j += 32) {
-        float f[32];
-        if (t.ks != 0) {
-          uint32_t u[32];
-          tmem_ld32(tmem + lane_base + ac.i * kTile + half * cols + j, u);
-          if (j + 32 == cols) {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(empty_addr + ac.i * 8);
-            ac.next();
+      const uint32_t col0 = tmem + lane_base + half * cols;
+      if constexpr (SPLIT) {
+        float f[4][32];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int i = 0; i < 32; ++i) f[j][i] = 0.0f;
+        for (int ks0 = 0; ks0 < t.ks && ok; ks0 += Passes<SPLIT>::kStep) {
+          ok = warp_wait(&bars->acc_full[ac.i], ac.phase, a.err, abort_flag, kSite + 9);
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            if (j * 16 >= cols) break;
+            uint32_t u[16];
+            tmem_ld16(col0 + ac.i * kTile + j * 16, u);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              float& x = f[j >> 1][(j & 1) * 16 + i];
+              x = __fadd_rn(x, __uint_as_float(u[i]));
+            }
           }
-#pragma unroll
-          for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(u[i]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) f[i] = 0.0f;
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(empty_addr + ac.i * 8);
+          ac.next();
         }
-        store_rows32(out, pitch, rows, c0 + j, a.K, f, a.out_dtype, a.store, stage, lane);
+        if (!ok) break;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (j * 32 < cols) store_rows32(out, pitch, rows, c0 + j * 32, a.K, f[j], a.out_dtype, a.store, stage, lane);
+      } else {
+        if (t.ks != 0) {
+          ok = warp_wait(&bars->acc_full[ac.i], ac.phase, a.err, abort_flag, kSite + 9);
+          if (!ok) break;
+          tc_fence_after();
+        }
+        for (int j = 0; j < cols; j += 32) {
+          float f[32];
+          if (t.ks != 0) {
+            uint32_t u[32];
+            tmem_ld32(col0 + ac.i * kTile + j, u);
+            if (j + 32 == cols) {
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive_cluster(empty_addr + ac.i * 8);
+              ac.next();
+            }
+#pragma unroll
+            for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(u[i]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) f[i] = 0.0f;
+          }
+          store_rows32(out, pitch, rows, c0 + j, a.K, f, a.out_dtype, a.store, stage, lane);
+        }
       }
     }
   }
@@ -350,30 +434,89 @@ int pad_rows(const void* src, int64_t rows, int cols, int pitch, void* dst, cons
   return cuda_status(cudaGetLastError());
 }
 
-template <int FORM>
+template <int FORM, bool SPLIT>
 int launch(const CUtensorMap& ta, const CUtensorMap& ta32, const CUtensorMap& tb, const GradArgs& a, int grid,
            cudaStream_t stream) {
   constexpr size_t smem = 1024 + kStages * kStageBytes + kEpiWarps * kStoreStageBytes + sizeof(Bars);
   static_assert(smem <= 232448, "shared memory budget");
-  auto fn = grad_gemm_kernel<FORM>;
+  auto fn = grad_gemm_kernel<FORM, SPLIT>;
   const int st = set_max_dynamic_smem(reinterpret_cast<const void*>(fn), smem);
   if (st != LMOE_OK) return st;
   fn<<<grid, kThreads, smem, stream>>>(ta, ta32, tb, a);
   return cuda_status(cudaGetLastError());
 }
 
+// The three planes of src [rows, cols] fp32: dst [3][rows, pitch] bf16, zero behind the columns.
+// Rounding each remainder to nearest leaves at most 2^-27 of the value; values that would round to
+// an infinity are cut instead, values that are not finite stay in the high plane.
+__global__ void __launch_bounds__(256) split_rows_kernel(const float* __restrict__ src, int64_t rows, int cols,
+                                                         int pitch, int vec, uint4* __restrict__ dst) {
+  const int per = pitch / 8;
+  const int64_t total = rows * per;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t r = i / per;
+    const int c = (int)(i - r * per) * 8;
+    const float* p = src + r * cols + c;
+    float v[8];
+    if (vec) {
+      const float4 x = __ldg(reinterpret_cast<const float4*>(p)), y = __ldg(reinterpret_cast<const float4*>(p) + 1);
+      v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w, v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = c + j < cols ? __ldg(p + j) : 0.0f;
+    }
+    uint32_t w[3][4];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      uint32_t b[3];
+      const uint32_t bits = __float_as_uint(v[j]);
+      __nv_bfloat16 h = __float2bfloat16_rn(v[j]);
+      if ((bits & 0x7f800000u) == 0x7f800000u) {
+        b[1] = b[2] = 0u;
+      } else {
+        if ((__bfloat16_as_ushort(h) & 0x7f80u) == 0x7f80u) h = __float2bfloat16_rz(v[j]);
+        const float e = __fsub_rn(v[j], __bfloat162float(h));   // exact
+        const __nv_bfloat16 m = __float2bfloat16_rn(e);
+        b[1] = __bfloat16_as_ushort(m);
+        b[2] = __bfloat16_as_ushort(__float2bfloat16_rn(__fsub_rn(e, __bfloat162float(m))));
+      }
+      b[0] = __bfloat16_as_ushort(h);
+#pragma unroll
+      for (int k = 0; k < 3; ++k) w[k][j >> 1] = (j & 1) ? w[k][j >> 1] | b[k] << 16 : b[k];
+    }
+#pragma unroll
+    for (int k = 0; k < 3; ++k) dst[k * total + i] = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
+  }
+}
+
+int split_rows(const void* src, int64_t rows, int cols, int pitch, void* dst, const DeviceInfo& dev, cudaStream_t s) {
+  const int64_t blocks = (rows * (pitch / 8) + 255) / 256, most = (int64_t)dev.num_sms * 8;
+  split_rows_kernel<<<(unsigned)(blocks < most ? blocks : most), 256, 0, s>>>(
+      static_cast<const float*>(src), rows, cols, pitch, cols % 8 == 0 && aligned16(src), static_cast<uint4*>(dst));
+  return cuda_status(cudaGetLastError());
+}
+
 inline int64_t pitch8(int64_t cols) { return (cols + 7) / 8 * 8; }
 inline size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
+inline int64_t other_rows(const GradProblem& p) {
+  return p.weight_grad ? p.total_rows : (int64_t)p.num_experts * p.N;
+}
 
 }  // namespace
 
+bool grad_splits(const GradProblem& p) {
+  if (p.dtype != LMOE_DTYPE_F32 || p.total_rows * 3 > INT32_MAX) return false;
+  return p.total_rows >= (int64_t)p.num_experts * (p.weight_grad ? kSplitRowsW : kSplitRowsX);
+}
+
 size_t grad_gemm_workspace(const GradProblem& p) {
-  if (p.dtype == LMOE_DTYPE_F32) return 0;
+  if (p.dtype == LMOE_DTYPE_F32) {
+    if (!grad_splits(p)) return 0;
+    return align256((size_t)p.total_rows * pitch8(p.N) * 6) + align256((size_t)other_rows(p) * pitch8(p.K) * 6);
+  }
   size_t b = 0;
   if (p.N % 8) b += align256((size_t)p.total_rows * pitch8(p.N) * 2);
-  if (p.K % 8)
-    b += align256(p.weight_grad ? (size_t)p.total_rows * pitch8(p.K) * 2
-                                : (size_t)p.num_experts * p.N * pitch8(p.K) * 2);
+  if (p.K % 8) b += align256((size_t)other_rows(p) * pitch8(p.K) * 2);
   return b;
 }
 
@@ -386,14 +529,24 @@ int run_grad_gemm(const GradProblem& p, cudaStream_t stream) {
   const void* other = p.other;
   const int64_t ldy = pitch8(p.N), ldo = pitch8(p.K);
   uint8_t* ws = static_cast<uint8_t*>(p.workspace);
-  if (ldy != p.N) {
+  const bool split = p.dtype == LMOE_DTYPE_F32;
+  if (split) {
+    st = split_rows(p.dy, p.total_rows, p.N, (int)ldy, ws, dev, stream);
+    if (st != LMOE_OK) return st;
+    dy = ws;
+    ws += align256((size_t)p.total_rows * ldy * 6);
+    st = split_rows(p.other, other_rows(p), p.K, (int)ldo, ws, dev, stream);
+    if (st != LMOE_OK) return st;
+    other = ws;
+  }
+  if (!split && ldy != p.N) {
     st = pad_rows(p.dy, p.total_rows, p.N, (int)ldy, ws, dev, stream);
     if (st != LMOE_OK) return st;
     dy = ws;
     ws += align256((size_t)p.total_rows * ldy * 2);
   }
-  if (ldo != p.K) {
-    st = pad_rows(p.other, p.weight_grad ? p.total_rows : (int64_t)p.num_experts * p.N, p.K, (int)ldo, ws, dev, stream);
+  if (!split && ldo != p.K) {
+    st = pad_rows(p.other, other_rows(p), p.K, (int)ldo, ws, dev, stream);
     if (st != LMOE_OK) return st;
     other = ws;
   }
@@ -419,24 +572,28 @@ int run_grad_gemm(const GradProblem& p, cudaStream_t stream) {
   const int widths[] = {256, 128};
   a.width = pick_width(widths, grid / 2, 0, 16, [&](int w) { return row_tiles * ((p.K + w - 1) / w); });
   a.raster = Raster((p.K + a.width - 1) / a.width);
-  // the maps end at the true sizes, so that TMA fills what lies behind them with zeros
+  // the maps end at the true sizes, so that TMA fills what lies behind them with zeros; the planes
+  // of split operands follow one another along the rows (or the experts)
+  const uint64_t planes = split ? 3 : 1;
   if (p.weight_grad) {
-    st = encode_tmap_2d(&ta, dy, dt, 2, (uint64_t)p.total_rows, (uint64_t)p.N, (uint64_t)ldy * 2, kSK, 64, true);
+    st = encode_tmap_2d(&ta, dy, dt, 2, planes * p.total_rows, (uint64_t)p.N, (uint64_t)ldy * 2, kSK, 64, true);
     if (st != LMOE_OK) return st;
-    st = encode_tmap_2d(&tb, other, dt, 2, (uint64_t)p.total_rows, (uint64_t)p.K, (uint64_t)ldo * 2, kSK, 64, true);
+    st = encode_tmap_2d(&tb, other, dt, 2, planes * p.total_rows, (uint64_t)p.K, (uint64_t)ldo * 2, kSK, 64, true);
     if (st != LMOE_OK) return st;
-    return launch<kWeightGrad>(ta, ta, tb, a, grid, stream);
+    return split ? launch<kWeightGrad, true>(ta, ta, tb, a, grid, stream)
+                 : launch<kWeightGrad, false>(ta, ta, tb, a, grid, stream);
   }
-  st = encode_tmap_2d(&ta, dy, dt, 2, (uint64_t)p.total_rows, (uint64_t)p.N, (uint64_t)ldy * 2, kCta, 64, true);
+  st = encode_tmap_2d(&ta, dy, dt, 2, planes * p.total_rows, (uint64_t)p.N, (uint64_t)ldy * 2, kCta, 64, true);
   if (st != LMOE_OK) return st;
-  st = encode_tmap_2d(&ta32, dy, dt, 2, (uint64_t)p.total_rows, (uint64_t)p.N, (uint64_t)ldy * 2, 32, 64, true);
+  st = encode_tmap_2d(&ta32, dy, dt, 2, planes * p.total_rows, (uint64_t)p.N, (uint64_t)ldy * 2, 32, 64, true);
   if (st != LMOE_OK) return st;
-  const uint64_t dims[3] = {(uint64_t)p.K, (uint64_t)p.N, (uint64_t)p.num_experts};
+  const uint64_t dims[3] = {(uint64_t)p.K, (uint64_t)p.N, planes * p.num_experts};
   const uint64_t strides[2] = {(uint64_t)ldo * 2, (uint64_t)ldo * 2 * (uint64_t)p.N};
   const uint32_t box[3] = {64, (uint32_t)kSK, 1};
   st = encode_tmap_3d(&tb, other, dt, 2, dims, strides, box);
   if (st != LMOE_OK) return st;
-  return launch<kInputGrad>(ta, ta32, tb, a, grid, stream);
+  return split ? launch<kInputGrad, true>(ta, ta32, tb, a, grid, stream)
+               : launch<kInputGrad, false>(ta, ta32, tb, a, grid, stream);
 }
 
 }  // namespace lmoe
@@ -459,9 +616,10 @@ int grad_entry(GradProblem& p, const void* offsets, void* out, void* workspace, 
   }
   LMOE_ARG_CHECK(p.dy && p.other && offsets);
   LMOE_ARG_CHECK(reinterpret_cast<uintptr_t>(p.dy) % esize == 0 && reinterpret_cast<uintptr_t>(p.other) % esize == 0);
-  if (p.dtype == LMOE_DTYPE_F32) return run_grad_f32(p, stream);
+  if (p.dtype == LMOE_DTYPE_F32 && (!workspace || !grad_splits(p))) return run_grad_f32(p, stream);
   // rows that TMA reads where they lie start at multiples of 16 bytes
-  LMOE_ARG_CHECK((p.N % 8 || aligned16(p.dy)) && (p.K % 8 || aligned16(p.other)));
+  LMOE_ARG_CHECK(p.dtype == LMOE_DTYPE_F32 ||
+                 ((p.N % 8 || aligned16(p.dy)) && (p.K % 8 || aligned16(p.other))));
   const size_t need = grad_gemm_workspace(p);
   if (need && (!workspace || workspace_bytes < need || !aligned16(workspace))) return LMOE_ERR_WORKSPACE;
   p.workspace = workspace;

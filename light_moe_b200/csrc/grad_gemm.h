@@ -1,5 +1,5 @@
-// grad_gemm.h -- internal interface of the grouped product's gradients (grad_gemm.cu for 16-bit
-// operands on tensor cores, grad_f32.cu for fp32 operands).
+// grad_gemm.h -- internal interface of the grouped product's gradients (grad_gemm.cu on tensor
+// cores, grad_f32.cu for fp32 operands on CUDA cores).
 #pragma once
 #include <cuda_runtime.h>
 
@@ -19,11 +19,13 @@ struct GradProblem {
   const void* offsets = nullptr;
   int offsets_i64 = 0;
   void* out = nullptr;
-  void* workspace = nullptr;     // padded copies of operands whose rows TMA cannot read
+  void* workspace = nullptr;     // copies of operands: padded rows, or planes of fp32
   uint32_t* err = nullptr;
 };
 
 size_t grad_gemm_workspace(const GradProblem& p);
+// Whether fp32 operands go to the tensor cores as three bf16 planes each.
+bool grad_splits(const GradProblem& p);
 int run_grad_gemm(const GradProblem& p, cudaStream_t stream);
 int run_grad_f32(const GradProblem& p, cudaStream_t stream);
 
