@@ -5,12 +5,13 @@
 //   weight gradient  dw[e, n, k] = sum_{r in e} dy[r, n] * x[r, k]       contraction over rows
 //
 // Neither needs a transposed copy: an operand whose contraction index is the slow one in memory
-// (w and both operands of dw) is loaded by TMA as it lies, in chunks of 64 columns x 64
+// (w and both operands of dw) is loaded by TMA as it lies, in chunks of 64 columns x 128
 // contraction rows, and read by tcgen05.mma as an M- or N-major operand.
 //
 // Tile: 256 x 256 on a CTA pair (128 rows of A and 128 columns of B per CTA), two accumulators
-// of 256 columns fill the 512 TMEM columns, six stages of 64 contraction values (32 KB per CTA);
-// 256 x 128 where the last round of tiles would leave pairs idle.
+// of 256 columns fill the 512 TMEM columns, three stages of 128 contraction values (64 KB per CTA:
+// a stage costs the issuing warp ~600 cycles beside its MMAs, so they are few and long); 256 x 128
+// where the last round of tiles would leave pairs idle. 
 // Bound by the tensor pipe for prompt-sized segments; with few rows per expert the input
 // gradient is bound by reading w and the weight gradient by writing dw (HBM).
 //
@@ -29,6 +30,10 @@
 // Warps: 0 TMA producer, whose copies complete on the leader's stage barrier; 1 MMA issuer
 // (leader CTA); 2 clears the tail of a segment's last stage (whose copies complete on a barrier
 // of its own CTA) and hands it to the leader; 4-11 epilogue, eight warps of 32 rows x 128 columns.
+// Measured and not kept: sixteen epilogue warps (dw of 12288 rows on 64 experts 128 us against
+// 123), stores of 32-row blocks by TMA from shared memory (121 us; 22.5 against 20.7 us for 1024
+// rows on 8 experts), 64 contraction values a stage (six stages: the same within 2 % for whole
+// tiles, 21 against 18.8 us for dx of 1024 rows in 128-column tiles).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -40,12 +45,13 @@ namespace lmoe {
 namespace {
 
 constexpr int kTile = 256, kCta = 128;
-constexpr int kSK = 64;            // contraction values per stage
-constexpr int kStages = 6, kAcc = 2;
+constexpr int kSK = 128;           // contraction values per stage
+constexpr int kStages = 3, kAcc = 2;
 constexpr int kEpiWarp0 = 4, kEpiWarps = 8;
 constexpr int kThreads = (kEpiWarp0 + kEpiWarps) * 32;
-constexpr uint32_t kChunk = 64 * 128;             // 64 contraction rows of 64 columns
-constexpr uint32_t kOperand = 2 * kChunk;         // 128 x 64 values of one operand
+constexpr uint32_t kChunk = kSK * 128;            // 128 contraction rows of 64 columns, or 128 rows
+                                                  // of 64 contraction values
+constexpr uint32_t kOperand = 2 * kChunk;         // 128 x 128 values of one operand
 constexpr uint32_t kStageBytes = 2 * kOperand;
 constexpr uint32_t kSite = 0x600u;
 
@@ -109,25 +115,21 @@ __device__ __forceinline__ Tile tile_at(const SegTable& t, const GradArgs& a, in
   return r;
 }
 
-// The stages of a tile: one after another into one accumulator, or (SPLIT) two at a time into an
-// accumulator of their own, once for each pair of planes, the small products first.
+// The stages of a tile: one after another into one accumulator, or (SPLIT) each into an accumulator
+// of its own, once for each pair of planes, the small products first.
 template <bool SPLIT>
 struct Passes {
-  static constexpr int kStep = 2, kPairs = 6;
+  static constexpr int kPairs = 6;
   int step;
-  __device__ __forceinline__ explicit Passes(int ks) : step(SPLIT ? kStep : (ks > 0 ? ks : 1)) {}
-  __device__ __forceinline__ int stages(int ks0, int ks) const {
-    const int n = ks - ks0 < step ? ks - ks0 : step;
-    return SPLIT ? n * kPairs : n;
-  }
-  // Stage i of n: its offset in contraction stages, and the planes (0 high, 1 middle, 2 low).
-  __device__ __forceinline__ int at(int i, int n, int& pa, int& pb) const {
+  __device__ __forceinline__ explicit Passes(int ks) : step(SPLIT ? 1 : (ks > 0 ? ks : 1)) {}
+  __device__ __forceinline__ int stages() const { return SPLIT ? kPairs : step; }
+  // Stage i of them: its offset in contraction stages, and the planes (0 high, 1 middle, 2 low).
+  __device__ __forceinline__ int at(int i, int& pa, int& pb) const {
     pa = pb = 0;
     if (!SPLIT) return i;
-    const int pair = n == 2 * kPairs ? i >> 1 : i;
-    pa = (0x001102 >> (4 * pair)) & 15;   // l, h, m, m, h, h
-    pb = (0x010120 >> (4 * pair)) & 15;   // h, l, m, h, m, h
-    return n == 2 * kPairs ? i & 1 : 0;
+    pa = (0x001102 >> (4 * i)) & 15;   // l, h, m, m, h, h
+    pb = (0x010120 >> (4 * i)) & 15;   // h, l, m, h, m, h
+    return 0;
   }
 };
 
@@ -138,8 +140,7 @@ template <int FORM, bool SPLIT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     grad_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_a32,
                      const __grid_constant__ CUtensorMap tm_b, const GradArgs a) {
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) uint8_t base[];   // whole swizzle atoms
   uint8_t* store_stage = base + kStages * kStageBytes;
   Bars* bars = reinterpret_cast<Bars*>(store_stage + kEpiWarps * kStoreStageBytes);
   volatile int* abort_flag = &bars->abort;
@@ -201,41 +202,55 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const uint32_t b_bytes = wide ? kOperand : kChunk;
       const Passes<SPLIT> ps(t.ks);
       for (int ks0 = 0; ks0 < t.ks && ok; ks0 += ps.step) {
-        const int n = ps.stages(ks0, t.ks);
+        const int n = ps.stages();
         for (int i = 0; i < n; ++i, st.next()) {
           ok = warp_wait(&bars->empty[st.i], st.phase ^ 1u, a.err, abort_flag, kSite + 2);
           if (!ok) break;
           int pa, pb;   // planes of the operands
-          const int ks = ks0 + ps.at(i, n, pa, pb);
+          const int ks = ks0 + ps.at(i, pa, pb);
           if (elect_one()) {
             uint8_t* sa = base + st.i * kStageBytes;
             uint8_t* sb = sa + kOperand;
             const uint32_t bar = full_addr + st.i * 8;
             if (FORM == kInputGrad) {
               const int y = m0 + pa * (int)a.R;
-              mbar_arrive_expect_tx_cluster(bar, (uint32_t)boxes * 4096u + b_bytes);
-              if (boxes == 4) {
-                tma_load_2d_pair(sa, &tm_a, bar, ks * kSK, y);
-              } else {
-                for (int b = 0; b < boxes; ++b) tma_load_2d_pair(sa + b * 4096, &tm_a32, bar, ks * kSK, y + b * 32);
+              const int blocks = a.N - ks * kSK > 64 ? 2 : 1;
+              mbar_arrive_expect_tx_cluster(bar, (uint32_t)(blocks * boxes) * 4096u + b_bytes);
+              for (int h = 0; h < blocks; ++h) {
+                const int x = ks * kSK + h * 64;
+                if (boxes == 4) {
+                  tma_load_2d_pair(sa + h * kChunk, &tm_a, bar, x, y);
+                } else {
+                  for (int b = 0; b < boxes; ++b)
+                    tma_load_2d_pair(sa + h * kChunk + b * 4096, &tm_a32, bar, x, y + b * 32);
+                }
               }
               tma_load_3d_pair(sb, &tm_b, bar, c0, ks * kSK, t.e + pb * a.E);
               if (wide) tma_load_3d_pair(sb + kChunk, &tm_b, bar, c0 + 64, ks * kSK, t.e + pb * a.E);
             } else {
               const int r = t.row0 + ks * kSK, ra = r + pa * (int)a.R, rb = r + pb * (int)a.R;
-              if (has_tail(t.row_end - r)) {
+              const int left = t.row_end - r;
+              const int halves = left > 64 ? 2 : 1;   // 64-row boxes that hold rows of the segment
+              const uint32_t bytes = (uint32_t)halves * (kOperand + b_bytes) / 2;
+              if (has_tail(left)) {
                 uint64_t* own = &bars->tail[st.i];
-                mbar_arrive_expect_tx(own, kOperand + b_bytes);
-                tma_load_2d(sa, &tm_a, own, m0, ra);
-                tma_load_2d(sa + kChunk, &tm_a, own, m0 + 64, ra);
-                tma_load_2d(sb, &tm_b, own, c0, rb);
-                if (wide) tma_load_2d(sb + kChunk, &tm_b, own, c0 + 64, rb);
+                mbar_arrive_expect_tx(own, bytes);
+                for (int h = 0; h < halves; ++h) {
+                  uint8_t *da = sa + h * (kChunk / 2), *db = sb + h * (kChunk / 2);
+                  tma_load_2d(da, &tm_a, own, m0, ra + h * 64);
+                  tma_load_2d(da + kChunk, &tm_a, own, m0 + 64, ra + h * 64);
+                  tma_load_2d(db, &tm_b, own, c0, rb + h * 64);
+                  if (wide) tma_load_2d(db + kChunk, &tm_b, own, c0 + 64, rb + h * 64);
+                }
               } else {
-                mbar_arrive_expect_tx_cluster(bar, kOperand + b_bytes);
-                tma_load_2d_pair(sa, &tm_a, bar, m0, ra);
-                tma_load_2d_pair(sa + kChunk, &tm_a, bar, m0 + 64, ra);
-                tma_load_2d_pair(sb, &tm_b, bar, c0, rb);
-                if (wide) tma_load_2d_pair(sb + kChunk, &tm_b, bar, c0 + 64, rb);
+                mbar_arrive_expect_tx_cluster(bar, bytes);
+                for (int h = 0; h < halves; ++h) {
+                  uint8_t *da = sa + h * (kChunk / 2), *db = sb + h * (kChunk / 2);
+                  tma_load_2d_pair(da, &tm_a, bar, m0, ra + h * 64);
+                  tma_load_2d_pair(da + kChunk, &tm_a, bar, m0 + 64, ra + h * 64);
+                  tma_load_2d_pair(db, &tm_b, bar, c0, rb + h * 64);
+                  if (wide) tma_load_2d_pair(db + kChunk, &tm_b, bar, c0 + 64, rb + h * 64);
+                }
               }
             }
           }
@@ -264,19 +279,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           ok = warp_wait(&bars->acc_empty[ac.i], ac.phase ^ 1u, a.err, abort_flag, kSite + 4);
           if (!ok) break;
           const uint32_t d = tmem + ac.i * kTile;
-          const int n = ps.stages(ks0, t.ks);
+          const int n = ps.stages();
           for (int i = 0; i < n; ++i, st.next()) {
             ok = warp_wait(&bars->full[st.i], st.phase, a.err, abort_flag, kSite + 6);
             if (!ok) break;
             tc_fence_after();
             int pa, pb;
-            const int left = depth - (ks0 + ps.at(i, n, pa, pb)) * kSK;
+            const int left = depth - (ks0 + ps.at(i, pa, pb)) * kSK;
             if (elect_one()) {
               const uint64_t ad = adesc0 + st.i * (kStageBytes >> 4), bd = bdesc0 + st.i * (kStageBytes >> 4);
 #pragma unroll
-              for (int kk = 0; kk < 4; ++kk)
-                if (kk * 16 < left)
-                  mma_ss_pair(d, ad + kk * (FORM == kInputGrad ? 2 : 128), bd + kk * 128, idesc, (i | kk) != 0 ? 1u : 0u);
+              for (int kk = 0; kk < kSK / 16; ++kk) {
+                // 16 contraction values: 32 bytes of the lines of a K-major block, or 16 lines
+                const uint32_t step = FORM == kInputGrad ? (kk >> 2) * (kChunk >> 4) + (kk & 3) * 2 : kk * 128;
+                if (kk * 16 < left) mma_ss_pair(d, ad + step, bd + kk * 128, idesc, (i | kk) != 0 ? 1u : 0u);
+              }
               mma_commit_pair(&bars->empty[st.i]);
               if (i == n - 1) mma_commit_pair(&bars->acc_full[ac.i]);
             }
@@ -300,10 +317,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const Passes<SPLIT> ps(t.ks);
         const int left = t.row_end - t.row0 - (t.ks - 1) * kSK;   // rows of the last stage
         for (int ks0 = 0; ks0 < t.ks && ok; ks0 += ps.step) {
-          const int n = ps.stages(ks0, t.ks);
+          const int n = ps.stages();
           for (int i = 0; i < n && ok; ++i, st.next()) {
             int pa, pb;
-            if (ks0 + ps.at(i, n, pa, pb) != t.ks - 1 || !has_tail(left)) continue;
+            if (ks0 + ps.at(i, pa, pb) != t.ks - 1 || !has_tail(left)) continue;
             ok = warp_wait(&bars->tail[st.i], tail_parity >> st.i & 1u, a.err, abort_flag, kSite + 8);
             if (!ok) break;
             tail_parity ^= 1u << st.i;
@@ -327,7 +344,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const int q = warp & 3, half = (warp - kEpiWarp0) >> 2;
     const uint32_t lane_base = (uint32_t)(q * 32) << 16;
     const uint32_t empty_addr = mapa_u32(&bars->acc_empty[0], 0);
-    const int64_t pitch = (int64_t)a.K * (a.out_dtype == LMOE_DTYPE_F32 ? 4 : 2);
+    const int odt = SPLIT ? LMOE_DTYPE_F32 : a.out_dtype;   // planes come from fp32
+    const int64_t pitch = (int64_t)a.K * (odt == LMOE_DTYPE_F32 ? 4 : 2);
     uint8_t* stage = store_stage + (warp - kEpiWarp0) * kStoreStageBytes;
     Ring<kAcc> ac;
     int hint = 0;
@@ -349,7 +367,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         for (int j = 0; j < 4; ++j)
 #pragma unroll
           for (int i = 0; i < 32; ++i) f[j][i] = 0.0f;
-        for (int ks0 = 0; ks0 < t.ks && ok; ks0 += Passes<SPLIT>::kStep) {
+        for (int ks0 = 0; ks0 < t.ks && ok; ++ks0) {
           ok = warp_wait(&bars->acc_full[ac.i], ac.phase, a.err, abort_flag, kSite + 9);
           if (!ok) break;
           tc_fence_after();
@@ -372,7 +390,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         if (!ok) break;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (j * 32 < cols) store_rows32(out, pitch, rows, c0 + j * 32, a.K, f[j], a.out_dtype, a.store, stage, lane);
+          if (j * 32 < cols) store_rows32(out, pitch, rows, c0 + j * 32, a.K, f[j], odt, a.store, stage, lane);
       } else {
         if (t.ks != 0) {
           ok = warp_wait(&bars->acc_full[ac.i], ac.phase, a.err, abort_flag, kSite + 9);
@@ -396,7 +414,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int i = 0; i < 32; ++i) f[i] = 0.0f;
           }
-          store_rows32(out, pitch, rows, c0 + j, a.K, f, a.out_dtype, a.store, stage, lane);
+          store_rows32(out, pitch, rows, c0 + j, a.K, f, odt, a.store, stage, lane);
         }
       }
     }
@@ -437,7 +455,7 @@ int pad_rows(const void* src, int64_t rows, int cols, int pitch, void* dst, cons
 template <int FORM, bool SPLIT>
 int launch(const CUtensorMap& ta, const CUtensorMap& ta32, const CUtensorMap& tb, const GradArgs& a, int grid,
            cudaStream_t stream) {
-  constexpr size_t smem = 1024 + kStages * kStageBytes + kEpiWarps * kStoreStageBytes + sizeof(Bars);
+  constexpr size_t smem = kStages * kStageBytes + kEpiWarps * kStoreStageBytes + sizeof(Bars);
   static_assert(smem <= 232448, "shared memory budget");
   auto fn = grad_gemm_kernel<FORM, SPLIT>;
   const int st = set_max_dynamic_smem(reinterpret_cast<const void*>(fn), smem);
@@ -576,9 +594,9 @@ int run_grad_gemm(const GradProblem& p, cudaStream_t stream) {
   // of split operands follow one another along the rows (or the experts)
   const uint64_t planes = split ? 3 : 1;
   if (p.weight_grad) {
-    st = encode_tmap_2d(&ta, dy, dt, 2, planes * p.total_rows, (uint64_t)p.N, (uint64_t)ldy * 2, kSK, 64, true);
+    st = encode_tmap_2d(&ta, dy, dt, 2, planes * p.total_rows, (uint64_t)p.N, (uint64_t)ldy * 2, 64, 64, true);
     if (st != LMOE_OK) return st;
-    st = encode_tmap_2d(&tb, other, dt, 2, planes * p.total_rows, (uint64_t)p.K, (uint64_t)ldo * 2, kSK, 64, true);
+    st = encode_tmap_2d(&tb, other, dt, 2, planes * p.total_rows, (uint64_t)p.K, (uint64_t)ldo * 2, 64, 64, true);
     if (st != LMOE_OK) return st;
     return split ? launch<kWeightGrad, true>(ta, ta, tb, a, grid, stream)
                  : launch<kWeightGrad, false>(ta, ta, tb, a, grid, stream);
