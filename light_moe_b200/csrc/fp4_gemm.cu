@@ -36,20 +36,16 @@
 // reads them beside its own rows); 7-18 epilogue, twelve warps of 32 rows x 64 columns.
 #include <cuda_bf16.h>
 
-#include "fp4_format.cuh"
-#include "fp4_gemm.h"
+#include "fp4_mma.cuh"
 #include "host_util.h"
-#include "pair_gemm.cuh"
 
 namespace lmoe {
 namespace {
 
 constexpr int kRowsCta = 128, kTM = 256, kTN = 192, kHalf = 96;
-constexpr int kBK = 256;          // values of a 128-byte swizzle line of codes
-constexpr int kSK = 512;          // values per stage
+constexpr int kBK = kFp4Block, kSK = kFp4Stage;
 constexpr int kStages = 3, kAcc = 2;
 constexpr int kSfSlots = 3;       // steps of scales in shared memory
-constexpr int kSfAhead = 3;       // steps of scales in registers
 constexpr int kUnits = 2;         // units of scales in TMEM
 constexpr uint32_t kUnitCols = 48;   // 4 words x (4 columns of the rows' scales, 8 of the columns')
 constexpr int kSfWarp0 = 2, kSfWarps = 5, kEpiWarp0 = 7, kEpiWarps = 12;
@@ -58,27 +54,6 @@ constexpr uint32_t kABlock = kRowsCta * 128, kBBlock = kHalf * 128;
 constexpr uint32_t kABytes = 2 * kABlock, kBBytes = 2 * kBBlock;
 constexpr uint32_t kSite = 0x500u;
 constexpr int kTmemCols = 512;
-
-struct Fp4Args {
-  const uint8_t* xs;     // scales of the rows
-  int64_t xs_pitch;
-  const uint8_t* ws;     // scales of the weights (gate), and of up
-  const uint8_t* ws_up;
-  int64_t ws_pitch;
-  const void* offsets;
-  int offsets_i64;
-  int E, N, K;
-  int64_t R;
-  Raster raster;         // of the column tiles
-  int KS;                // stages
-  int width, half;       // columns of a tile, of one CTA's half
-  const float* alpha;    // per expert, or NULL
-  const float* alpha_up;
-  void* out;
-  int out_dtype;
-  int store;             // StoreMode
-  uint32_t* err;
-};
 
 struct __align__(8) Bars {
   uint64_t full[kStages];       // leader: both CTAs' codes landed (one arrival each)
@@ -94,66 +69,6 @@ struct __align__(8) Bars {
   SegTable seg;
 };
 
-struct Tile {
-  int e, m, n, row0, row_end;
-  bool zero;   // rows outside every expert
-};
-
-__device__ __forceinline__ Tile tile_at(const SegTable& t, int E, const Raster& ra, int tile, int& hint) {
-  int j = hint;
-  while (tile >= t.tile_start[j + 1]) ++j;
-  hint = j;
-  Tile r;
-  const int rows = t.row[j + 1] - t.row[j];
-  ra.at(tile - t.tile_start[j], (rows + kTM - 1) / kTM, r.m, r.n);
-  r.e = j - 1;
-  r.zero = j == 0 || j == E + 1;
-  r.row0 = t.row[j] + r.m * kTM;
-  r.row_end = t.row[j + 1];
-  return r;
-}
-
-// Instruction descriptor of the block-scaled kinds: E2M1 operands, K-major, M = 256, N = width.
-__host__ __device__ constexpr uint32_t idesc_fp4(bool ue8m0, uint32_t sf_id, uint32_t width) {
-  return (sf_id << 4) | (1u << 7) | (1u << 10) | ((width >> 3) << 17) | ((ue8m0 ? 1u : 0u) << 23) |
-         ((uint32_t)(kTM >> 4) << 24) | (sf_id << 29);
-}
-
-// Unswizzled descriptor of a 512-byte scale tile (32 rows of 16 bytes).
-__device__ __forceinline__ uint64_t sdesc_scales(uint32_t smem_addr) {
-  return (uint64_t)((smem_addr >> 4) & 0x3fffu) | ((uint64_t)(128u >> 4) << 32) | ((uint64_t)1u << 46);
-}
-
-__device__ __forceinline__ void copy_scales_pair(uint32_t taddr, uint64_t desc) {
-  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
-}
-
-template <int FORMAT>
-__device__ __forceinline__ void mma_fp4_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa,
-                                             uint32_t sfb, uint32_t accumulate) {
-  if constexpr (FORMAT == LMOE_FP4_MX)
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
-        : "memory");
-  else
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(
-            d),
-        "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
-        : "memory");
-}
-
-template <int FORMAT>
-struct Cfg {
-  static constexpr int kUnitK = FORMAT == LMOE_FP4_MX ? 512 : 256;   // values of a unit (4 words)
-  static constexpr int kStageUnits = kSK / kUnitK;
-  static constexpr int kStepK = 2 * kUnitK;                          // values of a step (8 words)
-};
 static_assert(kAcc * kTN + kUnits * kUnitCols <= kTmemCols, "tensor memory budget");
 constexpr uint32_t kStageBytes = kABytes + kBBytes;
 constexpr uint32_t kSfABytes = 8 * 512, kSfBBytes = 8 * 1024, kSfSlotBytes = kSfABytes + kSfBBytes;
@@ -162,14 +77,12 @@ constexpr uint32_t kSmem =
 static_assert(kStageBytes % 1024 == 0, "swizzle atoms");
 static_assert(kSmem <= 232448, "shared memory budget");
 
-__device__ __forceinline__ float silu(float g) { return __fdividef(g, 1.0f + __expf(-g)); }
-
 template <int FORMAT, bool SWIGLU>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     fp4_gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_x32,
                     const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_up,
                     const Fp4Args a) {
-  using C = Cfg<FORMAT>;
+  using C = Fp4Units<FORMAT>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sf_base = base + kStages * kStageBytes;
@@ -227,7 +140,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     int hint = 0;
     bool ok = true;
     for (int tile = first; tile < total && ok; tile += stride) {
-      const Tile t = tile_at(seg, a.E, a.raster, tile, hint);
+      const Fp4Tile t = fp4_tile_at<kTM>(seg, a, tile, hint);
       if (t.zero) continue;
       const int r0 = t.row0 + (int)rank * kRowsCta;
       int rows = t.row_end - r0;
@@ -269,7 +182,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       int hint = 0;
       bool ok = true;
       for (int tile = first; tile < total && ok; tile += stride) {
-        const Tile t = tile_at(seg, a.E, a.raster, tile, hint);
+        const Fp4Tile t = fp4_tile_at<kTM>(seg, a, tile, hint);
         if (t.zero) continue;
         ok = warp_wait(&bars->acc_empty[ac.i], ac.phase ^ 1u, a.err, abort_flag, kSite + 4);
         const uint32_t d = tmem + ac.i * kTN;
@@ -342,93 +255,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   } else if (warp < kEpiWarp0) {
     // ------------------------------------------------------------------ scales
     const int part = warp - kSfWarp0;   // 0, 1: rows 0-63, 64-127; 2, 3, 4: columns 0-63, 64-127, 128-191
-    const int nb = a.K / fp4_block(FORMAT);
-    // rows lane, lane + 32 of the 64 are words 0, 1 or 2, 3 of the lane's 16 bytes in a tile
-    uint8_t* dst = sf_base + lane * 16 +
-                   (part < 2 ? part * 8u : kSfABytes + (part == 4 ? 512u : (uint32_t)(part - 2) * 8u));
-    const uint32_t dst_word = part < 2 ? 512u : 1024u;
-    const int steps = (a.K + C::kStepK - 1) / C::kStepK;   // 32-byte loads a row
-    const uint32_t full_addr = mapa_u32(&bars->sf_full[0], 0);
-    int hint = 0, ltile = first, lstep = 0;   // the next load: tile and step
-    const uint8_t* lp[2];                     // the lane's two rows of that tile, NULL where there is none
-    auto next_tile = [&]() {   // first tile at or behind ltile that has an expert
-      for (; ltile < total; ltile += stride) {
-        const Tile t = tile_at(seg, a.E, a.raster, ltile, hint);
-        if (t.zero) continue;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          lp[i] = nullptr;
-          if (part < 2) {
-            const int row = t.row0 + (int)rank * kRowsCta + part * 64 + lane + 32 * i;
-            if (row < t.row_end) lp[i] = a.xs + (int64_t)row * a.xs_pitch;
-          } else {
-            const int c = (part - 2) * 64 + lane + 32 * i;
-            const bool up = SWIGLU && c >= a.half;
-            const int n = SWIGLU ? t.n * a.half + (up ? c - a.half : c) : t.n * a.width + c;
-            if (c < a.width && n < a.N) lp[i] = (up ? a.ws_up : a.ws) + ((int64_t)t.e * a.N + n) * a.ws_pitch;
-          }
-        }
-        return;
-      }
-    };
-    uint4 v[kSfAhead][2][2];
-    int pending = 0;
-    auto load = [&](uint4 (&b)[2][2]) {
-      if (ltile >= total) return;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-          b[i][h] = lp[i] ? __ldg(reinterpret_cast<const uint4*>(lp[i] + lstep * 32) + h) : make_uint4(0, 0, 0, 0);
-      }
-      ++pending;
-      if (++lstep == steps) {
-        lstep = 0;
-        ltile += stride;
-        next_tile();
-      }
-    };
-    next_tile();
-#pragma unroll
-    for (int j = 0; j < kSfAhead; ++j) load(v[j]);
-    Ring<kSfSlots> sl;
-    int step = 0;
-    bool ok = true;
-    while (ok && pending > 0) {
-#pragma unroll
-      for (int j = 0; j < kSfAhead; ++j) {
-        if (!ok || pending == 0) break;
-        --pending;
-        if ((step + 1) * 32 > nb) {
-          // scale bytes behind the last block are padding: zero, whatever they hold
+    int hint = 0;
+    write_scales<FORMAT, kSfSlots>(
+        first, total, stride, a.K,
+        sf_base + lane * 16 + (part < 2 ? part * 8u : kSfABytes + (part == 4 ? 512u : (uint32_t)(part - 2) * 8u)),
+        part < 2 ? 512u : 1024u, kSfSlotBytes, bars->sf_empty, mapa_u32(&bars->sf_full[0], 0), a.err, abort_flag,
+        kSite + 8, lane, [&](int tile, const uint8_t* (&p)[2]) {
+          const Fp4Tile t = fp4_tile_at<kTM>(seg, a, tile, hint);
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            uint32_t* w = reinterpret_cast<uint32_t*>(&v[j][i][0]);
-#pragma unroll
-            for (int q = 0; q < 8; ++q) {
-              const int valid = nb - (step * 32 + q * 4);
-              if (valid < 4) w[q] = valid <= 0 ? 0u : (w[q] & ((1u << (8 * valid)) - 1u));
+            p[i] = nullptr;
+            if (part < 2) {
+              const int row = t.row0 + (int)rank * kRowsCta + part * 64 + lane + 32 * i;
+              if (row < t.row_end) p[i] = a.xs + (int64_t)row * a.xs_pitch;
+            } else if (!t.zero) {
+              const int c = (part - 2) * 64 + lane + 32 * i;
+              const bool up = SWIGLU && c >= a.half;
+              const int n = SWIGLU ? t.n * a.half + (up ? c - a.half : c) : t.n * a.width + c;
+              if (c < a.width && n < a.N) p[i] = (up ? a.ws_up : a.ws) + ((int64_t)t.e * a.N + n) * a.ws_pitch;
             }
           }
-        }
-        step = step + 1 == steps ? 0 : step + 1;
-        ok = warp_wait(&bars->sf_empty[sl.i], sl.phase ^ 1u, a.err, abort_flag, kSite + 8);
-        if (!ok) break;
-#pragma unroll
-        for (int q = 0; q < 8; ++q) {
-          const uint4 x = v[j][0][q >> 2], y = v[j][1][q >> 2];
-          const uint2 o = (q & 3) == 0 ? make_uint2(x.x, y.x)
-                                       : (q & 3) == 1 ? make_uint2(x.y, y.y)
-                                                      : (q & 3) == 2 ? make_uint2(x.z, y.z) : make_uint2(x.w, y.w);
-          *reinterpret_cast<uint2*>(dst + sl.i * kSfSlotBytes + q * dst_word) = o;
-        }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(full_addr + sl.i * 8);
-        sl.next();
-        load(v[j]);
-      }
-    }
+          return !t.zero;
+        });
   } else {
     // ------------------------------------------------------------------ epilogue
     const int q = warp & 3, cg = (warp - kEpiWarp0) >> 2;
@@ -439,7 +287,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     Ring<kAcc> ac;
     int hint = 0;
     for (int tile = first; tile < total; tile += stride) {
-      const Tile t = tile_at(seg, a.E, a.raster, tile, hint);
+      const Fp4Tile t = fp4_tile_at<kTM>(seg, a, tile, hint);
       const int row = t.row0 + (int)rank * kRowsCta + q * 32;   // the warp's first
       const int rows = t.row_end - row < 32 ? t.row_end - row : 32;
       uint8_t* out = static_cast<uint8_t*>(a.out) + (int64_t)row * pitch;
@@ -600,5 +448,5 @@ extern "C" int lmoe_fp4_grouped_gemm(const uint8_t* xq, const uint8_t* xs, int64
   p.out_dtype = out_dtype;
   p.out = output;
   p.err = error;
-  return run_fp4_gemm(p, stream);
+  return total_rows <= (int64_t)num_experts * kFp4DecodeRows ? run_fp4_decode(p, stream) : run_fp4_gemm(p, stream);
 }

@@ -1,4 +1,5 @@
-// fp4_gemm.h -- internal interface of the grouped product of 4-bit operands (fp4_gemm.cu).
+// fp4_gemm.h -- internal interface of the grouped product of 4-bit operands (fp4_gemm.cu,
+// fp4_decode.cu).
 #pragma once
 #include <cuda_runtime.h>
 
@@ -32,6 +33,8 @@ struct Fp4Problem {
   uint32_t* err = nullptr;
 };
 
-int run_fp4_gemm(const Fp4Problem& p, cudaStream_t stream);
+int run_fp4_gemm(const Fp4Problem& p, cudaStream_t stream);     // many rows per expert
+int run_fp4_decode(const Fp4Problem& p, cudaStream_t stream);   // few
+constexpr int kFp4DecodeRows = 64;   // rows of a tile of run_fp4_decode
 
 }  // namespace lmoe
