@@ -3,7 +3,8 @@
 // The same product as fp4_gemm.cu with the operands' roles exchanged: the MMA's M runs over 256
 // weight rows of a CTA pair (128 per CTA) and N over up to 64 rows of the batch, so a stage holds
 // weights, not padding of the batch to 256 rows, and an MMA takes 32 cycles.  Bound by reading the
-// weights (HBM): three stages of 32 KB of codes per SM are in flight.
+// weights (HBM): three stages of 32 KB of codes per SM are in flight (8 experts of 2 x 14336 x 4096,
+// a row each: 79 us for 499 MB, 97 % of the measured copy rate).
 //
 // A CTA's 128 TMEM lanes are 128 features, or (gate / up) 64 gate rows and the same 64 rows of up:
 // the up lanes hand their values to the gate lanes through shared memory, and a warp stores 32
@@ -21,14 +22,14 @@ namespace lmoe {
 namespace {
 
 constexpr int kRows = kFp4DecodeRows;      // rows of the batch in a tile
-constexpr int kStages = 4, kAcc = 2, kSfSlots = 4, kUnits = 4;
+constexpr int kStages = 4, kAcc = 2, kSfSlots = 3, kUnits = 4;
 constexpr uint32_t kUnitCols = 32;         // 4 words x (4 columns of the weights' scales, 4 of the rows')
 constexpr int kSfWarp0 = 2, kSfWarps = 3, kEpiWarp0 = 5, kEpiWarps = 4;
 constexpr int kThreads = (kEpiWarp0 + kEpiWarps) * 32;
 constexpr uint32_t kABlock = 128 * 128, kBBlock = (kRows / 2) * 128;
 constexpr uint32_t kABytes = 2 * kABlock, kBBytes = 2 * kBBlock, kStageBytes = kABytes + kBBytes;
 constexpr uint32_t kSfABytes = 8 * 512, kSfSlotBytes = 2 * kSfABytes;
-constexpr uint32_t kXchgBytes = 64 * (kRows + 1) * 4;
+constexpr uint32_t kXchgBytes = 2 * 64 * (kRows + 1) * 4;
 constexpr uint32_t kSite = 0x800u;
 constexpr int kTmemCols = 256;
 static_assert(kAcc * kRows + kUnits * kUnitCols <= kTmemCols, "tensor memory budget");
@@ -252,6 +253,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const uint32_t empty_addr = mapa_u32(&bars->acc_empty[0], 0);
     const bool up = SWIGLU && q >= 2;
     const int l = SWIGLU ? (q & 1) * 32 + lane : q * 32 + lane;   // feature within the CTA's tile
+    uint32_t turn = 0;
     Ring<kAcc> ac;
     int hint = 0;
     bool ok = true;
@@ -278,12 +280,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int i = 0; i < 32; ++i) u[i] = v[i] = 0u;
       }
+      // eight rows of the batch at a time, as many as the tile has; two exchange buffers in turn, so
+      // that one barrier a tile orders writes, reads and the writes of the tile after next
+      float* xb = xchg + (turn & 1u) * (64 * (kRows + 1)) + l * (kRows + 1);
+      ++turn;
       if (SWIGLU) {
         if (up) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            xchg[l * (kRows + 1) + i] = __fmul_rn(__uint_as_float(u[i]), al);
-            xchg[l * (kRows + 1) + 32 + i] = __fmul_rn(__uint_as_float(v[i]), al);
+          for (int i0 = 0; i0 < kRows; i0 += 8) {
+            if (i0 < rows) {
+#pragma unroll
+              for (int i = i0; i < i0 + 8; ++i) xb[i] = __fmul_rn(__uint_as_float(i < 32 ? u[i & 31] : v[i & 31]), al);
+            }
           }
         }
         named_bar_sync(2, kEpiWarps * 32);
@@ -291,15 +299,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       if (!up && f < a.N) {
         const int64_t at = (int64_t)t.row0 * a.N + f;
 #pragma unroll
-        for (int i = 0; i < 64; ++i) {
-          if (i < rows) {
-            float x = __fmul_rn(__uint_as_float(i < 32 ? u[i & 31] : v[i & 31]), al);
-            if (SWIGLU) x = silu(x) * xchg[l * (kRows + 1) + i];
-            store_value(a.out, at + (int64_t)i * a.N, x, a.out_dtype);
+        for (int i0 = 0; i0 < kRows; i0 += 8) {
+          if (i0 < rows) {
+#pragma unroll
+            for (int i = i0; i < i0 + 8; ++i) {
+              float x = __fmul_rn(__uint_as_float(i < 32 ? u[i & 31] : v[i & 31]), al);
+              if (SWIGLU) x = silu(x) * xb[i];
+              if (i < rows) store_value(a.out, at + (int64_t)i * a.N, x, a.out_dtype);
+            }
           }
         }
       }
-      if (SWIGLU) named_bar_sync(2, kEpiWarps * 32);   // the values are read before the next tile's
     }
   }
 

@@ -8,8 +8,9 @@
 // times the bf16 rate for a quarter of the bytes.  With few rows the weights' bytes bound it
 // (HBM), with many the tensor pipe.
 //
-// Tile: 256 rows (128 per CTA, TMEM lane = row) x 192 weight rows (96 per CTA in shared memory),
-// or fewer where the last round of tiles would leave pairs idle.
+// Tile: 256 rows (128 per CTA, TMEM lane = row) x 192 weight rows (96 per CTA in shared memory).
+// (Narrower tiles for a fuller last round measured slower from 64 rows per expert on: 119 against
+// 112 us for 8 experts of 2 x 14336 x 4096, 50 against 41 us for 64 of 2048 x 1408.)
 // 192 columns because two accumulators (2 x 192) and two buffers of scales (2 x 48 columns) fit
 // the 512 TMEM columns, so the epilogue of a tile overlaps the next tile's MMAs; 256 columns
 // would leave room for one accumulator only.  The lane being the row, a thread holds a row's
@@ -146,7 +147,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       int rows = t.row_end - r0;
       rows = rows < 0 ? 0 : (rows > kRowsCta ? kRowsCta : rows);
       const int boxes = (rows + 31) >> 5;   // only the boxes that hold this tile's rows
-      const int wrow = SWIGLU ? t.n * a.half : t.n * a.width + (int)rank * a.half;
+      const int wrow = SWIGLU ? t.n * kHalf : t.n * kTN + (int)rank * kHalf;
       for (int ks = 0; ks < KS; ++ks, st.next()) {
         ok = warp_wait(&bars->empty[st.i], st.phase ^ 1u, a.err, abort_flag, kSite + 2);
         if (!ok) break;
@@ -154,7 +155,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           uint8_t* dst = base + st.i * kStageBytes;
           const uint32_t bar = full_addr + st.i * 8;
           const int blocks = a.K - ks * kSK > kBK ? 2 : 1;
-          mbar_arrive_expect_tx_cluster(bar, (uint32_t)blocks * ((uint32_t)boxes * 4096u + (uint32_t)a.half * 128u));
+          mbar_arrive_expect_tx_cluster(bar, (uint32_t)blocks * ((uint32_t)boxes * 4096u + kBBlock));
           for (int h = 0; h < blocks; ++h) {
             const int x = ks * (kSK / 2) + h * 128;
             if (boxes == 4) {
@@ -228,10 +229,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                   const uint64_t bm = bd + (kk >> 2) * (kBBlock >> 4) + (kk & 3) * 2;
                   if (FORMAT == LMOE_FP4_MX)
                     // a word holds the scales of 128 values: of two MMAs (scale id 0 and 2)
-                    mma_fp4_pair<FORMAT>(d, am, bm, idesc_fp4(true, (m & 1) * 2, a.width), sfa + (m >> 1) * 4,
+                    mma_fp4_pair<FORMAT>(d, am, bm, idesc_fp4(true, (m & 1) * 2, kTN), sfa + (m >> 1) * 4,
                                          sfb + (m >> 1) * 8, accum | (uint32_t)(m > 0));
                   else
-                    mma_fp4_pair<FORMAT>(d, am, bm, idesc_fp4(false, 0, a.width), sfa + m * 4, sfb + m * 8,
+                    mma_fp4_pair<FORMAT>(d, am, bm, idesc_fp4(false, 0, kTN), sfa + m * 4, sfb + m * 8,
                                          accum | (uint32_t)(m > 0));
                 }
               }
@@ -270,9 +271,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
               if (row < t.row_end) p[i] = a.xs + (int64_t)row * a.xs_pitch;
             } else if (!t.zero) {
               const int c = (part - 2) * 64 + lane + 32 * i;
-              const bool up = SWIGLU && c >= a.half;
-              const int n = SWIGLU ? t.n * a.half + (up ? c - a.half : c) : t.n * a.width + c;
-              if (c < a.width && n < a.N) p[i] = (up ? a.ws_up : a.ws) + ((int64_t)t.e * a.N + n) * a.ws_pitch;
+              const bool up = SWIGLU && c >= kHalf;
+              const int n = SWIGLU ? t.n * kHalf + (up ? c - kHalf : c) : t.n * kTN + c;
+              if (c < kTN && n < a.N) p[i] = (up ? a.ws_up : a.ws) + ((int64_t)t.e * a.N + n) * a.ws_pitch;
             }
           }
           return !t.zero;
@@ -292,7 +293,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const int rows = t.row_end - row < 32 ? t.row_end - row : 32;
       uint8_t* out = static_cast<uint8_t*>(a.out) + (int64_t)row * pitch;
       // output columns of the tile, and the warp's first
-      const int tile_cols = SWIGLU ? a.half : a.width;
+      const int tile_cols = SWIGLU ? kHalf : kTN;
       const int end = (t.n + 1) * tile_cols < a.N ? (t.n + 1) * tile_cols : a.N;
       const int c0 = t.n * tile_cols + cg * (SWIGLU ? 32 : 64);
       uint32_t u[32], v[32];
@@ -301,7 +302,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         if (!warp_wait(&bars->acc_full[ac.i], ac.phase, a.err, abort_flag, kSite + 10)) break;
         tc_fence_after();
         const uint32_t col = tmem + lane_base + ac.i * kTN + cg * (SWIGLU ? 32 : 64);
-        tmem_ld32x2(col, col + (SWIGLU ? a.half : 32), u, v);   // inside the accumulators' columns
+        tmem_ld32x2(col, col + (SWIGLU ? kHalf : 32), u, v);   // inside the accumulators' columns
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(empty_addr + ac.i * 8);
@@ -367,13 +368,7 @@ int run_fp4_gemm(const Fp4Problem& p, cudaStream_t stream) {
   a.K = p.K;
   a.R = p.total_rows;
   const int grid = gemm_grid(dev) < 2 ? 2 : gemm_grid(dev) & ~1;   // whole pairs
-  // 160 columns instead of 192: 33.0 instead of 35.1 us for 2 rows x [2 x 14336, 4096]
-  const int64_t row_tiles = even_row_tiles(p.total_rows, p.num_experts, kTM);
-  const int widths[] = {192, 160, 128, 96};
-  auto col_tiles = [&](int w) { return swiglu ? (p.N + w / 2 - 1) / (w / 2) : (p.N + w - 1) / w; };
-  a.width = pick_width(widths, grid / 2, 112, 16, [&](int w) { return row_tiles * col_tiles(w); });
-  a.half = a.width / 2;
-  a.raster = Raster(col_tiles(a.width));
+  a.raster = Raster(swiglu ? (p.N + kHalf - 1) / kHalf : (p.N + kTN - 1) / kTN);
   a.KS = (p.K + kSK - 1) / kSK;
   a.alpha = p.alpha;
   a.alpha_up = p.alpha_up;
@@ -389,7 +384,7 @@ int run_fp4_gemm(const Fp4Problem& p, cudaStream_t stream) {
   if (st != LMOE_OK) return st;
   const uint64_t dims[3] = {kb, (uint64_t)p.N, (uint64_t)p.num_experts};
   const uint64_t strides[2] = {kb, kb * (uint64_t)p.N};
-  const uint32_t box[3] = {128, (uint32_t)a.half, 1};
+  const uint32_t box[3] = {128, (uint32_t)kHalf, 1};
   st = encode_tmap_3d(&tw, p.wq, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, dims, strides, box);
   if (st != LMOE_OK) return st;
   tu = tw;
@@ -448,5 +443,11 @@ extern "C" int lmoe_fp4_grouped_gemm(const uint8_t* xq, const uint8_t* xs, int64
   p.out_dtype = out_dtype;
   p.out = output;
   p.err = error;
-  return total_rows <= (int64_t)num_experts * kFp4DecodeRows ? run_fp4_decode(p, stream) : run_fp4_gemm(p, stream);
+  // Few rows: the weights' bytes bound, and tiles of 256 weight rows stream them best (8 experts of
+  // 4096 x 14336, rows per expert: 1 50 against 72 us, 64 63 against 77, 96 76 against 81; 64 of 2048
+  // x 1408: 25 against 37, 40 against 44, 54 against 48).  The SwiGLU's exchange between lanes makes
+  // up less (8 of 2 x 14336 x 4096: 1 79 against 103 us, 48 94 against 110, 64 120 against 111; 64 of
+  // 2 x 1408 x 2048: 38 against 50, 16 44 against 52, 32 55 against 53).
+  const int64_t few = (int64_t)num_experts * (wq_up ? kFp4DecodeRows / 2 : kFp4DecodeRows);
+  return total_rows <= few ? run_fp4_decode(p, stream) : run_fp4_gemm(p, stream);
 }

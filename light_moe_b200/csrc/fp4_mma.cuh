@@ -20,7 +20,6 @@ struct Fp4Args {
   int64_t R;
   Raster raster;         // of the feature tiles
   int KS;                // stages
-  int width, half;       // features of a tile, of one CTA's half (fp4_gemm.cu)
   const float* alpha;    // per expert, or NULL
   const float* alpha_up;
   void* out;
@@ -59,9 +58,9 @@ struct Fp4Units {
   static constexpr int kStepK = 2 * kUnitK;
 };
 
-// Instruction descriptor of the block-scaled kinds: E2M1 operands, K-major, M = 256, N = width.
-__host__ __device__ constexpr uint32_t idesc_fp4(bool ue8m0, uint32_t sf_id, uint32_t width) {
-  return (sf_id << 4) | (1u << 7) | (1u << 10) | ((width >> 3) << 17) | ((ue8m0 ? 1u : 0u) << 23) |
+// Instruction descriptor of the block-scaled kinds: E2M1 operands, K-major, M = 256, N = n.
+__host__ __device__ constexpr uint32_t idesc_fp4(bool ue8m0, uint32_t sf_id, uint32_t n) {
+  return (sf_id << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | ((ue8m0 ? 1u : 0u) << 23) |
          ((256u >> 4) << 24) | (sf_id << 29);
 }
 
