@@ -250,8 +250,8 @@ int lmoe_w4a16_grouped_gemm(const void* input, int64_t total_rows, int K, const 
  * [0, total_rows] set it, and every row then counts as outside every expert.
  * The reference's backward is autograd through one mm_out per expert (csrc/grouped_gemm.cu:30-40,
  * python/light_moe/ops/grouped_gemm.py:65-106). */
-size_t lmoe_grouped_gemm_grad_workspace_bytes(int weight_grad, int dtype, int64_t total_rows, int N, int K,
-                                              int num_experts);
+/* form: 0 dgrad, 1 wgrad, 2 lmoe_grouped_gemm_any. */
+size_t lmoe_grouped_gemm_grad_workspace_bytes(int form, int dtype, int64_t total_rows, int N, int K, int num_experts);
 int lmoe_grouped_gemm_dgrad(const void* grad_output, int dtype, int64_t total_rows, int N, const void* weights, int K,
                             const void* expert_offsets, int offsets_are_int64, int num_experts, void* grad_input,
                             void* workspace, size_t workspace_bytes, uint32_t* error, lmoe_stream_t stream);
@@ -259,6 +259,12 @@ int lmoe_grouped_gemm_wgrad(const void* grad_output, int dtype, int64_t total_ro
                             const void* expert_offsets, int offsets_are_int64, int num_experts, int out_dtype,
                             void* grad_weights, void* workspace, size_t workspace_bytes, uint32_t* error,
                             lmoe_stream_t stream);
+
+/* lmoe_grouped_gemm for any N, K >= 1 (that entry wants K a multiple of 64 or 4): output
+ * [total_rows, N], zero outside every expert; workspace and error as for the gradients. */
+int lmoe_grouped_gemm_any(const void* input, int dtype, int64_t total_rows, int K, const void* weights, int N,
+                          const void* expert_offsets, int offsets_are_int64, int num_experts, void* output,
+                          void* workspace, size_t workspace_bytes, uint32_t* error, lmoe_stream_t stream);
 
 /* ------------------------------------------------------------------------------------ */
 /* Microscaled 4-bit floating point.  A row of K values (K % 32 == 0) is K/2 bytes of E2M1   */

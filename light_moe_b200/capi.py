@@ -72,6 +72,7 @@ SIGNATURES = {
     "lmoe_grouped_gemm_grad_workspace_bytes": (_SZ, [_I, _I, _I64, _I, _I, _I]),
     "lmoe_grouped_gemm_dgrad": (_I, [_P, _I, _I64, _I, _P, _I, _P, _I, _I, _P, _P, _SZ, _P, _P]),
     "lmoe_grouped_gemm_wgrad": (_I, [_P, _I, _I64, _I, _P, _I, _P, _I, _I, _I, _P, _P, _SZ, _P, _P]),
+    "lmoe_grouped_gemm_any": (_I, [_P, _I, _I64, _I, _P, _I, _P, _I, _I, _P, _P, _SZ, _P, _P]),
     "lmoe_fp4_scale_pitch": (_I, [_I, _I]),
     "lmoe_quantize_fp4": (_I, [_P, _I, _I64, _I, _I64, _I, _P, _I64, _P, _I, _I64, _P, _P, _P]),
     "lmoe_dequantize_fp4": (_I, [_P, _P, _I64, _I64, _I, _I, _P, _I64, _P, _P]),

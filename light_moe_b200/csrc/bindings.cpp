@@ -56,6 +56,12 @@ torch::Tensor workspace(int64_t bytes, const torch::Tensor& like) {
   return torch::empty({bytes > 0 ? bytes : 1}, like.options().dtype(torch::kUInt8));
 }
 
+// Row-contiguous and 16-byte aligned (a view may start anywhere).
+torch::Tensor contig16(const torch::Tensor& t) {
+  auto c = t.contiguous();
+  return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 == 0 ? c : c.clone();
+}
+
 struct Routed {
   torch::Tensor ids, weights, counts, offsets, sorted_idx, positions, logits, probs;
 };
@@ -158,6 +164,17 @@ torch::Tensor grouped_gemm(torch::Tensor input, torch::Tensor weights, torch::Te
   TORCH_CHECK(off.scalar_type() == torch::kInt64 || off.scalar_type() == torch::kInt32, "offsets int64/int32");
   const int64_t T = x.size(0), K = x.size(1), N = w.size(1);
   auto out = torch::empty({T, N}, x.options());
+  // row lengths that the kernels above do not take
+  if (K > 0 && N > 0 && (x.scalar_type() == torch::kFloat32 ? K % 4 != 0 : K % 128 != 0)) {
+    auto xa = contig16(x), wa = contig16(w);
+    const int dt = dtype_code(xa);
+    auto ws = workspace((int64_t)lmoe_grouped_gemm_grad_workspace_bytes(2, dt, T, (int)N, (int)K, (int)num_experts), xa);
+    check_status(lmoe_grouped_gemm_any(xa.data_ptr(), dt, T, (int)K, wa.data_ptr(), (int)N, off.data_ptr(),
+                                       off.scalar_type() == torch::kInt64 ? 1 : 0, (int)num_experts, out.data_ptr(),
+                                       ws.data_ptr(), ws.numel(), nullptr, cur_stream()),
+                 "grouped_gemm");
+    return out.to(input.scalar_type());
+  }
   auto ws = workspace((int64_t)lmoe_gemm_workspace_bytes(), x);
   int st = lmoe_grouped_gemm(x.data_ptr(), dtype_code(x), T, (int)K, w.data_ptr(), (int)N, off.data_ptr(),
                              off.scalar_type() == torch::kInt64 ? 1 : 0, (int)num_experts, 1, out.data_ptr(),
@@ -324,12 +341,6 @@ std::vector<torch::Tensor> moe_layer_w4a16(torch::Tensor x, torch::Tensor gate_w
 void check_same_device(const torch::Tensor& t, const torch::Tensor& like, const char* name) {
   check_cuda(t, name);
   TORCH_CHECK(t.device() == like.device(), name, " must be on ", like.device(), ", is on ", t.device());
-}
-
-// Row-contiguous and 16-byte aligned (a view may start anywhere).
-torch::Tensor contig16(const torch::Tensor& t) {
-  auto c = t.contiguous();
-  return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 == 0 ? c : c.clone();
 }
 
 torch::Tensor check_offsets(const torch::Tensor& offsets, const torch::Tensor& like, int64_t num_experts) {

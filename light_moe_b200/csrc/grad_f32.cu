@@ -1,10 +1,13 @@
-// grad_f32.cu -- the gradients of the grouped product for fp32 operands, on CUDA cores.
+// grad_f32.cu -- the gradients of the grouped product, and the product of any row length, for fp32
+// operands of few rows per expert, on CUDA cores.
 //
 //   input gradient   dx[r, k]    = sum_n dy[r, n] * w[e(r), n, k]
 //   weight gradient  dw[e, n, k] = sum_{r in e} dy[r, n] * x[r, k]
+//   product          y[r, n]     = sum_k x[r, k] * w[e(r), n, k]
 //
-// The tensor cores have no fp32 operands; as for the forward product (simt_gemm.cu), fp32
-// operands are multiplied and summed with fp32 FFMA in contraction order.  Bound by the FFMA
+// With few rows, writing the operands as bf16 planes for the tensor cores (grad_gemm.cu) costs
+// more than the products.  As in simt_gemm.cu, fp32 operands are multiplied and summed with fp32
+// FFMA in contraction order.  Bound by the FFMA
 // rate.  Tiles of 128 x 128 outputs, 16 contraction values per step in shared memory (the next
 // step's loads are in registers meanwhile), 256 threads of 8 x 8 outputs: 16 shared-memory words
 // feed 64 FFMAs.  Any size: operands whose rows are not multiples of 16 bytes are read word by
@@ -44,8 +47,9 @@ __device__ __forceinline__ float4 load4(const float* row, int c, int cols) {
   return v;
 }
 
-template <bool WGRAD, bool VEC>
+template <int FORM, bool VEC>
 __global__ void __launch_bounds__(kNT, 2) grad_f32_kernel(const F32Args a) {
+  constexpr bool WGRAD = FORM == kGradWeight, kProduct = FORM == kGradProduct;
   __shared__ SegTable seg;
   __shared__ __align__(16) float as[kTK][kT + 4];
   __shared__ __align__(16) float bs[kTK][kT + 4];
@@ -73,8 +77,8 @@ __global__ void __launch_bounds__(kNT, 2) grad_f32_kernel(const F32Args a) {
     const int m_rows = WGRAD ? min(kT, a.N - m * kT) : min(kT, seg.row[j + 1] - r0);
     const int depth = zero ? 0 : (WGRAD ? rows : a.N);
     const int c0 = n * kT;
-    // contraction row d of B: w[e, d, :] or x[r0 + d, :]
-    const float* bbase = a.other + (WGRAD ? (int64_t)r0 : (int64_t)(zero ? 0 : e) * a.N) * a.K;
+    // contraction row d of B: w[e, d, :] or x[r0 + d, :]; the product: row c of w[e], d along it
+    const float* bbase = a.other + (WGRAD ? (int64_t)r0 * a.K : (int64_t)(zero ? 0 : e) * a.N * a.K);
     const float* abase = a.dy + (int64_t)r0 * a.N;
     float4 av[2], bv[2];
     auto load = [&](int d0) {
@@ -82,11 +86,15 @@ __global__ void __launch_bounds__(kNT, 2) grad_f32_kernel(const F32Args a) {
       for (int i = 0; i < 2; ++i) {
         const int idx = tid + i * kNT;
         const int d = d0 + (idx >> 5), c = (idx & 31) * 4;   // 32 quads of columns a contraction row
-        bv[i] = d < depth ? load4<VEC>(bbase + (int64_t)d * a.K, c0 + c, a.K) : make_float4(0.f, 0.f, 0.f, 0.f);
+        const int r = idx >> 2, q = (idx & 3) * 4;           // four quads of contraction values a row
+        if (kProduct)
+          bv[i] = c0 + r < a.K ? load4<VEC>(bbase + (int64_t)(c0 + r) * a.N, d0 + q, depth)
+                               : make_float4(0.f, 0.f, 0.f, 0.f);
+        else
+          bv[i] = d < depth ? load4<VEC>(bbase + (int64_t)d * a.K, c0 + c, a.K) : make_float4(0.f, 0.f, 0.f, 0.f);
         if (WGRAD) {
           av[i] = d < depth ? load4<VEC>(abase + (int64_t)d * a.N, m * kT + c, a.N) : make_float4(0.f, 0.f, 0.f, 0.f);
         } else {
-          const int r = idx >> 2, q = (idx & 3) * 4;         // four quads of contraction values a row
           av[i] = r < m_rows ? load4<VEC>(abase + (int64_t)r * a.N, d0 + q, depth) : make_float4(0.f, 0.f, 0.f, 0.f);
         }
       }
@@ -101,11 +109,18 @@ __global__ void __launch_bounds__(kNT, 2) grad_f32_kernel(const F32Args a) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int idx = tid + i * kNT;
-        *reinterpret_cast<float4*>(&bs[idx >> 5][(idx & 31) * 4]) = bv[i];
+        const int r = idx >> 2, q = (idx & 3) * 4;
+        if (kProduct) {
+          bs[q][r] = bv[i].x;
+          bs[q + 1][r] = bv[i].y;
+          bs[q + 2][r] = bv[i].z;
+          bs[q + 3][r] = bv[i].w;
+        } else {
+          *reinterpret_cast<float4*>(&bs[idx >> 5][(idx & 31) * 4]) = bv[i];
+        }
         if (WGRAD) {
           *reinterpret_cast<float4*>(&as[idx >> 5][(idx & 31) * 4]) = av[i];
         } else {
-          const int r = idx >> 2, q = (idx & 3) * 4;
           as[q][r] = av[i].x;
           as[q + 1][r] = av[i].y;
           as[q + 2][r] = av[i].z;
@@ -171,17 +186,10 @@ int run_grad_f32(const GradProblem& p, cudaStream_t stream) {
   a.err = p.err;
   const bool vec = p.N % 4 == 0 && p.K % 4 == 0 && aligned16(p.dy) && aligned16(p.other) && aligned16(p.out);
   const int grid = dev.num_sms * 2;   // two CTAs fit an SM's registers
-  if (p.weight_grad) {
-    if (vec)
-      grad_f32_kernel<true, true><<<grid, kNT, 0, stream>>>(a);
-    else
-      grad_f32_kernel<true, false><<<grid, kNT, 0, stream>>>(a);
-  } else {
-    if (vec)
-      grad_f32_kernel<false, true><<<grid, kNT, 0, stream>>>(a);
-    else
-      grad_f32_kernel<false, false><<<grid, kNT, 0, stream>>>(a);
-  }
+  auto fn = p.form == kGradWeight    ? (vec ? grad_f32_kernel<kGradWeight, true> : grad_f32_kernel<kGradWeight, false>)
+            : p.form == kGradInput   ? (vec ? grad_f32_kernel<kGradInput, true> : grad_f32_kernel<kGradInput, false>)
+                                     : (vec ? grad_f32_kernel<kGradProduct, true> : grad_f32_kernel<kGradProduct, false>);
+  fn<<<grid, kNT, 0, stream>>>(a);
   return cuda_status(cudaGetLastError());
 }
 

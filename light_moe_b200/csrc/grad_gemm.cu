@@ -1,10 +1,12 @@
 // grad_gemm.cu -- the two gradients of the grouped product y[r, n] = sum_k x[r, k] * w[e, n, k]
-// over ragged row segments, on CTA pairs (sm_100a).
+// over ragged row segments, and the product itself for any row length, on CTA pairs (sm_100a).
 //
 //   input gradient   dx[r, k]    = sum_n dy[r, n] * w[e(r), n, k]        contraction over n
 //   weight gradient  dw[e, n, k] = sum_{r in e} dy[r, n] * x[r, k]       contraction over rows
+//   product          y[r, n]     = sum_k x[r, k] * w[e(r), n, k]         contraction over k
+//                    (grouped_gemm.cu has it for k a multiple of 128)
 //
-// Neither needs a transposed copy: an operand whose contraction index is the slow one in memory
+// None needs a transposed copy: an operand whose contraction index is the slow one in memory
 // (w and both operands of dw) is loaded by TMA as it lies, in chunks of 64 columns x 128
 // contraction rows, and read by tcgen05.mma as an M- or N-major operand.
 //
@@ -59,16 +61,16 @@ constexpr uint32_t kSite = 0x600u;
 // CUDA cores' products).
 constexpr int kSplitRowsX = 48, kSplitRowsW = 16;
 
-enum Form { kInputGrad = 0, kWeightGrad = 1 };
+enum Form { kInputGrad = kGradInput, kWeightGrad = kGradWeight, kProduct = kGradProduct };
 
 struct GradArgs {
   const void* offsets;
   int offsets_i64;
-  int E, N, K;
+  int E, N, K;       // the product: N is its contraction, K its columns
   int64_t R;
   int MT;            // weight gradient: row tiles of N
   Raster raster;     // of the column tiles of K
-  int KS;            // input gradient: stages of N
+  int KS;            // stages of N (not the weight gradient)
   int f16;           // operands fp16 (else bf16)
   void* out;
   int out_dtype;
@@ -102,10 +104,10 @@ __device__ __forceinline__ Tile tile_at(const SegTable& t, const GradArgs& a, in
   hint = j;
   Tile r;
   const int rows = t.row[j + 1] - t.row[j];
-  a.raster.at(tile - t.tile_start[j], FORM == kInputGrad ? (rows + kTile - 1) / kTile : a.MT, r.m, r.n);
+  a.raster.at(tile - t.tile_start[j], FORM != kWeightGrad ? (rows + kTile - 1) / kTile : a.MT, r.m, r.n);
   r.e = j - 1;
   r.row_end = t.row[j + 1];
-  if (FORM == kInputGrad) {
+  if (FORM != kWeightGrad) {
     r.row0 = t.row[j] + r.m * kTile;
     r.ks = (j == 0 || j == a.E + 1) ? 0 : a.KS;
   } else {
@@ -170,7 +172,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const int segs = a.E + 2;
   if (warp == 0)
     scan_tiles(&bars->seg, segs, lane, [&](int j) {
-      if (FORM == kInputGrad) return (bars->seg.row[j + 1] - bars->seg.row[j] + kTile - 1) / kTile * a.raster.nb;
+      if (FORM != kWeightGrad) return (bars->seg.row[j + 1] - bars->seg.row[j] + kTile - 1) / kTile * a.raster.nb;
       return j == 0 || j == a.E + 1 ? 0 : a.MT * a.raster.nb;
     });
   if (tid == 0 && bars->seg.bad && blockIdx.x == 0) report_error(a.err, kErrBadArg, kSite + 1);
@@ -192,9 +194,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     for (int tile = first; tile < total && ok; tile += stride) {
       const Tile t = tile_at<FORM>(seg, a, tile, hint);
       const int c0 = t.n * a.width + (int)rank * (a.width / 2);   // first column of B
-      const int m0 = (FORM == kInputGrad ? t.row0 : t.m * kTile) + (int)rank * kCta;
+      const int m0 = (FORM != kWeightGrad ? t.row0 : t.m * kTile) + (int)rank * kCta;
       int boxes = 4;   // input gradient: 32-row boxes of dy that hold this CTA's rows
-      if (FORM == kInputGrad) {
+      if (FORM != kWeightGrad) {
         const int rows = t.row_end - m0;
         boxes = rows <= 0 ? 0 : (rows >= kCta ? 4 : (rows + 31) >> 5);
       }
@@ -212,10 +214,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             uint8_t* sa = base + st.i * kStageBytes;
             uint8_t* sb = sa + kOperand;
             const uint32_t bar = full_addr + st.i * 8;
-            if (FORM == kInputGrad) {
+            if (FORM != kWeightGrad) {
               const int y = m0 + pa * (int)a.R;
               const int blocks = a.N - ks * kSK > 64 ? 2 : 1;
-              mbar_arrive_expect_tx_cluster(bar, (uint32_t)(blocks * boxes) * 4096u + b_bytes);
+              const uint32_t b_block = (uint32_t)a.width * 64u;   // product: width / 2 rows of 64 values
+              mbar_arrive_expect_tx_cluster(
+                  bar, (uint32_t)(blocks * boxes) * 4096u + (FORM == kProduct ? blocks * b_block : b_bytes));
               for (int h = 0; h < blocks; ++h) {
                 const int x = ks * kSK + h * 64;
                 if (boxes == 4) {
@@ -225,8 +229,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     tma_load_2d_pair(sa + h * kChunk + b * 4096, &tm_a32, bar, x, y + b * 32);
                 }
               }
-              tma_load_3d_pair(sb, &tm_b, bar, c0, ks * kSK, t.e + pb * a.E);
-              if (wide) tma_load_3d_pair(sb + kChunk, &tm_b, bar, c0 + 64, ks * kSK, t.e + pb * a.E);
+              if (FORM == kProduct) {
+                for (int h = 0; h < blocks; ++h)
+                  tma_load_3d_pair(sb + h * b_block, &tm_b, bar, ks * kSK + h * 64, c0, t.e + pb * a.E);
+              } else {
+                tma_load_3d_pair(sb, &tm_b, bar, c0, ks * kSK, t.e + pb * a.E);
+                if (wide) tma_load_3d_pair(sb + kChunk, &tm_b, bar, c0 + 64, ks * kSK, t.e + pb * a.E);
+              }
             } else {
               const int r = t.row0 + ks * kSK, ra = r + pa * (int)a.R, rb = r + pb * (int)a.R;
               const int left = t.row_end - r;
@@ -262,11 +271,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer
     if (leader) {
-      const uint32_t idesc = idesc_f16kind_f32(kTile, a.width, a.f16) | kIdescBMajorMN |
+      const uint32_t idesc = idesc_f16kind_f32(kTile, a.width, a.f16) | (FORM == kProduct ? 0u : kIdescBMajorMN) |
                              (FORM == kWeightGrad ? kIdescAMajorMN : 0u);
       // descriptors count 16 bytes
-      const uint64_t adesc0 = FORM == kInputGrad ? sdesc_k_sw128(smem_u32(base)) : sdesc_mn_sw128(smem_u32(base), kChunk);
-      const uint64_t bdesc0 = sdesc_mn_sw128(smem_u32(base) + kOperand, kChunk);
+      const uint64_t adesc0 = FORM != kWeightGrad ? sdesc_k_sw128(smem_u32(base)) : sdesc_mn_sw128(smem_u32(base), kChunk);
+      const uint64_t bdesc0 = FORM == kProduct ? sdesc_k_sw128(smem_u32(base) + kOperand)
+                                               : sdesc_mn_sw128(smem_u32(base) + kOperand, kChunk);
+      const uint32_t b_step = (uint32_t)a.width * 4u;   // product: the next 64 contraction values
       Ring<kStages> st;
       Ring<kAcc> ac;
       int hint = 0;
@@ -274,7 +285,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       for (int tile = first; tile < total && ok; tile += stride) {
         const Tile t = tile_at<FORM>(seg, a, tile, hint);
         const Passes<SPLIT> ps(t.ks);
-        const int depth = FORM == kInputGrad ? a.N : t.row_end - t.row0;
+        const int depth = FORM != kWeightGrad ? a.N : t.row_end - t.row0;
         for (int ks0 = 0; ks0 < t.ks && ok; ks0 += ps.step) {
           ok = warp_wait(&bars->acc_empty[ac.i], ac.phase ^ 1u, a.err, abort_flag, kSite + 4);
           if (!ok) break;
@@ -291,8 +302,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 #pragma unroll
               for (int kk = 0; kk < kSK / 16; ++kk) {
                 // 16 contraction values: 32 bytes of the lines of a K-major block, or 16 lines
-                const uint32_t step = FORM == kInputGrad ? (kk >> 2) * (kChunk >> 4) + (kk & 3) * 2 : kk * 128;
-                if (kk * 16 < left) mma_ss_pair(d, ad + step, bd + kk * 128, idesc, (i | kk) != 0 ? 1u : 0u);
+                const uint32_t step = FORM != kWeightGrad ? (kk >> 2) * (kChunk >> 4) + (kk & 3) * 2 : kk * 128;
+                const uint32_t bstep = FORM == kProduct ? (kk >> 2) * b_step + (kk & 3) * 2 : kk * 128;
+                if (kk * 16 < left) mma_ss_pair(d, ad + step, bd + bstep, idesc, (i | kk) != 0 ? 1u : 0u);
               }
               mma_commit_pair(&bars->empty[st.i]);
               if (i == n - 1) mma_commit_pair(&bars->acc_full[ac.i]);
@@ -354,9 +366,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const Tile t = tile_at<FORM>(seg, a, tile, hint);
       // the warp's 32 rows, and the first of its half of the columns
       const int r = (int)rank * kCta + q * 32;
-      const int left = FORM == kInputGrad ? t.row_end - t.row0 - r : a.N - t.m * kTile - r;
+      const int left = FORM != kWeightGrad ? t.row_end - t.row0 - r : a.N - t.m * kTile - r;
       const int rows = left < 32 ? left : 32;
-      const int64_t row = FORM == kInputGrad ? (int64_t)t.row0 + r : (int64_t)t.e * a.N + t.m * kTile + r;
+      const int64_t row = FORM != kWeightGrad ? (int64_t)t.row0 + r : (int64_t)t.e * a.N + t.m * kTile + r;
       uint8_t* out = static_cast<uint8_t*>(a.out) + row * pitch;
       const int cols = a.width / 2;
       const int c0 = t.n * a.width + half * cols;
@@ -516,25 +528,28 @@ int split_rows(const void* src, int64_t rows, int cols, int pitch, void* dst, co
 
 inline int64_t pitch8(int64_t cols) { return (cols + 7) / 8 * 8; }
 inline size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
+inline bool weight_grad(const GradProblem& p) { return p.form == kGradWeight; }
+// Rows and columns of the second operand.
 inline int64_t other_rows(const GradProblem& p) {
-  return p.weight_grad ? p.total_rows : (int64_t)p.num_experts * p.N;
+  return weight_grad(p) ? p.total_rows : (int64_t)p.num_experts * (p.form == kGradProduct ? p.K : p.N);
 }
+inline int other_cols(const GradProblem& p) { return p.form == kGradProduct ? p.N : p.K; }
 
 }  // namespace
 
 bool grad_splits(const GradProblem& p) {
   if (p.dtype != LMOE_DTYPE_F32 || p.total_rows * 3 > INT32_MAX) return false;
-  return p.total_rows >= (int64_t)p.num_experts * (p.weight_grad ? kSplitRowsW : kSplitRowsX);
+  return p.total_rows >= (int64_t)p.num_experts * (weight_grad(p) ? kSplitRowsW : kSplitRowsX);
 }
 
 size_t grad_gemm_workspace(const GradProblem& p) {
   if (p.dtype == LMOE_DTYPE_F32) {
     if (!grad_splits(p)) return 0;
-    return align256((size_t)p.total_rows * pitch8(p.N) * 6) + align256((size_t)other_rows(p) * pitch8(p.K) * 6);
+    return align256((size_t)p.total_rows * pitch8(p.N) * 6) + align256((size_t)other_rows(p) * pitch8(other_cols(p)) * 6);
   }
   size_t b = 0;
   if (p.N % 8) b += align256((size_t)p.total_rows * pitch8(p.N) * 2);
-  if (p.K % 8) b += align256((size_t)other_rows(p) * pitch8(p.K) * 2);
+  if (other_cols(p) % 8) b += align256((size_t)other_rows(p) * pitch8(other_cols(p)) * 2);
   return b;
 }
 
@@ -545,7 +560,7 @@ int run_grad_gemm(const GradProblem& p, cudaStream_t stream) {
   if (dev.cc_major != 10) return LMOE_ERR_DEVICE;
   const void* dy = p.dy;
   const void* other = p.other;
-  const int64_t ldy = pitch8(p.N), ldo = pitch8(p.K);
+  const int64_t ldy = pitch8(p.N), ldo = pitch8(other_cols(p));
   uint8_t* ws = static_cast<uint8_t*>(p.workspace);
   const bool split = p.dtype == LMOE_DTYPE_F32;
   if (split) {
@@ -553,7 +568,7 @@ int run_grad_gemm(const GradProblem& p, cudaStream_t stream) {
     if (st != LMOE_OK) return st;
     dy = ws;
     ws += align256((size_t)p.total_rows * ldy * 6);
-    st = split_rows(p.other, other_rows(p), p.K, (int)ldo, ws, dev, stream);
+    st = split_rows(p.other, other_rows(p), other_cols(p), (int)ldo, ws, dev, stream);
     if (st != LMOE_OK) return st;
     other = ws;
   }
@@ -563,8 +578,8 @@ int run_grad_gemm(const GradProblem& p, cudaStream_t stream) {
     dy = ws;
     ws += align256((size_t)p.total_rows * ldy * 2);
   }
-  if (!split && ldo != p.K) {
-    st = pad_rows(p.other, other_rows(p), p.K, (int)ldo, ws, dev, stream);
+  if (!split && ldo != other_cols(p)) {
+    st = pad_rows(p.other, other_rows(p), other_cols(p), (int)ldo, ws, dev, stream);
     if (st != LMOE_OK) return st;
     other = ws;
   }
@@ -585,7 +600,7 @@ int run_grad_gemm(const GradProblem& p, cudaStream_t stream) {
   const CUtensorMapDataType dt = a.f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   CUtensorMap ta, ta32, tb;
   const int grid = gemm_grid(dev) < 2 ? 2 : gemm_grid(dev) & ~1;   // whole pairs
-  const int64_t row_tiles = p.weight_grad ? (int64_t)a.MT * p.num_experts
+  const int64_t row_tiles = weight_grad(p) ? (int64_t)a.MT * p.num_experts
                                           : even_row_tiles(p.total_rows, p.num_experts, kTile);
   const int widths[] = {256, 128};
   a.width = pick_width(widths, grid / 2, 0, 16, [&](int w) { return row_tiles * ((p.K + w - 1) / w); });
@@ -593,7 +608,7 @@ int run_grad_gemm(const GradProblem& p, cudaStream_t stream) {
   // the maps end at the true sizes, so that TMA fills what lies behind them with zeros; the planes
   // of split operands follow one another along the rows (or the experts)
   const uint64_t planes = split ? 3 : 1;
-  if (p.weight_grad) {
+  if (weight_grad(p)) {
     st = encode_tmap_2d(&ta, dy, dt, 2, planes * p.total_rows, (uint64_t)p.N, (uint64_t)ldy * 2, 64, 64, true);
     if (st != LMOE_OK) return st;
     st = encode_tmap_2d(&tb, other, dt, 2, planes * p.total_rows, (uint64_t)p.K, (uint64_t)ldo * 2, 64, 64, true);
@@ -605,11 +620,16 @@ int run_grad_gemm(const GradProblem& p, cudaStream_t stream) {
   if (st != LMOE_OK) return st;
   st = encode_tmap_2d(&ta32, dy, dt, 2, planes * p.total_rows, (uint64_t)p.N, (uint64_t)ldy * 2, 32, 64, true);
   if (st != LMOE_OK) return st;
-  const uint64_t dims[3] = {(uint64_t)p.K, (uint64_t)p.N, planes * p.num_experts};
-  const uint64_t strides[2] = {(uint64_t)ldo * 2, (uint64_t)ldo * 2 * (uint64_t)p.N};
-  const uint32_t box[3] = {64, (uint32_t)kSK, 1};
+  const bool product = p.form == kGradProduct;
+  const uint64_t rows = (uint64_t)(product ? p.K : p.N);   // of one expert's matrix
+  const uint64_t dims[3] = {(uint64_t)other_cols(p), rows, planes * p.num_experts};
+  const uint64_t strides[2] = {(uint64_t)ldo * 2, (uint64_t)ldo * 2 * rows};
+  const uint32_t box[3] = {64, product ? (uint32_t)a.width / 2 : (uint32_t)kSK, 1};
   st = encode_tmap_3d(&tb, other, dt, 2, dims, strides, box);
   if (st != LMOE_OK) return st;
+  if (product)
+    return split ? launch<kProduct, true>(ta, ta32, tb, a, grid, stream)
+                 : launch<kProduct, false>(ta, ta32, tb, a, grid, stream);
   return split ? launch<kInputGrad, true>(ta, ta32, tb, a, grid, stream)
                : launch<kInputGrad, false>(ta, ta32, tb, a, grid, stream);
 }
@@ -623,13 +643,13 @@ namespace {
 int grad_entry(GradProblem& p, const void* offsets, void* out, void* workspace, size_t workspace_bytes,
                cudaStream_t stream) {
   LMOE_ARG_CHECK(p.dtype == LMOE_DTYPE_BF16 || p.dtype == LMOE_DTYPE_F16 || p.dtype == LMOE_DTYPE_F32);
-  LMOE_ARG_CHECK(p.out_dtype == p.dtype || (p.weight_grad && p.out_dtype == LMOE_DTYPE_F32));
+  LMOE_ARG_CHECK(p.out_dtype == p.dtype || (weight_grad(p) && p.out_dtype == LMOE_DTYPE_F32));
   LMOE_ARG_CHECK(p.total_rows >= 0 && p.total_rows <= INT32_MAX - 1024 && p.N > 0 && p.K > 0 && p.num_experts >= 1);
   if (p.num_experts > kMaxGemmExperts) return LMOE_ERR_UNSUPPORTED;
   const int64_t esize = p.dtype == LMOE_DTYPE_F32 ? 4 : 2, osize = p.out_dtype == LMOE_DTYPE_F32 ? 4 : 2;
   LMOE_ARG_CHECK(out && reinterpret_cast<uintptr_t>(out) % osize == 0);
   if (p.total_rows == 0) {
-    if (!p.weight_grad) return LMOE_OK;
+    if (!weight_grad(p)) return LMOE_OK;
     return cuda_status(cudaMemsetAsync(out, 0, (size_t)p.num_experts * p.N * p.K * osize, stream));
   }
   LMOE_ARG_CHECK(p.dy && p.other && offsets);
@@ -637,7 +657,7 @@ int grad_entry(GradProblem& p, const void* offsets, void* out, void* workspace, 
   if (p.dtype == LMOE_DTYPE_F32 && (!workspace || !grad_splits(p))) return run_grad_f32(p, stream);
   // rows that TMA reads where they lie start at multiples of 16 bytes
   LMOE_ARG_CHECK(p.dtype == LMOE_DTYPE_F32 ||
-                 ((p.N % 8 || aligned16(p.dy)) && (p.K % 8 || aligned16(p.other))));
+                 ((p.N % 8 || aligned16(p.dy)) && (other_cols(p) % 8 || aligned16(p.other))));
   const size_t need = grad_gemm_workspace(p);
   if (need && (!workspace || workspace_bytes < need || !aligned16(workspace))) return LMOE_ERR_WORKSPACE;
   p.workspace = workspace;
@@ -646,15 +666,15 @@ int grad_entry(GradProblem& p, const void* offsets, void* out, void* workspace, 
 
 }  // namespace
 
-extern "C" size_t lmoe_grouped_gemm_grad_workspace_bytes(int weight_grad, int dtype, int64_t total_rows, int N, int K,
+extern "C" size_t lmoe_grouped_gemm_grad_workspace_bytes(int form, int dtype, int64_t total_rows, int N, int K,
                                                          int num_experts) {
-  if (total_rows < 0 || N <= 0 || K <= 0 || num_experts <= 0) return 0;
+  if (form < 0 || form > 2 || total_rows < 0 || N <= 0 || K <= 0 || num_experts <= 0) return 0;
   GradProblem p;
-  p.weight_grad = weight_grad != 0;
+  p.form = form;
   p.dtype = dtype;
   p.total_rows = total_rows;
-  p.N = N;
-  p.K = K;
+  p.N = form == kGradProduct ? K : N;   // contraction and columns
+  p.K = form == kGradProduct ? N : K;
   p.num_experts = num_experts;
   return grad_gemm_workspace(p);
 }
@@ -664,7 +684,7 @@ extern "C" int lmoe_grouped_gemm_dgrad(const void* grad_output, int dtype, int64
                                        int num_experts, void* grad_input, void* workspace, size_t workspace_bytes,
                                        uint32_t* error, lmoe_stream_t stream) {
   GradProblem p;
-  p.weight_grad = false;
+  p.form = kGradInput;
   p.dtype = p.out_dtype = dtype;
   p.total_rows = total_rows;
   p.N = N;
@@ -685,7 +705,7 @@ extern "C" int lmoe_grouped_gemm_wgrad(const void* grad_output, int dtype, int64
                                        int num_experts, int out_dtype, void* grad_weights, void* workspace,
                                        size_t workspace_bytes, uint32_t* error, lmoe_stream_t stream) {
   GradProblem p;
-  p.weight_grad = true;
+  p.form = kGradWeight;
   p.dtype = dtype;
   p.out_dtype = out_dtype;
   p.total_rows = total_rows;
@@ -700,4 +720,24 @@ extern "C" int lmoe_grouped_gemm_wgrad(const void* grad_output, int dtype, int64
   p.err = error;
   return grad_entry(p, expert_offsets, grad_weights, workspace, workspace_bytes,
                     reinterpret_cast<cudaStream_t>(stream));
+}
+
+extern "C" int lmoe_grouped_gemm_any(const void* input, int dtype, int64_t total_rows, int K, const void* weights, int N,
+                                     const void* expert_offsets, int offsets_are_int64, int num_experts, void* output,
+                                     void* workspace, size_t workspace_bytes, uint32_t* error, lmoe_stream_t stream) {
+  GradProblem p;
+  p.form = kGradProduct;
+  p.dtype = p.out_dtype = dtype;
+  p.total_rows = total_rows;
+  p.N = K;
+  p.K = N;
+  p.num_experts = num_experts;
+  p.dy = input;
+  p.other = weights;
+  p.offsets = expert_offsets;
+  p.offsets_i64 = offsets_are_int64;
+  p.out = output;
+  p.err = error;
+  if (total_rows == 0 && !output) return N > 0 && K > 0 && num_experts >= 1 ? LMOE_OK : LMOE_ERR_INVALID_ARG;
+  return grad_entry(p, expert_offsets, output, workspace, workspace_bytes, reinterpret_cast<cudaStream_t>(stream));
 }

@@ -1,4 +1,4 @@
-// grad_gemm.h -- internal interface of the grouped product's gradients (grad_gemm.cu on tensor
+// grad_gemm.h -- internal interface of the grouped product's gradients and the product of any row length (grad_gemm.cu on tensor
 // cores, grad_f32.cu for fp32 operands on CUDA cores).
 #pragma once
 #include <cuda_runtime.h>
@@ -7,15 +7,21 @@
 
 namespace lmoe {
 
+enum GradForm : int {
+  kGradInput = 0,     // dx[r, k] from dy and w
+  kGradWeight = 1,    // dw[e, n, k] from dy and x
+  kGradProduct = 2,   // y[r, n] from x and w: N below is the contraction (x's columns), K y's columns
+};
+
 struct GradProblem {
-  bool weight_grad = false;   // dw[e, n, k] from dy and x, else dx[r, k] from dy and w
+  int form = kGradInput;
   int dtype = 0;              // operands
   int out_dtype = 0;
   int64_t total_rows = 0;
   int N = 0, K = 0;
   int num_experts = 0;
-  const void* dy = nullptr;      // [total_rows, N]
-  const void* other = nullptr;   // x [total_rows, K] or w [num_experts, N, K]
+  const void* dy = nullptr;      // [total_rows, N] (the product: x)
+  const void* other = nullptr;   // w [num_experts, N, K], x [total_rows, K], or w [num_experts, K, N]
   const void* offsets = nullptr;
   int offsets_i64 = 0;
   void* out = nullptr;

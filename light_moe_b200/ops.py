@@ -35,7 +35,8 @@ def extension():
 
 
 def grouped_gemm(input, weights, expert_offsets, num_experts):
-    """Dense bf16 grouped GEMM; rows outside every expert range are zero (grouped_gemm.cu:24)."""
+    """Dense grouped GEMM in the input dtype, any row length; rows outside every expert range are
+    zero (grouped_gemm.cu:24)."""
     return extension().grouped_gemm(input, weights, expert_offsets, num_experts)
 
 
