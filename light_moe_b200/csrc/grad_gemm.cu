@@ -33,8 +33,7 @@
 // (leader CTA); 2 clears the tail of a segment's last stage (whose copies complete on a barrier
 // of its own CTA) and hands it to the leader; 4-11 epilogue, eight warps of 32 rows x 128 columns.
 // Measured and not kept: sixteen epilogue warps (dw of 12288 rows on 64 experts 128 us against
-// 123), stores of 32-row blocks by TMA from shared memory (121 us; 22.5 against 20.7 us for 1024
-// rows on 8 experts), 64 contraction values a stage (six stages: the same within 2 % for whole
+// 123), 64 contraction values a stage (six stages: the same within 2 % for whole
 // tiles, 21 against 18.8 us for dx of 1024 rows in 128-column tiles).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -55,6 +54,7 @@ constexpr uint32_t kChunk = kSK * 128;            // 128 contraction rows of 64 
                                                   // of 64 contraction values
 constexpr uint32_t kOperand = 2 * kChunk;         // 128 x 128 values of one operand
 constexpr uint32_t kStageBytes = 2 * kOperand;
+constexpr uint32_t kBlockBytes = 32 * 128;        // a warp's block on its way out
 constexpr uint32_t kSite = 0x600u;
 
 // fp32 operands are split from this many rows per expert on (below, the copies cost more than the
@@ -141,10 +141,11 @@ __device__ __forceinline__ bool has_tail(int left) { return left < kSK && (left 
 template <int FORM, bool SPLIT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     grad_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_a32,
-                     const __grid_constant__ CUtensorMap tm_b, const GradArgs a) {
+                     const __grid_constant__ CUtensorMap tm_b, const __grid_constant__ CUtensorMap tm_out,
+                     const GradArgs a) {
   extern __shared__ __align__(1024) uint8_t base[];   // whole swizzle atoms
   uint8_t* store_stage = base + kStages * kStageBytes;
-  Bars* bars = reinterpret_cast<Bars*>(store_stage + kEpiWarps * kStoreStageBytes);
+  Bars* bars = reinterpret_cast<Bars*>(store_stage + kEpiWarps * kBlockBytes);
   volatile int* abort_flag = &bars->abort;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t rank = cluster_ctarank();
@@ -358,7 +359,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const uint32_t empty_addr = mapa_u32(&bars->acc_empty[0], 0);
     const int odt = SPLIT ? LMOE_DTYPE_F32 : a.out_dtype;   // planes come from fp32
     const int64_t pitch = (int64_t)a.K * (odt == LMOE_DTYPE_F32 ? 4 : 2);
-    uint8_t* stage = store_stage + (warp - kEpiWarp0) * kStoreStageBytes;
+    uint8_t* stage = store_stage + (warp - kEpiWarp0) * kBlockBytes;
     Ring<kAcc> ac;
     int hint = 0;
     bool ok = true;
@@ -373,6 +374,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const int cols = a.width / 2;
       const int c0 = t.n * a.width + half * cols;
       const uint32_t col0 = tmem + lane_base + half * cols;
+      // whole 32-row blocks leave by TMA; a weight gradient's rows behind N are cut by the tensor map
+      const bool whole = a.store != kStoreStaged && (FORM == kWeightGrad ? rows > 0 : rows == 32);
+      const int y = FORM == kWeightGrad ? t.m * kTile + r : (int)row, z = FORM == kWeightGrad ? t.e : 0;
+      if (!whole) {   // the lanes' stores may use the stage
+        if (elect_one()) bulk_wait_read();
+        __syncwarp();
+      }
       if constexpr (SPLIT) {
         float f[4][32];
 #pragma unroll
@@ -390,8 +398,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             tmem_ld16(col0 + ac.i * kTile + j * 16, u);
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-              float& x = f[j >> 1][(j & 1) * 16 + i];
-              x = __fadd_rn(x, __uint_as_float(u[i]));
+              float& v = f[j >> 1][(j & 1) * 16 + i];
+              v = __fadd_rn(v, __uint_as_float(u[i]));
             }
           }
           tc_fence_before();
@@ -401,35 +409,55 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         }
         if (!ok) break;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (j * 32 < cols) store_rows32(out, pitch, rows, c0 + j * 32, a.K, f[j], odt, a.store, stage, lane);
+        for (int j = 0; j < 4; ++j) {
+          if (j * 32 >= cols || c0 + j * 32 >= a.K) break;
+          if (whole)
+            store_block<128>(&tm_out, f[j], odt, stage, lane, c0 + j * 32, y, z);
+          else
+            store_rows32(out, pitch, rows, c0 + j * 32, a.K, f[j], odt, a.store, stage, lane);
+        }
       } else {
         if (t.ks != 0) {
           ok = warp_wait(&bars->acc_full[ac.i], ac.phase, a.err, abort_flag, kSite + 9);
           if (!ok) break;
           tc_fence_after();
         }
-        for (int j = 0; j < cols; j += 32) {
-          float f[32];
+        for (int j = 0; j < cols; j += 64) {
+          float f[64];
           if (t.ks != 0) {
-            uint32_t u[32];
-            tmem_ld32(col0 + ac.i * kTile + j, u);
-            if (j + 32 == cols) {
+            uint32_t u[32], v[32];
+            tmem_ld32x2(col0 + ac.i * kTile + j, col0 + ac.i * kTile + j + 32, u, v);
+            if (j + 64 == cols) {
               tc_fence_before();
               __syncwarp();
               if (lane == 0) mbar_arrive_cluster(empty_addr + ac.i * 8);
               ac.next();
             }
 #pragma unroll
-            for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(u[i]);
+            for (int i = 0; i < 32; ++i) {
+              f[i] = __uint_as_float(u[i]);
+              f[32 + i] = __uint_as_float(v[i]);
+            }
           } else {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) f[i] = 0.0f;
+            for (int i = 0; i < 64; ++i) f[i] = 0.0f;
           }
-          store_rows32(out, pitch, rows, c0 + j, a.K, f, odt, a.store, stage, lane);
+          const int c = c0 + j;
+          if (c >= a.K) continue;
+          if (whole && odt != LMOE_DTYPE_F32) {
+            store_block<128>(&tm_out, f, odt, stage, lane, c, y, z);
+          } else if (whole) {
+            store_block<128>(&tm_out, f, odt, stage, lane, c, y, z);
+            if (c + 32 < a.K) store_block<128>(&tm_out, f + 32, odt, stage, lane, c + 32, y, z);
+          } else {
+            store_rows32(out, pitch, rows, c, a.K, reinterpret_cast<const float(&)[32]>(f[0]), odt, a.store, stage, lane);
+            store_rows32(out, pitch, rows, c + 32, a.K, reinterpret_cast<const float(&)[32]>(f[32]), odt, a.store, stage,
+                         lane);
+          }
         }
       }
     }
+    if (elect_one()) bulk_wait_all();   // the stores are complete
   }
 
   tc_fence_before();
@@ -465,14 +493,14 @@ int pad_rows(const void* src, int64_t rows, int cols, int pitch, void* dst, cons
 }
 
 template <int FORM, bool SPLIT>
-int launch(const CUtensorMap& ta, const CUtensorMap& ta32, const CUtensorMap& tb, const GradArgs& a, int grid,
-           cudaStream_t stream) {
-  constexpr size_t smem = kStages * kStageBytes + kEpiWarps * kStoreStageBytes + sizeof(Bars);
+int launch(const CUtensorMap& ta, const CUtensorMap& ta32, const CUtensorMap& tb, const CUtensorMap& to,
+           const GradArgs& a, int grid, cudaStream_t stream) {
+  constexpr size_t smem = kStages * kStageBytes + kEpiWarps * kBlockBytes + sizeof(Bars);
   static_assert(smem <= 232448, "shared memory budget");
   auto fn = grad_gemm_kernel<FORM, SPLIT>;
   const int st = set_max_dynamic_smem(reinterpret_cast<const void*>(fn), smem);
   if (st != LMOE_OK) return st;
-  fn<<<grid, kThreads, smem, stream>>>(ta, ta32, tb, a);
+  fn<<<grid, kThreads, smem, stream>>>(ta, ta32, tb, to, a);
   return cuda_status(cudaGetLastError());
 }
 
@@ -598,7 +626,13 @@ int run_grad_gemm(const GradProblem& p, cudaStream_t stream) {
   a.store = store_mode(p.out, p.K, p.out_dtype);
   a.err = p.err;
   const CUtensorMapDataType dt = a.f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  CUtensorMap ta, ta32, tb;
+  CUtensorMap ta, ta32, tb, to = {};
+  if (a.store != kStoreStaged) {
+    const bool wg = weight_grad(p);
+    st = encode_store_map(&to, p.out, p.out_dtype, (uint64_t)p.K, wg ? (uint64_t)p.N : (uint64_t)p.total_rows,
+                          wg ? (uint64_t)p.num_experts : 1, 128);
+    if (st != LMOE_OK) return st;
+  }
   const int grid = gemm_grid(dev) < 2 ? 2 : gemm_grid(dev) & ~1;   // whole pairs
   const int64_t row_tiles = weight_grad(p) ? (int64_t)a.MT * p.num_experts
                                           : even_row_tiles(p.total_rows, p.num_experts, kTile);
@@ -613,8 +647,8 @@ int run_grad_gemm(const GradProblem& p, cudaStream_t stream) {
     if (st != LMOE_OK) return st;
     st = encode_tmap_2d(&tb, other, dt, 2, planes * p.total_rows, (uint64_t)p.K, (uint64_t)ldo * 2, 64, 64, true);
     if (st != LMOE_OK) return st;
-    return split ? launch<kWeightGrad, true>(ta, ta, tb, a, grid, stream)
-                 : launch<kWeightGrad, false>(ta, ta, tb, a, grid, stream);
+    return split ? launch<kWeightGrad, true>(ta, ta, tb, to, a, grid, stream)
+                 : launch<kWeightGrad, false>(ta, ta, tb, to, a, grid, stream);
   }
   st = encode_tmap_2d(&ta, dy, dt, 2, planes * p.total_rows, (uint64_t)p.N, (uint64_t)ldy * 2, kCta, 64, true);
   if (st != LMOE_OK) return st;
@@ -628,10 +662,10 @@ int run_grad_gemm(const GradProblem& p, cudaStream_t stream) {
   st = encode_tmap_3d(&tb, other, dt, 2, dims, strides, box);
   if (st != LMOE_OK) return st;
   if (product)
-    return split ? launch<kProduct, true>(ta, ta32, tb, a, grid, stream)
-                 : launch<kProduct, false>(ta, ta32, tb, a, grid, stream);
-  return split ? launch<kInputGrad, true>(ta, ta32, tb, a, grid, stream)
-               : launch<kInputGrad, false>(ta, ta32, tb, a, grid, stream);
+    return split ? launch<kProduct, true>(ta, ta32, tb, to, a, grid, stream)
+                 : launch<kProduct, false>(ta, ta32, tb, to, a, grid, stream);
+  return split ? launch<kInputGrad, true>(ta, ta32, tb, to, a, grid, stream)
+               : launch<kInputGrad, false>(ta, ta32, tb, to, a, grid, stream);
 }
 
 }  // namespace lmoe

@@ -12,6 +12,7 @@
 #include <cuda_fp16.h>
 
 #include "grouped_gemm.h"
+#include "host_util.h"
 #include "lmoe_b200.h"
 #include "ptx.cuh"
 
@@ -408,6 +409,55 @@ __device__ __forceinline__ void store_rows32(uint8_t* base, int64_t pitch, int r
       __syncwarp();
     }
   }
+}
+
+// A block of a warp's 32 rows x LINE bytes (lane l: row l; LINE / 2 16-bit values or LINE / 4 of fp32
+// from v) into `stage`, in the LINE-byte swizzle of the output's tensor map, ready for a tiled
+// store.  (The lanes' own 32-byte stores, each to another row, keep the L1 data pipe busy ~54 cycles
+// per instruction: 62 % of the kernel in a weight gradient of short segments.)
+template <int LINE>
+__device__ __forceinline__ void stage_block(const float* v, int dtype, uint8_t* stage, int lane) {
+  uint8_t* row = stage + lane * LINE;
+  const int x = LINE == 128 ? lane & 7 : (lane >> 1) & 3;   // 16-byte piece j of the row lies at j ^ x
+#pragma unroll
+  for (int j = 0; j < LINE / 16; ++j) {
+    uint4 w;
+    if (dtype == LMOE_DTYPE_F32) {
+      w = make_uint4(__float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]), __float_as_uint(v[4 * j + 2]),
+                     __float_as_uint(v[4 * j + 3]));
+    } else {
+      const bool f16 = dtype == LMOE_DTYPE_F16;
+      w = make_uint4(pack16(v[8 * j], v[8 * j + 1], f16), pack16(v[8 * j + 2], v[8 * j + 3], f16),
+                     pack16(v[8 * j + 4], v[8 * j + 5], f16), pack16(v[8 * j + 6], v[8 * j + 7], f16));
+    }
+    *reinterpret_cast<uint4*>(row + ((j ^ x) * 16)) = w;
+  }
+}
+// The block's way out: called by the whole warp; `stage` must not be read by an earlier store.
+template <int LINE>
+__device__ __forceinline__ void store_block(const CUtensorMap* map, const float* v, int dtype, uint8_t* stage,
+                                            int lane, int x, int y, int z) {
+  if (elect_one()) bulk_wait_read();
+  __syncwarp();
+  stage_block<LINE>(v, dtype, stage, lane);
+  fence_proxy_async_smem();
+  __syncwarp();
+  if (elect_one()) {
+    tma_store_3d(map, stage, x, y, z);
+    bulk_commit();
+  }
+  __syncwarp();
+}
+// The tensor map of an output [count][rows][cols] for blocks of `line` bytes x 32 rows.
+inline int encode_store_map(CUtensorMap* map, const void* out, int dtype, uint64_t cols, uint64_t rows, uint64_t count,
+                            uint32_t line) {
+  const uint32_t es = dtype == LMOE_DTYPE_F32 ? 4 : 2;
+  const CUtensorMapDataType dt = dtype == LMOE_DTYPE_F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                 : dtype == LMOE_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                           : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const uint64_t dims[3] = {cols, rows, count}, strides[2] = {cols * es, cols * es * rows};
+  const uint32_t box[3] = {line / es, 32, 1};
+  return encode_tmap_3d(map, out, dt, es, dims, strides, box);
 }
 
 // Width of the column tiles: the one with the shortest static schedule of `tiles(width)` tiles on
