@@ -34,7 +34,7 @@
 //
 // Warps: 0 TMA producer, whose copies complete on the leader's stage barrier; 1 MMA issuer
 // (leader CTA); 2-3 scales of the rows, 4-6 scales of the 192 columns (each CTA keeps all: the MMA
-// reads them beside its own rows); 7-18 epilogue, twelve warps of 32 rows x 64 columns.
+// reads them beside its own rows); 7-14 epilogue, eight warps of 32 rows.
 #include <cuda_bf16.h>
 
 #include "fp4_mma.cuh"
@@ -49,12 +49,14 @@ constexpr int kStages = 3, kAcc = 2;
 constexpr int kSfSlots = 3;       // steps of scales in shared memory
 constexpr int kUnits = 2;         // units of scales in TMEM
 constexpr uint32_t kUnitCols = 48;   // 4 words x (4 columns of the rows' scales, 8 of the columns')
-constexpr int kSfWarp0 = 2, kSfWarps = 5, kEpiWarp0 = 7, kEpiWarps = 12;
+constexpr int kSfWarp0 = 2, kSfWarps = 5, kEpiWarp0 = 7, kEpiWarps = 8;
 constexpr int kThreads = (kEpiWarp0 + kEpiWarps) * 32;
 constexpr uint32_t kABlock = kRowsCta * 128, kBBlock = kHalf * 128;
 constexpr uint32_t kABytes = 2 * kABlock, kBBytes = 2 * kBBlock;
 constexpr uint32_t kSite = 0x500u;
 constexpr int kTmemCols = 512;
+constexpr uint32_t kBlockBytes = 32 * 64;   // a warp's block on its way out
+static_assert(kBlockBytes >= kStoreStageBytes, "the lanes' stores stage there too");
 
 struct __align__(8) Bars {
   uint64_t full[kStages];       // leader: both CTAs' codes landed (one arrival each)
@@ -74,7 +76,7 @@ static_assert(kAcc * kTN + kUnits * kUnitCols <= kTmemCols, "tensor memory budge
 constexpr uint32_t kStageBytes = kABytes + kBBytes;
 constexpr uint32_t kSfABytes = 8 * 512, kSfBBytes = 8 * 1024, kSfSlotBytes = kSfABytes + kSfBBytes;
 constexpr uint32_t kSmem =
-    1024 + kStages * kStageBytes + kSfSlots * kSfSlotBytes + kEpiWarps * kStoreStageBytes + sizeof(Bars);
+    1024 + kStages * kStageBytes + kSfSlots * kSfSlotBytes + kEpiWarps * kBlockBytes + sizeof(Bars);
 static_assert(kStageBytes % 1024 == 0, "swizzle atoms");
 static_assert(kSmem <= 232448, "shared memory budget");
 
@@ -82,13 +84,13 @@ template <int FORMAT, bool SWIGLU>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     fp4_gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_x32,
                     const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_up,
-                    const Fp4Args a) {
+                    const __grid_constant__ CUtensorMap tm_out, const Fp4Args a) {
   using C = Fp4Units<FORMAT>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sf_base = base + kStages * kStageBytes;
   uint8_t* store_stage = sf_base + kSfSlots * kSfSlotBytes;
-  Bars* bars = reinterpret_cast<Bars*>(store_stage + kEpiWarps * kStoreStageBytes);
+  Bars* bars = reinterpret_cast<Bars*>(store_stage + kEpiWarps * kBlockBytes);
   volatile int* abort_flag = &bars->abort;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t rank = cluster_ctarank();
@@ -284,7 +286,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const uint32_t lane_base = (uint32_t)(q * 32) << 16;
     const uint32_t empty_addr = mapa_u32(&bars->acc_empty[0], 0);
     const int64_t pitch = (int64_t)a.N * (a.out_dtype == LMOE_DTYPE_F32 ? 4 : 2);
-    uint8_t* stage = store_stage + (warp - kEpiWarp0) * kStoreStageBytes;
+    uint8_t* stage = store_stage + (warp - kEpiWarp0) * kBlockBytes;
+    // blocks of 32 output columns: the warp's first, and how many (SwiGLU: 2 and 1 of the tile's 3)
+    const int b0 = SWIGLU ? cg * 2 : cg * 3, nb = SWIGLU ? 2 - cg : 3;
     Ring<kAcc> ac;
     int hint = 0;
     for (int tile = first; tile < total; tile += stride) {
@@ -292,40 +296,50 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const int row = t.row0 + (int)rank * kRowsCta + q * 32;   // the warp's first
       const int rows = t.row_end - row < 32 ? t.row_end - row : 32;
       uint8_t* out = static_cast<uint8_t*>(a.out) + (int64_t)row * pitch;
-      // output columns of the tile, and the warp's first
-      const int tile_cols = SWIGLU ? kHalf : kTN;
-      const int end = (t.n + 1) * tile_cols < a.N ? (t.n + 1) * tile_cols : a.N;
-      const int c0 = t.n * tile_cols + cg * (SWIGLU ? 32 : 64);
-      uint32_t u[32], v[32];
+      const bool whole = rows == 32 && a.store != kStoreStaged;   // blocks leave by TMA
       float al = 1.0f, au = 1.0f;
       if (!t.zero) {
         if (!warp_wait(&bars->acc_full[ac.i], ac.phase, a.err, abort_flag, kSite + 10)) break;
         tc_fence_after();
-        const uint32_t col = tmem + lane_base + ac.i * kTN + cg * (SWIGLU ? 32 : 64);
-        tmem_ld32x2(col, col + (SWIGLU ? kHalf : 32), u, v);   // inside the accumulators' columns
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(empty_addr + ac.i * 8);
-        ac.next();
         if (a.alpha) al = __ldg(a.alpha + t.e);
         if (SWIGLU && a.alpha_up) au = __ldg(a.alpha_up + t.e);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 32; ++i) u[i] = v[i] = 0u;
       }
-      float f[32];
+      for (int b = b0; b < b0 + nb; ++b) {
+        float f[32];
+        if (!t.zero) {
+          uint32_t u[32], v[32];
+          const uint32_t col = tmem + lane_base + ac.i * kTN + b * 32;
+          if (SWIGLU)
+            tmem_ld32x2(col, col + kHalf, u, v);
+          else
+            tmem_ld32(col, u);
+          if (b == b0 + nb - 1) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(empty_addr + ac.i * 8);
+            ac.next();
+          }
 #pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        f[i] = __fmul_rn(__uint_as_float(u[i]), al);
-        if (SWIGLU) f[i] = silu(f[i]) * __fmul_rn(__uint_as_float(v[i]), au);
-      }
-      store_rows32(out, pitch, rows, c0, end, f, a.out_dtype, a.store, stage, lane);
-      if (!SWIGLU) {
+          for (int i = 0; i < 32; ++i) {
+            f[i] = __fmul_rn(__uint_as_float(u[i]), al);
+            if (SWIGLU) f[i] = silu(f[i]) * __fmul_rn(__uint_as_float(v[i]), au);
+          }
+        } else {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) f[i] = __fmul_rn(__uint_as_float(v[i]), al);
-        store_rows32(out, pitch, rows, c0 + 32, end, f, a.out_dtype, a.store, stage, lane);
+          for (int i = 0; i < 32; ++i) f[i] = 0.0f;
+        }
+        const int c = t.n * (SWIGLU ? kHalf : kTN) + b * 32;
+        if (c >= a.N) continue;
+        if (!whole) {
+          store_rows32(out, pitch, rows, c, a.N, f, a.out_dtype, a.store, stage, lane);
+        } else {
+          store_block<64>(&tm_out, f, a.out_dtype, stage, lane, c, row, 0);
+          if (a.out_dtype == LMOE_DTYPE_F32 && c + 16 < a.N)
+            store_block<64>(&tm_out, f + 16, a.out_dtype, stage, lane, c + 16, row, 0);
+        }
       }
     }
+    if (elect_one()) bulk_wait_all();   // the stores are complete
   }
 
   tc_fence_before();
@@ -338,12 +352,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 }
 
 template <int FORMAT, bool SWIGLU>
-int launch(const CUtensorMap& x, const CUtensorMap& x32, const CUtensorMap& w, const CUtensorMap& up, const Fp4Args& a,
-           int grid, cudaStream_t stream) {
+int launch(const CUtensorMap& x, const CUtensorMap& x32, const CUtensorMap& w, const CUtensorMap& up,
+           const CUtensorMap& out, const Fp4Args& a, int grid, cudaStream_t stream) {
   auto fn = fp4_gemm_kernel<FORMAT, SWIGLU>;
   const int st = set_max_dynamic_smem(reinterpret_cast<const void*>(fn), kSmem);
   if (st != LMOE_OK) return st;
-  fn<<<grid, kThreads, kSmem, stream>>>(x, x32, w, up, a);
+  fn<<<grid, kThreads, kSmem, stream>>>(x, x32, w, up, out, a);
   return cuda_status(cudaGetLastError());
 }
 
@@ -376,7 +390,11 @@ int run_fp4_gemm(const Fp4Problem& p, cudaStream_t stream) {
   a.out_dtype = p.out_dtype;
   a.store = store_mode(p.out, p.N, p.out_dtype);
   a.err = p.err;
-  CUtensorMap tx, tx32, tw, tu;
+  CUtensorMap tx, tx32, tw, tu, to = {};
+  if (a.store != kStoreStaged) {
+    st = encode_store_map(&to, p.out, p.out_dtype, (uint64_t)p.N, (uint64_t)p.total_rows, 1, 64);
+    if (st != LMOE_OK) return st;
+  }
   const uint64_t kb = (uint64_t)p.K / 2;
   st = encode_tmap_2d(&tx, p.xq, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, (uint64_t)p.total_rows, kb, kb, kRowsCta, 128, true);
   if (st != LMOE_OK) return st;
@@ -393,10 +411,10 @@ int run_fp4_gemm(const Fp4Problem& p, cudaStream_t stream) {
     if (st != LMOE_OK) return st;
   }
   if (p.format == LMOE_FP4_MX)
-    return swiglu ? launch<LMOE_FP4_MX, true>(tx, tx32, tw, tu, a, grid, stream)
-                  : launch<LMOE_FP4_MX, false>(tx, tx32, tw, tu, a, grid, stream);
-  return swiglu ? launch<LMOE_FP4_NV, true>(tx, tx32, tw, tu, a, grid, stream)
-                : launch<LMOE_FP4_NV, false>(tx, tx32, tw, tu, a, grid, stream);
+    return swiglu ? launch<LMOE_FP4_MX, true>(tx, tx32, tw, tu, to, a, grid, stream)
+                  : launch<LMOE_FP4_MX, false>(tx, tx32, tw, tu, to, a, grid, stream);
+  return swiglu ? launch<LMOE_FP4_NV, true>(tx, tx32, tw, tu, to, a, grid, stream)
+                : launch<LMOE_FP4_NV, false>(tx, tx32, tw, tu, to, a, grid, stream);
 }
 
 }  // namespace lmoe

@@ -377,10 +377,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       // whole 32-row blocks leave by TMA; a weight gradient's rows behind N are cut by the tensor map
       const bool whole = a.store != kStoreStaged && (FORM == kWeightGrad ? rows > 0 : rows == 32);
       const int y = FORM == kWeightGrad ? t.m * kTile + r : (int)row, z = FORM == kWeightGrad ? t.e : 0;
-      if (!whole) {   // the lanes' stores may use the stage
-        if (elect_one()) bulk_wait_read();
-        __syncwarp();
-      }
       if constexpr (SPLIT) {
         float f[4][32];
 #pragma unroll
