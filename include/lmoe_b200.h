@@ -299,7 +299,7 @@ int lmoe_dequantize_fp4(const uint8_t* q, const uint8_t* scales, int64_t scale_p
  *   output[r, n] = silu(alpha[e] * x . w[e, n]) * (alpha_up[e] * x . up[e, n])   otherwise
  * exact products, fp32 accumulation.  x: codes xq [total_rows, K/2], scales xs; w (and up): codes
  * [E, N, K/2], scales [E, N, ws_pitch]; both operands of the same format, pitches multiples of 32
- * and at least lmoe_fp4_scale_pitch, pointers 16-byte aligned.  alpha, alpha_up: fp32 [E] or NULL
+ * and at least lmoe_fp4_scale_pitch, codes 16-byte and scales 32-byte aligned.  alpha, alpha_up: fp32 [E] or NULL
  * (1): the product of the two tensor scales.  output [total_rows, N] of out_dtype; rows outside
  * every expert are zero.  error: as above. */
 int lmoe_fp4_grouped_gemm(const uint8_t* xq, const uint8_t* xs, int64_t xs_pitch, int64_t total_rows, int K,

@@ -511,7 +511,7 @@ Fp4Operand fp4_operand(const torch::Tensor& q, const torch::Tensor& s, const tor
   }
   if (!pitch) pitch = padded;
   const int64_t have = (int64_t)s.storage().nbytes() - s.storage_offset();
-  const bool fits = even && (reinterpret_cast<uintptr_t>(s.data_ptr()) % 16 == 0) &&
+  const bool fits = even && (reinterpret_cast<uintptr_t>(s.data_ptr()) % 32 == 0) &&
                     (pad ? pitch % 32 == 0 && pitch >= padded && (rows - 1) * pitch + padded <= have
                          : pitch >= s.size(-1));
   if (fits) {

@@ -10,7 +10,7 @@
 //
 // Tile: 256 rows (128 per CTA, TMEM lane = row) x 192 weight rows (96 per CTA in shared memory).
 // (Narrower tiles for a fuller last round measured slower from 64 rows per expert on: 119 against
-// 112 us for 8 experts of 2 x 14336 x 4096, 50 against 41 us for 64 of 2048 x 1408.)
+// 112 us for 8 experts of 2 x 14336 x 4096.)
 // 192 columns because two accumulators (2 x 192) and two buffers of scales (2 x 48 columns) fit
 // the 512 TMEM columns, so the epilogue of a tile overlaps the next tile's MMAs; 256 columns
 // would leave room for one accumulator only.  The lane being the row, a thread holds a row's
@@ -34,7 +34,11 @@
 //
 // Warps: 0 TMA producer, whose copies complete on the leader's stage barrier; 1 MMA issuer
 // (leader CTA); 2-3 scales of the rows, 4-6 scales of the 192 columns (each CTA keeps all: the MMA
-// reads them beside its own rows); 7-14 epilogue, eight warps of 32 rows.
+// reads them beside its own rows); from 7 on the epilogue: eight warps of 32 rows x 96 columns, or
+// twelve of 32 rows x 32 features for the SwiGLU, whose arithmetic wants more warps.  Whole blocks
+// of 32 rows x 64 bytes (SwiGLU 32) leave by tiled stores; lanes that store rows of their own kept
+// the L1 data pipe busy (64 experts of 2048 x 1408, 700 rows each: 100 us, was 134).  With eight
+// warps the SwiGLU of 64 experts of 2 x 1408 x 2048 takes 163 us, with twelve 139.
 #include <cuda_bf16.h>
 
 #include "fp4_mma.cuh"
@@ -49,15 +53,18 @@ constexpr int kStages = 3, kAcc = 2;
 constexpr int kSfSlots = 3;       // steps of scales in shared memory
 constexpr int kUnits = 2;         // units of scales in TMEM
 constexpr uint32_t kUnitCols = 48;   // 4 words x (4 columns of the rows' scales, 8 of the columns')
-constexpr int kSfWarp0 = 2, kSfWarps = 5, kEpiWarp0 = 7, kEpiWarps = 8;
-constexpr int kThreads = (kEpiWarp0 + kEpiWarps) * 32;
+constexpr int kSfWarp0 = 2, kSfWarps = 5, kEpiWarp0 = 7;
+// The epilogue's warps: SwiGLU twelve of 32 features, a product eight of 96 columns.
+template <bool SWIGLU>
+struct Epi {
+  static constexpr int kWarps = SWIGLU ? 12 : 8, kThreads = (kEpiWarp0 + kWarps) * 32;
+  static constexpr int kCols = SWIGLU ? 16 : 32, kBlocks = SWIGLU ? 2 : 3;   // of a block; blocks a warp
+  static constexpr uint32_t kBlockBytes = 32 * kCols * 2;                   // a block on its way out
+};
 constexpr uint32_t kABlock = kRowsCta * 128, kBBlock = kHalf * 128;
 constexpr uint32_t kABytes = 2 * kABlock, kBBytes = 2 * kBBlock;
 constexpr uint32_t kSite = 0x500u;
 constexpr int kTmemCols = 512;
-constexpr uint32_t kBlockBytes = 32 * 64;   // a warp's block on its way out
-static_assert(kBlockBytes >= kStoreStageBytes, "the lanes' stores stage there too");
-
 struct __align__(8) Bars {
   uint64_t full[kStages];       // leader: both CTAs' codes landed (one arrival each)
   uint64_t empty[kStages];      // the stage's MMAs finished (both CTAs)
@@ -75,22 +82,23 @@ struct __align__(8) Bars {
 static_assert(kAcc * kTN + kUnits * kUnitCols <= kTmemCols, "tensor memory budget");
 constexpr uint32_t kStageBytes = kABytes + kBBytes;
 constexpr uint32_t kSfABytes = 8 * 512, kSfBBytes = 8 * 1024, kSfSlotBytes = kSfABytes + kSfBBytes;
-constexpr uint32_t kSmem =
-    1024 + kStages * kStageBytes + kSfSlots * kSfSlotBytes + kEpiWarps * kBlockBytes + sizeof(Bars);
+constexpr uint32_t kEpiBytes = 12 * kStoreStageBytes > 8 * 2048 ? 12 * kStoreStageBytes : 8 * 2048;
+constexpr uint32_t kSmem = 1024 + kStages * kStageBytes + kSfSlots * kSfSlotBytes + kEpiBytes + sizeof(Bars);
 static_assert(kStageBytes % 1024 == 0, "swizzle atoms");
 static_assert(kSmem <= 232448, "shared memory budget");
 
 template <int FORMAT, bool SWIGLU>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Epi<SWIGLU>::kThreads, 1)
     fp4_gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_x32,
                     const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_up,
                     const __grid_constant__ CUtensorMap tm_out, const Fp4Args a) {
   using C = Fp4Units<FORMAT>;
+  using Ep = Epi<SWIGLU>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sf_base = base + kStages * kStageBytes;
   uint8_t* store_stage = sf_base + kSfSlots * kSfSlotBytes;
-  Bars* bars = reinterpret_cast<Bars*>(store_stage + kEpiWarps * kBlockBytes);
+  Bars* bars = reinterpret_cast<Bars*>(store_stage + kEpiBytes);
   volatile int* abort_flag = &bars->abort;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t rank = cluster_ctarank();
@@ -108,7 +116,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     for (int s = 0; s < kUnits; ++s) mbar_init(&bars->unit_empty[s], 1);
     for (int s = 0; s < kAcc; ++s) {
       mbar_init(&bars->acc_full[s], 1);
-      mbar_init(&bars->acc_empty[s], 2 * kEpiWarps);
+      mbar_init(&bars->acc_empty[s], 2 * Ep::kWarps);
     }
     mbar_init(&bars->mma_done, 1);
     bars->abort = 0;
@@ -118,7 +126,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     tmem_alloc_pair(&bars->tmem_base, kTmemCols);
     tmem_relinquish_pair();
   }
-  load_segments(&bars->seg, a.offsets, a.offsets_i64, a.E, a.R, tid, kThreads);
+  load_segments(&bars->seg, a.offsets, a.offsets_i64, a.E, a.R, tid, Ep::kThreads);
   const int segs = a.E + 2;
   if (warp == 0)
     scan_tiles(&bars->seg, segs, lane, [&](int j) {
@@ -286,9 +294,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const uint32_t lane_base = (uint32_t)(q * 32) << 16;
     const uint32_t empty_addr = mapa_u32(&bars->acc_empty[0], 0);
     const int64_t pitch = (int64_t)a.N * (a.out_dtype == LMOE_DTYPE_F32 ? 4 : 2);
-    uint8_t* stage = store_stage + (warp - kEpiWarp0) * kBlockBytes;
-    // blocks of 32 output columns: the warp's first, and how many (SwiGLU: 2 and 1 of the tile's 3)
-    const int b0 = SWIGLU ? cg * 2 : cg * 3, nb = SWIGLU ? 2 - cg : 3;
+    uint8_t* stage = store_stage + (warp - kEpiWarp0) * (kEpiBytes / Ep::kWarps / 128 * 128);
     Ring<kAcc> ac;
     int hint = 0;
     for (int tile = first; tile < total; tile += stride) {
@@ -301,41 +307,46 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       if (!t.zero) {
         if (!warp_wait(&bars->acc_full[ac.i], ac.phase, a.err, abort_flag, kSite + 10)) break;
         tc_fence_after();
+        if (rows <= 0) {   // the segment ends before this warp's rows
+          if (lane == 0) mbar_arrive_cluster(empty_addr + ac.i * 8);
+          ac.next();
+          continue;
+        }
         if (a.alpha) al = __ldg(a.alpha + t.e);
         if (SWIGLU && a.alpha_up) au = __ldg(a.alpha_up + t.e);
       }
-      for (int b = b0; b < b0 + nb; ++b) {
-        float f[32];
+      for (int b = cg * Ep::kBlocks; b < (cg + 1) * Ep::kBlocks; ++b) {
+        float f[Ep::kCols];
         if (!t.zero) {
-          uint32_t u[32], v[32];
-          const uint32_t col = tmem + lane_base + ac.i * kTN + b * 32;
-          if (SWIGLU)
-            tmem_ld32x2(col, col + kHalf, u, v);
+          uint32_t u[Ep::kCols], v[Ep::kCols];
+          const uint32_t col = tmem + lane_base + ac.i * kTN + b * Ep::kCols;
+          if constexpr (SWIGLU)
+            tmem_ld16x2(col, col + kHalf, u, v);
           else
             tmem_ld32(col, u);
-          if (b == b0 + nb - 1) {
+          if (b == (cg + 1) * Ep::kBlocks - 1) {
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster(empty_addr + ac.i * 8);
             ac.next();
           }
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
+          for (int i = 0; i < Ep::kCols; ++i) {
             f[i] = __fmul_rn(__uint_as_float(u[i]), al);
             if (SWIGLU) f[i] = silu(f[i]) * __fmul_rn(__uint_as_float(v[i]), au);
           }
         } else {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) f[i] = 0.0f;
+          for (int i = 0; i < Ep::kCols; ++i) f[i] = 0.0f;
         }
-        const int c = t.n * (SWIGLU ? kHalf : kTN) + b * 32;
+        const int c = t.n * (SWIGLU ? kHalf : kTN) + b * Ep::kCols;
         if (c >= a.N) continue;
         if (!whole) {
-          store_rows32(out, pitch, rows, c, a.N, f, a.out_dtype, a.store, stage, lane);
+          store_rows(out, pitch, rows, c, a.N, f, a.out_dtype, a.store, stage, lane);
         } else {
-          store_block<64>(&tm_out, f, a.out_dtype, stage, lane, c, row, 0);
-          if (a.out_dtype == LMOE_DTYPE_F32 && c + 16 < a.N)
-            store_block<64>(&tm_out, f + 16, a.out_dtype, stage, lane, c + 16, row, 0);
+          store_block<Ep::kCols * 2>(&tm_out, f, a.out_dtype, stage, lane, c, row, 0);
+          if (a.out_dtype == LMOE_DTYPE_F32 && c + Ep::kCols / 2 < a.N)
+            store_block<Ep::kCols * 2>(&tm_out, f + Ep::kCols / 2, a.out_dtype, stage, lane, c + Ep::kCols / 2, row, 0);
         }
       }
     }
@@ -357,7 +368,7 @@ int launch(const CUtensorMap& x, const CUtensorMap& x32, const CUtensorMap& w, c
   auto fn = fp4_gemm_kernel<FORMAT, SWIGLU>;
   const int st = set_max_dynamic_smem(reinterpret_cast<const void*>(fn), kSmem);
   if (st != LMOE_OK) return st;
-  fn<<<grid, kThreads, kSmem, stream>>>(x, x32, w, up, out, a);
+  fn<<<grid, Epi<SWIGLU>::kThreads, kSmem, stream>>>(x, x32, w, up, out, a);
   return cuda_status(cudaGetLastError());
 }
 
@@ -392,7 +403,7 @@ int run_fp4_gemm(const Fp4Problem& p, cudaStream_t stream) {
   a.err = p.err;
   CUtensorMap tx, tx32, tw, tu, to = {};
   if (a.store != kStoreStaged) {
-    st = encode_store_map(&to, p.out, p.out_dtype, (uint64_t)p.N, (uint64_t)p.total_rows, 1, 64);
+    st = encode_store_map(&to, p.out, p.out_dtype, (uint64_t)p.N, (uint64_t)p.total_rows, 1, swiglu ? 32 : 64);
     if (st != LMOE_OK) return st;
   }
   const uint64_t kb = (uint64_t)p.K / 2;
@@ -437,8 +448,8 @@ extern "C" int lmoe_fp4_grouped_gemm(const uint8_t* xq, const uint8_t* xs, int64
   LMOE_ARG_CHECK(xs_pitch >= fp4_scale_pitch(K, format) && ws_pitch >= fp4_scale_pitch(K, format));
   if (total_rows == 0) return LMOE_OK;
   LMOE_ARG_CHECK(xq && xs && wq && ws && expert_offsets && output);
-  LMOE_ARG_CHECK(aligned16(xq) && aligned16(xs) && aligned16(wq) && aligned16(ws) && aligned16(wq_up) &&
-                 aligned16(ws_up));
+  LMOE_ARG_CHECK(aligned16(xq) && aligned16(wq) && aligned16(wq_up) && aligned32(xs) && aligned32(ws) &&
+                 aligned32(ws_up));
   LMOE_ARG_CHECK(reinterpret_cast<uintptr_t>(output) % (out_dtype == LMOE_DTYPE_F32 ? 4 : 2) == 0);
   Fp4Problem p;
   p.xq = xq;
@@ -462,10 +473,10 @@ extern "C" int lmoe_fp4_grouped_gemm(const uint8_t* xq, const uint8_t* xs, int64
   p.out = output;
   p.err = error;
   // Few rows: the weights' bytes bound, and tiles of 256 weight rows stream them best (8 experts of
-  // 4096 x 14336, rows per expert: 1 50 against 72 us, 64 63 against 77, 96 76 against 81; 64 of 2048
-  // x 1408: 25 against 37, 40 against 44, 54 against 48).  The SwiGLU's exchange between lanes makes
-  // up less (8 of 2 x 14336 x 4096: 1 79 against 103 us, 48 94 against 110, 64 120 against 111; 64 of
-  // 2 x 1408 x 2048: 38 against 50, 16 44 against 52, 32 55 against 53).
+  // 4096 x 14336, us by rows per expert: 1 50 against 68, 64 63 against 72, 96 76 against 73; 64 of
+  // 2048 x 1408: 25 against 34, 39 against 37, 54 against 39).  The SwiGLU's exchange between lanes
+  // makes up less (8 of 2 x 14336 x 4096: 1 80 against 102, 32 87 against 107, 64 124 against 110; 64
+  // of 2 x 1408 x 2048: 38 against 50, 16 45 against 52, 32 55 against 52).
   const int64_t few = (int64_t)num_experts * (wq_up ? kFp4DecodeRows / 2 : kFp4DecodeRows);
   return total_rows <= few ? run_fp4_decode(p, stream) : run_fp4_gemm(p, stream);
 }

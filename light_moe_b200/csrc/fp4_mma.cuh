@@ -113,15 +113,15 @@ __device__ __forceinline__ void write_scales(int first, int total, int stride, i
   auto next_tile = [&]() {   // first tile at or behind ltile that has an expert
     while (ltile < total && !rows(ltile, lp)) ltile += stride;
   };
-  uint4 v[kAhead][2][2];
+  uint32_t v[kAhead][2][8];
   int pending = 0;
-  auto load = [&](uint4 (&b)[2][2]) {
+  auto load = [&](uint32_t (&b)[2][8]) {
     if (ltile >= total) return;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        b[i][h] = lp[i] ? __ldg(reinterpret_cast<const uint4*>(lp[i] + lstep * 32) + h) : make_uint4(0, 0, 0, 0);
+      for (int q = 0; q < 8; ++q) b[i][q] = 0u;
+      if (lp[i]) ld_global_nc_v8(lp[i] + lstep * 32, b[i]);
     }
     ++pending;
     if (++lstep == steps) {
@@ -145,7 +145,7 @@ __device__ __forceinline__ void write_scales(int first, int total, int stride, i
         // scale bytes behind the last block are padding: zero, whatever they hold
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          uint32_t* w = reinterpret_cast<uint32_t*>(&v[j][i][0]);
+          uint32_t (&w)[8] = v[j][i];
 #pragma unroll
           for (int q = 0; q < 8; ++q) {
             const int valid = nb - (step * 32 + q * 4);
@@ -158,11 +158,7 @@ __device__ __forceinline__ void write_scales(int first, int total, int stride, i
       if (!ok) break;
 #pragma unroll
       for (int q = 0; q < 8; ++q) {
-        const uint4 x = v[j][0][q >> 2], y = v[j][1][q >> 2];
-        const uint2 o = (q & 3) == 0 ? make_uint2(x.x, y.x)
-                                     : (q & 3) == 1 ? make_uint2(x.y, y.y)
-                                                    : (q & 3) == 2 ? make_uint2(x.z, y.z) : make_uint2(x.w, y.w);
-        *reinterpret_cast<uint2*>(dst + sl.i * slot_bytes + q * dst_word) = o;
+        *reinterpret_cast<uint2*>(dst + sl.i * slot_bytes + q * dst_word) = make_uint2(v[j][0][q], v[j][1][q]);
       }
       fence_proxy_async_smem();
       __syncwarp();

@@ -410,7 +410,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           if (whole)
             store_block<128>(&tm_out, f[j], odt, stage, lane, c0 + j * 32, y, z);
           else
-            store_rows32(out, pitch, rows, c0 + j * 32, a.K, f[j], odt, a.store, stage, lane);
+            store_rows(out, pitch, rows, c0 + j * 32, a.K, f[j], odt, a.store, stage, lane);
         }
       } else {
         if (t.ks != 0) {
@@ -446,8 +446,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             store_block<128>(&tm_out, f, odt, stage, lane, c, y, z);
             if (c + 32 < a.K) store_block<128>(&tm_out, f + 32, odt, stage, lane, c + 32, y, z);
           } else {
-            store_rows32(out, pitch, rows, c, a.K, reinterpret_cast<const float(&)[32]>(f[0]), odt, a.store, stage, lane);
-            store_rows32(out, pitch, rows, c + 32, a.K, reinterpret_cast<const float(&)[32]>(f[32]), odt, a.store, stage,
+            store_rows(out, pitch, rows, c, a.K, reinterpret_cast<const float(&)[32]>(f[0]), odt, a.store, stage, lane);
+            store_rows(out, pitch, rows, c + 32, a.K, reinterpret_cast<const float(&)[32]>(f[32]), odt, a.store, stage,
                          lane);
           }
         }

@@ -232,10 +232,10 @@ int encode_tmap_3d(CUtensorMap* map, const void* base, CUtensorMapDataType dtype
   if (!g_encode) return LMOE_ERR_DEVICE;
   if (!aligned16(base) || (strides[0] % 16) != 0 || (strides[1] % 16) != 0) return LMOE_ERR_INVALID_ARG;
   const uint32_t line = box[0] * elem_bytes;
-  if ((line != 128 && line != 64) || box[1] == 0 || box[1] > 256 || box[2] == 0 || box[2] > 256)
+  if ((line != 128 && line != 64 && line != 32) || box[1] == 0 || box[1] > 256 || box[2] == 0 || box[2] > 256)
     return LMOE_ERR_INVALID_ARG;
   const TmapKey key = {base, {dims[0], dims[1], dims[2]}, {strides[0], strides[1]}, {box[0], box[1], box[2]},
-                       (uint32_t)dtype, 3u, line == 128 ? 1u : 2u};
+                       (uint32_t)dtype, 3u, line == 128 ? 1u : line == 64 ? 2u : 3u};
   if (tmap_lookup(key, map)) return LMOE_OK;
   cuuint64_t gdim[3] = {dims[0], dims[1], dims[2]};
   cuuint64_t gstride[2] = {strides[0], strides[1]};
@@ -243,7 +243,9 @@ int encode_tmap_3d(CUtensorMap* map, const void* base, CUtensorMapDataType dtype
   cuuint32_t estride[3] = {1, 1, 1};
   CUresult r = g_encode(map, dtype, 3, const_cast<void*>(base), gdim, gstride, bx, estride,
                         CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        line == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                        line == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
+                        : line == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                     : CU_TENSOR_MAP_SWIZZLE_32B,
                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return LMOE_ERR_INVALID_ARG;

@@ -69,6 +69,7 @@ int encode_tmap_kblocks(CUtensorMap* map, const void* base, CUtensorMapDataType 
 int encode_tmap_3d(CUtensorMap* map, const void* base, CUtensorMapDataType dtype, uint32_t elem_bytes,
                    const uint64_t (&dims)[3], const uint64_t (&strides)[2], const uint32_t (&box)[3]);
 
+inline bool aligned32(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 31u) == 0; }
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 }  // namespace lmoe

@@ -334,13 +334,14 @@ inline int store_mode(const void* out, int64_t cols, int dtype) {
 }
 constexpr uint32_t kStoreStageBytes = 1152;   // per warp
 
-// Called by a whole warp: lane l holds 32 values of row l (of `rows` valid ones) from column c0;
+// Called by a whole warp: lane l holds COLS values of row l (of `rows` valid ones) from column c0;
 // columns at or behind `cols` are not written.  Rows that start at odd addresses go through
 // `stage` (kStoreStageBytes of the warp's own), so that neighbouring lanes write neighbouring
 // columns: storing them value by value from the lanes that hold them touches 32 sectors per
 // instruction (the gradients of fp16 rows of odd lengths took 7.9 ms, of which ~7 ms stores).
-__device__ __forceinline__ void store_rows32(uint8_t* base, int64_t pitch, int rows, int c0, int cols,
-                                             const float (&v)[32], int dtype, int mode, uint8_t* stage, int lane) {
+template <int COLS>
+__device__ __forceinline__ void store_rows(uint8_t* base, int64_t pitch, int rows, int c0, int cols,
+                                           const float (&v)[COLS], int dtype, int mode, uint8_t* stage, int lane) {
   if (c0 >= cols || rows <= 0) return;
   const bool f16 = dtype == LMOE_DTYPE_F16;
   if (mode != kStoreStaged) {
@@ -349,7 +350,7 @@ __device__ __forceinline__ void store_rows32(uint8_t* base, int64_t pitch, int r
     if (dtype == LMOE_DTYPE_F32) {
       float* p = reinterpret_cast<float*>(row) + c0;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < COLS / 8; ++j) {
         if (mode == kStore32 && c0 + 8 * j < cols) {
           uint32_t w[8];
 #pragma unroll
@@ -366,7 +367,7 @@ __device__ __forceinline__ void store_rows32(uint8_t* base, int64_t pitch, int r
     } else {
       uint16_t* p = reinterpret_cast<uint16_t*>(row) + c0;
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
+      for (int j = 0; j < COLS / 16; ++j) {
         uint32_t w[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) w[i] = pack16(v[16 * j + 2 * i], v[16 * j + 2 * i + 1], f16);
@@ -385,7 +386,7 @@ __device__ __forceinline__ void store_rows32(uint8_t* base, int64_t pitch, int r
   if (dtype == LMOE_DTYPE_F32) {
     float* st = reinterpret_cast<float*>(stage);   // [32][9]
 #pragma unroll
-    for (int ch = 0; ch < 4; ++ch) {
+    for (int ch = 0; ch < COLS / 8; ++ch) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) st[lane * 9 + i] = v[8 * ch + i];
       __syncwarp();
@@ -396,7 +397,7 @@ __device__ __forceinline__ void store_rows32(uint8_t* base, int64_t pitch, int r
     }
   } else {
 #pragma unroll
-    for (int ch = 0; ch < 2; ++ch) {   // [32][18] 16-bit values
+    for (int ch = 0; ch < COLS / 16; ++ch) {   // [32][18] 16-bit values
 #pragma unroll
       for (int i = 0; i < 8; ++i)
         *reinterpret_cast<uint32_t*>(stage + lane * 36 + i * 4) = pack16(v[16 * ch + 2 * i], v[16 * ch + 2 * i + 1], f16);
@@ -418,7 +419,7 @@ __device__ __forceinline__ void store_rows32(uint8_t* base, int64_t pitch, int r
 template <int LINE>
 __device__ __forceinline__ void stage_block(const float* v, int dtype, uint8_t* stage, int lane) {
   uint8_t* row = stage + lane * LINE;
-  const int x = LINE == 128 ? lane & 7 : (lane >> 1) & 3;   // 16-byte piece j of the row lies at j ^ x
+  const int x = LINE == 128 ? lane & 7 : LINE == 64 ? (lane >> 1) & 3 : (lane >> 2) & 1;   // 16-byte piece j of the row lies at j ^ x
 #pragma unroll
   for (int j = 0; j < LINE / 16; ++j) {
     uint4 w;

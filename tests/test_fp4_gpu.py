@@ -381,3 +381,44 @@ def test_streams_graphs_and_the_sm_limit():
             assert torch.equal(step(), y)
     finally:
         lib.lmoe_set_gemm_sm_limit(before)
+
+
+@pytest.mark.parametrize("odt", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("swiglu", [False, True])
+@pytest.mark.parametrize("N", [8, 40, 104, 264])
+def test_blocks_of_rows_cut_by_the_last_column(odt, swiglu, N):
+    """Whole blocks of 32 rows leave together, also where the output ends inside a block."""
+    _check_product([200, 0, 96, 165], N, 96, "mxfp4", swiglu, odt=odt, head=7, tail=40, seed=N)
+
+
+@pytest.mark.parametrize("swiglu", [False, True])
+@pytest.mark.parametrize("shift", [2, 16, 32])
+def test_output_anywhere_and_nothing_beside_it(swiglu, shift):
+    """An output at an address of `shift` bytes behind a 256-byte boundary; bytes around it stay."""
+    gen = torch.Generator(device="cuda").manual_seed(shift)
+    R, N, K, fmt = 300, 136, 128, "nvfp4"
+    off = torch.tensor([0, 130, 300], dtype=torch.int32, device="cuda")
+    xq, xs = _operand((R, K), fmt, gen)
+    wq, ws = _operand((2, N, K), fmt, gen)
+    up = dict(weights_up=wq, weight_scales_up=ws) if swiglu else {}
+    want = ops.fp4_grouped_gemm(xq, xs, wq, ws, off, 2, fmt, **up)
+    buf = torch.full((R * N * 2 + 512,), 0x5A, dtype=torch.uint8, device="cuda")
+    u = (wq.data_ptr(), ws.data_ptr()) if swiglu else (None, None)
+    capi.call("lmoe_fp4_grouped_gemm", xq.data_ptr(), xs.data_ptr(), 32, R, K, wq.data_ptr(), ws.data_ptr(), *u, 32, N, 1,
+              off.data_ptr(), 0, 2, None, None, 0, buf.data_ptr() + 256 + shift, None, capi.stream_handle())
+    y = buf[256 + shift:256 + shift + R * N * 2]
+    assert torch.equal(y, want.view(torch.uint8).flatten())
+    assert (buf[:256 + shift] == 0x5A).all() and (buf[256 + shift + R * N * 2:] == 0x5A).all()
+
+
+def test_scales_at_odd_addresses():
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    R, N, K, fmt = 90, 64, 512, "nvfp4"
+    off = torch.tensor([0, 90], dtype=torch.int32, device="cuda")
+    xq, xs = _operand((R, K), fmt, gen)
+    wq, ws = _operand((1, N, K), fmt, gen)
+    want = ops.fp4_grouped_gemm(xq, xs, wq, ws, off, 1, fmt)
+    for shift in (1, 16):
+        moved = torch.zeros(R * 32 + shift, dtype=torch.uint8, device="cuda")[shift:].view(R, 32)
+        moved.copy_(xs)
+        assert torch.equal(ops.fp4_grouped_gemm(xq, moved, wq, ws, off, 1, fmt), want)

@@ -138,3 +138,8 @@ def test_reference_codes():
     c, s = ref.quantize(x[:, :16] / 7.9 * 6, "nvfp4")
     assert s[0, 0] == 56 and c[0, 9] == 7                                              # byte 56 = 1.0
     assert ref.e4m3_table()[[1, 8, 56, 126]].tolist() == [2.0 ** -9, 2.0 ** -6, 1.0, 448.0]
+
+
+@pytest.mark.parametrize("bad", [dict(xs=P + 16), dict(ws=P + 16), dict(uq=P, us=P + 16)])
+def test_gemm_wants_scales_on_whole_sectors(bad):
+    assert _gemm(**bad) == INVALID
