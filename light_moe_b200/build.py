@@ -29,9 +29,11 @@ CUDA_HOME = os.environ.get("CUDA_HOME", "/usr/local/cuda")
 NVCC = os.path.join(CUDA_HOME, "bin", "nvcc")
 
 CU_SOURCES = ["host_util.cu", "router.cu", "quant.cu", "grouped_gemm.cu", "decode_gemm.cu", "simt_gemm.cu",
-              "layer.cu", "dispatch.cu", "ep_p2p.cu", "fp4_quant.cu", "fp4_gemm.cu", "fp4_decode.cu", "grad_gemm.cu", "grad_f32.cu"]
+              "layer.cu", "dispatch.cu", "ep_p2p.cu", "fp4_quant.cu", "fp4_gemm.cu", "fp4_decode.cu",
+              "grad_gemm.cu", "grad_split.cu", "grad_f32.cu"]
 HEADERS = ["ptx.cuh", "lmoe_math.cuh", "host_util.h", "w4_layout.cuh", "w4_dequant.cuh", "grouped_gemm.h",
-           "decode_gemm.h", "pair_gemm.cuh", "fp4_format.cuh", "fp4_mma.cuh", "fp4_gemm.h", "grad_gemm.h"]
+           "decode_gemm.h", "pair_gemm.cuh", "fp4_format.cuh", "fp4_mma.cuh", "fp4_gemm.h", "grad_gemm.h",
+           "grad_tile.cuh"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-std=c++17", "-lineinfo",

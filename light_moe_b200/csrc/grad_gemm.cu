@@ -22,13 +22,6 @@
 // a product with a zero row would not do, since those rows may hold infinities or NaN.  Experts
 // without rows get a zero dw, rows outside every expert a zero dx.
 //
-// fp32 operands (SPLIT) are first written as three bf16 planes each, x = high + middle + low to
-// 2^-26, and the tile sums the six products of planes down to 2^-18: (l, h), (h, l), (m, m),
-// (m, h), (h, m), (h, h), six times the bf16 work at ~16 times the FFMA rate.  The tensor pipe
-// truncates its sums (measured: 1024 bf16 products of mean 1 come out 8e-7 low, 8192 2.5e-5), so
-// a TMEM accumulator takes 128 contraction values only, small products first, and the epilogue
-// adds the accumulators in registers, rounding to nearest.
-//
 // Warps: 0 TMA producer, whose copies complete on the leader's stage barrier; 1 MMA issuer
 // (leader CTA); 2 clears the tail of a segment's last stage (whose copies complete on a barrier
 // of its own CTA) and hands it to the leader; 4-11 epilogue, eight warps of 32 rows x 128 columns.
@@ -38,14 +31,11 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
-#include "grad_gemm.h"
-#include "host_util.h"
-#include "pair_gemm.cuh"
+#include "grad_tile.cuh"
 
 namespace lmoe {
 namespace {
 
-constexpr int kTile = 256, kCta = 128;
 constexpr int kSK = 128;           // contraction values per stage
 constexpr int kStages = 3, kAcc = 2;
 constexpr int kEpiWarp0 = 4, kEpiWarps = 8;
@@ -56,28 +46,6 @@ constexpr uint32_t kOperand = 2 * kChunk;         // 128 x 128 values of one ope
 constexpr uint32_t kStageBytes = 2 * kOperand;
 constexpr uint32_t kBlockBytes = 32 * 128;        // a warp's block on its way out
 constexpr uint32_t kSite = 0x600u;
-
-// fp32 operands are split from this many rows per expert on (below, the copies cost more than the
-// CUDA cores' products).
-constexpr int kSplitRowsX = 48, kSplitRowsW = 16;
-
-enum Form { kInputGrad = kGradInput, kWeightGrad = kGradWeight, kProduct = kGradProduct };
-
-struct GradArgs {
-  const void* offsets;
-  int offsets_i64;
-  int E, N, K;       // the product: N is its contraction, K its columns
-  int64_t R;
-  int MT;            // weight gradient: row tiles of N
-  Raster raster;     // of the column tiles of K
-  int KS;            // stages of N (not the weight gradient)
-  int f16;           // operands fp16 (else bf16)
-  void* out;
-  int out_dtype;
-  int width;         // columns of a tile: 256 or 128
-  int store;         // StoreMode
-  uint32_t* err;
-};
 
 struct __align__(8) Bars {
   uint64_t full[kStages];       // leader: both CTAs' operands landed (one arrival each)
@@ -91,54 +59,10 @@ struct __align__(8) Bars {
   SegTable seg;
 };
 
-struct Tile {
-  int e, m, n;
-  int row0, row_end;   // input gradient: output rows; weight gradient: the expert's rows
-  int ks;              // stages; 0: the tile is zero
-};
-
-template <int FORM>
-__device__ __forceinline__ Tile tile_at(const SegTable& t, const GradArgs& a, int tile, int& hint) {
-  int j = hint;
-  while (tile >= t.tile_start[j + 1]) ++j;
-  hint = j;
-  Tile r;
-  const int rows = t.row[j + 1] - t.row[j];
-  a.raster.at(tile - t.tile_start[j], FORM != kWeightGrad ? (rows + kTile - 1) / kTile : a.MT, r.m, r.n);
-  r.e = j - 1;
-  r.row_end = t.row[j + 1];
-  if (FORM != kWeightGrad) {
-    r.row0 = t.row[j] + r.m * kTile;
-    r.ks = (j == 0 || j == a.E + 1) ? 0 : a.KS;
-  } else {
-    r.row0 = t.row[j];
-    r.ks = (rows + kSK - 1) / kSK;
-  }
-  return r;
-}
-
-// The stages of a tile: one after another into one accumulator, or (SPLIT) each into an accumulator
-// of its own, once for each pair of planes, the small products first.
-template <bool SPLIT>
-struct Passes {
-  static constexpr int kPairs = 6;
-  int step;
-  __device__ __forceinline__ explicit Passes(int ks) : step(SPLIT ? 1 : (ks > 0 ? ks : 1)) {}
-  __device__ __forceinline__ int stages() const { return SPLIT ? kPairs : step; }
-  // Stage i of them: its offset in contraction stages, and the planes (0 high, 1 middle, 2 low).
-  __device__ __forceinline__ int at(int i, int& pa, int& pb) const {
-    pa = pb = 0;
-    if (!SPLIT) return i;
-    pa = (0x001102 >> (4 * i)) & 15;   // l, h, m, m, h, h
-    pb = (0x010120 >> (4 * i)) & 15;   // h, l, m, h, m, h
-    return 0;
-  }
-};
-
 // Whether a stage with `left` rows of its segment ends inside the 16 rows of an MMA.
 __device__ __forceinline__ bool has_tail(int left) { return left < kSK && (left & 15) != 0; }
 
-template <int FORM, bool SPLIT>
+template <int FORM>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     grad_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_a32,
                      const __grid_constant__ CUtensorMap tm_b, const __grid_constant__ CUtensorMap tm_out,
@@ -173,7 +97,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const int segs = a.E + 2;
   if (warp == 0)
     scan_tiles(&bars->seg, segs, lane, [&](int j) {
-      if (FORM != kWeightGrad) return (bars->seg.row[j + 1] - bars->seg.row[j] + kTile - 1) / kTile * a.raster.nb;
+      if (FORM != kGradWeight) return (bars->seg.row[j + 1] - bars->seg.row[j] + kTile - 1) / kTile * a.raster.nb;
       return j == 0 || j == a.E + 1 ? 0 : a.MT * a.raster.nb;
     });
   if (tid == 0 && bars->seg.bad && blockIdx.x == 0) report_error(a.err, kErrBadArg, kSite + 1);
@@ -193,74 +117,67 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     int hint = 0;
     bool ok = true;
     for (int tile = first; tile < total && ok; tile += stride) {
-      const Tile t = tile_at<FORM>(seg, a, tile, hint);
+      const Tile t = tile_at<FORM, kSK>(seg, a, tile, hint);
       const int c0 = t.n * a.width + (int)rank * (a.width / 2);   // first column of B
-      const int m0 = (FORM != kWeightGrad ? t.row0 : t.m * kTile) + (int)rank * kCta;
+      const int m0 = (FORM != kGradWeight ? t.row0 : t.m * kTile) + (int)rank * kCta;
       int boxes = 4;   // input gradient: 32-row boxes of dy that hold this CTA's rows
-      if (FORM != kWeightGrad) {
+      if (FORM != kGradWeight) {
         const int rows = t.row_end - m0;
         boxes = rows <= 0 ? 0 : (rows >= kCta ? 4 : (rows + 31) >> 5);
       }
       const bool wide = a.width == kTile;
       const uint32_t b_bytes = wide ? kOperand : kChunk;
-      const Passes<SPLIT> ps(t.ks);
-      for (int ks0 = 0; ks0 < t.ks && ok; ks0 += ps.step) {
-        const int n = ps.stages();
-        for (int i = 0; i < n; ++i, st.next()) {
-          ok = warp_wait(&bars->empty[st.i], st.phase ^ 1u, a.err, abort_flag, kSite + 2);
-          if (!ok) break;
-          int pa, pb;   // planes of the operands
-          const int ks = ks0 + ps.at(i, pa, pb);
-          if (elect_one()) {
-            uint8_t* sa = base + st.i * kStageBytes;
-            uint8_t* sb = sa + kOperand;
-            const uint32_t bar = full_addr + st.i * 8;
-            if (FORM != kWeightGrad) {
-              const int y = m0 + pa * (int)a.R;
-              const int blocks = a.N - ks * kSK > 64 ? 2 : 1;
-              const uint32_t b_block = (uint32_t)a.width * 64u;   // product: width / 2 rows of 64 values
-              mbar_arrive_expect_tx_cluster(
-                  bar, (uint32_t)(blocks * boxes) * 4096u + (FORM == kProduct ? blocks * b_block : b_bytes));
-              for (int h = 0; h < blocks; ++h) {
-                const int x = ks * kSK + h * 64;
-                if (boxes == 4) {
-                  tma_load_2d_pair(sa + h * kChunk, &tm_a, bar, x, y);
-                } else {
-                  for (int b = 0; b < boxes; ++b)
-                    tma_load_2d_pair(sa + h * kChunk + b * 4096, &tm_a32, bar, x, y + b * 32);
-                }
-              }
-              if (FORM == kProduct) {
-                for (int h = 0; h < blocks; ++h)
-                  tma_load_3d_pair(sb + h * b_block, &tm_b, bar, ks * kSK + h * 64, c0, t.e + pb * a.E);
+      for (int ks = 0; ks < t.ks; ++ks, st.next()) {
+        ok = warp_wait(&bars->empty[st.i], st.phase ^ 1u, a.err, abort_flag, kSite + 2);
+        if (!ok) break;
+        if (elect_one()) {
+          uint8_t* sa = base + st.i * kStageBytes;
+          uint8_t* sb = sa + kOperand;
+          const uint32_t bar = full_addr + st.i * 8;
+          if (FORM != kGradWeight) {
+            const int blocks = a.N - ks * kSK > 64 ? 2 : 1;
+            const uint32_t b_block = (uint32_t)a.width * 64u;   // product: width / 2 rows of 64 values
+            mbar_arrive_expect_tx_cluster(
+                bar, (uint32_t)(blocks * boxes) * 4096u + (FORM == kGradProduct ? blocks * b_block : b_bytes));
+            for (int h = 0; h < blocks; ++h) {
+              const int x = ks * kSK + h * 64;
+              if (boxes == 4) {
+                tma_load_2d_pair(sa + h * kChunk, &tm_a, bar, x, m0);
               } else {
-                tma_load_3d_pair(sb, &tm_b, bar, c0, ks * kSK, t.e + pb * a.E);
-                if (wide) tma_load_3d_pair(sb + kChunk, &tm_b, bar, c0 + 64, ks * kSK, t.e + pb * a.E);
+                for (int b = 0; b < boxes; ++b)
+                  tma_load_2d_pair(sa + h * kChunk + b * 4096, &tm_a32, bar, x, m0 + b * 32);
+              }
+            }
+            if (FORM == kGradProduct) {
+              for (int h = 0; h < blocks; ++h)
+                tma_load_3d_pair(sb + h * b_block, &tm_b, bar, ks * kSK + h * 64, c0, t.e);
+            } else {
+              tma_load_3d_pair(sb, &tm_b, bar, c0, ks * kSK, t.e);
+              if (wide) tma_load_3d_pair(sb + kChunk, &tm_b, bar, c0 + 64, ks * kSK, t.e);
+            }
+          } else {
+            const int r = t.row0 + ks * kSK;
+            const int left = t.row_end - r;
+            const int halves = left > 64 ? 2 : 1;   // 64-row boxes that hold rows of the segment
+            const uint32_t bytes = (uint32_t)halves * (kOperand + b_bytes) / 2;
+            if (has_tail(left)) {
+              uint64_t* own = &bars->tail[st.i];
+              mbar_arrive_expect_tx(own, bytes);
+              for (int h = 0; h < halves; ++h) {
+                uint8_t *da = sa + h * (kChunk / 2), *db = sb + h * (kChunk / 2);
+                tma_load_2d(da, &tm_a, own, m0, r + h * 64);
+                tma_load_2d(da + kChunk, &tm_a, own, m0 + 64, r + h * 64);
+                tma_load_2d(db, &tm_b, own, c0, r + h * 64);
+                if (wide) tma_load_2d(db + kChunk, &tm_b, own, c0 + 64, r + h * 64);
               }
             } else {
-              const int r = t.row0 + ks * kSK, ra = r + pa * (int)a.R, rb = r + pb * (int)a.R;
-              const int left = t.row_end - r;
-              const int halves = left > 64 ? 2 : 1;   // 64-row boxes that hold rows of the segment
-              const uint32_t bytes = (uint32_t)halves * (kOperand + b_bytes) / 2;
-              if (has_tail(left)) {
-                uint64_t* own = &bars->tail[st.i];
-                mbar_arrive_expect_tx(own, bytes);
-                for (int h = 0; h < halves; ++h) {
-                  uint8_t *da = sa + h * (kChunk / 2), *db = sb + h * (kChunk / 2);
-                  tma_load_2d(da, &tm_a, own, m0, ra + h * 64);
-                  tma_load_2d(da + kChunk, &tm_a, own, m0 + 64, ra + h * 64);
-                  tma_load_2d(db, &tm_b, own, c0, rb + h * 64);
-                  if (wide) tma_load_2d(db + kChunk, &tm_b, own, c0 + 64, rb + h * 64);
-                }
-              } else {
-                mbar_arrive_expect_tx_cluster(bar, bytes);
-                for (int h = 0; h < halves; ++h) {
-                  uint8_t *da = sa + h * (kChunk / 2), *db = sb + h * (kChunk / 2);
-                  tma_load_2d_pair(da, &tm_a, bar, m0, ra + h * 64);
-                  tma_load_2d_pair(da + kChunk, &tm_a, bar, m0 + 64, ra + h * 64);
-                  tma_load_2d_pair(db, &tm_b, bar, c0, rb + h * 64);
-                  if (wide) tma_load_2d_pair(db + kChunk, &tm_b, bar, c0 + 64, rb + h * 64);
-                }
+              mbar_arrive_expect_tx_cluster(bar, bytes);
+              for (int h = 0; h < halves; ++h) {
+                uint8_t *da = sa + h * (kChunk / 2), *db = sb + h * (kChunk / 2);
+                tma_load_2d_pair(da, &tm_a, bar, m0, r + h * 64);
+                tma_load_2d_pair(da + kChunk, &tm_a, bar, m0 + 64, r + h * 64);
+                tma_load_2d_pair(db, &tm_b, bar, c0, r + h * 64);
+                if (wide) tma_load_2d_pair(db + kChunk, &tm_b, bar, c0 + 64, r + h * 64);
               }
             }
           }
@@ -272,11 +189,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer
     if (leader) {
-      const uint32_t idesc = idesc_f16kind_f32(kTile, a.width, a.f16) | (FORM == kProduct ? 0u : kIdescBMajorMN) |
-                             (FORM == kWeightGrad ? kIdescAMajorMN : 0u);
+      const uint32_t idesc = idesc_f16kind_f32(kTile, a.width, a.f16) | (FORM == kGradProduct ? 0u : kIdescBMajorMN) |
+                             (FORM == kGradWeight ? kIdescAMajorMN : 0u);
       // descriptors count 16 bytes
-      const uint64_t adesc0 = FORM != kWeightGrad ? sdesc_k_sw128(smem_u32(base)) : sdesc_mn_sw128(smem_u32(base), kChunk);
-      const uint64_t bdesc0 = FORM == kProduct ? sdesc_k_sw128(smem_u32(base) + kOperand)
+      const uint64_t adesc0 = FORM != kGradWeight ? sdesc_k_sw128(smem_u32(base)) : sdesc_mn_sw128(smem_u32(base), kChunk);
+      const uint64_t bdesc0 = FORM == kGradProduct ? sdesc_k_sw128(smem_u32(base) + kOperand)
                                                : sdesc_mn_sw128(smem_u32(base) + kOperand, kChunk);
       const uint32_t b_step = (uint32_t)a.width * 4u;   // product: the next 64 contraction values
       Ring<kStages> st;
@@ -284,31 +201,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       int hint = 0;
       bool ok = true;
       for (int tile = first; tile < total && ok; tile += stride) {
-        const Tile t = tile_at<FORM>(seg, a, tile, hint);
-        const Passes<SPLIT> ps(t.ks);
-        const int depth = FORM != kWeightGrad ? a.N : t.row_end - t.row0;
-        for (int ks0 = 0; ks0 < t.ks && ok; ks0 += ps.step) {
+        const Tile t = tile_at<FORM, kSK>(seg, a, tile, hint);
+        const int depth = FORM != kGradWeight ? a.N : t.row_end - t.row0;
+        if (t.ks != 0) {
           ok = warp_wait(&bars->acc_empty[ac.i], ac.phase ^ 1u, a.err, abort_flag, kSite + 4);
           if (!ok) break;
           const uint32_t d = tmem + ac.i * kTile;
-          const int n = ps.stages();
-          for (int i = 0; i < n; ++i, st.next()) {
+          for (int ks = 0; ks < t.ks; ++ks, st.next()) {
             ok = warp_wait(&bars->full[st.i], st.phase, a.err, abort_flag, kSite + 6);
             if (!ok) break;
             tc_fence_after();
-            int pa, pb;
-            const int left = depth - (ks0 + ps.at(i, pa, pb)) * kSK;
+            const int left = depth - ks * kSK;
             if (elect_one()) {
               const uint64_t ad = adesc0 + st.i * (kStageBytes >> 4), bd = bdesc0 + st.i * (kStageBytes >> 4);
 #pragma unroll
               for (int kk = 0; kk < kSK / 16; ++kk) {
                 // 16 contraction values: 32 bytes of the lines of a K-major block, or 16 lines
-                const uint32_t step = FORM != kWeightGrad ? (kk >> 2) * (kChunk >> 4) + (kk & 3) * 2 : kk * 128;
-                const uint32_t bstep = FORM == kProduct ? (kk >> 2) * b_step + (kk & 3) * 2 : kk * 128;
-                if (kk * 16 < left) mma_ss_pair(d, ad + step, bd + bstep, idesc, (i | kk) != 0 ? 1u : 0u);
+                const uint32_t step = FORM != kGradWeight ? (kk >> 2) * (kChunk >> 4) + (kk & 3) * 2 : kk * 128;
+                const uint32_t bstep = FORM == kGradProduct ? (kk >> 2) * b_step + (kk & 3) * 2 : kk * 128;
+                if (kk * 16 < left) mma_ss_pair(d, ad + step, bd + bstep, idesc, (ks | kk) != 0 ? 1u : 0u);
               }
               mma_commit_pair(&bars->empty[st.i]);
-              if (i == n - 1) mma_commit_pair(&bars->acc_full[ac.i]);
+              if (ks == t.ks - 1) mma_commit_pair(&bars->acc_full[ac.i]);
             }
             __syncwarp();
           }
@@ -320,35 +234,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     }
   } else if (warp == 2) {
     // ------------------------------------------------------------------ segment tails
-    if (FORM == kWeightGrad) {
+    if (FORM == kGradWeight) {
       Ring<kStages> st;
       uint32_t tail_parity = 0;   // a bit per stage
       int hint = 0;
       bool ok = true;
       for (int tile = first; tile < total && ok; tile += stride) {
-        const Tile t = tile_at<FORM>(seg, a, tile, hint);
-        const Passes<SPLIT> ps(t.ks);
+        const Tile t = tile_at<FORM, kSK>(seg, a, tile, hint);
         const int left = t.row_end - t.row0 - (t.ks - 1) * kSK;   // rows of the last stage
-        for (int ks0 = 0; ks0 < t.ks && ok; ks0 += ps.step) {
-          const int n = ps.stages();
-          for (int i = 0; i < n && ok; ++i, st.next()) {
-            int pa, pb;
-            if (ks0 + ps.at(i, pa, pb) != t.ks - 1 || !has_tail(left)) continue;
-            ok = warp_wait(&bars->tail[st.i], tail_parity >> st.i & 1u, a.err, abort_flag, kSite + 8);
-            if (!ok) break;
-            tail_parity ^= 1u << st.i;
-            // contraction rows [left, next multiple of 16) of the four chunks; a row is one
-            // 128-byte line, which the swizzle only permutes
-            const int m = (16 - (left & 15)) * 8;
-            uint8_t* at = base + st.i * kStageBytes + left * 128;
-            for (int k = lane; k < 4 * m; k += 32) {
-              const int c = k / m;
-              *reinterpret_cast<uint4*>(at + c * kChunk + (k - c * m) * 16) = make_uint4(0, 0, 0, 0);
-            }
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(mapa_u32(&bars->full[st.i], 0));
+        for (int ks = 0; ks < t.ks && ok; ++ks, st.next()) {
+          if (ks != t.ks - 1 || !has_tail(left)) continue;
+          ok = warp_wait(&bars->tail[st.i], tail_parity >> st.i & 1u, a.err, abort_flag, kSite + 8);
+          if (!ok) break;
+          tail_parity ^= 1u << st.i;
+          // contraction rows [left, next multiple of 16) of the four chunks; a row is one
+          // 128-byte line, which the swizzle only permutes
+          const int m = (16 - (left & 15)) * 8;
+          uint8_t* at = base + st.i * kStageBytes + left * 128;
+          for (int k = lane; k < 4 * m; k += 32) {
+            const int c = k / m;
+            *reinterpret_cast<uint4*>(at + c * kChunk + (k - c * m) * 16) = make_uint4(0, 0, 0, 0);
           }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(mapa_u32(&bars->full[st.i], 0));
         }
       }
     }
@@ -357,99 +266,62 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const int q = warp & 3, half = (warp - kEpiWarp0) >> 2;
     const uint32_t lane_base = (uint32_t)(q * 32) << 16;
     const uint32_t empty_addr = mapa_u32(&bars->acc_empty[0], 0);
-    const int odt = SPLIT ? LMOE_DTYPE_F32 : a.out_dtype;   // planes come from fp32
+    const int odt = a.out_dtype;
     const int64_t pitch = (int64_t)a.K * (odt == LMOE_DTYPE_F32 ? 4 : 2);
     uint8_t* stage = store_stage + (warp - kEpiWarp0) * kBlockBytes;
     Ring<kAcc> ac;
     int hint = 0;
     bool ok = true;
     for (int tile = first; tile < total; tile += stride) {
-      const Tile t = tile_at<FORM>(seg, a, tile, hint);
+      const Tile t = tile_at<FORM, kSK>(seg, a, tile, hint);
       // the warp's 32 rows, and the first of its half of the columns
       const int r = (int)rank * kCta + q * 32;
-      const int left = FORM != kWeightGrad ? t.row_end - t.row0 - r : a.N - t.m * kTile - r;
+      const int left = FORM != kGradWeight ? t.row_end - t.row0 - r : a.N - t.m * kTile - r;
       const int rows = left < 32 ? left : 32;
-      const int64_t row = FORM != kWeightGrad ? (int64_t)t.row0 + r : (int64_t)t.e * a.N + t.m * kTile + r;
+      const int64_t row = FORM != kGradWeight ? (int64_t)t.row0 + r : (int64_t)t.e * a.N + t.m * kTile + r;
       uint8_t* out = static_cast<uint8_t*>(a.out) + row * pitch;
       const int cols = a.width / 2;
       const int c0 = t.n * a.width + half * cols;
       const uint32_t col0 = tmem + lane_base + half * cols;
       // whole 32-row blocks leave by TMA; a weight gradient's rows behind N are cut by the tensor map
-      const bool whole = a.store != kStoreStaged && (FORM == kWeightGrad ? rows > 0 : rows == 32);
-      const int y = FORM == kWeightGrad ? t.m * kTile + r : (int)row, z = FORM == kWeightGrad ? t.e : 0;
-      if constexpr (SPLIT) {
-        float f[4][32];
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-          for (int i = 0; i < 32; ++i) f[j][i] = 0.0f;
-        for (int ks0 = 0; ks0 < t.ks && ok; ++ks0) {
-          ok = warp_wait(&bars->acc_full[ac.i], ac.phase, a.err, abort_flag, kSite + 9);
-          if (!ok) break;
-          tc_fence_after();
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            if (j * 16 >= cols) break;
-            uint32_t u[16];
-            tmem_ld16(col0 + ac.i * kTile + j * 16, u);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              float& v = f[j >> 1][(j & 1) * 16 + i];
-              v = __fadd_rn(v, __uint_as_float(u[i]));
-            }
-          }
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(empty_addr + ac.i * 8);
-          ac.next();
-        }
+      const bool whole = a.store != kStoreStaged && (FORM == kGradWeight ? rows > 0 : rows == 32);
+      const int y = FORM == kGradWeight ? t.m * kTile + r : (int)row, z = FORM == kGradWeight ? t.e : 0;
+      if (t.ks != 0) {
+        ok = warp_wait(&bars->acc_full[ac.i], ac.phase, a.err, abort_flag, kSite + 9);
         if (!ok) break;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (j * 32 >= cols || c0 + j * 32 >= a.K) break;
-          if (whole)
-            store_block<128>(&tm_out, f[j], odt, stage, lane, c0 + j * 32, y, z);
-          else
-            store_rows(out, pitch, rows, c0 + j * 32, a.K, f[j], odt, a.store, stage, lane);
-        }
-      } else {
+        tc_fence_after();
+      }
+      for (int j = 0; j < cols; j += 64) {
+        float f[64];
         if (t.ks != 0) {
-          ok = warp_wait(&bars->acc_full[ac.i], ac.phase, a.err, abort_flag, kSite + 9);
-          if (!ok) break;
-          tc_fence_after();
+          uint32_t u[32], v[32];
+          tmem_ld32x2(col0 + ac.i * kTile + j, col0 + ac.i * kTile + j + 32, u, v);
+          if (j + 64 == cols) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(empty_addr + ac.i * 8);
+            ac.next();
+          }
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            f[i] = __uint_as_float(u[i]);
+            f[32 + i] = __uint_as_float(v[i]);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 64; ++i) f[i] = 0.0f;
         }
-        for (int j = 0; j < cols; j += 64) {
-          float f[64];
-          if (t.ks != 0) {
-            uint32_t u[32], v[32];
-            tmem_ld32x2(col0 + ac.i * kTile + j, col0 + ac.i * kTile + j + 32, u, v);
-            if (j + 64 == cols) {
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive_cluster(empty_addr + ac.i * 8);
-              ac.next();
-            }
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              f[i] = __uint_as_float(u[i]);
-              f[32 + i] = __uint_as_float(v[i]);
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < 64; ++i) f[i] = 0.0f;
-          }
-          const int c = c0 + j;
-          if (c >= a.K) continue;
-          if (whole && odt != LMOE_DTYPE_F32) {
-            store_block<128>(&tm_out, f, odt, stage, lane, c, y, z);
-          } else if (whole) {
-            store_block<128>(&tm_out, f, odt, stage, lane, c, y, z);
-            if (c + 32 < a.K) store_block<128>(&tm_out, f + 32, odt, stage, lane, c + 32, y, z);
-          } else {
-            store_rows(out, pitch, rows, c, a.K, reinterpret_cast<const float(&)[32]>(f[0]), odt, a.store, stage, lane);
-            store_rows(out, pitch, rows, c + 32, a.K, reinterpret_cast<const float(&)[32]>(f[32]), odt, a.store, stage,
-                         lane);
-          }
+        const int c = c0 + j;
+        if (c >= a.K) continue;
+        if (whole && odt != LMOE_DTYPE_F32) {
+          store_block<128>(&tm_out, f, odt, stage, lane, c, y, z);
+        } else if (whole) {
+          store_block<128>(&tm_out, f, odt, stage, lane, c, y, z);
+          if (c + 32 < a.K) store_block<128>(&tm_out, f + 32, odt, stage, lane, c + 32, y, z);
+        } else {
+          store_rows(out, pitch, rows, c, a.K, reinterpret_cast<const float(&)[32]>(f[0]), odt, a.store, stage, lane);
+          store_rows(out, pitch, rows, c + 32, a.K, reinterpret_cast<const float(&)[32]>(f[32]), odt, a.store, stage,
+                       lane);
         }
       }
     }
@@ -488,89 +360,22 @@ int pad_rows(const void* src, int64_t rows, int cols, int pitch, void* dst, cons
   return cuda_status(cudaGetLastError());
 }
 
-template <int FORM, bool SPLIT>
+template <int FORM>
 int launch(const CUtensorMap& ta, const CUtensorMap& ta32, const CUtensorMap& tb, const CUtensorMap& to,
            const GradArgs& a, int grid, cudaStream_t stream) {
   constexpr size_t smem = kStages * kStageBytes + kEpiWarps * kBlockBytes + sizeof(Bars);
   static_assert(smem <= 232448, "shared memory budget");
-  auto fn = grad_gemm_kernel<FORM, SPLIT>;
+  auto fn = grad_gemm_kernel<FORM>;
   const int st = set_max_dynamic_smem(reinterpret_cast<const void*>(fn), smem);
   if (st != LMOE_OK) return st;
   fn<<<grid, kThreads, smem, stream>>>(ta, ta32, tb, to, a);
   return cuda_status(cudaGetLastError());
 }
 
-// The three planes of src [rows, cols] fp32: dst [3][rows, pitch] bf16, zero behind the columns.
-// Rounding each remainder to nearest leaves at most 2^-27 of the value; values that would round to
-// an infinity are cut instead, values that are not finite stay in the high plane.
-__global__ void __launch_bounds__(256) split_rows_kernel(const float* __restrict__ src, int64_t rows, int cols,
-                                                         int pitch, int vec, uint4* __restrict__ dst) {
-  const int per = pitch / 8;
-  const int64_t total = rows * per;
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t r = i / per;
-    const int c = (int)(i - r * per) * 8;
-    const float* p = src + r * cols + c;
-    float v[8];
-    if (vec) {
-      const float4 x = __ldg(reinterpret_cast<const float4*>(p)), y = __ldg(reinterpret_cast<const float4*>(p) + 1);
-      v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w, v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = c + j < cols ? __ldg(p + j) : 0.0f;
-    }
-    uint32_t w[3][4];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      uint32_t b[3];
-      const uint32_t bits = __float_as_uint(v[j]);
-      __nv_bfloat16 h = __float2bfloat16_rn(v[j]);
-      if ((bits & 0x7f800000u) == 0x7f800000u) {
-        b[1] = b[2] = 0u;
-      } else {
-        if ((__bfloat16_as_ushort(h) & 0x7f80u) == 0x7f80u) h = __float2bfloat16_rz(v[j]);
-        const float e = __fsub_rn(v[j], __bfloat162float(h));   // exact
-        const __nv_bfloat16 m = __float2bfloat16_rn(e);
-        b[1] = __bfloat16_as_ushort(m);
-        b[2] = __bfloat16_as_ushort(__float2bfloat16_rn(__fsub_rn(e, __bfloat162float(m))));
-      }
-      b[0] = __bfloat16_as_ushort(h);
-#pragma unroll
-      for (int k = 0; k < 3; ++k) w[k][j >> 1] = (j & 1) ? w[k][j >> 1] | b[k] << 16 : b[k];
-    }
-#pragma unroll
-    for (int k = 0; k < 3; ++k) dst[k * total + i] = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
-  }
-}
-
-int split_rows(const void* src, int64_t rows, int cols, int pitch, void* dst, const DeviceInfo& dev, cudaStream_t s) {
-  const int64_t blocks = (rows * (pitch / 8) + 255) / 256, most = (int64_t)dev.num_sms * 8;
-  split_rows_kernel<<<(unsigned)(blocks < most ? blocks : most), 256, 0, s>>>(
-      static_cast<const float*>(src), rows, cols, pitch, cols % 8 == 0 && aligned16(src), static_cast<uint4*>(dst));
-  return cuda_status(cudaGetLastError());
-}
-
-inline int64_t pitch8(int64_t cols) { return (cols + 7) / 8 * 8; }
-inline size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
-inline bool weight_grad(const GradProblem& p) { return p.form == kGradWeight; }
-// Rows and columns of the second operand.
-inline int64_t other_rows(const GradProblem& p) {
-  return weight_grad(p) ? p.total_rows : (int64_t)p.num_experts * (p.form == kGradProduct ? p.K : p.N);
-}
-inline int other_cols(const GradProblem& p) { return p.form == kGradProduct ? p.N : p.K; }
-
 }  // namespace
 
-bool grad_splits(const GradProblem& p) {
-  if (p.dtype != LMOE_DTYPE_F32 || p.total_rows * 3 > INT32_MAX) return false;
-  return p.total_rows >= (int64_t)p.num_experts * (weight_grad(p) ? kSplitRowsW : kSplitRowsX);
-}
-
 size_t grad_gemm_workspace(const GradProblem& p) {
-  if (p.dtype == LMOE_DTYPE_F32) {
-    if (!grad_splits(p)) return 0;
-    return align256((size_t)p.total_rows * pitch8(p.N) * 6) + align256((size_t)other_rows(p) * pitch8(other_cols(p)) * 6);
-  }
+  if (p.dtype == LMOE_DTYPE_F32) return grad_split_workspace(p);
   size_t b = 0;
   if (p.N % 8) b += align256((size_t)p.total_rows * pitch8(p.N) * 2);
   if (other_cols(p) % 8) b += align256((size_t)other_rows(p) * pitch8(other_cols(p)) * 2);
@@ -586,82 +391,49 @@ int run_grad_gemm(const GradProblem& p, cudaStream_t stream) {
   const void* other = p.other;
   const int64_t ldy = pitch8(p.N), ldo = pitch8(other_cols(p));
   uint8_t* ws = static_cast<uint8_t*>(p.workspace);
-  const bool split = p.dtype == LMOE_DTYPE_F32;
-  if (split) {
-    st = split_rows(p.dy, p.total_rows, p.N, (int)ldy, ws, dev, stream);
-    if (st != LMOE_OK) return st;
-    dy = ws;
-    ws += align256((size_t)p.total_rows * ldy * 6);
-    st = split_rows(p.other, other_rows(p), other_cols(p), (int)ldo, ws, dev, stream);
-    if (st != LMOE_OK) return st;
-    other = ws;
-  }
-  if (!split && ldy != p.N) {
+  if (ldy != p.N) {
     st = pad_rows(p.dy, p.total_rows, p.N, (int)ldy, ws, dev, stream);
     if (st != LMOE_OK) return st;
     dy = ws;
     ws += align256((size_t)p.total_rows * ldy * 2);
   }
-  if (!split && ldo != other_cols(p)) {
+  if (ldo != other_cols(p)) {
     st = pad_rows(p.other, other_rows(p), other_cols(p), (int)ldo, ws, dev, stream);
     if (st != LMOE_OK) return st;
     other = ws;
   }
   GradArgs a = {};
-  a.offsets = p.offsets;
-  a.offsets_i64 = p.offsets_i64;
-  a.E = p.num_experts;
-  a.N = p.N;
-  a.K = p.K;
-  a.R = p.total_rows;
-  a.MT = (p.N + kTile - 1) / kTile;
-  a.KS = (p.N + kSK - 1) / kSK;
-  a.f16 = p.dtype == LMOE_DTYPE_F16;
-  a.out = p.out;
-  a.out_dtype = p.out_dtype;
-  a.store = store_mode(p.out, p.K, p.out_dtype);
-  a.err = p.err;
-  const CUtensorMapDataType dt = a.f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   CUtensorMap ta, ta32, tb, to = {};
-  if (a.store != kStoreStaged) {
-    const bool wg = weight_grad(p);
-    st = encode_store_map(&to, p.out, p.out_dtype, (uint64_t)p.K, wg ? (uint64_t)p.N : (uint64_t)p.total_rows,
-                          wg ? (uint64_t)p.num_experts : 1, 128);
-    if (st != LMOE_OK) return st;
-  }
+  st = fill_args(p, kSK, a, to);
+  if (st != LMOE_OK) return st;
+  const CUtensorMapDataType dt = a.f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   const int grid = gemm_grid(dev) < 2 ? 2 : gemm_grid(dev) & ~1;   // whole pairs
   const int64_t row_tiles = weight_grad(p) ? (int64_t)a.MT * p.num_experts
                                           : even_row_tiles(p.total_rows, p.num_experts, kTile);
   const int widths[] = {256, 128};
   a.width = pick_width(widths, grid / 2, 0, 16, [&](int w) { return row_tiles * ((p.K + w - 1) / w); });
   a.raster = Raster((p.K + a.width - 1) / a.width);
-  // the maps end at the true sizes, so that TMA fills what lies behind them with zeros; the planes
-  // of split operands follow one another along the rows (or the experts)
-  const uint64_t planes = split ? 3 : 1;
+  // the maps end at the true sizes, so that TMA fills what lies behind them with zeros
   if (weight_grad(p)) {
-    st = encode_tmap_2d(&ta, dy, dt, 2, planes * p.total_rows, (uint64_t)p.N, (uint64_t)ldy * 2, 64, 64, true);
+    st = encode_tmap_2d(&ta, dy, dt, 2, (uint64_t)p.total_rows, (uint64_t)p.N, (uint64_t)ldy * 2, 64, 64, true);
     if (st != LMOE_OK) return st;
-    st = encode_tmap_2d(&tb, other, dt, 2, planes * p.total_rows, (uint64_t)p.K, (uint64_t)ldo * 2, 64, 64, true);
+    st = encode_tmap_2d(&tb, other, dt, 2, (uint64_t)p.total_rows, (uint64_t)p.K, (uint64_t)ldo * 2, 64, 64, true);
     if (st != LMOE_OK) return st;
-    return split ? launch<kWeightGrad, true>(ta, ta, tb, to, a, grid, stream)
-                 : launch<kWeightGrad, false>(ta, ta, tb, to, a, grid, stream);
+    return launch<kGradWeight>(ta, ta, tb, to, a, grid, stream);
   }
-  st = encode_tmap_2d(&ta, dy, dt, 2, planes * p.total_rows, (uint64_t)p.N, (uint64_t)ldy * 2, kCta, 64, true);
+  st = encode_tmap_2d(&ta, dy, dt, 2, (uint64_t)p.total_rows, (uint64_t)p.N, (uint64_t)ldy * 2, kCta, 64, true);
   if (st != LMOE_OK) return st;
-  st = encode_tmap_2d(&ta32, dy, dt, 2, planes * p.total_rows, (uint64_t)p.N, (uint64_t)ldy * 2, 32, 64, true);
+  st = encode_tmap_2d(&ta32, dy, dt, 2, (uint64_t)p.total_rows, (uint64_t)p.N, (uint64_t)ldy * 2, 32, 64, true);
   if (st != LMOE_OK) return st;
   const bool product = p.form == kGradProduct;
   const uint64_t rows = (uint64_t)(product ? p.K : p.N);   // of one expert's matrix
-  const uint64_t dims[3] = {(uint64_t)other_cols(p), rows, planes * p.num_experts};
+  const uint64_t dims[3] = {(uint64_t)other_cols(p), rows, (uint64_t)p.num_experts};
   const uint64_t strides[2] = {(uint64_t)ldo * 2, (uint64_t)ldo * 2 * rows};
   const uint32_t box[3] = {64, product ? (uint32_t)a.width / 2 : (uint32_t)kSK, 1};
   st = encode_tmap_3d(&tb, other, dt, 2, dims, strides, box);
   if (st != LMOE_OK) return st;
-  if (product)
-    return split ? launch<kProduct, true>(ta, ta32, tb, to, a, grid, stream)
-                 : launch<kProduct, false>(ta, ta32, tb, to, a, grid, stream);
-  return split ? launch<kInputGrad, true>(ta, ta32, tb, to, a, grid, stream)
-               : launch<kInputGrad, false>(ta, ta32, tb, to, a, grid, stream);
+  return product ? launch<kGradProduct>(ta, ta32, tb, to, a, grid, stream)
+                 : launch<kGradInput>(ta, ta32, tb, to, a, grid, stream);
 }
 
 }  // namespace lmoe
@@ -691,7 +463,7 @@ int grad_entry(GradProblem& p, const void* offsets, void* out, void* workspace, 
   const size_t need = grad_gemm_workspace(p);
   if (need && (!workspace || workspace_bytes < need || !aligned16(workspace))) return LMOE_ERR_WORKSPACE;
   p.workspace = workspace;
-  return run_grad_gemm(p, stream);
+  return p.dtype == LMOE_DTYPE_F32 ? run_grad_split(p, stream) : run_grad_gemm(p, stream);
 }
 
 }  // namespace

@@ -1,5 +1,6 @@
-// grad_gemm.h -- internal interface of the grouped product's gradients and the product of any row length (grad_gemm.cu on tensor
-// cores, grad_f32.cu for fp32 operands on CUDA cores).
+// grad_gemm.h -- internal interface of the grouped product's gradients and the product of any row
+// length (grad_gemm.cu for 16-bit operands; for fp32 grad_split.cu on tensor cores and grad_f32.cu
+// on CUDA cores).
 #pragma once
 #include <cuda_runtime.h>
 
@@ -30,9 +31,11 @@ struct GradProblem {
 };
 
 size_t grad_gemm_workspace(const GradProblem& p);
+int run_grad_gemm(const GradProblem& p, cudaStream_t stream);
 // Whether fp32 operands go to the tensor cores as three bf16 planes each.
 bool grad_splits(const GradProblem& p);
-int run_grad_gemm(const GradProblem& p, cudaStream_t stream);
+size_t grad_split_workspace(const GradProblem& p);
+int run_grad_split(const GradProblem& p, cudaStream_t stream);
 int run_grad_f32(const GradProblem& p, cudaStream_t stream);
 
 }  // namespace lmoe
