@@ -30,11 +30,10 @@ namespace lmoe {
 namespace {
 
 constexpr int kSK = 64;            // contraction values per stage
-constexpr int kStages = 2, kAcc = 2;
-constexpr int kEpiWarp0 = 4, kEpiWarps = 8, kConvWarp0 = 12, kConvWarps = 4;
+constexpr int kAcc = 2;
+constexpr int kEpiWarp0 = 4, kEpiWarps = 8, kConvWarp0 = 12, kConvWarps = 8;
 constexpr uint32_t kChunk = 64 * 128;             // 64 lines of 64 values
 constexpr uint32_t kPlane = 2 * kChunk;           // a plane of 128 rows or columns
-constexpr uint32_t kBlockBytes = 32 * 128;        // a warp's block on its way out
 constexpr uint32_t kSite = 0x700u;
 // The products of planes (0 high, 1 middle, 2 low), in their order.
 constexpr int kPairs = 6;
@@ -50,9 +49,13 @@ struct Cfg {
   static constexpr int kThreads = (kConv ? kConvWarp0 + kConvWarps : kConvWarp0) * 32;
   static constexpr uint32_t kPlaneOfB = kConv ? kChunk : kPlane;
   static constexpr uint32_t kStageBytes = 3 * (kPlane + kPlaneOfB);
+  static constexpr int kStages = kConv ? 3 : 2;
+  // a warp's block on its way out (weights converted: rows of odd lengths only)
+  static constexpr uint32_t kBlockBytes = kConv ? kStoreStageF32 : 32 * 128;
   static constexpr int kBlocks = kConv ? 2 : 4;        // blocks of 32 columns of an epilogue warp
 };
 
+template <int kStages>
 struct __align__(8) Bars {
   uint64_t full[kStages];       // leader: both CTAs' operands landed (and weights were converted)
   uint64_t empty[kStages];      // the stage's MMAs finished (both CTAs)
@@ -130,9 +133,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<FORM>::kThreads,
                       const __grid_constant__ CUtensorMap tm_b, const __grid_constant__ CUtensorMap tm_out,
                       const float* weights, int vec, const GradArgs a) {
   using C = Cfg<FORM>;
+  using B = Bars<C::kStages>;
+  constexpr int kStages = C::kStages;
+  constexpr uint32_t kBlockBytes = C::kBlockBytes;
   extern __shared__ __align__(1024) uint8_t base[];   // whole swizzle atoms
   uint8_t* store_stage = base + kStages * C::kStageBytes;
-  Bars* bars = reinterpret_cast<Bars*>(store_stage + kEpiWarps * kBlockBytes);
+  B* bars = reinterpret_cast<B*>(store_stage + kEpiWarps * kBlockBytes);
   volatile int* abort_flag = &bars->abort;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t rank = cluster_ctarank();
@@ -330,7 +336,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<FORM>::kThreads,
       const int c0 = t.n * a.width + half * cols;
       const uint32_t col0 = tmem + lane_base + half * cols;
       // whole 32-row blocks leave by TMA; a weight gradient's rows behind N are cut by the tensor map
-      const bool whole = a.store != kStoreStaged && (FORM == kGradWeight ? rows > 0 : rows == 32);
+      const bool whole = !C::kConv && a.store != kStoreStaged && (FORM == kGradWeight ? rows > 0 : rows == 32);
       const int y = FORM == kGradWeight ? t.m * kTile + r : (int)row, z = FORM == kGradWeight ? t.e : 0;
       float f[C::kBlocks][32];
 #pragma unroll
@@ -361,7 +367,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<FORM>::kThreads,
 #pragma unroll
       for (int j = 0; j < C::kBlocks; ++j) {
         if (j * 32 >= cols || c0 + j * 32 >= a.K) break;
-        if (whole)
+        if (!C::kConv && whole)
           store_block<128>(&tm_out, f[j], LMOE_DTYPE_F32, stage, lane, c0 + j * 32, y, z);
         else
           store_rows(out, pitch, rows, c0 + j * 32, a.K, f[j], LMOE_DTYPE_F32, a.store, stage, lane);
@@ -373,15 +379,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<FORM>::kThreads,
     // A stage's 64 x 64 values, a warp two rows of 64 at a time: dx 64 contraction rows of 64
     // columns, the product 64 of its columns' rows of 64 contraction values.
     const int rows_of = FORM == kGradProduct ? a.K : a.N, cols_of = FORM == kGradProduct ? a.N : a.K;
+    constexpr int kRows = 2 * kConvWarps, kPieces = 64 / kRows;   // rows at a time, values of four a lane
     const int r = (warp - kConvWarp0) * 2 + (lane >> 4), c = (lane & 15) * 4;
     const uint32_t full_addr = mapa_u32(&bars->full[0], 0);
     // its eight bytes of a line: 16-byte piece j of line r lies at j ^ (r & 7)
     uint8_t* dst = base + 3 * kPlane + r * 128 + (((lane & 15) >> 1) ^ (r & 7)) * 16 + (lane & 1) * 8;
     constexpr int kAhead = 2;
-    float4 v[kAhead][8];
+    float4 v[kAhead][kPieces];
     int pending = 0, hint = 0, ltile = first, lks = 0;   // the next load: tile and stage
     Tile lt = {};
-    auto load = [&](float4 (&b)[8]) {
+    auto load = [&](float4 (&b)[kPieces]) {
       while (lks == 0) {   // the next tile that has an expert
         if (ltile >= total) return;
         lt = tile_at<FORM, kSK>(seg, a, ltile, hint);
@@ -392,7 +399,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<FORM>::kThreads,
       const int r0 = FORM == kGradProduct ? across : along, c0 = FORM == kGradProduct ? along : across;
       const float* src = weights + (int64_t)lt.e * rows_of * cols_of;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) b[i] = load4(src, cols_of, r0 + r + 8 * i, c0 + c, rows_of, cols_of, vec);
+      for (int i = 0; i < kPieces; ++i) b[i] = load4(src, cols_of, r0 + r + kRows * i, c0 + c, rows_of, cols_of, vec);
       ++pending;
       if (++lks == lt.ks) {
         lks = 0;
@@ -408,21 +415,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<FORM>::kThreads,
       for (int j = 0; j < kAhead; ++j) {
         if (!ok || pending == 0) break;
         --pending;
+        uint32_t lo[kPieces][3], hi[kPieces][3];
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) split4(v[j][i], lo[i], hi[i]);
+        load(v[j]);
         ok = warp_wait(&bars->empty[st.i], st.phase ^ 1u, a.err, abort_flag, kSite + 10);
         if (!ok) break;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          uint32_t lo[3], hi[3];
-          split4(v[j][i], lo, hi);
+        for (int i = 0; i < kPieces; ++i)
 #pragma unroll
           for (int p = 0; p < 3; ++p)
-            *reinterpret_cast<uint2*>(dst + st.i * C::kStageBytes + p * C::kPlaneOfB + i * 1024) = make_uint2(lo[p], hi[p]);
-        }
+            *reinterpret_cast<uint2*>(dst + st.i * C::kStageBytes + p * C::kPlaneOfB + i * (kRows * 128)) =
+                make_uint2(lo[i][p], hi[i][p]);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(full_addr + st.i * 8);
         st.next();
-        load(v[j]);
       }
     }
   }
@@ -440,9 +448,9 @@ template <int FORM>
 int launch(const CUtensorMap& ta, const CUtensorMap& ta32, const CUtensorMap& tb, const CUtensorMap& to,
            const float* weights, int vec, const GradArgs& a, int grid, cudaStream_t stream) {
   using C = Cfg<FORM>;
-  constexpr size_t smem = kStages * C::kStageBytes + kEpiWarps * kBlockBytes + sizeof(Bars);
+  constexpr size_t smem = C::kStages * C::kStageBytes + kEpiWarps * C::kBlockBytes + sizeof(Bars<C::kStages>);
   static_assert(smem <= 232448, "shared memory budget");
-  static_assert(C::kStageBytes % 1024 == 0, "swizzle atoms");
+  static_assert(C::kStageBytes % 1024 == 0 && 2 * kConvWarps % 8 == 0, "swizzle atoms");
   auto fn = grad_split_kernel<FORM>;
   const int st = set_max_dynamic_smem(reinterpret_cast<const void*>(fn), smem);
   if (st != LMOE_OK) return st;

@@ -332,7 +332,7 @@ inline int store_mode(const void* out, int64_t cols, int dtype) {
   const uintptr_t a = reinterpret_cast<uintptr_t>(out) | (uintptr_t)(cols * (dtype == LMOE_DTYPE_F32 ? 4 : 2));
   return a % 32 == 0 ? kStore32 : (a % 16 == 0 ? kStore16 : kStoreStaged);
 }
-constexpr uint32_t kStoreStageBytes = 1152;   // per warp
+constexpr uint32_t kStoreStageBytes = 1152, kStoreStageF32 = 1024;   // per warp: any type, fp32
 
 // Called by a whole warp: lane l holds COLS values of row l (of `rows` valid ones) from column c0;
 // columns at or behind `cols` are not written.  Rows that start at odd addresses go through
@@ -384,15 +384,15 @@ __device__ __forceinline__ void store_rows(uint8_t* base, int64_t pitch, int row
     return;
   }
   if (dtype == LMOE_DTYPE_F32) {
-    float* st = reinterpret_cast<float*>(stage);   // [32][9]
+    float* st = reinterpret_cast<float*>(stage);   // [32][8], value j of row r at j ^ (r & 7)
 #pragma unroll
     for (int ch = 0; ch < COLS / 8; ++ch) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) st[lane * 9 + i] = v[8 * ch + i];
+      for (int i = 0; i < 8; ++i) st[lane * 8 + (i ^ (lane & 7))] = v[8 * ch + i];
       __syncwarp();
       const int c = c0 + 8 * ch + (lane & 7);
       for (int r = lane >> 3; r < rows; r += 4)
-        if (c < cols) reinterpret_cast<float*>(base + r * pitch)[c] = st[r * 9 + (lane & 7)];
+        if (c < cols) reinterpret_cast<float*>(base + r * pitch)[c] = st[r * 8 + ((lane ^ r) & 7)];
       __syncwarp();
     }
   } else {
