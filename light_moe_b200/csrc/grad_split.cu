@@ -9,7 +9,7 @@
 // accumulators in registers, rounding to nearest.
 //
 // A stage holds 64 contraction values of all planes of both operands (16 KB a plane of 128 rows or
-// columns), so that each is loaded once for its products; two stages, two accumulators.  (With a
+// columns), so that each is loaded once for its products; two or three stages, two accumulators.  (With a
 // stage for each pair of planes the copies bound it: dx of 1021 rows on 8 experts of 1024 x 2816
 // 120 us.)
 //
@@ -18,10 +18,17 @@
 // values two stages ahead into registers and write their planes into shared memory, which saves
 // writing and reading 12 bytes a weight.  Their tiles are 256 x 128, so that planes and registers
 // fit; the weight gradient's are 256 x 256 or, where the last round would leave pairs idle, 256 x
-// 128.
+// 128.  The weights' values are split before their stage is free, so that only eight-byte stores lie
+// between one stage's MMAs and the next (four warps that split them afterwards, two stages: 108
+// against 83 us for dx of 1021 rows on 8 experts of 1024 x 2816).
+//
+// The weight gradient is bound by the tensor pipe (44 us for those sizes, six products of 2 * 1021 *
+// 1024 * 2816 operations are 43 us at the rate of whole tiles); the input gradient by shared memory
+// (an MMA of 128 columns reads operands in all of its 64 cycles, the copies and planes come on top)
+// and, with few rows per expert, by the tile's empty rows.
 //
 // Warps: 0 TMA producer; 1 MMA issuer (leader CTA); 2 clears the tails of segments (weight
-// gradient); 4-11 epilogue, eight warps of 32 rows x half the columns; 12-15 weights.
+// gradient); 4-11 epilogue, eight warps of 32 rows x half the columns; 12-19 weights.
 #include <cuda_bf16.h>
 
 #include "grad_tile.cuh"
@@ -38,10 +45,6 @@ constexpr uint32_t kSite = 0x700u;
 // The products of planes (0 high, 1 middle, 2 low), in their order.
 constexpr int kPairs = 6;
 constexpr uint32_t kPlaneA = 0x001021, kPlaneB = 0x010201;   // hex digit i: of product i
-
-// fp32 operands are split from this many rows per expert on (below, the copies cost more than the
-// CUDA cores' products).
-constexpr int kSplitRowsX = 48, kSplitRowsW = 16;
 
 template <int FORM>
 struct Cfg {
@@ -485,8 +488,15 @@ int split_rows(const void* src, int64_t rows, int cols, int pitch, void* dst, co
 }  // namespace
 
 bool grad_splits(const GradProblem& p) {
+  // Beside the planes' passes and the launches (~10 us) the tensor cores win.  us on CUDA cores against
+  // planes, E x N x K: input gradient, 4 rows an expert, 8 x 32 x 256 8.4 : 12.5, 8 x 96 x 256 14.6 :
+  // 14.5, 8 x 128 x 128 18.7 : 14.5, 8 x 1024 x 2816 199 : 70 (its tiles there cost what full ones do);
+  // 64 rows, 8 x 64 x 2816 17.4 : 20.7.  Weight gradient, 64 x 128 x 512, 64 rows 22.9 : 26.9; 4 x 2048 x
+  // 2048, 1 row 27 : 33, 16 rows 29 : 28, 24 rows 41 : 29; 64 x 512 x 1024, 1 row 50 : 39.
   if (p.dtype != LMOE_DTYPE_F32 || p.total_rows * 3 > INT32_MAX) return false;
-  return p.total_rows >= (int64_t)p.num_experts * (weight_grad(p) ? kSplitRowsW : kSplitRowsX);
+  const double weights = (double)p.N * p.K, work = (double)p.total_rows * weights;
+  if (work > 1 << 28) return true;
+  return weight_grad(p) ? weights * p.num_experts > 1 << 24 : p.N >= 96;
 }
 
 size_t grad_split_workspace(const GradProblem& p) {
