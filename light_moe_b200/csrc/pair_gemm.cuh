@@ -49,35 +49,6 @@ __device__ __forceinline__ void mbar_arrive_expect_tx_cluster(uint32_t cluster_a
                "r"(bytes)
                : "memory");
 }
-__device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-// mbar_wait for a barrier that the other CTA arrives on (acquire at cluster scope).
-__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity, uint32_t* err, volatile int* abort,
-                                                  uint32_t site) {
-  if (mbar_try_wait_cluster(bar, parity)) return true;
-  const uint64_t t0 = globaltimer_ns();
-  uint32_t spins = 0;
-  while (true) {
-    if (mbar_try_wait_cluster(bar, parity)) return true;
-    if (((++spins) & 63u) == 0u) {
-      if (abort && *abort) return false;
-      if (globaltimer_ns() - t0 > kWaitBudgetNs) {
-        report_error(err, kErrTimeout, site);
-        if (abort) *abort = 1;
-        return false;
-      }
-    }
-  }
-}
 
 // Tiled loads into this CTA's shared memory that complete on a barrier of the leader CTA
 // (`bar`: its shared-cluster address).  A hand-over by a warp of each CTA would cost an arrival
