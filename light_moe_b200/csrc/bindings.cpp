@@ -164,6 +164,7 @@ torch::Tensor grouped_gemm(torch::Tensor input, torch::Tensor weights, torch::Te
   TORCH_CHECK(off.scalar_type() == torch::kInt64 || off.scalar_type() == torch::kInt32, "offsets int64/int32");
   const int64_t T = x.size(0), K = x.size(1), N = w.size(1);
   auto out = torch::empty({T, N}, x.options());
+  if (T == 0 && num_experts >= 1) return out.to(input.scalar_type());   // no rows, nothing to launch
   // row lengths that the kernels above do not take
   if (K > 0 && N > 0 && (x.scalar_type() == torch::kFloat32 ? K % 4 != 0 : K % 128 != 0)) {
     auto xa = contig16(x), wa = contig16(w);
@@ -343,6 +344,12 @@ void check_same_device(const torch::Tensor& t, const torch::Tensor& like, const 
   TORCH_CHECK(t.device() == like.device(), name, " must be on ", like.device(), ", is on ", t.device());
 }
 
+// Sizes that the kernels count in 32 bits.
+void check_sizes(int64_t rows, int64_t n, int64_t k, int64_t num_experts) {
+  TORCH_CHECK(rows <= INT32_MAX && n <= INT32_MAX && k <= INT32_MAX && num_experts <= INT32_MAX,
+              "sizes must fit 32 bits");
+}
+
 torch::Tensor check_offsets(const torch::Tensor& offsets, const torch::Tensor& like, int64_t num_experts) {
   check_same_device(offsets, like, "expert_offsets");
   TORCH_CHECK(num_experts >= 1, "num_experts must be at least 1");
@@ -370,6 +377,7 @@ torch::Tensor grouped_gemm_dgrad(torch::Tensor grad_output, torch::Tensor weight
   auto dy = contig16(grad_output);
   auto w = contig16(weights);
   const int64_t T = dy.size(0), N = w.size(1), K = w.size(2);
+  check_sizes(T, N, K, num_experts);
   auto out = torch::empty({T, K}, dy.options());
   const int dt = dtype_code(dy);
   auto ws = workspace((int64_t)lmoe_grouped_gemm_grad_workspace_bytes(0, dt, T, (int)N, (int)K, (int)num_experts), dy);
@@ -395,6 +403,7 @@ torch::Tensor grouped_gemm_wgrad(torch::Tensor grad_output, torch::Tensor input,
   auto dy = contig16(grad_output);
   auto x = contig16(input);
   const int64_t T = dy.size(0), N = dy.size(1), K = x.size(1);
+  check_sizes(T, N, K, num_experts);
   auto out = torch::empty({num_experts, N, K}, dy.options().dtype(ot));
   const int dt = dtype_code(dy);
   auto ws = workspace((int64_t)lmoe_grouped_gemm_grad_workspace_bytes(1, dt, T, (int)N, (int)K, (int)num_experts), dy);
@@ -499,17 +508,17 @@ Fp4Operand fp4_operand(const torch::Tensor& q, const torch::Tensor& s, const tor
   }
   // rows evenly spaced over all leading dimensions
   bool even = s.size(-1) == 1 || s.stride(-1) == 1;
-  int64_t pitch = 0;   // of the innermost dimension with more than one row
+  int64_t pitch = -1;   // of the innermost dimension with more than one row
   int64_t span = 0;
   for (int64_t i = s.dim() - 2; i >= 0 && even; --i) {
     if (s.size(i) == 1) continue;
-    if (!pitch)
-      pitch = s.stride(i);
+    if (pitch < 0)
+      pitch = s.stride(i);   // 0 where the rows are one broadcast row
     else
       even = s.stride(i) == span;
     span = s.stride(i) * s.size(i);
   }
-  if (!pitch) pitch = padded;
+  if (pitch < 0) pitch = padded;
   const int64_t have = (int64_t)s.storage().nbytes() - s.storage_offset();
   const bool fits = even && (reinterpret_cast<uintptr_t>(s.data_ptr()) % 32 == 0) &&
                     (pad ? pitch % 32 == 0 && pitch >= padded && (rows - 1) * pitch + padded <= have
@@ -591,6 +600,7 @@ torch::Tensor fp4_grouped_gemm(torch::Tensor input, torch::Tensor input_scales, 
     }
   }
   const int64_t T = input.size(0), K = input.size(1) * 2, N = weights.size(1);
+  check_sizes(T, N, K, num_experts);
   const float* al = fp4_alpha(alpha, input, num_experts, "alpha");
   const float* au = fp4_alpha(alpha_up, input, num_experts, "alpha_up");
   const auto ot = out_dtype.value_or(torch::kBFloat16);

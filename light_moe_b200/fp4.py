@@ -52,6 +52,8 @@ class FP4Experts:
         """Quantise dense expert weights on the GPU: w1, w3 [E, ffn, d] (gate, up), w2 [E, d, ffn];
         ``shared``: list of (w1, w3, w2) of always-on experts, as ``W4A16Experts.from_dense``."""
         E, F, d = w1.shape
+        if w3.shape != w1.shape or w2.shape != (E, d, F):
+            raise ValueError("w1 and w3 must be [E, ffn, d], w2 [E, d, ffn]")
         if d % 32 or F % 32:
             raise ValueError("hidden and ffn sizes must be multiples of 32")
         if shared:

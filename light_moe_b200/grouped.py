@@ -95,6 +95,9 @@ class GroupedExperts(torch.nn.Module):
     def forward(self, hidden_states: torch.Tensor, expert_indices: torch.Tensor,
                 routing_weights: torch.Tensor) -> torch.Tensor:
         """hidden_states [T, d]; expert_indices, routing_weights [T, k] (as the router gives them)."""
+        if expert_indices.dim() != 2 or expert_indices.shape[1] < 1 or routing_weights.shape != expert_indices.shape \
+                or hidden_states.dim() != 2 or hidden_states.shape[0] != expert_indices.shape[0]:
+            raise ValueError("hidden_states must be [T, d], expert_indices and routing_weights [T, k]")
         T, k = expert_indices.shape
         flat = expert_indices.reshape(-1).long()
         ids, order = torch.sort(flat, stable=True)             # (expert, token, slot) order
@@ -104,4 +107,4 @@ class GroupedExperts(torch.nn.Module):
         out = self.down_proj(h, offsets).float() * routing_weights.reshape(-1)[order].float()[:, None]
         back = torch.empty_like(order)                         # the row of each (token, slot)
         back[order] = torch.arange(T * k, device=order.device)
-        return out[back].view(T, k, -1).sum(1).to(hidden_states.dtype)
+        return out[back].view(T, k, out.shape[1]).sum(1).to(hidden_states.dtype)

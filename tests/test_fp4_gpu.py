@@ -422,3 +422,18 @@ def test_scales_at_odd_addresses():
         moved = torch.zeros(R * 32 + shift, dtype=torch.uint8, device="cuda")[shift:].view(R, 32)
         moved.copy_(xs)
         assert torch.equal(ops.fp4_grouped_gemm(xq, moved, wq, ws, off, 1, fmt), want)
+
+
+def test_broadcast_scales():
+    """Scales that are one row for many (stride 0), in either leading dimension."""
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    E, N, K, fmt = 3, 40, 64, "mxfp4"
+    q = torch.randint(0, 256, (E, N, K // 2), generator=gen, device="cuda", dtype=torch.uint8)
+    xq, xs = _operand((70, K), fmt, gen)
+    off = torch.tensor([0, 20, 25, 70], dtype=torch.int32, device="cuda")
+    for shape in ((E, 1, 32), (1, N, 32), (1, 1, 32)):
+        rows = torch.randint(120, 130, shape, generator=gen, device="cuda", dtype=torch.uint8)
+        s = rows[..., :K // 32].expand(E, N, K // 32)
+        assert torch.equal(ops.dequantize_fp4(q, s, fmt), ops.dequantize_fp4(q, s.contiguous(), fmt))
+        assert torch.equal(ops.fp4_grouped_gemm(xq, xs, q, s, off, E, fmt),
+                           ops.fp4_grouped_gemm(xq, xs, q, s.contiguous(), off, E, fmt))

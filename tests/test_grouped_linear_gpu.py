@@ -156,3 +156,19 @@ def test_training_step_in_a_graph():
     torch.cuda.synchronize()
     for a, b in zip(out, step()):
         assert torch.equal(a, b)
+
+
+def test_experts_without_tokens_and_with_odd_indices():
+    m = GroupedExperts(3, 32, 64, device="cuda", dtype=torch.float32)
+    x = torch.zeros(0, 32, device="cuda", requires_grad=True)
+    ids, w = torch.zeros(0, 2, dtype=torch.int32, device="cuda"), torch.zeros(0, 2, device="cuda")
+    y = m(x, ids, w)
+    y.sum().backward()
+    assert y.shape == (0, 32) and x.grad.shape == (0, 32)
+    assert all((p.grad == 0).all() for p in m.parameters())
+    # the same expert twice counts twice; indices that name no expert add nothing
+    x = torch.randn(5, 32, device="cuda")
+    one = m(x, torch.full((5, 1), 2, device="cuda"), torch.ones(5, 1, device="cuda"))
+    two = m(x, torch.full((5, 2), 2, device="cuda"), torch.full((5, 2), 0.5, device="cuda"))
+    none = m(x, torch.tensor([[-1, 2, 3]], device="cuda").expand(5, 3), torch.ones(5, 3, device="cuda"))
+    assert torch.equal(one, two) and torch.equal(one, none)
