@@ -82,7 +82,7 @@ struct __align__(8) Bars {
 static_assert(kAcc * kTN + kUnits * kUnitCols <= kTmemCols, "tensor memory budget");
 constexpr uint32_t kStageBytes = kABytes + kBBytes;
 constexpr uint32_t kSfABytes = 8 * 512, kSfBBytes = 8 * 1024, kSfSlotBytes = kSfABytes + kSfBBytes;
-constexpr uint32_t kEpiBytes = 12 * kStoreStageBytes > 8 * 2048 ? 12 * kStoreStageBytes : 8 * 2048;
+constexpr uint32_t kEpiBytes = 8 * 2048;   // of the epilogue's blocks (SwiGLU 12 * 1024)
 constexpr uint32_t kSmem = 1024 + kStages * kStageBytes + kSfSlots * kSfSlotBytes + kEpiBytes + sizeof(Bars);
 static_assert(kStageBytes % 1024 == 0, "swizzle atoms");
 static_assert(kSmem <= 232448, "shared memory budget");
@@ -294,7 +294,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Epi<SWIGLU>::kThread
     const uint32_t lane_base = (uint32_t)(q * 32) << 16;
     const uint32_t empty_addr = mapa_u32(&bars->acc_empty[0], 0);
     const int64_t pitch = (int64_t)a.N * (a.out_dtype == LMOE_DTYPE_F32 ? 4 : 2);
-    uint8_t* stage = store_stage + (warp - kEpiWarp0) * (kEpiBytes / Ep::kWarps / 128 * 128);
+    uint8_t* stage = store_stage + (warp - kEpiWarp0) * Ep::kBlockBytes;
     Ring<kAcc> ac;
     int hint = 0;
     for (int tile = first; tile < total; tile += stride) {
@@ -342,7 +342,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Epi<SWIGLU>::kThread
         const int c = t.n * (SWIGLU ? kHalf : kTN) + b * Ep::kCols;
         if (c >= a.N) continue;
         if (!whole) {
-          store_rows(out, pitch, rows, c, a.N, f, a.out_dtype, a.store, stage, lane);
+          store_rows<Ep::kCols, Ep::kBlockBytes>(out, pitch, rows, c, a.N, f, a.out_dtype, a.store, stage, lane);
         } else {
           store_block<Ep::kCols * 2>(&tm_out, f, a.out_dtype, stage, lane, c, row, 0);
           if (a.out_dtype == LMOE_DTYPE_F32 && c + Ep::kCols / 2 < a.N)

@@ -319,9 +319,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           store_block<128>(&tm_out, f, odt, stage, lane, c, y, z);
           if (c + 32 < a.K) store_block<128>(&tm_out, f + 32, odt, stage, lane, c + 32, y, z);
         } else {
-          store_rows(out, pitch, rows, c, a.K, reinterpret_cast<const float(&)[32]>(f[0]), odt, a.store, stage, lane);
-          store_rows(out, pitch, rows, c + 32, a.K, reinterpret_cast<const float(&)[32]>(f[32]), odt, a.store, stage,
-                       lane);
+          store_rows<64, kBlockBytes>(out, pitch, rows, c, a.K, f, odt, a.store, stage, lane);
         }
       }
     }
@@ -338,18 +336,39 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 }
 
 // dst[r, 0 .. pitch) = src[r, 0 .. cols) and zeros: 16-bit rows whose length is not a multiple of
-// 16 bytes cannot be read by TMA where they lie.
+// 16 bytes cannot be read by TMA where they lie.  Rows start at any even address: a thread reads
+// the five aligned words around its eight values and shifts them into place (value by value, 8
+// loads, the copies of 11147 x 6965 values took three times as long).
 __global__ void __launch_bounds__(256) pad_rows_kernel(const uint16_t* __restrict__ src, int64_t rows, int cols,
                                                        int pitch, uint4* __restrict__ dst) {
   const int per = pitch / 8;
   const int64_t total = rows * per;
+  const int head = (int)(reinterpret_cast<uintptr_t>(src) >> 1 & 1);   // values of the first word before src
+  const uint16_t* base = src - head;
+  const int64_t end = rows * cols + head;   // values from base
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
     const int64_t r = i / per;
     const int c = (int)(i - r * per) * 8;
-    uint16_t v[8];
+    const int64_t at = r * cols + c + head, x = at & ~int64_t(1);
+    uint32_t w[5];
+    if (x >= head && x + 10 <= end) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = c + j < cols ? src[r * cols + c + j] : (uint16_t)0;
-    dst[i] = *reinterpret_cast<const uint4*>(v);
+      for (int j = 0; j < 5; ++j) w[j] = __ldg(reinterpret_cast<const uint32_t*>(base + x) + j);
+    } else {   // the ends of src: values that are its own
+#pragma unroll
+      for (int j = 0; j < 5; ++j) {
+        const int64_t k = x + 2 * j;
+        w[j] = (k >= head && k < end ? __ldg(base + k) : 0u) | (k + 1 < end ? (uint32_t)__ldg(base + k + 1) << 16 : 0u);
+      }
+    }
+    uint32_t v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      v[j] = (at & 1) ? __funnelshift_r(w[j], w[j + 1], 16) : w[j];
+      const int left = cols - c - 2 * j;   // values of the row from here on
+      if (left < 2) v[j] = left == 1 ? v[j] & 0xffffu : 0u;
+    }
+    dst[i] = make_uint4(v[0], v[1], v[2], v[3]);
   }
 }
 

@@ -54,7 +54,7 @@ struct Cfg {
   static constexpr uint32_t kStageBytes = 3 * (kPlane + kPlaneOfB);
   static constexpr int kStages = kConv ? 3 : 2;
   // a warp's block on its way out (weights converted: rows of odd lengths only)
-  static constexpr uint32_t kBlockBytes = kConv ? kStoreStageF32 : 32 * 128;
+  static constexpr uint32_t kBlockBytes = kConv ? 32 * 32 : 32 * 128;
   static constexpr int kBlocks = kConv ? 2 : 4;        // blocks of 32 columns of an epilogue warp
 };
 
@@ -373,7 +373,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Cfg<FORM>::kThreads,
         if (!C::kConv && whole)
           store_block<128>(&tm_out, f[j], LMOE_DTYPE_F32, stage, lane, c0 + j * 32, y, z);
         else
-          store_rows(out, pitch, rows, c0 + j * 32, a.K, f[j], LMOE_DTYPE_F32, a.store, stage, lane);
+          store_rows<32, kBlockBytes>(out, pitch, rows, c0 + j * 32, a.K, f[j], LMOE_DTYPE_F32, a.store, stage, lane);
       }
     }
     if (elect_one()) bulk_wait_all();   // the stores are complete

@@ -303,14 +303,13 @@ inline int store_mode(const void* out, int64_t cols, int dtype) {
   const uintptr_t a = reinterpret_cast<uintptr_t>(out) | (uintptr_t)(cols * (dtype == LMOE_DTYPE_F32 ? 4 : 2));
   return a % 32 == 0 ? kStore32 : (a % 16 == 0 ? kStore16 : kStoreStaged);
 }
-constexpr uint32_t kStoreStageBytes = 1152, kStoreStageF32 = 1024;   // per warp: any type, fp32
-
 // Called by a whole warp: lane l holds COLS values of row l (of `rows` valid ones) from column c0;
-// columns at or behind `cols` are not written.  Rows that start at odd addresses go through
-// `stage` (kStoreStageBytes of the warp's own), so that neighbouring lanes write neighbouring
-// columns: storing them value by value from the lanes that hold them touches 32 sectors per
-// instruction (the gradients of fp16 rows of odd lengths took 7.9 ms, of which ~7 ms stores).
-template <int COLS>
+// columns at or behind `cols` are not written.  Rows that do not start at whole vectors go through
+// `stage` (STAGE bytes of the warp's own), so that neighbouring lanes write neighbouring columns, up
+// to 128 bytes of a row at a time: storing them value by value from the lanes that hold them touches
+// 32 sectors per instruction (the gradients of fp16 rows of odd lengths took 7.9 ms, of which ~7 ms
+// stores).
+template <int COLS, uint32_t STAGE>
 __device__ __forceinline__ void store_rows(uint8_t* base, int64_t pitch, int rows, int c0, int cols,
                                            const float (&v)[COLS], int dtype, int mode, uint8_t* stage, int lane) {
   if (c0 >= cols || rows <= 0) return;
@@ -354,30 +353,49 @@ __device__ __forceinline__ void store_rows(uint8_t* base, int64_t pitch, int row
     }
     return;
   }
+  // W words of a row at a time, word j of row r at j ^ r (mod W)
+  uint32_t* st = reinterpret_cast<uint32_t*>(stage);
   if (dtype == LMOE_DTYPE_F32) {
-    float* st = reinterpret_cast<float*>(stage);   // [32][8], value j of row r at j ^ (r & 7)
+    constexpr int W = COLS < (int)STAGE / 128 ? COLS : (int)STAGE / 128;
+    static_assert((W & (W - 1)) == 0 && W <= 32 && COLS % W == 0, "words of a row");
 #pragma unroll
-    for (int ch = 0; ch < COLS / 8; ++ch) {
+    for (int ch = 0; ch < COLS / W; ++ch) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) st[lane * 8 + (i ^ (lane & 7))] = v[8 * ch + i];
+      for (int i = 0; i < W; ++i) st[lane * W + ((i ^ lane) & (W - 1))] = __float_as_uint(v[W * ch + i]);
       __syncwarp();
-      const int c = c0 + 8 * ch + (lane & 7);
-      for (int r = lane >> 3; r < rows; r += 4)
-        if (c < cols) reinterpret_cast<float*>(base + r * pitch)[c] = st[r * 8 + ((lane ^ r) & 7)];
+      const int j = lane & (W - 1), c = c0 + W * ch + j;
+      if (c < cols)
+        for (int r = lane / W; r < rows; r += 32 / W)
+          reinterpret_cast<uint32_t*>(base + r * pitch)[c] = st[r * W + ((j ^ r) & (W - 1))];
       __syncwarp();
     }
   } else {
+    constexpr int W = COLS / 2 < (int)STAGE / 128 ? COLS / 2 : (int)STAGE / 128;
+    static_assert((W & (W - 1)) == 0 && W <= 32 && COLS % (2 * W) == 0, "words of a row");
+    const bool pairs = ((reinterpret_cast<uintptr_t>(base) | (uintptr_t)pitch) & 3) == 0;   // rows of whole words
 #pragma unroll
-    for (int ch = 0; ch < COLS / 16; ++ch) {   // [32][18] 16-bit values
+    for (int ch = 0; ch < COLS / (2 * W); ++ch) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        *reinterpret_cast<uint32_t*>(stage + lane * 36 + i * 4) = pack16(v[16 * ch + 2 * i], v[16 * ch + 2 * i + 1], f16);
+      for (int i = 0; i < W; ++i)
+        st[lane * W + ((i ^ lane) & (W - 1))] = pack16(v[2 * (W * ch + i)], v[2 * (W * ch + i) + 1], f16);
       __syncwarp();
-      const int c = c0 + 16 * ch + (lane & 15);
-      for (int r = lane >> 4; r < rows; r += 2)
+      const int at = c0 + 2 * W * ch;
+      if (pairs) {
+        const int j = lane & (W - 1), c = at + 2 * j;
         if (c < cols)
-          reinterpret_cast<uint16_t*>(base + r * pitch)[c] =
-              *reinterpret_cast<const uint16_t*>(stage + r * 36 + (lane & 15) * 2);
+          for (int r = lane / W; r < rows; r += 32 / W)
+            *reinterpret_cast<uint32_t*>(base + r * pitch + c * 2) = st[r * W + ((j ^ r) & (W - 1))];
+      } else {
+        constexpr int P = W < 16 ? 2 * W : 32;   // values of a row at a time
+#pragma unroll
+        for (int h = 0; h < 2 * W / P; ++h) {
+          const int k = h * P + (lane & (P - 1)), c = at + k, j = k >> 1;
+          if (c < cols)
+            for (int r = lane / P; r < rows; r += 32 / P)
+              reinterpret_cast<uint16_t*>(base + r * pitch)[c] =
+                  (uint16_t)(st[r * W + ((j ^ r) & (W - 1))] >> (16 * (k & 1)));
+        }
+      }
       __syncwarp();
     }
   }
