@@ -243,8 +243,9 @@ int lmoe_w4a16_grouped_gemm(const void* input, int64_t total_rows, int K, const 
  * 16-bit operands with row lengths that are multiples of 8 are read where they lie and must be
  * 16-byte aligned; other row lengths are copied into the workspace first.  fp32 activations are
  * written to the workspace as three bf16 planes each, unless the product is small; without a
- * workspace (NULL) fp32 operands take the CUDA cores.  lmoe_grouped_gemm_grad_workspace_bytes: 0 where no copy is
- * made.  Operands that are not finite give results that are not finite (fp32 on tensor cores: NaN
+ * workspace (NULL) fp32 operands take the CUDA cores.  Few rows with a long contraction are summed
+ * in ranges, whose sums lie in the workspace too; where only the copies fit, in one.
+ * lmoe_grouped_gemm_grad_workspace_bytes: 0 where none is needed.  Operands that are not finite give results that are not finite (fp32 on tensor cores: NaN
  * where fp32 may give an infinity).
  * error: a device word that the caller has zeroed, or NULL.  Offsets that decrease or leave
  * [0, total_rows] set it, and every row then counts as outside every expert.

@@ -22,6 +22,8 @@
 // a product with a zero row would not do, since those rows may hold infinities or NaN.  Experts
 // without rows get a zero dw, rows outside every expert a zero dx.
 //
+// Few tiles with a long contraction are cut along it (splits_of).
+//
 // Warps: 0 TMA producer, whose copies complete on the leader's stage barrier; 1 MMA issuer
 // (leader CTA); 2 clears the tail of a segment's last stage (whose copies complete on a barrier
 // of its own CTA) and hands it to the leader; 4-11 epilogue, eight warps of 32 rows x 128 columns.
@@ -58,6 +60,27 @@ struct __align__(8) Bars {
   int abort;
   SegTable seg;
 };
+
+// The part of a tile that unit `unit` sums: one of a.splits ranges of its stages, from k0 on.
+struct Part {
+  Tile t;
+  int k0, s;
+};
+template <int FORM>
+__device__ __forceinline__ Part part_at(const SegTable& seg, const GradArgs& a, int unit, int& hint) {
+  Part p;
+  p.k0 = p.s = 0;
+  if (FORM != kGradWeight && a.splits > 1) {
+    p.s = unit % a.splits;
+    unit /= a.splits;
+  }
+  p.t = tile_at<FORM, kSK>(seg, a, unit, hint);
+  if (FORM != kGradWeight && a.splits > 1) {
+    p.k0 = p.t.ks * p.s / a.splits;
+    p.t.ks = p.t.ks * (p.s + 1) / a.splits - p.k0;
+  }
+  return p;
+}
 
 // Whether a stage with `left` rows of its segment ends inside the 16 rows of an MMA.
 __device__ __forceinline__ bool has_tail(int left) { return left < kSK && (left & 15) != 0; }
@@ -107,7 +130,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = bars->tmem_base;
   const SegTable& seg = bars->seg;
-  const int total = seg.tile_start[segs];
+  const int total = seg.tile_start[segs] * (FORM != kGradWeight ? a.splits : 1);
   const int first = blockIdx.x >> 1, stride = gridDim.x >> 1;
 
   if (warp == 0) {
@@ -117,7 +140,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     int hint = 0;
     bool ok = true;
     for (int tile = first; tile < total && ok; tile += stride) {
-      const Tile t = tile_at<FORM, kSK>(seg, a, tile, hint);
+      const Part part = part_at<FORM>(seg, a, tile, hint);
+      const Tile& t = part.t;
       const int c0 = t.n * a.width + (int)rank * (a.width / 2);   // first column of B
       const int m0 = (FORM != kGradWeight ? t.row0 : t.m * kTile) + (int)rank * kCta;
       int boxes = 4;   // input gradient: 32-row boxes of dy that hold this CTA's rows
@@ -127,7 +151,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       }
       const bool wide = a.width == kTile;
       const uint32_t b_bytes = wide ? kOperand : kChunk;
-      for (int ks = 0; ks < t.ks; ++ks, st.next()) {
+      for (int i = 0; i < t.ks; ++i, st.next()) {
+        const int ks = part.k0 + i;
         ok = warp_wait(&bars->empty[st.i], st.phase ^ 1u, a.err, abort_flag, kSite + 2);
         if (!ok) break;
         if (elect_one()) {
@@ -201,7 +226,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       int hint = 0;
       bool ok = true;
       for (int tile = first; tile < total && ok; tile += stride) {
-        const Tile t = tile_at<FORM, kSK>(seg, a, tile, hint);
+        const Part part = part_at<FORM>(seg, a, tile, hint);
+        const Tile& t = part.t;
         const int depth = FORM != kGradWeight ? a.N : t.row_end - t.row0;
         if (t.ks != 0) {
           ok = warp_wait(&bars->acc_empty[ac.i], ac.phase ^ 1u, a.err, abort_flag, kSite + 4);
@@ -211,7 +237,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             ok = warp_wait(&bars->full[st.i], st.phase, a.err, abort_flag, kSite + 6);
             if (!ok) break;
             tc_fence_after();
-            const int left = depth - ks * kSK;
+            const int left = depth - (part.k0 + ks) * kSK;
             if (elect_one()) {
               const uint64_t ad = adesc0 + st.i * (kStageBytes >> 4), bd = bdesc0 + st.i * (kStageBytes >> 4);
 #pragma unroll
@@ -273,19 +299,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     int hint = 0;
     bool ok = true;
     for (int tile = first; tile < total; tile += stride) {
-      const Tile t = tile_at<FORM, kSK>(seg, a, tile, hint);
+      const Part part = part_at<FORM>(seg, a, tile, hint);
+      const Tile& t = part.t;
       // the warp's 32 rows, and the first of its half of the columns
       const int r = (int)rank * kCta + q * 32;
       const int left = FORM != kGradWeight ? t.row_end - t.row0 - r : a.N - t.m * kTile - r;
       const int rows = left < 32 ? left : 32;
-      const int64_t row = FORM != kGradWeight ? (int64_t)t.row0 + r : (int64_t)t.e * a.N + t.m * kTile + r;
+      const int64_t row = FORM != kGradWeight ? part.s * a.R + t.row0 + r : (int64_t)t.e * a.N + t.m * kTile + r;
       uint8_t* out = static_cast<uint8_t*>(a.out) + row * pitch;
       const int cols = a.width / 2;
       const int c0 = t.n * a.width + half * cols;
       const uint32_t col0 = tmem + lane_base + half * cols;
       // whole 32-row blocks leave by TMA; a weight gradient's rows behind N are cut by the tensor map
       const bool whole = a.store != kStoreStaged && (FORM == kGradWeight ? rows > 0 : rows == 32);
-      const int y = FORM == kGradWeight ? t.m * kTile + r : (int)row, z = FORM == kGradWeight ? t.e : 0;
+      const int y = FORM == kGradWeight ? t.m * kTile + r : t.row0 + r, z = FORM == kGradWeight ? t.e : part.s;
       if (t.ks != 0) {
         ok = warp_wait(&bars->acc_full[ac.i], ac.phase, a.err, abort_flag, kSite + 9);
         if (!ok) break;
@@ -339,8 +366,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 // 16 bytes cannot be read by TMA where they lie.  Rows start at any even address: a thread reads
 // the five aligned words around its eight values and shifts them into place (value by value, 8
 // loads, the copies of 11147 x 6965 values took three times as long).
-__global__ void __launch_bounds__(256) pad_rows_kernel(const uint16_t* __restrict__ src, int64_t rows, int cols,
-                                                       int pitch, uint4* __restrict__ dst) {
+__global__ void __launch_bounds__(256) pad_rows_kernel(const __grid_constant__ CopyJobs jobs) {
+  const CopyJob& job = jobs.job[blockIdx.y];
+  const uint16_t* __restrict__ src = static_cast<const uint16_t*>(job.src);
+  const int64_t rows = job.rows;
+  const int cols = job.cols, pitch = job.pitch;
+  uint4* __restrict__ dst = job.dst;
   const int per = pitch / 8;
   const int64_t total = rows * per;
   const int head = (int)(reinterpret_cast<uintptr_t>(src) >> 1 & 1);   // values of the first word before src
@@ -372,11 +403,31 @@ __global__ void __launch_bounds__(256) pad_rows_kernel(const uint16_t* __restric
   }
 }
 
-int pad_rows(const void* src, int64_t rows, int cols, int pitch, void* dst, const DeviceInfo& dev, cudaStream_t s) {
-  const int64_t blocks = (rows * (pitch / 8) + 255) / 256, most = (int64_t)dev.num_sms * 8;
-  pad_rows_kernel<<<(unsigned)(blocks < most ? blocks : most), 256, 0, s>>>(static_cast<const uint16_t*>(src), rows,
-                                                                          cols, pitch, static_cast<uint4*>(dst));
-  return cuda_status(cudaGetLastError());
+// out[i] = the sum of part[s][i] over s, in its order; 16-bit values.
+__global__ void __launch_bounds__(256) join_kernel(const float* __restrict__ part, int splits, int64_t n, int f16,
+                                                   uint16_t* __restrict__ out) {
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
+    float v = part[i];
+    for (int s = 1; s < splits; ++s) v += part[s * n + i];
+    out[i] = (uint16_t)pack16(v, 0.0f, f16);
+  }
+}
+
+// Ranges that the contraction is summed in where few tiles (of 128 columns) would leave most pairs
+// idle, at least four stages each: their fp32 sums go to the workspace and are joined in order (both
+// gradients of 5 rows, N = 7680, K = 856: 28 us, were 42).
+constexpr int kPairs = 74;   // of a B200
+inline int splits_of(const GradProblem& p) {
+  if (weight_grad(p) || p.total_rows == 0) return 1;
+  const int64_t tiles = even_row_tiles(p.total_rows, p.num_experts, kTile) * ((p.K + 127) / 128);
+  const int64_t most = ((int64_t)p.N + kSK - 1) / kSK / 4, fit = kPairs / tiles;
+  return (int)(fit < most ? (fit < 1 ? 1 : fit) : (most < 1 ? 1 : most));
+}
+inline size_t copies_bytes(const GradProblem& p) {
+  size_t b = 0;
+  if (p.N % 8) b += align256((size_t)p.total_rows * pitch8(p.N) * 2);
+  if (other_cols(p) % 8) b += align256((size_t)other_rows(p) * pitch8(other_cols(p)) * 2);
+  return b;
 }
 
 template <int FORM>
@@ -395,10 +446,11 @@ int launch(const CUtensorMap& ta, const CUtensorMap& ta32, const CUtensorMap& tb
 
 size_t grad_gemm_workspace(const GradProblem& p) {
   if (p.dtype == LMOE_DTYPE_F32) return grad_split_workspace(p);
-  size_t b = 0;
-  if (p.N % 8) b += align256((size_t)p.total_rows * pitch8(p.N) * 2);
-  if (other_cols(p) % 8) b += align256((size_t)other_rows(p) * pitch8(other_cols(p)) * 2);
-  return b;
+  const int splits = splits_of(p);
+  return copies_bytes(p) + (splits > 1 ? (size_t)splits * p.total_rows * p.K * 4 : 0);
+}
+size_t grad_gemm_needs(const GradProblem& p) {
+  return p.dtype == LMOE_DTYPE_F32 ? grad_split_workspace(p) : copies_bytes(p);
 }
 
 int run_grad_gemm(const GradProblem& p, cudaStream_t stream) {
@@ -410,27 +462,39 @@ int run_grad_gemm(const GradProblem& p, cudaStream_t stream) {
   const void* other = p.other;
   const int64_t ldy = pitch8(p.N), ldo = pitch8(other_cols(p));
   uint8_t* ws = static_cast<uint8_t*>(p.workspace);
+  CopyJobs jobs = {};
   if (ldy != p.N) {
-    st = pad_rows(p.dy, p.total_rows, p.N, (int)ldy, ws, dev, stream);
-    if (st != LMOE_OK) return st;
+    jobs.add(p.dy, p.total_rows, p.N, ldy, ws);
     dy = ws;
     ws += align256((size_t)p.total_rows * ldy * 2);
   }
   if (ldo != other_cols(p)) {
-    st = pad_rows(p.other, other_rows(p), other_cols(p), (int)ldo, ws, dev, stream);
-    if (st != LMOE_OK) return st;
+    jobs.add(p.other, other_rows(p), other_cols(p), ldo, ws);
     other = ws;
+    ws += align256((size_t)other_rows(p) * ldo * 2);
+  }
+  if (jobs.count) {
+    pad_rows_kernel<<<jobs.grid(dev), 256, 0, stream>>>(jobs);
+    st = cuda_status(cudaGetLastError());
+    if (st != LMOE_OK) return st;
   }
   GradArgs a = {};
   CUtensorMap ta, ta32, tb, to = {};
-  st = fill_args(p, kSK, a, to);
+  int splits = splits_of(p);
+  if (p.workspace_bytes < grad_gemm_workspace(p)) splits = 1;
+  GradProblem q = p;
+  if (splits > 1) {   // the sums of the ranges: splits matrices like the output, in fp32
+    q.out = ws;
+    q.out_dtype = LMOE_DTYPE_F32;
+  }
+  st = fill_args(q, kSK, splits, a, to);
   if (st != LMOE_OK) return st;
   const CUtensorMapDataType dt = a.f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   const int grid = gemm_grid(dev) < 2 ? 2 : gemm_grid(dev) & ~1;   // whole pairs
   const int64_t row_tiles = weight_grad(p) ? (int64_t)a.MT * p.num_experts
                                           : even_row_tiles(p.total_rows, p.num_experts, kTile);
   const int widths[] = {256, 128};
-  a.width = pick_width(widths, grid / 2, 0, 16, [&](int w) { return row_tiles * ((p.K + w - 1) / w); });
+  a.width = splits > 1 ? 128 : pick_width(widths, grid / 2, 0, 16, [&](int w) { return row_tiles * ((p.K + w - 1) / w); });
   a.raster = Raster((p.K + a.width - 1) / a.width);
   // the maps end at the true sizes, so that TMA fills what lies behind them with zeros
   if (weight_grad(p)) {
@@ -451,8 +515,13 @@ int run_grad_gemm(const GradProblem& p, cudaStream_t stream) {
   const uint32_t box[3] = {64, product ? (uint32_t)a.width / 2 : (uint32_t)kSK, 1};
   st = encode_tmap_3d(&tb, other, dt, 2, dims, strides, box);
   if (st != LMOE_OK) return st;
-  return product ? launch<kGradProduct>(ta, ta32, tb, to, a, grid, stream)
-                 : launch<kGradInput>(ta, ta32, tb, to, a, grid, stream);
+  st = product ? launch<kGradProduct>(ta, ta32, tb, to, a, grid, stream)
+               : launch<kGradInput>(ta, ta32, tb, to, a, grid, stream);
+  if (st != LMOE_OK || splits == 1) return st;
+  const int64_t n = p.total_rows * p.K, blocks = (n + 255) / 256, enough = (int64_t)dev.num_sms * 8;
+  join_kernel<<<(unsigned)(blocks < enough ? blocks : enough), 256, 0, stream>>>(
+      static_cast<const float*>(q.out), splits, n, a.f16, static_cast<uint16_t*>(p.out));
+  return cuda_status(cudaGetLastError());
 }
 
 }  // namespace lmoe
@@ -479,9 +548,10 @@ int grad_entry(GradProblem& p, const void* offsets, void* out, void* workspace, 
   // rows that TMA reads where they lie start at multiples of 16 bytes
   LMOE_ARG_CHECK(p.dtype == LMOE_DTYPE_F32 ||
                  ((p.N % 8 || aligned16(p.dy)) && (other_cols(p) % 8 || aligned16(p.other))));
-  const size_t need = grad_gemm_workspace(p);
+  const size_t need = grad_gemm_needs(p);
   if (need && (!workspace || workspace_bytes < need || !aligned16(workspace))) return LMOE_ERR_WORKSPACE;
   p.workspace = workspace;
+  p.workspace_bytes = workspace && aligned16(workspace) ? workspace_bytes : 0;
   return p.dtype == LMOE_DTYPE_F32 ? run_grad_split(p, stream) : run_grad_gemm(p, stream);
 }
 

@@ -26,11 +26,13 @@ struct GradProblem {
   const void* offsets = nullptr;
   int offsets_i64 = 0;
   void* out = nullptr;
-  void* workspace = nullptr;     // copies of operands: padded rows, or planes of fp32
+  void* workspace = nullptr;     // copies of operands: padded rows, or planes of fp32; sums of ranges
+  size_t workspace_bytes = 0;
   uint32_t* err = nullptr;
 };
 
 size_t grad_gemm_workspace(const GradProblem& p);
+size_t grad_gemm_needs(const GradProblem& p);   // without it a call is refused
 int run_grad_gemm(const GradProblem& p, cudaStream_t stream);
 // Whether fp32 operands go to the tensor cores as three bf16 planes each.
 bool grad_splits(const GradProblem& p);

@@ -462,8 +462,13 @@ int launch(const CUtensorMap& ta, const CUtensorMap& ta32, const CUtensorMap& tb
 }
 
 // The planes of src [rows, cols]: dst [3][rows, pitch] bf16, zero behind the columns.
-__global__ void __launch_bounds__(256) split_rows_kernel(const float* __restrict__ src, int64_t rows, int cols,
-                                                         int pitch, int vec, uint4* __restrict__ dst) {
+__global__ void __launch_bounds__(256) split_rows_kernel(const __grid_constant__ CopyJobs jobs) {
+  const CopyJob& job = jobs.job[blockIdx.y];
+  const float* __restrict__ src = static_cast<const float*>(job.src);
+  const int64_t rows = job.rows;
+  const int cols = job.cols, pitch = job.pitch;
+  const bool vec = cols % 4 == 0 && (reinterpret_cast<uintptr_t>(src) & 15) == 0;
+  uint4* __restrict__ dst = job.dst;
   const int per = pitch / 8;
   const int64_t total = rows * per;
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
@@ -476,13 +481,6 @@ __global__ void __launch_bounds__(256) split_rows_kernel(const float* __restrict
 #pragma unroll
     for (int k = 0; k < 3; ++k) dst[k * total + i] = make_uint4(w[0][k], w[1][k], w[2][k], w[3][k]);
   }
-}
-
-int split_rows(const void* src, int64_t rows, int cols, int pitch, void* dst, const DeviceInfo& dev, cudaStream_t s) {
-  const int64_t blocks = (rows * (pitch / 8) + 255) / 256, most = (int64_t)dev.num_sms * 8;
-  split_rows_kernel<<<(unsigned)(blocks < most ? blocks : most), 256, 0, s>>>(
-      static_cast<const float*>(src), rows, cols, pitch, cols % 4 == 0 && aligned16(src), static_cast<uint4*>(dst));
-  return cuda_status(cudaGetLastError());
 }
 
 }  // namespace
@@ -513,19 +511,21 @@ int run_grad_split(const GradProblem& p, cudaStream_t stream) {
   const int64_t ldy = pitch8(p.N), ldx = pitch8(p.K);
   uint8_t* dy = static_cast<uint8_t*>(p.workspace);
   uint8_t* x = dy + align256((size_t)p.total_rows * ldy * 6);
-  st = split_rows(p.dy, p.total_rows, p.N, (int)ldy, dy, dev, stream);
+  CopyJobs jobs = {};
+  jobs.add(p.dy, p.total_rows, p.N, ldy, dy);
+  if (weight_grad(p)) jobs.add(p.other, p.total_rows, p.K, ldx, x);
+  split_rows_kernel<<<jobs.grid(dev), 256, 0, stream>>>(jobs);
+  st = cuda_status(cudaGetLastError());
   if (st != LMOE_OK) return st;
   GradArgs a = {};
   CUtensorMap ta, ta32, tb, to = {};
-  st = fill_args(p, kSK, a, to);
+  st = fill_args(p, kSK, 1, a, to);
   if (st != LMOE_OK) return st;
   const int grid = gemm_grid(dev) < 2 ? 2 : gemm_grid(dev) & ~1;   // whole pairs
   const CUtensorMapDataType dt = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   const uint64_t rows = 3 * (uint64_t)p.total_rows;   // of the planes, one behind the other
   // the maps end at the true sizes, so that TMA fills what lies behind them with zeros
   if (weight_grad(p)) {
-    st = split_rows(p.other, p.total_rows, p.K, (int)ldx, x, dev, stream);
-    if (st != LMOE_OK) return st;
     const int widths[] = {256, 128};
     a.width = pick_width(widths, grid / 2, 0, 16,
                          [&](int w) { return (int64_t)a.MT * p.num_experts * ((p.K + w - 1) / w); });

@@ -20,6 +20,7 @@ struct GradArgs {
   void* out;
   int out_dtype;
   int width;         // columns of a tile: 256 or 128
+  int splits;        // of the contraction (grad_gemm.cu, not the weight gradient)
   int store;         // StoreMode
   uint32_t* err;
 };
@@ -59,8 +60,33 @@ inline int other_cols(const GradProblem& p) { return p.form == kGradProduct ? p.
 inline int64_t pitch8(int64_t cols) { return (cols + 7) / 8 * 8; }
 inline size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
+// Rows to copy for TMA: dst rows of `pitch` values from src rows of `cols`.  A call's copies are one
+// launch, a job per blockIdx.y.
+struct CopyJob {
+  const void* src;
+  int64_t rows;
+  int cols, pitch;
+  uint4* dst;
+};
+struct CopyJobs {
+  CopyJob job[2];
+  int count;
+  void add(const void* src, int64_t rows, int cols, int64_t pitch, void* dst) {
+    job[count++] = {src, rows, cols, (int)pitch, static_cast<uint4*>(dst)};
+  }
+  dim3 grid(const DeviceInfo& dev) const {   // blocks of 256 threads, eight values a thread
+    int64_t blocks = 1;
+    for (int i = 0; i < count; ++i) {
+      const int64_t b = (job[i].rows * (job[i].pitch / 8) + 255) / 256;
+      blocks = b > blocks ? b : blocks;
+    }
+    const int64_t most = (int64_t)dev.num_sms * 8;
+    return dim3((unsigned)(blocks < most ? blocks : most), (unsigned)count);
+  }
+};
+
 // The arguments that both kernels take, and the map of the output's blocks.
-inline int fill_args(const GradProblem& p, int sk, GradArgs& a, CUtensorMap& to) {
+inline int fill_args(const GradProblem& p, int sk, int splits, GradArgs& a, CUtensorMap& to) {
   a.offsets = p.offsets;
   a.offsets_i64 = p.offsets_i64;
   a.E = p.num_experts;
@@ -74,10 +100,11 @@ inline int fill_args(const GradProblem& p, int sk, GradArgs& a, CUtensorMap& to)
   a.out_dtype = p.out_dtype;
   a.store = store_mode(p.out, p.K, p.out_dtype);
   a.err = p.err;
+  a.splits = splits;
   if (a.store == kStoreStaged) return LMOE_OK;
   const bool wg = weight_grad(p);
   return encode_store_map(&to, p.out, p.out_dtype, (uint64_t)p.K, wg ? (uint64_t)p.N : (uint64_t)p.total_rows,
-                          wg ? (uint64_t)p.num_experts : 1, 128);
+                          wg ? (uint64_t)p.num_experts : (uint64_t)splits, 128);
 }
 
 }  // namespace lmoe

@@ -354,6 +354,7 @@ __device__ __forceinline__ void store_rows(uint8_t* base, int64_t pitch, int row
     return;
   }
   // W words of a row at a time, word j of row r at j ^ r (mod W)
+  constexpr int kUnroll = COLS == 64 ? 1 : 4;   // 64 values leave no registers for more
   uint32_t* st = reinterpret_cast<uint32_t*>(stage);
   if (dtype == LMOE_DTYPE_F32) {
     constexpr int W = COLS < (int)STAGE / 128 ? COLS : (int)STAGE / 128;
@@ -365,6 +366,7 @@ __device__ __forceinline__ void store_rows(uint8_t* base, int64_t pitch, int row
       __syncwarp();
       const int j = lane & (W - 1), c = c0 + W * ch + j;
       if (c < cols)
+#pragma unroll kUnroll
         for (int r = lane / W; r < rows; r += 32 / W)
           reinterpret_cast<uint32_t*>(base + r * pitch)[c] = st[r * W + ((j ^ r) & (W - 1))];
       __syncwarp();
@@ -383,14 +385,16 @@ __device__ __forceinline__ void store_rows(uint8_t* base, int64_t pitch, int row
       if (pairs) {
         const int j = lane & (W - 1), c = at + 2 * j;
         if (c < cols)
+#pragma unroll kUnroll
           for (int r = lane / W; r < rows; r += 32 / W)
             *reinterpret_cast<uint32_t*>(base + r * pitch + c * 2) = st[r * W + ((j ^ r) & (W - 1))];
       } else {
         constexpr int P = W < 16 ? 2 * W : 32;   // values of a row at a time
-#pragma unroll
+#pragma unroll kUnroll
         for (int h = 0; h < 2 * W / P; ++h) {
           const int k = h * P + (lane & (P - 1)), c = at + k, j = k >> 1;
           if (c < cols)
+#pragma unroll kUnroll
             for (int r = lane / P; r < rows; r += 32 / P)
               reinterpret_cast<uint16_t*>(base + r * pitch)[c] =
                   (uint16_t)(st[r * W + ((j ^ r) & (W - 1))] >> (16 * (k & 1)));

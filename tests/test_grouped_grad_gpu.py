@@ -191,3 +191,26 @@ def test_streams_and_graphs():
     torch.cuda.synchronize()
     assert torch.equal(gx, ops.grouped_gemm_dgrad(dy, w, off, 3))
     assert torch.equal(gw, ops.grouped_gemm_wgrad(dy, x, off, 3))
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp16"])
+@pytest.mark.parametrize("counts,N,K,head,tail", [([5], 7680, 856, 0, 0), ([3, 0, 2], 4099, 130, 2, 9), ([1], 1025, 1, 0, 3),
+                                                  ([200, 90], 2048, 264, 1, 0)])
+def test_long_contractions_of_few_tiles(dt, counts, N, K, head, tail):
+    """The contraction is summed in ranges that are joined in order: the formula's values, the same
+    bits in every run, and, without a workspace for the ranges, one sum."""
+    dy, x, w, b, off = _inputs(counts, N, K, DT[dt], head, tail, seed=N)
+    dx, _ = _check(dy, x, w, b, off)
+    assert torch.equal(dx, ops.grouped_gemm_dgrad(dy, w, off, len(counts)))
+    y = ops.grouped_gemm(dy, w.transpose(1, 2).contiguous(), off, len(counts))   # the same sums, K-major
+    assert (y[:head] == 0).all() and (y[b[-1]:] == 0).all()
+    for e in range(len(counts)):
+        r = slice(b[e], b[e + 1])
+        g, we = dy[r].double(), w[e].double()
+        _close(y[r], g @ we, g.abs() @ we.abs(), N, f"product {e}")
+    if N % 8 == 0 and K % 8 == 0:
+        one = torch.empty_like(dx)
+        capi.call("lmoe_grouped_gemm_dgrad", dy.data_ptr(), 0 if dt == "bf16" else 1, dy.shape[0], N, w.data_ptr(), K,
+                  off.data_ptr(), 0, len(counts), one.data_ptr(), None, 0, None, capi.stream_handle())
+        e = b[-1] - 1
+        _close(one[e:e + 1], dy[e:e + 1].double() @ w[-1].double(), dy[e:e + 1].double().abs() @ w[-1].double().abs(), N, "one sum")
