@@ -8,6 +8,9 @@
 // order like the values and put infinities and NaN on top.  With `positions` each row is
 // written to several output rows, so that a MoE layer's permutation costs no pass of its own:
 // the row is quantised once and the copies are 4-bit.
+//
+// 32768 x 4096 values: MX bf16 52 us (6.6 TB/s), fp32 99 us (6.2); NV fp32 101 us (6.1); NV bf16 75 us
+// (4.6 TB/s), bound by the issue of its instructions (the quotients' corrections, fp4_format.cuh).
 #include <cuda_bf16.h>
 
 #include "fp4_format.cuh"
@@ -123,8 +126,8 @@ __global__ void __launch_bounds__(256) quantize_fp4_kernel(const QuantArgs a) {
                                        : 1.0f;
         const bool fine = g > 0.0f && g < __uint_as_float(kInf);
         const float r6 = rcp_approx(__fmul_rn(6.0f, g));
-        scale[0] = fine && t0 < kInf ? fp4_encode_nv(v, __uint_as_float(t0), g, r6, codes[0]) : 0x7fu;
-        scale[1] = fine && t1 < kInf ? fp4_encode_nv(v + 16, __uint_as_float(t1), g, r6, codes[1]) : 0x7fu;
+        scale[0] = fine && t0 < kInf ? fp4_encode_nv<sizeof(T) == 2>(v, __uint_as_float(t0), g, r6, codes[0]) : 0x7fu;
+        scale[1] = fine && t1 < kInf ? fp4_encode_nv<sizeof(T) == 2>(v + 16, __uint_as_float(t1), g, r6, codes[1]) : 0x7fu;
       }
     }
     for (int j = 0; j < a.copies; ++j) {

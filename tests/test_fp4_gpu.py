@@ -437,3 +437,40 @@ def test_broadcast_scales():
         assert torch.equal(ops.dequantize_fp4(q, s, fmt), ops.dequantize_fp4(q, s.contiguous(), fmt))
         assert torch.equal(ops.fp4_grouped_gemm(xq, xs, q, s, off, E, fmt),
                            ops.fp4_grouped_gemm(xq, xs, q, s.contiguous(), off, E, fmt))
+
+
+def test_quantize_borders_of_tiny_and_short_values():
+    """Values at the borders between codes: fp32 ones so small that their distance from a border lies
+    below the smallest fp32, and 16-bit ones that meet borders exactly, under scales of every mantissa."""
+    borders = np.array([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0])
+    gen = np.random.default_rng(3)
+    rows = []
+    g = np.float32(1.37e-37)
+    for c in np.concatenate([np.arange(8, 16) / 8, np.arange(8, 16) * 4]):
+        d = np.float64(g) * c
+        v = (borders * d).astype(np.float32)
+        near = np.concatenate([v, np.nextafter(v, np.float32(1))])
+        rows.append(np.concatenate([[np.float32(6 * d)], near, [0]]) * gen.choice([-1, 1], 16))
+    x = torch.from_numpy(np.array(rows, dtype=np.float32)).reshape(-1, 32).cuda()
+    _check_quantize(x, "nvfp4", float(g))
+    for dt in (torch.bfloat16, torch.float16):
+        for g in (None, 1.0, 0.25, 8.0, 0.3):
+            rows = []
+            for c in np.arange(8, 16) / 8 * (1.0 if g is None else g):
+                for k in range(8):
+                    v = borders * c * 2.0 ** gen.integers(-1, 2, 7)
+                    rows.append(np.concatenate([[6 * c], v, [6 * c * (k + 8.5) / 16], gen.standard_normal(7) * c]))
+            x = torch.from_numpy(np.array(rows)).to(dt).reshape(-1, 32).cuda()
+            _check_quantize(x, "nvfp4", g)
+
+
+def test_quantize_scales_at_midpoints():
+    """Largest values whose sixth lies half way between two scales, in every type."""
+    for dt in DT.values():
+        for g in (None, 0.5, 0.7):
+            n = np.arange(0, 16) + 0.5
+            top = np.concatenate([6 * n * 2.0 ** e for e in (-9, -6, -3, 0, 3)]) * (1.0 if g is None else g)
+            x = torch.zeros(80, 16, dtype=torch.float64)
+            x[:, 3] = torch.from_numpy(top)
+            x[:, 5] = x[:, 3] / 3
+            _check_quantize(x.to(dt).reshape(-1, 32).cuda(), "nvfp4", g)
