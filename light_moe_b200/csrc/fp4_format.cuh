@@ -114,15 +114,27 @@ __device__ __forceinline__ uint32_t fp4_exact_code(float x, float s, float g) {
   return c | (__float_as_uint(x) >> 31 << 3);
 }
 
+// Codes of 16 values of at most 11 significant bits under a scale d of at most four, r = rcp_approx(d).
+// They may meet a border between codes exactly, and one that is missed is missed by 2^-12 (11 bits
+// against 7).  The quotient is corrected by its exact remainder: a quotient that is a border comes out
+// as that border (the remainder is a few units of q times d, which fp32 holds, and the correction is
+// off by 2^-23 of them), and the conversion takes the even code.
+__device__ __forceinline__ uint2 fp4_short_codes(const float* a, float d, float r) {
+  float q[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const float q0 = __fmul_rn(a[i], -r);   // of the quotient's opposite: then zeros keep their signs
+    q[i] = __fmaf_rn(-__fmaf_rn(q0, d, a[i]), r, q0);
+  }
+  return make_uint2(fp4_pack8(q) ^ 0x88888888u, fp4_pack8(q + 8) ^ 0x88888888u);
+}
+
 // The codes come from the rounded product with the reciprocal (three roundings and the reciprocal's
 // unit, below 2^-21 relative); where a border lies that near, they come from fp4_exact_code.
 //
-// SHORT: the values are 16-bit.  Under a g that is a power of two they meet borders exactly, in nearly
-// every warp, and a border that is missed is missed by 2^-12 (11 bits against 7).  Then the quotient
-// q is corrected by its exact remainder: a quotient that is a border comes out as that border (the
-// remainder is a few units of q times d, which fp32 holds, and the correction is off by 2^-23 of
-// them), and the conversion takes the even code.  (32768 x 4096 bf16
-// values, nv, g = 1: 75 us; with the comparisons of all 16 values in every such warp 195.)
+// SHORT: the values are 16-bit.  Under a g that is a power of two they meet borders in nearly every
+// warp, and take fp4_short_codes at once (32768 x 4096 bf16 values, g = 1: 75 us; with the comparisons
+// in every such warp 195).
 template <bool SHORT>
 __device__ __forceinline__ uint32_t fp4_encode_nv(const float* a, float amax, float g, float r6, uint2& codes) {
   const float s = fp4_nv_scale(amax, g, r6);
@@ -131,14 +143,9 @@ __device__ __forceinline__ uint32_t fp4_encode_nv(const float* a, float amax, fl
     const float d = __fmul_rn(s, g);
     const bool plain = d > 1e-30f && d < 1e30f;
     const float r = rcp_approx(plain ? d : 1.0f);
-    if (SHORT && plain && (__float_as_uint(g) & 0x7fffffu) == 0) {
-      float q[16];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float q0 = __fmul_rn(a[i], r);
-        q[i] = __fmaf_rn(__fmaf_rn(-q0, d, a[i]), r, q0);
-      }
-      codes = make_uint2(fp4_pack8(q), fp4_pack8(q + 8));
+    const bool even_g = plain && (__float_as_uint(g) & 0x7fffffu) == 0;
+    if (SHORT && even_g) {
+      codes = fp4_short_codes(a, d, r);
       return (uint32_t)__nv_cvt_float_to_fp8(s, __NV_SATFINITE, __NV_E4M3);
     }
     float lo[16], hi[16];
@@ -152,10 +159,17 @@ __device__ __forceinline__ uint32_t fp4_encode_nv(const float* a, float amax, fl
     codes.x = fp4_pack8(lo);
     codes.y = fp4_pack8(lo + 8);
     if (!plain || codes.x != fp4_pack8(hi) || codes.y != fp4_pack8(hi + 8)) {
-      uint32_t w[2] = {0u, 0u};
+      uint32_t low = 0;   // bits that 16-bit values, widened to fp32, do not have
 #pragma unroll
-      for (int i = 0; i < 16; ++i) w[i >> 3] |= fp4_exact_code(a[i], s, g) << (4 * (i & 7));
-      codes = make_uint2(w[0], w[1]);
+      for (int i = 0; i < 16; ++i) low |= __float_as_uint(a[i]) & 0x1fffu;
+      if (even_g && low == 0) {
+        codes = fp4_short_codes(a, d, r);
+      } else {
+        uint32_t w[2] = {0u, 0u};
+#pragma unroll
+        for (int i = 0; i < 16; ++i) w[i >> 3] |= fp4_exact_code(a[i], s, g) << (4 * (i & 7));
+        codes = make_uint2(w[0], w[1]);
+      }
     }
   }
   return (uint32_t)__nv_cvt_float_to_fp8(s, __NV_SATFINITE, __NV_E4M3);

@@ -474,3 +474,15 @@ def test_quantize_scales_at_midpoints():
             x[:, 3] = torch.from_numpy(top)
             x[:, 5] = x[:, 3] / 3
             _check_quantize(x.to(dt).reshape(-1, 32).cuda(), "nvfp4", g)
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("dt", ["bf16", "fp16", "fp32"])
+def test_quantize_keeps_the_sign_of_zeros_and_tiny_values(fmt, dt):
+    x = torch.zeros(4, 64)
+    x[:, ::8] = 6.0
+    x[:, 1::4] = -0.0
+    x[:, 2::4] = -6e-8
+    x[2:, 3::4] = -1.0
+    x[3] = -0.0
+    _check_quantize(x.to(DT[dt]).cuda(), fmt)
