@@ -4,6 +4,8 @@
 * ``ops``    the reference's ``light_moe._C`` operator surface plus the W4A16 / layer ops
 * ``layer``  ``W4A16Experts`` and ``W4A16MoELayer`` (drop-in for ``SparseMoEBlock``)
 * ``expert_parallel``  the expert-parallel layer over NCCL
+* ``fp4``    ``FP4Experts`` and ``FP4MoELayer`` (mxfp4 / nvfp4 experts and activations)
+* ``grouped``  ``grouped_linear``, ``GroupedLinear``, ``GroupedExperts`` (trainable grouped products)
 
 Build with ``python -m light_moe_b200.build``.  Nothing here falls back to a CPU or
 PyTorch implementation: an op called without the built library raises.
