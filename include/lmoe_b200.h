@@ -246,7 +246,8 @@ int lmoe_w4a16_grouped_gemm(const void* input, int64_t total_rows, int K, const 
  * workspace (NULL) fp32 operands take the CUDA cores.  Few rows with a long contraction are summed
  * in ranges, whose sums lie in the workspace too; where only the copies fit, in one.
  * lmoe_grouped_gemm_grad_workspace_bytes: 0 where none is needed.  Operands that are not finite give results that are not finite (fp32 on tensor cores: NaN
- * where fp32 may give an infinity).
+ * where fp32 may give an infinity).  The lowest of the three planes ends at 2^-133, so fp32 operands
+ * below 2^-107 count with an error of up to 2^-134 each on tensor cores.
  * error: a device word that the caller has zeroed, or NULL.  Offsets that decrease or leave
  * [0, total_rows] set it, and every row then counts as outside every expert.
  * The reference's backward is autograd through one mm_out per expert (csrc/grouped_gemm.cu:30-40,

@@ -1,7 +1,8 @@
 // grad_split.cu -- the gradients of grad_gemm.cu (and the product of any row length) for fp32 operands
 // on tensor cores (sm_100a).
 //
-// A value is the sum of three bf16 planes, x = high + middle + low to 2^-26, and a product of two
+// A value is the sum of three bf16 planes, x = high + middle + low to 2^-26 (but not below 2^-134, half
+// of the smallest bf16), and a product of two
 // values the sum of the six products of planes down to 2^-18: (m, m), (l, h), (h, l), (m, h),
 // (h, m), (h, h); six times the bf16 work at ~16 times the FFMA rate.  The tensor pipe truncates
 // its sums (measured: 1024 bf16 products of mean 1 come out 8e-7 low, 8192 2.5e-5), so a TMEM

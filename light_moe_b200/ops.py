@@ -84,7 +84,8 @@ def w4a16_grouped_gemm(input, packed, expert_offsets, num_experts, N, group_size
 
 def grouped_gemm_dgrad(grad_output, weights, expert_offsets, num_experts):
     """Input gradient of grouped_gemm: [T, N] x [E, N, K] -> [T, K] (rows outside every expert are
-    zero).  bf16 / fp16 on tensor cores, fp32 in fp32; any N, K; operands of one dtype."""
+    zero).  bf16 / fp16 on tensor cores, fp32 in fp32 accuracy (values below 2**-107 to 2**-134);
+    any N, K; operands of one dtype."""
     return extension().grouped_gemm_dgrad(grad_output, weights, expert_offsets, num_experts)
 
 

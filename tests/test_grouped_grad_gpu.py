@@ -214,3 +214,50 @@ def test_long_contractions_of_few_tiles(dt, counts, N, K, head, tail):
                   off.data_ptr(), 0, len(counts), one.data_ptr(), None, 0, None, capi.stream_handle())
         e = b[-1] - 1
         _close(one[e:e + 1], dy[e:e + 1].double() @ w[-1].double(), dy[e:e + 1].double().abs() @ w[-1].double().abs(), N, "one sum")
+
+
+def test_fp32_of_every_magnitude():
+    """fp32 operands near the largest value (whose high plane would round to an infinity) and tiny ones
+    (whose lower planes end at 2^-133: half of that, 2^-134, is lost of each value) on tensor cores."""
+    counts, N, K = [70, 33], 256, 200
+    dy, x, w, b, off = _inputs(counts, N, K, torch.float32, seed=5)
+    for scale, other in ((2.0 ** 126, 2.0 ** -60), (2.0 ** -115, 2.0 ** 40), (2.0 ** -124, 2.0 ** 30), (2.0 ** 60, 2.0 ** -100)):
+        d, v, u = (dy.clamp(-3.9, 3.9) * scale), w * other, x * other
+        dx, dw = ops.grouped_gemm_dgrad(d, v, off, 2), ops.grouped_gemm_wgrad(d, u, off, 2)
+        lost = 2.0 ** -134
+        for e in range(2):
+            r = slice(b[e], b[e + 1])
+            for got, p, q, depth in ((dx[r], d[r].double(), v[e].double(), N),
+                                     (dw[e], d[r].double().T, u[r].double(), counts[e])):
+                tol = (depth + 1) * 2.0 ** -23 * (p.abs() @ q.abs()) + 2.0 ** -148
+                tol = tol + lost * (q.abs().sum(0)[None] + p.abs().sum(1)[:, None])
+                assert torch.isfinite(got).all() and ((got.double() - p @ q).abs() <= tol).all(), (scale, other, e)
+
+
+@pytest.mark.parametrize("dt,counts,N,K", [("fp32", [140, 0, 161], 264, 200), ("bf16", [5, 3], 4096, 256),
+                                           ("fp16", [90, 41], 131, 77), ("fp32", [3, 2], 40, 24)])
+def test_calls_at_once_and_replayed(dt, counts, N, K):
+    """Two streams with calls in flight together, each with its workspaces; a captured pair replayed with
+    other rows."""
+    E = len(counts)
+    dy, x, w, b, off = _inputs(counts, N, K, DT[dt])
+    other = dy.flip(0).contiguous()
+    want = [(ops.grouped_gemm_dgrad(g, w, off, E), ops.grouped_gemm_wgrad(g, x, off, E)) for g in (dy, other)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(8):
+        for i, g in enumerate((dy, other)):
+            with torch.cuda.stream(streams[i]):
+                got[i].append((ops.grouped_gemm_dgrad(g, w, off, E), ops.grouped_gemm_wgrad(g, x, off, E)))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(a, want[i][0]) and torch.equal(c, want[i][1]) for a, c in got[i])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        gx, gw = ops.grouped_gemm_dgrad(dy, w, off, E), ops.grouped_gemm_wgrad(dy, x, off, E)
+    dy.copy_(other)
+    for _ in range(2):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(gx, want[1][0]) and torch.equal(gw, want[1][1])
