@@ -372,6 +372,7 @@ torch::Tensor grouped_gemm_dgrad(torch::Tensor grad_output, torch::Tensor weight
   TORCH_CHECK(grad_output.dim() == 2 && weights.dim() == 3, "grad_output [T,N], weights [E,N,K]");
   TORCH_CHECK(weights.size(0) >= num_experts && weights.size(1) == grad_output.size(1), "shape mismatch");
   TORCH_CHECK(weights.scalar_type() == grad_output.scalar_type(), "grad_output and weights differ in dtype");
+  const at::AutoDispatchBelowADInplaceOrView below_autograd;   // no graph is recorded
   const c10::cuda::OptionalCUDAGuard guard(grad_output.device());
   auto off = check_offsets(expert_offsets, grad_output, num_experts);
   auto dy = contig16(grad_output);
@@ -398,6 +399,7 @@ torch::Tensor grouped_gemm_wgrad(torch::Tensor grad_output, torch::Tensor input,
   TORCH_CHECK(input.scalar_type() == grad_output.scalar_type(), "grad_output and input differ in dtype");
   const auto ot = out_dtype.value_or(grad_output.scalar_type());
   TORCH_CHECK(ot == grad_output.scalar_type() || ot == torch::kFloat32, "out_dtype must be the operands' or float32");
+  const at::AutoDispatchBelowADInplaceOrView below_autograd;   // no graph is recorded
   const c10::cuda::OptionalCUDAGuard guard(grad_output.device());
   auto off = check_offsets(expert_offsets, grad_output, num_experts);
   auto dy = contig16(grad_output);
@@ -445,6 +447,7 @@ std::tuple<torch::Tensor, torch::Tensor> quantize_fp4(torch::Tensor x, const std
   TORCH_CHECK(x.dim() >= 2, "x must be [..., rows, K]");
   const int64_t K = x.size(-1);
   TORCH_CHECK(K > 0 && K % 32 == 0 && K <= INT32_MAX, "K must be a positive multiple of 32");
+  const at::AutoDispatchBelowADInplaceOrView below_autograd;   // no graph is recorded
   const c10::cuda::OptionalCUDAGuard guard(x.device());
   const bool strided = x.dim() == 2 && x.stride(1) == 1 && (x.size(0) <= 1 || x.stride(0) >= K);
   auto xc = strided ? x : x.contiguous();
@@ -476,7 +479,11 @@ std::tuple<torch::Tensor, torch::Tensor> quantize_fp4(torch::Tensor x, const std
                                    pos.defined() ? pos.data_ptr<int32_t>() : nullptr, (int)copies, out_rows,
                                    q.data_ptr<uint8_t>(), s.data_ptr<uint8_t>(), cur_stream()),
                  "quantize_fp4");
-  return {q, s.narrow(-1, 0, K / fp4_block(fmt))};
+  // the columns of the scale rows, without the padding (in place: a view costs the host a microsecond)
+  const auto strides = s.strides().vec();
+  shape.back() = K / fp4_block(fmt);
+  s.unsafeGetTensorImpl()->set_sizes_and_strides(shape, strides);
+  return {q, s};
 }
 
 struct Fp4Operand {
@@ -540,6 +547,7 @@ torch::Tensor dequantize_fp4(torch::Tensor q, torch::Tensor scales, const std::s
                              std::optional<torch::Tensor> global_scale) {
   check_cuda(q, "q");
   const int fmt = fp4_format(format);
+  const at::AutoDispatchBelowADInplaceOrView below_autograd;   // no graph is recorded
   const c10::cuda::OptionalCUDAGuard guard(q.device());
   const Fp4Operand o = fp4_operand(q, scales, q, fmt, false, "q");
   const int64_t K = q.size(-1) * 2, rows = q.numel() / (K / 2);
@@ -573,6 +581,7 @@ torch::Tensor fp4_grouped_gemm(torch::Tensor input, torch::Tensor input_scales, 
   const int fmt = fp4_format(format);
   TORCH_CHECK(input.dim() == 2 && weights.dim() == 3, "input [T,K/2], weights [E,N,K/2]");
   TORCH_CHECK(weights.size(0) >= num_experts && weights.size(2) == input.size(1), "shape mismatch");
+  const at::AutoDispatchBelowADInplaceOrView below_autograd;   // no graph is recorded
   const c10::cuda::OptionalCUDAGuard guard(input.device());
   auto off = check_offsets(expert_offsets, input, num_experts);
   const Fp4Operand x = fp4_operand(input, input_scales, input, fmt, true, "input");
