@@ -3,7 +3,7 @@
 // The same product as fp4_gemm.cu with the operands' roles exchanged: the MMA's M runs over 256
 // weight rows of a CTA pair (128 per CTA) and N over up to 64 rows of the batch, so a stage holds
 // weights, not padding of the batch to 256 rows, and an MMA takes 32 cycles.  Bound by reading the
-// weights (HBM): three stages of 32 KB of codes per SM are in flight (8 experts of 2 x 14336 x 4096,
+// weights (HBM): four stages of 32 KB of codes per SM are in flight (8 experts of 2 x 14336 x 4096,
 // a row each: 79 us for 499 MB, 97 % of the measured copy rate).
 //
 // A CTA's 128 TMEM lanes are 128 features, or (gate / up) 64 gate rows and the same 64 rows of up:

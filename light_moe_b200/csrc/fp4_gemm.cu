@@ -5,8 +5,11 @@
 //
 // Both operands are E2M1 with a scale byte per 32 (MX) or 16 (NV) values (fp4_format.cuh); the
 // block-scaled tcgen05.mma multiplies codes and scales exactly and accumulates in fp32, four
-// times the bf16 rate for a quarter of the bytes.  With few rows the weights' bytes bound it
-// (HBM), with many the tensor pipe.
+// times the bf16 rate for a quarter of the bytes.  With few rows the weights' bytes bound it (HBM).
+// With many, a long run of calls is bound by power (8 experts of 2 x 14336 x 4096, 700 rows each: 373 us at
+// the 1327 MHz that 1000 W leave), a single call by no one part: 310 us at 1965 MHz, 153 of them MMAs;
+// with half of the codes' copies 285, without the loads of the scales too 256, without the copies
+// of the scales to tensor memory 309, without the stores ~295.
 //
 // Tile: 256 rows (128 per CTA, TMEM lane = row) x 192 weight rows (96 per CTA in shared memory).
 // (Narrower tiles for a fuller last round measured slower from 64 rows per expert on: 119 against
@@ -26,11 +29,11 @@
 //
 // One thread issues a unit of four 4-scale words a row (512 values of MX, 256 of NV: twelve copies
 // into one of two TMEM buffers of 48 columns) and its MMAs, in whose order the tensor pipe runs
-// them.  Its waits and issue slots are what a stage costs beside the MMAs: ~65 cycles a wait, ~25
-// an instruction, against 96 cycles an MMA; so a stage holds 512 values and the waits of a unit
-// start together.  (With 256 values and one wait after another: 650 cycles per 384 of MMAs, 0.88
-// ms for the gate / up product of 16384 rows; with the copies issued by a warp of their own they
-// queue behind the MMAs issued before, and the hand-over then stands in the pipe.)
+// them.  A wait costs it ~65 cycles and an instruction ~25, against 96 cycles an MMA; so a stage holds
+// 512 values and the waits of a unit start together.  (With 256 values and one wait after another:
+// 650 cycles per 384 of MMAs, 0.88 ms for the gate / up product of 16384 rows, now 0.79; with the
+// copies issued by a warp of their own they queue behind the MMAs issued before, and the hand-over
+// then stands in the pipe.)
 //
 // Warps: 0 TMA producer, whose copies complete on the leader's stage barrier; 1 MMA issuer
 // (leader CTA); 2-3 scales of the rows, 4-6 scales of the 192 columns (each CTA keeps all: the MMA
