@@ -262,7 +262,7 @@ int lmoe_grouped_gemm_wgrad(const void* grad_output, int dtype, int64_t total_ro
                             void* grad_weights, void* workspace, size_t workspace_bytes, uint32_t* error,
                             lmoe_stream_t stream);
 
-/* lmoe_grouped_gemm for any N, K >= 1 (that entry wants K a multiple of 64 or 4): output
+/* lmoe_grouped_gemm for any N, K >= 1 (that entry wants K a multiple of 128, or for fp32 of 4): output
  * [total_rows, N], zero outside every expert; workspace and error as for the gradients. */
 int lmoe_grouped_gemm_any(const void* input, int dtype, int64_t total_rows, int K, const void* weights, int N,
                           const void* expert_offsets, int offsets_are_int64, int num_experts, void* output,
