@@ -105,7 +105,7 @@ def build_extension(force: bool = False) -> str:
     cmd = ["g++", "-shared", "-fPIC", "-O2", "-std=c++17", src, "-o", out,
            "-DTORCH_EXTENSION_NAME=_C", "-DTORCH_API_INCLUDE_EXTENSION_H", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
            *[f"-I{p}" for p in inc], *[f"-L{p}" for p in libdirs], f"-L{LIBDIR}",
-           "-llmoe_b200", "-lc10", "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10_cuda",
+           "-llmoe_b200", "-lc10", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-lc10_cuda",
            "-Wl,-rpath,$ORIGIN/lib", *[f"-Wl,-rpath,{p}" for p in libdirs]]
     _run(cmd)
     return out

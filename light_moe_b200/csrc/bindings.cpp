@@ -8,6 +8,7 @@
 // the PyTorch caching allocator, the device guard, and launching on the *current* CUDA
 // stream (the reference launches its kernel on the legacy default stream).
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -339,6 +340,11 @@ std::vector<torch::Tensor> moe_layer_w4a16(torch::Tensor x, torch::Tensor gate_w
 
 // ---------------------------------------------------------------- gradients of grouped_gemm
 
+// An uninitialised tensor beside `like`, straight from the allocator.
+torch::Tensor empty_like_device(at::IntArrayRef sizes, torch::ScalarType type, const torch::Tensor& like) {
+  return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt);
+}
+
 void check_same_device(const torch::Tensor& t, const torch::Tensor& like, const char* name) {
   check_cuda(t, name);
   TORCH_CHECK(t.device() == like.device(), name, " must be on ", like.device(), ", is on ", t.device());
@@ -379,7 +385,7 @@ torch::Tensor grouped_gemm_dgrad(torch::Tensor grad_output, torch::Tensor weight
   auto w = contig16(weights);
   const int64_t T = dy.size(0), N = w.size(1), K = w.size(2);
   check_sizes(T, N, K, num_experts);
-  auto out = torch::empty({T, K}, dy.options());
+  auto out = empty_like_device({T, K}, dy.scalar_type(), dy);
   const int dt = dtype_code(dy);
   auto ws = workspace((int64_t)lmoe_grouped_gemm_grad_workspace_bytes(0, dt, T, (int)N, (int)K, (int)num_experts), dy);
   check_status(lmoe_grouped_gemm_dgrad(dy.data_ptr(), dt, T, (int)N, w.data_ptr(), (int)K, off.data_ptr(),
@@ -406,7 +412,7 @@ torch::Tensor grouped_gemm_wgrad(torch::Tensor grad_output, torch::Tensor input,
   auto x = contig16(input);
   const int64_t T = dy.size(0), N = dy.size(1), K = x.size(1);
   check_sizes(T, N, K, num_experts);
-  auto out = torch::empty({num_experts, N, K}, dy.options().dtype(ot));
+  auto out = empty_like_device({num_experts, N, K}, ot, dy);
   const int dt = dtype_code(dy);
   auto ws = workspace((int64_t)lmoe_grouped_gemm_grad_workspace_bytes(1, dt, T, (int)N, (int)K, (int)num_experts), dy);
   check_status(lmoe_grouped_gemm_wgrad(dy.data_ptr(), dt, T, (int)N, x.data_ptr(), (int)K, off.data_ptr(),
@@ -469,11 +475,10 @@ std::tuple<torch::Tensor, torch::Tensor> quantize_fp4(torch::Tensor x, const std
     out_rows = pos.numel();
     shape[0] = out_rows;
   }
-  auto u8 = x.options().dtype(torch::kUInt8);
   shape.back() = K / 2;
-  auto q = torch::empty(shape, u8);
+  auto q = empty_like_device(shape, torch::kUInt8, x);
   shape.back() = lmoe_fp4_scale_pitch((int)K, fmt);
-  auto s = torch::empty(shape, u8);
+  auto s = empty_like_device(shape, torch::kUInt8, x);
   if (rows > 0)
     check_status(lmoe_quantize_fp4(xc.data_ptr(), dtype_code(xc), rows, (int)K, ldx, fmt, g, rps,
                                    pos.defined() ? pos.data_ptr<int32_t>() : nullptr, (int)copies, out_rows,
@@ -555,7 +560,7 @@ torch::Tensor dequantize_fp4(torch::Tensor q, torch::Tensor scales, const std::s
   const float* g = fp4_global_scale(global_scale, q, q.dim() == 3 ? q.size(0) : 1, rows, fmt, &rps);
   auto shape = q.sizes().vec();
   shape.back() = K;
-  auto out = torch::empty(shape, q.options().dtype(torch::kBFloat16));
+  auto out = empty_like_device(shape, torch::kBFloat16, q);
   if (rows > 0)
     check_status(lmoe_dequantize_fp4(o.q.data_ptr<uint8_t>(), o.s.data_ptr<uint8_t>(), o.pitch, rows, (int)K, fmt, g,
                                      rps, out.data_ptr(), cur_stream()),
@@ -615,7 +620,7 @@ torch::Tensor fp4_grouped_gemm(torch::Tensor input, torch::Tensor input_scales, 
   const auto ot = out_dtype.value_or(torch::kBFloat16);
   TORCH_CHECK(ot == torch::kBFloat16 || ot == torch::kFloat16 || ot == torch::kFloat32,
               "out_dtype must be bf16, fp16 or fp32");
-  auto out = torch::empty({T, N}, input.options().dtype(ot));
+  auto out = empty_like_device({T, N}, ot, input);
   if (T > 0 && N > 0)
     check_status(lmoe_fp4_grouped_gemm(x.q.data_ptr<uint8_t>(), x.s.data_ptr<uint8_t>(), x.pitch, T, (int)K,
                                        wp.q.data_ptr<uint8_t>(), wp.s.data_ptr<uint8_t>(),
