@@ -486,3 +486,24 @@ def test_quantize_keeps_the_sign_of_zeros_and_tiny_values(fmt, dt):
     x[2:, 3::4] = -1.0
     x[3] = -0.0
     _check_quantize(x.to(DT[dt]).cuda(), fmt)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+@pytest.mark.parametrize("g", [2.0 ** e for e in (-126, -120, -100, -80, -64, -30, -20, -12, -10, -9, -8, -4, 0, 20, 100)]
+                         + [0.3, 3.7e-5, 1e-33])
+def test_quantize_saturates_values_far_beyond_the_range(dt, g):
+    """Values of both signs up to the largest of their type, alone and beside values at the borders
+    between codes, under a scale at its limit of 448."""
+    gen = np.random.default_rng(5)
+    big = float(torch.finfo(torch.bfloat16).max)
+    rows = []
+    for top in (big, big / 2, 2.0 ** 100, 1.0, 448 * 6 * g, 448 * 6 * g * 1.0625, 448 * 8 * g, 448 * 8 * g * 1.125,
+                448 * g * 2.0 ** 20):
+        for lone in (top, -top):
+            v = gen.choice([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 1.0, -2.5, -5.0, -0.0], 16) * 448 * g
+            v[3] = lone
+            rows += [v, np.full(16, lone)]
+    x = torch.from_numpy(np.clip(np.array(rows), -big, big)).to(torch.bfloat16).to(DT[dt]).reshape(-1, 32).cuda()
+    _check_quantize(x, "nvfp4", g)
+    if dt == "fp32":
+        _check_quantize(torch.nextafter(x, x * 0), "nvfp4", g)   # every bit of the mantissa in use
