@@ -440,7 +440,7 @@ const float* fp4_global_scale(const std::optional<torch::Tensor>& g, const torch
   check_same_device(*g, x, "global_scale");
   TORCH_CHECK(g->scalar_type() == torch::kFloat32 && g->is_contiguous(), "global_scale must be contiguous fp32");
   TORCH_CHECK(g->numel() == 1 || g->numel() == lead, "global_scale must have 1 or ", lead, " elements");
-  *rows_per_scale = std::max<int64_t>(1, g->numel() == 1 ? rows : rows / lead);
+  if (rows > 0) *rows_per_scale = g->numel() == 1 ? rows : rows / lead;   // rows: lead is not 0 either
   return g->data_ptr<float>();
 }
 

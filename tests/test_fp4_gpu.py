@@ -507,3 +507,14 @@ def test_quantize_saturates_values_far_beyond_the_range(dt, g):
     _check_quantize(x, "nvfp4", g)
     if dt == "fp32":
         _check_quantize(torch.nextafter(x, x * 0), "nvfp4", g)   # every bit of the mantissa in use
+
+
+@pytest.mark.parametrize("shape", [(0, 4, 64), (3, 0, 64), (0, 64)])
+def test_empty_batches_with_their_tensor_scales(shape):
+    """No matrices and no scales, no rows under a scale each, and one scale for nothing."""
+    lead = shape[0] if len(shape) == 3 else 1
+    for n in {lead, 1}:
+        g = torch.ones(n, device="cuda")
+        q, s = ops.quantize_fp4(torch.empty(shape, device="cuda"), "nvfp4", g)
+        assert q.shape == shape[:-1] + (32,) and s.shape == shape[:-1] + (4,)
+        assert ops.dequantize_fp4(q, s, "nvfp4", g).shape == shape

@@ -109,3 +109,10 @@ def test_refusals_and_scales():
     assert torch.equal(g, torch.ones(2, device="cuda"))
     g = nvfp4_global_scale(torch.full((4, 32), -5.376, device="cuda"))
     assert g.shape == (1,) and abs(g.item() - 0.002) < 1e-9
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+def test_no_experts(fmt):
+    z = lambda *s: torch.empty(*s, device="cuda")
+    ex = FP4Experts.from_dense(z(0, 64, 32), z(0, 64, 32), z(0, 32, 64), fmt)
+    assert ex.num_experts == 0 and ex.w1[0].shape == (0, 64, 16) and ex.w2[0].shape == (0, 32, 32)
