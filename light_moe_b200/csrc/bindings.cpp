@@ -57,6 +57,12 @@ torch::Tensor workspace(int64_t bytes, const torch::Tensor& like) {
   return torch::empty({bytes > 0 ? bytes : 1}, like.options().dtype(torch::kUInt8));
 }
 
+// Sizes that the kernels count in 32 bits.
+void check_sizes(int64_t rows, int64_t n, int64_t k, int64_t num_experts) {
+  TORCH_CHECK(rows <= INT32_MAX && n <= INT32_MAX && k <= INT32_MAX && num_experts <= INT32_MAX,
+              "sizes must fit 32 bits");
+}
+
 // Row-contiguous and 16-byte aligned (a view may start anywhere).
 torch::Tensor contig16(const torch::Tensor& t) {
   auto c = t.contiguous();
@@ -156,6 +162,7 @@ torch::Tensor grouped_gemm(torch::Tensor input, torch::Tensor weights, torch::Te
   TORCH_CHECK(input.dim() == 2 && weights.dim() == 3, "input [T,K], weights [E,N,K]");
   TORCH_CHECK(weights.size(0) >= num_experts && weights.size(2) == input.size(1), "shape mismatch");
   TORCH_CHECK(expert_offsets.numel() >= num_experts + 1, "expert_offsets must have num_experts + 1 entries");
+  check_sizes(input.size(0), weights.size(1), input.size(1), num_experts);
   const c10::cuda::OptionalCUDAGuard guard(input.device());
   // computed in the input dtype (bf16 / fp16 on tensor cores, fp32 on CUDA cores), like the
   // reference's per-expert mm_out (csrc/grouped_gemm.cu:24-40); the weights follow the input
@@ -348,12 +355,6 @@ torch::Tensor empty_like_device(at::IntArrayRef sizes, torch::ScalarType type, c
 void check_same_device(const torch::Tensor& t, const torch::Tensor& like, const char* name) {
   check_cuda(t, name);
   TORCH_CHECK(t.device() == like.device(), name, " must be on ", like.device(), ", is on ", t.device());
-}
-
-// Sizes that the kernels count in 32 bits.
-void check_sizes(int64_t rows, int64_t n, int64_t k, int64_t num_experts) {
-  TORCH_CHECK(rows <= INT32_MAX && n <= INT32_MAX && k <= INT32_MAX && num_experts <= INT32_MAX,
-              "sizes must fit 32 bits");
 }
 
 torch::Tensor check_offsets(const torch::Tensor& offsets, const torch::Tensor& like, int64_t num_experts) {

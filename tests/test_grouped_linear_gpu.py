@@ -172,3 +172,16 @@ def test_experts_without_tokens_and_with_odd_indices():
     two = m(x, torch.full((5, 2), 2, device="cuda"), torch.full((5, 2), 0.5, device="cuda"))
     none = m(x, torch.tensor([[-1, 2, 3]], device="cuda").expand(5, 3), torch.ones(5, 3, device="cuda"))
     assert torch.equal(one, two) and torch.equal(one, none)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+def test_sizes_beyond_32_bits_are_refused(dt):
+    """A size is never cut to its lower 32 bits (2^32 + 5 would count as 5).  The operands are views of
+    one value: nothing of that size is allocated."""
+    one = torch.ones(1, device="cuda", dtype=DT[dt])
+    off = torch.tensor([0, 1], device="cuda")
+    big = 2 ** 32 + 5
+    for x, w in ((one.view(1, 1), one.expand(1, big, 1)), (one.expand(1, big), one.expand(1, 1, big)),
+                 (one.expand(big, 1), one.view(1, 1, 1))):
+        with pytest.raises(RuntimeError, match="32 bits"):
+            ops.grouped_gemm(x, w, off, 1)
