@@ -166,8 +166,8 @@ torch::Tensor grouped_gemm(torch::Tensor input, torch::Tensor weights, torch::Te
   const c10::cuda::OptionalCUDAGuard guard(input.device());
   // computed in the input dtype (bf16 / fp16 on tensor cores, fp32 on CUDA cores), like the
   // reference's per-expert mm_out (csrc/grouped_gemm.cu:24-40); the weights follow the input
-  auto x = as_kernel_type(input);
-  auto w = weights.scalar_type() == x.scalar_type() ? weights.contiguous() : weights.to(x.scalar_type()).contiguous();
+  auto x = contig16(as_kernel_type(input));
+  auto w = contig16(weights.scalar_type() == x.scalar_type() ? weights : weights.to(x.scalar_type()));
   auto off = expert_offsets.contiguous();
   TORCH_CHECK(off.scalar_type() == torch::kInt64 || off.scalar_type() == torch::kInt32, "offsets int64/int32");
   const int64_t T = x.size(0), K = x.size(1), N = w.size(1);
@@ -175,10 +175,9 @@ torch::Tensor grouped_gemm(torch::Tensor input, torch::Tensor weights, torch::Te
   if (T == 0 && num_experts >= 1) return out.to(input.scalar_type());   // no rows, nothing to launch
   // row lengths that the kernels above do not take
   if (K > 0 && N > 0 && (x.scalar_type() == torch::kFloat32 ? K % 4 != 0 : K % 128 != 0)) {
-    auto xa = contig16(x), wa = contig16(w);
-    const int dt = dtype_code(xa);
-    auto ws = workspace((int64_t)lmoe_grouped_gemm_grad_workspace_bytes(2, dt, T, (int)N, (int)K, (int)num_experts), xa);
-    check_status(lmoe_grouped_gemm_any(xa.data_ptr(), dt, T, (int)K, wa.data_ptr(), (int)N, off.data_ptr(),
+    const int dt = dtype_code(x);
+    auto ws = workspace((int64_t)lmoe_grouped_gemm_grad_workspace_bytes(2, dt, T, (int)N, (int)K, (int)num_experts), x);
+    check_status(lmoe_grouped_gemm_any(x.data_ptr(), dt, T, (int)K, w.data_ptr(), (int)N, off.data_ptr(),
                                        off.scalar_type() == torch::kInt64 ? 1 : 0, (int)num_experts, out.data_ptr(),
                                        ws.data_ptr(), ws.numel(), nullptr, cur_stream()),
                  "grouped_gemm");

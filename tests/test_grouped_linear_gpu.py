@@ -185,3 +185,20 @@ def test_sizes_beyond_32_bits_are_refused(dt):
                  (one.expand(big, 1), one.view(1, 1, 1))):
         with pytest.raises(RuntimeError, match="32 bits"):
             ops.grouped_gemm(x, w, off, 1)
+
+
+@pytest.mark.parametrize("dt,k", [("bf16", 128), ("fp16", 128), ("fp32", 64), ("bf16", 130), ("fp32", 33)])
+def test_operands_that_start_anywhere(dt, k):
+    """Contiguous views one value behind an aligned address, forward and through autograd."""
+    gen = torch.Generator(device="cuda").manual_seed(k)
+    x = torch.randn(5 * k + 1, generator=gen, device="cuda").to(DT[dt])[1:].view(5, k)
+    w = torch.randn(2 * 24 * k + 1, generator=gen, device="cuda").to(DT[dt])[1:].view(2, 24, k)
+    off = torch.tensor([0, 2, 5], device="cuda")
+    want = ops.grouped_gemm(x.clone(), w.clone(), off, 2)
+    assert torch.equal(ops.grouped_gemm(x, w, off, 2), want)
+    xl, wl = x.detach().requires_grad_(), w.detach().requires_grad_()
+    y = grouped_linear(xl, wl, off)
+    y.sum().backward()
+    assert torch.equal(y, want)
+    assert torch.equal(xl.grad, ops.grouped_gemm_dgrad(torch.ones_like(y), w.clone(), off, 2))
+    assert torch.equal(wl.grad, ops.grouped_gemm_wgrad(torch.ones_like(y), x.clone(), off, 2))
