@@ -235,7 +235,7 @@ int lmoe_w4a16_grouped_gemm(const void* input, int64_t total_rows, int K, const 
 /* Gradients of lmoe_grouped_gemm, y[r, n] = sum_k input[r, k] * weights[e, n, k], for the rows
  * [offsets[e], offsets[e + 1]) of expert e; dtype of all operands LMOE_DTYPE_* (bf16 and fp16 on
  * tensor cores with fp32 accumulation; fp32 as sums of bf16 products of fp32 accuracy on tensor
- * cores, or in fp32 on CUDA cores); any N, K >= 1.
+ * cores, or in fp32 on CUDA cores); any N, K >= 1.  total_rows, N and K up to 2^31 - 1025.
  *   dgrad: grad_input [total_rows, K] = grad_output [total_rows, N] * weights [E, N, K] of the
  *          row's expert; rows outside every expert are zero
  *   wgrad: grad_weights [E, N, K] (out_dtype: dtype or LMOE_DTYPE_F32), the sum over the
@@ -263,7 +263,7 @@ int lmoe_grouped_gemm_wgrad(const void* grad_output, int dtype, int64_t total_ro
                             lmoe_stream_t stream);
 
 /* lmoe_grouped_gemm for any N, K >= 1 (that entry wants K a multiple of 128, or for fp32 of 4): output
- * [total_rows, N], zero outside every expert; workspace and error as for the gradients. */
+ * [total_rows, N], zero outside every expert; sizes, workspace and error as for the gradients. */
 int lmoe_grouped_gemm_any(const void* input, int dtype, int64_t total_rows, int K, const void* weights, int N,
                           const void* expert_offsets, int offsets_are_int64, int num_experts, void* output,
                           void* workspace, size_t workspace_bytes, uint32_t* error, lmoe_stream_t stream);
@@ -303,7 +303,7 @@ int lmoe_dequantize_fp4(const uint8_t* q, const uint8_t* scales, int64_t scale_p
  * [E, N, K/2], scales [E, N, ws_pitch]; both operands of the same format, pitches multiples of 32
  * and at least lmoe_fp4_scale_pitch, codes 16-byte and scales 32-byte aligned.  alpha, alpha_up: fp32 [E] or NULL
  * (1): the product of the two tensor scales.  output [total_rows, N] of out_dtype; rows outside
- * every expert are zero.  error: as above. */
+ * every expert are zero.  total_rows, N and K up to 2^31 - 1025.  error: as above. */
 int lmoe_fp4_grouped_gemm(const uint8_t* xq, const uint8_t* xs, int64_t xs_pitch, int64_t total_rows, int K,
                           const uint8_t* wq, const uint8_t* ws, const uint8_t* wq_up, const uint8_t* ws_up,
                           int64_t ws_pitch, int N, int format, const void* expert_offsets, int offsets_are_int64,

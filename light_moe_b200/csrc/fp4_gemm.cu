@@ -443,7 +443,9 @@ extern "C" int lmoe_fp4_grouped_gemm(const uint8_t* xq, const uint8_t* xs, int64
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
   LMOE_ARG_CHECK(format == LMOE_FP4_MX || format == LMOE_FP4_NV);
   LMOE_ARG_CHECK(out_dtype == LMOE_DTYPE_BF16 || out_dtype == LMOE_DTYPE_F16 || out_dtype == LMOE_DTYPE_F32);
-  LMOE_ARG_CHECK(total_rows >= 0 && total_rows <= INT32_MAX - 1024 && N > 0 && K > 0 && K % 32 == 0);
+  LMOE_ARG_CHECK(total_rows >= 0 && N > 0 && K > 0 && K % 32 == 0);
+  // indexes of whole tiles and stages stay within 32 bits
+  LMOE_ARG_CHECK(total_rows <= kMaxGemmSize && N <= kMaxGemmSize && K <= kMaxGemmSize);
   LMOE_ARG_CHECK(num_experts >= 1);
   if (num_experts > kMaxGemmExperts) return LMOE_ERR_UNSUPPORTED;
   LMOE_ARG_CHECK((wq_up == nullptr) == (ws_up == nullptr));

@@ -535,7 +535,9 @@ int grad_entry(GradProblem& p, const void* offsets, void* out, void* workspace, 
                cudaStream_t stream) {
   LMOE_ARG_CHECK(p.dtype == LMOE_DTYPE_BF16 || p.dtype == LMOE_DTYPE_F16 || p.dtype == LMOE_DTYPE_F32);
   LMOE_ARG_CHECK(p.out_dtype == p.dtype || (weight_grad(p) && p.out_dtype == LMOE_DTYPE_F32));
-  LMOE_ARG_CHECK(p.total_rows >= 0 && p.total_rows <= INT32_MAX - 1024 && p.N > 0 && p.K > 0 && p.num_experts >= 1);
+  LMOE_ARG_CHECK(p.total_rows >= 0 && p.N > 0 && p.K > 0 && p.num_experts >= 1);
+  // indexes of whole tiles and stages stay within 32 bits
+  LMOE_ARG_CHECK(p.total_rows <= kMaxGemmSize && p.N <= kMaxGemmSize && p.K <= kMaxGemmSize);
   if (p.num_experts > kMaxGemmExperts) return LMOE_ERR_UNSUPPORTED;
   const int64_t esize = p.dtype == LMOE_DTYPE_F32 ? 4 : 2, osize = p.out_dtype == LMOE_DTYPE_F32 ? 4 : 2;
   LMOE_ARG_CHECK(out && reinterpret_cast<uintptr_t>(out) % osize == 0);

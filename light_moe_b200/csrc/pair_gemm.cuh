@@ -18,6 +18,9 @@
 
 namespace lmoe {
 
+// The most rows and columns of an operand: the next tile or stage (at most 1024) starts below 2^31.
+constexpr int64_t kMaxGemmSize = INT32_MAX - 1024;
+
 // ---------------------------------------------------------------------------------------
 // clusters
 // ---------------------------------------------------------------------------------------

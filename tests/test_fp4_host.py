@@ -143,3 +143,17 @@ def test_reference_codes():
 @pytest.mark.parametrize("bad", [dict(xs=P + 16), dict(ws=P + 16), dict(uq=P, us=P + 16)])
 def test_gemm_wants_scales_on_whole_sectors(bad):
     assert _gemm(**bad) == INVALID
+
+
+TOP = 2 ** 31 - 1024   # sizes from here on leave no room for the index of the tile behind the last
+
+
+def test_sizes_whose_tiles_pass_32_bits_are_refused():
+    for K in (TOP, 2 ** 31 - 32):
+        assert _gemm(K=K, xp=2 ** 27, wp=2 ** 27) == INVALID
+    assert _gemm(N=TOP) == INVALID and _gemm(R=TOP) == INVALID
+    for n in (TOP, 2 ** 31 - 1):
+        assert _dgrad(N=n, ws=P, wb=2 ** 62) == INVALID and _dgrad(K=n, ws=P, wb=2 ** 62) == INVALID
+        assert _wgrad(N=n, ws=P, wb=2 ** 62) == INVALID and _wgrad(K=n, ws=P, wb=2 ** 62) == INVALID
+        for nk in ((n, 8), (8, n)):
+            assert capi.lib().lmoe_grouped_gemm_any(P, 2, 4, nk[1], P, nk[0], P, 0, 2, P, None, 0, None, None) == INVALID
