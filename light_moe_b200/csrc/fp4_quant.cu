@@ -207,7 +207,7 @@ RowGrid row_grid(int chunks, int64_t rows) {
 template <typename T>
 void launch_quantize(const QuantArgs& a, cudaStream_t stream) {
   // chunks of the padded scale row: the threads behind the last column zero its padding
-  const int chunks = (int)a.pitch * fp4_block(a.format) / 32;
+  const int chunks = (int)(a.pitch * fp4_block(a.format) / 32);
   const RowGrid g = row_grid(chunks, a.rows);
   if (a.format == LMOE_FP4_MX)
     quantize_fp4_kernel<T, LMOE_FP4_MX><<<g.grid, g.block, 0, stream>>>(a);

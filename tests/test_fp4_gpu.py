@@ -518,3 +518,18 @@ def test_empty_batches_with_their_tensor_scales(shape):
         q, s = ops.quantize_fp4(torch.empty(shape, device="cuda"), "nvfp4", g)
         assert q.shape == shape[:-1] + (32,) and s.shape == shape[:-1] + (4,)
         assert ops.dequantize_fp4(q, s, "nvfp4", g).shape == shape
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+def test_quantize_the_longest_row(fmt):
+    """K = 2^31 - 32: the padded scale row stands for 2^31 values."""
+    K = 2 ** 31 - 32
+    x = torch.zeros(1, K, device="cuda", dtype=torch.bfloat16)
+    places = torch.tensor([0, 40, 2 ** 30 + 64, K - 1], device="cuda")
+    x[0, places] = torch.tensor([6.0, -3.0, 1.5, 4.0], device="cuda", dtype=torch.bfloat16)
+    q, s = ops.quantize_fp4(x, fmt)
+    assert q.shape == (1, K // 2) and s.shape == (1, K // ref.BLOCK[fmt])
+    v = ops.dequantize_fp4(q, s, fmt)
+    if fmt == "nvfp4":
+        x[0, K - 1] = 4.125   # 4 / 6 has the scale 0.6875, between 0.625 and 0.6875, and 4 / 0.6875 the code 6
+    assert torch.equal(v, x)
