@@ -70,7 +70,8 @@ class FP4MoELayer(HostBufferCalls, torch.nn.Module):
 
     ``input_scale`` / ``hidden_scale``: nvfp4 tensor scales (fp32, one value) of the tokens and of
     the experts' hidden rows, from a calibration; None = 1, which suits blocks whose largest value
-    lies between about 0.1 and 2688."""
+    lies between about 0.1 and 2688.  They are buffers: values copied into them hold from the next
+    call (or graph replay) on."""
 
     def __init__(self, gate_weight: torch.Tensor, experts: FP4Experts, top_k: int,
                  gate_bias: Optional[torch.Tensor] = None, input_scale: Optional[torch.Tensor] = None,
@@ -88,10 +89,11 @@ class FP4MoELayer(HostBufferCalls, torch.nn.Module):
         self.register_buffer("hidden_scale", one(hidden_scale))
         self.experts = e
         self.top_k = int(top_k)
-        times = lambda g, s: None if g is None else (g if s is None else (g * s).contiguous())
-        self.register_buffer("_alpha1", times(e.g1, self.input_scale))
-        self.register_buffer("_alpha3", times(e.g3, self.input_scale))
-        self.register_buffer("_alpha2", times(e.g2, self.hidden_scale))
+
+    def _load_from_state_dict(self, state_dict, prefix, *args, **kwargs):
+        for name in ("_alpha1", "_alpha2", "_alpha3"):   # factors that earlier layers saved beside their scales
+            state_dict.pop(prefix + name, None)
+        super()._load_from_state_dict(state_dict, prefix, *args, **kwargs)
 
     def forward(self, x: torch.Tensor, return_routing: bool = False):
         e, k = self.experts, self.top_k
@@ -112,10 +114,13 @@ class FP4MoELayer(HostBufferCalls, torch.nn.Module):
             offsets = torch.cat([offsets[:-1], base])
             combine = torch.cat([weights, weights.new_ones(T, S)], 1)
             segments, slots = segments + S, k + S
+        # the products' factors, from the scales as they are now (a new calibration may have been copied in)
+        times = lambda g, s: g if g is None or s is None else g * s
         xq, xs = ops.quantize_fp4(x2, e.format, self.input_scale, positions=positions.contiguous())
-        h = ops.fp4_grouped_gemm(xq, xs, *e.w1, offsets, segments, e.format, alpha=self._alpha1,
-                                 weights_up=e.w3[0], weight_scales_up=e.w3[1], alpha_up=self._alpha3)
+        h = ops.fp4_grouped_gemm(xq, xs, *e.w1, offsets, segments, e.format, alpha=times(e.g1, self.input_scale),
+                                 weights_up=e.w3[0], weight_scales_up=e.w3[1],
+                                 alpha_up=times(e.g3, self.input_scale))
         hq, hs = ops.quantize_fp4(h, e.format, self.hidden_scale)
-        o = ops.fp4_grouped_gemm(hq, hs, *e.w2, offsets, segments, e.format, alpha=self._alpha2)
+        o = ops.fp4_grouped_gemm(hq, hs, *e.w2, offsets, segments, e.format, alpha=times(e.g2, self.hidden_scale))
         y = ops.combine_rows(o, positions, combine, T, slots).view(shape)
         return (y, ids, weights) if return_routing else y

@@ -116,3 +116,25 @@ def test_no_experts(fmt):
     z = lambda *s: torch.empty(*s, device="cuda")
     ex = FP4Experts.from_dense(z(0, 64, 32), z(0, 64, 32), z(0, 32, 64), fmt)
     assert ex.num_experts == 0 and ex.w1[0].shape == (0, 64, 16) and ex.w2[0].shape == (0, 32, 32)
+
+
+def test_new_scales_hold_from_the_next_call_on():
+    """Values copied into the layer's scales, loaded or copied before a replay reach the quantisers and
+    the products alike."""
+    x, mod, _ = _make(37, 256, 96, 8, 2, "nvfp4", 1, 1, True)
+    graph = torch.cuda.CUDAGraph()
+    mod(x)
+    with torch.cuda.graph(graph):
+        yg = mod(x)
+    for scale in (4.0, 0.25):
+        mod.input_scale.fill_(0.002 * scale)
+        mod.hidden_scale.mul_(scale)
+        want = _by_hand(mod, x, 37, 2)[0]
+        assert torch.equal(mod(x), want)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(yg, want)
+    other = _make(37, 256, 96, 8, 2, "nvfp4", 1, 1, True)[1]
+    saved = dict(mod.state_dict(), _alpha1=torch.ones(9), _alpha2=torch.ones(9), _alpha3=torch.ones(9))
+    other.load_state_dict(saved)
+    assert torch.equal(other(x), want)
