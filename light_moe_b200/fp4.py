@@ -90,6 +90,15 @@ class FP4MoELayer(HostBufferCalls, torch.nn.Module):
         self.experts = e
         self.top_k = int(top_k)
 
+    def _apply(self, fn, *args, **kwargs):
+        # a move to another device takes the scales along, a cast leaves them in fp32
+        scales = {n: b for n, b in self._buffers.items() if b is not None and n in ("input_scale", "hidden_scale")}
+        super()._apply(fn, *args, **kwargs)
+        for name, scale in scales.items():
+            if self._buffers[name].dtype != torch.float32:
+                self._buffers[name] = scale.to(self._buffers[name].device)
+        return self
+
     def _load_from_state_dict(self, state_dict, prefix, *args, **kwargs):
         for name in ("_alpha1", "_alpha2", "_alpha3"):   # factors that earlier layers saved beside their scales
             state_dict.pop(prefix + name, None)

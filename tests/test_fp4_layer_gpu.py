@@ -138,3 +138,20 @@ def test_new_scales_hold_from_the_next_call_on():
     saved = dict(mod.state_dict(), _alpha1=torch.ones(9), _alpha2=torch.ones(9), _alpha3=torch.ones(9))
     other.load_state_dict(saved)
     assert torch.equal(other(x), want)
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16, torch.float32, torch.float64])
+def test_casts_leave_the_scales_in_fp32(dt):
+    x, mod, _ = _make(37, 256, 96, 8, 2, "nvfp4", 1, 1, True)
+    y, scales = mod(x), (mod.input_scale.clone(), mod.hidden_scale.clone())
+    mod.to(dt)
+    assert mod.gate_weight.dtype == dt
+    for a, b in zip((mod.input_scale, mod.hidden_scale), scales):
+        assert a.dtype == torch.float32 and torch.equal(a, b)
+    z = mod(x)
+    assert z.shape == y.shape and z.dtype == y.dtype
+    if dt == torch.bfloat16:
+        assert torch.equal(z, y)
+    mod.cpu()
+    assert all(b.device.type == "cpu" for b in mod.buffers())
+    assert mod.cuda().input_scale.device == x.device
