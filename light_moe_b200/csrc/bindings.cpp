@@ -370,8 +370,16 @@ void check_float(const torch::Tensor& t, const char* name) {
               " must be bf16, fp16 or fp32, is ", st);
 }
 
+// The caller's error word, or none.
+uint32_t* error_word(const std::optional<torch::Tensor>& error, const torch::Tensor& like) {
+  if (!error.has_value() || !error->defined()) return nullptr;
+  check_same_device(*error, like, "error");
+  TORCH_CHECK(error->scalar_type() == torch::kInt32 && error->numel() == 1, "error must be one int32 value");
+  return reinterpret_cast<uint32_t*>(error->data_ptr());
+}
+
 torch::Tensor grouped_gemm_dgrad(torch::Tensor grad_output, torch::Tensor weights, torch::Tensor expert_offsets,
-                                 int64_t num_experts) {
+                                 int64_t num_experts, std::optional<torch::Tensor> error) {
   check_cuda(grad_output, "grad_output");
   check_same_device(weights, grad_output, "weights");
   check_float(grad_output, "grad_output");
@@ -390,13 +398,14 @@ torch::Tensor grouped_gemm_dgrad(torch::Tensor grad_output, torch::Tensor weight
   auto ws = workspace((int64_t)lmoe_grouped_gemm_grad_workspace_bytes(0, dt, T, (int)N, (int)K, (int)num_experts), dy);
   check_status(lmoe_grouped_gemm_dgrad(dy.data_ptr(), dt, T, (int)N, w.data_ptr(), (int)K, off.data_ptr(),
                                        off.scalar_type() == torch::kInt64, (int)num_experts, out.data_ptr(),
-                                       ws.data_ptr(), ws.numel(), nullptr, cur_stream()),
+                                       ws.data_ptr(), ws.numel(), error_word(error, dy), cur_stream()),
                "grouped_gemm_dgrad");
   return out;
 }
 
 torch::Tensor grouped_gemm_wgrad(torch::Tensor grad_output, torch::Tensor input, torch::Tensor expert_offsets,
-                                 int64_t num_experts, std::optional<torch::ScalarType> out_dtype) {
+                                 int64_t num_experts, std::optional<torch::ScalarType> out_dtype,
+                                 std::optional<torch::Tensor> error) {
   check_cuda(grad_output, "grad_output");
   check_same_device(input, grad_output, "input");
   check_float(grad_output, "grad_output");
@@ -417,7 +426,7 @@ torch::Tensor grouped_gemm_wgrad(torch::Tensor grad_output, torch::Tensor input,
   auto ws = workspace((int64_t)lmoe_grouped_gemm_grad_workspace_bytes(1, dt, T, (int)N, (int)K, (int)num_experts), dy);
   check_status(lmoe_grouped_gemm_wgrad(dy.data_ptr(), dt, T, (int)N, x.data_ptr(), (int)K, off.data_ptr(),
                                        off.scalar_type() == torch::kInt64, (int)num_experts, dtype_code(out),
-                                       out.data_ptr(), ws.data_ptr(), ws.numel(), nullptr, cur_stream()),
+                                       out.data_ptr(), ws.data_ptr(), ws.numel(), error_word(error, dy), cur_stream()),
                "grouped_gemm_wgrad");
   return out;
 }
@@ -581,7 +590,8 @@ torch::Tensor fp4_grouped_gemm(torch::Tensor input, torch::Tensor input_scales, 
                                torch::Tensor weight_scales, torch::Tensor expert_offsets, int64_t num_experts,
                                const std::string& format, std::optional<torch::Tensor> alpha,
                                std::optional<torch::Tensor> weights_up, std::optional<torch::Tensor> weight_scales_up,
-                               std::optional<torch::Tensor> alpha_up, std::optional<torch::ScalarType> out_dtype) {
+                               std::optional<torch::Tensor> alpha_up, std::optional<torch::ScalarType> out_dtype,
+                               std::optional<torch::Tensor> error) {
   check_cuda(input, "input");
   const int fmt = fp4_format(format);
   TORCH_CHECK(input.dim() == 2 && weights.dim() == 3, "input [T,K/2], weights [E,N,K/2]");
@@ -620,6 +630,7 @@ torch::Tensor fp4_grouped_gemm(torch::Tensor input, torch::Tensor input_scales, 
   const auto ot = out_dtype.value_or(torch::kBFloat16);
   TORCH_CHECK(ot == torch::kBFloat16 || ot == torch::kFloat16 || ot == torch::kFloat32,
               "out_dtype must be bf16, fp16 or fp32");
+  uint32_t* err = error_word(error, input);
   auto out = empty_like_device({T, N}, ot, input);
   if (T > 0 && N > 0)
     check_status(lmoe_fp4_grouped_gemm(x.q.data_ptr<uint8_t>(), x.s.data_ptr<uint8_t>(), x.pitch, T, (int)K,
@@ -627,7 +638,7 @@ torch::Tensor fp4_grouped_gemm(torch::Tensor input, torch::Tensor input_scales, 
                                        swiglu ? u.q.data_ptr<uint8_t>() : nullptr,
                                        swiglu ? u.s.data_ptr<uint8_t>() : nullptr, wp.pitch, (int)N, fmt,
                                        off.data_ptr(), off.scalar_type() == torch::kInt64, (int)num_experts, al, au,
-                                       dtype_code(out), out.data_ptr(), nullptr, cur_stream()),
+                                       dtype_code(out), out.data_ptr(), err, cur_stream()),
                  "fp4_grouped_gemm");
   return out;
 }
@@ -658,9 +669,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("row_scale") = py::none(), py::arg("out_rows") = 0, py::arg("max_rows_per_expert") = 0,
         py::arg("segment_expert") = py::none());
   m.def("grouped_gemm_dgrad", &grouped_gemm_dgrad, "Input gradient of grouped_gemm", py::arg("grad_output"),
-        py::arg("weights"), py::arg("expert_offsets"), py::arg("num_experts"));
+        py::arg("weights"), py::arg("expert_offsets"), py::arg("num_experts"), py::arg("error") = py::none());
   m.def("grouped_gemm_wgrad", &grouped_gemm_wgrad, "Weight gradient of grouped_gemm", py::arg("grad_output"),
-        py::arg("input"), py::arg("expert_offsets"), py::arg("num_experts"), py::arg("out_dtype") = py::none());
+        py::arg("input"), py::arg("expert_offsets"), py::arg("num_experts"), py::arg("out_dtype") = py::none(),
+        py::arg("error") = py::none());
   m.def("quantize_fp4", &quantize_fp4, "Rows -> microscaled 4-bit floating point", py::arg("x"), py::arg("format"),
         py::arg("global_scale") = py::none(), py::arg("positions") = py::none());
   m.def("dequantize_fp4", &dequantize_fp4, "Microscaled 4-bit floating point -> bf16", py::arg("q"),
@@ -669,7 +681,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("input_scales"), py::arg("weights"), py::arg("weight_scales"), py::arg("expert_offsets"),
         py::arg("num_experts"), py::arg("format"), py::arg("alpha") = py::none(), py::arg("weights_up") = py::none(),
         py::arg("weight_scales_up") = py::none(), py::arg("alpha_up") = py::none(),
-        py::arg("out_dtype") = py::none());
+        py::arg("out_dtype") = py::none(), py::arg("error") = py::none());
   m.def("combine_rows", &combine_rows, "Weighted combine of slot rows back to tokens", py::arg("rows"),
         py::arg("positions"), py::arg("weights"), py::arg("num_tokens"), py::arg("top_k"),
         py::arg("extra_rows") = py::none(), py::arg("num_extra") = 0);

@@ -82,18 +82,22 @@ def w4a16_grouped_gemm(input, packed, expert_offsets, num_experts, N, group_size
                                           max_rows_per_expert, segment_expert)
 
 
-def grouped_gemm_dgrad(grad_output, weights, expert_offsets, num_experts):
+def grouped_gemm_dgrad(grad_output, weights, expert_offsets, num_experts, error=None):
     """Input gradient of grouped_gemm: [T, N] x [E, N, K] -> [T, K] (rows outside every expert are
     zero).  bf16 / fp16 on tensor cores, fp32 in fp32 accuracy (values below 2**-107 to 2**-134);
-    any N, K; operands of one dtype."""
-    return extension().grouped_gemm_dgrad(grad_output, weights, expert_offsets, num_experts)
+    any N, K; operands of one dtype.
+
+    Offsets that decrease or leave [0, T] put every row outside the experts.  ``error``: one int32
+    value on the device, zeroed by the caller (None: nobody asks); such offsets and a kernel that gave
+    up waiting, whose output is not whole, set it.  Nothing waits for the device to look at it."""
+    return extension().grouped_gemm_dgrad(grad_output, weights, expert_offsets, num_experts, error)
 
 
-def grouped_gemm_wgrad(grad_output, input, expert_offsets, num_experts, out_dtype=None):
+def grouped_gemm_wgrad(grad_output, input, expert_offsets, num_experts, out_dtype=None, error=None):
     """Weight gradient of grouped_gemm: sum over each expert's rows of grad_output^T input ->
     [E, N, K] in the operands' dtype or, with ``out_dtype=torch.float32``, unrounded; experts
-    without rows are zero."""
-    return extension().grouped_gemm_wgrad(grad_output, input, expert_offsets, num_experts, out_dtype)
+    without rows are zero.  ``error`` as for the input gradient."""
+    return extension().grouped_gemm_wgrad(grad_output, input, expert_offsets, num_experts, out_dtype, error)
 
 
 def quantize_fp4(x, format, global_scale=None, positions=None):
@@ -116,13 +120,14 @@ def dequantize_fp4(q, scales, format, global_scale=None):
 
 
 def fp4_grouped_gemm(input, input_scales, weights, weight_scales, expert_offsets, num_experts, format,
-                     alpha=None, weights_up=None, weight_scales_up=None, alpha_up=None, out_dtype=None):
+                     alpha=None, weights_up=None, weight_scales_up=None, alpha_up=None, out_dtype=None, error=None):
     """Grouped product of 4-bit operands (codes and scales as quantize_fp4 returns them): rows
     [T, K] x weights [E, N, K] -> [T, N] of ``out_dtype`` (bf16 by default), times ``alpha[e]``
     (fp32 [E], the product of the operands' global scales).  With ``weights_up``:
-    silu(gate) * up.  Exact products, fp32 accumulation; rows outside every expert are zero."""
+    silu(gate) * up.  Exact products, fp32 accumulation; rows outside every expert are zero.
+    ``error`` as for grouped_gemm_dgrad."""
     return extension().fp4_grouped_gemm(input, input_scales, weights, weight_scales, expert_offsets, num_experts,
-                                        format, alpha, weights_up, weight_scales_up, alpha_up, out_dtype)
+                                        format, alpha, weights_up, weight_scales_up, alpha_up, out_dtype, error)
 
 
 def combine_rows(rows, positions, weights, num_tokens, top_k, extra_rows=None, num_extra=0):

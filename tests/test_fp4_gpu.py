@@ -533,3 +533,15 @@ def test_quantize_the_longest_row(fmt):
     if fmt == "nvfp4":
         x[0, K - 1] = 4.125   # 4 / 6 has the scale 0.6875, between 0.625 and 0.6875, and 4 / 0.6875 the code 6
     assert torch.equal(v, x)
+
+
+@pytest.mark.parametrize("rows", [100, 400])   # one for each kernel
+def test_error_words_of_the_product(rows):
+    x, w = ops.quantize_fp4(torch.ones(rows, 64, device="cuda"), "mxfp4"), ops.quantize_fp4(torch.ones(3, 40, 64, device="cuda"), "mxfp4")
+    for offsets, bad in (([0, 50, 40, rows], True), ([0, 20, 40, rows + 1], True), ([0, 20, 40, rows], False)):
+        off = torch.tensor(offsets, dtype=torch.int32, device="cuda")
+        e = torch.zeros(1, dtype=torch.int32, device="cuda")
+        y = ops.fp4_grouped_gemm(*x, *w, off, 3, "mxfp4", error=e)
+        assert (e.item() != 0) == bad and (y != 0).any().item() != bad
+    with pytest.raises(RuntimeError):
+        ops.fp4_grouped_gemm(*x, *w, off, 3, "mxfp4", error=e.float())

@@ -261,3 +261,23 @@ def test_calls_at_once_and_replayed(dt, counts, N, K):
         graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(gx, want[1][0]) and torch.equal(gw, want[1][1])
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+@pytest.mark.parametrize("offsets", [[0, 50, 40, 100], [0, 20, 40, 101], [0, 50, 60, 100]])
+def test_error_words_of_the_operators(dt, offsets):
+    """Bad offsets set the caller's word and good ones leave it; fp32 sizes for CUDA cores and for planes."""
+    bad = offsets != [0, 50, 60, 100]
+    off = torch.tensor(offsets, dtype=torch.int32, device="cuda")
+    for N, K in ((64, 64), (2048, 2880)):
+        dy, x, w = (torch.ones(*s, device="cuda", dtype=DT[dt]) for s in ((100, N), (100, K), (3, N, K)))
+        for call in (lambda e: ops.grouped_gemm_dgrad(dy, w, off, 3, error=e),
+                     lambda e: ops.grouped_gemm_wgrad(dy, x, off, 3, error=e)):
+            e = torch.zeros(1, dtype=torch.int32, device="cuda")
+            y = call(e)
+            assert (e.item() != 0) == bad and (y != 0).any().item() != bad
+    for e in (torch.zeros(1, device="cuda"), torch.zeros(1, dtype=torch.int32), torch.zeros(2, dtype=torch.int32, device="cuda")):
+        with pytest.raises(RuntimeError):
+            ops.grouped_gemm_dgrad(dy, w, off, 3, error=e)
+        with pytest.raises(RuntimeError):
+            ops.grouped_gemm_wgrad(dy, x, off, 3, error=e)
