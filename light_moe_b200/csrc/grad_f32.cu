@@ -20,7 +20,7 @@ namespace lmoe {
 namespace {
 
 constexpr int kT = 128, kTK = 16, kNT = 256;
-constexpr uint32_t kSite = 0x700u;
+constexpr uint32_t kSite = 0xa00u;
 
 struct F32Args {
   const float* dy;      // [R, N]

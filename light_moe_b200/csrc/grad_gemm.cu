@@ -48,7 +48,7 @@ constexpr uint32_t kChunk = kSK * 128;            // 128 contraction rows of 64 
 constexpr uint32_t kOperand = 2 * kChunk;         // 128 x 128 values of one operand
 constexpr uint32_t kStageBytes = 2 * kOperand;
 constexpr uint32_t kBlockBytes = 32 * 128;        // a warp's block on its way out
-constexpr uint32_t kSite = 0x600u;
+constexpr uint32_t kSite = 0x900u;
 
 struct __align__(8) Bars {
   uint64_t full[kStages];       // leader: both CTAs' operands landed (one arrival each)

@@ -281,3 +281,18 @@ def test_error_words_of_the_operators(dt, offsets):
             ops.grouped_gemm_dgrad(dy, w, off, 3, error=e)
         with pytest.raises(RuntimeError):
             ops.grouped_gemm_wgrad(dy, x, off, 3, error=e)
+
+
+def test_error_words_name_the_kernel():
+    """The low 24 bits of a word tell where it was set: another place for each kernel."""
+    off = torch.tensor([0, 60, 40], dtype=torch.int32, device="cuda")
+    sites = set()
+    for dt, n in ((torch.bfloat16, 64), (torch.float32, 64), (torch.float32, 128)):   # 16-bit, CUDA cores, planes
+        planes = capi.lib().lmoe_grouped_gemm_grad_workspace_bytes(0, capi.dtype_code(dt), 50, n, 64, 2) > 0
+        assert planes == (n == 128)
+        e = torch.zeros(1, dtype=torch.int32, device="cuda")
+        ops.grouped_gemm_dgrad(torch.ones(50, n, device="cuda", dtype=dt), torch.ones(2, n, 64, device="cuda", dtype=dt),
+                               off, 2, error=e)
+        assert e.item() >> 24 == 2   # an argument outside its range
+        sites.add(e.item() & 0xffffff)
+    assert len(sites) == 3
