@@ -545,3 +545,47 @@ def test_error_words_of_the_product(rows):
         assert (e.item() != 0) == bad and (y != 0).any().item() != bad
     with pytest.raises(RuntimeError):
         ops.fp4_grouped_gemm(*x, *w, off, 3, "mxfp4", error=e.float())
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("limit", [2, 0])
+def test_swiglu_of_many_tiles_a_pair(fmt, limit):
+    """Several tiles on each pair of CTAs, so that accumulators, exchange buffers and scales are handed
+    back and used again: all tiles on one pair, and more than three rounds on all of them."""
+    lib = capi.lib()
+    before = lib.lmoe_get_gemm_sm_limit()
+    try:
+        lib.lmoe_set_gemm_sm_limit(limit)
+        few = [i % 3 for i in range(64)]             # the kernel for few rows; one expert with two tiles of rows
+        few[5], few[40] = 70, 0
+        _check_product(few, 200 if limit else 1000, 160, fmt, swiglu=True, head=3, tail=5)
+        _check_product(few, 200 if limit else 1000, 1056, fmt, swiglu=True, odt=torch.float32)
+        many = [700, 0, 300, 129]
+        _check_product(many, 1000 if limit else 4096, 96, fmt, swiglu=True, head=300, tail=40)
+        _check_product(many, 1000 if limit else 4096, 608, fmt, swiglu=True, odt=torch.float32)
+    finally:
+        lib.lmoe_set_gemm_sm_limit(before)
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("odt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("swiglu", [False, True])
+@pytest.mark.parametrize("N,K", [(200, 32), (7, 96), (384, 1408), (264, 14336)])
+def test_both_kernels_give_the_same_bits(fmt, odt, swiglu, N, K):
+    """The rule chooses by all rows, so rows outside the experts move a call to the other kernel: what a
+    row gives does not depend on how many come with it."""
+    gen = torch.Generator(device="cuda").manual_seed(N + K)
+    counts = [1, 0, 70, 3, 33]
+    E, R = len(counts), sum(counts)
+    few = E * (32 if swiglu else 64)
+    off = torch.tensor(np.cumsum([0] + counts), dtype=torch.int32, device="cuda")
+    xq, xs = _operand((few + 64, K), fmt, gen)
+    wq, ws = _operand((E, N, K), fmt, gen, 0.1)
+    al = torch.rand(E, generator=gen, device="cuda") + 0.5
+    kw = dict(alpha=al, out_dtype=odt)
+    if swiglu:
+        uq, us = _operand((E, N, K), fmt, gen, 0.1)
+        kw.update(weights_up=uq, weight_scales_up=us, alpha_up=al * 0.7)
+    a = ops.fp4_grouped_gemm(xq[:R], xs[:R], wq, ws, off, E, fmt, **kw)
+    b = ops.fp4_grouped_gemm(xq, xs, wq, ws, off, E, fmt, **kw)
+    assert torch.equal(a, b[:R]) and (b[R:] == 0).all()
