@@ -296,3 +296,163 @@ def test_error_words_name_the_kernel():
         assert e.item() >> 24 == 2   # an argument outside its range
         sites.add(e.item() & 0xffffff)
     assert len(sites) == 3
+
+
+# ------------------------------------------------------------------- fp32 as three bf16 planes
+def _on_planes(form, R, N, K, E):
+    """Whether a call of fp32 operands takes the kernel that splits them into planes."""
+    return capi.lib().lmoe_grouped_gemm_grad_workspace_bytes(form, capi.LMOE_DTYPE_F32, R, N, K, E) > 0
+
+
+def _one_per_column(shape, place, gen):
+    """Random values at [.., place[c], c] and zeros elsewhere."""
+    w = torch.zeros(shape, device="cuda")
+    c = torch.arange(shape[-1], device="cuda")
+    w[..., place, c] = torch.randn(*shape[:-2], shape[-1], generator=gen, device="cuda")
+    return w
+
+
+def test_planes_hold_every_bit():
+    """One product x * y in each output: its error is that of the planes alone.  x = h + m + l exactly
+    (8 bits each), |m| <= 2^-8 |x| and |l| <= 2^-16 |x|; the products (m, l), (l, m) and (l, l) are left
+    out, 2^-23 |x y|; five additions of the other six are off by a unit in the last place, 2^-23 of at
+    most (1 + 2^-7) |x y| each.  Together below 7 * 2^-23; without a plane it would be 2^-17 or more."""
+    gen = torch.Generator(device="cuda").manual_seed(11)
+    near = lambda got, want: ((got.double() - want).abs() <= 7 * 2.0 ** -23 * want.abs()).all()
+    counts = [1, 70, 0, 33]
+    b = _bounds(counts)
+    off = torch.tensor(b, dtype=torch.int32, device="cuda")
+    R, N, K = b[-1], 161, 200
+    dy = torch.randn(R, N, generator=gen, device="cuda")
+    assert _on_planes(0, R, N, K, 4)
+    place = torch.arange(K, device="cuda") * 7 % N
+    w = _one_per_column((4, N, K), place, gen)
+    dx = ops.grouped_gemm_dgrad(dy, w, off, 4)
+    assert _on_planes(2, R, K, N, 4)
+    y = ops.grouped_gemm(dy, w.transpose(1, 2).contiguous(), off, 4)   # the same sums as a product of 161 values
+    for e in range(4):
+        r = slice(b[e], b[e + 1])
+        want = dy[r][:, place].double() * w[e].sum(0).double()
+        assert near(dx[r], want) and near(y[r], want)
+    counts = [1, 70, 3, 130]
+    b = _bounds(counts)
+    off = torch.tensor(b, dtype=torch.int32, device="cuda")
+    R, N, K = b[-1], 2048, 2056
+    assert _on_planes(1, R, N, K, 4)
+    dy, x = torch.randn(R, N, generator=gen, device="cuda"), torch.zeros(R, K, device="cuda")
+    for e in range(4):
+        x[b[e]:b[e + 1]] = _one_per_column((counts[e], K), torch.arange(K, device="cuda") * 3 % counts[e], gen)
+    dw = ops.grouped_gemm_wgrad(dy, x, off, 4)
+    for e in range(4):
+        r = slice(b[e], b[e + 1])
+        assert near(dw[e], dy[r][torch.arange(K, device="cuda") * 3 % counts[e]].T.double() * x[r].sum(0).double())
+
+
+@pytest.mark.parametrize("positive", [False, True])
+def test_long_sums_of_planes(positive):
+    """Sums of D products: 64 of them in an accumulator that truncates (64 additions of the largest
+    products and 320 of products below 2^-7 of those, a unit in the last place each), D / 64 such sums
+    rounded to nearest (half a unit each), and 2^-23 for the products left out: below (68 + D / 128) *
+    2^-23 of the sum of absolute products, where one accumulator would be off by up to D * 2^-23."""
+    gen = torch.Generator(device="cuda").manual_seed(12)
+    R, N, K = 8192, 160, 328
+    off = torch.tensor([0, R], dtype=torch.int32, device="cuda")
+    make = lambda *s: (lambda t: t.abs() + 0.5 if positive else t)(torch.randn(*s, generator=gen, device="cuda"))
+
+    def check(got, a, c, depth):
+        a, c = a.double(), c.double()
+        assert ((got.double() - a @ c).abs() <= (68 + depth / 128) * 2.0 ** -23 * (a.abs() @ c.abs())).all()
+
+    dy, x = make(R, N), make(R, K)
+    assert _on_planes(1, R, N, K, 1)
+    check(ops.grouped_gemm_wgrad(dy, x, off, 1)[0], dy.T, x, R)
+    off[1] = 100
+    dy, w = make(100, R), make(1, R, K)
+    assert _on_planes(0, 100, R, K, 1)
+    check(ops.grouped_gemm_dgrad(dy, w, off, 1), dy, w[0], R)
+    dy, w = dy[:, 1:].contiguous(), w[:, 1:].transpose(1, 2).contiguous()
+    assert _on_planes(2, 100, K, R - 1, 1)
+    check(ops.grouped_gemm(dy, w, off, 1), dy, w[0].T, R - 1)
+
+
+@pytest.mark.parametrize("K", [1032, 1027, 1536])   # rows stored whole, by words, and from 256-column tiles
+def test_weight_gradient_of_planes_with_tails_beside_what_is_not_finite(K):
+    """Segments of every length mod 16, whose last stage's box holds rows of the next expert, of no expert
+    and of the next plane: NaN and infinities there reach the experts that hold them only."""
+    counts = [i + 64 * (i % 3) for i in range(17)]
+    N, head, tail = 1024, 5, 7
+    dy, x, w, b, off = _inputs(counts, N, K, torch.float32, head, tail, seed=K)
+    E, R = len(counts), dy.shape[0]
+    assert _on_planes(1, R, N, K, E)
+    want = ops.grouped_gemm_wgrad(dy, x, off, E)
+    for e in range(E):
+        r = slice(b[e], b[e + 1])
+        _close(want[e], dy[r].double().T @ x[r].double(), dy[r].double().abs().T @ x[r].double().abs(), counts[e] + 1, e)
+    dy[:head], x[:head] = float("nan"), float("inf")
+    dy[b[-1]:], x[b[-1]:] = float("inf"), float("nan")
+    hit = [e for e in range(E) if e % 2 == 1]
+    for e in hit:
+        dy[b[e]], x[b[e + 1] - 1] = float("nan"), float("-inf")   # rows at both ends of the segment
+    dw = ops.grouped_gemm_wgrad(dy, x, off, E)
+    for e in range(E):
+        if e in hit:
+            assert torch.isnan(dw[e]).all()
+        else:
+            assert torch.equal(dw[e], want[e])
+
+
+def test_weight_gradient_of_planes_of_every_magnitude():
+    """Near the largest value and tiny ones, as in test_fp32_of_every_magnitude, where the weight
+    gradient runs on planes."""
+    counts, N, K = [70, 33], 2048, 4104
+    dy, x, w, b, off = _inputs(counts, N, K, torch.float32, seed=6)
+    assert _on_planes(1, dy.shape[0], N, K, 2)
+    for scale, other in ((2.0 ** 126, 2.0 ** -60), (2.0 ** -115, 2.0 ** 40), (2.0 ** -124, 2.0 ** 30), (2.0 ** 60, 2.0 ** -100)):
+        d, u = dy.clamp(-3.9, 3.9) * scale, x * other
+        dw = ops.grouped_gemm_wgrad(d, u, off, 2)
+        for e in range(2):
+            p, q = d[b[e]:b[e + 1]].double().T, u[b[e]:b[e + 1]].double()
+            tol = (counts[e] + 1) * 2.0 ** -23 * (p.abs() @ q.abs()) + 2.0 ** -148
+            tol = tol + 2.0 ** -134 * (q.abs().sum(0)[None] + p.abs().sum(1)[:, None])
+            assert torch.isfinite(dw[e]).all() and ((dw[e].double() - p @ q).abs() <= tol).all(), (scale, other, e)
+
+
+def test_weight_gradient_of_planes_at_once_replayed_and_under_a_limit():
+    counts, N, K = [140, 0, 161, 5], 2048, 2056
+    dy, x, w, b, off = _inputs(counts, N, K, torch.float32)
+    assert _on_planes(1, dy.shape[0], N, K, 4)
+    other = dy.flip(0).contiguous()
+    want = [ops.grouped_gemm_wgrad(g, x, off, 4) for g in (dy, other)]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for _ in range(4):
+        for i, g in enumerate((dy, other)):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(ops.grouped_gemm_wgrad(g, x, off, 4))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, want[i]) for i in range(2) for a in got[i])
+    lib = capi.lib()
+    before = lib.lmoe_get_gemm_sm_limit()
+    try:
+        lib.lmoe_set_gemm_sm_limit(6)                # many tiles a pair
+        assert torch.equal(ops.grouped_gemm_wgrad(dy, x, off, 4), want[0])
+    finally:
+        lib.lmoe_set_gemm_sm_limit(before)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        gw = ops.grouped_gemm_wgrad(dy, x, off, 4)
+    dy.copy_(other)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(gw, want[1])
+
+
+@pytest.mark.parametrize("offsets", [[0, 50, 40, 100, 100], [0, 20, 40, 90, 101]])
+def test_planes_and_bad_offsets(offsets):
+    N, K = 2048, 2056
+    dy, x, w = torch.ones(100, N, device="cuda"), torch.ones(100, K, device="cuda"), torch.ones(4, N, K, device="cuda")
+    off = torch.tensor(offsets, dtype=torch.int32, device="cuda")
+    assert _on_planes(0, 100, N, K, 4) and _on_planes(1, 100, N, K, 4)
+    for call in (lambda e: ops.grouped_gemm_dgrad(dy, w, off, 4, error=e), lambda e: ops.grouped_gemm_wgrad(dy, x, off, 4, error=e)):
+        e = torch.zeros(1, dtype=torch.int32, device="cuda")
+        assert (call(e) == 0).all() and e.item() != 0
