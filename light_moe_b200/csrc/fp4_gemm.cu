@@ -481,7 +481,11 @@ extern "C" int lmoe_fp4_grouped_gemm(const uint8_t* xq, const uint8_t* xs, int64
   // 4096 x 14336, us by rows per expert: 1 50 against 68, 64 63 against 72, 96 76 against 73; 64 of
   // 2048 x 1408: 25 against 34, 39 against 37, 54 against 39).  The SwiGLU's exchange between lanes
   // makes up less (8 of 2 x 14336 x 4096: 1 80 against 102, 32 87 against 107, 64 124 against 110; 64
-  // of 2 x 1408 x 2048: 38 against 50, 16 45 against 52, 32 55 against 52).
+  // of 2 x 1408 x 2048: 38 against 50, 16 45 against 52, 32 55 against 52).  The counts are on the
+  // device, so the rule takes all rows; it holds for uneven loads (mx, with half of the rows on one expert of
+  // 64 of 2048 x 1408, 4096 rows 40 against 43; 64 of 2 x 1408 x 2048, 2048 rows 55 against 61; 8 of
+  // 2 x 14336 x 4096, 256 rows 103 against 122) up to nearly all rows on one (all: 31 against 23, 39
+  // against 21, 53 against 35).
   const int64_t few = (int64_t)num_experts * (wq_up ? kFp4DecodeRows / 2 : kFp4DecodeRows);
   return total_rows <= few ? run_fp4_decode(p, stream) : run_fp4_gemm(p, stream);
 }

@@ -5,7 +5,7 @@
 //   weight gradient  dw[e, n, k] = sum_{r in e} dy[r, n] * x[r, k]
 //   product          y[r, n]     = sum_k x[r, k] * w[e(r), n, k]
 //
-// With few rows, writing the operands as bf16 planes for the tensor cores (grad_gemm.cu) costs
+// With few rows, writing the operands as bf16 planes for the tensor cores (grad_split.cu) costs
 // more than the products.  As in simt_gemm.cu, fp32 operands are multiplied and summed with fp32
 // FFMA in contraction order.  Bound by the FFMA
 // rate.  Tiles of 128 x 128 outputs, 16 contraction values per step in shared memory (the next

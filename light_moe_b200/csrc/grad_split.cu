@@ -15,7 +15,7 @@
 // 120 us.)
 //
 // Activations (dy, x) are written as planes by a pass of their own: a row is read by every column
-// tile.  Weights are not: in the input gradient and the product four warps read a tile's fp32
+// tile.  Weights are not: in the input gradient and the product eight warps read a tile's fp32
 // values two stages ahead into registers and write their planes into shared memory, which saves
 // writing and reading 12 bytes a weight.  Their tiles are 256 x 128, so that planes and registers
 // fit; the weight gradient's are 256 x 256 or, where the last round would leave pairs idle, 256 x

@@ -65,7 +65,7 @@ int encode_tmap_kblocks(CUtensorMap* map, const void* base, CUtensorMapDataType 
                         uint32_t box_blocks);
 
 // Encode a row-major 3-D tensor (dims and box from the innermost; strides in bytes of the two
-// outer dimensions), 128- or 64-byte swizzle as box[0] elements are 128 or 64 bytes.
+// outer dimensions), 128-, 64- or 32-byte swizzle as box[0] elements are 128, 64 or 32 bytes.
 int encode_tmap_3d(CUtensorMap* map, const void* base, CUtensorMapDataType dtype, uint32_t elem_bytes,
                    const uint64_t (&dims)[3], const uint64_t (&strides)[2], const uint32_t (&box)[3]);
 

@@ -2,9 +2,11 @@
 // grouped_gemm op.
 //
 // The reference multiplies each expert's rows in the input dtype with cuBLAS
-// (csrc/grouped_gemm.cu:30-40, torch::mm_out); for fp32 inputs that is an fp32 GEMM, which the
-// tcgen05 tensor cores (16-bit, 8-bit and tf32 operands) cannot reproduce.  This kernel keeps
-// fp32 operands and accumulates each output with fp32 FFMA in K order.
+// (csrc/grouped_gemm.cu:30-40, torch::mm_out); for fp32 inputs that is an fp32 GEMM.  This kernel
+// keeps fp32 operands and accumulates each output with fp32 FFMA in K order.  It takes rows that are
+// multiples of 16 bytes.  Rows of other lengths go to grad_split.cu and grad_f32.cu, the first on tensor
+// cores as sums of products of bf16 planes: faster (1021 rows, 8 experts of 1024 x 2816 here 322 us,
+// of 1024 x 2815 there 84), but NaN where this one may give an infinity.
 //
 // Tiles of 64 rows (of one segment) x 64 output columns, 16 K values per step staged in
 // shared memory, each of the 256 threads owning 4 x 4 outputs.  The offsets are read on the
