@@ -571,6 +571,7 @@ int grad_entry(GradProblem& p, const void* offsets, void* out, void* workspace, 
 extern "C" size_t lmoe_grouped_gemm_grad_workspace_bytes(int form, int dtype, int64_t total_rows, int N, int K,
                                                          int num_experts) {
   if (form < 0 || form > 2 || total_rows < 0 || N <= 0 || K <= 0 || num_experts <= 0) return 0;
+  if (total_rows > kMaxGemmSize || N > kMaxGemmSize || K > kMaxGemmSize) return 0;   // refused
   GradProblem p;
   p.form = form;
   p.dtype = dtype;

@@ -157,3 +157,12 @@ def test_sizes_whose_tiles_pass_32_bits_are_refused():
         assert _wgrad(N=n, ws=P, wb=2 ** 62) == INVALID and _wgrad(K=n, ws=P, wb=2 ** 62) == INVALID
         for nk in ((n, 8), (8, n)):
             assert capi.lib().lmoe_grouped_gemm_any(P, 2, 4, nk[1], P, nk[0], P, 0, 2, P, None, 0, None, None) == INVALID
+
+
+def test_no_workspace_for_sizes_that_are_refused():
+    size = capi.lib().lmoe_grouped_gemm_grad_workspace_bytes
+    for form in range(3):
+        for dt in range(3):
+            assert size(form, dt, 10, TOP, 33, 2) == 0 and size(form, dt, 10, 33, TOP, 2) == 0
+            assert size(form, dt, TOP, 33, 33, 2) == 0
+            assert size(form, dt, 10, TOP - 1, 33, 2) > 0
