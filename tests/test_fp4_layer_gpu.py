@@ -155,3 +155,15 @@ def test_casts_leave_the_scales_in_fp32(dt):
     mod.cpu()
     assert all(b.device.type == "cpu" for b in mod.buffers())
     assert mod.cuda().input_scale.device == x.device
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+def test_ranges_of_a_host_batch_on_the_other_kernel(fmt):
+    """1400 tokens are more rows than the products' rule gives to the kernel for few, a third of them
+    are not: the ranges' results are the whole batch's, bit by bit."""
+    x, mod, _ = _make(1400, 256, 96, 64, 2, fmt, S=1)
+    xh = x.cpu().pin_memory()
+    for chunks in (1, 2, 3):
+        yh = mod.forward_host(xh, chunks=chunks)
+        torch.cuda.synchronize()
+        assert torch.equal(yh, mod(x).cpu())
