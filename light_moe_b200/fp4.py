@@ -20,6 +20,7 @@ from .layer import HostBufferCalls
 NVFP4_RANGE = 448.0 * 6.0
 
 
+@torch.no_grad()
 def nvfp4_global_scale(x: torch.Tensor) -> torch.Tensor:
     """The tensor scale that maps the largest magnitude of ``x`` (of each x[i] of a 3-D tensor) to
     the end of nvfp4's range: fp32 [1] or [x.shape[0]]; 1 where everything is zero."""
@@ -47,6 +48,7 @@ class FP4Experts:
     ffn_size: int
 
     @classmethod
+    @torch.no_grad()
     def from_dense(cls, w1: torch.Tensor, w3: torch.Tensor, w2: torch.Tensor, format: str = "nvfp4",
                    shared: Optional[Sequence[Tuple[torch.Tensor, torch.Tensor, torch.Tensor]]] = None) -> "FP4Experts":
         """Quantise dense expert weights on the GPU: w1, w3 [E, ffn, d] (gate, up), w2 [E, d, ffn];
@@ -82,8 +84,8 @@ class FP4MoELayer(HostBufferCalls, torch.nn.Module):
             raise ValueError("gate_weight must be [num_experts, hidden_size]")
         if e.format != "nvfp4" and (input_scale is not None or hidden_scale is not None):
             raise ValueError("input_scale and hidden_scale belong to nvfp4")
-        self.register_buffer("gate_weight", gate_weight.to(torch.bfloat16).contiguous())
-        self.register_buffer("gate_bias", None if gate_bias is None else gate_bias.float().contiguous())
+        self.register_buffer("gate_weight", gate_weight.detach().to(torch.bfloat16).contiguous())
+        self.register_buffer("gate_bias", None if gate_bias is None else gate_bias.detach().float().contiguous())
         one = lambda s: None if s is None else s.detach().to(gate_weight.device, torch.float32).reshape(1).contiguous()
         self.register_buffer("input_scale", one(input_scale))
         self.register_buffer("hidden_scale", one(hidden_scale))

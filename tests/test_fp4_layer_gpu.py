@@ -167,3 +167,16 @@ def test_ranges_of_a_host_batch_on_the_other_kernel(fmt):
         yh = mod.forward_host(xh, chunks=chunks)
         torch.cuda.synchronize()
         assert torch.equal(yh, mod(x).cpu())
+
+
+def test_experts_of_parameters_keep_no_graph():
+    """Quantised from trainable weights: scales without a history, which would hold the dense weights."""
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    r = lambda *s: torch.nn.Parameter(torch.randn(*s, generator=gen, device="cuda"))
+    w1, w3, w2, gate, scale = r(4, 96, 64), r(4, 96, 64), r(4, 64, 96), r(4, 64), r(1)
+    ex = FP4Experts.from_dense(w1, w3, w2, "nvfp4", shared=[(r(96, 64), r(96, 64), r(64, 96))])
+    assert not nvfp4_global_scale(w1).requires_grad
+    assert not any(t.requires_grad for t in (ex.g1, ex.g3, ex.g2, *ex.w1, *ex.w3, *ex.w2))
+    mod = FP4MoELayer(gate, ex, 2, gate_bias=r(4), input_scale=scale.abs(), hidden_scale=scale.abs())
+    assert not any(b.requires_grad for b in mod.buffers())
+    assert not mod(torch.randn(5, 64, device="cuda")).requires_grad
