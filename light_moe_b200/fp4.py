@@ -82,6 +82,8 @@ class FP4MoELayer(HostBufferCalls, torch.nn.Module):
         e = experts
         if gate_weight.shape != (e.num_experts, e.hidden_size):
             raise ValueError("gate_weight must be [num_experts, hidden_size]")
+        if e.hidden_size % 64:
+            raise ValueError("the router takes hidden sizes that are multiples of 64")
         if e.format != "nvfp4" and (input_scale is not None or hidden_scale is not None):
             raise ValueError("input_scale and hidden_scale belong to nvfp4")
         self.register_buffer("gate_weight", gate_weight.detach().to(torch.bfloat16).contiguous())

@@ -40,3 +40,13 @@ def test_fp4_layer_refusals():
         FP4MoELayer(z(3, 32), ex, 1)
     with pytest.raises(ValueError):
         FP4MoELayer(z(2, 32), ex, 1, input_scale=torch.ones(1))
+
+
+def test_fp4_layer_refuses_hidden_sizes_that_its_router_does_not_take():
+    z = torch.zeros
+    for d in (32, 96):
+        ex = FP4Experts("mxfp4", (None, None), (None, None), (None, None), None, None, None, 2, 0, d, 64)
+        with pytest.raises(ValueError, match="64"):
+            FP4MoELayer(z(2, d), ex, 1)
+    ex = FP4Experts("mxfp4", (None, None), (None, None), (None, None), None, None, None, 2, 0, 192, 32)
+    FP4MoELayer(z(2, 192), ex, 1)
