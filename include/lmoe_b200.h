@@ -313,6 +313,47 @@ int lmoe_fp4_grouped_gemm(const uint8_t* xq, const uint8_t* xs, int64_t xs_pitch
                           int num_experts, const float* alpha, const float* alpha_up, int out_dtype, void* output,
                           uint32_t* error, lmoe_stream_t stream);
 
+/* ------------------------------------------------------------------------------------ */
+/* 8-bit floating point (E4M3) with one fp32 scale per block of 128 columns: of one row        */
+/* (activations) or of 128 rows (weights).  The last blocks may be partial; K % 16 == 0.       */
+/*   s = max(max|x| / 448, 2^-126), or with power_of_two the next power of two; code = x / s to */
+/*   the nearest E4M3 value, ties to even; a block with an infinity or a NaN gets the scale NaN  */
+/*   and zero codes, so it reads as NaN.                                                        */
+/* The reference has no 8-bit floating point.                                                  */
+/* ------------------------------------------------------------------------------------ */
+
+/* Blocks of one row.  x: [rows, K] of LMOE_DTYPE_*, rows ldx elements apart.  positions (optional): int32
+ * [rows, copies], the output rows that row r is written to (entries outside [0, out_rows) are skipped);
+ * without it copies = 1 and out_rows = rows.  q [out_rows, K] 16-byte aligned; the scale of row r and
+ * block b at scales[b * scale_pitch + r], scale_pitch >= out_rows. */
+int lmoe_quantize_fp8(const void* x, int dtype, int64_t rows, int K, int64_t ldx, int power_of_two,
+                      const int32_t* positions, int copies, int64_t out_rows, uint8_t* q, float* scales,
+                      int64_t scale_pitch, lmoe_stream_t stream);
+
+/* Blocks of 128 x 128 of `count` matrices [rows, K]: q [count, rows, K] 16-byte aligned, scales [count,
+ * ceil(rows / 128), ceil(K / 128)]. */
+int lmoe_quantize_fp8_blocks(const void* x, int dtype, int64_t count, int64_t rows, int K, int power_of_two,
+                             uint8_t* q, float* scales, lmoe_stream_t stream);
+
+/* q and out ([count, rows, K] of out_dtype) 16-byte aligned; block_rows 1 or 128; strides of the scales in
+ * elements between matrices, row blocks and column blocks. */
+int lmoe_dequantize_fp8(const uint8_t* q, const float* scales, int64_t scale_mat_stride, int64_t scale_row_stride,
+                        int64_t scale_block_stride, int64_t count, int64_t rows, int K, int block_rows, int out_dtype,
+                        void* out, lmoe_stream_t stream);
+
+/* Grouped product of such operands: for the rows r of expert e
+ *   output[r, n] = sum_b xs[b, r] * ws[e, n / 128, b] * (x . w[e, n] over block b)   (wq_up == NULL)
+ *   output[r, n] = silu(x . w[e, n]) * (x . up[e, n])                                  otherwise
+ * exact products, fp32 sums of a block on the tensor cores, fp32 sums over the blocks rounded to nearest.
+ * x: codes xq [total_rows, K], scales xs [K blocks][xs_pitch]; w (and up): codes [E, N, K], scales
+ * [E, ceil(N / 128), ceil(K / 128)]; codes 16-byte aligned.  The product of the two scales of a block has to
+ * be an fp32 number too (a factor that overflows makes NaN of sums that are zero).  output [total_rows, N] of out_dtype; rows
+ * outside every expert are zero.  total_rows and K up to 2^31 - 1025, N up to 2^30 - 513.  error: as above. */
+int lmoe_fp8_grouped_gemm(const uint8_t* xq, const float* xs, int64_t xs_pitch, int64_t total_rows, int K,
+                          const uint8_t* wq, const float* ws, const uint8_t* wq_up, const float* ws_up, int N,
+                          const void* expert_offsets, int offsets_are_int64, int num_experts, int out_dtype,
+                          void* output, uint32_t* error, lmoe_stream_t stream);
+
 /* Weighted combine of per-slot expert rows back to tokens:
  *   y[t, :] = sum_j weights[t*top_k+j] * rows[positions[t*top_k+j], :]
  *             + sum_s extra_rows[s*num_tokens + t, :]

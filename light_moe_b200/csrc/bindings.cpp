@@ -643,6 +643,173 @@ torch::Tensor fp4_grouped_gemm(torch::Tensor input, torch::Tensor input_scales, 
   return out;
 }
 
+// ---------------------------------------------------------------- 8-bit operands with block scales
+
+constexpr int64_t kFp8Block = 128;
+int64_t fp8_blocks(int64_t n) { return (n + kFp8Block - 1) / kFp8Block; }
+
+void check_block_rows(int64_t block_rows) {
+  TORCH_CHECK(block_rows == 1 || block_rows == kFp8Block, "block_rows must be 1 or 128, is ", block_rows);
+}
+int64_t check_fp8_columns(int64_t K, const char* name) {
+  TORCH_CHECK(K > 0 && K % 16 == 0 && K <= INT32_MAX - 1024, name, ": K must be a positive multiple of 16");
+  return K;
+}
+
+std::tuple<torch::Tensor, torch::Tensor> quantize_fp8(torch::Tensor x, int64_t block_rows, bool power_of_two,
+                                                      std::optional<torch::Tensor> positions) {
+  check_cuda(x, "x");
+  check_float(x, "x");
+  check_block_rows(block_rows);
+  TORCH_CHECK(x.dim() >= 2, "x must be [..., rows, K]");
+  const int64_t K = check_fp8_columns(x.size(-1), "x"), KB = fp8_blocks(K);
+  const at::AutoDispatchBelowADInplaceOrView below_autograd;   // no graph is recorded
+  const c10::cuda::OptionalCUDAGuard guard(x.device());
+  auto shape = x.sizes().vec();
+  const bool have_positions = positions.has_value() && positions->defined();
+  if (block_rows != 1) {
+    TORCH_CHECK(!have_positions, "positions needs block_rows=1");
+    auto xc = x.contiguous();
+    const int64_t rows = x.size(-2), count = rows ? xc.numel() / K / rows : 0;
+    TORCH_CHECK(rows <= INT32_MAX - 1024, "too many rows");
+    auto q = empty_like_device(shape, torch::kFloat8_e4m3fn, x);
+    shape[shape.size() - 2] = fp8_blocks(rows);
+    shape.back() = KB;
+    auto s = empty_like_device(shape, torch::kFloat32, x);
+    if (count > 0)
+      check_status(lmoe_quantize_fp8_blocks(xc.data_ptr(), dtype_code(xc), count, rows, (int)K, power_of_two,
+                                            static_cast<uint8_t*>(q.data_ptr()), s.data_ptr<float>(), cur_stream()),
+                   "quantize_fp8");
+    return {q, s};
+  }
+  const bool strided = x.dim() == 2 && x.stride(1) == 1 && (x.size(0) <= 1 || x.stride(0) >= K);
+  auto xc = strided ? x : x.contiguous();
+  const int64_t rows = xc.numel() / K;
+  const int64_t ldx = strided && x.size(0) > 1 ? x.stride(0) : K;
+  torch::Tensor pos;
+  int64_t copies = 1, out_rows = rows;
+  if (have_positions) {
+    TORCH_CHECK(x.dim() == 2, "positions needs x [rows, K]");
+    check_same_device(*positions, x, "positions");
+    TORCH_CHECK(positions->scalar_type() == torch::kInt32, "positions must be int32");
+    TORCH_CHECK(rows == 0 ? positions->numel() == 0 : (positions->numel() % rows == 0 && positions->numel() > 0),
+                "positions must hold the same number of entries for each row");
+    pos = positions->contiguous();
+    copies = rows ? pos.numel() / rows : 1;
+    out_rows = pos.numel();
+    shape[0] = out_rows;
+  }
+  auto q = empty_like_device(shape, torch::kFloat8_e4m3fn, x);
+  // block after block, the rows of a block padded to 16 bytes; the tensor shows them as [..., rows, KB]
+  const int64_t pitch = (out_rows + 3) / 4 * 4;
+  auto s = empty_like_device({KB, pitch}, torch::kFloat32, x);
+  if (rows > 0)
+    check_status(lmoe_quantize_fp8(xc.data_ptr(), dtype_code(xc), rows, (int)K, ldx, power_of_two,
+                                   pos.defined() ? pos.data_ptr<int32_t>() : nullptr, (int)copies, out_rows,
+                                   static_cast<uint8_t*>(q.data_ptr()), s.data_ptr<float>(), pitch, cur_stream()),
+                 "quantize_fp8");
+  std::vector<int64_t> strides(shape.size());
+  int64_t step = 1;
+  for (int64_t i = (int64_t)shape.size() - 2; i >= 0; --i) {
+    strides[i] = step;
+    step *= shape[i];
+  }
+  shape.back() = KB;
+  strides.back() = pitch;
+  s.unsafeGetTensorImpl()->set_sizes_and_strides(shape, strides);
+  return {q, s};
+}
+
+void check_fp8(const torch::Tensor& q, const torch::Tensor& s, const torch::Tensor& like, const char* name) {
+  check_same_device(q, like, name);
+  check_same_device(s, like, name);
+  TORCH_CHECK(q.scalar_type() == torch::kFloat8_e4m3fn, name, ": codes must be float8_e4m3fn");
+  TORCH_CHECK(s.scalar_type() == torch::kFloat32, name, ": scales must be fp32");
+  check_fp8_columns(q.size(-1), name);
+}
+
+torch::Tensor dequantize_fp8(torch::Tensor q, torch::Tensor scales, int64_t block_rows,
+                             std::optional<torch::ScalarType> out_dtype) {
+  check_cuda(q, "q");
+  check_block_rows(block_rows);
+  TORCH_CHECK(q.dim() >= 2 && scales.dim() == q.dim(), "q [..., rows, K], scales [..., row blocks, K / 128]");
+  check_fp8(q, scales, q, "q");
+  const int64_t K = q.size(-1), rows = q.size(-2), RB = block_rows == 1 ? rows : fp8_blocks(rows);
+  for (int64_t i = 0; i + 2 < q.dim(); ++i) TORCH_CHECK(q.size(i) == scales.size(i), "scales shape mismatch");
+  TORCH_CHECK(scales.size(-2) == RB && scales.size(-1) == fp8_blocks(K), "scales shape mismatch");
+  const auto ot = out_dtype.value_or(torch::kBFloat16);
+  TORCH_CHECK(ot == torch::kBFloat16 || ot == torch::kFloat16 || ot == torch::kFloat32,
+              "out_dtype must be bf16, fp16 or fp32");
+  const at::AutoDispatchBelowADInplaceOrView below_autograd;   // no graph is recorded
+  const c10::cuda::OptionalCUDAGuard guard(q.device());
+  auto out = empty_like_device(q.sizes(), ot, q);
+  const int64_t count = rows ? q.numel() / K / rows : 0;
+  if (count > 0) {
+    auto c = contig16(q);
+    auto s = q.dim() == 3 ? scales : scales.reshape({count, RB, scales.size(-1)});
+    check_status(lmoe_dequantize_fp8(static_cast<const uint8_t*>(c.data_ptr()), s.data_ptr<float>(), s.stride(0),
+                                     s.stride(1), s.stride(2), count, rows, (int)K, (int)block_rows,
+                                     dtype_code(out), out.data_ptr(), cur_stream()),
+                 "dequantize_fp8");
+  }
+  return out;
+}
+
+// Weight codes [>= matrices, N, K] and scales [.., N / 128, K / 128], contiguous.
+struct Fp8Weights {
+  torch::Tensor q, s;
+};
+Fp8Weights fp8_weights(const torch::Tensor& q, const torch::Tensor& s, const torch::Tensor& like, int64_t matrices,
+                       int64_t N, int64_t K, const char* name) {
+  check_fp8(q, s, like, name);
+  TORCH_CHECK(q.dim() == 3 && s.dim() == 3, name, ": codes [E, N, K], scales [E, N / 128, K / 128]");
+  TORCH_CHECK(q.size(0) >= matrices && q.size(1) == N && q.size(2) == K, name, ": shape mismatch");
+  TORCH_CHECK(s.size(0) == q.size(0) && s.size(1) == fp8_blocks(N) && s.size(2) == fp8_blocks(K), name,
+              ": scales shape mismatch");
+  return {contig16(q), s.contiguous()};
+}
+
+torch::Tensor fp8_grouped_gemm(torch::Tensor input, torch::Tensor input_scales, torch::Tensor weights,
+                               torch::Tensor weight_scales, torch::Tensor expert_offsets, int64_t num_experts,
+                               std::optional<torch::Tensor> weights_up, std::optional<torch::Tensor> weight_scales_up,
+                               std::optional<torch::ScalarType> out_dtype, std::optional<torch::Tensor> error) {
+  check_cuda(input, "input");
+  TORCH_CHECK(input.dim() == 2 && input_scales.dim() == 2 && weights.dim() == 3,
+              "input [T,K], input_scales [T,K/128], weights [E,N,K]");
+  check_fp8(input, input_scales, input, "input");
+  const int64_t T = input.size(0), K = input.size(1), N = weights.size(1), KB = fp8_blocks(K);
+  TORCH_CHECK(input_scales.size(0) == T && input_scales.size(1) == KB, "input: scales shape mismatch");
+  const bool swiglu = weights_up.has_value() && weights_up->defined();
+  TORCH_CHECK(swiglu == (weight_scales_up.has_value() && weight_scales_up->defined()),
+              "weights_up and weight_scales_up belong together");
+  const at::AutoDispatchBelowADInplaceOrView below_autograd;   // no graph is recorded
+  const c10::cuda::OptionalCUDAGuard guard(input.device());
+  auto off = check_offsets(expert_offsets, input, num_experts);
+  const auto w = fp8_weights(weights, weight_scales, input, num_experts, N, K, "weights");
+  Fp8Weights u;
+  if (swiglu) u = fp8_weights(*weights_up, *weight_scales_up, input, num_experts, N, K, "weights_up");
+  check_sizes(T, N, K, num_experts);
+  auto xq = contig16(input);
+  // the rows of a block next to each other
+  torch::Tensor xs = input_scales;
+  if (!((T <= 1 || xs.stride(0) == 1) && (KB <= 1 || xs.stride(1) >= T))) xs = xs.t().contiguous().t();
+  const int64_t pitch = KB <= 1 ? T : xs.stride(1);
+  const auto ot = out_dtype.value_or(torch::kBFloat16);
+  TORCH_CHECK(ot == torch::kBFloat16 || ot == torch::kFloat16 || ot == torch::kFloat32,
+              "out_dtype must be bf16, fp16 or fp32");
+  uint32_t* err = error_word(error, input);
+  auto out = empty_like_device({T, N}, ot, input);
+  if (T > 0 && N > 0)
+    check_status(lmoe_fp8_grouped_gemm(static_cast<const uint8_t*>(xq.data_ptr()), xs.data_ptr<float>(), pitch, T,
+                                       (int)K, static_cast<const uint8_t*>(w.q.data_ptr()), w.s.data_ptr<float>(),
+                                       swiglu ? static_cast<const uint8_t*>(u.q.data_ptr()) : nullptr,
+                                       swiglu ? u.s.data_ptr<float>() : nullptr, (int)N, off.data_ptr(),
+                                       off.scalar_type() == torch::kInt64, (int)num_experts, dtype_code(out),
+                                       out.data_ptr(), err, cur_stream()),
+                 "fp8_grouped_gemm");
+  return out;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -681,6 +848,14 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("input_scales"), py::arg("weights"), py::arg("weight_scales"), py::arg("expert_offsets"),
         py::arg("num_experts"), py::arg("format"), py::arg("alpha") = py::none(), py::arg("weights_up") = py::none(),
         py::arg("weight_scales_up") = py::none(), py::arg("alpha_up") = py::none(),
+        py::arg("out_dtype") = py::none(), py::arg("error") = py::none());
+  m.def("quantize_fp8", &quantize_fp8, "Values -> 8-bit floating point with block scales", py::arg("x"),
+        py::arg("block_rows") = 1, py::arg("power_of_two") = false, py::arg("positions") = py::none());
+  m.def("dequantize_fp8", &dequantize_fp8, "8-bit floating point with block scales -> values", py::arg("q"),
+        py::arg("scales"), py::arg("block_rows") = 1, py::arg("out_dtype") = py::none());
+  m.def("fp8_grouped_gemm", &fp8_grouped_gemm, "Grouped GEMM of block-scaled 8-bit operands", py::arg("input"),
+        py::arg("input_scales"), py::arg("weights"), py::arg("weight_scales"), py::arg("expert_offsets"),
+        py::arg("num_experts"), py::arg("weights_up") = py::none(), py::arg("weight_scales_up") = py::none(),
         py::arg("out_dtype") = py::none(), py::arg("error") = py::none());
   m.def("combine_rows", &combine_rows, "Weighted combine of slot rows back to tokens", py::arg("rows"),
         py::arg("positions"), py::arg("weights"), py::arg("num_tokens"), py::arg("top_k"),

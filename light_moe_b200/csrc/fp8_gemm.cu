@@ -1,0 +1,536 @@
+// fp8_gemm.cu -- grouped product of block-scaled 8-bit operands on CTA pairs (sm_100a).
+//
+//   y[r, n] = sum_b sx[r, b] * sw[e, n / 128, b] * sum_{k in block b} x[r, k] * w[e, n, k]
+//   y[r, f] = silu(gate[r, f]) * up[r, f]                with a gate and an up matrix
+//
+// for the rows r of expert e: E4M3 codes, fp32 scales of 128 columns of a row (x) or of 128 x 128
+// values (w, fp8_format.cuh).  The scales are any fp32 numbers, so the block-scaled MMA kinds (power
+// of two scales) do not apply: the tensor core sums one block of 128 columns at a time in tensor
+// memory (exact products, fp32 sums), and the epilogue's warps add each block's sums times
+// sx * sw to fp32 accumulators in registers.  So no sum of more than 128 products is left to the
+// tensor core, whose additions truncate.
+//
+// Tile: 256 rows (128 per CTA, TMEM lane = row) x 256 or 128 weight rows (half of them per CTA in
+// shared memory).  A block of 128 x 256 x 128 takes the tensor core 512 cycles; reading its sums
+// from tensor memory and adding them, 8 warps of 32 rows x 128 columns, about 260 each, beside the
+// next block's MMAs in the other half of tensor memory.  128 accumulators a thread: the epilogue's
+// two warpgroups take the registers that the other warps give up.
+//
+// The lane being the row, a thread holds a row's gate and up values of the same features, and the
+// SwiGLU needs no exchange: the leader's half of the columns is gate rows and the follower's the
+// same rows of up.
+//
+// Warps: 0 TMA producer, whose copies complete on the leader's stage barrier; 1 MMA issuer (leader
+// CTA); 2 scales (both CTAs), which brings four blocks' scales at a time into a ring in shared
+// memory, coalesced because rows' scales are stored block after block; 4-11 the epilogue.
+#include <cuda_bf16.h>
+
+#include "fp8_format.cuh"
+#include "fp8_gemm.h"
+#include "pair_gemm.cuh"
+
+namespace lmoe {
+namespace {
+
+constexpr int kRowsCta = 128, kTM = 256, kBK = kFp8Block;
+constexpr int kEpiWarps = 8, kEpiWarp0 = 4, kThreads = (kEpiWarp0 + kEpiWarps) * 32;
+constexpr int kTmemCols = 512;
+constexpr int kSlotBlocks = 4, kSlots = 4;   // a slot of the scales' ring holds four blocks
+constexpr uint32_t kSite = 0x700u;
+constexpr uint32_t kStoreBytes = 2048;       // a block on its way out: 32 rows x 64 bytes
+// Registers: 384 threads x 168 at launch = 128 x 56 + 256 x 224.
+constexpr int kRegsLaunch = 168, kRegsOther = 56, kRegsEpi = 224;
+static_assert(128 * kRegsOther + 256 * kRegsEpi <= kThreads * kRegsLaunch, "register split");
+
+template <int TN>
+struct Cfg {
+  static constexpr int kHalf = TN / 2;                  // columns a CTA loads
+  static constexpr int kStages = TN == 256 ? 6 : 8;
+  static constexpr int kAcc = kTmemCols / TN;           // blocks' sums in tensor memory
+  static constexpr int kCols = TN / 2;                  // accumulators of an epilogue thread
+  static constexpr uint32_t kABytes = kRowsCta * kBK, kBBytes = kHalf * kBK, kStageBytes = kABytes + kBBytes;
+};
+
+struct ScaleSlot {
+  float row[kSlotBlocks][kRowsCta];
+  float col[kSlotBlocks][2];   // of the tile's two column blocks, or of gate and up
+};
+
+template <int TN>
+struct __align__(8) Bars {
+  using C = Cfg<TN>;
+  uint64_t full[C::kStages];     // leader: both CTAs' codes landed (one arrival each)
+  uint64_t empty[C::kStages];    // the stage's MMAs finished (both CTAs)
+  uint64_t acc_full[C::kAcc];    // a block's sums are in tensor memory (both CTAs)
+  uint64_t acc_empty[C::kAcc];   // leader: both CTAs' epilogue warps have read them
+  uint64_t sc_full[kSlots];      // this CTA: the slot's scales are written
+  uint64_t sc_empty[kSlots];     // this CTA: its epilogue warps have read them
+  uint64_t mma_done;
+  uint32_t tmem_base;
+  int abort;
+  SegTable seg;
+};
+
+template <int TN>
+constexpr uint32_t smem_bytes() {
+  return 1024 + Cfg<TN>::kStages * Cfg<TN>::kStageBytes + kEpiWarps * kStoreBytes + kSlots * sizeof(ScaleSlot) +
+         sizeof(Bars<TN>);
+}
+static_assert(smem_bytes<256>() <= 232448 && smem_bytes<128>() <= 232448, "shared memory budget");
+static_assert(sizeof(ScaleSlot) % 16 == 0, "alignment of what follows");
+
+struct Fp8Args {
+  const float* xs;
+  int64_t xs_pitch;
+  const float* ws;       // [E, NB, KB]; gate
+  const float* ws_up;
+  const void* offsets;
+  int offsets_i64;
+  int E, N, KB, NB;
+  int64_t R;
+  Raster raster;         // of the column tiles
+  void* out;
+  int out_dtype;
+  int store;             // StoreMode
+  uint32_t* err;
+};
+
+struct Fp8Tile {
+  int e, m, n, row0, row_end;
+  bool zero;   // rows outside every expert
+};
+__device__ __forceinline__ Fp8Tile fp8_tile_at(const SegTable& t, const Fp8Args& a, int tile, int& hint) {
+  int j = hint;
+  while (tile >= t.tile_start[j + 1]) ++j;
+  hint = j;
+  Fp8Tile r;
+  const int rows = t.row[j + 1] - t.row[j];
+  a.raster.at(tile - t.tile_start[j], (rows + kTM - 1) / kTM, r.m, r.n);
+  r.e = j - 1;
+  r.zero = j == 0 || j == a.E + 1;
+  r.row0 = t.row[j] + r.m * kTM;
+  r.row_end = t.row[j + 1];
+  return r;
+}
+
+// Instruction descriptor of kind::f8f6f4: E4M3 operands, K-major, fp32 sums, M = 256, N = n.
+__host__ __device__ constexpr uint32_t idesc_fp8(uint32_t n) {
+  return (1u << 4) | ((n >> 3) << 17) | ((256u >> 4) << 24);
+}
+__device__ __forceinline__ void mma_fp8_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// 32 columns of the thread's lane; the registers hold them after tmem_arrived.
+__device__ __forceinline__ void tmem_ld32_async(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+      "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+// Completes the thread's loads; the operands keep uses of the registers behind it.
+__device__ __forceinline__ void tmem_arrived(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
+                 "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                 "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
+}
+
+// acc[i] += f * r[i] for 32 values, two to an instruction.
+__device__ __forceinline__ void add_scaled(float* acc, const uint32_t (&r)[32], float f) {
+  uint64_t f2;
+  asm("mov.b64 %0, {%1, %1};" : "=l"(f2) : "f"(f));
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    uint64_t p, c;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "r"(r[2 * i]), "r"(r[2 * i + 1]));
+    asm("mov.b64 %0, {%1, %2};" : "=l"(c) : "f"(acc[2 * i]), "f"(acc[2 * i + 1]));
+    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(c) : "l"(p), "l"(f2));
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(acc[2 * i]), "=f"(acc[2 * i + 1]) : "l"(c));
+  }
+}
+
+__device__ __forceinline__ float silu(float g) { return __fdividef(g, 1.0f + __expf(-g)); }
+
+template <int TN, bool SWIGLU>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_x32,
+                    const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_up,
+                    const __grid_constant__ CUtensorMap tm_out, const Fp8Args a) {
+  using C = Cfg<TN>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* store_stage = base + C::kStages * C::kStageBytes;
+  ScaleSlot* slots = reinterpret_cast<ScaleSlot*>(store_stage + kEpiWarps * kStoreBytes);
+  Bars<TN>* bars = reinterpret_cast<Bars<TN>*>(slots + kSlots);
+  volatile int* abort_flag = &bars->abort;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = rank == 0;
+
+  if (tid == 0) {
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(&bars->full[s], 2);
+      mbar_init(&bars->empty[s], 1);
+    }
+    for (int s = 0; s < C::kAcc; ++s) {
+      mbar_init(&bars->acc_full[s], 1);
+      mbar_init(&bars->acc_empty[s], 2 * kEpiWarps);
+    }
+    for (int s = 0; s < kSlots; ++s) {
+      mbar_init(&bars->sc_full[s], 1);
+      mbar_init(&bars->sc_empty[s], kEpiWarps);
+    }
+    mbar_init(&bars->mma_done, 1);
+    bars->abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(&bars->tmem_base, kTmemCols);
+    tmem_relinquish_pair();
+  }
+  load_segments(&bars->seg, a.offsets, a.offsets_i64, a.E, a.R, tid, kThreads);
+  const int segs = a.E + 2;
+  if (warp == 0)
+    scan_tiles(&bars->seg, segs, lane, [&](int j) {
+      return (bars->seg.row[j + 1] - bars->seg.row[j] + kTM - 1) / kTM * a.raster.nb;
+    });
+  if (tid == 0 && bars->seg.bad && blockIdx.x == 0) report_error(a.err, kErrBadArg, kSite + 1);
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem = bars->tmem_base;
+  const SegTable& seg = bars->seg;
+  const int total = seg.tile_start[segs];
+  const int KB = a.KB;
+  const int first = blockIdx.x >> 1, stride = gridDim.x >> 1;
+
+  if (warp < kEpiWarp0) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
+    if (warp == 0) {
+      // ---------------------------------------------------------------- TMA producer
+      const uint32_t full_addr = mapa_u32(&bars->full[0], 0);
+      const CUtensorMap* wmap = SWIGLU && !leader ? &tm_up : &tm_w;
+      Ring<C::kStages> st;
+      int hint = 0;
+      bool ok = true;
+      for (int tile = first; tile < total && ok; tile += stride) {
+        const Fp8Tile t = fp8_tile_at(seg, a, tile, hint);
+        if (t.zero) continue;
+        const int r0 = t.row0 + (int)rank * kRowsCta;
+        int rows = t.row_end - r0;
+        rows = rows < 0 ? 0 : (rows > kRowsCta ? kRowsCta : rows);
+        const int boxes = (rows + 31) >> 5;   // only the boxes that hold this tile's rows
+        const int wrow = SWIGLU ? t.n * C::kHalf : t.n * TN + (int)rank * C::kHalf;
+        for (int kb = 0; kb < KB; ++kb, st.next()) {
+          ok = warp_wait(&bars->empty[st.i], st.phase ^ 1u, a.err, abort_flag, kSite + 2);
+          if (!ok) break;
+          if (elect_one()) {
+            uint8_t* dst = base + st.i * C::kStageBytes;
+            const uint32_t bar = full_addr + st.i * 8;
+            mbar_arrive_expect_tx_cluster(bar, (uint32_t)boxes * 4096u + C::kBBytes);
+            if (boxes == 4) {
+              tma_load_2d_pair(dst, &tm_x, bar, kb * kBK, r0);
+            } else {
+              for (int b = 0; b < boxes; ++b) tma_load_2d_pair(dst + b * 4096, &tm_x32, bar, kb * kBK, r0 + b * 32);
+            }
+            tma_load_3d_pair(dst + C::kABytes, wmap, bar, kb * kBK, wrow, t.e);
+          }
+        }
+      }
+      // the copies of a finished tile have landed (its MMAs read them)
+      if (!ok) let_copies_land();
+    } else if (warp == 1) {
+      // ---------------------------------------------------------------- MMA issuer
+      if (leader) {
+        const uint64_t adesc0 = sdesc_k_sw128(smem_u32(base)), bdesc0 = sdesc_k_sw128(smem_u32(base) + C::kABytes);
+        Ring<C::kStages> st;
+        Ring<C::kAcc> ac;
+        int hint = 0;
+        bool ok = true;
+        for (int tile = first; tile < total && ok; tile += stride) {
+          const Fp8Tile t = fp8_tile_at(seg, a, tile, hint);
+          if (t.zero) continue;
+          for (int kb = 0; kb < KB; ++kb) {
+            // the waits start together; what has not come yet is waited for below
+            const bool w0 = mbar_test(&bars->acc_empty[ac.i], ac.phase ^ 1u);
+            const bool w1 = mbar_test(&bars->full[st.i], st.phase);
+            if (!(w0 && w1)) {
+              ok = mbar_wait(&bars->acc_empty[ac.i], ac.phase ^ 1u, a.err, abort_flag, kSite + 3);
+              if (ok) ok = mbar_wait(&bars->full[st.i], st.phase, a.err, abort_flag, kSite + 4);
+            }
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc_fence_after();
+            if (elect_one()) {
+              const uint64_t ad = adesc0 + st.i * (C::kStageBytes >> 4), bd = bdesc0 + st.i * (C::kStageBytes >> 4);
+              const uint32_t d = tmem + ac.i * TN;
+#pragma unroll
+              for (int m = 0; m < kBK / 32; ++m)   // 32 bytes of the lines: two descriptor units
+                mma_fp8_pair(d, ad + m * 2, bd + m * 2, idesc_fp8(TN), (uint32_t)(m > 0));
+              mma_commit_pair(&bars->acc_full[ac.i]);
+              mma_commit_pair(&bars->empty[st.i]);
+            }
+            __syncwarp();
+            st.next();
+            ac.next();
+          }
+        }
+        if (elect_one()) mma_commit_leader(&bars->mma_done);
+        mbar_wait(&bars->mma_done, 0, a.err, nullptr, kSite + 5);
+      }
+    } else if (warp == 2) {
+      // ---------------------------------------------------------------- scales
+      Ring<kSlots> sl;
+      int hint = 0;
+      bool ok = true;
+      for (int tile = first; tile < total && ok; tile += stride) {
+        const Fp8Tile t = fp8_tile_at(seg, a, tile, hint);
+        if (t.zero) continue;
+        const int r0 = t.row0 + (int)rank * kRowsCta;
+        // lanes 0-3: the four blocks' scales of the first columns (gate), 4-7 of the second (up)
+        const int nb0 = SWIGLU ? t.n * C::kHalf / kFp8Block : t.n * TN / kFp8Block;
+        const int nb1 = SWIGLU || TN == 128 ? nb0 : nb0 + 1;
+        const int nb = (lane & 4) ? (nb1 < a.NB ? nb1 : a.NB - 1) : nb0;
+        const float* ws = (SWIGLU && (lane & 4) ? a.ws_up : a.ws) + ((int64_t)t.e * a.NB + nb) * KB + (lane & 3);
+        for (int kb = 0; kb < KB; kb += kSlotBlocks, sl.next()) {
+          float v[kSlotBlocks][4], w = 0.0f;
+#pragma unroll
+          for (int j = 0; j < kSlotBlocks; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int row = r0 + i * 32 + lane;
+              v[j][i] = kb + j < KB && row < t.row_end ? __ldg(a.xs + (int64_t)(kb + j) * a.xs_pitch + row) : 0.0f;
+            }
+          if (lane < 8 && kb + (lane & 3) < KB) w = __ldg(ws + kb);
+          ok = warp_wait(&bars->sc_empty[sl.i], sl.phase ^ 1u, a.err, abort_flag, kSite + 6);
+          if (!ok) break;
+          ScaleSlot* s = slots + sl.i;
+#pragma unroll
+          for (int j = 0; j < kSlotBlocks; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s->row[j][i * 32 + lane] = v[j][i];
+          if (lane < 8) s->col[lane & 3][lane >> 2] = w;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars->sc_full[sl.i]);   // (release: the warp's stores are before it)
+        }
+      }
+    }
+  } else {
+    // ------------------------------------------------------------------ epilogue
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsEpi));
+    const int q = warp & 3, half = (warp - kEpiWarp0) >> 2;
+    const uint32_t lane_base = (uint32_t)(q * 32) << 16;
+    const uint32_t empty_addr = mapa_u32(&bars->acc_empty[0], 0);
+    const int64_t pitch = (int64_t)a.N * (a.out_dtype == LMOE_DTYPE_F32 ? 4 : 2);
+    uint8_t* stage = store_stage + (warp - kEpiWarp0) * kStoreBytes;
+    constexpr int kChunks = C::kCols / 32;
+    // first column of chunk c in the tile: SwiGLU half of the gate's columns, then the same of up
+    auto column = [&](int c) {
+      if (!SWIGLU) return half * C::kCols + c * 32;
+      return c < kChunks / 2 ? half * (C::kHalf / 2) + c * 32
+                             : C::kHalf + half * (C::kHalf / 2) + (c - kChunks / 2) * 32;
+    };
+    Ring<C::kAcc> ac;
+    Ring<kSlots> sl;
+    int hint = 0;
+    bool ok = true;
+    for (int tile = first; tile < total && ok; tile += stride) {
+      const Fp8Tile t = fp8_tile_at(seg, a, tile, hint);
+      const int row = t.row0 + (int)rank * kRowsCta + q * 32;   // the warp's first
+      const int rows = t.row_end - row < 32 ? t.row_end - row : 32;
+      float acc[C::kCols];
+#pragma unroll
+      for (int i = 0; i < C::kCols; ++i) acc[i] = 0.0f;
+      if (!t.zero) {
+        for (int kb = 0; kb < KB && ok; ++kb) {
+          const int j = kb % kSlotBlocks;
+          if (j == 0) ok = warp_wait(&bars->sc_full[sl.i], sl.phase, a.err, abort_flag, kSite + 7);
+          if (ok) ok = warp_wait(&bars->acc_full[ac.i], ac.phase, a.err, abort_flag, kSite + 8);
+          if (!ok) break;
+          tc_fence_after();
+          if (rows > 0) {   // else the segment ends before this warp's rows
+            const ScaleSlot* s = slots + sl.i;
+            const float sx = s->row[j][q * 32 + lane];
+            const float f0 = __fmul_rn(sx, s->col[j][SWIGLU || TN == 128 ? 0 : half]);
+            const float f1 = SWIGLU ? __fmul_rn(sx, s->col[j][1]) : f0;
+            const uint32_t col = tmem + lane_base + ac.i * TN;
+            uint32_t r[2][32];
+            tmem_ld32_async(col + column(0), r[0]);
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c) {
+              tmem_arrived(r[c & 1]);
+              if (c + 1 < kChunks) tmem_ld32_async(col + column(c + 1), r[(c + 1) & 1]);
+              add_scaled(acc + c * 32, r[c & 1], SWIGLU && c >= kChunks / 2 ? f1 : f0);
+            }
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(empty_addr + ac.i * 8);
+          ac.next();
+          if (j == kSlotBlocks - 1 || kb == KB - 1) {
+            if (lane == 0) mbar_arrive(&bars->sc_empty[sl.i]);
+            sl.next();
+          }
+        }
+        if (!ok) break;
+      }
+      if (rows <= 0) continue;
+      uint8_t* out = static_cast<uint8_t*>(a.out) + (int64_t)row * pitch;
+      const bool whole = rows == 32 && a.store != kStoreStaged;   // blocks leave by TMA
+      constexpr int kOut = SWIGLU ? kChunks / 2 : kChunks;
+#pragma unroll
+      for (int b = 0; b < kOut; ++b) {
+        float f[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          f[i] = SWIGLU ? silu(acc[b * 32 + i]) * acc[(b + kOut) * 32 + i] : acc[b * 32 + i];
+        const int c = t.n * (SWIGLU ? C::kHalf : TN) + column(b);
+        if (c >= a.N) continue;
+        if (!whole) {
+          store_rows<32, kStoreBytes>(out, pitch, rows, c, a.N, f, a.out_dtype, a.store, stage, lane);
+        } else {
+          store_block<64>(&tm_out, f, a.out_dtype, stage, lane, c, row, 0);
+          if (a.out_dtype == LMOE_DTYPE_F32 && c + 16 < a.N)
+            store_block<64>(&tm_out, f + 16, a.out_dtype, stage, lane, c + 16, row, 0);
+        }
+      }
+    }
+    if (elect_one()) bulk_wait_all();   // the stores are complete
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();   // the other CTA's arrivals and the MMAs on this CTA's memory are done
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem, kTmemCols);
+  }
+}
+
+template <int TN, bool SWIGLU>
+int launch(const CUtensorMap& x, const CUtensorMap& x32, const CUtensorMap& w, const CUtensorMap& up,
+           const CUtensorMap& out, const Fp8Args& a, int grid, cudaStream_t stream) {
+  auto fn = fp8_gemm_kernel<TN, SWIGLU>;
+  const int st = set_max_dynamic_smem(reinterpret_cast<const void*>(fn), smem_bytes<TN>());
+  if (st != LMOE_OK) return st;
+  fn<<<grid, kThreads, smem_bytes<TN>(), stream>>>(x, x32, w, up, out, a);
+  return cuda_status(cudaGetLastError());
+}
+
+}  // namespace
+
+int run_fp8_gemm(const Fp8Problem& p, cudaStream_t stream) {
+  DeviceInfo dev;
+  int st = get_device_info(&dev);
+  if (st != LMOE_OK) return st;
+  if (dev.cc_major != 10) return LMOE_ERR_DEVICE;
+  const bool swiglu = p.wq_up != nullptr;
+  const int grid = gemm_grid(dev) < 2 ? 2 : gemm_grid(dev) & ~1;   // whole pairs
+  const int widths[2] = {256, 128};
+  const int mats = swiglu ? 2 : 1;
+  const int tn = pick_width(widths, grid / 2, 0, 0, [&](int w) {
+    return even_row_tiles(p.total_rows, p.num_experts, kTM) * (((int64_t)p.N * mats + w - 1) / w);
+  });
+  Fp8Args a = {};
+  a.xs = p.xs;
+  a.xs_pitch = p.xs_pitch;
+  a.ws = p.ws;
+  a.ws_up = p.ws_up;
+  a.offsets = p.offsets;
+  a.offsets_i64 = p.offsets_i64;
+  a.E = p.num_experts;
+  a.N = p.N;
+  a.KB = (p.K + kBK - 1) / kBK;
+  a.NB = (p.N + kFp8Block - 1) / kFp8Block;
+  a.R = p.total_rows;
+  a.raster = Raster((int)(((int64_t)p.N * mats + tn - 1) / tn));
+  a.out = p.out;
+  a.out_dtype = p.out_dtype;
+  a.store = store_mode(p.out, p.N, p.out_dtype);
+  a.err = p.err;
+  CUtensorMap tx, tx32, tw, tu, to = {};
+  if (a.store != kStoreStaged) {
+    st = encode_store_map(&to, p.out, p.out_dtype, (uint64_t)p.N, (uint64_t)p.total_rows, 1, 64);
+    if (st != LMOE_OK) return st;
+  }
+  const uint64_t kb = (uint64_t)p.K;
+  st = encode_tmap_2d(&tx, p.xq, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, (uint64_t)p.total_rows, kb, kb, kRowsCta, kBK, true);
+  if (st != LMOE_OK) return st;
+  st = encode_tmap_2d(&tx32, p.xq, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, (uint64_t)p.total_rows, kb, kb, 32, kBK, true);
+  if (st != LMOE_OK) return st;
+  const uint64_t dims[3] = {kb, (uint64_t)p.N, (uint64_t)p.num_experts};
+  const uint64_t strides[2] = {kb, kb * (uint64_t)p.N};
+  const uint32_t box[3] = {(uint32_t)kBK, (uint32_t)tn / 2, 1};
+  st = encode_tmap_3d(&tw, p.wq, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, dims, strides, box);
+  if (st != LMOE_OK) return st;
+  tu = tw;
+  if (swiglu) {
+    st = encode_tmap_3d(&tu, p.wq_up, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, dims, strides, box);
+    if (st != LMOE_OK) return st;
+  }
+  if (tn == 256)
+    return swiglu ? launch<256, true>(tx, tx32, tw, tu, to, a, grid, stream)
+                  : launch<256, false>(tx, tx32, tw, tu, to, a, grid, stream);
+  return swiglu ? launch<128, true>(tx, tx32, tw, tu, to, a, grid, stream)
+                : launch<128, false>(tx, tx32, tw, tu, to, a, grid, stream);
+}
+
+}  // namespace lmoe
+
+using namespace lmoe;
+
+extern "C" int lmoe_fp8_grouped_gemm(const uint8_t* xq, const float* xs, int64_t xs_pitch, int64_t total_rows, int K,
+                                     const uint8_t* wq, const float* ws, const uint8_t* wq_up, const float* ws_up,
+                                     int N, const void* expert_offsets, int offsets_are_int64, int num_experts,
+                                     int out_dtype, void* output, uint32_t* error, lmoe_stream_t stream_) {
+  cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
+  LMOE_ARG_CHECK(out_dtype == LMOE_DTYPE_BF16 || out_dtype == LMOE_DTYPE_F16 || out_dtype == LMOE_DTYPE_F32);
+  LMOE_ARG_CHECK(total_rows >= 0 && N > 0 && K > 0 && K % 16 == 0);
+  // indexes of whole tiles and stages stay within 32 bits
+  LMOE_ARG_CHECK(total_rows <= kMaxGemmSize && N <= kMaxGemmSize / 2 && K <= kMaxGemmSize);
+  LMOE_ARG_CHECK(num_experts >= 1);
+  if (num_experts > kMaxGemmExperts) return LMOE_ERR_UNSUPPORTED;
+  LMOE_ARG_CHECK((wq_up == nullptr) == (ws_up == nullptr));
+  LMOE_ARG_CHECK(xs_pitch >= total_rows);
+  if (total_rows == 0) return LMOE_OK;
+  LMOE_ARG_CHECK(xq && xs && wq && ws && expert_offsets && output);
+  LMOE_ARG_CHECK(aligned16(xq) && aligned16(wq) && aligned16(wq_up));
+  LMOE_ARG_CHECK(((reinterpret_cast<uintptr_t>(xs) | reinterpret_cast<uintptr_t>(ws) |
+                   reinterpret_cast<uintptr_t>(ws_up)) & 3) == 0);
+  LMOE_ARG_CHECK(reinterpret_cast<uintptr_t>(expert_offsets) % (offsets_are_int64 ? 8 : 4) == 0);
+  LMOE_ARG_CHECK(reinterpret_cast<uintptr_t>(output) % (out_dtype == LMOE_DTYPE_F32 ? 4 : 2) == 0);
+  Fp8Problem p;
+  p.xq = xq;
+  p.xs = xs;
+  p.xs_pitch = xs_pitch;
+  p.total_rows = total_rows;
+  p.K = K;
+  p.wq = wq;
+  p.ws = ws;
+  p.wq_up = wq_up;
+  p.ws_up = ws_up;
+  p.N = N;
+  p.offsets = expert_offsets;
+  p.offsets_i64 = offsets_are_int64;
+  p.num_experts = num_experts;
+  p.out_dtype = out_dtype;
+  p.out = output;
+  p.err = error;
+  return run_fp8_gemm(p, stream);
+}

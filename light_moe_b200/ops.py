@@ -11,7 +11,7 @@ Same names, argument names and return types as the reference's ``light_moe._C``
 plus the new ops (``fused_gate_topk_ex``, ``quantize_w4``, ``dequantize_w4``, ``prepack_w4``,
 ``w4a16_grouped_gemm``, ``moe_layer_w4a16``; the gradients ``grouped_gemm_dgrad`` and
 ``grouped_gemm_wgrad``; the 4-bit floating point ``quantize_fp4``, ``dequantize_fp4`` and
-``fp4_grouped_gemm``).  Every op runs the CUDA library; if the
+``fp4_grouped_gemm``; the 8-bit ``quantize_fp8``, ``dequantize_fp8`` and ``fp8_grouped_gemm``).  Every op runs the CUDA library; if the
 ``_C`` extension has not been built, calling any op raises -- there is no fallback path.
 """
 from __future__ import annotations
@@ -132,6 +132,37 @@ def fp4_grouped_gemm(input, input_scales, weights, weight_scales, expert_offsets
     ``error`` as for grouped_gemm_dgrad."""
     return extension().fp4_grouped_gemm(input, input_scales, weights, weight_scales, expert_offsets, num_experts,
                                         format, alpha, weights_up, weight_scales_up, alpha_up, out_dtype, error)
+
+
+def quantize_fp8(x, block_rows=1, power_of_two=False, positions=None):
+    """x [..., rows, K] (bf16 / fp16 / fp32, K % 16 == 0) -> (codes float8_e4m3fn [..., rows, K], scales fp32
+    [..., rows / block_rows, K / 128], both rounded up): one scale per 128 columns of a row (``block_rows=1``,
+    activations) or per block of 128 x 128 (``block_rows=128``, weights).
+
+    scale = max(max|x| / 448, 2**-126), rounded up to a power of two with ``power_of_two``; codes are the
+    nearest E4M3 values of x / scale, ties to even; blocks with an infinity or NaN read back as NaN.
+    Scales of rows lie block after block (the returned tensor is a view with stride 1 along the rows).
+
+    ``positions`` (``block_rows=1``) int32 [rows, copies] (a permutation of 0 .. rows * copies - 1): row r
+    is written to rows positions[r, :], as for ``quantize_fp4``."""
+    return extension().quantize_fp8(x, block_rows, power_of_two, positions)
+
+
+def dequantize_fp8(q, scales, block_rows=1, out_dtype=None):
+    """Codes and scales (any strides) -> ``out_dtype`` (bf16 by default) [..., rows, K]:
+    rn(fp32_rn(code * scale))."""
+    return extension().dequantize_fp8(q, scales, block_rows, out_dtype)
+
+
+def fp8_grouped_gemm(input, input_scales, weights, weight_scales, expert_offsets, num_experts, weights_up=None,
+                     weight_scales_up=None, out_dtype=None, error=None):
+    """Grouped product of 8-bit operands (codes and scales as quantize_fp8 returns them): rows [T, K] with
+    scales [T, K / 128] x weights [E, N, K] with scales [E, N / 128, K / 128] -> [T, N] of ``out_dtype`` (bf16 by
+    default).  With ``weights_up``: silu(gate) * up.  Exact products, fp32 sums; rows outside every expert
+    are zero.  Scales of rows that do not have stride 1 along the rows are copied.  ``error`` as for
+    grouped_gemm_dgrad."""
+    return extension().fp8_grouped_gemm(input, input_scales, weights, weight_scales, expert_offsets, num_experts,
+                                        weights_up, weight_scales_up, out_dtype, error)
 
 
 def combine_rows(rows, positions, weights, num_tokens, top_k, extra_rows=None, num_extra=0):
