@@ -354,6 +354,30 @@ int lmoe_fp8_grouped_gemm(const uint8_t* xq, const float* xs, int64_t xs_pitch, 
                           const void* expert_offsets, int offsets_are_int64, int num_experts, int out_dtype,
                           void* output, uint32_t* error, lmoe_stream_t stream);
 
+/* A whole MoE layer for at most 16 tokens in two kernels: router (softmax, top-k with ties to the lower
+ * id, renormalised weights), y[t] = sum_j weights[t, j] * w2 (silu(w1 x) * (w3 x)) of expert ids[t, j], plus
+ * the num_shared experts behind the routed ones (weight 1).
+ *   x [num_tokens, hidden_size], gate_weight [num_experts, hidden_size] of dtype (LMOE_DTYPE_BF16 or _F16),
+ *     16-byte aligned; gate_bias fp32 [num_experts] or NULL
+ *   w1, w3 [E + S, ffn, hidden], w2 [E + S, hidden, ffn], 32-byte aligned: of dtype, or (with the three
+ *     scales) E4M3 codes with fp32 scales of blocks of 128 x 128 as lmoe_quantize_fp8_blocks writes them
+ *   y [num_tokens, hidden_size] of dtype; ids int32, weights fp32 [num_tokens, top_k]
+ * Hidden values stay in fp32 between the kernels and enter the second product as a sum of two 16-bit
+ * numbers; all sums are fp32.  Values below 2^-39 of a token's largest (bf16 tokens with E4M3 weights) or
+ * of its largest hidden value nearby (fp16 products) are lost.
+ * hidden_size % 64 == 0, at most 16384; ffn_size % 32 == 0, at most 65536; num_experts <= 256, top_k <= 16,
+ * num_shared <= 16; LMOE_ERR_UNSUPPORTED where eight tokens of that hidden size do not fit shared memory
+ * (from about 11000 on for eight).  The result does not depend on timing.  The workspace
+ * (lmoe_few_tokens_workspace_bytes; 0 for sizes that are refused), 16-byte aligned, need not be cleared;
+ * calls that may run at the same time need one each. */
+size_t lmoe_few_tokens_workspace_bytes(int64_t num_tokens, int hidden_size, int ffn_size, int num_experts, int top_k,
+                                       int num_shared);
+int lmoe_moe_layer_few_tokens(const void* x, int dtype, int64_t num_tokens, int hidden_size, const void* gate_weight,
+                              const float* gate_bias, int num_experts, int top_k, int num_shared, const void* w1,
+                              const void* w3, const void* w2, const float* w1_scales, const float* w3_scales,
+                              const float* w2_scales, int ffn_size, void* y, int32_t* ids, float* weights,
+                              void* workspace, size_t workspace_bytes, lmoe_stream_t stream);
+
 /* Weighted combine of per-slot expert rows back to tokens:
  *   y[t, :] = sum_j weights[t*top_k+j] * rows[positions[t*top_k+j], :]
  *             + sum_s extra_rows[s*num_tokens + t, :]

@@ -82,6 +82,9 @@ SIGNATURES = {
     "lmoe_quantize_fp8_blocks": (_I, [_P, _I, _I64, _I64, _I, _I, _P, _P, _P]),
     "lmoe_dequantize_fp8": (_I, [_P, _P, _I64, _I64, _I64, _I64, _I64, _I, _I, _I, _P, _P]),
     "lmoe_fp8_grouped_gemm": (_I, [_P, _P, _I64, _I64, _I, _P, _P, _P, _P, _I, _P, _I, _I, _I, _P, _P, _P]),
+    "lmoe_few_tokens_workspace_bytes": (_SZ, [_I64, _I, _I, _I, _I, _I]),
+    "lmoe_moe_layer_few_tokens": (_I, [_P, _I, _I64, _I, _P, _P, _I, _I, _I, _P, _P, _P, _P, _P, _P, _I, _P, _P, _P, _P,
+                                       _SZ, _P]),
     "lmoe_combine_rows": (_I, [_P, _P, _P, _I64, _I, _I, _P, _I, _P, _P]),
     "lmoe_moe_layer_workspace_bytes": (_SZ, [_I64, _I, _I, _I, _I, _I]),
     "lmoe_moe_layer_w4a16": (_I, [_P, _I64, _I, _P, _P, _I, _I, _I, _P, _P, _I, _I, _P, _P, _P, _P, _SZ, _P]),

@@ -810,6 +810,83 @@ torch::Tensor fp8_grouped_gemm(torch::Tensor input, torch::Tensor input_scales, 
   return out;
 }
 
+// ---------------------------------------------------------------- a whole layer for a few tokens
+
+torch::Tensor aligned32_contig(const torch::Tensor& t) {
+  auto c = t.contiguous();
+  return reinterpret_cast<uintptr_t>(c.data_ptr()) % 32 == 0 ? c : c.clone();
+}
+
+std::vector<torch::Tensor> moe_layer_few_tokens(torch::Tensor x, torch::Tensor gate_weight, torch::Tensor w1,
+                                                torch::Tensor w3, torch::Tensor w2, int64_t top_k,
+                                                std::optional<torch::Tensor> w1_scales,
+                                                std::optional<torch::Tensor> w3_scales,
+                                                std::optional<torch::Tensor> w2_scales, int64_t num_shared,
+                                                std::optional<torch::Tensor> gate_bias) {
+  check_cuda(x, "x");
+  const auto xt = x.scalar_type();
+  TORCH_CHECK(xt == torch::kBFloat16 || xt == torch::kFloat16, "x must be bf16 or fp16, is ", xt);
+  TORCH_CHECK(x.dim() == 2 && gate_weight.dim() == 2 && w1.dim() == 3 && w2.dim() == 3,
+              "x [T,d], gate_weight [E,d], w1 and w3 [E+S,ffn,d], w2 [E+S,d,ffn]");
+  check_same_device(gate_weight, x, "gate_weight");
+  TORCH_CHECK(gate_weight.scalar_type() == xt, "x and gate_weight differ in dtype");
+  const int64_t T = x.size(0), d = x.size(1), E = gate_weight.size(0), F = w1.size(1);
+  TORCH_CHECK(T <= 16, "moe_layer_few_tokens takes at most 16 tokens, got ", T);
+  TORCH_CHECK(gate_weight.size(1) == d, "gate_weight must be [E, d]");
+  TORCH_CHECK(num_shared >= 0 && num_shared <= 16, "num_shared must be 0 .. 16");
+  TORCH_CHECK(E >= 1 && E <= 256, "1 to 256 experts");
+  TORCH_CHECK(top_k >= 1 && top_k <= 16 && top_k <= E, "top_k must be 1 .. min(16, num_experts)");
+  TORCH_CHECK(d >= 64 && d % 64 == 0 && d <= 16384, "the hidden size must be a multiple of 64, at most 16384");
+  TORCH_CHECK(F >= 32 && F % 32 == 0 && F <= 65536, "the ffn size must be a multiple of 32, at most 65536");
+  const int64_t n = E + num_shared;
+  TORCH_CHECK(w1.sizes() == w3.sizes() && w1.size(0) == n && w1.size(2) == d && w2.size(0) == n && w2.size(1) == d &&
+                  w2.size(2) == F,
+              "w1 and w3 must be [E+S, ffn, d], w2 [E+S, d, ffn]");
+  const bool fp8 = w1_scales.has_value() && w1_scales->defined();
+  TORCH_CHECK(fp8 == (w3_scales.has_value() && w3_scales->defined()) &&
+                  fp8 == (w2_scales.has_value() && w2_scales->defined()),
+              "w1_scales, w3_scales and w2_scales belong together");
+  const at::AutoDispatchBelowADInplaceOrView below_autograd;   // no graph is recorded
+  const c10::cuda::OptionalCUDAGuard guard(x.device());
+  torch::Tensor w[3] = {w1, w3, w2}, s[3];
+  const char* names[3] = {"w1", "w3", "w2"};
+  for (int i = 0; i < 3; ++i) {
+    if (fp8) {
+      const auto c = fp8_weights(w[i], i == 0 ? *w1_scales : i == 1 ? *w3_scales : *w2_scales, x, n, i < 2 ? F : d,
+                                 i < 2 ? d : F, names[i]);
+      w[i] = c.q;
+      s[i] = c.s;
+    } else {
+      check_same_device(w[i], x, names[i]);
+      TORCH_CHECK(w[i].scalar_type() == xt, names[i], " must be of x's dtype, or float8_e4m3fn with scales");
+    }
+    w[i] = aligned32_contig(w[i]);
+  }
+  torch::Tensor b;
+  if (gate_bias.has_value() && gate_bias->defined()) {
+    check_same_device(*gate_bias, x, "gate_bias");
+    TORCH_CHECK(gate_bias->scalar_type() == torch::kFloat32 && gate_bias->numel() == E, "gate_bias must be fp32 [E]");
+    b = gate_bias->contiguous();
+  }
+  auto xc = contig16(x);
+  auto gw = contig16(gate_weight);
+  auto y = empty_like_device({T, d}, xt, x);
+  auto ids = empty_like_device({T, top_k}, torch::kInt32, x);
+  auto wts = empty_like_device({T, top_k}, torch::kFloat32, x);
+  if (T > 0) {
+    const auto bytes = (int64_t)lmoe_few_tokens_workspace_bytes(T, (int)d, (int)F, (int)E, (int)top_k, (int)num_shared);
+    auto ws = empty_like_device({bytes}, torch::kUInt8, x);
+    check_status(lmoe_moe_layer_few_tokens(
+                     xc.data_ptr(), dtype_code(xc), T, (int)d, gw.data_ptr(), b.defined() ? b.data_ptr<float>() : nullptr,
+                     (int)E, (int)top_k, (int)num_shared, w[0].data_ptr(), w[1].data_ptr(), w[2].data_ptr(),
+                     fp8 ? s[0].data_ptr<float>() : nullptr, fp8 ? s[1].data_ptr<float>() : nullptr,
+                     fp8 ? s[2].data_ptr<float>() : nullptr, (int)F, y.data_ptr(), ids.data_ptr<int32_t>(),
+                     wts.data_ptr<float>(), ws.data_ptr(), (size_t)bytes, cur_stream()),
+                 "moe_layer_few_tokens");
+  }
+  return {y, ids, wts};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -857,6 +934,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("input_scales"), py::arg("weights"), py::arg("weight_scales"), py::arg("expert_offsets"),
         py::arg("num_experts"), py::arg("weights_up") = py::none(), py::arg("weight_scales_up") = py::none(),
         py::arg("out_dtype") = py::none(), py::arg("error") = py::none());
+  m.def("moe_layer_few_tokens", &moe_layer_few_tokens, "MoE layer for up to 16 tokens", py::arg("x"),
+        py::arg("gate_weight"), py::arg("w1"), py::arg("w3"), py::arg("w2"), py::arg("top_k"),
+        py::arg("w1_scales") = py::none(), py::arg("w3_scales") = py::none(), py::arg("w2_scales") = py::none(),
+        py::arg("num_shared") = 0, py::arg("gate_bias") = py::none());
   m.def("combine_rows", &combine_rows, "Weighted combine of slot rows back to tokens", py::arg("rows"),
         py::arg("positions"), py::arg("weights"), py::arg("num_tokens"), py::arg("top_k"),
         py::arg("extra_rows") = py::none(), py::arg("num_extra") = 0);

@@ -1,0 +1,873 @@
+// few_tokens.cu -- a whole MoE layer for up to 16 tokens in two kernels (sm_100a).
+//
+//   p = softmax(x G^T + bias), the k most probable experts (ties to the lower id), w = p / sum of theirs
+//   y[t] = sum_j w[t, j] * W2[e_j] (silu(W1[e_j] x[t]) * (W3[e_j] x[t]))  + the same of every shared expert, w = 1
+//
+// Weights dense (the tokens' 16-bit type) or E4M3 with a scale per 128 x 128 block (fp8_format.cuh).  A
+// few tokens read every weight of their experts once and do a few operations with it: the kernels
+// are bound by HBM, and what they have to do is keep enough loads in flight and spend few
+// instructions on a weight.
+//
+// Warps load weights straight into the fragments of mma.sync.m16n8k16, whose 16 rows are weight rows
+// and whose 8 columns are tokens: which contraction index a lane's register stands for is free as
+// long as both operands agree, so a lane takes 32 consecutive bytes of a row (the quad of a row 128)
+// and no weight passes through shared memory.  One instruction multiplies 256 weights with all
+// tokens, against 256 x tokens / 32 multiply-adds on the CUDA cores; a 5th-generation MMA would
+// want its operands in shared memory, which costs more than it gives for 8 columns.  E4M3 values are
+// exact in fp16.
+//
+// Every expert that some token chose is multiplied with ALL tokens, since columns are free; results
+// of tokens that did not choose it are dropped.  So there is no permutation, and the second kernel
+// is one product over the contraction (expert, hidden feature) whose sum is the weighted combine.
+//
+// 1. gate_up_kernel.  Every CTA computes the routing for itself (a few microseconds of L2 reads; a
+//    kernel of its own would cost more), then the CTAs share the tiles of 8 hidden features: rows 0-7
+//    of an MMA are gate rows and rows 8-15 the same rows of up, so one thread holds gate and up of
+//    a feature.  The 16 warps of a CTA split a tile's contraction and join it in shared memory.
+//    Writes w * silu(gate) * up in fp32.
+// 2. down_kernel.  A CTA owns 256 output rows (a warp 16) and a slice of the contraction; the last
+//    CTA of a row block to finish adds the slices in their order, so the result does not depend on
+//    timing.  Hidden values enter the MMA as a sum of two 16-bit numbers (22 bits in fp16, 16 in bf16),
+//    which costs a second MMA but no weight traffic: rounding them to one would be an error as large
+//    as the output's own rounding.
+//
+// fp16 operands need a range: tokens (bf16 times E4M3 weights) and hidden values are scaled by powers of
+// two, per token and per staged chunk, so that the largest lies in [2^14, 2^15); what is 2^-39 of it or
+// smaller is lost.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <type_traits>
+
+#include "fp8_format.cuh"
+#include "host_util.h"
+#include "lmoe_math.cuh"
+#include "ptx.cuh"
+
+namespace lmoe {
+namespace {
+
+constexpr int kWarps = 16, kThreads = kWarps * 32;
+constexpr int kMaxTokens = 16, kMaxExperts = 256, kMaxShared = 16, kMaxTopK = 16;
+constexpr int kMaxUsed = kMaxExperts + kMaxShared;
+constexpr int kAhead = 3;        // steps of weights in flight per warp
+constexpr int kRowBlock = kWarps * 16;   // output rows of a CTA of the second kernel
+constexpr int kSplitCtas = 148;  // CTAs that the second kernel's slices aim at: one per SM
+constexpr int kChunk = 6;        // steps of hidden values staged at a time
+static_assert(kChunk % kAhead == 0, "a chunk starts at the first of the buffers in flight");
+constexpr float kInf = __builtin_huge_valf();
+
+// What the first kernel tells the second.
+struct Header {
+  int used;                  // experts with tokens
+  int pad[3];
+  int expert[kMaxUsed];      // ascending, shared ones last
+  uint32_t tokens[kMaxUsed]; // bit t: token t chose it
+};
+
+struct FewArgs {
+  const void* x;             // [T, d]
+  const void* gate;          // [E, d]
+  const float* bias;
+  const uint8_t* w1;         // [E + S, F, d]
+  const uint8_t* w3;
+  const uint8_t* w2;         // [E + S, d, F]
+  const float* s1;           // block scales (fp8)
+  const float* s3;
+  const float* s2;
+  int T, d, F, E, k, S;
+  int groups;                // token groups of the first kernel
+  int split;                 // slices of the second kernel
+  void* y;
+  int32_t* ids;
+  float* weights;
+  Header* head;
+  uint32_t* counters;        // arrivals per row block
+  float* h;                  // [used][T][F]
+  float* part;               // [split][T][d]
+};
+
+// A weight row's 32 bytes per lane and step.
+template <bool FP8>
+struct Geo {
+  static constexpr int kPer = FP8 ? 32 : 16;      // values of a lane
+  static constexpr int kStep = 4 * kPer;          // values of a step: of the quad of a row
+  static constexpr int kPieces = kPer / 8;        // 16-byte pieces (8 values) of the 16-bit operand
+  static constexpr int kBytes = FP8 ? 1 : 2;
+};
+
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                         uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<T, __half>::value)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Two rows' 32 bytes (rows g and g + 8 of the MMA) times piece p of the other operand.
+template <bool FP8, typename M>
+__device__ __forceinline__ void mma_piece(float (&c)[4], const uint32_t (&lo)[8], const uint32_t (&hi)[8], int p,
+                                          const uint4& b) {
+  if constexpr (FP8) {
+    mma16816<M>(c, e4m3x2_half2(lo[2 * p]), e4m3x2_half2(hi[2 * p]), e4m3x2_half2_high(lo[2 * p]),
+                e4m3x2_half2_high(hi[2 * p]), b.x, b.y);
+    mma16816<M>(c, e4m3x2_half2(lo[2 * p + 1]), e4m3x2_half2(hi[2 * p + 1]), e4m3x2_half2_high(lo[2 * p + 1]),
+                e4m3x2_half2_high(hi[2 * p + 1]), b.z, b.w);
+  } else {
+    mma16816<M>(c, lo[4 * p], hi[4 * p], lo[4 * p + 1], hi[4 * p + 1], b.x, b.y);
+    mma16816<M>(c, lo[4 * p + 2], hi[4 * p + 2], lo[4 * p + 3], hi[4 * p + 3], b.z, b.w);
+  }
+}
+
+// Offset of the 16-byte piece with values 8 * q .. 8 * q + 7 of token t in an operand of `tokens` tokens:
+// [step][piece][token][lane of the quad], so that a quarter warp reads 128 consecutive bytes.
+template <bool FP8>
+__device__ __forceinline__ uint32_t piece_offset(int q, int t, int tokens) {
+  using G = Geo<FP8>;
+  const int step = q / (G::kStep / 8), in = q % (G::kStep / 8);
+  return (((uint32_t)step * G::kPieces + in % G::kPieces) * tokens + t) * 64 + in / G::kPieces * 16;
+}
+
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }   // -126 .. 127
+
+// Exponent that brings the largest absolute value (its fp32 bits, finite) to [2^14, 2^15).
+__device__ __forceinline__ int range_exponent(uint32_t top) {
+  if (top == 0) return 0;
+  const int e = 14 - ((int)(top >> 23) - 127);   // subnormals count as 2^-127
+  return e > 126 ? 126 : e;
+}
+
+template <typename T>
+__device__ __forceinline__ float2 widen2(uint32_t w) {
+  if constexpr (std::is_same<T, __half>::value)
+    return __half22float2(*reinterpret_cast<const __half2*>(&w));
+  else
+    return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w));
+}
+template <typename T>
+__device__ __forceinline__ uint32_t narrow2(float a, float b) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+// fp32 bits of the largest finite absolute value of a 16-bit pair.
+template <typename T>
+__device__ __forceinline__ uint32_t finite_top(uint32_t w) {
+  const float2 v = widen2<T>(w);
+  const uint32_t a = __float_as_uint(v.x) & 0x7fffffffu, b = __float_as_uint(v.y) & 0x7fffffffu;
+  return max(a < 0x7f800000u ? a : 0u, b < 0x7f800000u ? b : 0u);
+}
+
+// ---------------------------------------------------------------------------------------
+// first kernel
+// ---------------------------------------------------------------------------------------
+struct FewShared {
+  uint32_t used_tokens[kMaxUsed];   // bit t: token t chose expert e (all experts)
+  int list[kMaxUsed];               // experts with tokens
+  int group[kMaxUsed];              // positions in `list` that have tokens of the group
+  int used, group_used;
+  uint32_t top[kMaxTokens];         // largest absolute value of the group's tokens
+  float unscale[kMaxTokens];
+  int chosen[kMaxTokens][kMaxTopK];
+  float weight[kMaxTokens][kMaxTopK];
+};
+
+// Dynamic shared memory of the first kernel.
+struct FewLayout {
+  uint32_t x, red, logits, share, total;
+};
+__host__ __device__ inline FewLayout few_layout(int d, int step, int group_tokens, int T, int E, int S) {
+  FewLayout l;
+  const uint32_t kpad = (uint32_t)(d + step - 1) / step * step;
+  const uint32_t nt = group_tokens > 8 ? 2 : 1;
+  l.x = 0;
+  l.red = kpad * group_tokens * 2;
+  l.logits = l.red + 2 * kWarps * 16 * 8 * nt * 4;
+  l.share = l.logits + (uint32_t)(T * E + 3) / 4 * 16;
+  l.total = l.share + (uint32_t)((E + S) * T + 3) / 4 * 16;
+  return l;
+}
+
+template <bool FP8, typename X, int NT>
+__global__ void __launch_bounds__(kThreads, 1) gate_up_kernel(const FewArgs a) {
+  using G = Geo<FP8>;
+  using M = typename std::conditional<FP8, __half, X>::type;   // type of the products
+  constexpr bool kScaled = FP8 && std::is_same<X, __nv_bfloat16>::value;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ FewShared sh;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
+  const int steps = (a.d + G::kStep - 1) / G::kStep;
+  const int per_group = a.groups == 1 ? a.T : 8;
+  const FewLayout lay = few_layout(a.d, G::kStep, per_group, a.T, a.E, a.S);
+  float* red = reinterpret_cast<float*>(smem + lay.red);
+  float* logits = reinterpret_cast<float*>(smem + lay.logits);   // [T][E]
+  float* share = reinterpret_cast<float*>(smem + lay.share);     // [E + S][T]: routing weights
+  constexpr int kRedRow = 8 * NT, kRedWarp = 16 * kRedRow, kRedBuf = kWarps * kRedWarp;
+  const int experts = a.E + a.S;
+
+  // tokens t0 .. t0 + n - 1 into shared memory, in the order of the fragments
+  auto load_x = [&](int t0, int n) {
+    if (kScaled && tid < kMaxTokens) sh.top[tid] = 0;
+    __syncthreads();   // earlier readers of the tokens too
+    const int pieces = steps * G::kStep / 8;   // behind d: zeros
+    for (int i = tid; i < pieces * n; i += kThreads) {
+      const int t = i / pieces, q = i - t * pieces;
+      uint4 v = make_uint4(0u, 0u, 0u, 0u);
+      if (q * 8 < a.d) v = __ldg(reinterpret_cast<const uint4*>(static_cast<const X*>(a.x) + (int64_t)(t0 + t) * a.d) + q);
+      *reinterpret_cast<uint4*>(smem + lay.x + piece_offset<FP8>(q, t, n)) = v;
+      if (kScaled) {
+        const uint32_t m = max(max(finite_top<X>(v.x), finite_top<X>(v.y)), max(finite_top<X>(v.z), finite_top<X>(v.w)));
+        atomicMax(&sh.top[t], m);
+      }
+    }
+    __syncthreads();
+  };
+  // ... and to scaled fp16 in place
+  auto scale_x = [&](int n) {
+    if constexpr (kScaled) {
+      const int pieces = steps * G::kStep / 8;
+      for (int i = tid; i < pieces * n; i += kThreads) {
+        const int t = i / pieces, q = i - t * pieces;
+        const float f = pow2(range_exponent(sh.top[t]));
+        uint4* p = reinterpret_cast<uint4*>(smem + lay.x + piece_offset<FP8>(q, t, n));
+        uint4 v = *p;
+        uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 f2 = widen2<X>(w[j]);
+          w[j] = narrow2<M>(f2.x * f, f2.y * f);
+        }
+        *p = v;
+      }
+    }
+    if (tid < n) sh.unscale[tid] = kScaled ? pow2(-range_exponent(sh.top[tid])) : 1.0f;
+    __syncthreads();
+  };
+
+  // ---- routing: logits, 16 experts at a time
+  for (int t0 = 0; t0 < a.T; t0 += per_group) {
+    const int n = a.T - t0 < per_group ? a.T - t0 : per_group;
+    load_x(t0, n);
+    for (int e0 = 0; e0 < a.E; e0 += 16) {
+      float acc[NT][4];
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
+      const X* r0 = static_cast<const X*>(a.gate) + (int64_t)(e0 + g) * a.d;
+      const X* r1 = r0 + (int64_t)8 * a.d;
+      const bool ok0 = e0 + g < a.E, ok1 = e0 + g + 8 < a.E;
+      for (int s = warp; s < steps; s += kWarps) {
+        uint4 w0[G::kPieces], w1[G::kPieces];
+#pragma unroll
+        for (int p = 0; p < G::kPieces; ++p) {
+          const int at = s * G::kStep + c * G::kPer + p * 8;
+          w0[p] = w1[p] = make_uint4(0u, 0u, 0u, 0u);
+          if (ok0 && at < a.d) w0[p] = __ldg(reinterpret_cast<const uint4*>(r0 + at));
+          if (ok1 && at < a.d) w1[p] = __ldg(reinterpret_cast<const uint4*>(r1 + at));
+        }
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+          float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          const int t = i * 8 + g;
+#pragma unroll
+          for (int p = 0; p < G::kPieces; ++p) {
+            uint4 b = make_uint4(0u, 0u, 0u, 0u);
+            if (t < n) b = *reinterpret_cast<const uint4*>(smem + lay.x + ((uint32_t)(s * G::kPieces + p) * n + t) * 64 + c * 16);
+            mma16816<X>(part, w0[p].x, w1[p].x, w0[p].y, w1[p].y, b.x, b.y);
+            mma16816<X>(part, w0[p].z, w1[p].z, w0[p].w, w1[p].w, b.z, b.w);
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[i][j] += part[j];
+        }
+      }
+      float* mine = red + warp * kRedWarp;
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        *reinterpret_cast<float2*>(mine + g * kRedRow + i * 8 + c * 2) = make_float2(acc[i][0], acc[i][1]);
+        *reinterpret_cast<float2*>(mine + (g + 8) * kRedRow + i * 8 + c * 2) = make_float2(acc[i][2], acc[i][3]);
+      }
+      __syncthreads();
+      for (int i = tid; i < 16 * n; i += kThreads) {
+        const int e = i / n, t = i - e * n;
+        if (e0 + e < a.E) {
+          float v = 0.0f;
+#pragma unroll
+          for (int w = 0; w < kWarps; ++w) v += red[w * kRedWarp + e * kRedRow + t];
+          if (a.bias) v += __ldg(a.bias + e0 + e);
+          logits[(t0 + t) * a.E + e0 + e] = v;
+        }
+      }
+      __syncthreads();
+    }
+  }
+
+  // ---- routing: one warp per token
+  for (int i = tid; i < experts * a.T; i += kThreads) share[i] = i >= a.E * a.T ? 1.0f : 0.0f;
+  for (int e = tid; e < experts; e += kThreads) sh.used_tokens[e] = e >= a.E ? (1u << a.T) - 1u : 0u;
+  __syncthreads();
+  if (warp < a.T) {
+    const int t = warp;
+    float v[kMaxExperts / 32];
+    uint32_t key[kMaxExperts / 32];   // orders like the logits; NaN lowest, 0: none or taken
+#pragma unroll
+    for (int i = 0; i < kMaxExperts / 32; ++i) {
+      const int e = i * 32 + lane;
+      v[i] = e < a.E ? logits[t * a.E + e] : 0.0f;
+      const uint32_t b = __float_as_uint(v[i]);
+      key[i] = e >= a.E ? 0u : (v[i] == v[i] ? ((b & 0x80000000u) ? ~b : (b | 0x80000000u)) : 1u);
+    }
+    float top = 0.0f, sum = 0.0f, mine = 0.0f;
+    int chosen = 0;
+    for (int j = 0; j < a.k; ++j) {
+      uint32_t best = 0u;
+#pragma unroll
+      for (int i = 0; i < kMaxExperts / 32; ++i) best = max(best, key[i]);
+      best = __reduce_max_sync(0xffffffffu, best);
+      int e = kMaxExperts;
+      float l = 0.0f;
+#pragma unroll
+      for (int i = kMaxExperts / 32 - 1; i >= 0; --i)
+        if (key[i] == best) {
+          e = i * 32 + lane;
+          l = v[i];
+        }
+      const int lowest = (int)__reduce_min_sync(0xffffffffu, (unsigned)e);
+      l = __shfl_sync(0xffffffffu, l, lowest & 31);   // the lowest id's lane found it
+#pragma unroll
+      for (int i = 0; i < kMaxExperts / 32; ++i)
+        if (i * 32 + lane == lowest) key[i] = 0u;
+      if (j == 0) top = l;
+      const float p = l == top ? 1.0f : (l == l ? softmax_exp(l - top) : l);
+      sum += p;
+      if (lane == j) {
+        mine = p;
+        chosen = lowest;
+      }
+    }
+    if (lane < a.k) {
+      const float w = __fdiv_rn(mine, sum);
+      share[chosen * a.T + t] = w;
+      atomicOr(&sh.used_tokens[chosen], 1u << t);
+      if (blockIdx.x == 0) {
+        a.ids[t * a.k + lane] = chosen;
+        a.weights[t * a.k + lane] = w;
+      }
+    }
+  }
+  __syncthreads();
+  if (warp == 0) {
+    int n = 0;
+    for (int e0 = 0; e0 < experts; e0 += 32) {
+      const int e = e0 + lane;
+      const bool used = e < experts && sh.used_tokens[e] != 0u;
+      const uint32_t m = __ballot_sync(0xffffffffu, used);
+      if (used) sh.list[n + __popc(m & ((1u << lane) - 1u))] = e;
+      n += __popc(m);
+    }
+    if (lane == 0) sh.used = n;
+  }
+  __syncthreads();
+  if (blockIdx.x == 0) {
+    for (int i = tid; i < sh.used; i += kThreads) {
+      a.head->expert[i] = sh.list[i];
+      a.head->tokens[i] = sh.used_tokens[sh.list[i]];
+    }
+    if (tid == 0) a.head->used = sh.used;
+    for (int i = tid; i < (a.d + kRowBlock - 1) / kRowBlock; i += kThreads) a.counters[i] = 0u;
+  }
+
+  // ---- the experts' gate and up products
+  int wpt = kWarps;   // warps of a tile: a power of two, each with a step at least
+  while (wpt > steps) wpt >>= 1;
+  const int tpp = kWarps / wpt, wi = warp & (wpt - 1), wt = warp / wpt;   // tiles of a pass; this warp's share and tile
+  const int ftiles = a.F / 8;
+  const int kblocks = (a.d + kFp8Block - 1) / kFp8Block, fblocks = (a.F + kFp8Block - 1) / kFp8Block;
+  for (int t0 = 0; t0 < a.T; t0 += per_group) {
+    const int n = a.T - t0 < per_group ? a.T - t0 : per_group;
+    if (a.groups > 1) load_x(t0, n);   // else they are there
+    scale_x(n);
+    const uint32_t in_group = ((1u << n) - 1u) << t0;
+    if (warp == 0) {
+      int m = 0;
+      for (int u0 = 0; u0 < sh.used; u0 += 32) {
+        const int u = u0 + lane;
+        const bool has = u < sh.used && (sh.used_tokens[sh.list[u]] & in_group) != 0u;
+        const uint32_t b = __ballot_sync(0xffffffffu, has);
+        if (has) sh.group[m + __popc(b & ((1u << lane) - 1u))] = u;
+        m += __popc(b);
+      }
+      if (lane == 0) sh.group_used = m;
+    }
+    __syncthreads();
+    const int tiles = sh.group_used * ftiles;
+    const int passes = (tiles + tpp - 1) / tpp;
+    const int my_passes = passes > (int)blockIdx.x ? (passes - 1 - (int)blockIdx.x) / (int)gridDim.x + 1 : 0;
+
+    uint32_t w0[kAhead][8], w1[kAhead][8];
+    float f0[kAhead], f1[kAhead];
+    // the next load: pass and step, and the tile's rows
+    int lp = 0, ls = wi;
+    const uint8_t *p0 = nullptr, *p1 = nullptr;
+    const float *q0 = nullptr, *q1 = nullptr;
+    auto aim = [&]() {
+      const int tile = ((int)blockIdx.x + lp * (int)gridDim.x) * tpp + wt;
+      p0 = nullptr;
+      if (lp < my_passes && tile < tiles) {
+        const int gu = tile / ftiles, ft = tile - gu * ftiles;
+        const int e = sh.list[sh.group[gu]];
+        const int64_t at = ((int64_t)e * a.F + ft * 8 + g) * a.d * G::kBytes + c * 32;
+        p0 = a.w1 + at;
+        p1 = a.w3 + at;
+        if (FP8) {
+          const int64_t sat = ((int64_t)e * fblocks + ft * 8 / kFp8Block) * kblocks;
+          q0 = a.s1 + sat;
+          q1 = a.s3 + sat;
+        }
+      }
+    };
+    auto load = [&](uint32_t (&x0)[8], uint32_t (&x1)[8], float& y0, float& y1) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x0[i] = x1[i] = 0u;
+      if (p0) {
+        if (ls * G::kStep + c * G::kPer < a.d) {
+          ld_global_nc_v8(p0 + (int64_t)ls * 128, x0);
+          ld_global_nc_v8(p1 + (int64_t)ls * 128, x1);
+        }
+        if (FP8) {
+          y0 = __ldg(q0 + ls);
+          y1 = __ldg(q1 + ls);
+        }
+      }
+      ls += wpt;
+      if (ls >= steps) {
+        ls = wi;
+        ++lp;
+        aim();
+      }
+    };
+    aim();
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) load(w0[i], w1[i], f0[i], f1[i]);
+
+    float acc[NT][4];
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
+    int pass = 0, s = wi, buf = 0;
+    while (pass < my_passes) {
+#pragma unroll
+      for (int b = 0; b < kAhead; ++b) {
+        if (pass >= my_passes) break;
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+          float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          const int t = i * 8 + g;
+#pragma unroll
+          for (int p = 0; p < G::kPieces; ++p) {
+            uint4 v = make_uint4(0u, 0u, 0u, 0u);
+            if (t < n) v = *reinterpret_cast<const uint4*>(smem + lay.x + ((uint32_t)(s * G::kPieces + p) * n + t) * 64 + c * 16);
+            mma_piece<FP8, M>(part, w0[b], w1[b], p, v);
+          }
+          if (FP8) {
+            acc[i][0] = fmaf(part[0], f0[b], acc[i][0]);
+            acc[i][1] = fmaf(part[1], f0[b], acc[i][1]);
+            acc[i][2] = fmaf(part[2], f1[b], acc[i][2]);
+            acc[i][3] = fmaf(part[3], f1[b], acc[i][3]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[i][j] += part[j];
+          }
+        }
+        load(w0[b], w1[b], f0[b], f1[b]);
+        s += wpt;
+        if (s < steps) continue;
+        // the tile's end: join the warps' sums
+        s = wi;
+        float* mine = red + buf * kRedBuf + warp * kRedWarp;
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+          *reinterpret_cast<float2*>(mine + g * kRedRow + i * 8 + c * 2) = make_float2(acc[i][0], acc[i][1]);
+          *reinterpret_cast<float2*>(mine + (g + 8) * kRedRow + i * 8 + c * 2) = make_float2(acc[i][2], acc[i][3]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
+        }
+        __syncthreads();   // the other buffer's readers are behind the next one
+        for (int i = tid; i < tpp * n * 8; i += kThreads) {
+          const int f = i & 7, t = (i >> 3) % n, ti = (i >> 3) / n;
+          const int tile = ((int)blockIdx.x + pass * (int)gridDim.x) * tpp + ti;
+          if (tile >= tiles) continue;
+          const int gu = tile / ftiles, ft = tile - gu * ftiles;
+          const int u = sh.group[gu], e = sh.list[u];
+          if (!((sh.used_tokens[e] >> (t0 + t)) & 1u)) continue;
+          const float* r = red + buf * kRedBuf + ti * wpt * kRedWarp + f * kRedRow + t;
+          float gate = 0.0f, up = 0.0f;
+          for (int w = 0; w < wpt; ++w) {
+            gate += r[w * kRedWarp];
+            up += r[w * kRedWarp + 8 * kRedRow];
+          }
+          gate *= sh.unscale[t];
+          up *= sh.unscale[t];
+          a.h[((int64_t)u * a.T + t0 + t) * a.F + ft * 8 + f] =
+              gate / (1.0f + expf(-gate)) * up * share[e * a.T + t0 + t];
+        }
+        buf ^= 1;
+        ++pass;
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// second kernel
+// ---------------------------------------------------------------------------------------
+template <bool FP8>
+constexpr uint32_t stage_bytes(int tokens) {   // hidden values of a chunk, both halves
+  return (uint32_t)kChunk * Geo<FP8>::kStep * tokens * 2 * 2;
+}
+
+template <bool FP8, typename X, int NT>
+__global__ void __launch_bounds__(kThreads, 1) down_kernel(const FewArgs a) {
+  using G = Geo<FP8>;
+  using M = typename std::conditional<FP8, __half, X>::type;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ int expert[kMaxUsed];
+  __shared__ uint32_t tokens[kMaxUsed];
+  __shared__ uint32_t top[2][kMaxTokens];
+  __shared__ int last;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
+  const int T = a.T;
+  const int used = a.head->used;
+  for (int i = tid; i < used; i += kThreads) {
+    expert[i] = a.head->expert[i];
+    tokens[i] = a.head->tokens[i];
+  }
+  if (tid < 2 * kMaxTokens) top[tid / kMaxTokens][tid % kMaxTokens] = 0u;
+  __syncthreads();
+  const int fsteps = (a.F + G::kStep - 1) / G::kStep;
+  const int total = used * fsteps;
+  const int slices = a.split < total ? a.split : total;
+  const int rb = blockIdx.x / a.split, slice = blockIdx.x % a.split;
+  if (slice >= slices) return;
+  const int begin = (int)((int64_t)total * slice / slices), end = (int)((int64_t)total * (slice + 1) / slices);
+  const int row0 = rb * kRowBlock + warp * 16;
+  const bool rows_ok = row0 < a.d;   // d is a multiple of 16
+  const int fblocks = (a.F + kFp8Block - 1) / kFp8Block, dblocks = (a.d + kFp8Block - 1) / kFp8Block;
+
+  // weights: the same pipeline as in the first kernel
+  uint32_t w0[kAhead][8], w1[kAhead][8];
+  float f[kAhead];
+  int ls = begin, lu = begin / fsteps, lk = begin - lu * fsteps;
+  const uint8_t* p0 = nullptr;
+  const float* q0 = nullptr;
+  const int64_t pitch = (int64_t)a.F * G::kBytes;
+  auto aim = [&]() {
+    if (ls >= end) return;
+    const int e = expert[lu];
+    p0 = a.w2 + ((int64_t)e * a.d + row0 + g) * pitch + c * 32;
+    if (FP8) q0 = a.s2 + ((int64_t)e * dblocks + row0 / kFp8Block) * fblocks;
+  };
+  auto load = [&](uint32_t (&x0)[8], uint32_t (&x1)[8], float& y) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x0[i] = x1[i] = 0u;
+    if (ls >= end || !rows_ok) return;
+    if (lk * G::kStep + c * G::kPer < a.F) {
+      ld_global_nc_v8(p0 + (int64_t)lk * 128, x0);
+      ld_global_nc_v8(p0 + 8 * pitch + (int64_t)lk * 128, x1);
+    }
+    if (FP8) y = __ldg(q0 + lk);
+    ++ls;
+    if (++lk == fsteps) {
+      lk = 0;
+      ++lu;
+      aim();
+    }
+  };
+  aim();
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) load(w0[i], w1[i], f[i]);
+
+  float acc[NT][4], part_acc[NT][4];
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
+
+  constexpr int kUnits = kChunk * G::kStep / 8;   // 16-byte pieces of a token
+  const uint32_t half_bytes = (uint32_t)kUnits * T * 16;
+  int buf = 0;
+  for (int at = begin; at < end; at += kChunk, buf ^= 1) {
+    const int n = end - at < kChunk ? end - at : kChunk;
+    // ---- stage the chunk's hidden values, as two 16-bit numbers of [2^14, 2^15) at most
+    constexpr int kMine = (NT * 8 * kUnits + kThreads - 1) / kThreads;   // pieces of a thread at most
+    float v[kMine][8];
+#pragma unroll
+    for (int m = 0; m < kMine; ++m) {
+      const int i = tid + m * kThreads;
+      const int t = i / kUnits, q = i - t * kUnits, st = q / (G::kStep / 8);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[m][j] = 0.0f;
+      if (t < T && st < n) {
+        const int u = (at + st) / fsteps, kk = (at + st - u * fsteps) * G::kStep + (q % (G::kStep / 8)) * 8;
+        if (((tokens[u] >> t) & 1u) && kk < a.F) {
+          const float4* src = reinterpret_cast<const float4*>(a.h + ((int64_t)u * T + t) * a.F + kk);
+          const float4 lo = __ldg(src), hi = __ldg(src + 1);
+          v[m][0] = lo.x; v[m][1] = lo.y; v[m][2] = lo.z; v[m][3] = lo.w;
+          v[m][4] = hi.x; v[m][5] = hi.y; v[m][6] = hi.z; v[m][7] = hi.w;
+        }
+      }
+      if (t < T) {
+        uint32_t mx = 0u;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const uint32_t b = __float_as_uint(v[m][j]) & 0x7fffffffu;
+          mx = max(mx, b < 0x7f800000u ? b : 0u);
+        }
+        if (mx) atomicMax(&top[buf][t], mx);
+      }
+    }
+    __syncthreads();
+    if (tid < kMaxTokens) top[buf ^ 1][tid] = 0u;   // read before this barrier, written behind the next
+    uint8_t* stage = smem + buf * 2 * half_bytes;
+#pragma unroll
+    for (int m = 0; m < kMine; ++m) {
+      const int i = tid + m * kThreads;
+      const int t = i / kUnits, q = i - t * kUnits;
+      if (t >= T) continue;
+      const float sc = pow2(range_exponent(top[buf][t]));
+      uint32_t hi[4], lo[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float x = v[m][2 * j] * sc, y = v[m][2 * j + 1] * sc;
+        hi[j] = narrow2<M>(x, y);
+        const float2 r = widen2<M>(hi[j]);
+        // (of an infinity or NaN there is no rest)
+        lo[j] = narrow2<M>(fabsf(r.x) < kInf ? x - r.x : 0.0f, fabsf(r.y) < kInf ? y - r.y : 0.0f);
+      }
+      const uint32_t off = piece_offset<FP8>(q, t, T);
+      *reinterpret_cast<uint4*>(stage + off) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+      *reinterpret_cast<uint4*>(stage + half_bytes + off) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    }
+    __syncthreads();
+    float un[NT][2];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int t = i * 8 + c * 2 + j;
+        un[i][j] = t < T ? pow2(-range_exponent(top[buf][t])) : 0.0f;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) part_acc[i][j] = 0.0f;
+    }
+    // ---- multiply
+    for (int s0 = 0; s0 < n; s0 += kAhead) {
+#pragma unroll
+      for (int b = 0; b < kAhead; ++b) {
+        const int s = s0 + b;
+        if (s >= n) break;
+        const uint32_t mask = tokens[(at + s) / fsteps];
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+          float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          const int t = i * 8 + g;
+          const bool has = (mask >> t) & 1u;
+#pragma unroll
+          for (int p = 0; p < G::kPieces; ++p) {
+            uint4 hi = make_uint4(0u, 0u, 0u, 0u), lo = hi;
+            if (has) {
+              const uint8_t* src = stage + ((uint32_t)(s * G::kPieces + p) * T + t) * 64 + c * 16;
+              hi = *reinterpret_cast<const uint4*>(src);
+              lo = *reinterpret_cast<const uint4*>(src + half_bytes);
+            }
+            mma_piece<FP8, M>(part, w0[b], w1[b], p, hi);
+            mma_piece<FP8, M>(part, w0[b], w1[b], p, lo);
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) part_acc[i][j] = FP8 ? fmaf(part[j], f[b], part_acc[i][j]) : part_acc[i][j] + part[j];
+        }
+        load(w0[b], w1[b], f[b]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(part_acc[i][j], un[i][j & 1], acc[i][j]);
+  }
+
+  // ---- the slices' sum
+  auto put = [&](int t, int row, float v) {
+    if constexpr (std::is_same<X, __half>::value)
+      static_cast<__half*>(a.y)[(int64_t)t * a.d + row] = __float2half_rn(v);
+    else
+      static_cast<__nv_bfloat16*>(a.y)[(int64_t)t * a.d + row] = __float2bfloat16_rn(v);
+  };
+  if (rows_ok) {
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int t = i * 8 + c * 2 + (j & 1), row = row0 + g + (j >> 1) * 8;
+        if (t >= T) continue;
+        if (slices == 1)
+          put(t, row, acc[i][j]);
+        else
+          a.part[((int64_t)slice * T + t) * a.d + row] = acc[i][j];
+      }
+  }
+  if (slices == 1) return;
+  __threadfence();
+  __syncthreads();
+  if (tid == 0) last = atomicAdd(&a.counters[rb], 1u) == (uint32_t)slices - 1u;
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  for (int i = tid; i < T * kRowBlock; i += kThreads) {
+    const int t = i / kRowBlock, row = rb * kRowBlock + i % kRowBlock;
+    if (row >= a.d) continue;
+    float v = 0.0f;
+    for (int s = 0; s < slices; ++s) v += __ldcg(a.part + ((int64_t)s * T + t) * a.d + row);
+    put(t, row, v);
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+struct FewWorkspace {
+  size_t head, counters, h, part, total;
+};
+FewWorkspace few_workspace(int T, int d, int F, int E, int k, int S) {
+  auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+  const int used = (E < T * k ? E : T * k) + S;
+  const int blocks = (d + kRowBlock - 1) / kRowBlock;
+  const int split = kSplitCtas / blocks > 1 ? kSplitCtas / blocks : 1;
+  FewWorkspace w;
+  w.head = 0;
+  w.counters = up(sizeof(Header));
+  w.h = w.counters + up((size_t)blocks * 4);
+  w.part = w.h + up((size_t)used * T * F * 4);
+  w.total = w.part + up((size_t)split * T * d * 4);
+  return w;
+}
+
+template <bool FP8, typename X, int NT>
+int launch(const FewArgs& a, int grid1, int grid2, uint32_t smem1, cudaStream_t stream) {
+  auto k1 = gate_up_kernel<FP8, X, NT>;
+  const int nt2 = a.T > 8 ? 2 : 1;
+  auto k2 = nt2 == 1 ? down_kernel<FP8, X, 1> : down_kernel<FP8, X, 2>;
+  const uint32_t smem2 = 2 * stage_bytes<FP8>(a.T);
+  int st = set_max_dynamic_smem(reinterpret_cast<const void*>(k1), smem1);
+  if (st != LMOE_OK) return st;
+  st = set_max_dynamic_smem(reinterpret_cast<const void*>(k2), smem2);
+  if (st != LMOE_OK) return st;
+  k1<<<grid1, kThreads, smem1, stream>>>(a);
+  LMOE_CUDA_TRY(cudaGetLastError());
+  k2<<<grid2, kThreads, smem2, stream>>>(a);
+  return cuda_status(cudaGetLastError());
+}
+
+bool few_sizes(int64_t T, int d, int F, int E, int k, int S) {
+  return T >= 0 && T <= kMaxTokens && d >= 64 && d % 64 == 0 && d <= 16384 && F >= 32 && F % 32 == 0 && F <= 65536 &&
+         E >= 1 && E <= kMaxExperts && k >= 1 && k <= kMaxTopK && k <= E && S >= 0 && S <= kMaxShared;
+}
+
+}  // namespace
+}  // namespace lmoe
+
+using namespace lmoe;
+
+extern "C" size_t lmoe_few_tokens_workspace_bytes(int64_t num_tokens, int hidden_size, int ffn_size, int num_experts,
+                                                  int top_k, int num_shared) {
+  if (!few_sizes(num_tokens, hidden_size, ffn_size, num_experts, top_k, num_shared)) return 0;
+  return few_workspace((int)num_tokens, hidden_size, ffn_size, num_experts, top_k, num_shared).total;
+}
+
+extern "C" int lmoe_moe_layer_few_tokens(const void* x, int dtype, int64_t num_tokens, int hidden_size,
+                                         const void* gate_weight, const float* gate_bias, int num_experts, int top_k,
+                                         int num_shared, const void* w1, const void* w3, const void* w2,
+                                         const float* w1_scales, const float* w3_scales, const float* w2_scales,
+                                         int ffn_size, void* y, int32_t* ids, float* weights, void* workspace,
+                                         size_t workspace_bytes, lmoe_stream_t stream_) {
+  cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
+  LMOE_ARG_CHECK(dtype == LMOE_DTYPE_BF16 || dtype == LMOE_DTYPE_F16);
+  LMOE_ARG_CHECK(few_sizes(num_tokens, hidden_size, ffn_size, num_experts, top_k, num_shared));
+  const bool fp8 = w1_scales != nullptr;
+  LMOE_ARG_CHECK((w3_scales != nullptr) == fp8 && (w2_scales != nullptr) == fp8);
+  if (num_tokens == 0) return LMOE_OK;
+  LMOE_ARG_CHECK(x && gate_weight && w1 && w3 && w2 && y && ids && weights);
+  LMOE_ARG_CHECK(aligned16(x) && aligned16(gate_weight) && aligned32(w1) && aligned32(w3) && aligned32(w2));
+  LMOE_ARG_CHECK(((reinterpret_cast<uintptr_t>(gate_bias) | reinterpret_cast<uintptr_t>(w1_scales) |
+                   reinterpret_cast<uintptr_t>(w3_scales) | reinterpret_cast<uintptr_t>(w2_scales) |
+                   reinterpret_cast<uintptr_t>(ids) | reinterpret_cast<uintptr_t>(weights)) & 3) == 0);
+  LMOE_ARG_CHECK((reinterpret_cast<uintptr_t>(y) & 1) == 0);
+  const int T = (int)num_tokens;
+  const FewWorkspace ws = few_workspace(T, hidden_size, ffn_size, num_experts, top_k, num_shared);
+  if (!workspace || workspace_bytes < ws.total || !aligned16(workspace)) return LMOE_ERR_WORKSPACE;
+  DeviceInfo dev;
+  int st = get_device_info(&dev);
+  if (st != LMOE_OK) return st;
+  if (dev.cc_major != 10) return LMOE_ERR_DEVICE;
+  FewArgs a = {};
+  a.x = x;
+  a.gate = gate_weight;
+  a.bias = gate_bias;
+  a.w1 = static_cast<const uint8_t*>(w1);
+  a.w3 = static_cast<const uint8_t*>(w3);
+  a.w2 = static_cast<const uint8_t*>(w2);
+  a.s1 = w1_scales;
+  a.s3 = w3_scales;
+  a.s2 = w2_scales;
+  a.T = T;
+  a.d = hidden_size;
+  a.F = ffn_size;
+  a.E = num_experts;
+  a.k = top_k;
+  a.S = num_shared;
+  a.y = y;
+  a.ids = ids;
+  a.weights = weights;
+  uint8_t* base = static_cast<uint8_t*>(workspace);
+  a.head = reinterpret_cast<Header*>(base + ws.head);
+  a.counters = reinterpret_cast<uint32_t*>(base + ws.counters);
+  a.h = reinterpret_cast<float*>(base + ws.h);
+  a.part = reinterpret_cast<float*>(base + ws.part);
+  // All tokens of a large layer may not fit shared memory: then eight at a time, each group reading
+  // its experts' gate and up weights.
+  const uint32_t limit = (uint32_t)dev.max_smem_optin - (uint32_t)sizeof(FewShared) - 1024;
+  const int step = fp8 ? 128 : 64;
+  a.groups = 1;
+  uint32_t smem1 = few_layout(a.d, step, T, T, a.E, a.S).total;
+  if (smem1 > limit) {
+    a.groups = (T + 7) / 8;
+    smem1 = few_layout(a.d, step, 8, T, a.E, a.S).total;
+    if (smem1 > limit || a.groups < 2) return LMOE_ERR_UNSUPPORTED;
+  }
+  const int blocks = (a.d + kRowBlock - 1) / kRowBlock;
+  a.split = kSplitCtas / blocks > 1 ? kSplitCtas / blocks : 1;
+  const int grid1 = gemm_grid(dev), grid2 = blocks * a.split;
+  const bool two = T > 8 && a.groups == 1;
+  if (dtype == LMOE_DTYPE_BF16) {
+    if (fp8)
+      return two ? launch<true, __nv_bfloat16, 2>(a, grid1, grid2, smem1, stream)
+                 : launch<true, __nv_bfloat16, 1>(a, grid1, grid2, smem1, stream);
+    return two ? launch<false, __nv_bfloat16, 2>(a, grid1, grid2, smem1, stream)
+               : launch<false, __nv_bfloat16, 1>(a, grid1, grid2, smem1, stream);
+  }
+  if (fp8)
+    return two ? launch<true, __half, 2>(a, grid1, grid2, smem1, stream)
+               : launch<true, __half, 1>(a, grid1, grid2, smem1, stream);
+  return two ? launch<false, __half, 2>(a, grid1, grid2, smem1, stream)
+             : launch<false, __half, 1>(a, grid1, grid2, smem1, stream);
+}

@@ -11,7 +11,8 @@ Same names, argument names and return types as the reference's ``light_moe._C``
 plus the new ops (``fused_gate_topk_ex``, ``quantize_w4``, ``dequantize_w4``, ``prepack_w4``,
 ``w4a16_grouped_gemm``, ``moe_layer_w4a16``; the gradients ``grouped_gemm_dgrad`` and
 ``grouped_gemm_wgrad``; the 4-bit floating point ``quantize_fp4``, ``dequantize_fp4`` and
-``fp4_grouped_gemm``; the 8-bit ``quantize_fp8``, ``dequantize_fp8`` and ``fp8_grouped_gemm``).  Every op runs the CUDA library; if the
+``fp4_grouped_gemm``; the 8-bit ``quantize_fp8``, ``dequantize_fp8`` and ``fp8_grouped_gemm``;
+``moe_layer_few_tokens``).  Every op runs the CUDA library; if the
 ``_C`` extension has not been built, calling any op raises -- there is no fallback path.
 """
 from __future__ import annotations
@@ -175,3 +176,16 @@ def moe_layer_w4a16(x, gate_weight, w13_packed, w2_packed, top_k, ffn_size, grou
     """[y bf16 [T, d], ids int32 [T, k], weights fp32 [T, k]]."""
     return extension().moe_layer_w4a16(x, gate_weight, w13_packed, w2_packed, top_k, ffn_size, group_size,
                                        num_shared, gate_bias)
+
+
+def moe_layer_few_tokens(x, gate_weight, w1, w3, w2, top_k, w1_scales=None, w3_scales=None, w2_scales=None,
+                         num_shared=0, gate_bias=None):
+    """[y [T, d] in x's dtype, ids int32 [T, k], weights fp32 [T, k]]: the whole MoE layer (router, SwiGLU
+    experts, weighted sum) for at most 16 tokens, in two kernels.
+
+    x [T, d] and gate_weight [E, d] bf16 or fp16 (the same); w1, w3 [E + S, ffn, d] and w2 [E + S, d, ffn] of
+    that dtype, or float8_e4m3fn with the scales of ``quantize_fp8(w, block_rows=128)``; the last
+    ``num_shared`` experts take every token with weight 1; gate_bias fp32 [E].  The activations are not
+    quantised.  d % 64 == 0, ffn % 32 == 0."""
+    return extension().moe_layer_few_tokens(x, gate_weight, w1, w3, w2, top_k, w1_scales, w3_scales, w2_scales,
+                                            num_shared, gate_bias)

@@ -85,6 +85,35 @@ def test_gemm_refuses_too_many_experts():
     assert _gemm(E=257) == UNSUPPORTED
 
 
+def _few(x=P, dtype=0, T=4, d=128, gw=P, gb=None, E=4, k=2, S=0, w1=P, w3=P, w2=P, s1=None, s3=None, s2=None, F=64,
+         y=P, ids=P, wts=P, ws=P, wsb=1 << 30):
+    return capi.lib().lmoe_moe_layer_few_tokens(x, dtype, T, d, gw, gb, E, k, S, w1, w3, w2, s1, s3, s2, F, y, ids, wts,
+                                                ws, wsb, None)
+
+
+@pytest.mark.parametrize("bad", [
+    dict(dtype=2), dict(dtype=-1), dict(T=17), dict(T=-1), dict(d=32), dict(d=96), dict(d=16448), dict(F=48), dict(F=0),
+    dict(F=65568), dict(E=0), dict(E=257), dict(k=0), dict(k=5), dict(E=20, k=17), dict(S=-1), dict(S=17),
+    dict(s1=P), dict(s3=P), dict(s1=P, s3=P), dict(x=None), dict(gw=None), dict(w1=None), dict(w3=None),
+    dict(w2=None), dict(y=None), dict(ids=None), dict(wts=None), dict(x=P + 8), dict(gw=P + 8), dict(w1=P + 16),
+    dict(w3=P + 16), dict(w2=P + 16), dict(gb=P + 2), dict(y=P + 1), dict(ids=P + 2), dict(wts=P + 2),
+    dict(s1=P + 1, s3=P, s2=P),
+])
+def test_few_tokens_refusals(bad):
+    assert _few(**bad) == INVALID
+
+
+def test_few_tokens_workspace():
+    size = capi.lib().lmoe_few_tokens_workspace_bytes
+    for bad in ((17, 128, 64, 4, 2, 0), (-1, 128, 64, 4, 2, 0), (1, 100, 64, 4, 2, 0), (1, 128, 40, 4, 2, 0),
+                (1, 128, 64, 257, 2, 0), (1, 128, 64, 4, 5, 0), (1, 128, 64, 4, 2, 17)):
+        assert size(*bad) == 0
+    one = size(1, 128, 64, 4, 2, 0)
+    assert one > 0 and size(2, 128, 64, 4, 2, 0) > one
+    assert _few(ws=None) == _few(wsb=size(4, 128, 64, 4, 2, 0) - 1) == _few(ws=P + 8) == capi.LMOE_ERR_WORKSPACE
+    assert _few(T=0, ws=None) == OK
+
+
 def test_empty_calls_need_no_gpu():
     assert _rows(rows=0, out_rows=0, pitch=0) == OK
     assert _blocks(count=0) == OK and _blocks(rows=0) == OK
