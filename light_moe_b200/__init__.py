@@ -5,6 +5,7 @@
 * ``layer``  ``W4A16Experts`` and ``W4A16MoELayer`` (drop-in for ``SparseMoEBlock``)
 * ``expert_parallel``  the expert-parallel layer over NCCL
 * ``fp4``    ``FP4Experts`` and ``FP4MoELayer`` (mxfp4 / nvfp4 experts and activations)
+* ``fp8``    ``FP8Experts`` and ``FP8MoELayer`` (8-bit experts with block scales)
 * ``grouped``  ``grouped_linear``, ``GroupedLinear``, ``GroupedExperts`` (trainable grouped products)
 
 Build with ``python -m light_moe_b200.build``.  Nothing here falls back to a CPU or
