@@ -53,14 +53,17 @@ constexpr int kMaxUsed = kMaxExperts + kMaxShared;
 constexpr int kAhead = 3;        // steps of weights in flight per warp
 constexpr int kRowBlock = kWarps * 16;   // output rows of a CTA of the second kernel
 constexpr int kSplitCtas = 148;  // CTAs that the second kernel's slices aim at: one per SM
-constexpr int kChunk = 6;        // steps of hidden values staged at a time
-static_assert(kChunk % kAhead == 0, "a chunk starts at the first of the buffers in flight");
+constexpr int kMaxCtas = 256;    // of the first kernel
+constexpr int kJoins = 4;        // tiles whose parts may wait to be joined
+constexpr uint32_t kStageBytes = 96 * 1024;   // of each of two buffers of hidden values at most
+constexpr uint32_t kSite = 0x800u;
 constexpr float kInf = __builtin_huge_valf();
 
 // What the first kernel tells the second.
 struct Header {
+  uint32_t error;            // of the kernels' waits
   int used;                  // experts with tokens
-  int pad[3];
+  int pad[2];
   int expert[kMaxUsed];      // ascending, shared ones last
   uint32_t tokens[kMaxUsed]; // bit t: token t chose it
 };
@@ -78,11 +81,14 @@ struct FewArgs {
   int T, d, F, E, k, S;
   int groups;                // token groups of the first kernel
   int split;                 // slices of the second kernel
+  int grid1;                 // CTAs of the first
+  int chunk;                 // steps of hidden values that the second stages at a time
   void* y;
   int32_t* ids;
   float* weights;
   Header* head;
   uint32_t* counters;        // arrivals per row block
+  uint32_t* tops;            // [CTA of the first kernel][T]: fp32 bits of its largest hidden value
   float* h;                  // [used][T][F]
   float* part;               // [split][T][d]
 };
@@ -177,6 +183,10 @@ struct FewShared {
   int list[kMaxUsed];               // experts with tokens
   int group[kMaxUsed];              // positions in `list` that have tokens of the group
   int used, group_used;
+  uint64_t full[kJoins][kWarps];    // a tile's parts are written (its warps)
+  uint64_t empty[kJoins][kWarps];   // ... and joined
+  int abort;
+  uint32_t htop[kMaxTokens];        // largest hidden values
   uint32_t top[kMaxTokens];         // largest absolute value of the group's tokens
   float unscale[kMaxTokens];
   int chosen[kMaxTokens][kMaxTopK];
@@ -193,7 +203,7 @@ __host__ __device__ inline FewLayout few_layout(int d, int step, int group_token
   const uint32_t nt = group_tokens > 8 ? 2 : 1;
   l.x = 0;
   l.red = kpad * group_tokens * 2;
-  l.logits = l.red + 2 * kWarps * 16 * 8 * nt * 4;
+  l.logits = l.red + kJoins * kWarps * 16 * 8 * nt * 4;
   l.share = l.logits + (uint32_t)(T * E + 3) / 4 * 16;
   l.total = l.share + (uint32_t)((E + S) * T + 3) / 4 * 16;
   return l;
@@ -215,6 +225,9 @@ __global__ void __launch_bounds__(kThreads, 1) gate_up_kernel(const FewArgs a) {
   float* share = reinterpret_cast<float*>(smem + lay.share);     // [E + S][T]: routing weights
   constexpr int kRedRow = 8 * NT, kRedWarp = 16 * kRedRow, kRedBuf = kWarps * kRedWarp;
   const int experts = a.E + a.S;
+  if (tid < kMaxTokens) sh.htop[tid] = 0u;
+  if (tid == 0) sh.abort = 0;
+  if (tid == 0 && blockIdx.x == 0) a.head->error = 0u;
 
   // tokens t0 .. t0 + n - 1 into shared memory, in the order of the fragments
   auto load_x = [&](int t0, int n) {
@@ -389,11 +402,30 @@ __global__ void __launch_bounds__(kThreads, 1) gate_up_kernel(const FewArgs a) {
   }
 
   // ---- the experts' gate and up products
-  int wpt = kWarps;   // warps of a tile: a power of two, each with a step at least
-  while (wpt > steps) wpt >>= 1;
-  const int tpp = kWarps / wpt, wi = warp & (wpt - 1), wt = warp / wpt;   // tiles of a pass; this warp's share and tile
   const int ftiles = a.F / 8;
   const int kblocks = (a.d + kFp8Block - 1) / kFp8Block, fblocks = (a.F + kFp8Block - 1) / kFp8Block;
+  // Warps of a tile: a power of two, each with a step at least.  Many balance the last round, few have
+  // less to join (half a step's time a tile).  Reckoned for all SMs whatever the grid: the order of the
+  // sums, and so their last bits, do not depend on a limit of CTAs.
+  int wpt = 1;
+  for (int w = 1, best = INT32_MAX; w <= kWarps && w <= steps; w <<= 1) {
+    const int groups = kSplitCtas * (kWarps / w), rounds = (sh.used * ftiles + groups - 1) / groups;
+    const int cost = rounds * (2 * ((steps + w - 1) / w) + 1);
+    if (cost < best) {
+      best = cost;
+      wpt = w;
+    }
+  }
+  const int wi = warp & (wpt - 1), wt = warp / wpt;   // this warp's share of a tile, and its group of warps
+  const int stride = (int)gridDim.x * (kWarps / wpt);
+  if (tid < kJoins * kWarps) {
+    mbar_init(&sh.full[tid / kWarps][tid % kWarps], (uint32_t)wpt);
+    mbar_init(&sh.empty[tid / kWarps][tid % kWarps], 1);
+  }
+  fence_mbar_init();
+  int join = 0;   // the warps of a group count their tiles alike
+  uint32_t parity = 0, joined = 0;
+  float most[2 * NT] = {};
   for (int t0 = 0; t0 < a.T; t0 += per_group) {
     const int n = a.T - t0 < per_group ? a.T - t0 : per_group;
     if (a.groups > 1) load_x(t0, n);   // else they are there
@@ -412,48 +444,48 @@ __global__ void __launch_bounds__(kThreads, 1) gate_up_kernel(const FewArgs a) {
     }
     __syncthreads();
     const int tiles = sh.group_used * ftiles;
-    const int passes = (tiles + tpp - 1) / tpp;
-    const int my_passes = passes > (int)blockIdx.x ? (passes - 1 - (int)blockIdx.x) / (int)gridDim.x + 1 : 0;
 
     uint32_t w0[kAhead][8], w1[kAhead][8];
     float f0[kAhead], f1[kAhead];
-    // the next load: pass and step, and the tile's rows
-    int lp = 0, ls = wi;
+    const int first = (int)blockIdx.x * (kWarps / wpt) + wt;
+    // the next load: tile and step
+    int lt = first, ls = wi;
     const uint8_t *p0 = nullptr, *p1 = nullptr;
     const float *q0 = nullptr, *q1 = nullptr;
     auto aim = [&]() {
-      const int tile = ((int)blockIdx.x + lp * (int)gridDim.x) * tpp + wt;
-      p0 = nullptr;
-      if (lp < my_passes && tile < tiles) {
-        const int gu = tile / ftiles, ft = tile - gu * ftiles;
-        const int e = sh.list[sh.group[gu]];
-        const int64_t at = ((int64_t)e * a.F + ft * 8 + g) * a.d * G::kBytes + c * 32;
-        p0 = a.w1 + at;
-        p1 = a.w3 + at;
-        if (FP8) {
-          const int64_t sat = ((int64_t)e * fblocks + ft * 8 / kFp8Block) * kblocks;
-          q0 = a.s1 + sat;
-          q1 = a.s3 + sat;
-        }
+      if (lt >= tiles) return;
+      const int gu = lt / ftiles, ft = lt - gu * ftiles;
+      const int e = sh.list[sh.group[gu]];
+      const int64_t at = ((int64_t)e * a.F + ft * 8 + g) * a.d * G::kBytes + c * 32 + ls * 128;
+      p0 = a.w1 + at;
+      p1 = a.w3 + at;
+      if (FP8) {
+        const int64_t sat = ((int64_t)e * fblocks + ft * 8 / kFp8Block) * kblocks + ls;
+        q0 = a.s1 + sat;
+        q1 = a.s3 + sat;
       }
     };
     auto load = [&](uint32_t (&x0)[8], uint32_t (&x1)[8], float& y0, float& y1) {
+      if (lt >= tiles) return;
+      if (ls * G::kStep + c * G::kPer < a.d) {
+        ld_global_nc_v8(p0, x0);
+        ld_global_nc_v8(p1, x1);
+      } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x0[i] = x1[i] = 0u;
-      if (p0) {
-        if (ls * G::kStep + c * G::kPer < a.d) {
-          ld_global_nc_v8(p0 + (int64_t)ls * 128, x0);
-          ld_global_nc_v8(p1 + (int64_t)ls * 128, x1);
-        }
-        if (FP8) {
-          y0 = __ldg(q0 + ls);
-          y1 = __ldg(q1 + ls);
-        }
+        for (int i = 0; i < 8; ++i) x0[i] = x1[i] = 0u;
       }
+      if (FP8) {
+        y0 = __ldg(q0);
+        y1 = __ldg(q1);
+        q0 += wpt;
+        q1 += wpt;
+      }
+      p0 += wpt * 128;
+      p1 += wpt * 128;
       ls += wpt;
       if (ls >= steps) {
         ls = wi;
-        ++lp;
+        lt += stride;
         aim();
       }
     };
@@ -466,96 +498,135 @@ __global__ void __launch_bounds__(kThreads, 1) gate_up_kernel(const FewArgs a) {
     for (int i = 0; i < NT; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
-    int pass = 0, s = wi, buf = 0;
-    while (pass < my_passes) {
+    // this lane's place in the tokens' fragments
+    const uint32_t step_bytes = (uint32_t)G::kPieces * n * 64;
+    const uint8_t* xl = smem + lay.x + g * 64 + c * 16;
+    int s = wi;
+    bool ok = true;
+    for (int tile = first; tile < tiles && ok;) {
 #pragma unroll
       for (int b = 0; b < kAhead; ++b) {
-        if (pass >= my_passes) break;
+        if (tile >= tiles || !ok) break;
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
-          float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-          const int t = i * 8 + g;
+          // two chains of dependent products
+          float part[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+          const bool has = i * 8 + g < n;
+          const uint8_t* src = xl + s * step_bytes + i * 512;
 #pragma unroll
           for (int p = 0; p < G::kPieces; ++p) {
             uint4 v = make_uint4(0u, 0u, 0u, 0u);
-            if (t < n) v = *reinterpret_cast<const uint4*>(smem + lay.x + ((uint32_t)(s * G::kPieces + p) * n + t) * 64 + c * 16);
-            mma_piece<FP8, M>(part, w0[b], w1[b], p, v);
+            if (has) v = *reinterpret_cast<const uint4*>(src + p * n * 64);
+            mma_piece<FP8, M>(part[p & 1], w0[b], w1[b], p, v);
           }
           if (FP8) {
-            acc[i][0] = fmaf(part[0], f0[b], acc[i][0]);
-            acc[i][1] = fmaf(part[1], f0[b], acc[i][1]);
-            acc[i][2] = fmaf(part[2], f1[b], acc[i][2]);
-            acc[i][3] = fmaf(part[3], f1[b], acc[i][3]);
+            acc[i][0] = fmaf(part[0][0] + part[1][0], f0[b], acc[i][0]);
+            acc[i][1] = fmaf(part[0][1] + part[1][1], f0[b], acc[i][1]);
+            acc[i][2] = fmaf(part[0][2] + part[1][2], f1[b], acc[i][2]);
+            acc[i][3] = fmaf(part[0][3] + part[1][3], f1[b], acc[i][3]);
           } else {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) acc[i][j] += part[j];
+            for (int j = 0; j < 4; ++j) acc[i][j] += part[0][j] + part[1][j];
           }
         }
         load(w0[b], w1[b], f0[b], f1[b]);
         s += wpt;
         if (s < steps) continue;
-        // the tile's end: join the warps' sums
+        // the tile's end: this warp's part
         s = wi;
-        float* mine = red + buf * kRedBuf + warp * kRedWarp;
+        uint64_t *full = &sh.full[join][wt], *empty = &sh.empty[join][wt];
+        ok = mbar_wait(empty, parity ^ 1u, &a.head->error, &sh.abort, kSite + 1);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        float* parts = red + join * kRedBuf + wt * wpt * kRedWarp;
+        float* mine = parts + wi * kRedWarp;
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
-          *reinterpret_cast<float2*>(mine + g * kRedRow + i * 8 + c * 2) = make_float2(acc[i][0], acc[i][1]);
-          *reinterpret_cast<float2*>(mine + (g + 8) * kRedRow + i * 8 + c * 2) = make_float2(acc[i][2], acc[i][3]);
+          if (i * 8 + c * 2 < n) {
+            *reinterpret_cast<float2*>(mine + g * kRedRow + i * 8 + c * 2) = make_float2(acc[i][0], acc[i][1]);
+            *reinterpret_cast<float2*>(mine + (g + 8) * kRedRow + i * 8 + c * 2) = make_float2(acc[i][2], acc[i][3]);
+          }
 #pragma unroll
           for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
         }
-        __syncthreads();   // the other buffer's readers are behind the next one
-        for (int i = tid; i < tpp * n * 8; i += kThreads) {
-          const int f = i & 7, t = (i >> 3) % n, ti = (i >> 3) / n;
-          const int tile = ((int)blockIdx.x + pass * (int)gridDim.x) * tpp + ti;
-          if (tile >= tiles) continue;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(full);
+        // ... and one of its warps, another each time, joins the parts
+        if ((joined & (uint32_t)(wpt - 1)) == (uint32_t)wi) {
+          ok = mbar_wait(full, parity, &a.head->error, &sh.abort, kSite + 2);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
           const int gu = tile / ftiles, ft = tile - gu * ftiles;
           const int u = sh.group[gu], e = sh.list[u];
-          if (!((sh.used_tokens[e] >> (t0 + t)) & 1u)) continue;
-          const float* r = red + buf * kRedBuf + ti * wpt * kRedWarp + f * kRedRow + t;
-          float gate = 0.0f, up = 0.0f;
-          for (int w = 0; w < wpt; ++w) {
-            gate += r[w * kRedWarp];
-            up += r[w * kRedWarp + 8 * kRedRow];
+          const uint32_t chosen = sh.used_tokens[e] >> t0;
+          const int f = lane & 7;
+#pragma unroll
+          for (int i = 0; i < 2 * NT; ++i) {
+            const int t = (lane >> 3) + 4 * i;
+            if (t < n && ((chosen >> t) & 1u)) {
+              const float* r = parts + f * kRedRow + t;
+              float gate = 0.0f, up = 0.0f;
+#pragma unroll 4
+              for (int w = 0; w < wpt; ++w) {
+                gate += r[w * kRedWarp];
+                up += r[w * kRedWarp + 8 * kRedRow];
+              }
+              gate *= sh.unscale[t];
+              up *= sh.unscale[t];
+              const float h = gate / (1.0f + expf(-gate)) * up * share[e * a.T + t0 + t];
+              a.h[((int64_t)u * a.T + t0 + t) * a.F + ft * 8 + f] = h;
+              if (fabsf(h) < kInf) most[i] = fmaxf(most[i], fabsf(h));
+            }
           }
-          gate *= sh.unscale[t];
-          up *= sh.unscale[t];
-          a.h[((int64_t)u * a.T + t0 + t) * a.F + ft * 8 + f] =
-              gate / (1.0f + expf(-gate)) * up * share[e * a.T + t0 + t];
+          __syncwarp();
+          if (lane == 0) mbar_arrive(empty);
         }
-        buf ^= 1;
-        ++pass;
+        ++joined;
+        if (++join == kJoins) {
+          join = 0;
+          parity ^= 1u;
+        }
+        tile += stride;
       }
+    }
+#pragma unroll
+    for (int i = 0; i < 2 * NT; ++i) {
+      const int t = (lane >> 3) + 4 * i;
+      if (t < n && most[i] > 0.0f) atomicMax(&sh.htop[t0 + t], __float_as_uint(most[i]));
+      most[i] = 0.0f;
     }
     __syncthreads();
   }
+  if (tid < a.T) a.tops[(int64_t)blockIdx.x * a.T + tid] = sh.htop[tid];
 }
 
 // ---------------------------------------------------------------------------------------
 // second kernel
 // ---------------------------------------------------------------------------------------
-template <bool FP8>
-constexpr uint32_t stage_bytes(int tokens) {   // hidden values of a chunk, both halves
-  return (uint32_t)kChunk * Geo<FP8>::kStep * tokens * 2 * 2;
-}
-
-template <bool FP8, typename X, int NT>
+// MODE 0: up to 4 tokens, whose two halves are columns t and t + 4 of one MMA; 1: up to 8; 2: up to 16.
+template <bool FP8, typename X, int MODE>
 __global__ void __launch_bounds__(kThreads, 1) down_kernel(const FewArgs a) {
   using G = Geo<FP8>;
   using M = typename std::conditional<FP8, __half, X>::type;
+  constexpr int NT = MODE == 2 ? 2 : 1;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int expert[kMaxUsed];
   __shared__ uint32_t tokens[kMaxUsed];
-  __shared__ uint32_t top[2][kMaxTokens];
+  __shared__ uint32_t top[kMaxTokens];
   __shared__ int last;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   const int T = a.T;
+  if (tid < kMaxTokens) top[tid] = 0u;
+  __syncthreads();
   const int used = a.head->used;
   for (int i = tid; i < used; i += kThreads) {
     expert[i] = a.head->expert[i];
     tokens[i] = a.head->tokens[i];
   }
-  if (tid < 2 * kMaxTokens) top[tid / kMaxTokens][tid % kMaxTokens] = 0u;
+  for (int i = tid; i < a.grid1 * T; i += kThreads) {
+    const uint32_t v = a.tops[i];
+    if (v) atomicMax(&top[i % T], v);
+  }
   __syncthreads();
   const int fsteps = (a.F + G::kStep - 1) / G::kStep;
   const int total = used * fsteps;
@@ -577,18 +648,20 @@ __global__ void __launch_bounds__(kThreads, 1) down_kernel(const FewArgs a) {
   auto aim = [&]() {
     if (ls >= end) return;
     const int e = expert[lu];
-    p0 = a.w2 + ((int64_t)e * a.d + row0 + g) * pitch + c * 32;
-    if (FP8) q0 = a.s2 + ((int64_t)e * dblocks + row0 / kFp8Block) * fblocks;
+    p0 = a.w2 + ((int64_t)e * a.d + row0 + g) * pitch + c * 32 + lk * 128;
+    if (FP8) q0 = a.s2 + ((int64_t)e * dblocks + row0 / kFp8Block) * fblocks + lk;
   };
   auto load = [&](uint32_t (&x0)[8], uint32_t (&x1)[8], float& y) {
+    if (ls >= end) return;
+    if (rows_ok && lk * G::kStep + c * G::kPer < a.F) {
+      ld_global_nc_v8(p0, x0);
+      ld_global_nc_v8(p0 + 8 * pitch, x1);
+    } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x0[i] = x1[i] = 0u;
-    if (ls >= end || !rows_ok) return;
-    if (lk * G::kStep + c * G::kPer < a.F) {
-      ld_global_nc_v8(p0 + (int64_t)lk * 128, x0);
-      ld_global_nc_v8(p0 + 8 * pitch + (int64_t)lk * 128, x1);
+      for (int i = 0; i < 8; ++i) x0[i] = x1[i] = 0u;
     }
-    if (FP8) y = __ldg(q0 + lk);
+    if (FP8) y = rows_ok ? __ldg(q0++) : 0.0f;
+    p0 += 128;
     ++ls;
     if (++lk == fsteps) {
       lk = 0;
@@ -600,113 +673,128 @@ __global__ void __launch_bounds__(kThreads, 1) down_kernel(const FewArgs a) {
 #pragma unroll
   for (int i = 0; i < kAhead; ++i) load(w0[i], w1[i], f[i]);
 
-  float acc[NT][4], part_acc[NT][4];
+  // Hidden values: of each step, a thread stages at most one piece of 8 values of a token, as two 16-bit
+  // numbers (of values scaled to at most 2^15).  The pieces of the next chunk's steps are loaded beside this
+  // chunk's products.
+  constexpr int kStepPieces = G::kStep / 8;
+  const int piece = lane * kWarps + warp;
+  const int st = piece / kStepPieces, sq = piece % kStepPieces;
+  const bool stager = st < T;
+  const float sc = stager ? pow2(range_exponent(top[st])) : 0.0f;
+  const uint32_t step_bytes = (uint32_t)G::kPieces * T * 64;    // of one half
+  const uint32_t half_bytes = step_bytes * a.chunk;
+  const uint32_t piece_at = ((uint32_t)(sq % G::kPieces) * T + st) * 64 + sq / G::kPieces * 16;
+  // Piece q of token t in a step of the contraction; zeros where there is none.
+  auto fetch = [&](int step, int t, int q, float4& v0, float4& v1) {
+    const int u = step / fsteps, kk = (step - u * fsteps) * G::kStep + q * 8;
+    v0 = v1 = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (((tokens[u] >> t) & 1u) && kk < a.F) {
+      const float4* src = reinterpret_cast<const float4*>(a.h + ((int64_t)u * T + t) * a.F + kk);
+      v0 = __ldcg(src);
+      v1 = __ldcg(src + 1);
+    }
+  };
+  auto put_piece = [&](uint8_t* dst, float scale, const float4& v0, const float4& v1) {
+    const float v[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
+    uint32_t hi[4], lo[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float x = v[2 * j] * scale, y = v[2 * j + 1] * scale;
+      hi[j] = narrow2<M>(x, y);
+      const float2 r = widen2<M>(hi[j]);
+      // (of an infinity or NaN there is no rest)
+      lo[j] = narrow2<M>(fabsf(r.x) < kInf ? x - r.x : 0.0f, fabsf(r.y) < kInf ? y - r.y : 0.0f);
+    }
+    *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+    *reinterpret_cast<uint4*>(dst + half_bytes) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+  };
+  {
+    // the first chunk: all pieces at once, four in flight a thread
+    const int n = end - begin < a.chunk ? end - begin : a.chunk;
+    const int pieces = n * T * kStepPieces;
+    for (int i0 = tid; i0 < pieces; i0 += 4 * kThreads) {
+      float4 v[4][2];
+#pragma unroll
+      for (int m = 0; m < 4; ++m) {
+        const int i = i0 + m * kThreads, q = i % kStepPieces, r = i / kStepPieces;
+        if (i < pieces) fetch(begin + r / T, r % T, q, v[m][0], v[m][1]);
+      }
+#pragma unroll
+      for (int m = 0; m < 4; ++m) {
+        const int i = i0 + m * kThreads, q = i % kStepPieces, r = i / kStepPieces, t = r % T;
+        if (i < pieces)
+          put_piece(smem + r / T * step_bytes + ((uint32_t)(q % G::kPieces) * T + t) * 64 + q / G::kPieces * 16,
+                    pow2(range_exponent(top[t])), v[m][0], v[m][1]);
+      }
+    }
+  }
+  __syncthreads();
+  float4 v0, v1;
+
+  float acc[NT][4];
 #pragma unroll
   for (int i = 0; i < NT; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
-
-  constexpr int kUnits = kChunk * G::kStep / 8;   // 16-byte pieces of a token
-  const uint32_t half_bytes = (uint32_t)kUnits * T * 16;
-  int buf = 0;
-  for (int at = begin; at < end; at += kChunk, buf ^= 1) {
-    const int n = end - at < kChunk ? end - at : kChunk;
-    // ---- stage the chunk's hidden values, as two 16-bit numbers of [2^14, 2^15) at most
-    constexpr int kMine = (NT * 8 * kUnits + kThreads - 1) / kThreads;   // pieces of a thread at most
-    float v[kMine][8];
-#pragma unroll
-    for (int m = 0; m < kMine; ++m) {
-      const int i = tid + m * kThreads;
-      const int t = i / kUnits, q = i - t * kUnits, st = q / (G::kStep / 8);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[m][j] = 0.0f;
-      if (t < T && st < n) {
-        const int u = (at + st) / fsteps, kk = (at + st - u * fsteps) * G::kStep + (q % (G::kStep / 8)) * 8;
-        if (((tokens[u] >> t) & 1u) && kk < a.F) {
-          const float4* src = reinterpret_cast<const float4*>(a.h + ((int64_t)u * T + t) * a.F + kk);
-          const float4 lo = __ldg(src), hi = __ldg(src + 1);
-          v[m][0] = lo.x; v[m][1] = lo.y; v[m][2] = lo.z; v[m][3] = lo.w;
-          v[m][4] = hi.x; v[m][5] = hi.y; v[m][6] = hi.z; v[m][7] = hi.w;
-        }
-      }
-      if (t < T) {
-        uint32_t mx = 0u;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const uint32_t b = __float_as_uint(v[m][j]) & 0x7fffffffu;
-          mx = max(mx, b < 0x7f800000u ? b : 0u);
-        }
-        if (mx) atomicMax(&top[buf][t], mx);
-      }
-    }
-    __syncthreads();
-    if (tid < kMaxTokens) top[buf ^ 1][tid] = 0u;   // read before this barrier, written behind the next
-    uint8_t* stage = smem + buf * 2 * half_bytes;
-#pragma unroll
-    for (int m = 0; m < kMine; ++m) {
-      const int i = tid + m * kThreads;
-      const int t = i / kUnits, q = i - t * kUnits;
-      if (t >= T) continue;
-      const float sc = pow2(range_exponent(top[buf][t]));
-      uint32_t hi[4], lo[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float x = v[m][2 * j] * sc, y = v[m][2 * j + 1] * sc;
-        hi[j] = narrow2<M>(x, y);
-        const float2 r = widen2<M>(hi[j]);
-        // (of an infinity or NaN there is no rest)
-        lo[j] = narrow2<M>(fabsf(r.x) < kInf ? x - r.x : 0.0f, fabsf(r.y) < kInf ? y - r.y : 0.0f);
-      }
-      const uint32_t off = piece_offset<FP8>(q, t, T);
-      *reinterpret_cast<uint4*>(stage + off) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-      *reinterpret_cast<uint4*>(stage + half_bytes + off) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-    }
-    __syncthreads();
-    float un[NT][2];
-#pragma unroll
-    for (int i = 0; i < NT; ++i) {
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int t = i * 8 + c * 2 + j;
-        un[i][j] = t < T ? pow2(-range_exponent(top[buf][t])) : 0.0f;
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) part_acc[i][j] = 0.0f;
-    }
-    // ---- multiply
+  // this lane's column: token, and (MODE 0) half
+  const uint8_t* col = smem + (MODE == 0 ? (g & 3) * 64 + (g >> 2) * half_bytes : g * 64) + c * 16;
+  const uint32_t buf_bytes = 2 * half_bytes;
+  int u = begin / fsteps, k = begin - u * fsteps, buf = 0;
+  for (int at = begin; at < end; at += a.chunk, buf ^= 1) {
+    const int n = end - at < a.chunk ? end - at : a.chunk;
+    const int next = end - at - n < a.chunk ? end - at - n : a.chunk;   // steps of the next chunk
+    uint8_t* other = smem + (buf ^ 1) * buf_bytes;
     for (int s0 = 0; s0 < n; s0 += kAhead) {
 #pragma unroll
       for (int b = 0; b < kAhead; ++b) {
         const int s = s0 + b;
         if (s >= n) break;
-        const uint32_t mask = tokens[(at + s) / fsteps];
+        if (stager) {
+          if (s > 0 && s - 1 < next) put_piece(other + (s - 1) * step_bytes + piece_at, sc, v0, v1);
+          if (s < next) fetch(at + n + s, st, sq, v0, v1);
+        }
+        const uint32_t mask = tokens[u];
+        const uint8_t* src = col + buf * buf_bytes + s * step_bytes;
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
-          float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-          const int t = i * 8 + g;
-          const bool has = (mask >> t) & 1u;
+          float part[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+          const bool has = (mask >> (MODE == 0 ? g & 3 : i * 8 + g)) & 1u;
 #pragma unroll
           for (int p = 0; p < G::kPieces; ++p) {
             uint4 hi = make_uint4(0u, 0u, 0u, 0u), lo = hi;
             if (has) {
-              const uint8_t* src = stage + ((uint32_t)(s * G::kPieces + p) * T + t) * 64 + c * 16;
-              hi = *reinterpret_cast<const uint4*>(src);
-              lo = *reinterpret_cast<const uint4*>(src + half_bytes);
+              hi = *reinterpret_cast<const uint4*>(src + p * T * 64 + i * 512);
+              if (MODE != 0) lo = *reinterpret_cast<const uint4*>(src + p * T * 64 + i * 512 + half_bytes);
             }
-            mma_piece<FP8, M>(part, w0[b], w1[b], p, hi);
-            mma_piece<FP8, M>(part, w0[b], w1[b], p, lo);
+            mma_piece<FP8, M>(part[MODE == 0 ? p & 1 : 0], w0[b], w1[b], p, hi);
+            if (MODE != 0) mma_piece<FP8, M>(part[1], w0[b], w1[b], p, lo);
           }
 #pragma unroll
-          for (int j = 0; j < 4; ++j) part_acc[i][j] = FP8 ? fmaf(part[j], f[b], part_acc[i][j]) : part_acc[i][j] + part[j];
+          for (int j = 0; j < 4; ++j) {
+            const float v = part[0][j] + part[1][j];
+            acc[i][j] = FP8 ? fmaf(v, f[b], acc[i][j]) : acc[i][j] + v;
+          }
         }
         load(w0[b], w1[b], f[b]);
+        if (++k == fsteps) {
+          k = 0;
+          ++u;
+        }
       }
     }
-#pragma unroll
-    for (int i = 0; i < NT; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(part_acc[i][j], un[i][j & 1], acc[i][j]);
+    if (next > 0) {
+      if (stager && n - 1 < next) put_piece(other + (n - 1) * step_bytes + piece_at, sc, v0, v1);
+      __syncthreads();
+    }
   }
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (MODE == 0) acc[i][j] += __shfl_xor_sync(0xffffffffu, acc[i][j], 2);   // columns t and t + 4
+      const int t = i * 8 + c * 2 + (j & 1);
+      acc[i][j] *= t < T ? pow2(-range_exponent(top[t])) : 0.0f;
+    }
 
   // ---- the slices' sum
   auto put = [&](int t, int row, float v) {
@@ -721,7 +809,7 @@ __global__ void __launch_bounds__(kThreads, 1) down_kernel(const FewArgs a) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int t = i * 8 + c * 2 + (j & 1), row = row0 + g + (j >> 1) * 8;
-        if (t >= T) continue;
+        if (t >= T) continue;   // (MODE 0: the other half's columns too)
         if (slices == 1)
           put(t, row, acc[i][j]);
         else
@@ -746,7 +834,7 @@ __global__ void __launch_bounds__(kThreads, 1) down_kernel(const FewArgs a) {
 
 // ---------------------------------------------------------------------------------------
 struct FewWorkspace {
-  size_t head, counters, h, part, total;
+  size_t head, counters, tops, h, part, total;
 };
 FewWorkspace few_workspace(int T, int d, int F, int E, int k, int S) {
   auto up = [](size_t n) { return (n + 255) / 256 * 256; };
@@ -756,18 +844,24 @@ FewWorkspace few_workspace(int T, int d, int F, int E, int k, int S) {
   FewWorkspace w;
   w.head = 0;
   w.counters = up(sizeof(Header));
-  w.h = w.counters + up((size_t)blocks * 4);
+  w.tops = w.counters + up((size_t)blocks * 4);
+  w.h = w.tops + up((size_t)kMaxCtas * T * 4);
   w.part = w.h + up((size_t)used * T * F * 4);
   w.total = w.part + up((size_t)split * T * d * 4);
   return w;
 }
 
-template <bool FP8, typename X, int NT>
-int launch(const FewArgs& a, int grid1, int grid2, uint32_t smem1, cudaStream_t stream) {
-  auto k1 = gate_up_kernel<FP8, X, NT>;
-  const int nt2 = a.T > 8 ? 2 : 1;
-  auto k2 = nt2 == 1 ? down_kernel<FP8, X, 1> : down_kernel<FP8, X, 2>;
-  const uint32_t smem2 = 2 * stage_bytes<FP8>(a.T);
+template <bool FP8, typename X>
+int launch(FewArgs a, int grid1, int grid2, uint32_t smem1, cudaStream_t stream) {
+  // the slices' hidden values whole, if they fit; else chunks of whole rounds of the buffers in flight
+  const uint32_t step_bytes = (uint32_t)Geo<FP8>::kStep * a.T * 4;
+  a.chunk = (int)(kStageBytes / step_bytes) / kAhead * kAhead;
+  const int used = (a.E < a.T * a.k ? a.E : a.T * a.k) + a.S;
+  const int64_t most = ((int64_t)used * ((a.F + Geo<FP8>::kStep - 1) / Geo<FP8>::kStep) + a.split - 1) / a.split + 1;
+  const uint32_t smem2 = (most <= a.chunk ? 1 : 2) * a.chunk * step_bytes;
+  const bool two = a.T > 8 && a.groups == 1;
+  auto k1 = two ? gate_up_kernel<FP8, X, 2> : gate_up_kernel<FP8, X, 1>;
+  auto k2 = a.T <= 4 ? down_kernel<FP8, X, 0> : (a.T <= 8 ? down_kernel<FP8, X, 1> : down_kernel<FP8, X, 2>);
   int st = set_max_dynamic_smem(reinterpret_cast<const void*>(k1), smem1);
   if (st != LMOE_OK) return st;
   st = set_max_dynamic_smem(reinterpret_cast<const void*>(k2), smem2);
@@ -841,6 +935,7 @@ extern "C" int lmoe_moe_layer_few_tokens(const void* x, int dtype, int64_t num_t
   uint8_t* base = static_cast<uint8_t*>(workspace);
   a.head = reinterpret_cast<Header*>(base + ws.head);
   a.counters = reinterpret_cast<uint32_t*>(base + ws.counters);
+  a.tops = reinterpret_cast<uint32_t*>(base + ws.tops);
   a.h = reinterpret_cast<float*>(base + ws.h);
   a.part = reinterpret_cast<float*>(base + ws.part);
   // All tokens of a large layer may not fit shared memory: then eight at a time, each group reading
@@ -856,18 +951,11 @@ extern "C" int lmoe_moe_layer_few_tokens(const void* x, int dtype, int64_t num_t
   }
   const int blocks = (a.d + kRowBlock - 1) / kRowBlock;
   a.split = kSplitCtas / blocks > 1 ? kSplitCtas / blocks : 1;
-  const int grid1 = gemm_grid(dev), grid2 = blocks * a.split;
-  const bool two = T > 8 && a.groups == 1;
-  if (dtype == LMOE_DTYPE_BF16) {
-    if (fp8)
-      return two ? launch<true, __nv_bfloat16, 2>(a, grid1, grid2, smem1, stream)
-                 : launch<true, __nv_bfloat16, 1>(a, grid1, grid2, smem1, stream);
-    return two ? launch<false, __nv_bfloat16, 2>(a, grid1, grid2, smem1, stream)
-               : launch<false, __nv_bfloat16, 1>(a, grid1, grid2, smem1, stream);
-  }
-  if (fp8)
-    return two ? launch<true, __half, 2>(a, grid1, grid2, smem1, stream)
-               : launch<true, __half, 1>(a, grid1, grid2, smem1, stream);
-  return two ? launch<false, __half, 2>(a, grid1, grid2, smem1, stream)
-             : launch<false, __half, 1>(a, grid1, grid2, smem1, stream);
+  a.grid1 = gemm_grid(dev) < kMaxCtas ? gemm_grid(dev) : kMaxCtas;
+  const int grid2 = blocks * a.split;
+  if (dtype == LMOE_DTYPE_BF16)
+    return fp8 ? launch<true, __nv_bfloat16>(a, a.grid1, grid2, smem1, stream)
+               : launch<false, __nv_bfloat16>(a, a.grid1, grid2, smem1, stream);
+  return fp8 ? launch<true, __half>(a, a.grid1, grid2, smem1, stream)
+             : launch<false, __half>(a, a.grid1, grid2, smem1, stream);
 }
