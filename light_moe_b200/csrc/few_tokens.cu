@@ -175,6 +175,11 @@ __device__ __forceinline__ uint32_t finite_top(uint32_t w) {
   return max(a < 0x7f800000u ? a : 0u, b < 0x7f800000u ? b : 0u);
 }
 
+// The second kernel is launched while the first one runs: its CTAs start as the first one's leave
+// their SMs, and wait here for all of it.
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_launcher() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // ---------------------------------------------------------------------------------------
 // first kernel
 // ---------------------------------------------------------------------------------------
@@ -182,30 +187,27 @@ struct FewShared {
   uint32_t used_tokens[kMaxUsed];   // bit t: token t chose expert e (all experts)
   int list[kMaxUsed];               // experts with tokens
   int group[kMaxUsed];              // positions in `list` that have tokens of the group
-  int used, group_used;
+  int used, group_used, warps_per_tile;
   uint64_t full[kJoins][kWarps];    // a tile's parts are written (its warps)
   uint64_t empty[kJoins][kWarps];   // ... and joined
   int abort;
   uint32_t htop[kMaxTokens];        // largest hidden values
   uint32_t top[kMaxTokens];         // largest absolute value of the group's tokens
   float unscale[kMaxTokens];
-  int chosen[kMaxTokens][kMaxTopK];
-  float weight[kMaxTokens][kMaxTopK];
 };
 
 // Dynamic shared memory of the first kernel.
 struct FewLayout {
-  uint32_t x, red, logits, share, total;
+  uint32_t x, red, share, total;
 };
-__host__ __device__ inline FewLayout few_layout(int d, int step, int group_tokens, int T, int E, int S) {
+__host__ __device__ inline FewLayout few_layout(int d, int step, int group_tokens, int T, int experts) {
   FewLayout l;
   const uint32_t kpad = (uint32_t)(d + step - 1) / step * step;
   const uint32_t nt = group_tokens > 8 ? 2 : 1;
   l.x = 0;
   l.red = kpad * group_tokens * 2;
-  l.logits = l.red + kJoins * kWarps * 16 * 8 * nt * 4;
-  l.share = l.logits + (uint32_t)(T * E + 3) / 4 * 16;
-  l.total = l.share + (uint32_t)((E + S) * T + 3) / 4 * 16;
+  l.share = l.red + kJoins * kWarps * 16 * 8 * nt * 4;
+  l.total = l.share + (uint32_t)(experts * T + 3) / 4 * 16;
   return l;
 }
 
@@ -219,39 +221,67 @@ __global__ void __launch_bounds__(kThreads, 1) gate_up_kernel(const FewArgs a) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   const int steps = (a.d + G::kStep - 1) / G::kStep;
   const int per_group = a.groups == 1 ? a.T : 8;
-  const FewLayout lay = few_layout(a.d, G::kStep, per_group, a.T, a.E, a.S);
+  const int experts = a.E + a.S;
+  const FewLayout lay = few_layout(a.d, G::kStep, per_group, a.T, experts);
   float* red = reinterpret_cast<float*>(smem + lay.red);
-  float* logits = reinterpret_cast<float*>(smem + lay.logits);   // [T][E]
   float* share = reinterpret_cast<float*>(smem + lay.share);     // [E + S][T]: routing weights
   constexpr int kRedRow = 8 * NT, kRedWarp = 16 * kRedRow, kRedBuf = kWarps * kRedWarp;
-  const int experts = a.E + a.S;
-  if (tid < kMaxTokens) sh.htop[tid] = 0u;
+  const int pieces = steps * G::kStep / 8;   // of a token; behind d: zeros
+  launch_dependents();
+
+  // The router's weights are 16 experts a fragment; warps that have the same one share its steps.  The
+  // first two steps' loads start before the tokens are there.
+  const int mtiles = (a.E + 15) / 16;
+  const int wpm = mtiles == 1 ? 16 : (mtiles == 2 ? 8 : (mtiles <= 4 ? 4 : (mtiles <= 8 ? 2 : 1)));
+  const int e0 = warp / wpm * 16;
+  const X* r0 = static_cast<const X*>(a.gate) + (int64_t)(e0 + g) * a.d + c * G::kPer;
+  const X* r1 = r0 + (int64_t)8 * a.d;
+  auto load_gate = [&](int s, uint4 (&v0)[G::kPieces], uint4 (&v1)[G::kPieces]) {
+#pragma unroll
+    for (int p = 0; p < G::kPieces; ++p) {
+      const int at = s * G::kStep + p * 8;
+      const bool in = at + c * G::kPer < a.d && s < steps;
+      v0[p] = v1[p] = make_uint4(0u, 0u, 0u, 0u);
+      if (in && e0 + g < a.E) v0[p] = __ldg(reinterpret_cast<const uint4*>(r0 + at));
+      if (in && e0 + g + 8 < a.E) v1[p] = __ldg(reinterpret_cast<const uint4*>(r1 + at));
+    }
+  };
+
+  if (tid < kMaxTokens) {
+    sh.htop[tid] = 0u;
+    sh.top[tid] = 0u;
+  }
   if (tid == 0) sh.abort = 0;
   if (tid == 0 && blockIdx.x == 0) a.head->error = 0u;
+  for (int i = tid; i < experts * a.T; i += kThreads) share[i] = i >= a.E * a.T ? 1.0f : 0.0f;
+  for (int e = tid; e < experts; e += kThreads) sh.used_tokens[e] = e >= a.E ? (1u << a.T) - 1u : 0u;
 
   // tokens t0 .. t0 + n - 1 into shared memory, in the order of the fragments
   auto load_x = [&](int t0, int n) {
-    if (kScaled && tid < kMaxTokens) sh.top[tid] = 0;
-    __syncthreads();   // earlier readers of the tokens too
-    const int pieces = steps * G::kStep / 8;   // behind d: zeros
-    for (int i = tid; i < pieces * n; i += kThreads) {
-      const int t = i / pieces, q = i - t * pieces;
-      uint4 v = make_uint4(0u, 0u, 0u, 0u);
-      if (q * 8 < a.d) v = __ldg(reinterpret_cast<const uint4*>(static_cast<const X*>(a.x) + (int64_t)(t0 + t) * a.d) + q);
-      *reinterpret_cast<uint4*>(smem + lay.x + piece_offset<FP8>(q, t, n)) = v;
+    __syncthreads();   // earlier readers of the tokens, and their largest values set to 0
+    for (int i0 = warp * 32; i0 < pieces * n; i0 += kThreads) {
+      const int i = i0 + lane, t = n == 1 ? 0 : i / pieces, q = i - t * pieces;
+      uint32_t m = 0u;
+      if (t < n && q < pieces) {
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        if (q * 8 < a.d) v = __ldg(reinterpret_cast<const uint4*>(static_cast<const X*>(a.x) + (int64_t)(t0 + t) * a.d) + q);
+        *reinterpret_cast<uint4*>(smem + lay.x + piece_offset<FP8>(q, t, n)) = v;
+        if (kScaled) m = max(max(finite_top<X>(v.x), finite_top<X>(v.y)), max(finite_top<X>(v.z), finite_top<X>(v.w)));
+      }
       if (kScaled) {
-        const uint32_t m = max(max(finite_top<X>(v.x), finite_top<X>(v.y)), max(finite_top<X>(v.z), finite_top<X>(v.w)));
-        atomicMax(&sh.top[t], m);
+        const uint32_t same = __match_any_sync(0xffffffffu, t);
+        const uint32_t most = __reduce_max_sync(same, m);
+        if (t < n && lane == __ffs(same) - 1) atomicMax(&sh.top[t], most);
       }
     }
     __syncthreads();
   };
-  // ... and to scaled fp16 in place
-  auto scale_x = [&](int n) {
+  // ... and to scaled fp16 in place, by the warps from `first` on
+  auto scale_x = [&](int n, int first) {
     if constexpr (kScaled) {
-      const int pieces = steps * G::kStep / 8;
-      for (int i = tid; i < pieces * n; i += kThreads) {
-        const int t = i / pieces, q = i - t * pieces;
+      if (warp < first) return;
+      for (int i = tid - first * 32; i < pieces * n; i += kThreads - first * 32) {
+        const int t = n == 1 ? 0 : i / pieces, q = i - t * pieces;
         const float f = pow2(range_exponent(sh.top[t]));
         uint4* p = reinterpret_cast<uint4*>(smem + lay.x + piece_offset<FP8>(q, t, n));
         uint4 v = *p;
@@ -263,186 +293,180 @@ __global__ void __launch_bounds__(kThreads, 1) gate_up_kernel(const FewArgs a) {
         }
         *p = v;
       }
+      if (warp == first && lane < n) sh.unscale[lane] = pow2(-range_exponent(sh.top[lane]));
     }
-    if (tid < n) sh.unscale[tid] = kScaled ? pow2(-range_exponent(sh.top[tid])) : 1.0f;
-    __syncthreads();
   };
+  if (!kScaled && tid < kMaxTokens) sh.unscale[tid] = 1.0f;
 
-  // ---- routing: logits, 16 experts at a time
+  // ---- routing
   for (int t0 = 0; t0 < a.T; t0 += per_group) {
     const int n = a.T - t0 < per_group ? a.T - t0 : per_group;
+    uint4 v[2][2][G::kPieces];
+    load_gate(warp % wpm, v[0][0], v[0][1]);
+    load_gate(warp % wpm + wpm, v[1][0], v[1][1]);
     load_x(t0, n);
-    for (int e0 = 0; e0 < a.E; e0 += 16) {
-      float acc[NT][4];
+    float acc[NT][4];
 #pragma unroll
-      for (int i = 0; i < NT; ++i)
+    for (int i = 0; i < NT; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
-      const X* r0 = static_cast<const X*>(a.gate) + (int64_t)(e0 + g) * a.d;
-      const X* r1 = r0 + (int64_t)8 * a.d;
-      const bool ok0 = e0 + g < a.E, ok1 = e0 + g + 8 < a.E;
-      for (int s = warp; s < steps; s += kWarps) {
-        uint4 w0[G::kPieces], w1[G::kPieces];
+      for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
+    for (int s0 = warp % wpm; s0 < steps; s0 += 2 * wpm) {
 #pragma unroll
-        for (int p = 0; p < G::kPieces; ++p) {
-          const int at = s * G::kStep + c * G::kPer + p * 8;
-          w0[p] = w1[p] = make_uint4(0u, 0u, 0u, 0u);
-          if (ok0 && at < a.d) w0[p] = __ldg(reinterpret_cast<const uint4*>(r0 + at));
-          if (ok1 && at < a.d) w1[p] = __ldg(reinterpret_cast<const uint4*>(r1 + at));
-        }
+      for (int b = 0; b < 2; ++b) {
+        const int s = s0 + b * wpm;
+        if (s >= steps) break;
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
           float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
           const int t = i * 8 + g;
 #pragma unroll
           for (int p = 0; p < G::kPieces; ++p) {
-            uint4 b = make_uint4(0u, 0u, 0u, 0u);
-            if (t < n) b = *reinterpret_cast<const uint4*>(smem + lay.x + ((uint32_t)(s * G::kPieces + p) * n + t) * 64 + c * 16);
-            mma16816<X>(part, w0[p].x, w1[p].x, w0[p].y, w1[p].y, b.x, b.y);
-            mma16816<X>(part, w0[p].z, w1[p].z, w0[p].w, w1[p].w, b.z, b.w);
+            uint4 x = make_uint4(0u, 0u, 0u, 0u);
+            if (t < n) x = *reinterpret_cast<const uint4*>(smem + lay.x + ((uint32_t)(s * G::kPieces + p) * n + t) * 64 + c * 16);
+            mma16816<X>(part, v[b][0][p].x, v[b][1][p].x, v[b][0][p].y, v[b][1][p].y, x.x, x.y);
+            mma16816<X>(part, v[b][0][p].z, v[b][1][p].z, v[b][0][p].w, v[b][1][p].w, x.z, x.w);
           }
 #pragma unroll
           for (int j = 0; j < 4; ++j) acc[i][j] += part[j];
         }
+        load_gate(s + 2 * wpm, v[b][0], v[b][1]);
       }
-      float* mine = red + warp * kRedWarp;
+    }
+    float* mine = red + warp * kRedWarp;
 #pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        *reinterpret_cast<float2*>(mine + g * kRedRow + i * 8 + c * 2) = make_float2(acc[i][0], acc[i][1]);
-        *reinterpret_cast<float2*>(mine + (g + 8) * kRedRow + i * 8 + c * 2) = make_float2(acc[i][2], acc[i][3]);
-      }
-      __syncthreads();
-      for (int i = tid; i < 16 * n; i += kThreads) {
-        const int e = i / n, t = i - e * n;
-        if (e0 + e < a.E) {
-          float v = 0.0f;
+    for (int i = 0; i < NT; ++i) {
+      *reinterpret_cast<float2*>(mine + g * kRedRow + i * 8 + c * 2) = make_float2(acc[i][0], acc[i][1]);
+      *reinterpret_cast<float2*>(mine + (g + 8) * kRedRow + i * 8 + c * 2) = make_float2(acc[i][2], acc[i][3]);
+    }
+    __syncthreads();
+    if (warp < n) {
+      // one warp per token
+      const int t = warp;
+      float v[kMaxExperts / 32];
+      uint32_t key[kMaxExperts / 32];   // orders like the logits; NaN lowest, 0: none or taken
 #pragma unroll
-          for (int w = 0; w < kWarps; ++w) v += red[w * kRedWarp + e * kRedRow + t];
-          if (a.bias) v += __ldg(a.bias + e0 + e);
-          logits[(t0 + t) * a.E + e0 + e] = v;
+      for (int i = 0; i < kMaxExperts / 32; ++i) {
+        v[i] = 0.0f;
+        key[i] = 0u;
+        if (i * 32 >= a.E) continue;
+        const int e = i * 32 + lane;
+        if (e < a.E) {
+          const float* r = red + (e >> 4) * wpm * kRedWarp + (e & 15) * kRedRow + t;
+          if (a.bias) v[i] = __ldg(a.bias + e);
+          float sum = 0.0f;
+#pragma unroll 4
+          for (int w = 0; w < wpm; ++w) sum += r[w * kRedWarp];
+          v[i] += sum;
+          const uint32_t b = __float_as_uint(v[i]);
+          key[i] = v[i] == v[i] ? ((b & 0x80000000u) ? ~b : (b | 0x80000000u)) : 1u;
         }
       }
-      __syncthreads();
+      float top = 0.0f, sum = 0.0f, mine_p = 0.0f;
+      int chosen = 0;
+      for (int j = 0; j < a.k; ++j) {
+        uint32_t best = 0u;
+#pragma unroll
+        for (int i = 0; i < kMaxExperts / 32; ++i) best = max(best, key[i]);
+        best = __reduce_max_sync(0xffffffffu, best);
+        int e = kMaxExperts;
+        float l = 0.0f;
+#pragma unroll
+        for (int i = kMaxExperts / 32 - 1; i >= 0; --i)
+          if (key[i] == best) {
+            e = i * 32 + lane;
+            l = v[i];
+          }
+        const int lowest = (int)__reduce_min_sync(0xffffffffu, (unsigned)e);
+        l = __shfl_sync(0xffffffffu, l, lowest & 31);   // the lowest id's lane found it
+#pragma unroll
+        for (int i = 0; i < kMaxExperts / 32; ++i)
+          if (i * 32 + lane == lowest) key[i] = 0u;
+        if (j == 0) top = l;
+        const float p = l == top ? 1.0f : (l == l ? softmax_exp(l - top) : l);
+        sum += p;
+        if (lane == j) {
+          mine_p = p;
+          chosen = lowest;
+        }
+      }
+      if (lane < a.k) {
+        const float w = __fdiv_rn(mine_p, sum);
+        share[chosen * a.T + t0 + t] = w;
+        atomicOr(&sh.used_tokens[chosen], 1u << (t0 + t));
+        if (blockIdx.x == 0) {
+          a.ids[(t0 + t) * a.k + lane] = chosen;
+          a.weights[(t0 + t) * a.k + lane] = w;
+        }
+      }
     }
+    // the warps without a token meanwhile
+    if (a.groups == 1) scale_x(n, n < kWarps ? n : 0);
+    if (a.groups > 1 && tid < kMaxTokens) sh.top[tid] = 0u;
+    __syncthreads();
   }
 
-  // ---- routing: one warp per token
-  for (int i = tid; i < experts * a.T; i += kThreads) share[i] = i >= a.E * a.T ? 1.0f : 0.0f;
-  for (int e = tid; e < experts; e += kThreads) sh.used_tokens[e] = e >= a.E ? (1u << a.T) - 1u : 0u;
-  __syncthreads();
-  if (warp < a.T) {
-    const int t = warp;
-    float v[kMaxExperts / 32];
-    uint32_t key[kMaxExperts / 32];   // orders like the logits; NaN lowest, 0: none or taken
-#pragma unroll
-    for (int i = 0; i < kMaxExperts / 32; ++i) {
-      const int e = i * 32 + lane;
-      v[i] = e < a.E ? logits[t * a.E + e] : 0.0f;
-      const uint32_t b = __float_as_uint(v[i]);
-      key[i] = e >= a.E ? 0u : (v[i] == v[i] ? ((b & 0x80000000u) ? ~b : (b | 0x80000000u)) : 1u);
-    }
-    float top = 0.0f, sum = 0.0f, mine = 0.0f;
-    int chosen = 0;
-    for (int j = 0; j < a.k; ++j) {
-      uint32_t best = 0u;
-#pragma unroll
-      for (int i = 0; i < kMaxExperts / 32; ++i) best = max(best, key[i]);
-      best = __reduce_max_sync(0xffffffffu, best);
-      int e = kMaxExperts;
-      float l = 0.0f;
-#pragma unroll
-      for (int i = kMaxExperts / 32 - 1; i >= 0; --i)
-        if (key[i] == best) {
-          e = i * 32 + lane;
-          l = v[i];
-        }
-      const int lowest = (int)__reduce_min_sync(0xffffffffu, (unsigned)e);
-      l = __shfl_sync(0xffffffffu, l, lowest & 31);   // the lowest id's lane found it
-#pragma unroll
-      for (int i = 0; i < kMaxExperts / 32; ++i)
-        if (i * 32 + lane == lowest) key[i] = 0u;
-      if (j == 0) top = l;
-      const float p = l == top ? 1.0f : (l == l ? softmax_exp(l - top) : l);
-      sum += p;
-      if (lane == j) {
-        mine = p;
-        chosen = lowest;
-      }
-    }
-    if (lane < a.k) {
-      const float w = __fdiv_rn(mine, sum);
-      share[chosen * a.T + t] = w;
-      atomicOr(&sh.used_tokens[chosen], 1u << t);
-      if (blockIdx.x == 0) {
-        a.ids[t * a.k + lane] = chosen;
-        a.weights[t * a.k + lane] = w;
-      }
-    }
-  }
-  __syncthreads();
+  // ---- the used experts, and the warps of a tile: a power of two, each with a step at least.  Many balance
+  // the last round, few have less to join (half a step's time a tile).  Reckoned for all SMs whatever the grid:
+  // the order of the sums, and so their last bits, do not depend on a limit of CTAs.
+  const int ftiles = a.F / 8;
   if (warp == 0) {
     int n = 0;
-    for (int e0 = 0; e0 < experts; e0 += 32) {
-      const int e = e0 + lane;
+    for (int b0 = 0; b0 < experts; b0 += 32) {
+      const int e = b0 + lane;
       const bool used = e < experts && sh.used_tokens[e] != 0u;
       const uint32_t m = __ballot_sync(0xffffffffu, used);
-      if (used) sh.list[n + __popc(m & ((1u << lane) - 1u))] = e;
+      const int at = n + __popc(m & ((1u << lane) - 1u));
+      if (used) {
+        sh.list[at] = e;
+        sh.group[at] = at;
+      }
       n += __popc(m);
     }
-    if (lane == 0) sh.used = n;
+    const int w = 1 << lane, groups = kSplitCtas * kWarps >> lane;   // lanes 0 .. 4
+    unsigned cost = 0xffffffffu;
+    if (lane < 5 && w <= steps)
+      cost = (unsigned)((n * ftiles + groups - 1) / groups * (2 * ((steps + w - 1) >> lane) + 1)) << 3 | lane;
+    const int wpt = 1 << (__reduce_min_sync(0xffffffffu, cost) & 7u);
+    if (lane == 0) {
+      sh.used = sh.group_used = n;
+      sh.warps_per_tile = wpt;
+    }
+    for (int i = lane; i < kJoins * kWarps; i += 32) {
+      mbar_init(&sh.full[i / kWarps][i % kWarps], (uint32_t)wpt);
+      mbar_init(&sh.empty[i / kWarps][i % kWarps], 1);
+    }
+    fence_mbar_init();
   }
   __syncthreads();
-  if (blockIdx.x == 0) {
-    for (int i = tid; i < sh.used; i += kThreads) {
-      a.head->expert[i] = sh.list[i];
-      a.head->tokens[i] = sh.used_tokens[sh.list[i]];
-    }
-    if (tid == 0) a.head->used = sh.used;
-    for (int i = tid; i < (a.d + kRowBlock - 1) / kRowBlock; i += kThreads) a.counters[i] = 0u;
-  }
 
   // ---- the experts' gate and up products
-  const int ftiles = a.F / 8;
   const int kblocks = (a.d + kFp8Block - 1) / kFp8Block, fblocks = (a.F + kFp8Block - 1) / kFp8Block;
-  // Warps of a tile: a power of two, each with a step at least.  Many balance the last round, few have
-  // less to join (half a step's time a tile).  Reckoned for all SMs whatever the grid: the order of the
-  // sums, and so their last bits, do not depend on a limit of CTAs.
-  int wpt = 1;
-  for (int w = 1, best = INT32_MAX; w <= kWarps && w <= steps; w <<= 1) {
-    const int groups = kSplitCtas * (kWarps / w), rounds = (sh.used * ftiles + groups - 1) / groups;
-    const int cost = rounds * (2 * ((steps + w - 1) / w) + 1);
-    if (cost < best) {
-      best = cost;
-      wpt = w;
-    }
-  }
+  const int wpt = sh.warps_per_tile;
   const int wi = warp & (wpt - 1), wt = warp / wpt;   // this warp's share of a tile, and its group of warps
   const int stride = (int)gridDim.x * (kWarps / wpt);
-  if (tid < kJoins * kWarps) {
-    mbar_init(&sh.full[tid / kWarps][tid % kWarps], (uint32_t)wpt);
-    mbar_init(&sh.empty[tid / kWarps][tid % kWarps], 1);
-  }
-  fence_mbar_init();
   int join = 0;   // the warps of a group count their tiles alike
   uint32_t parity = 0, joined = 0;
   float most[2 * NT] = {};
   for (int t0 = 0; t0 < a.T; t0 += per_group) {
     const int n = a.T - t0 < per_group ? a.T - t0 : per_group;
-    if (a.groups > 1) load_x(t0, n);   // else they are there
-    scale_x(n);
-    const uint32_t in_group = ((1u << n) - 1u) << t0;
-    if (warp == 0) {
-      int m = 0;
-      for (int u0 = 0; u0 < sh.used; u0 += 32) {
-        const int u = u0 + lane;
-        const bool has = u < sh.used && (sh.used_tokens[sh.list[u]] & in_group) != 0u;
-        const uint32_t b = __ballot_sync(0xffffffffu, has);
-        if (has) sh.group[m + __popc(b & ((1u << lane) - 1u))] = u;
-        m += __popc(b);
+    if (a.groups > 1) {   // else the tokens are there, and all experts are of the group
+      load_x(t0, n);
+      scale_x(n, 0);
+      const uint32_t in_group = ((1u << n) - 1u) << t0;
+      if (warp == 0) {
+        int m = 0;
+        for (int u0 = 0; u0 < sh.used; u0 += 32) {
+          const int u = u0 + lane;
+          const bool has = u < sh.used && (sh.used_tokens[sh.list[u]] & in_group) != 0u;
+          const uint32_t b = __ballot_sync(0xffffffffu, has);
+          if (has) sh.group[m + __popc(b & ((1u << lane) - 1u))] = u;
+          m += __popc(b);
+        }
+        if (lane == 0) sh.group_used = m;
       }
-      if (lane == 0) sh.group_used = m;
+      __syncthreads();
+      if (tid < kMaxTokens) sh.top[tid] = 0u;   // for the next group, behind load_x's barrier
     }
-    __syncthreads();
     const int tiles = sh.group_used * ftiles;
 
     uint32_t w0[kAhead][8], w1[kAhead][8];
@@ -598,6 +622,14 @@ __global__ void __launch_bounds__(kThreads, 1) gate_up_kernel(const FewArgs a) {
     __syncthreads();
   }
   if (tid < a.T) a.tops[(int64_t)blockIdx.x * a.T + tid] = sh.htop[tid];
+  if (blockIdx.x == 0) {
+    for (int i = tid; i < sh.used; i += kThreads) {
+      a.head->expert[i] = sh.list[i];
+      a.head->tokens[i] = sh.used_tokens[sh.list[i]];
+    }
+    if (tid == 0) a.head->used = sh.used;
+    for (int i = tid; i < (a.d + kRowBlock - 1) / kRowBlock; i += kThreads) a.counters[i] = 0u;
+  }
 }
 
 // ---------------------------------------------------------------------------------------
@@ -618,14 +650,15 @@ __global__ void __launch_bounds__(kThreads, 1) down_kernel(const FewArgs a) {
   const int T = a.T;
   if (tid < kMaxTokens) top[tid] = 0u;
   __syncthreads();
-  const int used = a.head->used;
-  for (int i = tid; i < used; i += kThreads) {
-    expert[i] = a.head->expert[i];
-    tokens[i] = a.head->tokens[i];
+  wait_for_launcher();
+  const int used = __ldcg(&a.head->used);
+  for (int i = tid; i < a.E + a.S; i += kThreads) {   // (behind `used`: never looked at)
+    expert[i] = __ldcg(&a.head->expert[i]);
+    tokens[i] = __ldcg(&a.head->tokens[i]);
   }
   for (int i = tid; i < a.grid1 * T; i += kThreads) {
-    const uint32_t v = a.tops[i];
-    if (v) atomicMax(&top[i % T], v);
+    const uint32_t v = __ldcg(a.tops + i);
+    if (v) atomicMax(&top[T == 1 ? 0 : i % T], v);
   }
   __syncthreads();
   const int fsteps = (a.F + G::kStep - 1) / G::kStep;
@@ -669,9 +702,6 @@ __global__ void __launch_bounds__(kThreads, 1) down_kernel(const FewArgs a) {
       aim();
     }
   };
-  aim();
-#pragma unroll
-  for (int i = 0; i < kAhead; ++i) load(w0[i], w1[i], f[i]);
 
   // Hidden values: of each step, a thread stages at most one piece of 8 values of a token, as two 16-bit
   // numbers (of values scaled to at most 2^15).  The pieces of the next chunk's steps are loaded beside this
@@ -709,15 +739,22 @@ __global__ void __launch_bounds__(kThreads, 1) down_kernel(const FewArgs a) {
     *reinterpret_cast<uint4*>(dst + half_bytes) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
   };
   {
-    // the first chunk: all pieces at once, four in flight a thread
+    // the first chunk: all pieces at once, four in flight a thread; the first ones are asked for before the weights
     const int n = end - begin < a.chunk ? end - begin : a.chunk;
     const int pieces = n * T * kStepPieces;
-    for (int i0 = tid; i0 < pieces; i0 += 4 * kThreads) {
+    bool primed = false;
+    for (int i0 = tid; i0 < pieces || !primed; i0 += 4 * kThreads) {
       float4 v[4][2];
 #pragma unroll
       for (int m = 0; m < 4; ++m) {
         const int i = i0 + m * kThreads, q = i % kStepPieces, r = i / kStepPieces;
         if (i < pieces) fetch(begin + r / T, r % T, q, v[m][0], v[m][1]);
+      }
+      if (!primed) {
+        primed = true;
+        aim();
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) load(w0[j], w1[j], f[j]);
       }
 #pragma unroll
       for (int m = 0; m < 4; ++m) {
@@ -817,17 +854,33 @@ __global__ void __launch_bounds__(kThreads, 1) down_kernel(const FewArgs a) {
       }
   }
   if (slices == 1) return;
-  __threadfence();
-  __syncthreads();
-  if (tid == 0) last = atomicAdd(&a.counters[rb], 1u) == (uint32_t)slices - 1u;
+  __syncthreads();   // all parts are written before thread 0's release
+  if (tid == 0) {
+    uint32_t before;
+    asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], %2;" : "=r"(before) : "l"(a.counters + rb), "r"(1u) : "memory");
+    last = before == (uint32_t)slices - 1u;
+  }
   __syncthreads();
   if (!last) return;
-  __threadfence();
   for (int i = tid; i < T * kRowBlock; i += kThreads) {
     const int t = i / kRowBlock, row = rb * kRowBlock + i % kRowBlock;
     if (row >= a.d) continue;
+    const float* src = a.part + (int64_t)t * a.d + row;
+    const int64_t step = (int64_t)T * a.d;
     float v = 0.0f;
-    for (int s = 0; s < slices; ++s) v += __ldcg(a.part + ((int64_t)s * T + t) * a.d + row);
+    int s = 0;
+    for (; s + 8 <= slices; s += 8) {   // eight loads at a time, added in order
+      float p[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) p[j] = __ldcg(src + (s + j) * step);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v += p[j];
+    }
+    float p[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) p[j] = s + j < slices ? __ldcg(src + (s + j) * step) : 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v += p[j];
     put(t, row, v);
   }
 }
@@ -868,8 +921,17 @@ int launch(FewArgs a, int grid1, int grid2, uint32_t smem1, cudaStream_t stream)
   if (st != LMOE_OK) return st;
   k1<<<grid1, kThreads, smem1, stream>>>(a);
   LMOE_CUDA_TRY(cudaGetLastError());
-  k2<<<grid2, kThreads, smem2, stream>>>(a);
-  return cuda_status(cudaGetLastError());
+  cudaLaunchAttribute early = {};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3((unsigned)grid2);
+  config.blockDim = dim3(kThreads);
+  config.dynamicSmemBytes = smem2;
+  config.stream = stream;
+  config.attrs = &early;
+  config.numAttrs = 1;
+  return cuda_status(cudaLaunchKernelEx(&config, k2, a));
 }
 
 bool few_sizes(int64_t T, int d, int F, int E, int k, int S) {
@@ -943,10 +1005,10 @@ extern "C" int lmoe_moe_layer_few_tokens(const void* x, int dtype, int64_t num_t
   const uint32_t limit = (uint32_t)dev.max_smem_optin - (uint32_t)sizeof(FewShared) - 1024;
   const int step = fp8 ? 128 : 64;
   a.groups = 1;
-  uint32_t smem1 = few_layout(a.d, step, T, T, a.E, a.S).total;
+  uint32_t smem1 = few_layout(a.d, step, T, T, a.E + a.S).total;
   if (smem1 > limit) {
     a.groups = (T + 7) / 8;
-    smem1 = few_layout(a.d, step, 8, T, a.E, a.S).total;
+    smem1 = few_layout(a.d, step, 8, T, a.E + a.S).total;
     if (smem1 > limit || a.groups < 2) return LMOE_ERR_UNSUPPORTED;
   }
   const int blocks = (a.d + kRowBlock - 1) / kRowBlock;
