@@ -226,6 +226,8 @@ __global__ void __launch_bounds__(kThreads, 1) gate_up_kernel(const FewArgs a) {
   float* red = reinterpret_cast<float*>(smem + lay.red);
   float* share = reinterpret_cast<float*>(smem + lay.share);     // [E + S][T]: routing weights
   constexpr int kRedRow = 8 * NT, kRedWarp = 16 * kRedRow, kRedBuf = kWarps * kRedWarp;
+  float* logits = red + kRedBuf;   // [tokens of the group][256], while routing
+  static_assert((kJoins - 1) * kRedBuf >= 8 * NT * kMaxExperts, "room for the logits");
   const int pieces = steps * G::kStep / 8;   // of a token; behind d: zeros
   launch_dependents();
 
@@ -340,53 +342,45 @@ __global__ void __launch_bounds__(kThreads, 1) gate_up_kernel(const FewArgs a) {
     }
     __syncthreads();
     if (warp < n) {
-      // one warp per token
+      // One warp per token.  A pick is the best one behind the last pick, in the order of logits and ids
+      // (little code: what runs once waits for its instructions).
       const int t = warp;
-      float v[kMaxExperts / 32];
-      uint32_t key[kMaxExperts / 32];   // orders like the logits; NaN lowest, 0: none or taken
-#pragma unroll
-      for (int i = 0; i < kMaxExperts / 32; ++i) {
-        v[i] = 0.0f;
-        key[i] = 0u;
-        if (i * 32 >= a.E) continue;
-        const int e = i * 32 + lane;
-        if (e < a.E) {
-          const float* r = red + (e >> 4) * wpm * kRedWarp + (e & 15) * kRedRow + t;
-          if (a.bias) v[i] = __ldg(a.bias + e);
-          float sum = 0.0f;
+      float* mine_l = logits + t * kMaxExperts;
+      for (int e = lane; e < a.E; e += 32) {
+        const float* r = red + (e >> 4) * wpm * kRedWarp + (e & 15) * kRedRow + t;
+        float sum = 0.0f;
 #pragma unroll 4
-          for (int w = 0; w < wpm; ++w) sum += r[w * kRedWarp];
-          v[i] += sum;
-          const uint32_t b = __float_as_uint(v[i]);
-          key[i] = v[i] == v[i] ? ((b & 0x80000000u) ? ~b : (b | 0x80000000u)) : 1u;
-        }
+        for (int w = 0; w < wpm; ++w) sum += r[w * kRedWarp];
+        mine_l[e] = a.bias ? sum + __ldg(a.bias + e) : sum;
       }
       float top = 0.0f, sum = 0.0f, mine_p = 0.0f;
-      int chosen = 0;
+      int chosen = 0, last = -1;
+      uint32_t last_key = 0xffffffffu;
+#pragma unroll 1
       for (int j = 0; j < a.k; ++j) {
-        uint32_t best = 0u;
-#pragma unroll
-        for (int i = 0; i < kMaxExperts / 32; ++i) best = max(best, key[i]);
-        best = __reduce_max_sync(0xffffffffu, best);
-        int e = kMaxExperts;
+        uint32_t key = 0u;   // orders like the logits; NaN lowest, 0: none
+        int at = kMaxExperts;
         float l = 0.0f;
-#pragma unroll
-        for (int i = kMaxExperts / 32 - 1; i >= 0; --i)
-          if (key[i] == best) {
-            e = i * 32 + lane;
-            l = v[i];
+#pragma unroll 1
+        for (int e = lane; e < a.E; e += 32) {
+          const float v = mine_l[e];
+          const uint32_t b = __float_as_uint(v);
+          const uint32_t k = v == v ? ((b & 0x80000000u) ? ~b : (b | 0x80000000u)) : 1u;
+          if ((k < last_key || (k == last_key && e > last)) && k > key) {
+            key = k;
+            at = e;
+            l = v;
           }
-        const int lowest = (int)__reduce_min_sync(0xffffffffu, (unsigned)e);
-        l = __shfl_sync(0xffffffffu, l, lowest & 31);   // the lowest id's lane found it
-#pragma unroll
-        for (int i = 0; i < kMaxExperts / 32; ++i)
-          if (i * 32 + lane == lowest) key[i] = 0u;
+        }
+        last_key = __reduce_max_sync(0xffffffffu, key);
+        last = (int)__reduce_min_sync(0xffffffffu, key == last_key ? (unsigned)at : (unsigned)kMaxExperts);
+        l = __shfl_sync(0xffffffffu, l, last & 31);
         if (j == 0) top = l;
         const float p = l == top ? 1.0f : (l == l ? softmax_exp(l - top) : l);
         sum += p;
         if (lane == j) {
           mine_p = p;
-          chosen = lowest;
+          chosen = last;
         }
       }
       if (lane < a.k) {
@@ -739,30 +733,33 @@ __global__ void __launch_bounds__(kThreads, 1) down_kernel(const FewArgs a) {
     *reinterpret_cast<uint4*>(dst + half_bytes) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
   };
   {
-    // the first chunk: all pieces at once, four in flight a thread; the first ones are asked for before the weights
+    // the first chunk, its first pieces asked for before the weights; four pieces in flight a thread if there are many
     const int n = end - begin < a.chunk ? end - begin : a.chunk;
     const int pieces = n * T * kStepPieces;
-    bool primed = false;
-    for (int i0 = tid; i0 < pieces || !primed; i0 += 4 * kThreads) {
+    auto place = [&](int i) {
+      const int q = i % kStepPieces, r = i / kStepPieces, t = T == 1 ? 0 : r % T, step = T == 1 ? r : r / T;
+      return smem + step * step_bytes + ((uint32_t)(q % G::kPieces) * T + t) * 64 + q / G::kPieces * 16;
+    };
+    auto ask = [&](int i, float4& x, float4& y) {
+      const int r = i / kStepPieces;
+      fetch(begin + (T == 1 ? r : r / T), T == 1 ? 0 : r % T, i % kStepPieces, x, y);
+    };
+    auto scale_of = [&](int i) { return pow2(range_exponent(top[T == 1 ? 0 : i / kStepPieces % T])); };
+    float4 x, y;
+    if (tid < pieces) ask(tid, x, y);
+    aim();
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) load(w0[j], w1[j], f[j]);
+    if (tid < pieces) put_piece(place(tid), scale_of(tid), x, y);
+#pragma unroll 1
+    for (int i0 = tid + kThreads; i0 < pieces; i0 += 4 * kThreads) {
       float4 v[4][2];
 #pragma unroll
-      for (int m = 0; m < 4; ++m) {
-        const int i = i0 + m * kThreads, q = i % kStepPieces, r = i / kStepPieces;
-        if (i < pieces) fetch(begin + r / T, r % T, q, v[m][0], v[m][1]);
-      }
-      if (!primed) {
-        primed = true;
-        aim();
+      for (int m = 0; m < 4; ++m)
+        if (i0 + m * kThreads < pieces) ask(i0 + m * kThreads, v[m][0], v[m][1]);
 #pragma unroll
-        for (int j = 0; j < kAhead; ++j) load(w0[j], w1[j], f[j]);
-      }
-#pragma unroll
-      for (int m = 0; m < 4; ++m) {
-        const int i = i0 + m * kThreads, q = i % kStepPieces, r = i / kStepPieces, t = r % T;
-        if (i < pieces)
-          put_piece(smem + r / T * step_bytes + ((uint32_t)(q % G::kPieces) * T + t) * 64 + q / G::kPieces * 16,
-                    pow2(range_exponent(top[t])), v[m][0], v[m][1]);
-      }
+      for (int m = 0; m < 4; ++m)
+        if (i0 + m * kThreads < pieces) put_piece(place(i0 + m * kThreads), scale_of(i0 + m * kThreads), v[m][0], v[m][1]);
     }
   }
   __syncthreads();
@@ -868,19 +865,14 @@ __global__ void __launch_bounds__(kThreads, 1) down_kernel(const FewArgs a) {
     const float* src = a.part + (int64_t)t * a.d + row;
     const int64_t step = (int64_t)T * a.d;
     float v = 0.0f;
-    int s = 0;
-    for (; s + 8 <= slices; s += 8) {   // eight loads at a time, added in order
-      float p[8];
+#pragma unroll 1
+    for (int s0 = 0; s0 < slices; s0 += 16) {   // sixteen loads at a time, added in order
+      float p[16];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) p[j] = __ldcg(src + (s + j) * step);
+      for (int j = 0; j < 16; ++j) p[j] = s0 + j < slices ? __ldcg(src + (s0 + j) * step) : 0.0f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v += p[j];
+      for (int j = 0; j < 16; ++j) v += p[j];
     }
-    float p[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) p[j] = s + j < slices ? __ldcg(src + (s + j) * step) : 0.0f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v += p[j];
     put(t, row, v);
   }
 }
