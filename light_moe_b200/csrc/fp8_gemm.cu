@@ -35,20 +35,21 @@ namespace {
 constexpr int kRowsCta = 128, kTM = 256, kBK = kFp8Block;
 constexpr int kEpiWarps = 8, kEpiWarp0 = 4, kThreads = (kEpiWarp0 + kEpiWarps) * 32;
 constexpr int kTmemCols = 512;
-constexpr int kSlotBlocks = 4, kSlots = 4;   // a slot of the scales' ring holds four blocks
+constexpr int kSlotBlocks = 8, kSlots = 3;   // a slot of the scales' ring holds eight blocks
 constexpr uint32_t kSite = 0x700u;
-constexpr uint32_t kStoreBytes = 2048;       // a block on its way out: 32 rows x 64 bytes
 // Registers: 384 threads x 168 at launch = 128 x 56 + 256 x 224.
 constexpr int kRegsLaunch = 168, kRegsOther = 56, kRegsEpi = 224;
 static_assert(128 * kRegsOther + 256 * kRegsEpi <= kThreads * kRegsLaunch, "register split");
 
-template <int TN>
+template <int TN, bool SWIGLU>
 struct Cfg {
   static constexpr int kHalf = TN / 2;                  // columns a CTA loads
-  static constexpr int kStages = TN == 256 ? 6 : 8;
+  static constexpr int kCols = TN / 2;                  // of an MMA, and of an epilogue thread
   static constexpr int kAcc = kTmemCols / TN;           // blocks' sums in tensor memory
-  static constexpr int kCols = TN / 2;                  // accumulators of an epilogue thread
+  static constexpr int kOutCols = SWIGLU ? kCols / 2 : kCols;       // of a warp's output
+  static constexpr uint32_t kStoreBytes = kOutCols / 32 * 2048;    // a warp's tile on its way out: blocks of 32 rows x 64 bytes
   static constexpr uint32_t kABytes = kRowsCta * kBK, kBBytes = kHalf * kBK, kStageBytes = kABytes + kBBytes;
+  static constexpr int kStages = TN == 256 ? (SWIGLU ? 5 : 4) : 6;
 };
 
 struct ScaleSlot {
@@ -56,27 +57,27 @@ struct ScaleSlot {
   float col[kSlotBlocks][2];   // of the tile's two column blocks, or of gate and up
 };
 
-template <int TN>
+template <class C>
 struct __align__(8) Bars {
-  using C = Cfg<TN>;
-  uint64_t full[C::kStages];     // leader: both CTAs' codes landed (one arrival each)
-  uint64_t empty[C::kStages];    // the stage's MMAs finished (both CTAs)
-  uint64_t acc_full[C::kAcc];    // a block's sums are in tensor memory (both CTAs)
-  uint64_t acc_empty[C::kAcc];   // leader: both CTAs' epilogue warps have read them
-  uint64_t sc_full[kSlots];      // this CTA: the slot's scales are written
-  uint64_t sc_empty[kSlots];     // this CTA: its epilogue warps have read them
+  uint64_t full[C::kStages];        // leader: both CTAs' codes landed (one arrival each)
+  uint64_t empty[C::kStages];       // both halves' MMAs of the stage finished (both CTAs)
+  uint64_t acc_full[2][C::kAcc];    // half of a block's sums is in tensor memory (both CTAs)
+  uint64_t acc_empty[2][C::kAcc];   // leader: both CTAs' epilogue warps of the half have read it
+  uint64_t sc_full[kSlots];         // this CTA: the slot's scales are written
+  uint64_t sc_empty[kSlots];        // this CTA: its epilogue warps have read them
   uint64_t mma_done;
   uint32_t tmem_base;
   int abort;
   SegTable seg;
 };
 
-template <int TN>
+template <class C>
 constexpr uint32_t smem_bytes() {
-  return 1024 + Cfg<TN>::kStages * Cfg<TN>::kStageBytes + kEpiWarps * kStoreBytes + kSlots * sizeof(ScaleSlot) +
-         sizeof(Bars<TN>);
+  return 1024 + C::kStages * C::kStageBytes + kEpiWarps * C::kStoreBytes + kSlots * sizeof(ScaleSlot) + sizeof(Bars<C>);
 }
-static_assert(smem_bytes<256>() <= 232448 && smem_bytes<128>() <= 232448, "shared memory budget");
+static_assert(smem_bytes<Cfg<256, false>>() <= 232448 && smem_bytes<Cfg<256, true>>() <= 232448 &&
+                  smem_bytes<Cfg<128, false>>() <= 232448 && smem_bytes<Cfg<128, true>>() <= 232448,
+              "shared memory budget");
 static_assert(sizeof(ScaleSlot) % 16 == 0, "alignment of what follows");
 
 struct Fp8Args {
@@ -171,12 +172,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     fp8_gemm_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_x32,
                     const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_up,
                     const __grid_constant__ CUtensorMap tm_out, const Fp8Args a) {
-  using C = Cfg<TN>;
+  using C = Cfg<TN, SWIGLU>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* store_stage = base + C::kStages * C::kStageBytes;
-  ScaleSlot* slots = reinterpret_cast<ScaleSlot*>(store_stage + kEpiWarps * kStoreBytes);
-  Bars<TN>* bars = reinterpret_cast<Bars<TN>*>(slots + kSlots);
+  ScaleSlot* slots = reinterpret_cast<ScaleSlot*>(store_stage + kEpiWarps * C::kStoreBytes);
+  Bars<C>* bars = reinterpret_cast<Bars<C>*>(slots + kSlots);
   volatile int* abort_flag = &bars->abort;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t rank = cluster_ctarank();
@@ -185,17 +186,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   if (tid == 0) {
     for (int s = 0; s < C::kStages; ++s) {
       mbar_init(&bars->full[s], 2);
-      mbar_init(&bars->empty[s], 1);
+      mbar_init(&bars->empty[s], 2);
     }
-    for (int s = 0; s < C::kAcc; ++s) {
-      mbar_init(&bars->acc_full[s], 1);
-      mbar_init(&bars->acc_empty[s], 2 * kEpiWarps);
-    }
+    for (int h = 0; h < 2; ++h)
+      for (int s = 0; s < C::kAcc; ++s) {
+        mbar_init(&bars->acc_full[h][s], 1);
+        mbar_init(&bars->acc_empty[h][s], kEpiWarps);
+      }
     for (int s = 0; s < kSlots; ++s) {
       mbar_init(&bars->sc_full[s], 1);
       mbar_init(&bars->sc_empty[s], kEpiWarps);
     }
-    mbar_init(&bars->mma_done, 1);
+    mbar_init(&bars->mma_done, 2);   // both issuers
     bars->abort = 0;
     fence_mbar_init();
   }
@@ -255,41 +257,41 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       }
       // the copies of a finished tile have landed (its MMAs read them)
       if (!ok) let_copies_land();
-    } else if (warp == 1) {
-      // ---------------------------------------------------------------- MMA issuer
+    } else if (warp == 1 || warp == 3) {
+      // ---------------------------------------------------------------- MMA issuers, one for each half of the columns
       if (leader) {
-        const uint64_t adesc0 = sdesc_k_sw128(smem_u32(base)), bdesc0 = sdesc_k_sw128(smem_u32(base) + C::kABytes);
+        const int h = warp >> 1;
+        const uint64_t adesc0 = sdesc_k_sw128(smem_u32(base));
+        const uint64_t bdesc0 = sdesc_k_sw128(smem_u32(base) + C::kABytes + h * (C::kHalf / 2 * kBK));
         Ring<C::kStages> st;
         Ring<C::kAcc> ac;
-        int hint = 0;
+        int blocks = 0, hint = 0;   // of all this pair's tiles
+        for (int tile = first; tile < total; tile += stride)
+          if (!fp8_tile_at(seg, a, tile, hint).zero) blocks += KB;
         bool ok = true;
-        for (int tile = first; tile < total && ok; tile += stride) {
-          const Fp8Tile t = fp8_tile_at(seg, a, tile, hint);
-          if (t.zero) continue;
-          for (int kb = 0; kb < KB; ++kb) {
-            // the waits start together; what has not come yet is waited for below
-            const bool w0 = mbar_test(&bars->acc_empty[ac.i], ac.phase ^ 1u);
-            const bool w1 = mbar_test(&bars->full[st.i], st.phase);
-            if (!(w0 && w1)) {
-              ok = mbar_wait(&bars->acc_empty[ac.i], ac.phase ^ 1u, a.err, abort_flag, kSite + 3);
-              if (ok) ok = mbar_wait(&bars->full[st.i], st.phase, a.err, abort_flag, kSite + 4);
-            }
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-            tc_fence_after();
-            if (elect_one()) {
-              const uint64_t ad = adesc0 + st.i * (C::kStageBytes >> 4), bd = bdesc0 + st.i * (C::kStageBytes >> 4);
-              const uint32_t d = tmem + ac.i * TN;
-#pragma unroll
-              for (int m = 0; m < kBK / 32; ++m)   // 32 bytes of the lines: two descriptor units
-                mma_fp8_pair(d, ad + m * 2, bd + m * 2, idesc_fp8(TN), (uint32_t)(m > 0));
-              mma_commit_pair(&bars->acc_full[ac.i]);
-              mma_commit_pair(&bars->empty[st.i]);
-            }
-            __syncwarp();
-            st.next();
-            ac.next();
+        for (; blocks > 0; --blocks) {
+          // the waits start together; what has not come yet is waited for below
+          const bool w0 = mbar_test(&bars->acc_empty[h][ac.i], ac.phase ^ 1u);
+          const bool w1 = mbar_test(&bars->full[st.i], st.phase);
+          if (!(w0 && w1)) {
+            ok = mbar_wait(&bars->acc_empty[h][ac.i], ac.phase ^ 1u, a.err, abort_flag, kSite + 3);
+            if (ok) ok = mbar_wait(&bars->full[st.i], st.phase, a.err, abort_flag, kSite + 4);
           }
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          tc_fence_after();
+          if (elect_one()) {
+            const uint64_t ad = adesc0 + st.i * (C::kStageBytes >> 4), bd = bdesc0 + st.i * (C::kStageBytes >> 4);
+            const uint32_t d = tmem + (ac.i * 2 + h) * C::kCols;
+#pragma unroll
+            for (int m = 0; m < kBK / 32; ++m)   // 32 bytes of the lines: two descriptor units
+              mma_fp8_pair(d, ad + m * 2, bd + m * 2, idesc_fp8(C::kCols), (uint32_t)(m > 0));
+            mma_commit_pair(&bars->acc_full[h][ac.i]);
+            mma_commit_pair(&bars->empty[st.i]);
+          }
+          __syncwarp();
+          st.next();
+          ac.next();
         }
         if (elect_one()) mma_commit_leader(&bars->mma_done);
         mbar_wait(&bars->mma_done, 0, a.err, nullptr, kSite + 5);
@@ -303,29 +305,31 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const Fp8Tile t = fp8_tile_at(seg, a, tile, hint);
         if (t.zero) continue;
         const int r0 = t.row0 + (int)rank * kRowsCta;
-        // lanes 0-3: the four blocks' scales of the first columns (gate), 4-7 of the second (up)
+        // lanes 0-7: the slot's scales of the first columns (gate), 8-15 of the second (up)
         const int nb0 = SWIGLU ? t.n * C::kHalf / kFp8Block : t.n * TN / kFp8Block;
         const int nb1 = SWIGLU || TN == 128 ? nb0 : nb0 + 1;
-        const int nb = (lane & 4) ? (nb1 < a.NB ? nb1 : a.NB - 1) : nb0;
-        const float* ws = (SWIGLU && (lane & 4) ? a.ws_up : a.ws) + ((int64_t)t.e * a.NB + nb) * KB + (lane & 3);
+        const int nb = (lane & 8) ? (nb1 < a.NB ? nb1 : a.NB - 1) : nb0;
+        const float* ws = (SWIGLU && (lane & 8) ? a.ws_up : a.ws) + ((int64_t)t.e * a.NB + nb) * KB + (lane & 7);
         for (int kb = 0; kb < KB; kb += kSlotBlocks, sl.next()) {
-          float v[kSlotBlocks][4], w = 0.0f;
-#pragma unroll
-          for (int j = 0; j < kSlotBlocks; ++j)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int row = r0 + i * 32 + lane;
-              v[j][i] = kb + j < KB && row < t.row_end ? __ldg(a.xs + (int64_t)(kb + j) * a.xs_pitch + row) : 0.0f;
-            }
-          if (lane < 8 && kb + (lane & 3) < KB) w = __ldg(ws + kb);
           ok = warp_wait(&bars->sc_empty[sl.i], sl.phase ^ 1u, a.err, abort_flag, kSite + 6);
           if (!ok) break;
           ScaleSlot* s = slots + sl.i;
+          if (lane < 16) s->col[lane & 7][lane >> 3] = kb + (lane & 7) < KB ? __ldg(ws + kb) : 0.0f;
 #pragma unroll
-          for (int j = 0; j < kSlotBlocks; ++j)
+          for (int j0 = 0; j0 < kSlotBlocks; j0 += 4) {
+            float v[4][4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s->row[j][i * 32 + lane] = v[j][i];
-          if (lane < 8) s->col[lane & 3][lane >> 2] = w;
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int row = r0 + i * 32 + lane;
+                v[j][i] = kb + j0 + j < KB && row < t.row_end ? __ldg(a.xs + (int64_t)(kb + j0 + j) * a.xs_pitch + row) : 0.0f;
+              }
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) s->row[j0 + j][i * 32 + lane] = v[j][i];
+          }
           __syncwarp();
           if (lane == 0) mbar_arrive(&bars->sc_full[sl.i]);   // (release: the warp's stores are before it)
         }
@@ -336,20 +340,41 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsEpi));
     const int q = warp & 3, half = (warp - kEpiWarp0) >> 2;
     const uint32_t lane_base = (uint32_t)(q * 32) << 16;
-    const uint32_t empty_addr = mapa_u32(&bars->acc_empty[0], 0);
+    const uint32_t empty_addr = mapa_u32(&bars->acc_empty[half][0], 0);
     const int64_t pitch = (int64_t)a.N * (a.out_dtype == LMOE_DTYPE_F32 ? 4 : 2);
-    uint8_t* stage = store_stage + (warp - kEpiWarp0) * kStoreBytes;
-    constexpr int kChunks = C::kCols / 32;
-    // first column of chunk c in the tile: SwiGLU half of the gate's columns, then the same of up
-    auto column = [&](int c) {
-      if (!SWIGLU) return half * C::kCols + c * 32;
-      return c < kChunks / 2 ? half * (C::kHalf / 2) + c * 32
-                             : C::kHalf + half * (C::kHalf / 2) + (c - kChunks / 2) * 32;
-    };
+    uint8_t* stage = store_stage + (warp - kEpiWarp0) * C::kStoreBytes;
+    constexpr int kChunks = C::kCols / 32, kPart = kChunks / 2;
+    // first column of chunk c in the tile: the half's rows of the leader's, then of the follower's operand
+    auto column = [&](int c) { return c / kPart * C::kHalf + half * (C::kHalf / 2) + c % kPart * 32; };
     Ring<C::kAcc> ac;
     Ring<kSlots> sl;
-    int hint = 0;
+    int hint = 0, in_slot = 0;
+    float f0 = 0.0f, f1 = 0.0f;
     bool ok = true;
+    // Waits for the next block's sums and reads its factors.
+    auto next_block = [&]() {
+      if (in_slot == 0) ok = ok && mbar_wait(&bars->sc_full[sl.i], sl.phase, a.err, abort_flag, kSite + 7);
+      const ScaleSlot* s = slots + sl.i;
+      const float sx = s->row[in_slot][q * 32 + lane];
+      const float2 w = *reinterpret_cast<const float2*>(s->col[in_slot]);
+      f0 = __fmul_rn(sx, w.x);
+      f1 = __fmul_rn(sx, w.y);
+      ok = ok && mbar_wait(&bars->acc_full[half][ac.i], ac.phase, a.err, abort_flag, kSite + 8);
+      __syncwarp();
+      tc_fence_after();
+    };
+    // Gives the block's sums back, and its factors' slot.
+    auto pass_block = [&](bool last) {
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(empty_addr + ac.i * 8);
+      ac.next();
+      if (++in_slot == kSlotBlocks || last) {
+        if (lane == 0) mbar_arrive(&bars->sc_empty[sl.i]);
+        sl.next();
+        in_slot = 0;
+      }
+    };
     for (int tile = first; tile < total && ok; tile += stride) {
       const Fp8Tile t = fp8_tile_at(seg, a, tile, hint);
       const int row = t.row0 + (int)rank * kRowsCta + q * 32;   // the warp's first
@@ -358,56 +383,73 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int i = 0; i < C::kCols; ++i) acc[i] = 0.0f;
       if (!t.zero) {
-        for (int kb = 0; kb < KB && ok; ++kb) {
-          const int j = kb % kSlotBlocks;
-          if (j == 0) ok = warp_wait(&bars->sc_full[sl.i], sl.phase, a.err, abort_flag, kSite + 7);
-          if (ok) ok = warp_wait(&bars->acc_full[ac.i], ac.phase, a.err, abort_flag, kSite + 8);
-          if (!ok) break;
-          tc_fence_after();
-          if (rows > 0) {   // else the segment ends before this warp's rows
-            const ScaleSlot* s = slots + sl.i;
-            const float sx = s->row[j][q * 32 + lane];
-            const float f0 = __fmul_rn(sx, s->col[j][SWIGLU || TN == 128 ? 0 : half]);
-            const float f1 = SWIGLU ? __fmul_rn(sx, s->col[j][1]) : f0;
-            const uint32_t col = tmem + lane_base + ac.i * TN;
-            uint32_t r[2][32];
-            tmem_ld32_async(col + column(0), r[0]);
+        next_block();
+        if (rows <= 0) {   // the segment ends before this warp's rows
+          for (int left = KB; left > 0 && ok; --left) {
+            pass_block(left == 1);
+            if (left > 1) next_block();
+          }
+        } else {
+          // 32 columns at a time, the next ones (of the next block behind the last) on their way meanwhile
+          const uint32_t lanes = tmem + lane_base + half * C::kCols;
+          uint32_t r[2][32];
+          tmem_ld32_async(lanes + ac.i * TN, r[0]);
+          for (int left = KB; left > 0 && ok; --left) {
+            const uint32_t col = lanes + ac.i * TN;
+            const float g0 = f0, g1 = f1;
 #pragma unroll
             for (int c = 0; c < kChunks; ++c) {
               tmem_arrived(r[c & 1]);
-              if (c + 1 < kChunks) tmem_ld32_async(col + column(c + 1), r[(c + 1) & 1]);
-              add_scaled(acc + c * 32, r[c & 1], SWIGLU && c >= kChunks / 2 ? f1 : f0);
+              if (c + 1 < kChunks) {
+                tmem_ld32_async(col + (c + 1) * 32, r[(c + 1) & 1]);
+              } else {
+                pass_block(left == 1);
+                if (left > 1) {
+                  next_block();
+                  tmem_ld32_async(lanes + ac.i * TN, r[0]);
+                }
+              }
+              add_scaled(acc + c * 32, r[c & 1], c < kPart ? g0 : g1);
             }
           }
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(empty_addr + ac.i * 8);
-          ac.next();
-          if (j == kSlotBlocks - 1 || kb == KB - 1) {
-            if (lane == 0) mbar_arrive(&bars->sc_empty[sl.i]);
-            sl.next();
-          }
+          if (!ok) tmem_arrived(r[0]);   // (a load that was on its way when a wait gave up)
         }
         if (!ok) break;
       }
       if (rows <= 0) continue;
+      constexpr int kOut = SWIGLU ? kPart : kChunks;
+      if (SWIGLU) {
+#pragma unroll
+        for (int i = 0; i < C::kCols / 2; ++i) acc[i] = silu(acc[i]) * acc[C::kCols / 2 + i];
+      }
       uint8_t* out = static_cast<uint8_t*>(a.out) + (int64_t)row * pitch;
       const bool whole = rows == 32 && a.store != kStoreStaged;   // blocks leave by TMA
-      constexpr int kOut = SWIGLU ? kChunks / 2 : kChunks;
+      const int c0 = t.n * (SWIGLU ? C::kHalf : TN);
+      if (elect_one()) bulk_wait_read();   // of the last tile's stores
+      __syncwarp();
+      if (!whole) {
 #pragma unroll
-      for (int b = 0; b < kOut; ++b) {
-        float f[32];
+        for (int b = 0; b < kOut; ++b)
+          store_rows<32, C::kStoreBytes>(out, pitch, rows, c0 + column(b), a.N, reinterpret_cast<const float(&)[32]>(acc[b * 32]),
+                                         a.out_dtype, a.store, stage, lane);
+      } else if (a.out_dtype != LMOE_DTYPE_F32) {
+        // all blocks into shared memory, then out together
 #pragma unroll
-        for (int i = 0; i < 32; ++i)
-          f[i] = SWIGLU ? silu(acc[b * 32 + i]) * acc[(b + kOut) * 32 + i] : acc[b * 32 + i];
-        const int c = t.n * (SWIGLU ? C::kHalf : TN) + column(b);
-        if (c >= a.N) continue;
-        if (!whole) {
-          store_rows<32, kStoreBytes>(out, pitch, rows, c, a.N, f, a.out_dtype, a.store, stage, lane);
-        } else {
-          store_block<64>(&tm_out, f, a.out_dtype, stage, lane, c, row, 0);
-          if (a.out_dtype == LMOE_DTYPE_F32 && c + 16 < a.N)
-            store_block<64>(&tm_out, f + 16, a.out_dtype, stage, lane, c + 16, row, 0);
+        for (int b = 0; b < kOut; ++b) stage_block<64>(acc + b * 32, a.out_dtype, stage + b * 2048, lane);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (elect_one()) {
+#pragma unroll
+          for (int b = 0; b < kOut; ++b)
+            if (c0 + column(b) < a.N) tma_store_3d(&tm_out, stage + b * 2048, c0 + column(b), row, 0);
+          bulk_commit();
+        }
+        __syncwarp();
+      } else {
+#pragma unroll
+        for (int b = 0; b < 2 * kOut; ++b) {
+          const int c = c0 + column(b / 2) + b % 2 * 16;
+          if (c < a.N) store_block<64>(&tm_out, acc + b * 16, a.out_dtype, stage, lane, c, row, 0);
         }
       }
     }
@@ -427,9 +469,9 @@ template <int TN, bool SWIGLU>
 int launch(const CUtensorMap& x, const CUtensorMap& x32, const CUtensorMap& w, const CUtensorMap& up,
            const CUtensorMap& out, const Fp8Args& a, int grid, cudaStream_t stream) {
   auto fn = fp8_gemm_kernel<TN, SWIGLU>;
-  const int st = set_max_dynamic_smem(reinterpret_cast<const void*>(fn), smem_bytes<TN>());
+  const int st = set_max_dynamic_smem(reinterpret_cast<const void*>(fn), smem_bytes<Cfg<TN, SWIGLU>>());
   if (st != LMOE_OK) return st;
-  fn<<<grid, kThreads, smem_bytes<TN>(), stream>>>(x, x32, w, up, out, a);
+  fn<<<grid, kThreads, smem_bytes<Cfg<TN, SWIGLU>>(), stream>>>(x, x32, w, up, out, a);
   return cuda_status(cudaGetLastError());
 }
 
