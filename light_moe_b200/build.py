@@ -30,7 +30,7 @@ NVCC = os.path.join(CUDA_HOME, "bin", "nvcc")
 
 CU_SOURCES = ["host_util.cu", "router.cu", "quant.cu", "grouped_gemm.cu", "decode_gemm.cu", "simt_gemm.cu",
               "layer.cu", "dispatch.cu", "ep_p2p.cu", "fp4_quant.cu", "fp4_gemm.cu", "fp4_decode.cu",
-              "grad_gemm.cu", "grad_split.cu", "grad_f32.cu", "fp8_quant.cu", "fp8_gemm.cu", "few_tokens.cu"]
+              "grad_gemm.cu", "grad_split.cu", "grad_f32.cu", "fp8_quant.cu", "fp8_gemm.cu", "fp8_decode.cu", "few_tokens.cu"]
 HEADERS = ["ptx.cuh", "lmoe_math.cuh", "host_util.h", "w4_layout.cuh", "w4_dequant.cuh", "grouped_gemm.h",
            "decode_gemm.h", "pair_gemm.cuh", "fp4_format.cuh", "fp4_mma.cuh", "fp4_gemm.h", "grad_gemm.h",
            "grad_tile.cuh", "fp8_format.cuh", "fp8_gemm.h"]

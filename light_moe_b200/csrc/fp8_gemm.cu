@@ -37,8 +37,8 @@ constexpr int kEpiWarps = 8, kEpiWarp0 = 4, kThreads = (kEpiWarp0 + kEpiWarps) *
 constexpr int kTmemCols = 512;
 constexpr int kSlotBlocks = 8, kSlots = 3;   // a slot of the scales' ring holds eight blocks
 constexpr uint32_t kSite = 0x700u;
-// Registers: 384 threads x 168 at launch = 128 x 56 + 256 x 224.
-constexpr int kRegsLaunch = 168, kRegsOther = 56, kRegsEpi = 224;
+// Registers: 384 threads x 168 at launch = 128 x 72 + 256 x 216.
+constexpr int kRegsLaunch = 168, kRegsOther = 72, kRegsEpi = 216;
 static_assert(128 * kRegsOther + 256 * kRegsEpi <= kThreads * kRegsLaunch, "register split");
 
 template <int TN, bool SWIGLU>
@@ -112,19 +112,6 @@ __device__ __forceinline__ Fp8Tile fp8_tile_at(const SegTable& t, const Fp8Args&
   r.row0 = t.row[j] + r.m * kTM;
   r.row_end = t.row[j + 1];
   return r;
-}
-
-// Instruction descriptor of kind::f8f6f4: E4M3 operands, K-major, fp32 sums, M = 256, N = n.
-__host__ __device__ constexpr uint32_t idesc_fp8(uint32_t n) {
-  return (1u << 4) | ((n >> 3) << 17) | ((256u >> 4) << 24);
-}
-__device__ __forceinline__ void mma_fp8_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
-      : "memory");
 }
 
 // 32 columns of the thread's lane; the registers hold them after tmem_arrived.
@@ -316,17 +303,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           ScaleSlot* s = slots + sl.i;
           if (lane < 16) s->col[lane & 7][lane >> 3] = kb + (lane & 7) < KB ? __ldg(ws + kb) : 0.0f;
 #pragma unroll
-          for (int j0 = 0; j0 < kSlotBlocks; j0 += 4) {
-            float v[4][4];
+          for (int j0 = 0; j0 < kSlotBlocks; j0 += 2) {
+            float v[2][4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+            for (int j = 0; j < 2; ++j)
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 const int row = r0 + i * 32 + lane;
                 v[j][i] = kb + j0 + j < KB && row < t.row_end ? __ldg(a.xs + (int64_t)(kb + j0 + j) * a.xs_pitch + row) : 0.0f;
               }
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+            for (int j = 0; j < 2; ++j)
 #pragma unroll
               for (int i = 0; i < 4; ++i) s->row[j0 + j][i * 32 + lane] = v[j][i];
           }
@@ -390,29 +377,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             if (left > 1) next_block();
           }
         } else {
-          // 32 columns at a time, the next ones (of the next block behind the last) on their way meanwhile
+          // 32 columns at a time
           const uint32_t lanes = tmem + lane_base + half * C::kCols;
-          uint32_t r[2][32];
-          tmem_ld32_async(lanes + ac.i * TN, r[0]);
           for (int left = KB; left > 0 && ok; --left) {
             const uint32_t col = lanes + ac.i * TN;
             const float g0 = f0, g1 = f1;
 #pragma unroll
             for (int c = 0; c < kChunks; ++c) {
-              tmem_arrived(r[c & 1]);
-              if (c + 1 < kChunks) {
-                tmem_ld32_async(col + (c + 1) * 32, r[(c + 1) & 1]);
-              } else {
-                pass_block(left == 1);
-                if (left > 1) {
-                  next_block();
-                  tmem_ld32_async(lanes + ac.i * TN, r[0]);
-                }
-              }
-              add_scaled(acc + c * 32, r[c & 1], c < kPart ? g0 : g1);
+              uint32_t r[32];
+              tmem_ld32_async(col + c * 32, r);
+              tmem_arrived(r);
+              if (c == kChunks - 1) pass_block(left == 1);
+              add_scaled(acc + c * 32, r, c < kPart ? g0 : g1);
             }
+            if (left > 1) next_block();
           }
-          if (!ok) tmem_arrived(r[0]);   // (a load that was on its way when a wait gave up)
         }
         if (!ok) break;
       }
@@ -486,7 +465,9 @@ int run_fp8_gemm(const Fp8Problem& p, cudaStream_t stream) {
   const int grid = gemm_grid(dev) < 2 ? 2 : gemm_grid(dev) & ~1;   // whole pairs
   const int widths[2] = {256, 128};
   const int mats = swiglu ? 2 : 1;
-  const int tn = pick_width(widths, grid / 2, 0, 0, [&](int w) {
+  // A block of a narrow tile takes about four fifths of a wide one's time (8 experts of 2 x 14336 x 4096, 18 rows: 322 us
+  // with narrow tiles, 252 with wide ones; 16384 rows: 3090 against 2290), so they pay only where they save a round.
+  const int tn = pick_width(widths, grid / 2, 200, 0, [&](int w) {
     return even_row_tiles(p.total_rows, p.num_experts, kTM) * (((int64_t)p.N * mats + w - 1) / w);
   });
   Fp8Args a = {};
@@ -574,5 +555,10 @@ extern "C" int lmoe_fp8_grouped_gemm(const uint8_t* xq, const float* xs, int64_t
   p.out_dtype = out_dtype;
   p.out = output;
   p.err = error;
-  return run_fp8_gemm(p, stream);
+  // Few rows: tiles of 256 weight rows stream the weights best (us by rows per expert, that kernel against
+  // the other; 8 experts of 4096 x 14336: 1 93 against 132, 64 134 against 137, 96 172 against 137; of 2 x 14336 x 4096:
+  // 1 166 against 252, 64 189 against 255, 96 277 against 257; 64 of 2048 x 1408: 1 50 against 75, 64 73 against 77, 96 89
+  // against 77; of 2 x 1408 x 2048: 1 80 against 128, 64 110 against 131, 96 141 against 132).  Both give the same bits.  The counts are on
+  // the device, so the rule takes all rows.
+  return total_rows <= (int64_t)num_experts * kFp8DecodeRows ? run_fp8_decode(p, stream) : run_fp8_gemm(p, stream);
 }
