@@ -90,31 +90,42 @@ __device__ __forceinline__ uint4 encode16(const uint32_t (&w)[4 * sizeof(T)], fl
   float v[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) v[i] = to_float<T>(reinterpret_cast<const T*>(w)[i]);
-  return make_uint4(fp8_encode4(v, inv), fp8_encode4(v + 4, inv), fp8_encode4(v + 8, inv), fp8_encode4(v + 12, inv));
+  return fp8_encode16(v, inv);
 }
 
-// blockDim = (chunks of 16 columns, a multiple of 32; rows); grid.x walks the chunks, grid.y the rows.
+// blockDim = (chunks of 16 columns, a multiple of 32; rows); grid.x walks the chunks, grid.y the rows.  A
+// thread has kRows rows' loads in flight: with one (a CTA of a row of 4096 holds 8 KB, five CTAs an SM)
+// 8192 x 4096 bf16 took 39 us, bound by the loads' latency.
+template <typename T>
+constexpr int kRows = 2;
 template <typename T>
 __global__ void __launch_bounds__(256) quantize_fp8_rows_kernel(const Fp8RowArgs a) {
   const int chunk = blockIdx.x * blockDim.x + threadIdx.x;
   const bool ok = chunk < a.K / 16;
-  for (int64_t r = (int64_t)blockIdx.y * blockDim.y + threadIdx.y; r < a.rows; r += (int64_t)gridDim.y * blockDim.y) {
-    uint32_t w[4 * sizeof(T)], top = 0;
-    if (ok) {
-      load16<T>(static_cast<const T*>(a.x) + r * a.ldx + (int64_t)chunk * 16, a.vec, w);
-      top = top16<T>(w);
-    }
-    // all 32 lanes are of one row, eight of one block
+  const int64_t stride = (int64_t)gridDim.y * blockDim.y;
+  const T* x = static_cast<const T*>(a.x) + (int64_t)chunk * 16;
+  for (int64_t r0 = (int64_t)blockIdx.y * blockDim.y + threadIdx.y; r0 < a.rows; r0 += kRows<T> * stride) {
+    uint32_t w[kRows<T>][4 * sizeof(T)];
 #pragma unroll
-    for (int o = 1; o < 8; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (!ok) continue;
-    const float s = fp8_scale(top, a.power_of_two != 0);
-    const uint4 codes = encode16<T>(w, s);
-    for (int j = 0; j < a.copies; ++j) {
-      const int64_t o = a.positions ? (int64_t)__ldg(a.positions + r * a.copies + j) : r;
-      if (o < 0 || o >= a.out_rows) continue;
-      *reinterpret_cast<uint4*>(a.q + o * a.K + (int64_t)chunk * 16) = codes;
-      if ((chunk & 7) == 0) a.scales[(int64_t)(chunk >> 3) * a.pitch + o] = s;
+    for (int i = 0; i < kRows<T>; ++i)
+      if (ok && r0 + i * stride < a.rows) load16<T>(x + (r0 + i * stride) * a.ldx, a.vec, w[i]);
+#pragma unroll
+    for (int i = 0; i < kRows<T>; ++i) {
+      const int64_t r = r0 + i * stride;
+      if (r >= a.rows) break;
+      uint32_t top = ok ? top16<T>(w[i]) : 0u;
+      // all 32 lanes are of one row, eight of one block
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      if (!ok) continue;
+      const float s = fp8_scale(top, a.power_of_two != 0);
+      const uint4 codes = encode16<T>(w[i], s);
+      for (int j = 0; j < a.copies; ++j) {
+        const int64_t o = a.positions ? (int64_t)__ldg(a.positions + r * a.copies + j) : r;
+        if (o < 0 || o >= a.out_rows) continue;
+        *reinterpret_cast<uint4*>(a.q + o * a.K + (int64_t)chunk * 16) = codes;
+        if ((chunk & 7) == 0) a.scales[(int64_t)(chunk >> 3) * a.pitch + o] = s;
+      }
     }
   }
 }
@@ -203,27 +214,40 @@ template <typename T>
 __global__ void __launch_bounds__(256)
     dequantize_fp8_kernel(const uint8_t* __restrict__ q, const float* __restrict__ scales, Fp8ScaleStrides st,
                           int64_t rows, int64_t total_rows, int K, int block_shift, T* __restrict__ out) {
+  constexpr int kAhead = 4;   // rows whose loads are in flight
   const bool vec32 = (reinterpret_cast<uintptr_t>(out) & 31) == 0;   // K % 16 == 0: then every chunk
   const int chunk = blockIdx.x * blockDim.x + threadIdx.x;
   if (chunk >= K / 16) return;
-  for (int64_t r = (int64_t)blockIdx.y * blockDim.y + threadIdx.y; r < total_rows;
-       r += (int64_t)gridDim.y * blockDim.y) {
-    const uint4 c = __ldg(reinterpret_cast<const uint4*>(q + r * K + (int64_t)chunk * 16));
-    const int64_t mat = rows == total_rows ? 0 : r / rows, in = r - mat * rows;
-    const float s = __ldg(scales + mat * st.mat + (in >> block_shift) * st.row + (int64_t)(chunk >> 3) * st.block);
-    const uint32_t w[4] = {c.x, c.y, c.z, c.w};
-    float v[16];
+  const int64_t stride = (int64_t)gridDim.y * blockDim.y;
+  for (int64_t r0 = (int64_t)blockIdx.y * blockDim.y + threadIdx.y; r0 < total_rows; r0 += kAhead * stride) {
+    uint4 c[kAhead];
+    float s[kAhead];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t lo = e4m3x2_half2(w[i]), hi = e4m3x2_half2_high(w[i]);
-      const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&lo));
-      const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-      v[4 * i] = __fmul_rn(a.x, s);
-      v[4 * i + 1] = __fmul_rn(a.y, s);
-      v[4 * i + 2] = __fmul_rn(b.x, s);
-      v[4 * i + 3] = __fmul_rn(b.y, s);
+    for (int i = 0; i < kAhead; ++i) {
+      const int64_t r = r0 + i * stride;
+      if (r >= total_rows) break;
+      c[i] = __ldg(reinterpret_cast<const uint4*>(q + r * K + (int64_t)chunk * 16));
+      const int64_t mat = rows == total_rows ? 0 : r / rows, in = r - mat * rows;
+      s[i] = __ldg(scales + mat * st.mat + (in >> block_shift) * st.row + (int64_t)(chunk >> 3) * st.block);
     }
-    store16<T>(out + r * K + (int64_t)chunk * 16, v, vec32);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int64_t r = r0 + i * stride;
+      if (r >= total_rows) break;
+      const uint32_t w[4] = {c[i].x, c[i].y, c[i].z, c[i].w};
+      float v[16];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t lo = e4m3x2_half2(w[j]), hi = e4m3x2_half2_high(w[j]);
+        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&lo));
+        const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+        v[4 * j] = __fmul_rn(a.x, s[i]);
+        v[4 * j + 1] = __fmul_rn(a.y, s[i]);
+        v[4 * j + 2] = __fmul_rn(b.x, s[i]);
+        v[4 * j + 3] = __fmul_rn(b.y, s[i]);
+      }
+      store16<T>(out + r * K + (int64_t)chunk * 16, v, vec32);
+    }
   }
 }
 
@@ -231,13 +255,15 @@ struct RowGrid {
   dim3 grid, block;
 };
 
-RowGrid row_grid(int chunks, int64_t rows) {
+// CTAs for all SMs to hold a few at a time, no more than there are rows for.
+RowGrid row_grid(int chunks, int64_t rows, int sms) {
   const int bx = chunks >= 256 ? 256 : (chunks + 31) / 32 * 32;
   const int by = 256 / bx;
-  const int64_t gy = (rows + by - 1) / by;
+  const int64_t gx = (chunks + bx - 1) / bx, gy = (rows + by - 1) / by;
+  const int64_t most = (8 * (int64_t)sms + gx - 1) / gx;
   RowGrid g;
   g.block = dim3((unsigned)bx, (unsigned)by);
-  g.grid = dim3((unsigned)((chunks + bx - 1) / bx), (unsigned)(gy < 32768 ? gy : 32768));
+  g.grid = dim3((unsigned)gx, (unsigned)(gy < most ? gy : most));
   return g;
 }
 
@@ -258,8 +284,8 @@ void launch_blocks(const void* x, int64_t rows, int K, int vec, int power, uint8
 
 template <typename T>
 void launch_dequantize(const uint8_t* q, const float* scales, const Fp8ScaleStrides& st, int64_t count, int64_t rows,
-                       int K, int shift, void* out, cudaStream_t stream) {
-  const RowGrid g = row_grid(K / 16, count * rows);
+                       int K, int shift, void* out, int sms, cudaStream_t stream) {
+  const RowGrid g = row_grid(K / 16, count * rows, sms);
   dequantize_fp8_kernel<T><<<g.grid, g.block, 0, stream>>>(q, scales, st, rows, count * rows, K, shift,
                                                           static_cast<T*>(out));
 }
@@ -296,7 +322,10 @@ extern "C" int lmoe_quantize_fp8(const void* x, int dtype, int64_t rows, int K, 
   a.scales = scales;
   a.pitch = scale_pitch;
   a.vec = vector_bytes(x, ldx * esize);
-  const RowGrid g = row_grid((K / 16 + 7) / 8 * 8, rows);
+  DeviceInfo dev;
+  const int st = get_device_info(&dev);
+  if (st != LMOE_OK) return st;
+  const RowGrid g = row_grid((K / 16 + 7) / 8 * 8, rows, dev.num_sms);
   if (dtype == LMOE_DTYPE_BF16)
     quantize_fp8_rows_kernel<__nv_bfloat16><<<g.grid, g.block, 0, stream>>>(a);
   else if (dtype == LMOE_DTYPE_F16)
@@ -339,13 +368,16 @@ extern "C" int lmoe_dequantize_fp8(const uint8_t* q, const float* scales, int64_
   if (count == 0 || rows == 0) return LMOE_OK;
   LMOE_ARG_CHECK(q && scales && out && aligned16(out) && aligned16(q) &&
                  (reinterpret_cast<uintptr_t>(scales) & 3) == 0);
+  DeviceInfo dev;
+  const int status = get_device_info(&dev);
+  if (status != LMOE_OK) return status;
   const Fp8ScaleStrides st = {scale_mat_stride, scale_row_stride, scale_block_stride};
   const int shift = block_rows == 1 ? 0 : 7;
   if (out_dtype == LMOE_DTYPE_BF16)
-    launch_dequantize<__nv_bfloat16>(q, scales, st, count, rows, K, shift, out, stream);
+    launch_dequantize<__nv_bfloat16>(q, scales, st, count, rows, K, shift, out, dev.num_sms, stream);
   else if (out_dtype == LMOE_DTYPE_F16)
-    launch_dequantize<__half>(q, scales, st, count, rows, K, shift, out, stream);
+    launch_dequantize<__half>(q, scales, st, count, rows, K, shift, out, dev.num_sms, stream);
   else
-    launch_dequantize<float>(q, scales, st, count, rows, K, shift, out, stream);
+    launch_dequantize<float>(q, scales, st, count, rows, K, shift, out, dev.num_sms, stream);
   return cuda_status(cudaGetLastError());
 }
