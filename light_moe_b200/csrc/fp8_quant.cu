@@ -93,38 +93,50 @@ __device__ __forceinline__ uint4 encode16(const uint32_t (&w)[4 * sizeof(T)], fl
   return fp8_encode16(v, inv);
 }
 
-// blockDim = (chunks of 16 columns, a multiple of 32; rows); grid.x walks the chunks, grid.y the rows.  A
-// thread has kRows rows' loads in flight: with one (a CTA of a row of 4096 holds 8 KB, five CTAs an SM)
-// 8192 x 4096 bf16 took 39 us, bound by the loads' latency.
+// blockDim = (chunks of 16 * kParts columns, a multiple of 32; rows); grid.x walks the chunks, grid.y the rows.
+// A thread has two rows' loads in flight (with one 8192 x 4096 bf16 was bound by their latency), and of
+// 16-bit values 32 of a row, which spreads a block's scale, its reciprocals and the addresses.
 template <typename T>
+constexpr int kParts = sizeof(T) == 2 ? 2 : 1;
 constexpr int kRows = 2;
 template <typename T>
 __global__ void __launch_bounds__(256) quantize_fp8_rows_kernel(const Fp8RowArgs a) {
-  const int chunk = blockIdx.x * blockDim.x + threadIdx.x;
-  const bool ok = chunk < a.K / 16;
+  constexpr int P = kParts<T>, kLanes = 8 / P;   // of a block
+  const int chunk = blockIdx.x * blockDim.x + threadIdx.x, col = chunk * 16 * P;
   const int64_t stride = (int64_t)gridDim.y * blockDim.y;
-  const T* x = static_cast<const T*>(a.x) + (int64_t)chunk * 16;
-  for (int64_t r0 = (int64_t)blockIdx.y * blockDim.y + threadIdx.y; r0 < a.rows; r0 += kRows<T> * stride) {
-    uint32_t w[kRows<T>][4 * sizeof(T)];
+  const T* x = static_cast<const T*>(a.x) + col;
+  for (int64_t r0 = (int64_t)blockIdx.y * blockDim.y + threadIdx.y; r0 < a.rows; r0 += kRows * stride) {
+    uint32_t w[kRows][P][4 * sizeof(T)];
 #pragma unroll
-    for (int i = 0; i < kRows<T>; ++i)
-      if (ok && r0 + i * stride < a.rows) load16<T>(x + (r0 + i * stride) * a.ldx, a.vec, w[i]);
+    for (int i = 0; i < kRows; ++i)
 #pragma unroll
-    for (int i = 0; i < kRows<T>; ++i) {
+      for (int p = 0; p < P; ++p)
+        if (col + 16 * p < a.K && r0 + i * stride < a.rows)
+          load16<T>(x + (r0 + i * stride) * a.ldx + 16 * p, a.vec, w[i][p]);
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
       const int64_t r = r0 + i * stride;
       if (r >= a.rows) break;
-      uint32_t top = ok ? top16<T>(w[i]) : 0u;
-      // all 32 lanes are of one row, eight of one block
+      uint32_t top = 0u;
 #pragma unroll
-      for (int o = 1; o < 8; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-      if (!ok) continue;
+      for (int p = 0; p < P; ++p)
+        if (col + 16 * p < a.K) top = max(top, top16<T>(w[i][p]));
+      // all 32 lanes are of one row, kLanes of one block
+#pragma unroll
+      for (int o = 1; o < kLanes; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      if (col >= a.K) continue;
       const float s = fp8_scale(top, a.power_of_two != 0);
-      const uint4 codes = encode16<T>(w[i], s);
+      uint4 codes[P];
+#pragma unroll
+      for (int p = 0; p < P; ++p)
+        if (col + 16 * p < a.K) codes[p] = encode16<T>(w[i][p], s);
       for (int j = 0; j < a.copies; ++j) {
         const int64_t o = a.positions ? (int64_t)__ldg(a.positions + r * a.copies + j) : r;
         if (o < 0 || o >= a.out_rows) continue;
-        *reinterpret_cast<uint4*>(a.q + o * a.K + (int64_t)chunk * 16) = codes;
-        if ((chunk & 7) == 0) a.scales[(int64_t)(chunk >> 3) * a.pitch + o] = s;
+#pragma unroll
+        for (int p = 0; p < P; ++p)
+          if (col + 16 * p < a.K) *reinterpret_cast<uint4*>(a.q + o * a.K + col + 16 * p) = codes[p];
+        if ((chunk & (kLanes - 1)) == 0) a.scales[(int64_t)(chunk / kLanes) * a.pitch + o] = s;
       }
     }
   }
@@ -325,7 +337,8 @@ extern "C" int lmoe_quantize_fp8(const void* x, int dtype, int64_t rows, int K, 
   DeviceInfo dev;
   const int st = get_device_info(&dev);
   if (st != LMOE_OK) return st;
-  const RowGrid g = row_grid((K / 16 + 7) / 8 * 8, rows, dev.num_sms);
+  const int wide = dtype == LMOE_DTYPE_F32 ? 16 : 32;   // columns of a thread
+  const RowGrid g = row_grid((K + wide - 1) / wide, rows, dev.num_sms);
   if (dtype == LMOE_DTYPE_BF16)
     quantize_fp8_rows_kernel<__nv_bfloat16><<<g.grid, g.block, 0, stream>>>(a);
   else if (dtype == LMOE_DTYPE_F16)
