@@ -175,6 +175,26 @@ __device__ __forceinline__ uint32_t finite_top(uint32_t w) {
   return max(a < 0x7f800000u ? a : 0u, b < 0x7f800000u ? b : 0u);
 }
 
+__device__ __forceinline__ uint32_t cluster_ctarank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Shared-cluster address of `p` (an address of this CTA) in CTA `rank` of the cluster, and a load from there.
+__device__ __forceinline__ uint32_t mapa_u32(const void* p, uint32_t rank) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ float ld_cluster(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
 // The second kernel is launched while the first one runs: its CTAs start as the first one's leave
 // their SMs, and wait here for all of it.
 __device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
@@ -212,7 +232,7 @@ __host__ __device__ inline FewLayout few_layout(int d, int step, int group_token
 }
 
 template <bool FP8, typename X, int NT>
-__global__ void __launch_bounds__(kThreads, 1) gate_up_kernel(const FewArgs a) {
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gate_up_kernel(const FewArgs a) {
   using G = Geo<FP8>;
   using M = typename std::conditional<FP8, __half, X>::type;   // type of the products
   constexpr bool kScaled = FP8 && std::is_same<X, __nv_bfloat16>::value;
@@ -227,12 +247,17 @@ __global__ void __launch_bounds__(kThreads, 1) gate_up_kernel(const FewArgs a) {
   float* share = reinterpret_cast<float*>(smem + lay.share);     // [E + S][T]: routing weights
   constexpr int kRedRow = 8 * NT, kRedWarp = 16 * kRedRow, kRedBuf = kWarps * kRedWarp;
   float* logits = red + kRedBuf;   // [tokens of the group][256], while routing
-  static_assert((kJoins - 1) * kRedBuf >= 8 * NT * kMaxExperts, "room for the logits");
+  float* halves = logits + 8 * NT * kMaxExperts;   // a CTA's share of them
+  static_assert((kJoins - 1) * kRedBuf >= 2 * 8 * NT * kMaxExperts, "room for the logits");
   const int pieces = steps * G::kStep / 8;   // of a token; behind d: zeros
   launch_dependents();
 
-  // The router's weights are 16 experts a fragment; warps that have the same one share its steps.  The
-  // first two steps' loads start before the tokens are there.
+  // The router's weights are 16 experts a fragment; warps that have the same one share its steps, and with many
+  // experts the two CTAs of a pair do: all CTAs read them at the same time, which L2 feeds at its own rate (64
+  // experts of 2048: 9.7 us until the logits, XX us shared).  The first two steps' loads start before the tokens
+  // are there.
+  const uint32_t rank = cluster_ctarank();
+  const int shares = a.E > 16 ? 2 : 1, lead = shares == 2 ? (int)rank : 0;   // steps lead, lead + shares, ...
   const int mtiles = (a.E + 15) / 16;
   const int wpm = mtiles == 1 ? 16 : (mtiles == 2 ? 8 : (mtiles <= 4 ? 4 : (mtiles <= 8 ? 2 : 1)));
   const int e0 = warp / wpm * 16;
@@ -304,18 +329,19 @@ __global__ void __launch_bounds__(kThreads, 1) gate_up_kernel(const FewArgs a) {
   for (int t0 = 0; t0 < a.T; t0 += per_group) {
     const int n = a.T - t0 < per_group ? a.T - t0 : per_group;
     uint4 v[2][2][G::kPieces];
-    load_gate(warp % wpm, v[0][0], v[0][1]);
-    load_gate(warp % wpm + wpm, v[1][0], v[1][1]);
+    const int s_first = warp % wpm * shares + lead, s_step = wpm * shares;
+    load_gate(s_first, v[0][0], v[0][1]);
+    load_gate(s_first + s_step, v[1][0], v[1][1]);
     load_x(t0, n);
     float acc[NT][4];
 #pragma unroll
     for (int i = 0; i < NT; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
-    for (int s0 = warp % wpm; s0 < steps; s0 += 2 * wpm) {
+    for (int s0 = s_first; s0 < steps; s0 += 2 * s_step) {
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
-        const int s = s0 + b * wpm;
+        const int s = s0 + b * s_step;
         if (s >= steps) break;
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
@@ -331,7 +357,7 @@ __global__ void __launch_bounds__(kThreads, 1) gate_up_kernel(const FewArgs a) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) acc[i][j] += part[j];
         }
-        load_gate(s + 2 * wpm, v[b][0], v[b][1]);
+        load_gate(s + 2 * s_step, v[b][0], v[b][1]);
       }
     }
     float* mine = red + warp * kRedWarp;
@@ -341,16 +367,37 @@ __global__ void __launch_bounds__(kThreads, 1) gate_up_kernel(const FewArgs a) {
       *reinterpret_cast<float2*>(mine + (g + 8) * kRedRow + i * 8 + c * 2) = make_float2(acc[i][2], acc[i][3]);
     }
     __syncthreads();
+    if (shares == 2) {
+      for (int i = tid; i < n * a.E; i += kThreads) {
+        const int t = n == 1 ? 0 : i / a.E, e = i - t * a.E;
+        const float* r = red + (e >> 4) * wpm * kRedWarp + (e & 15) * kRedRow + t;
+        float sum = 0.0f;
+#pragma unroll 4
+        for (int w = 0; w < wpm; ++w) sum += r[w * kRedWarp];
+        halves[t * kMaxExperts + e] = sum;
+      }
+      cluster_sync();
+    }
     if (warp < n) {
       // One warp per token.  A pick is the best one behind the last pick, in the order of logits and ids
       // (little code: what runs once waits for its instructions).
       const int t = warp;
       float* mine_l = logits + t * kMaxExperts;
-      for (int e = lane; e < a.E; e += 32) {
+      auto sum_parts = [&](int e) {
         const float* r = red + (e >> 4) * wpm * kRedWarp + (e & 15) * kRedRow + t;
         float sum = 0.0f;
 #pragma unroll 4
         for (int w = 0; w < wpm; ++w) sum += r[w * kRedWarp];
+        return sum;
+      };
+      for (int e = lane; e < a.E; e += 32) {
+        float sum;
+        if (shares == 2) {   // the CTAs' halves, in the order of their ranks
+          const float mine = halves[t * kMaxExperts + e], other = ld_cluster(mapa_u32(&halves[t * kMaxExperts + e], rank ^ 1u));
+          sum = rank == 0 ? mine + other : other + mine;
+        } else {
+          sum = sum_parts(e);
+        }
         mine_l[e] = a.bias ? sum + __ldg(a.bias + e) : sum;
       }
       float top = 0.0f, sum = 0.0f, mine_p = 0.0f;
@@ -396,7 +443,10 @@ __global__ void __launch_bounds__(kThreads, 1) gate_up_kernel(const FewArgs a) {
     // the warps without a token meanwhile
     if (a.groups == 1) scale_x(n, n < kWarps ? n : 0);
     if (a.groups > 1 && tid < kMaxTokens) sh.top[tid] = 0u;
-    __syncthreads();
+    if (shares == 2)
+      cluster_sync();   // the other CTA has read this one's share
+    else
+      __syncthreads();
   }
 
   // ---- the used experts, and the warps of a tile: a power of two, each with a step at least.  Many balance
@@ -708,15 +758,18 @@ __global__ void __launch_bounds__(kThreads, 1) down_kernel(const FewArgs a) {
   const uint32_t step_bytes = (uint32_t)G::kPieces * T * 64;    // of one half
   const uint32_t half_bytes = step_bytes * a.chunk;
   const uint32_t piece_at = ((uint32_t)(sq % G::kPieces) * T + st) * 64 + sq / G::kPieces * 16;
-  // Piece q of token t in a step of the contraction; zeros where there is none.
+  // Piece q of token t in a step of the contraction, zeros behind the last feature; false where the token did
+  // not choose the expert: nobody looks there.
   auto fetch = [&](int step, int t, int q, float4& v0, float4& v1) {
     const int u = step / fsteps, kk = (step - u * fsteps) * G::kStep + q * 8;
+    if (!((tokens[u] >> t) & 1u)) return false;
     v0 = v1 = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (((tokens[u] >> t) & 1u) && kk < a.F) {
+    if (kk < a.F) {
       const float4* src = reinterpret_cast<const float4*>(a.h + ((int64_t)u * T + t) * a.F + kk);
       v0 = __ldcg(src);
       v1 = __ldcg(src + 1);
     }
+    return true;
   };
   auto put_piece = [&](uint8_t* dst, float scale, const float4& v0, const float4& v1) {
     const float v[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
@@ -742,28 +795,29 @@ __global__ void __launch_bounds__(kThreads, 1) down_kernel(const FewArgs a) {
     };
     auto ask = [&](int i, float4& x, float4& y) {
       const int r = i / kStepPieces;
-      fetch(begin + (T == 1 ? r : r / T), T == 1 ? 0 : r % T, i % kStepPieces, x, y);
+      return i < pieces && fetch(begin + (T == 1 ? r : r / T), T == 1 ? 0 : r % T, i % kStepPieces, x, y);
     };
     auto scale_of = [&](int i) { return pow2(range_exponent(top[T == 1 ? 0 : i / kStepPieces % T])); };
     float4 x, y;
-    if (tid < pieces) ask(tid, x, y);
+    const bool have = ask(tid, x, y);
     aim();
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) load(w0[j], w1[j], f[j]);
-    if (tid < pieces) put_piece(place(tid), scale_of(tid), x, y);
+    if (have) put_piece(place(tid), scale_of(tid), x, y);
 #pragma unroll 1
     for (int i0 = tid + kThreads; i0 < pieces; i0 += 4 * kThreads) {
       float4 v[4][2];
+      bool got[4];
+#pragma unroll
+      for (int m = 0; m < 4; ++m) got[m] = ask(i0 + m * kThreads, v[m][0], v[m][1]);
 #pragma unroll
       for (int m = 0; m < 4; ++m)
-        if (i0 + m * kThreads < pieces) ask(i0 + m * kThreads, v[m][0], v[m][1]);
-#pragma unroll
-      for (int m = 0; m < 4; ++m)
-        if (i0 + m * kThreads < pieces) put_piece(place(i0 + m * kThreads), scale_of(i0 + m * kThreads), v[m][0], v[m][1]);
+        if (got[m]) put_piece(place(i0 + m * kThreads), scale_of(i0 + m * kThreads), v[m][0], v[m][1]);
     }
   }
   __syncthreads();
   float4 v0, v1;
+  bool pending = false;   // v0, v1 hold a piece of the step before
 
   float acc[NT][4];
 #pragma unroll
@@ -784,8 +838,8 @@ __global__ void __launch_bounds__(kThreads, 1) down_kernel(const FewArgs a) {
         const int s = s0 + b;
         if (s >= n) break;
         if (stager) {
-          if (s > 0 && s - 1 < next) put_piece(other + (s - 1) * step_bytes + piece_at, sc, v0, v1);
-          if (s < next) fetch(at + n + s, st, sq, v0, v1);
+          if (pending) put_piece(other + (s - 1) * step_bytes + piece_at, sc, v0, v1);
+          pending = s < next && fetch(at + n + s, st, sq, v0, v1);
         }
         const uint32_t mask = tokens[u];
         const uint8_t* src = col + buf * buf_bytes + s * step_bytes;
@@ -817,7 +871,8 @@ __global__ void __launch_bounds__(kThreads, 1) down_kernel(const FewArgs a) {
       }
     }
     if (next > 0) {
-      if (stager && n - 1 < next) put_piece(other + (n - 1) * step_bytes + piece_at, sc, v0, v1);
+      if (pending) put_piece(other + (n - 1) * step_bytes + piece_at, sc, v0, v1);
+      pending = false;
       __syncthreads();
     }
   }
@@ -859,21 +914,29 @@ __global__ void __launch_bounds__(kThreads, 1) down_kernel(const FewArgs a) {
   }
   __syncthreads();
   if (!last) return;
-  for (int i = tid; i < T * kRowBlock; i += kThreads) {
-    const int t = i / kRowBlock, row = rb * kRowBlock + i % kRowBlock;
+  // four rows a thread, ten slices' loads at a time, added in order
+  for (int i = tid; i < T * kRowBlock / 4; i += kThreads) {
+    const int t = i / (kRowBlock / 4), row = rb * kRowBlock + i % (kRowBlock / 4) * 4;
     if (row >= a.d) continue;
     const float* src = a.part + (int64_t)t * a.d + row;
     const int64_t step = (int64_t)T * a.d;
-    float v = 0.0f;
+    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 1
-    for (int s0 = 0; s0 < slices; s0 += 16) {   // sixteen loads at a time, added in order
-      float p[16];
+    for (int s0 = 0; s0 < slices; s0 += 10) {
+      float4 p[10];
 #pragma unroll
-      for (int j = 0; j < 16; ++j) p[j] = s0 + j < slices ? __ldcg(src + (s0 + j) * step) : 0.0f;
+      for (int j = 0; j < 10; ++j)
+        p[j] = s0 + j < slices ? __ldcg(reinterpret_cast<const float4*>(src + (s0 + j) * step)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-      for (int j = 0; j < 16; ++j) v += p[j];
+      for (int j = 0; j < 10; ++j) {
+        v[0] += p[j].x;
+        v[1] += p[j].y;
+        v[2] += p[j].z;
+        v[3] += p[j].w;
+      }
     }
-    put(t, row, v);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) put(t, row + j, v[j]);
   }
 }
 
@@ -1005,7 +1068,8 @@ extern "C" int lmoe_moe_layer_few_tokens(const void* x, int dtype, int64_t num_t
   }
   const int blocks = (a.d + kRowBlock - 1) / kRowBlock;
   a.split = kSplitCtas / blocks > 1 ? kSplitCtas / blocks : 1;
-  a.grid1 = gemm_grid(dev) < kMaxCtas ? gemm_grid(dev) : kMaxCtas;
+  const int ctas = gemm_grid(dev) < kMaxCtas ? gemm_grid(dev) : kMaxCtas;
+  a.grid1 = ctas < 2 ? 2 : ctas & ~1;   // whole pairs
   const int grid2 = blocks * a.split;
   if (dtype == LMOE_DTYPE_BF16)
     return fp8 ? launch<true, __nv_bfloat16>(a, a.grid1, grid2, smem1, stream)
