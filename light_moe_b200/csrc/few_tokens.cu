@@ -55,7 +55,8 @@ constexpr int kRowBlock = kWarps * 16;   // output rows of a CTA of the second k
 constexpr int kSplitCtas = 148;  // CTAs that the second kernel's slices aim at: one per SM
 constexpr int kMaxCtas = 256;    // of the first kernel
 constexpr int kJoins = 4;        // tiles whose parts may wait to be joined
-constexpr uint32_t kStageBytes = 96 * 1024;   // of each of two buffers of hidden values at most
+constexpr uint32_t kStageBytes = 96 * 1024;    // of each of two buffers of hidden values
+constexpr uint32_t kWholeBytes = 200 * 1024;   // of a slice's hidden values that are staged at once at most
 constexpr uint32_t kSite = 0x800u;
 constexpr float kInf = __builtin_huge_valf();
 
@@ -963,10 +964,11 @@ template <bool FP8, typename X>
 int launch(FewArgs a, int grid1, int grid2, uint32_t smem1, cudaStream_t stream) {
   // the slices' hidden values whole, if they fit; else chunks of whole rounds of the buffers in flight
   const uint32_t step_bytes = (uint32_t)Geo<FP8>::kStep * a.T * 4;
-  a.chunk = (int)(kStageBytes / step_bytes) / kAhead * kAhead;
   const int used = (a.E < a.T * a.k ? a.E : a.T * a.k) + a.S;
   const int64_t most = ((int64_t)used * ((a.F + Geo<FP8>::kStep - 1) / Geo<FP8>::kStep) + a.split - 1) / a.split + 1;
-  const uint32_t smem2 = (most <= a.chunk ? 1 : 2) * a.chunk * step_bytes;
+  const bool whole = most * step_bytes <= kWholeBytes;
+  a.chunk = whole ? (int)most : (int)(kStageBytes / step_bytes) / kAhead * kAhead;
+  const uint32_t smem2 = (whole ? 1 : 2) * a.chunk * step_bytes;
   const bool two = a.T > 8 && a.groups == 1;
   auto k1 = two ? gate_up_kernel<FP8, X, 2> : gate_up_kernel<FP8, X, 1>;
   auto k2 = a.T <= 4 ? down_kernel<FP8, X, 0> : (a.T <= 8 ? down_kernel<FP8, X, 1> : down_kernel<FP8, X, 2>);
