@@ -50,7 +50,13 @@ namespace {
 constexpr int kWarps = 16, kThreads = kWarps * 32;
 constexpr int kMaxTokens = 16, kMaxExperts = 256, kMaxShared = 16, kMaxTopK = 16;
 constexpr int kMaxUsed = kMaxExperts + kMaxShared;
-constexpr int kAhead = 3;        // steps of weights in flight per warp
+// Steps of weights in flight per warp (4 of E4M3 cost registers: 85.5 us for 78.6, one token, 8 experts of 4096 x 14336).
+template <bool FP8>
+constexpr int kAheadOf = FP8 ? 3 : 4;
+// The second kernel's warps each read rows of their own, and ask for a few steps of a row at a time: 128 bytes here
+// and there open as many pages of the memory (4 tokens, bf16, the same layer: 130 us of it step by step, 112 so).
+template <bool FP8>
+constexpr int kBurstOf = FP8 ? 3 : 2;
 constexpr int kRowBlock = kWarps * 16;   // output rows of a CTA of the second kernel
 constexpr int kSplitCtas = 148;  // CTAs that the second kernel's slices aim at: one per SM
 constexpr int kMaxCtas = 256;    // of the first kernel
@@ -236,6 +242,7 @@ template <bool FP8, typename X, int NT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gate_up_kernel(const FewArgs a) {
   using G = Geo<FP8>;
   using M = typename std::conditional<FP8, __half, X>::type;   // type of the products
+  constexpr int kAhead = kAheadOf<FP8>;
   constexpr bool kScaled = FP8 && std::is_same<X, __nv_bfloat16>::value;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ FewShared sh;
@@ -686,6 +693,8 @@ __global__ void __launch_bounds__(kThreads, 1) down_kernel(const FewArgs a) {
   using G = Geo<FP8>;
   using M = typename std::conditional<FP8, __half, X>::type;
   constexpr int NT = MODE == 2 ? 2 : 1;
+  constexpr int kAhead = kAheadOf<FP8>, kBurst = kBurstOf<FP8>;
+  static_assert(kAhead % kBurst == 0, "whole bursts");
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int expert[kMaxUsed];
   __shared__ uint32_t tokens[kMaxUsed];
@@ -864,7 +873,10 @@ __global__ void __launch_bounds__(kThreads, 1) down_kernel(const FewArgs a) {
             acc[i][j] = FP8 ? fmaf(v, f[b], acc[i][j]) : acc[i][j] + v;
           }
         }
-        load(w0[b], w1[b], f[b]);
+        if (b % kBurst == kBurst - 1) {
+#pragma unroll
+          for (int j = b - kBurst + 1; j <= b; ++j) load(w0[j], w1[j], f[j]);
+        }
         if (++k == fsteps) {
           k = 0;
           ++u;
@@ -967,7 +979,7 @@ int launch(FewArgs a, int grid1, int grid2, uint32_t smem1, cudaStream_t stream)
   const int used = (a.E < a.T * a.k ? a.E : a.T * a.k) + a.S;
   const int64_t most = ((int64_t)used * ((a.F + Geo<FP8>::kStep - 1) / Geo<FP8>::kStep) + a.split - 1) / a.split + 1;
   const bool whole = most * step_bytes <= kWholeBytes;
-  a.chunk = whole ? (int)most : (int)(kStageBytes / step_bytes) / kAhead * kAhead;
+  a.chunk = whole ? (int)most : (int)(kStageBytes / step_bytes) / kAheadOf<FP8> * kAheadOf<FP8>;
   const uint32_t smem2 = (whole ? 1 : 2) * a.chunk * step_bytes;
   const bool two = a.T > 8 && a.groups == 1;
   auto k1 = two ? gate_up_kernel<FP8, X, 2> : gate_up_kernel<FP8, X, 1>;
