@@ -579,12 +579,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gate_up
     const uint8_t* xl = smem + lay.x + g * 64 + c * 16;
     int s = wi;
     bool ok = true;
+    // the tokens of a tile's expert: eight of them without one need no products
+    auto tokens_of = [&](int tile) { return tile < tiles ? sh.used_tokens[sh.list[sh.group[tile / ftiles]]] >> t0 : 0u; };
+    uint32_t with = NT > 1 ? tokens_of(first) : 0u;
     for (int tile = first; tile < tiles && ok;) {
 #pragma unroll
       for (int b = 0; b < kAhead; ++b) {
         if (tile >= tiles || !ok) break;
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
+          if (NT > 1 && !(with >> (8 * i) & 0xffu)) continue;
           // two chains of dependent products
           float part[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
           const bool has = i * 8 + g < n;
@@ -663,6 +667,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gate_up
           parity ^= 1u;
         }
         tile += stride;
+        if (NT > 1) with = tokens_of(tile);
       }
     }
 #pragma unroll
@@ -855,6 +860,7 @@ __global__ void __launch_bounds__(kThreads, 1) down_kernel(const FewArgs a) {
         const uint8_t* src = col + buf * buf_bytes + s * step_bytes;
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
+          if (NT > 1 && !(mask >> (8 * i) & 0xffu)) continue;
           float part[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
           const bool has = (mask >> (MODE == 0 ? g & 3 : i * 8 + g)) & 1u;
 #pragma unroll
