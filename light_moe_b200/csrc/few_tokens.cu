@@ -16,9 +16,11 @@
 // want its operands in shared memory, which costs more than it gives for 8 columns.  E4M3 values are
 // exact in fp16.
 //
-// Every expert that some token chose is multiplied with ALL tokens, since columns are free; results
-// of tokens that did not choose it are dropped.  So there is no permutation, and the second kernel
-// is one product over the contraction (expert, hidden feature) whose sum is the weighted combine.
+// An expert that some token chose is multiplied with a whole fragment of tokens, since columns are free: with up to 8
+// tokens the first kernel takes all of them and drops the results of those that did not choose the expert; with more,
+// and with more than 4 in the second kernel, the expert's own tokens are packed into the fragment's columns.  There is
+// no permutation, and the second kernel is one product over the contraction (expert, hidden feature) whose sum is the
+// weighted combine.
 //
 // 1. gate_up_kernel.  Every CTA computes the routing for itself (a few microseconds of L2 reads; a
 //    kernel of its own would cost more), then the CTAs share the tiles of 8 hidden features: rows 0-7
@@ -28,12 +30,17 @@
 // 2. down_kernel.  A CTA owns 256 output rows (a warp 16) and a slice of the contraction; the last
 //    CTA of a row block to finish adds the slices in their order, so the result does not depend on
 //    timing.  Hidden values enter the MMA as a sum of two 16-bit numbers (22 bits in fp16, 16 in bf16),
-//    which costs a second MMA but no weight traffic: rounding them to one would be an error as large
-//    as the output's own rounding.
+//    which cost columns of the MMA (4 tokens to one instead of 8) but no weight traffic: rounding them to one would be
+//    an error as large as the output's own rounding.
 //
-// fp16 operands need a range: tokens (bf16 times E4M3 weights) and hidden values are scaled by powers of
-// two, per token and per staged chunk, so that the largest lies in [2^14, 2^15); what is 2^-39 of it or
-// smaller is lost.
+// fp16 operands need a range: tokens (bf16 times E4M3 weights) and hidden values are scaled by powers of two, per token
+// (hidden values over all of its experts), so that the largest lies in [2^14, 2^15); what is 2^-39 of it or smaller is
+// lost.
+//
+// Measured, first / second kernel, us: one token, E4M3, 2 of 8 experts of 4096 x 14336: 49 / 27 (352 MB of weights:
+// 4.6 TB/s over both; the routing, the joins and the two kernels' ramps take 22 us); 4 tokens, bf16, of the same layer,
+// 1.93 GB: 226 / 103, 5.9 TB/s; 16 tokens, E4M3, all 8 experts, 1.41 GB: 230 / 160; one token, fp16, 2 of 8 experts of
+// 1024 x 2816: 12 / 9, which is latency: two launches, a router, three joins.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -53,16 +60,19 @@ constexpr int kMaxUsed = kMaxExperts + kMaxShared;
 // Steps of weights in flight per warp (4 of E4M3 cost registers: 85.5 us for 78.6, one token, 8 experts of 4096 x 14336).
 template <bool FP8>
 constexpr int kAheadOf = FP8 ? 3 : 4;
-// The second kernel's warps each read rows of their own, and ask for a few steps of a row at a time: 128 bytes here
-// and there open as many pages of the memory (4 tokens, bf16, the same layer: 130 us of it step by step, 112 so).
-template <bool FP8>
-constexpr int kBurstOf = FP8 ? 3 : 2;
+// The second kernel's warps each read rows of their own, and ask for two or three steps of a row at a time: 128
+// bytes here and there open as many pages of the memory (4 tokens, bf16, the same layer: 130 us of it step by
+// step, 112 so).
 constexpr int kRowBlock = kWarps * 16;   // output rows of a CTA of the second kernel
 constexpr int kSplitCtas = 148;  // CTAs that the second kernel's slices aim at: one per SM
 constexpr int kMaxCtas = 256;    // of the first kernel
 constexpr int kJoins = 4;        // tiles whose parts may wait to be joined
-constexpr uint32_t kStageBytes = 96 * 1024;    // of each of two buffers of hidden values
-constexpr uint32_t kWholeBytes = 200 * 1024;   // of a slice's hidden values that are staged at once at most
+// Hidden values in shared memory at a time: a slice's, if they fit kWholeBytes, else chunks of a multiple of
+// kChunkSteps steps in two buffers of kStageBytes (of 12 steps at least: 96 KB for 16 tokens).  What shared memory
+// takes is missing in L1, through which the weights' loads go: with 200 KB the second kernel read bf16 weights at 4.3
+// TB/s (149 us of 4 tokens, 8 experts of 4096 x 14336), so at 6.2 (103 us).
+constexpr int kChunkSteps = 12;
+constexpr uint32_t kStageBytes = 64 * 1024, kWholeBytes = 128 * 1024;
 constexpr uint32_t kSite = 0x800u;
 constexpr float kInf = __builtin_huge_valf();
 
@@ -90,6 +100,7 @@ struct FewArgs {
   int split;                 // slices of the second kernel
   int grid1;                 // CTAs of the first
   int chunk;                 // steps of hidden values that the second stages at a time
+  uint32_t sums_at;          // offset of its tokens' sums in shared memory
   void* y;
   int32_t* ids;
   float* weights;
@@ -221,6 +232,7 @@ struct FewShared {
   uint32_t htop[kMaxTokens];        // largest hidden values
   uint32_t top[kMaxTokens];         // largest absolute value of the group's tokens
   float unscale[kMaxTokens];
+  uint8_t column[kMaxUsed][kMaxTokens];   // of more than 8 tokens: those of an expert, one after the other
 };
 
 // Dynamic shared memory of the first kernel.
@@ -262,7 +274,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gate_up
 
   // The router's weights are 16 experts a fragment; warps that have the same one share its steps, and with many
   // experts the two CTAs of a pair do: all CTAs read them at the same time, which L2 feeds at its own rate (64
-  // experts of 2048: 9.7 us until the logits, XX us shared).  The first two steps' loads start before the tokens
+  // experts of 2048: 7 tokens 96 us replayed, 88.5 shared).  The first two steps' loads start before the tokens
   // are there.
   const uint32_t rank = cluster_ctarank();
   const int shares = a.E > 16 ? 2 : 1, lead = shares == 2 ? (int)rank : 0;   // steps lead, lead + shares, ...
@@ -471,6 +483,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gate_up
       if (used) {
         sh.list[at] = e;
         sh.group[at] = at;
+        if (NT > 1) {
+          uint32_t left = sh.used_tokens[e];
+          for (int j = 0; left; ++j, left &= left - 1u) sh.column[at][j] = (uint8_t)(__ffs(left) - 1);
+        }
       }
       n += __popc(m);
     }
@@ -576,23 +592,35 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gate_up
       for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
     // this lane's place in the tokens' fragments
     const uint32_t step_bytes = (uint32_t)G::kPieces * n * 64;
-    const uint8_t* xl = smem + lay.x + g * 64 + c * 16;
+    const uint8_t* xl = smem + lay.x + c * 16;
     int s = wi;
     bool ok = true;
-    // the tokens of a tile's expert: eight of them without one need no products
-    auto tokens_of = [&](int tile) { return tile < tiles ? sh.used_tokens[sh.list[sh.group[tile / ftiles]]] >> t0 : 0u; };
-    uint32_t with = NT > 1 ? tokens_of(first) : 0u;
+    // The tokens of this lane's columns.  Up to 8 tokens: column t is token t, whether it chose the expert or not;
+    // more: the expert's own one after the other, so that 8 or fewer of 16 take one product and not two.
+    int mine_of[NT], columns = n;
+    auto choose = [&](int tile) {
+#pragma unroll
+      for (int i = 0; i < NT; ++i) mine_of[i] = i * 8 + g;
+      if (NT > 1 && tile < tiles) {
+        const int u = tile / ftiles;   // (one group of tokens: sh.group is the identity)
+        columns = __popc(sh.used_tokens[sh.list[u]]);
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+          if (i * 8 + g < columns) mine_of[i] = sh.column[u][i * 8 + g];
+      }
+    };
+    choose(first);
     for (int tile = first; tile < tiles && ok;) {
 #pragma unroll
       for (int b = 0; b < kAhead; ++b) {
         if (tile >= tiles || !ok) break;
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
-          if (NT > 1 && !(with >> (8 * i) & 0xffu)) continue;
+          if (i > 0 && columns <= 8 * i) continue;
           // two chains of dependent products
           float part[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
-          const bool has = i * 8 + g < n;
-          const uint8_t* src = xl + s * step_bytes + i * 512;
+          const bool has = i * 8 + g < columns;
+          const uint8_t* src = xl + s * step_bytes + mine_of[i] * 64;
 #pragma unroll
           for (int p = 0; p < G::kPieces; ++p) {
             uint4 v = make_uint4(0u, 0u, 0u, 0u);
@@ -622,7 +650,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gate_up
         float* mine = parts + wi * kRedWarp;
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
-          if (i * 8 + c * 2 < n) {
+          if (i * 8 + c * 2 < columns) {
             *reinterpret_cast<float2*>(mine + g * kRedRow + i * 8 + c * 2) = make_float2(acc[i][0], acc[i][1]);
             *reinterpret_cast<float2*>(mine + (g + 8) * kRedRow + i * 8 + c * 2) = make_float2(acc[i][2], acc[i][3]);
           }
@@ -642,9 +670,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gate_up
           const int f = lane & 7;
 #pragma unroll
           for (int i = 0; i < 2 * NT; ++i) {
-            const int t = (lane >> 3) + 4 * i;
-            if (t < n && ((chosen >> t) & 1u)) {
-              const float* r = parts + f * kRedRow + t;
+            const int at = (lane >> 3) + 4 * i;   // column
+            const int t = NT > 1 && at < columns ? sh.column[u][at] : at;
+            if (at < columns && ((chosen >> t) & 1u)) {
+              const float* r = parts + f * kRedRow + at;
               float gate = 0.0f, up = 0.0f;
 #pragma unroll 4
               for (int w = 0; w < wpt; ++w) {
@@ -655,7 +684,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gate_up
               up *= sh.unscale[t];
               const float h = gate / (1.0f + expf(-gate)) * up * share[e * a.T + t0 + t];
               a.h[((int64_t)u * a.T + t0 + t) * a.F + ft * 8 + f] = h;
-              if (fabsf(h) < kInf) most[i] = fmaxf(most[i], fabsf(h));
+              if (NT > 1) {   // a column is another token with every expert
+                if (fabsf(h) < kInf && __float_as_uint(fabsf(h)) > sh.htop[t]) atomicMax(&sh.htop[t], __float_as_uint(fabsf(h)));
+              } else if (fabsf(h) < kInf) {
+                most[i] = fmaxf(most[i], fabsf(h));
+              }
             }
           }
           __syncwarp();
@@ -667,7 +700,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gate_up
           parity ^= 1u;
         }
         tile += stride;
-        if (NT > 1) with = tokens_of(tile);
+        if (NT > 1) choose(tile);
       }
     }
 #pragma unroll
@@ -692,18 +725,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gate_up
 // ---------------------------------------------------------------------------------------
 // second kernel
 // ---------------------------------------------------------------------------------------
-// MODE 0: up to 4 tokens, whose two halves are columns t and t + 4 of one MMA; 1: up to 8; 2: up to 16.
-template <bool FP8, typename X, int MODE>
+// The two halves of a token's hidden values are columns t and t + 4 of one MMA.  MODE 0: up to 4 tokens, whose
+// sums stay in registers for the whole slice.  MODE 1, 2 (up to 8, 16): of each expert the tokens that chose it, four
+// to an MMA, whose sums go to the tokens' own in shared memory at the expert's end (with all tokens in every
+// expert's columns, 16 tokens through 8 experts of 4096 x 14336 took this kernel 187 us, now 121).
+// CHUNKS: a slice's hidden values do not fit shared memory at once.
+template <bool FP8, typename X, int MODE, bool CHUNKS>
 __global__ void __launch_bounds__(kThreads, 1) down_kernel(const FewArgs a) {
   using G = Geo<FP8>;
   using M = typename std::conditional<FP8, __half, X>::type;
-  constexpr int NT = MODE == 2 ? 2 : 1;
-  constexpr int kAhead = kAheadOf<FP8>, kBurst = kBurstOf<FP8>;
-  static_assert(kAhead % kBurst == 0, "whole bursts");
+  constexpr int Q = MODE == 2 ? 4 : (MODE == 1 ? 2 : 1);   // MMAs of four tokens at most
+  constexpr int kAhead = FP8 && MODE == 2 ? 2 : kAheadOf<FP8>, kBurst = kAhead == 4 ? 2 : kAhead;   // (16 sums: no registers for 3)
+  static_assert(kChunkSteps % kAhead == 0, "a chunk starts at the first of the buffers in flight");
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int expert[kMaxUsed];
   __shared__ uint32_t tokens[kMaxUsed];
   __shared__ uint32_t top[kMaxTokens];
+  __shared__ uint8_t column[kMaxUsed][kMaxTokens];   // an expert's tokens, one after the other
   __shared__ int last;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   const int T = a.T;
@@ -713,7 +751,10 @@ __global__ void __launch_bounds__(kThreads, 1) down_kernel(const FewArgs a) {
   const int used = __ldcg(&a.head->used);
   for (int i = tid; i < a.E + a.S; i += kThreads) {   // (behind `used`: never looked at)
     expert[i] = __ldcg(&a.head->expert[i]);
-    tokens[i] = __ldcg(&a.head->tokens[i]);
+    const uint32_t who = __ldcg(&a.head->tokens[i]);
+    tokens[i] = who;
+    uint32_t left = who & 0xffffu;
+    for (int j = 0; left; ++j, left &= left - 1u) column[i][j] = (uint8_t)(__ffs(left) - 1);
   }
   for (int i = tid; i < a.grid1 * T; i += kThreads) {
     const uint32_t v = __ldcg(a.tops + i);
@@ -762,17 +803,11 @@ __global__ void __launch_bounds__(kThreads, 1) down_kernel(const FewArgs a) {
     }
   };
 
-  // Hidden values: of each step, a thread stages at most one piece of 8 values of a token, as two 16-bit
-  // numbers (of values scaled to at most 2^15).  The pieces of the next chunk's steps are loaded beside this
-  // chunk's products.
+  // Hidden values are staged as two 16-bit numbers (of values scaled to at most 2^15), in pieces of 8 of a token;
+  // those of the next chunk beside this chunk's products.
   constexpr int kStepPieces = G::kStep / 8;
-  const int piece = lane * kWarps + warp;
-  const int st = piece / kStepPieces, sq = piece % kStepPieces;
-  const bool stager = st < T;
-  const float sc = stager ? pow2(range_exponent(top[st])) : 0.0f;
   const uint32_t step_bytes = (uint32_t)G::kPieces * T * 64;    // of one half
   const uint32_t half_bytes = step_bytes * a.chunk;
-  const uint32_t piece_at = ((uint32_t)(sq % G::kPieces) * T + st) * 64 + sq / G::kPieces * 16;
   // Piece q of token t in a step of the contraction, zeros behind the last feature; false where the token did
   // not choose the expert: nobody looks there.
   auto fetch = [&](int step, int t, int q, float4& v0, float4& v1) {
@@ -831,47 +866,106 @@ __global__ void __launch_bounds__(kThreads, 1) down_kernel(const FewArgs a) {
     }
   }
   __syncthreads();
+  // One step of the next chunk at a time, its pieces (of the tokens that there are) over as many warps as they fill,
+  // other warps each step.
   float4 v0, v1;
-  bool pending = false;   // v0, v1 hold a piece of the step before
+  uint32_t to = 0;
+  float v_scale = 0.0f;
+  bool pending = false;   // v0, v1 hold a piece
+  int nu = 0, nk = 0;     // the next step to stage: expert, and step of it
+  auto put_next = [&](uint8_t* stage) {
+    if (pending) put_piece(stage + to, v_scale, v0, v1);
+    pending = false;
+  };
+  auto fetch_next = [&](int step) {   // of the chunk
+    const int first = ((warp + 5 * step) & (kWarps - 1)) * 32, piece = first + lane;
+    const int pieces = __popc(tokens[nu]) * kStepPieces;
+    if (first < pieces) {
+      if (piece < pieces) {
+        const int t = column[nu][piece / kStepPieces], q = piece % kStepPieces;
+        pending = fetch(nu * fsteps + nk, t, q, v0, v1);
+        to = step * step_bytes + ((uint32_t)(q % G::kPieces) * T + t) * 64 + q / G::kPieces * 16;
+        v_scale = pow2(range_exponent(top[t]));
+      }
+      __syncwarp();
+    }
+    if (++nk == fsteps) {
+      nk = 0;
+      ++nu;
+    }
+  };
 
-  float acc[NT][4];
+  float acc[Q][4];
 #pragma unroll
-  for (int i = 0; i < NT; ++i)
+  for (int i = 0; i < Q; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
-  // this lane's column: token, and (MODE 0) half
-  const uint8_t* col = smem + (MODE == 0 ? (g & 3) * 64 + (g >> 2) * half_bytes : g * 64) + c * 16;
+  // MODE 1, 2: the tokens' sums of this warp's rows, [token][16 rows]
+  float* sums = reinterpret_cast<float*>(smem + a.sums_at) + warp * 16 * T;
+  if (MODE != 0) {
+    for (int i = lane; i < 16 * T; i += 32) sums[i] = 0.0f;
+    __syncwarp();
+  }
+  // this lane's columns: tokens, and of each a half
+  const uint32_t half_at = (g >> 2) * half_bytes + c * 16;
   const uint32_t buf_bytes = 2 * half_bytes;
-  int u = begin / fsteps, k = begin - u * fsteps, buf = 0;
+  int u = begin / fsteps, k = begin - u * fsteps, buf = 0, columns = 0;
+  uint32_t from[Q];
+  bool has[Q];
+  auto choose = [&]() {   // of expert u
+    if (MODE == 0) return;
+    columns = __popc(tokens[u]);
+#pragma unroll
+    for (int i = 0; i < Q; ++i) {
+      const int at = 4 * i + (g & 3);
+      has[i] = at < columns;
+      from[i] = half_at + (has[i] ? column[u][at] : 0) * 64;
+    }
+  };
+  auto deliver = [&]() {   // the sums of expert u's tokens
+    if constexpr (MODE != 0) {
+#pragma unroll
+      for (int i = 0; i < Q; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float v = acc[i][j] + __shfl_xor_sync(0xffffffffu, acc[i][j], 2);   // columns t and t + 4
+          const int at = 4 * i + c * 2 + (j & 1);
+          if (c < 2 && at < columns) sums[column[u][at] * 16 + g + (j >> 1) * 8] += v;
+          acc[i][j] = 0.0f;
+        }
+      __syncwarp();
+    }
+  };
+  if (begin < end) choose();
   for (int at = begin; at < end; at += a.chunk, buf ^= 1) {
     const int n = end - at < a.chunk ? end - at : a.chunk;
     const int next = end - at - n < a.chunk ? end - at - n : a.chunk;   // steps of the next chunk
     uint8_t* other = smem + (buf ^ 1) * buf_bytes;
+    if (CHUNKS) {
+      nu = (at + n) / fsteps;
+      nk = at + n - nu * fsteps;
+    }
     for (int s0 = 0; s0 < n; s0 += kAhead) {
 #pragma unroll
       for (int b = 0; b < kAhead; ++b) {
         const int s = s0 + b;
         if (s >= n) break;
-        if (stager) {
-          if (pending) put_piece(other + (s - 1) * step_bytes + piece_at, sc, v0, v1);
-          pending = s < next && fetch(at + n + s, st, sq, v0, v1);
+        if (CHUNKS) {
+          put_next(other);
+          if (s < next) fetch_next(s);
         }
-        const uint32_t mask = tokens[u];
-        const uint8_t* src = col + buf * buf_bytes + s * step_bytes;
+        const uint32_t mask = MODE == 0 ? tokens[u] : 0u;
+        const uint8_t* src = smem + buf * buf_bytes + s * step_bytes;
 #pragma unroll
-        for (int i = 0; i < NT; ++i) {
-          if (NT > 1 && !(mask >> (8 * i) & 0xffu)) continue;
+        for (int i = 0; i < Q; ++i) {
+          if (i > 0 && columns <= 4 * i) continue;
           float part[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
-          const bool has = (mask >> (MODE == 0 ? g & 3 : i * 8 + g)) & 1u;
 #pragma unroll
           for (int p = 0; p < G::kPieces; ++p) {
-            uint4 hi = make_uint4(0u, 0u, 0u, 0u), lo = hi;
-            if (has) {
-              hi = *reinterpret_cast<const uint4*>(src + p * T * 64 + i * 512);
-              if (MODE != 0) lo = *reinterpret_cast<const uint4*>(src + p * T * 64 + i * 512 + half_bytes);
-            }
-            mma_piece<FP8, M>(part[MODE == 0 ? p & 1 : 0], w0[b], w1[b], p, hi);
-            if (MODE != 0) mma_piece<FP8, M>(part[1], w0[b], w1[b], p, lo);
+            uint4 v = make_uint4(0u, 0u, 0u, 0u);
+            if (MODE == 0 ? (mask >> (g & 3) & 1u) != 0u : has[i])
+              v = *reinterpret_cast<const uint4*>(src + p * T * 64 + (MODE == 0 ? half_at + (g & 3) * 64 : from[i]));
+            mma_piece<FP8, M>(part[p & 1], w0[b], w1[b], p, v);
           }
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -884,25 +978,18 @@ __global__ void __launch_bounds__(kThreads, 1) down_kernel(const FewArgs a) {
           for (int j = b - kBurst + 1; j <= b; ++j) load(w0[j], w1[j], f[j]);
         }
         if (++k == fsteps) {
+          deliver();
           k = 0;
-          ++u;
+          if (++u < used) choose();
         }
       }
     }
-    if (next > 0) {
-      if (pending) put_piece(other + (n - 1) * step_bytes + piece_at, sc, v0, v1);
-      pending = false;
+    if (CHUNKS && next > 0) {
+      put_next(other);
       __syncthreads();
     }
   }
-#pragma unroll
-  for (int i = 0; i < NT; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (MODE == 0) acc[i][j] += __shfl_xor_sync(0xffffffffu, acc[i][j], 2);   // columns t and t + 4
-      const int t = i * 8 + c * 2 + (j & 1);
-      acc[i][j] *= t < T ? pow2(-range_exponent(top[t])) : 0.0f;
-    }
+  if (k > 0) deliver();
 
   // ---- the slices' sum
   auto put = [&](int t, int row, float v) {
@@ -911,18 +998,22 @@ __global__ void __launch_bounds__(kThreads, 1) down_kernel(const FewArgs a) {
     else
       static_cast<__nv_bfloat16*>(a.y)[(int64_t)t * a.d + row] = __float2bfloat16_rn(v);
   };
-  if (rows_ok) {
+  auto give = [&](int t, int row, float v) {
+    v *= pow2(-range_exponent(top[t]));
+    if (slices == 1)
+      put(t, row, v);
+    else
+      a.part[((int64_t)slice * T + t) * a.d + row] = v;
+  };
+  if constexpr (MODE == 0) {
 #pragma unroll
-    for (int i = 0; i < NT; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int t = i * 8 + c * 2 + (j & 1), row = row0 + g + (j >> 1) * 8;
-        if (t >= T) continue;   // (MODE 0: the other half's columns too)
-        if (slices == 1)
-          put(t, row, acc[i][j]);
-        else
-          a.part[((int64_t)slice * T + t) * a.d + row] = acc[i][j];
-      }
+    for (int j = 0; j < 4; ++j) {
+      const float v = acc[0][j] + __shfl_xor_sync(0xffffffffu, acc[0][j], 2);   // columns t and t + 4
+      const int t = c * 2 + (j & 1);
+      if (rows_ok && c < 2 && t < T) give(t, row0 + g + (j >> 1) * 8, v);
+    }
+  } else if (rows_ok) {
+    for (int i = lane; i < 16 * T; i += 32) give(i >> 4, row0 + (i & 15), sums[i]);
   }
   if (slices == 1) return;
   __syncthreads();   // all parts are written before thread 0's release
@@ -933,7 +1024,7 @@ __global__ void __launch_bounds__(kThreads, 1) down_kernel(const FewArgs a) {
   }
   __syncthreads();
   if (!last) return;
-  // four rows a thread, ten slices' loads at a time, added in order
+  // four rows a thread, six slices' loads at a time, added in order
   for (int i = tid; i < T * kRowBlock / 4; i += kThreads) {
     const int t = i / (kRowBlock / 4), row = rb * kRowBlock + i % (kRowBlock / 4) * 4;
     if (row >= a.d) continue;
@@ -941,13 +1032,13 @@ __global__ void __launch_bounds__(kThreads, 1) down_kernel(const FewArgs a) {
     const int64_t step = (int64_t)T * a.d;
     float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 1
-    for (int s0 = 0; s0 < slices; s0 += 10) {
-      float4 p[10];
+    for (int s0 = 0; s0 < slices; s0 += 6) {
+      float4 p[6];
 #pragma unroll
-      for (int j = 0; j < 10; ++j)
+      for (int j = 0; j < 6; ++j)
         p[j] = s0 + j < slices ? __ldcg(reinterpret_cast<const float4*>(src + (s0 + j) * step)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-      for (int j = 0; j < 10; ++j) {
+      for (int j = 0; j < 6; ++j) {
         v[0] += p[j].x;
         v[1] += p[j].y;
         v[2] += p[j].z;
@@ -980,16 +1071,22 @@ FewWorkspace few_workspace(int T, int d, int F, int E, int k, int S) {
 
 template <bool FP8, typename X>
 int launch(FewArgs a, int grid1, int grid2, uint32_t smem1, cudaStream_t stream) {
-  // the slices' hidden values whole, if they fit; else chunks of whole rounds of the buffers in flight
   const uint32_t step_bytes = (uint32_t)Geo<FP8>::kStep * a.T * 4;
   const int used = (a.E < a.T * a.k ? a.E : a.T * a.k) + a.S;
   const int64_t most = ((int64_t)used * ((a.F + Geo<FP8>::kStep - 1) / Geo<FP8>::kStep) + a.split - 1) / a.split + 1;
   const bool whole = most * step_bytes <= kWholeBytes;
-  a.chunk = whole ? (int)most : (int)(kStageBytes / step_bytes) / kAheadOf<FP8> * kAheadOf<FP8>;
-  const uint32_t smem2 = (whole ? 1 : 2) * a.chunk * step_bytes;
+  const int fit = (int)(kStageBytes / step_bytes) / kChunkSteps * kChunkSteps;
+  a.chunk = whole ? (int)most : (fit > kChunkSteps ? fit : kChunkSteps);
+  a.sums_at = (whole ? 1 : 2) * a.chunk * step_bytes;
+  const uint32_t smem2 = a.sums_at + (a.T > 4 ? kWarps * 16 * a.T * 4 : 0);
   const bool two = a.T > 8 && a.groups == 1;
   auto k1 = two ? gate_up_kernel<FP8, X, 2> : gate_up_kernel<FP8, X, 1>;
-  auto k2 = a.T <= 4 ? down_kernel<FP8, X, 0> : (a.T <= 8 ? down_kernel<FP8, X, 1> : down_kernel<FP8, X, 2>);
+  auto k2 = whole ? (a.T <= 4   ? down_kernel<FP8, X, 0, false>
+                     : a.T <= 8 ? down_kernel<FP8, X, 1, false>
+                                : down_kernel<FP8, X, 2, false>)
+                  : (a.T <= 4   ? down_kernel<FP8, X, 0, true>
+                     : a.T <= 8 ? down_kernel<FP8, X, 1, true>
+                                : down_kernel<FP8, X, 2, true>);
   int st = set_max_dynamic_smem(reinterpret_cast<const void*>(k1), smem1);
   if (st != LMOE_OK) return st;
   st = set_max_dynamic_smem(reinterpret_cast<const void*>(k2), smem2);

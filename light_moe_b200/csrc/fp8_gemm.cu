@@ -11,18 +11,24 @@
 // tensor core, whose additions truncate.
 //
 // Tile: 256 rows (128 per CTA, TMEM lane = row) x 256 or 128 weight rows (half of them per CTA in
-// shared memory).  A block of 128 x 256 x 128 takes the tensor core 512 cycles; reading its sums
-// from tensor memory and adding them, 8 warps of 32 rows x 128 columns, about 260 each, beside the
-// next block's MMAs in the other half of tensor memory.  128 accumulators a thread: the epilogue's
-// two warpgroups take the registers that the other warps give up.
+// shared memory).  A block of 256 x 256 x 128 takes the pair's tensor cores 512 cycles.  Meanwhile 8 warps a CTA,
+// of 32 rows x 128 columns each, read the block before it from the other half of tensor memory and add it, and a
+// half of the columns goes back to its issuer as soon as its four warps have read it.  128 accumulators a thread:
+// the epilogue's two warpgroups take the registers that the other warps give up.
+//
+// What bounds it is that work, not the tensor core: a warp waits for the half, reads 4 x 32 columns, one load after
+// another since two in flight do not fit the registers, and issues 64 paired multiply-adds, and a block takes ~900
+// cycles in all.  16384 rows through 8 experts of 2 x 14336 x 4096, a call by itself: ~2.0 ms, 1.9 PFLOP/s, 0.58 of
+// twice the measured bf16 rate; call after call the power limit lowers the clock (2.39 ms).
 //
 // The lane being the row, a thread holds a row's gate and up values of the same features, and the
 // SwiGLU needs no exchange: the leader's half of the columns is gate rows and the follower's the
 // same rows of up.
 //
-// Warps: 0 TMA producer, whose copies complete on the leader's stage barrier; 1 MMA issuer (leader
-// CTA); 2 scales (both CTAs), which brings four blocks' scales at a time into a ring in shared
-// memory, coalesced because rows' scales are stored block after block; 4-11 the epilogue.
+// Warps: 0 TMA producer, whose copies complete on the leader's stage barrier; 1 and 3 MMA issuers
+// (leader CTA), one for each half of the columns, so that neither half waits for the other's readers;
+// 2 scales (both CTAs), which brings eight blocks' scales at a time into a ring in shared memory,
+// coalesced because rows' scales are stored block after block; 4-11 the epilogue.
 #include <cuda_bf16.h>
 
 #include "fp8_format.cuh"

@@ -158,6 +158,18 @@ def test_layer_of_tokens_in_two_groups(kind, T):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("T", [4, 5, 8, 9, 16])
+def test_layer_of_hidden_values_staged_in_chunks(kind, T):
+    """A slice of the second kernel has up to 66 steps of 128 hidden values (132 of 64) of T tokens at 4 bytes, more
+    than 128 KB, and its last step ends inside an expert's last 128."""
+    m = Layer(kind, 8192, 4128, 8, 4, seed=T, std=0.02)
+    # The logits' bound is 8192 * 2^-23 of the sum of absolute values, here about 8192 * 0.8 * (12 * 0.8 + 24) / 13 / 90
+    # = 190, so 0.19 on either side, while five gaps of eight normal logits of size 8 are often smaller: too few tokens
+    # have clear choices to demand half.  The choice is checked against the bound all the same.
+    m.check(m.x(T), exact_ids=False)
+
+
+@pytest.mark.parametrize("kind", KINDS)
 def test_ties_go_to_the_lower_id(kind):
     m = Layer(kind, 128, 64, 12, 3)
     m.gate[5] = m.gate[2]
