@@ -315,7 +315,7 @@ int lmoe_fp4_grouped_gemm(const uint8_t* xq, const uint8_t* xs, int64_t xs_pitch
 
 /* ------------------------------------------------------------------------------------ */
 /* 8-bit floating point (E4M3) with one fp32 scale per block of 128 columns: of one row        */
-/* (activations) or of 128 rows (weights).  The last blocks may be partial; K % 16 == 0.       */
+/* (activations) or of 128 rows (weights).  The last blocks may be partial; K % 16 == 0, at most 2^31 - 8208. */
 /*   s = max(max|x| / 448, 2^-126), or with power_of_two the next power of two; code = x / s to */
 /*   the nearest E4M3 value, ties to even; a block with an infinity or a NaN gets the scale NaN  */
 /*   and zero codes, so it reads as NaN.                                                        */

@@ -652,7 +652,7 @@ void check_block_rows(int64_t block_rows) {
   TORCH_CHECK(block_rows == 1 || block_rows == kFp8Block, "block_rows must be 1 or 128, is ", block_rows);
 }
 int64_t check_fp8_columns(int64_t K, const char* name) {
-  TORCH_CHECK(K > 0 && K % 16 == 0 && K <= INT32_MAX - 1024, name, ": K must be a positive multiple of 16");
+  TORCH_CHECK(K > 0 && K % 16 == 0 && K <= INT32_MAX - 8192, name, ": K must be a positive multiple of 16, at most 2^31 - 8208");
   return K;
 }
 

@@ -263,6 +263,9 @@ __global__ void __launch_bounds__(256)
   }
 }
 
+// Column indexes are counted in 32 bits, up to the end of a CTA's last chunks (256 threads of 32 columns).
+constexpr int kMaxColumns = INT32_MAX - 256 * 32;
+
 struct RowGrid {
   dim3 grid, block;
 };
@@ -314,7 +317,7 @@ extern "C" int lmoe_quantize_fp8(const void* x, int dtype, int64_t rows, int K, 
                                  int64_t scale_pitch, lmoe_stream_t stream_) {
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
   LMOE_ARG_CHECK(fp8_dtype(dtype));
-  LMOE_ARG_CHECK(rows >= 0 && K > 0 && K % 16 == 0 && ldx >= K && out_rows >= 0 && scale_pitch >= out_rows);
+  LMOE_ARG_CHECK(rows >= 0 && K > 0 && K % 16 == 0 && K <= kMaxColumns && ldx >= K && out_rows >= 0 && scale_pitch >= out_rows);
   LMOE_ARG_CHECK(positions ? copies >= 1 : (copies == 1 && out_rows == rows));
   if (rows == 0) return LMOE_OK;
   LMOE_ARG_CHECK(x && q && scales && aligned16(q) && (reinterpret_cast<uintptr_t>(scales) & 3) == 0);
@@ -352,7 +355,7 @@ extern "C" int lmoe_quantize_fp8_blocks(const void* x, int dtype, int64_t count,
                                         uint8_t* q, float* scales, lmoe_stream_t stream_) {
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
   LMOE_ARG_CHECK(fp8_dtype(dtype));
-  LMOE_ARG_CHECK(count >= 0 && rows >= 0 && rows <= INT32_MAX && K > 0 && K % 16 == 0);
+  LMOE_ARG_CHECK(count >= 0 && rows >= 0 && rows <= INT32_MAX - kFp8Block && K > 0 && K % 16 == 0 && K <= kMaxColumns);
   if (count == 0 || rows == 0) return LMOE_OK;
   LMOE_ARG_CHECK(x && q && scales && aligned16(q) && (reinterpret_cast<uintptr_t>(scales) & 3) == 0);
   const int64_t esize = dtype == LMOE_DTYPE_F32 ? 4 : 2;
@@ -376,7 +379,7 @@ extern "C" int lmoe_dequantize_fp8(const uint8_t* q, const float* scales, int64_
   cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
   LMOE_ARG_CHECK(fp8_dtype(out_dtype));
   LMOE_ARG_CHECK(block_rows == 1 || block_rows == kFp8Block);
-  LMOE_ARG_CHECK(count >= 0 && rows >= 0 && K > 0 && K % 16 == 0);
+  LMOE_ARG_CHECK(count >= 0 && rows >= 0 && K > 0 && K % 16 == 0 && K <= kMaxColumns);
   LMOE_ARG_CHECK(scale_mat_stride >= 0 && scale_row_stride >= 0 && scale_block_stride >= 0);
   if (count == 0 || rows == 0) return LMOE_OK;
   LMOE_ARG_CHECK(q && scales && out && aligned16(out) && aligned16(q) &&

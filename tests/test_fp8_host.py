@@ -35,8 +35,8 @@ def _rows(x=P, dtype=0, rows=4, K=64, ldx=64, p2=0, pos=None, copies=1, out_rows
 
 
 @pytest.mark.parametrize("bad", [
-    dict(dtype=3), dict(dtype=-1), dict(rows=-1), dict(K=40), dict(K=0), dict(ldx=63), dict(copies=2),
-    dict(out_rows=5), dict(out_rows=-1), dict(pos=P, copies=0), dict(pitch=3), dict(x=None), dict(q=None),
+    dict(K=2 ** 31 - 8192, ldx=2 ** 31), dict(dtype=3), dict(dtype=-1), dict(rows=-1), dict(K=40), dict(K=0),
+    dict(ldx=63), dict(copies=2), dict(out_rows=5), dict(out_rows=-1), dict(pos=P, copies=0), dict(pitch=3), dict(x=None), dict(q=None),
     dict(s=None), dict(q=P + 8), dict(x=P + 1), dict(s=P + 2), dict(pos=P + 2),
 ])
 def test_quantize_rows_refusals(bad):
@@ -48,8 +48,8 @@ def _blocks(x=P, dtype=0, count=2, rows=4, K=64, p2=0, q=P, s=P):
 
 
 @pytest.mark.parametrize("bad", [
-    dict(dtype=3), dict(count=-1), dict(rows=-1), dict(rows=2 ** 31), dict(K=24), dict(K=0), dict(x=None),
-    dict(q=None), dict(s=None), dict(q=P + 4), dict(x=P + 1), dict(s=P + 1),
+    dict(K=2 ** 31 - 16), dict(rows=2 ** 31 - 16), dict(dtype=3), dict(count=-1), dict(rows=-1), dict(rows=2 ** 31),
+    dict(K=24), dict(K=0), dict(x=None), dict(q=None), dict(s=None), dict(q=P + 4), dict(x=P + 1), dict(s=P + 1),
 ])
 def test_quantize_blocks_refusals(bad):
     assert _blocks(**bad) == INVALID
@@ -60,8 +60,8 @@ def _deq(q=P, s=P, sm=4, sr=1, sb=4, count=1, rows=4, K=64, block=1, dtype=0, ou
 
 
 @pytest.mark.parametrize("bad", [
-    dict(dtype=3), dict(block=2), dict(block=0), dict(count=-1), dict(rows=-1), dict(K=8), dict(K=0), dict(sm=-1),
-    dict(sr=-1), dict(sb=-1), dict(q=None), dict(s=None), dict(out=None), dict(q=P + 1), dict(out=P + 8), dict(s=P + 2),
+    dict(K=2 ** 31 - 16), dict(dtype=3), dict(block=2), dict(block=0), dict(count=-1), dict(rows=-1), dict(K=8), dict(K=0),
+    dict(sm=-1), dict(sr=-1), dict(sb=-1), dict(q=None), dict(s=None), dict(out=None), dict(q=P + 1), dict(out=P + 8), dict(s=P + 2),
 ])
 def test_dequantize_refusals(bad):
     assert _deq(**bad) == INVALID
