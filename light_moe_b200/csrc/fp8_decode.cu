@@ -12,6 +12,9 @@
 // column: the scales' warp multiplies the two and leaves a block's 64 factors in shared memory, from where
 // every thread reads them as broadcasts.
 //
+// Bound by HBM: 18 rows, 8 experts of 2 x 14336 x 4096, 943 MB in 154 us (6.1 TB/s; tiles of rows 252 us); 128 uneven
+// rows, 8 of 4096 x 14336, 473 MB in 93 us, two rounds of 128 tiles on 74 pairs.
+//
 // Warps: 0 TMA producer, whose copies complete on the leader's stage barrier; 1 MMA issuer (leader
 // CTA); 2 scales; 4-11 the epilogue (lane quarter x half of the columns).
 #include <cuda_bf16.h>

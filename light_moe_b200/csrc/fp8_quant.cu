@@ -3,8 +3,11 @@
 // Rows: a thread owns 16 consecutive values and eight threads a block of 128 columns, whose largest
 // absolute value they find with three shuffles on the bit patterns (which order like the values
 // and put infinities and NaN on top).  Matrices: a CTA holds a block of 128 x 128 in registers, so
-// that the values are read once.  Both are bound by HBM.  Row scales are stored block after block
-// ([K blocks][rows], rows padded to four): the product reads a block's scales of 128 rows at a time.
+// that the values are read once.  Row scales are stored block after block ([K blocks][rows], rows padded
+// to four): the product reads a block's scales of 128 rows at a time.
+//
+// Matrices are bound by HBM (64 x 1408 x 2048 fp32 there and back 304 us, 1.85 GB: 6.1 TB/s); rows of 16-bit values by the
+// instructions of the exact rounding (32768 x 4096 bf16: 113 us, 3.6 TB/s).  Back, 8192 x 4096 to bf16: 16-20 us.
 #include <cuda_bf16.h>
 
 #include <type_traits>

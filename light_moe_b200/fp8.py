@@ -20,9 +20,9 @@ from .layer import HostBufferCalls
 
 # Batches of at most FEW_TOKENS tokens, of a hidden size up to FEW_TOKENS_HIDDEN (where 8 tokens fit shared
 # memory), take the few-token kernels.  Replayed, us, those against the kernels for larger batches: 8 experts of
-# 4096 / 14336, two a token: 1 token 84 against 111, 4 180 against 198, 8 274 against 245, 12 455 against 257; 64 of 2048 / 1408, six
-# a token and two shared: 1 41 against 77, 8 95 against 123, 12 157 against 129; 8 of 1024 / 2816: 8 40 against 52, 12 58 against
-# 52.
+# 4096 / 14336, two a token: 1 token 82 against 111, 4 173 against 196, 8 248 against 244, 12 357 against 257; 64 of 2048 /
+# 1408, six a token and two shared: 1 38 against 76, 8 97 against 124, 12 149 against 129; 8 of 1024 / 2816: 8 41 against
+# 50, 12 54 against 52.
 FEW_TOKENS, FEW_TOKENS_HIDDEN = 8, 8192
 
 
