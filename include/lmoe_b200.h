@@ -367,7 +367,8 @@ int lmoe_fp8_grouped_gemm(const uint8_t* xq, const float* xs, int64_t xs_pitch, 
  * of its largest hidden value over all of its experts (fp16 products) are lost.
  * hidden_size % 64 == 0, at most 16384; ffn_size % 32 == 0, at most 65536; num_experts <= 256, top_k <= 16,
  * num_shared <= 16; LMOE_ERR_UNSUPPORTED where eight tokens of that hidden size do not fit shared memory
- * (from about 11000 on for eight).  The result does not depend on timing.  The workspace
+ * (from about 11000 on for eight).  The result does not depend on timing; should a bounded wait of the kernels ever run
+ * out, y is NaN.  The workspace
  * (lmoe_few_tokens_workspace_bytes; 0 for sizes that are refused), 16-byte aligned, need not be cleared;
  * calls that may run at the same time need one each. */
 size_t lmoe_few_tokens_workspace_bytes(int64_t num_tokens, int hidden_size, int ffn_size, int num_experts, int top_k,

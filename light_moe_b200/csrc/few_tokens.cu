@@ -743,12 +743,14 @@ __global__ void __launch_bounds__(kThreads, 1) down_kernel(const FewArgs a) {
   __shared__ uint32_t top[kMaxTokens];
   __shared__ uint8_t column[kMaxUsed][kMaxTokens];   // an expert's tokens, one after the other
   __shared__ int last;
+  __shared__ uint32_t failed;   // a wait of the first kernel ran out: the output is NaN
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   const int T = a.T;
   if (tid < kMaxTokens) top[tid] = 0u;
   __syncthreads();
   wait_for_launcher();
   const int used = __ldcg(&a.head->used);
+  if (tid == 0) failed = __ldcg(&a.head->error);
   for (int i = tid; i < a.E + a.S; i += kThreads) {   // (behind `used`: never looked at)
     expert[i] = __ldcg(&a.head->expert[i]);
     const uint32_t who = __ldcg(&a.head->tokens[i]);
@@ -999,7 +1001,7 @@ __global__ void __launch_bounds__(kThreads, 1) down_kernel(const FewArgs a) {
       static_cast<__nv_bfloat16*>(a.y)[(int64_t)t * a.d + row] = __float2bfloat16_rn(v);
   };
   auto give = [&](int t, int row, float v) {
-    v *= pow2(-range_exponent(top[t]));
+    v = failed ? __uint_as_float(0x7fc00000u) : v * pow2(-range_exponent(top[t]));
     if (slices == 1)
       put(t, row, v);
     else

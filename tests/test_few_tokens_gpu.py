@@ -158,6 +158,16 @@ def test_layer_of_tokens_in_two_groups(kind, T):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("T", [9, 16])
+@pytest.mark.parametrize("E,k", [(17, 3), (130, 16)])
+def test_layer_of_two_groups_and_shared_router_weights(kind, T, E, k):
+    """Tokens in two groups, and experts enough for pairs of CTAs to share the router's weights.  (Most tokens have two
+    logits closer than the bound of 8192 products: the choice is checked against the bound.)"""
+    m = Layer(kind, 8192, 64, E, k, 2, bias=True, seed=T + E, std=0.02)
+    m.check(m.x(T), exact_ids=False)
+
+
+@pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("T", [4, 5, 8, 9, 16])
 def test_layer_of_hidden_values_staged_in_chunks(kind, T):
     """A slice of the second kernel has up to 66 steps of 128 hidden values (132 of 64) of T tokens at 4 bytes, more
