@@ -9,7 +9,8 @@
 // round to the same code that is the code.  Where they differ, by one step, x is compared with the
 // midpoint times s, whose difference a fused multiply-add gives exactly.  That is no rare case: 3/4 of a
 // block's largest value (and 3/8, 3/16 ...) is such a midpoint, 336 of 448, and one in 128 of 16-bit values;
-// with a division there, 32768 x 4096 bf16 values took 170 us instead of 121.
+// with a division there, 32768 x 4096 bf16 values took 170 us instead of 121, and as below, without
+// any comparison, 78.
 #pragma once
 #include <cstdint>
 #include <cuda_fp16.h>
@@ -59,7 +60,20 @@ struct Fp8Inverse {
   }
 };
 
+// For values of at most 11 significant bits no comparison is needed.  Where s = rn(max / 448) is no power of two, a
+// value x and a midpoint m (5 bits) either have 448 x = m max, or differ by more than 2^-16, integers of at most 16
+// bits; then s, which is within 2^-24 of max / 448, does not change their order.  Where they are equal, x / s lies
+// above m (in size) if 448 s < max, below if 448 s > max, and is m if they are equal: the same for the whole block.
+// So a reciprocal that is 2^-17 too large, too small or neither, and products rounded to 18 bits (midpoints stay, and
+// what is 2^-16 away stays on its side), give the code.  With a power of two the products are exact.
+__device__ __forceinline__ float fp8_inverse16(float scale, float top) {
+  const float r = __frcp_rn(scale), rest = __fmaf_rn(-kFp8Top, scale, top);   // (exact)
+  if ((__float_as_uint(scale) & 0x007fffffu) == 0 || rest == 0.0f) return r;
+  return __fmul_rn(r, rest > 0.0f ? 1.0f + 0x1p-17f : 1.0f - 0x1p-17f);
+}
+
 // Codes of four values times r, the first in the lowest byte (two products to an instruction).
+template <bool SNAP = false>
 __device__ __forceinline__ uint32_t fp8_scaled4(const float* x, float r) {
   float p[4];
 #pragma unroll
@@ -68,6 +82,9 @@ __device__ __forceinline__ uint32_t fp8_scaled4(const float* x, float r) {
         "mov.b64 {%0, %1}, a;\n\t}"
         : "=f"(p[2 * i]), "=f"(p[2 * i + 1])
         : "f"(x[2 * i]), "f"(x[2 * i + 1]), "f"(r));
+  if constexpr (SNAP)   // 18 significant bits
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p[i] = __uint_as_float((__float_as_uint(p[i]) + 0x20u) & ~0x3fu);
   return cvt_e4m3x4(p[0], p[1], p[2], p[3]);
 }
 
@@ -109,6 +126,11 @@ __device__ __forceinline__ uint4 fp8_encode16(const float (&x)[16], const Fp8Inv
     if (a[i] != b) a[i] = fp8_between4(a[i], b, x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3], v.s);
   }
   return make_uint4(a[0], a[1], a[2], a[3]);
+}
+// Of values of 16-bit types; r from fp8_inverse16.
+__device__ __forceinline__ uint4 fp8_encode16(const float (&x)[16], float r) {
+  return make_uint4(fp8_scaled4<true>(x, r), fp8_scaled4<true>(x + 4, r), fp8_scaled4<true>(x + 8, r),
+                    fp8_scaled4<true>(x + 12, r));
 }
 
 }  // namespace lmoe

@@ -6,8 +6,8 @@
 // that the values are read once.  Row scales are stored block after block ([K blocks][rows], rows padded
 // to four): the product reads a block's scales of 128 rows at a time.
 //
-// Matrices are bound by HBM (64 x 1408 x 2048 fp32 there and back 304 us, 1.85 GB: 6.1 TB/s); rows of 16-bit values by the
-// instructions of the exact rounding (32768 x 4096 bf16: 113 us, 3.6 TB/s).  Back, 8192 x 4096 to bf16: 16-20 us.
+// Matrices are bound by HBM (64 x 1408 x 2048 fp32 there and back 304 us, 1.85 GB: 6.1 TB/s), and so
+// are large calls of rows (32768 x 4096 bf16: 78 us, 5.2 TB/s; 8192 rows 25).  Back, 8192 x 4096 to bf16: 16-20 us.
 #include <cuda_bf16.h>
 
 #include <type_traits>
@@ -87,13 +87,15 @@ __device__ __forceinline__ uint32_t top16(const uint32_t (&w)[4 * sizeof(T)]) {
   }
 }
 template <typename T>
-__device__ __forceinline__ uint4 encode16(const uint32_t (&w)[4 * sizeof(T)], float s) {
+__device__ __forceinline__ uint4 encode16(const uint32_t (&w)[4 * sizeof(T)], float s, uint32_t top) {
   if (!(s == s)) return make_uint4(0u, 0u, 0u, 0u);
-  const Fp8Inverse inv(s);
   float v[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) v[i] = to_float<T>(reinterpret_cast<const T*>(w)[i]);
-  return fp8_encode16(v, inv);
+  if constexpr (sizeof(T) == 2)
+    return fp8_encode16(v, fp8_inverse16(s, __uint_as_float(top)));
+  else
+    return fp8_encode16(v, Fp8Inverse(s));
 }
 
 // blockDim = (chunks of 16 * kParts columns, a multiple of 32; rows); grid.x walks the chunks, grid.y the rows.
@@ -132,7 +134,7 @@ __global__ void __launch_bounds__(256) quantize_fp8_rows_kernel(const Fp8RowArgs
       uint4 codes[P];
 #pragma unroll
       for (int p = 0; p < P; ++p)
-        if (col + 16 * p < a.K) codes[p] = encode16<T>(w[i][p], s);
+        if (col + 16 * p < a.K) codes[p] = encode16<T>(w[i][p], s, top);
       for (int j = 0; j < a.copies; ++j) {
         const int64_t o = a.positions ? (int64_t)__ldg(a.positions + r * a.copies + j) : r;
         if (o < 0 || o >= a.out_rows) continue;
@@ -183,7 +185,7 @@ __global__ void __launch_bounds__(kBlockThreads)
     const float s = fp8_scale(top, power_of_two != 0);
 #pragma unroll
     for (int i = 0; i < 2; ++i)
-      if (ok[i]) *reinterpret_cast<uint4*>(q + at[i]) = encode16<T>(w[i], s);
+      if (ok[i]) *reinterpret_cast<uint4*>(q + at[i]) = encode16<T>(w[i], s, top);
     if (tid == 0) scales[b] = s;
   }
 }

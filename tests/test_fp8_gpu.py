@@ -91,6 +91,20 @@ def test_quantize_many_bit_patterns(seed):
     _check(near)
 
 
+@pytest.mark.parametrize("dt,bits,up", [("bf16", 8, 1.0), ("bf16", 8, 2.0 ** 100), ("bf16", 8, 2.0 ** -110), ("fp16", 11, 16.0)])
+def test_quantize_16_bit_neighbours_of_every_midpoint(dt, bits, up):
+    """Blocks of every significand of the largest value, and around each midpoint times the scale the type's values."""
+    tops = np.arange(2 ** (bits - 1), 2 ** bits) * up
+    mid = (ref.GRID[1:] + ref.GRID[:-1]) / 2
+    near = torch.from_numpy(np.outer(tops / 448, mid)).float().to(DT[dt])
+    top = torch.from_numpy(tops).float().to(DT[dt])[:, None]
+    for step in (-1, 0, 1):   # (positive: the next patterns are the next values)
+        v = (near.view(torch.int16) + step).view(DT[dt]).clamp(min=0)
+        x = torch.cat([top, torch.minimum(v, top), -top], 1).cuda()
+        assert x.shape[1] == 128
+        _check(x)
+
+
 @pytest.mark.parametrize("block_rows", [1, 128])
 def test_quantize_extremes(block_rows):
     x = torch.zeros(8, 256, device="cuda")
