@@ -7,7 +7,7 @@
 // to four): the product reads a block's scales of 128 rows at a time.
 //
 // Matrices are bound by HBM (64 x 1408 x 2048 fp32 there and back 304 us, 1.85 GB: 6.1 TB/s), and so
-// are large calls of rows (32768 x 4096 bf16: 78 us, 5.2 TB/s; 8192 rows 25).  Back, 8192 x 4096 to bf16: 16-20 us.
+// are large calls of rows (32768 x 4096 bf16: 71 us, 5.7 TB/s; 8192 rows 22.5).  Back, 8192 x 4096 to bf16: 16-20 us.
 #include <cuda_bf16.h>
 
 #include <type_traits>
@@ -99,27 +99,29 @@ __device__ __forceinline__ uint4 encode16(const uint32_t (&w)[4 * sizeof(T)], fl
 }
 
 // blockDim = (chunks of 16 * kParts columns, a multiple of 32; rows); grid.x walks the chunks, grid.y the rows.
-// A thread has two rows' loads in flight (with one 8192 x 4096 bf16 was bound by their latency), and of
-// 16-bit values 32 of a row, which spreads a block's scale, its reciprocals and the addresses.
+// Of 16-bit values a thread takes 32 of a row, which spreads a block's scale, its reciprocal and the addresses (32768 x
+// 4096 bf16: 86 us with 16), and one row at a time (72 us, with two 80); of fp32 16 of two rows, whose loads are in flight
+// together (115 us, with one row 117).
 template <typename T>
 constexpr int kParts = sizeof(T) == 2 ? 2 : 1;
-constexpr int kRows = 2;
+template <typename T>
+constexpr int kRows = sizeof(T) == 2 ? 1 : 2;
 template <typename T>
 __global__ void __launch_bounds__(256) quantize_fp8_rows_kernel(const Fp8RowArgs a) {
-  constexpr int P = kParts<T>, kLanes = 8 / P;   // of a block
+  constexpr int P = kParts<T>, R = kRows<T>, kLanes = 8 / P;   // of a block
   const int chunk = blockIdx.x * blockDim.x + threadIdx.x, col = chunk * 16 * P;
   const int64_t stride = (int64_t)gridDim.y * blockDim.y;
   const T* x = static_cast<const T*>(a.x) + col;
-  for (int64_t r0 = (int64_t)blockIdx.y * blockDim.y + threadIdx.y; r0 < a.rows; r0 += kRows * stride) {
-    uint32_t w[kRows][P][4 * sizeof(T)];
+  for (int64_t r0 = (int64_t)blockIdx.y * blockDim.y + threadIdx.y; r0 < a.rows; r0 += R * stride) {
+    uint32_t w[R][P][4 * sizeof(T)];
 #pragma unroll
-    for (int i = 0; i < kRows; ++i)
+    for (int i = 0; i < R; ++i)
 #pragma unroll
       for (int p = 0; p < P; ++p)
         if (col + 16 * p < a.K && r0 + i * stride < a.rows)
           load16<T>(x + (r0 + i * stride) * a.ldx + 16 * p, a.vec, w[i][p]);
 #pragma unroll
-    for (int i = 0; i < kRows; ++i) {
+    for (int i = 0; i < R; ++i) {
       const int64_t r = r0 + i * stride;
       if (r >= a.rows) break;
       uint32_t top = 0u;
