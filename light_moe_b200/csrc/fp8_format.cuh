@@ -106,11 +106,11 @@ static __device__ __noinline__ uint32_t fp8_between4(uint32_t lo, uint32_t hi, f
     const uint32_t l2 = h ? e4m3x2_half2_high(lo) : e4m3x2_half2(lo), h2 = h ? e4m3x2_half2_high(hi) : e4m3x2_half2(hi);
     const float2 l = __half22float2(*reinterpret_cast<const __half2*>(&l2));
     const float2 u = __half22float2(*reinterpret_cast<const __half2*>(&h2));
-    const float sums[2] = {l.x + u.x, l.y + u.y};   // twice the midpoints (of equal codes: no matter)
+    const float mid[2] = {0.5f * (l.x + u.x), 0.5f * (l.y + u.y)};   // exact: five bits (of equal codes: no matter)
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int at = 2 * h + i;
-      const float rest = __fmaf_rn(-sums[i], s, 2.0f * x[at]);
+      const float rest = __fmaf_rn(-mid[i], s, x[at]);   // (twice x may be infinite)
       const bool beyond = rest != 0.0f ? (rest < 0.0f) == (x[at] < 0.0f) : (lo >> (8 * at) & 1u) != 0u;   // ties to even
       if (beyond) step |= 0xffu << (8 * at);
     }

@@ -74,6 +74,28 @@ def test_quantize_ties_and_borders(unit):
     _check(x, 1, True)
 
 
+@pytest.mark.parametrize("block_rows", [1, 128])
+@pytest.mark.parametrize("top", [63 * 2.0 ** 122, 1.8e38, 3.0e38, 3.4028234663852886e38])
+def test_quantize_ties_and_borders_at_the_end_of_fp32(top, block_rows):
+    """Midpoints, codes and their fp32 neighbours in blocks whose values' doubles are infinite."""
+    s = float(ref.scale(np.array([top]))[0])
+    t = torch.from_numpy(np.concatenate([(ref.GRID[1:] + ref.GRID[:-1]) / 2, ref.GRID]) * s).clamp(max=top).float()
+    v = [t]
+    for way in (0.0, 3.4028234663852886e38):
+        u = t
+        for _ in range(2):
+            u = torch.nextafter(u, torch.full_like(t, way))
+            v.append(u)
+    v = torch.cat(v).clamp(max=top)
+    v = torch.cat([v, -v])
+    n = -(-len(v) // 127)
+    v = torch.cat([v, torch.zeros(n * 127 - len(v))]).view(n, 127)
+    x = torch.cat([torch.full((n, 1), top), v], 1).cuda()
+    assert (x.abs() >= 2.0 ** 127).any() and torch.isfinite(x).all()
+    _check(x, block_rows)
+    _check(x, block_rows, True)
+
+
 @pytest.mark.parametrize("seed", range(4))
 def test_quantize_many_bit_patterns(seed):
     """fp32 values of every magnitude, and 16-bit values in blocks of every top: quotients near borders."""
