@@ -971,6 +971,8 @@ __global__ void __launch_bounds__(kThreads, 1) down_kernel(const FewArgs a) {
           }
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
+            // (MODE 0: a token without the expert gets nothing, where zero times an infinite weight would be NaN)
+            if (MODE == 0 && (mask >> ((c * 2 + (j & 1)) & 3) & 1u) == 0u) continue;
             const float v = part[0][j] + part[1][j];
             acc[i][j] = FP8 ? fmaf(v, f[b], acc[i][j]) : acc[i][j] + v;
           }

@@ -212,6 +212,27 @@ def test_a_token_that_is_not_finite_spoils_only_itself(kind, bad):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("T", [2, 3, 4, 5, 8, 9, 16])
+@pytest.mark.parametrize("which", [0, 1, 2])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_weights_that_are_not_finite_spoil_only_their_experts_tokens(kind, T, which, bad):
+    """An infinite or NaN weight, or a block's scale (NaN where the quantiser met such a weight)."""
+    m = Layer(kind, 256, 160, 6, 2, seed=T)
+    x = m.x(T)
+    want = m(x)
+    hits = [(want[1] == e).any(1) for e in range(m.E)]
+    e = next(i for i in range(m.E) if hits[i].any() and not hits[i].all())
+    if m.scales:
+        list(m.scales.values())[which][e, -1, -1] = bad
+    else:
+        m.w[which][e, -3, -5] = bad
+    y, ids, w = m(x)
+    assert torch.equal(ids, want[1]) and torch.equal(w, want[2])
+    assert torch.equal(y[~hits[e]], want[0][~hits[e]])
+    assert not torch.isfinite(y[hits[e]]).all(1).any()
+
+
+@pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("size", [1e-30, 1e-6, 1e3, 1e25])
 def test_values_of_other_sizes(kind, size):
     """Tokens and weights far from 1 (where the type holds them)."""
