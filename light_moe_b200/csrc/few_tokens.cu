@@ -443,7 +443,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gate_up
         last = (int)__reduce_min_sync(0xffffffffu, key == last_key ? (unsigned)at : (unsigned)kMaxExperts);
         l = __shfl_sync(0xffffffffu, l, last & 31);
         if (j == 0) top = l;
-        const float p = l == top ? 1.0f : (l == l ? softmax_exp(l - top) : l);
+        // (a NaN, and what has no softmax: nothing but -inf, or +inf)
+        const float p = l == l && fabsf(top) < kInf ? softmax_exp(l - top) : __uint_as_float(0x7fc00000u);
         sum += p;
         if (lane == j) {
           mine_p = p;

@@ -233,6 +233,28 @@ def test_weights_that_are_not_finite_spoil_only_their_experts_tokens(kind, T, wh
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("E", [4, 40])
+@pytest.mark.parametrize("T", [1, 5, 16])
+def test_a_router_whose_bias_leaves_no_expert(kind, E, T):
+    """A softmax over nothing but -inf, or with +inf, has no value; experts masked by -inf among others weigh nothing."""
+    m = Layer(kind, 128, 64, E, 3, bias=True, seed=E + T)
+    x = m.x(T)
+    m.bias[1:] = -float("inf")
+    y, ids, w = m(x)
+    assert (ids[:, 0] == 0).all() and (w[:, 0] == 1).all() and (w[:, 1:] == 0).all()
+    assert torch.isfinite(y).all()
+    for value in (-float("inf"), float("inf")):
+        m.bias.fill_(value)
+        y, ids, w = m(x)
+        assert torch.isnan(w).all() and torch.isnan(y).all()
+        assert all(len(set(r)) == 3 and min(r) >= 0 and max(r) < E for r in ids.tolist())
+    m.bias.zero_()
+    m.bias[2] = float("inf")
+    y, ids, w = m(x)
+    assert (ids[:, 0] == 2).all() and torch.isnan(w).all() and torch.isnan(y).all()
+
+
+@pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("size", [1e-30, 1e-6, 1e3, 1e25])
 def test_values_of_other_sizes(kind, size):
     """Tokens and weights far from 1 (where the type holds them)."""
