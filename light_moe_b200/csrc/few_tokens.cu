@@ -64,7 +64,7 @@ constexpr int kAheadOf = FP8 ? 3 : 4;
 // bytes here and there open as many pages of the memory (4 tokens, bf16, the same layer: 130 us of it step by
 // step, 112 so).
 constexpr int kRowBlock = kWarps * 16;   // output rows of a CTA of the second kernel
-constexpr int kSplitCtas = 148;  // CTAs that the second kernel's slices aim at: one per SM
+constexpr int kSplitCtas = 148;  // CTAs that the second kernel's slices aim at: one per SM, whatever the limit of CTAs
 constexpr int kMaxCtas = 256;    // of the first kernel
 constexpr int kJoins = 4;        // tiles whose parts may wait to be joined
 // Hidden values in shared memory at a time: a slice's, if they fit kWholeBytes, else chunks of a multiple of
@@ -99,6 +99,7 @@ struct FewArgs {
   int groups;                // token groups of the first kernel
   int split;                 // slices of the second kernel
   int grid1;                 // CTAs of the first
+  int item0;                 // row block and slice of the second kernel's first CTA
   int chunk;                 // steps of hidden values that the second stages at a time
   uint32_t sums_at;          // offset of its tokens' sums in shared memory
   void* y;
@@ -767,7 +768,7 @@ __global__ void __launch_bounds__(kThreads, 1) down_kernel(const FewArgs a) {
   const int fsteps = (a.F + G::kStep - 1) / G::kStep;
   const int total = used * fsteps;
   const int slices = a.split < total ? a.split : total;
-  const int rb = blockIdx.x / a.split, slice = blockIdx.x % a.split;
+  const int item = a.item0 + blockIdx.x, rb = item / a.split, slice = item % a.split;
   if (slice >= slices) return;
   const int begin = (int)((int64_t)total * slice / slices), end = (int)((int64_t)total * (slice + 1) / slices);
   const int row0 = rb * kRowBlock + warp * 16;
@@ -1075,7 +1076,7 @@ FewWorkspace few_workspace(int T, int d, int F, int E, int k, int S) {
 }
 
 template <bool FP8, typename X>
-int launch(FewArgs a, int grid1, int grid2, uint32_t smem1, cudaStream_t stream) {
+int launch(FewArgs a, int items, int ctas, bool limited, uint32_t smem1, cudaStream_t stream) {
   const uint32_t step_bytes = (uint32_t)Geo<FP8>::kStep * a.T * 4;
   const int used = (a.E < a.T * a.k ? a.E : a.T * a.k) + a.S;
   const int64_t most = ((int64_t)used * ((a.F + Geo<FP8>::kStep - 1) / Geo<FP8>::kStep) + a.split - 1) / a.split + 1;
@@ -1096,19 +1097,25 @@ int launch(FewArgs a, int grid1, int grid2, uint32_t smem1, cudaStream_t stream)
   if (st != LMOE_OK) return st;
   st = set_max_dynamic_smem(reinterpret_cast<const void*>(k2), smem2);
   if (st != LMOE_OK) return st;
-  k1<<<grid1, kThreads, smem1, stream>>>(a);
+  k1<<<a.grid1, kThreads, smem1, stream>>>(a);
   LMOE_CUDA_TRY(cudaGetLastError());
   cudaLaunchAttribute early = {};
   early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   early.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t config = {};
-  config.gridDim = dim3((unsigned)grid2);
   config.blockDim = dim3(kThreads);
   config.dynamicSmemBytes = smem2;
   config.stream = stream;
   config.attrs = &early;
-  config.numAttrs = 1;
-  return cuda_status(cudaLaunchKernelEx(&config, k2, a));
+  // One launch (items <= SMs).  Under a limit of CTAs several, each behind the other and the first behind the first kernel,
+  // whose CTAs hold the limit's SMs: the slices, and with them the order of the sums, stay the same.
+  config.numAttrs = limited ? 0 : 1;
+  for (a.item0 = 0; a.item0 < items; a.item0 += ctas) {
+    config.gridDim = dim3((unsigned)(items - a.item0 < ctas ? items - a.item0 : ctas));
+    LMOE_CUDA_TRY(cudaLaunchKernelEx(&config, k2, a));
+    config.numAttrs = 0;
+  }
+  return LMOE_OK;
 }
 
 bool few_sizes(int64_t T, int d, int F, int E, int k, int S) {
@@ -1192,10 +1199,11 @@ extern "C" int lmoe_moe_layer_few_tokens(const void* x, int dtype, int64_t num_t
   a.split = kSplitCtas / blocks > 1 ? kSplitCtas / blocks : 1;
   const int ctas = gemm_grid(dev) < kMaxCtas ? gemm_grid(dev) : kMaxCtas;
   a.grid1 = ctas < 2 ? 2 : ctas & ~1;   // whole pairs
-  const int grid2 = blocks * a.split;
+  const int items = blocks * a.split;
+  const bool limited = gemm_grid(dev) < dev.num_sms;
   if (dtype == LMOE_DTYPE_BF16)
-    return fp8 ? launch<true, __nv_bfloat16>(a, a.grid1, grid2, smem1, stream)
-               : launch<false, __nv_bfloat16>(a, a.grid1, grid2, smem1, stream);
-  return fp8 ? launch<true, __half>(a, a.grid1, grid2, smem1, stream)
-             : launch<false, __half>(a, a.grid1, grid2, smem1, stream);
+    return fp8 ? launch<true, __nv_bfloat16>(a, items, ctas, limited, smem1, stream)
+               : launch<false, __nv_bfloat16>(a, items, ctas, limited, smem1, stream);
+  return fp8 ? launch<true, __half>(a, items, ctas, limited, smem1, stream)
+             : launch<false, __half>(a, items, ctas, limited, smem1, stream);
 }

@@ -362,6 +362,47 @@ def test_under_a_limit_of_ctas():
     assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+def _grids(call):
+    """Grid sizes of the kernels that a captured call launches."""
+    from cuda.bindings import driver
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(graph):
+        call()
+    raw = driver.CUgraph(graph.raw_cuda_graph())
+    ok = driver.CUresult.CUDA_SUCCESS
+    err, _, n = driver.cuGraphGetNodes(raw)
+    assert err == ok
+    err, nodes, n = driver.cuGraphGetNodes(raw, n)
+    assert err == ok
+    sizes = []
+    for node in nodes:
+        err, kind = driver.cuGraphNodeGetType(node)
+        assert err == ok
+        if kind == driver.CUgraphNodeType.CU_GRAPH_NODE_TYPE_KERNEL:
+            err, p = driver.cuGraphKernelNodeGetParams(node)
+            assert err == ok
+            sizes.append(p.gridDimX * p.gridDimY * p.gridDimZ)
+    return sizes
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("limit", [1, 3, 32])
+@pytest.mark.parametrize("T,d,E,S", [(1, 512, 8, 0), (4, 1024, 8, 1), (12, 512, 40, 2), (16, 8192, 4, 0)])
+def test_both_kernels_keep_a_limit_of_ctas(kind, limit, T, d, E, S):
+    m = Layer(kind, d, 608, E, 2, S, seed=T)
+    x = m.x(T)
+    want = m(x)
+    assert max(_grids(lambda: m(x))) > 32
+    capi.call("lmoe_set_gemm_sm_limit", limit)
+    try:
+        got = m(x)
+        sizes = _grids(lambda: m(x))
+    finally:
+        capi.call("lmoe_set_gemm_sm_limit", 0)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert max(sizes) <= max(limit, 2)   # the first kernel's CTAs come in pairs
+
+
 def test_refusals():
     m = Layer(("fp8", "bf16"), 128, 64, 4, 2)
     x = m.x(4)
