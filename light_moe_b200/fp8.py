@@ -24,6 +24,8 @@ from .layer import HostBufferCalls
 # 1408, six a token and two shared: 1 38 against 76, 8 97 against 124, 12 149 against 129; 8 of 1024 / 2816: 8 41 against
 # 50, 12 54 against 52.
 FEW_TOKENS, FEW_TOKENS_HIDDEN = 8, 8192
+# Experts that the router and one grouped product take.
+MOST_EXPERTS = 256
 
 
 @dataclass
@@ -87,6 +89,10 @@ class FP8MoELayer(HostBufferCalls, torch.nn.Module):
             raise ValueError("the router takes hidden sizes that are multiples of 64")
         if gate_bias is not None and gate_bias.shape != (e.num_experts,):
             raise ValueError("gate_bias must be [num_experts]")
+        if max(e.num_experts, e.num_shared) > MOST_EXPERTS:
+            raise ValueError(f"at most {MOST_EXPERTS} routed experts, and as many shared ones")
+        if not 1 <= top_k <= min(16, e.num_experts):
+            raise ValueError("top_k must be 1 .. min(16, num_experts)")
         self.register_buffer("gate_weight", gate_weight.detach().to(torch.bfloat16).contiguous())
         self.register_buffer("gate_bias", None if gate_bias is None else gate_bias.detach().float().contiguous())
         self.experts = e
@@ -111,17 +117,33 @@ class FP8MoELayer(HostBufferCalls, torch.nn.Module):
             return (y, ids, weights) if return_routing else y
         ids, weights, _, offsets, _, positions = ops.fused_gate_topk_ex(x2, self.gate_weight, k, self.gate_bias)[:6]
         positions, combine, segments, slots = positions.view(T, k), weights, e.num_experts, k
+        apart = 0   # shared experts beyond what one product takes: they have products of their own
         if e.num_shared:
             # shared expert s: rows T * k + s * T + t of every token t, weight 1
             S, dev = e.num_shared, x2.device
             base = T * k + T * torch.arange(S + 1, dtype=torch.int32, device=dev)
             positions = torch.cat([positions, base[:S] + torch.arange(T, dtype=torch.int32, device=dev)[:, None]], 1)
-            offsets = torch.cat([offsets[:-1], base])
-            combine = torch.cat([weights, weights.new_ones(T, S)], 1)
-            segments, slots = segments + S, k + S
+            if segments + S > MOST_EXPERTS:
+                apart = S
+            else:
+                offsets = torch.cat([offsets[:-1], base])
+                combine = torch.cat([weights, weights.new_ones(T, S)], 1)
+                segments, slots = segments + S, k + S
         xq, xs = ops.quantize_fp8(x2, positions=positions.contiguous())
-        h = ops.fp8_grouped_gemm(xq, xs, *e.w1, offsets, segments, weights_up=e.w3[0], weight_scales_up=e.w3[1])
-        hq, hs = ops.quantize_fp8(h)
-        o = ops.fp8_grouped_gemm(hq, hs, *e.w2, offsets, segments)
-        y = ops.combine_rows(o, positions, combine, T, slots).view(shape)
+        if apart:
+            n, cut = T * k, lambda a, b: ((q[a:b], s[a:b]) for q, s in (e.w1, e.w3, e.w2))
+            o = _products(xq[:n], xs[:n], offsets, segments, *cut(0, segments))
+            extra = _products(xq[n:], xs[n:], base - n, apart, *cut(segments, segments + apart))
+            y = ops.combine_rows(o, positions[:, :k], combine, T, k, extra, apart)
+        else:
+            o = _products(xq, xs, offsets, segments, e.w1, e.w3, e.w2)
+            y = ops.combine_rows(o, positions, combine, T, slots)
+        y = y.view(shape)
         return (y, ids, weights) if return_routing else y
+
+
+def _products(xq: torch.Tensor, xs: torch.Tensor, offsets: torch.Tensor, experts: int, w1, w3, w2) -> torch.Tensor:
+    """The rows between the offsets through their experts."""
+    h = ops.fp8_grouped_gemm(xq, xs, *w1, offsets, experts, weights_up=w3[0], weight_scales_up=w3[1])
+    hq, hs = ops.quantize_fp8(h)
+    return ops.fp8_grouped_gemm(hq, hs, *w2, offsets, experts)

@@ -51,6 +51,47 @@ def test_layer_equals_its_steps(T, d, F, E, k, S, bias, power):
     assert torch.equal(mod(x.view(1, T, d)).view(T, d), y)
 
 
+@pytest.mark.parametrize("T", [FEW_TOKENS + 1, 300])
+@pytest.mark.parametrize("S", [1, 3])
+def test_layer_of_256_experts_and_shared_ones(T, S):
+    """More experts than one product takes: routed and shared ones by themselves, for a few tokens together."""
+    x, mod, _ = _make(T, 64, 32, 256, 8, S, seed=T, bias=True)
+    y, ids, w = mod(x, return_routing=True)
+    e, k = mod.experts, 8
+    ids2, w2, _, off, sidx, pos = ops.fused_gate_topk_ex(x, mod.gate_weight, k, mod.gate_bias)[:6]
+    assert torch.equal(ids, ids2) and torch.equal(w, w2)
+
+    def run(rows, offsets, a, b):
+        part = lambda m: (m[0][a:b], m[1][a:b])
+        h = ops.fp8_grouped_gemm(*ops.quantize_fp8(rows), *part(e.w1), offsets, b - a, weights_up=e.w3[0][a:b],
+                                 weight_scales_up=e.w3[1][a:b])
+        return ops.fp8_grouped_gemm(*ops.quantize_fp8(h), *part(e.w2), offsets, b - a)
+
+    o = run(x[(sidx // k).long()], off, 0, 256)
+    want = torch.zeros(T, 64, device="cuda")
+    for j in range(k):
+        want = want + w[:, j:j + 1] * o[pos.view(T, k)[:, j].long()].float()
+    for s in range(S):
+        want = want + run(x, torch.tensor([0, T], dtype=torch.int32, device="cuda"), 256 + s, 257 + s).float()
+    assert torch.equal(y, want.to(torch.bfloat16))
+    few, ids, w = mod(x[:5], return_routing=True)
+    assert torch.equal(ids, ids2[:5]) and torch.allclose(w, w2[:5], rtol=1e-4)
+    assert (few.float() - y[:5].float()).norm() <= 2.0 ** -4 * few.float().norm()   # (E4M3 activations, as above)
+
+
+def test_layers_that_no_call_could_run_are_refused():
+    x, mod, (w1, w3, w2) = _make(1, 64, 32, 4, 2, 1)
+    many = lambda n: FP8Experts(*((q[:1].expand(n, -1, -1), s[:1].expand(n, -1, -1)) for q, s in
+                                  (mod.experts.w1, mod.experts.w3, mod.experts.w2)), n, 0, 64, 32)
+    for experts, k in ((many(257), 2), (mod.experts, 0), (mod.experts, 5), (many(40), 17)):
+        with pytest.raises(ValueError):
+            FP8MoELayer(torch.zeros(experts.num_experts, 64, device="cuda"), experts, k)
+    shared = FP8Experts(*((q[:1].expand(258, -1, -1), s[:1].expand(258, -1, -1)) for q, s in
+                          (mod.experts.w1, mod.experts.w3, mod.experts.w2)), 1, 257, 64, 32)
+    with pytest.raises(ValueError):
+        FP8MoELayer(torch.zeros(1, 64, device="cuda"), shared, 1)
+
+
 @pytest.mark.parametrize("T", [1, 5, FEW_TOKENS])
 def test_few_tokens_take_their_kernels(T):
     x, mod, _ = _make(T, 256, 96, 8, 2, 1, T, True)
