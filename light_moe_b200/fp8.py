@@ -24,6 +24,7 @@ from .layer import HostBufferCalls
 # 1408, six a token and two shared: 1 38 against 76, 8 97 against 124, 12 149 against 129; 8 of 1024 / 2816: 8 41 against
 # 50, 12 54 against 52.
 FEW_TOKENS, FEW_TOKENS_HIDDEN = 8, 8192
+FEW_TOKENS_FFN, FEW_TOKENS_SHARED = 65536, 16   # what those kernels take
 # Experts that the router and one grouped product take.
 MOST_EXPERTS = 256
 
@@ -107,7 +108,8 @@ class FP8MoELayer(HostBufferCalls, torch.nn.Module):
             y = x2.new_empty(shape)
             return (y, x2.new_empty((0, k), dtype=torch.int32), x2.new_empty((0, k), dtype=torch.float32)) \
                 if return_routing else y
-        if T <= FEW_TOKENS and e.hidden_size <= FEW_TOKENS_HIDDEN and e.ffn_size % 32 == 0 and e.num_shared <= 16:
+        if T <= FEW_TOKENS and e.hidden_size <= FEW_TOKENS_HIDDEN and e.ffn_size % 32 == 0 \
+                and e.ffn_size <= FEW_TOKENS_FFN and e.num_shared <= FEW_TOKENS_SHARED:
             # (a cast of the module may have changed the router's types)
             y, ids, weights = ops.moe_layer_few_tokens(
                 x2, self.gate_weight.to(torch.bfloat16), e.w1[0], e.w3[0], e.w2[0], k, w1_scales=e.w1[1],

@@ -129,3 +129,15 @@ def test_ops_refuse_host_tensors():
                  lambda: ops.fp8_grouped_gemm(q, s, q[None], s[None, :1], torch.zeros(2, dtype=torch.int32), 1)):
         with pytest.raises(RuntimeError, match="CUDA"):
             call()
+
+
+def test_layer_takes_the_few_token_kernels_only_for_their_sizes():
+    """The module's limits are the library's."""
+    from light_moe_b200 import fp8
+
+    size = capi.lib().lmoe_few_tokens_workspace_bytes
+    T, d, F, S = fp8.FEW_TOKENS, fp8.FEW_TOKENS_HIDDEN, fp8.FEW_TOKENS_FFN, fp8.FEW_TOKENS_SHARED
+    for E, k in ((1, 1), (fp8.MOST_EXPERTS, 16)):
+        assert size(T, d, F, E, k, S) > 0
+    assert size(T, d, F + 32, 4, 2, S) == 0 and size(T, d, F, 4, 2, S + 1) == 0
+    assert size(T, d, F, fp8.MOST_EXPERTS + 1, 2, S) == 0

@@ -92,6 +92,14 @@ def test_layers_that_no_call_could_run_are_refused():
         FP8MoELayer(torch.zeros(1, 64, device="cuda"), shared, 1)
 
 
+def test_ffn_sizes_beyond_the_few_token_kernels():
+    """They run like larger batches, row by row the same."""
+    x, mod, _ = _make(FEW_TOKENS + 1, 64, 65568, 1, 1)
+    y = mod(x)
+    for T in (1, 5):
+        assert torch.equal(mod(x[:T]), y[:T])
+
+
 @pytest.mark.parametrize("T", [1, 5, FEW_TOKENS])
 def test_few_tokens_take_their_kernels(T):
     x, mod, _ = _make(T, 256, 96, 8, 2, 1, T, True)
