@@ -344,6 +344,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     int hint = 0, in_slot = 0;
     float f0 = 0.0f, f1 = 0.0f;
     bool ok = true;
+    // A lane whose wait ran out still takes every step of its tile with the others, since the loads of tensor memory
+    // need the whole warp, but waits no more; lane 0 then gives nothing back.  The warp agrees at the tile's end (with a
+    // vote every block the prompt's product took 0.7 % longer).
     // Waits for the next block's sums and reads its factors.
     auto next_block = [&]() {
       if (in_slot == 0) ok = ok && mbar_wait(&bars->sc_full[sl.i], sl.phase, a.err, abort_flag, kSite + 7);
@@ -360,10 +363,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     auto pass_block = [&](bool last) {
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(empty_addr + ac.i * 8);
+      if (lane == 0 && ok) mbar_arrive_cluster(empty_addr + ac.i * 8);
       ac.next();
       if (++in_slot == kSlotBlocks || last) {
-        if (lane == 0) mbar_arrive(&bars->sc_empty[sl.i]);
+        if (lane == 0 && ok) mbar_arrive(&bars->sc_empty[sl.i]);
         sl.next();
         in_slot = 0;
       }
@@ -378,14 +381,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       if (!t.zero) {
         next_block();
         if (rows <= 0) {   // the segment ends before this warp's rows
-          for (int left = KB; left > 0 && ok; --left) {
+          for (int left = KB; left > 0; --left) {
             pass_block(left == 1);
             if (left > 1) next_block();
           }
         } else {
           // 32 columns at a time
           const uint32_t lanes = tmem + lane_base + half * C::kCols;
-          for (int left = KB; left > 0 && ok; --left) {
+          for (int left = KB; left > 0; --left) {
             const uint32_t col = lanes + ac.i * TN;
             const float g0 = f0, g1 = f1;
 #pragma unroll
@@ -399,6 +402,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             if (left > 1) next_block();
           }
         }
+        ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
       }
       if (rows <= 0) continue;
