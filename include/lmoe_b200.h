@@ -348,7 +348,8 @@ int lmoe_dequantize_fp8(const uint8_t* q, const float* scales, int64_t scale_mat
  * x: codes xq [total_rows, K], scales xs [K blocks][xs_pitch]; w (and up): codes [E, N, K], scales
  * [E, ceil(N / 128), ceil(K / 128)]; codes 16-byte aligned.  The product of the two scales of a block has to
  * be an fp32 number too (a factor that overflows makes NaN of sums that are zero).  output [total_rows, N] of out_dtype; rows
- * outside every expert are zero.  total_rows and K up to 2^31 - 1025, N up to 2^30 - 513.  error: as above. */
+ * outside every expert are zero.  total_rows and K up to 2^31 - 1025, N up to 2^30 - 513.  error: as above; should a
+ * bounded wait ever run out, what was not computed is NaN. */
 int lmoe_fp8_grouped_gemm(const uint8_t* xq, const float* xs, int64_t xs_pitch, int64_t total_rows, int K,
                           const uint8_t* wq, const float* ws, const uint8_t* wq_up, const float* ws_up, int N,
                           const void* expert_offsets, int offsets_are_int64, int num_experts, int out_dtype,

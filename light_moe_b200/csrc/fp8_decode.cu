@@ -279,7 +279,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     Ring<kSlots> sl;
     int hint = 0, in_slot = 0;
     bool ok = true;
-    for (int tile = first; tile < total && ok; tile += stride) {
+    for (int tile = first; tile < total; tile += stride) {
       const Tile t = tile_at(seg, a, tile, hint);
       const int row = t.row0 + half * 32;   // the warp's first column
       const int rows = t.row_end - row < 32 ? t.row_end - row : 32;
@@ -287,7 +287,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       float acc[C::kMats * 32];
 #pragma unroll
       for (int i = 0; i < C::kMats * 32; ++i) acc[i] = 0.0f;
-      if (!t.zero) {
+      if (!t.zero && ok) {
         for (int left = KB; left > 0; --left) {
           if (in_slot == 0) ok = mbar_wait(&bars->sc_full[sl.i], sl.phase, a.err, abort_flag, kSite + 7);
           ok = ok && mbar_wait(&bars->acc_full[ac.i], ac.phase, a.err, abort_flag, kSite + 8);
@@ -317,7 +317,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             in_slot = 0;
           }
         }
-        if (!ok) break;
+      }
+      if (!t.zero && !ok) {   // what was not computed is NaN
+#pragma unroll
+        for (int i = 0; i < C::kMats * 32; ++i) acc[i] = __uint_as_float(0x7fc00000u);
       }
       if (feature >= a.N) continue;
       // a row's 32 features of a warp are neighbours

@@ -371,14 +371,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         in_slot = 0;
       }
     };
-    for (int tile = first; tile < total && ok; tile += stride) {
+    for (int tile = first; tile < total; tile += stride) {
       const Fp8Tile t = fp8_tile_at(seg, a, tile, hint);
       const int row = t.row0 + (int)rank * kRowsCta + q * 32;   // the warp's first
       const int rows = t.row_end - row < 32 ? t.row_end - row : 32;
       float acc[C::kCols];
 #pragma unroll
       for (int i = 0; i < C::kCols; ++i) acc[i] = 0.0f;
-      if (!t.zero) {
+      if (!t.zero && ok) {
         next_block();
         if (rows <= 0) {   // the segment ends before this warp's rows
           for (int left = KB; left > 0; --left) {
@@ -403,9 +403,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           }
         }
         ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
       }
       if (rows <= 0) continue;
+      if (!t.zero && !ok) {   // what was not computed is NaN
+#pragma unroll
+        for (int i = 0; i < C::kCols; ++i) acc[i] = __uint_as_float(0x7fc00000u);
+      }
       constexpr int kOut = SWIGLU ? kPart : kChunks;
       if (SWIGLU) {
 #pragma unroll
