@@ -350,6 +350,27 @@ def test_views_and_strides():
     assert torch.equal(m(x)[0], want[0])
 
 
+@pytest.mark.parametrize("weights", ["fp8", "dense"])
+def test_layer_of_more_than_2_to_the_31_weights(weights):
+    """The last of several large experts is what it is as the only one."""
+    d, F, E = 16384, 14336, 10
+    m = Layer((weights, "bf16"), d, F, 1, 1, seed=9, std=0.02)
+    x = m.x(2)
+    want = m(x)
+    for i in range(3):
+        w = torch.zeros(E, *m.w[i].shape[1:], dtype=m.w[i].dtype, device="cuda")
+        w[-1:] = m.w[i]
+        m.w[i] = w
+    assert m.w[0].numel() > 2 ** 31
+    for name, s in m.scales.items():
+        m.scales[name] = torch.cat([torch.ones_like(s)] * (E - 1) + [s])
+    m.gate = torch.zeros(E, d, dtype=m.dt, device="cuda")
+    m.bias = torch.zeros(E, device="cuda")
+    m.bias[-1] = 1.0
+    y, ids, w = m(x)
+    assert (ids == E - 1).all() and (w == 1).all() and torch.equal(y, want[0])
+
+
 def test_under_a_limit_of_ctas():
     m = Layer(("dense", "fp16"), 512, 608, 8, 2, seed=7)
     x = m.x(4)

@@ -204,6 +204,21 @@ def test_quantize_positions():
     assert (scales[0, [3, 5]] != 9).all()
 
 
+@pytest.mark.parametrize("block_rows", [1, 128])
+def test_quantize_more_than_2_to_the_31_values(block_rows):
+    """The first rows, those around the 2^31st value and the last ones are what they are by themselves."""
+    K = 4096
+    rows = 2 ** 31 // K + 1024
+    x = torch.empty(rows, K, dtype=torch.bfloat16, device="cuda").normal_()
+    q, s = ops.quantize_fp8(x, block_rows=block_rows)
+    v = ops.dequantize_fp8(q, s, block_rows=block_rows)
+    for a in (0, rows - 1152, rows - 1024, rows - 128):
+        part, scales = ops.quantize_fp8(x[a:a + 128], block_rows=block_rows)
+        assert torch.equal(_bytes(q)[a:a + 128], _bytes(part))
+        assert torch.equal(s[a // block_rows:(a + 128) // block_rows], scales)
+        assert torch.equal(v[a:a + 128], ops.dequantize_fp8(part, scales, block_rows=block_rows))
+
+
 def _bytes(q):
     return q.view(torch.uint8)
 
@@ -440,6 +455,30 @@ def test_gemm_under_a_limit_of_ctas():
     finally:
         capi.lib().lmoe_set_gemm_sm_limit(0)
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("experts", [1, 250])
+def test_gemm_more_than_2_to_the_31_codes(experts):
+    """Of rows (tiles of rows, or with many experts the other kernel's limit of rows), and of weights."""
+    K = 16384
+    R = 2 ** 31 // K + 200 if experts == 1 else 64
+    N = 40 if experts == 1 else 2 ** 31 // K // 249
+    q = torch.randint(0, 2 ** 32, (R, K // 4), device="cuda").to(torch.int32).view(torch.uint8)
+    q[(q & 0x7f) == 0x7f] = 0   # NaN
+    q = q.view(torch.float8_e4m3fn)
+    xs = torch.rand(K // 128, R, device="cuda").t()
+    w = torch.randint(0, 2 ** 32, (experts, N, K // 4), device="cuda").to(torch.int32).view(torch.uint8)
+    w[(w & 0x7f) == 0x7f] = 0
+    w = w.view(torch.float8_e4m3fn)
+    ws = torch.rand(experts, -(-N // 128), K // 128, device="cuda")
+    assert max(q.numel(), w.numel()) > 2 ** 31
+    off = torch.zeros(experts + 1, dtype=torch.int64, device="cuda")
+    off[-1] = R                 # the last expert's
+    y = ops.fp8_grouped_gemm(q, xs, w, ws, off, experts, out_dtype=torch.float32)
+    for a, b in ((0, 64), (R - 64, R)):
+        few = torch.tensor([0, b - a], dtype=torch.int64, device="cuda")
+        want = ops.fp8_grouped_gemm(q[a:b], xs[a:b], w[-1:], ws[-1:], few, 1, out_dtype=torch.float32)
+        assert torch.isfinite(want).all() and torch.equal(y[a:b], want)
 
 
 def test_gemm_empty_and_refusals():

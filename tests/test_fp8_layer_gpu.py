@@ -176,6 +176,31 @@ def test_casts_of_the_module(T, dt):
         assert torch.equal(z, y)
 
 
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16, torch.float32, torch.float64])
+@pytest.mark.parametrize("T", [3, 37])
+def test_casts_of_the_module_keep_its_values(T, dt):
+    """A cast layer computes what its cast router says: a few tokens what a layer built from it computes, more tokens what
+    the steps called one by one do; and its routing is near the softmax in 64 bits."""
+    x, mod, _ = _make(T, 256, 96, 8, 2, 1, 1, True)
+    mod.to(dt)
+    gate, bias = mod.gate_weight, mod.gate_bias
+    y, ids, w = mod(x, return_routing=True)
+    if T <= FEW_TOKENS:
+        want, ids2, w2 = FP8MoELayer(gate, mod.experts, 2, bias)(x, return_routing=True)
+    else:
+        want, ids2, w2 = _by_hand(mod, x, T, 2)
+    assert torch.equal(y, want) and torch.equal(ids, ids2) and torch.equal(w, w2)
+    # 256 products and the bias in fp32, each sum off by 2^-23 of the sum of absolute values at most
+    l = x.double() @ gate.double().T + bias.double()
+    err = 257 * 2.0 ** -23 * (x.double().abs() @ gate.double().abs().T + bias.double().abs())
+    chosen = torch.zeros_like(l, dtype=torch.bool).scatter_(1, ids.long(), True)
+    assert (chosen.sum(1) == 2).all()
+    assert ((l + err)[chosen].view(T, 2).amin(1) >= (l - err).masked_fill(chosen, -float("inf")).amax(1)).all()
+    want = torch.softmax(l.gather(1, ids.long()), 1)
+    # the exponentials' errors, 2 units in the last place, the sum and the quotient: 2^-20
+    assert ((w.double() - want).abs() <= want * (torch.expm1(2 * err.amax(1, keepdim=True)) + 2.0 ** -20)).all()
+
+
 def test_experts_of_a_checkpoint():
     x, mod, _ = _make(20, 128, 208, 4, 2, 1)
     e = mod.experts
