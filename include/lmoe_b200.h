@@ -363,8 +363,8 @@ int lmoe_fp8_grouped_gemm(const uint8_t* xq, const float* xs, int64_t xs_pitch, 
  *   w1, w3 [E + S, ffn, hidden], w2 [E + S, hidden, ffn], 32-byte aligned: of dtype, or (with the three
  *     scales) E4M3 codes with fp32 scales of blocks of 128 x 128 as lmoe_quantize_fp8_blocks writes them
  *   y [num_tokens, hidden_size] of dtype; ids int32, weights fp32 [num_tokens, top_k]
- * Hidden values stay in fp32 between the kernels and enter the second product as a sum of two 16-bit
- * numbers; all sums are fp32.  Values below 2^-39 of a token's largest (bf16 tokens with E4M3 weights) or
+ * Hidden values stay in fp32 between the kernels and enter the second product as a sum of two fp16 numbers (22
+ * bits), or with dense bf16 weights of three bf16 numbers; all sums are fp32.  Values below 2^-39 of a token's largest (bf16 tokens with E4M3 weights) or
  * of its largest hidden value over all of its experts (fp16 products) are lost.
  * hidden_size % 64 == 0, at most 16384; ffn_size % 32 == 0, at most 65536; num_experts <= 256, top_k <= 16,
  * num_shared <= 16; LMOE_ERR_UNSUPPORTED where eight tokens of that hidden size do not fit shared memory

@@ -29,9 +29,11 @@
 //    Writes w * silu(gate) * up in fp32.
 // 2. down_kernel.  A CTA owns 256 output rows (a warp 16) and a slice of the contraction; the last
 //    CTA of a row block to finish adds the slices in their order, so the result does not depend on
-//    timing.  Hidden values enter the MMA as a sum of two 16-bit numbers (22 bits in fp16, 16 in bf16),
-//    which cost columns of the MMA (4 tokens to one instead of 8) but no weight traffic: rounding them to one would be
-//    an error as large as the output's own rounding.
+//    timing.  Hidden values enter the MMA as a sum of two fp16 numbers (22 bits) or three bf16 numbers (all 24), which
+//    cost columns of the MMA (8 hold 4 tokens, or 2) but no weight traffic: rounding them to one would be an error
+//    as large as the output's own rounding, and with two bf16 numbers (16 bits) 0.28 % of a layer's outputs lay on the
+//    other side of a bf16 step than in exact arithmetic, with three 0.04 %, in fp32 arithmetic 0.06 % (4 tokens, 8
+//    experts of 4096 x 14336; 318 us with two, 323 with three).
 //
 // fp16 operands need a range: tokens (bf16 times E4M3 weights) and hidden values are scaled by powers of two, per token
 // (hidden values over all of its experts), so that the largest lies in [2^14, 2^15); what is 2^-39 of it or smaller is
@@ -120,6 +122,10 @@ struct Geo {
   static constexpr int kPieces = kPer / 8;        // 16-byte pieces (8 values) of the 16-bit operand
   static constexpr int kBytes = FP8 ? 1 : 2;
 };
+
+// 16-bit numbers whose sum a hidden value is in the second kernel: of 11 significant bits, or of 8.
+template <bool FP8, typename X>
+constexpr int kTermsOf = !FP8 && std::is_same<X, __nv_bfloat16>::value ? 3 : 2;
 
 template <typename T>
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
@@ -727,17 +733,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gate_up
 // ---------------------------------------------------------------------------------------
 // second kernel
 // ---------------------------------------------------------------------------------------
-// The two halves of a token's hidden values are columns t and t + 4 of one MMA.  MODE 0: up to 4 tokens, whose
-// sums stay in registers for the whole slice.  MODE 1, 2 (up to 8, 16): of each expert the tokens that chose it, four
-// to an MMA, whose sums go to the tokens' own in shared memory at the expert's end (with all tokens in every
-// expert's columns, 16 tokens through 8 experts of 4096 x 14336 took this kernel 187 us, now 121).
+// The terms of a token's hidden values are neighbouring columns.  MODE 0: up to 4 tokens, in every expert's MMAs, whose
+// sums stay in registers for the whole slice.  MODE 1, 2 (up to 8, 16 tokens): of each expert the tokens that chose it, one
+// behind the other in as many MMAs as they fill, whose sums go to the tokens' own in shared memory at the expert's end (with
+// all tokens in every expert's columns, 16 tokens through 8 experts of 4096 x 14336 took this kernel 187 us, now 121).
 // CHUNKS: a slice's hidden values do not fit shared memory at once.
 template <bool FP8, typename X, int MODE, bool CHUNKS>
 __global__ void __launch_bounds__(kThreads, 1) down_kernel(const FewArgs a) {
   using G = Geo<FP8>;
   using M = typename std::conditional<FP8, __half, X>::type;
-  constexpr int Q = MODE == 2 ? 4 : (MODE == 1 ? 2 : 1);   // MMAs of four tokens at most
-  constexpr int kAhead = FP8 && MODE == 2 ? 2 : kAheadOf<FP8>, kBurst = kAhead == 4 ? 2 : kAhead;   // (16 sums: no registers for 3)
+  constexpr int kTerms = kTermsOf<FP8, X>;
+  constexpr int kCols = kTerms == 2 ? 2 : 4, kPerMma = 8 / kCols;   // columns of a token (a fourth stays empty)
+  constexpr int Q = (MODE == 2 ? 16 : (MODE == 1 ? 8 : 4)) / kPerMma;   // MMAs at most
+  // Steps of weights in flight.  The sums of 9 to 16 tokens (16 or 32 a thread) leave registers for two; three terms for
+  // three (with four, 4 tokens through 8 experts of 4096 x 14336 took 326 us, so 322; 8 tokens 554 and 492).
+  constexpr int kAhead = MODE == 2 && (FP8 || kTerms == 3) ? 2 : (kTerms == 3 ? 3 : kAheadOf<FP8>);
+  constexpr int kBurst = kAhead == 4 ? 2 : kAhead;
   static_assert(kChunkSteps % kAhead == 0, "a chunk starts at the first of the buffers in flight");
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int expert[kMaxUsed];
@@ -807,11 +818,10 @@ __global__ void __launch_bounds__(kThreads, 1) down_kernel(const FewArgs a) {
     }
   };
 
-  // Hidden values are staged as two 16-bit numbers (of values scaled to at most 2^15), in pieces of 8 of a token;
-  // those of the next chunk beside this chunk's products.
+  // Hidden values are staged as two or three 16-bit numbers (of values scaled to at most 2^15), in pieces of 8 of a
+  // token; those of the next chunk beside this chunk's products.
   constexpr int kStepPieces = G::kStep / 8;
-  const uint32_t step_bytes = (uint32_t)G::kPieces * T * 64;    // of one half
-  const uint32_t half_bytes = step_bytes * a.chunk;
+  const uint32_t step_bytes = (uint32_t)G::kPieces * T * kTerms * 64;   // [piece][token][term][lane of the quad]
   // Piece q of token t in a step of the contraction, zeros behind the last feature; false where the token did
   // not choose the expert: nobody looks there.
   auto fetch = [&](int step, int t, int q, float4& v0, float4& v1) {
@@ -827,17 +837,22 @@ __global__ void __launch_bounds__(kThreads, 1) down_kernel(const FewArgs a) {
   };
   auto put_piece = [&](uint8_t* dst, float scale, const float4& v0, const float4& v1) {
     const float v[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
-    uint32_t hi[4], lo[4];
+    uint32_t term[kTerms][4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float x = v[2 * j] * scale, y = v[2 * j + 1] * scale;
-      hi[j] = narrow2<M>(x, y);
-      const float2 r = widen2<M>(hi[j]);
-      // (of an infinity or NaN there is no rest)
-      lo[j] = narrow2<M>(fabsf(r.x) < kInf ? x - r.x : 0.0f, fabsf(r.y) < kInf ? y - r.y : 0.0f);
+      float x = v[2 * j] * scale, y = v[2 * j + 1] * scale;
+#pragma unroll
+      for (int i = 0; i < kTerms; ++i) {
+        term[i][j] = narrow2<M>(x, y);
+        const float2 r = widen2<M>(term[i][j]);
+        // what is left, exactly (of an infinity or NaN nothing)
+        x = fabsf(r.x) < kInf ? x - r.x : 0.0f;
+        y = fabsf(r.y) < kInf ? y - r.y : 0.0f;
+      }
     }
-    *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-    *reinterpret_cast<uint4*>(dst + half_bytes) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+#pragma unroll
+    for (int i = 0; i < kTerms; ++i)
+      *reinterpret_cast<uint4*>(dst + i * 64) = make_uint4(term[i][0], term[i][1], term[i][2], term[i][3]);
   };
   {
     // the first chunk, its first pieces asked for before the weights; four pieces in flight a thread if there are many
@@ -845,7 +860,7 @@ __global__ void __launch_bounds__(kThreads, 1) down_kernel(const FewArgs a) {
     const int pieces = n * T * kStepPieces;
     auto place = [&](int i) {
       const int q = i % kStepPieces, r = i / kStepPieces, t = T == 1 ? 0 : r % T, step = T == 1 ? r : r / T;
-      return smem + step * step_bytes + ((uint32_t)(q % G::kPieces) * T + t) * 64 + q / G::kPieces * 16;
+      return smem + step * step_bytes + ((uint32_t)(q % G::kPieces) * T + t) * (kTerms * 64) + q / G::kPieces * 16;
     };
     auto ask = [&](int i, float4& x, float4& y) {
       const int r = i / kStepPieces;
@@ -888,7 +903,7 @@ __global__ void __launch_bounds__(kThreads, 1) down_kernel(const FewArgs a) {
       if (piece < pieces) {
         const int t = column[nu][piece / kStepPieces], q = piece % kStepPieces;
         pending = fetch(nu * fsteps + nk, t, q, v0, v1);
-        to = step * step_bytes + ((uint32_t)(q % G::kPieces) * T + t) * 64 + q / G::kPieces * 16;
+        to = step * step_bytes + ((uint32_t)(q % G::kPieces) * T + t) * (kTerms * 64) + q / G::kPieces * 16;
         v_scale = pow2(range_exponent(top[t]));
       }
       __syncwarp();
@@ -910,33 +925,41 @@ __global__ void __launch_bounds__(kThreads, 1) down_kernel(const FewArgs a) {
     for (int i = lane; i < 16 * T; i += 32) sums[i] = 0.0f;
     __syncwarp();
   }
-  // this lane's columns: tokens, and of each a half
-  const uint32_t half_at = (g >> 2) * half_bytes + c * 16;
-  const uint32_t buf_bytes = 2 * half_bytes;
+  // this lane's columns: of MMA i a term of token i * kPerMma + g / kCols
+  const uint32_t buf_bytes = step_bytes * a.chunk;
   int u = begin / fsteps, k = begin - u * fsteps, buf = 0, columns = 0;
-  uint32_t from[Q];
-  bool has[Q];
+  constexpr uint32_t kNone = 0xffffffffu;
+  uint32_t from[Q];   // of the step's hidden values; kNone: no token
+  // MODE 0: of the first MMA
+  const uint32_t all_from = kTerms == 2 ? lane * 16 : (g / kCols * kTerms + g % kCols) * 64 + c * 16;
   auto choose = [&]() {   // of expert u
     if (MODE == 0) return;
     columns = __popc(tokens[u]);
 #pragma unroll
     for (int i = 0; i < Q; ++i) {
-      const int at = 4 * i + (g & 3);
-      has[i] = at < columns;
-      from[i] = half_at + (has[i] ? column[u][at] : 0) * 64;
+      const int at = i * kPerMma + g / kCols;
+      from[i] = at < columns && g % kCols < kTerms ? (column[u][at] * kTerms + g % kCols) * 64 + c * 16 : kNone;
     }
   };
+  // Sum of the terms of token i * kPerMma + c * 2 / kCols, rows g (r = 0) and g + 8 (r = 2), in the first of its lanes.
+  auto token_sum = [&](int i, int r) {
+    float v = acc[i][r] + acc[i][r + 1];
+    if (kCols == 4) v += __shfl_xor_sync(0xffffffffu, v, 1);
+    return v;
+  };
+  const bool first_lane = kCols == 2 || (c & 1) == 0;
   auto deliver = [&]() {   // the sums of expert u's tokens
     if constexpr (MODE != 0) {
 #pragma unroll
-      for (int i = 0; i < Q; ++i)
+      for (int i = 0; i < Q; ++i) {
+        const int at = i * kPerMma + c * 2 / kCols;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float v = acc[i][j] + __shfl_xor_sync(0xffffffffu, acc[i][j], 2);   // columns t and t + 4
-          const int at = 4 * i + c * 2 + (j & 1);
-          if (c < 2 && at < columns) sums[column[u][at] * 16 + g + (j >> 1) * 8] += v;
-          acc[i][j] = 0.0f;
+        for (int r = 0; r < 4; r += 2) {
+          const float v = token_sum(i, r);
+          if (first_lane && at < columns) sums[column[u][at] * 16 + g + r * 4] += v;
+          acc[i][r] = acc[i][r + 1] = 0.0f;
         }
+      }
       __syncwarp();
     }
   };
@@ -960,23 +983,43 @@ __global__ void __launch_bounds__(kThreads, 1) down_kernel(const FewArgs a) {
         }
         const uint32_t mask = MODE == 0 ? tokens[u] : 0u;
         const uint8_t* src = smem + buf * buf_bytes + s * step_bytes;
+        auto operand = [&](int i, int p) {
+          uint4 v = make_uint4(0u, 0u, 0u, 0u);
+          if (MODE == 0 ? (mask >> (i * kPerMma + g / kCols) & 1u) != 0u && g % kCols < kTerms : from[i] != kNone)
+            v = *reinterpret_cast<const uint4*>(src + p * T * (kTerms * 64) +
+                                                (MODE == 0 ? all_from + i * kPerMma * (kTerms * 64) : from[i]));
+          return v;
+        };
+        auto add = [&](int i, const float (&v)[4]) {
+          // (MODE 0: a token without the expert gets nothing, where zero times an infinite weight would be NaN)
+          if (MODE == 0 && (mask >> (i * kPerMma + c * 2 / kCols) & 1u) == 0u) return;
 #pragma unroll
-        for (int i = 0; i < Q; ++i) {
-          if (i > 0 && columns <= 4 * i) continue;
+          for (int j = 0; j < 4; ++j) acc[i][j] = FP8 ? fmaf(v[j], f[b], acc[i][j]) : acc[i][j] + v[j];
+        };
+        // Two MMAs at a time, a chain of dependent products each; one by itself: two chains.  (fp16, whose four steps in
+        // flight leave no registers for that: one at a time.)
+        constexpr bool kPairs = Q > 1 && (FP8 || kTerms == 3);
+        constexpr int kNext = kPairs ? 1 : 0;
+        const int have = MODE == 0 ? T : columns;
+#pragma unroll
+        for (int i = 0; i < Q; i += 1 + kNext) {
+          if (i > 0 && have <= i * kPerMma) break;
           float part[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+          if (kPairs && have > (i + 1) * kPerMma) {
 #pragma unroll
-          for (int p = 0; p < G::kPieces; ++p) {
-            uint4 v = make_uint4(0u, 0u, 0u, 0u);
-            if (MODE == 0 ? (mask >> (g & 3) & 1u) != 0u : has[i])
-              v = *reinterpret_cast<const uint4*>(src + p * T * 64 + (MODE == 0 ? half_at + (g & 3) * 64 : from[i]));
-            mma_piece<FP8, M>(part[p & 1], w0[b], w1[b], p, v);
-          }
+            for (int p = 0; p < G::kPieces; ++p) {
+              const uint4 v0 = operand(i, p), v1 = operand(i + kNext, p);
+              mma_piece<FP8, M>(part[0], w0[b], w1[b], p, v0);
+              mma_piece<FP8, M>(part[1], w0[b], w1[b], p, v1);
+            }
+            add(i, part[0]);
+            add(i + kNext, part[1]);
+          } else {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            // (MODE 0: a token without the expert gets nothing, where zero times an infinite weight would be NaN)
-            if (MODE == 0 && (mask >> ((c * 2 + (j & 1)) & 3) & 1u) == 0u) continue;
-            const float v = part[0][j] + part[1][j];
-            acc[i][j] = FP8 ? fmaf(v, f[b], acc[i][j]) : acc[i][j] + v;
+            for (int p = 0; p < G::kPieces; ++p) mma_piece<FP8, M>(part[p & 1], w0[b], w1[b], p, operand(i, p));
+#pragma unroll
+            for (int j = 0; j < 4; ++j) part[0][j] += part[1][j];
+            add(i, part[0]);
           }
         }
         if (b % kBurst == kBurst - 1) {
@@ -1013,11 +1056,13 @@ __global__ void __launch_bounds__(kThreads, 1) down_kernel(const FewArgs a) {
   };
   if constexpr (MODE == 0) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float v = acc[0][j] + __shfl_xor_sync(0xffffffffu, acc[0][j], 2);   // columns t and t + 4
-      const int t = c * 2 + (j & 1);
-      if (rows_ok && c < 2 && t < T) give(t, row0 + g + (j >> 1) * 8, v);
-    }
+    for (int i = 0; i < Q; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; r += 2) {
+        const int t = i * kPerMma + c * 2 / kCols;
+        const float v = token_sum(i, r);
+        if (rows_ok && first_lane && t < T) give(t, row0 + g + r * 4, v);
+      }
   } else if (rows_ok) {
     for (int i = lane; i < 16 * T; i += 32) give(i >> 4, row0 + (i & 15), sums[i]);
   }
@@ -1077,7 +1122,7 @@ FewWorkspace few_workspace(int T, int d, int F, int E, int k, int S) {
 
 template <bool FP8, typename X>
 int launch(FewArgs a, int items, int ctas, bool limited, uint32_t smem1, cudaStream_t stream) {
-  const uint32_t step_bytes = (uint32_t)Geo<FP8>::kStep * a.T * 4;
+  const uint32_t step_bytes = (uint32_t)Geo<FP8>::kStep * a.T * 2 * kTermsOf<FP8, X>;
   const int used = (a.E < a.T * a.k ? a.E : a.T * a.k) + a.S;
   const int64_t most = ((int64_t)used * ((a.F + Geo<FP8>::kStep - 1) / Geo<FP8>::kStep) + a.split - 1) / a.split + 1;
   const bool whole = most * step_bytes <= kWholeBytes;

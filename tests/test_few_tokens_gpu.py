@@ -350,6 +350,52 @@ def test_views_and_strides():
     assert torch.equal(m(x)[0], want[0])
 
 
+def _split_hidden_value():
+    """Gate and up, integers of 12 bits, whose product h has a bf16 part, a rest with a bf16 part, and a rest of that
+    of at least 2^-18 of h: (gate, up, first two parts, last part)."""
+    b = lambda v: torch.tensor(float(v), dtype=torch.float64).to(torch.bfloat16).double().item()
+    for g, u in itertools.product(range(2049, 2400, 2), range(2049, 2400, 2)):
+        h = g * u
+        parts = [b(h)]
+        parts.append(b(h - parts[0]))
+        last = h - parts[0] - parts[1]
+        if abs(last) >= h * 2.0 ** -18 and parts[1] != 0:
+            return g, u, parts, last
+    raise AssertionError
+
+
+@pytest.mark.parametrize("dt", list(DT))
+@pytest.mark.parametrize("T", [1, 2, 3, 4, 5, 8, 9, 16])
+@pytest.mark.parametrize("F", [32, 4160])
+def test_hidden_values_enter_the_second_product_with_all_bits(T, F, dt):
+    """Three features that cancel but for the last 8 of 24 bits of the first.  The gates are large enough for
+    silu(gate) = gate, and every number up to the second product is exact.  Two fp16 numbers lose at most 2^-22 of the value;
+    the second product adds a handful of numbers of its size, each sum off by 2^-23 of it at most: 2^-20 together, where a second
+    bf16 part's rest is 2^-18 or more."""
+    g, u, parts, last = _split_hidden_value()
+    d, t = 64, DT[dt]
+    w1, w3 = (torch.zeros(1, F, d, device="cuda") for _ in range(2))
+    w2 = torch.zeros(1, d, F, device="cuda")
+    at = [1, F // 2, F - 1]
+    # tokens are (1, 2^-8) times a power of two: a value of 12 bits is its high part + 256 * low part * 2^-8
+    for w, v in ((w1, g), (w3, u)):
+        w[0, at[0], 0], w[0, at[0], 1] = v // 16 * 16, (v % 16) * 256
+    for i, p in zip(at[1:], parts):
+        m, e = np.frexp(p)          # p = (m * 2^12) * 2^(e - 12): a gate of 2048 and more
+        w1[0, i, 0], w3[0, i, 0] = abs(m) * 4096, np.sign(p) * 2.0 ** (int(e) - 12)
+    w2[0, :, at[0]], w2[0, :, at[1]], w2[0, :, at[2]] = 1, -1, -1
+    w = [v.to(t) for v in (w1, w3, w2)]
+    assert all(torch.equal(a.float(), b) for a, b in zip(w, (w1, w3, w2)))
+    s = torch.exp2((torch.arange(T, device="cuda") % 3).float() - 3)
+    x = torch.zeros(T, d, device="cuda")
+    x[:, 0], x[:, 1] = s, s * 2.0 ** -8
+    y, _, _ = ops.moe_layer_few_tokens(x.to(t), torch.zeros(1, d, device="cuda", dtype=t), *w, 1)
+    want = (last * s.double() ** 2)[:, None].expand(T, d)
+    bound = 2.0 ** -20 * g * u * s.double()[:, None] ** 2 + HALF[t] * want.abs() * 1.01
+    assert (bound < 0.5 * want.abs()).all()
+    assert ((y.double() - want).abs() <= bound).all()
+
+
 @pytest.mark.parametrize("weights", ["fp8", "dense"])
 def test_layer_of_more_than_2_to_the_31_weights(weights):
     """The last of several large experts is what it is as the only one."""
