@@ -72,9 +72,10 @@ constexpr int kJoins = 4;        // tiles whose parts may wait to be joined
 // Hidden values in shared memory at a time: a slice's, if they fit kWholeBytes, else chunks of a multiple of
 // kChunkSteps steps in two buffers of kStageBytes (of 12 steps at least: 96 KB for 16 tokens).  What shared memory
 // takes is missing in L1, through which the weights' loads go: with 200 KB the second kernel read bf16 weights at 4.3
-// TB/s (149 us of 4 tokens, 8 experts of 4096 x 14336), so at 6.2 (103 us).
+// TB/s (149 us of 4 tokens, 8 experts of 4096 x 14336), so at 6.2 (103 us).  Three terms to a value take half as much
+// again, and chunks cost them more than L1 (7 tokens, 64 experts of 1408 x 2048 and two shared: 166 us in chunks, 160 whole).
 constexpr int kChunkSteps = 12;
-constexpr uint32_t kStageBytes = 64 * 1024, kWholeBytes = 128 * 1024;
+constexpr uint32_t kStageBytes = 64 * 1024, kWholeBytes = 128 * 1024, kWholeBytes3 = 176 * 1024;
 constexpr uint32_t kSite = 0x800u;
 constexpr float kInf = __builtin_huge_valf();
 
@@ -1125,7 +1126,7 @@ int launch(FewArgs a, int items, int ctas, bool limited, uint32_t smem1, cudaStr
   const uint32_t step_bytes = (uint32_t)Geo<FP8>::kStep * a.T * 2 * kTermsOf<FP8, X>;
   const int used = (a.E < a.T * a.k ? a.E : a.T * a.k) + a.S;
   const int64_t most = ((int64_t)used * ((a.F + Geo<FP8>::kStep - 1) / Geo<FP8>::kStep) + a.split - 1) / a.split + 1;
-  const bool whole = most * step_bytes <= kWholeBytes;
+  const bool whole = most * step_bytes <= (kTermsOf<FP8, X> == 3 ? kWholeBytes3 : kWholeBytes);
   const int fit = (int)(kStageBytes / step_bytes) / kChunkSteps * kChunkSteps;
   a.chunk = whole ? (int)most : (fit > kChunkSteps ? fit : kChunkSteps);
   a.sums_at = (whole ? 1 : 2) * a.chunk * step_bytes;
