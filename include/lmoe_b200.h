@@ -365,7 +365,8 @@ int lmoe_fp8_grouped_gemm(const uint8_t* xq, const float* xs, int64_t xs_pitch, 
  *   y [num_tokens, hidden_size] of dtype; ids int32, weights fp32 [num_tokens, top_k]
  * Hidden values stay in fp32 between the kernels and enter the second product as a sum of two fp16 numbers (22
  * bits), or with dense bf16 weights of three bf16 numbers; all sums are fp32.  Values below 2^-39 of a token's largest (bf16 tokens with E4M3 weights) or
- * of its largest hidden value over all of its experts (fp16 products) are lost.
+ * of its largest hidden value over all of its experts (fp16 products) are lost, and block scales of 2^84 and more may
+ * overflow the scaled sums.  Routing weights are NaN where the softmax has no value (a logit of +inf, or nothing but -inf).
  * hidden_size % 64 == 0, at most 16384; ffn_size % 32 == 0, at most 65536; num_experts <= 256, top_k <= 16,
  * num_shared <= 16; LMOE_ERR_UNSUPPORTED where eight tokens of that hidden size do not fit shared memory
  * (from about 11000 on for eight).  The result does not depend on timing; should a bounded wait of the kernels ever run

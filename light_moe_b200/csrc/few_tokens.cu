@@ -39,10 +39,11 @@
 // (hidden values over all of its experts), so that the largest lies in [2^14, 2^15); what is 2^-39 of it or smaller is
 // lost.
 //
-// Measured, first / second kernel, us: one token, E4M3, 2 of 8 experts of 4096 x 14336: 49 / 27 (352 MB of weights:
-// 4.6 TB/s over both; the routing, the joins and the two kernels' ramps take 22 us); 4 tokens, bf16, of the same layer,
-// 1.93 GB: 226 / 103, 5.9 TB/s; 16 tokens, E4M3, all 8 experts, 1.41 GB: 230 / 160; one token, fp16, 2 of 8 experts of
-// 1024 x 2816: 12 / 9, which is latency: two launches, a router, three joins.
+// Measured, whole calls, us: one token, E4M3, 2 of 8 experts of 4096 x 14336: 78 (352 MB of weights: 4.5 TB/s; the
+// routing, the joins and the two kernels' ramps take 22 us); 4 tokens, bf16, 5 or 6 experts of the same layer, 1.8-2.1 GB:
+// 309-331, 5.7-6.4 TB/s; 16 tokens, E4M3, all 8 experts, 1.41 GB: 403; one token, fp16, 2 of 8 experts of 1024 x 2816:
+// 22.5, which is latency: two launches, a router, three joins.  First / second kernel apart, from cold caches under a
+// profiler: one token, E4M3 54 / 31; 16 tokens, E4M3 241 / 152; 4 tokens, bf16, 4 experts (1.41 GB) 148 / 91.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -63,8 +64,8 @@ constexpr int kMaxUsed = kMaxExperts + kMaxShared;
 template <bool FP8>
 constexpr int kAheadOf = FP8 ? 3 : 4;
 // The second kernel's warps each read rows of their own, and ask for two or three steps of a row at a time: 128
-// bytes here and there open as many pages of the memory (4 tokens, bf16, the same layer: 130 us of it step by
-// step, 112 so).
+// bytes here and there open as many pages of the memory (4 tokens, bf16, the same layer, when this was chosen: 130 us of it
+// step by step, 112 so).
 constexpr int kRowBlock = kWarps * 16;   // output rows of a CTA of the second kernel
 constexpr int kSplitCtas = 148;  // CTAs that the second kernel's slices aim at: one per SM, whatever the limit of CTAs
 constexpr int kMaxCtas = 256;    // of the first kernel
@@ -72,7 +73,7 @@ constexpr int kJoins = 4;        // tiles whose parts may wait to be joined
 // Hidden values in shared memory at a time: a slice's, if they fit kWholeBytes, else chunks of a multiple of
 // kChunkSteps steps in two buffers of kStageBytes (of 12 steps at least: 96 KB for 16 tokens).  What shared memory
 // takes is missing in L1, through which the weights' loads go: with 200 KB the second kernel read bf16 weights at 4.3
-// TB/s (149 us of 4 tokens, 8 experts of 4096 x 14336), so at 6.2 (103 us).  Three terms to a value take half as much
+// TB/s (149 us of 4 tokens, 8 experts of 4096 x 14336, two terms to a hidden value), so at 6.2 (103 us).  Three terms to a value take half as much
 // again, and chunks cost them more than L1 (7 tokens, 64 experts of 1408 x 2048 and two shared: 166 us in chunks, 160 whole).
 constexpr int kChunkSteps = 12;
 constexpr uint32_t kStageBytes = 64 * 1024, kWholeBytes = 128 * 1024, kWholeBytes3 = 176 * 1024;
@@ -737,7 +738,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) gate_up
 // The terms of a token's hidden values are neighbouring columns.  MODE 0: up to 4 tokens, in every expert's MMAs, whose
 // sums stay in registers for the whole slice.  MODE 1, 2 (up to 8, 16 tokens): of each expert the tokens that chose it, one
 // behind the other in as many MMAs as they fill, whose sums go to the tokens' own in shared memory at the expert's end (with
-// all tokens in every expert's columns, 16 tokens through 8 experts of 4096 x 14336 took this kernel 187 us, now 121).
+// all tokens in every expert's columns, 16 E4M3 tokens through 8 experts of 4096 x 14336 took this kernel 187 us, so 152).
 // CHUNKS: a slice's hidden values do not fit shared memory at once.
 template <bool FP8, typename X, int MODE, bool CHUNKS>
 __global__ void __launch_bounds__(kThreads, 1) down_kernel(const FewArgs a) {

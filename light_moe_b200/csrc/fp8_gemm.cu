@@ -16,10 +16,12 @@
 // half of the columns goes back to its issuer as soon as its four warps have read it.  128 accumulators a thread:
 // the epilogue's two warpgroups take the registers that the other warps give up.
 //
-// What bounds it is that work, not the tensor core: a warp waits for the half, reads 4 x 32 columns, one load after
-// another since two in flight do not fit the registers, and issues 64 paired multiply-adds, and a block takes ~900
-// cycles in all.  16384 rows through 8 experts of 2 x 14336 x 4096, a call by itself: ~2.0 ms, 1.9 PFLOP/s, 0.58 of
-// twice the measured bf16 rate; call after call the power limit lowers the clock (2.39 ms).
+// What bounds it is the chain of a warp, not the tensor core (half of the cycles), and not the multiply-adds (256 cycles
+// of an SM a block): it waits for the half, reads 4 x 32 columns, one load after another since two in flight do not fit
+// the registers, so that each load's latency shows, and issues 64 paired multiply-adds.  A block takes ~1000 cycles in
+// all (3.19 M cycles for a pair's 97 tiles of 32 blocks).  16384 rows through 8 experts of 2 x 14336 x 4096: 1.9 ms in
+// single calls with pauses, 2.0 PFLOP/s, 0.6 of twice the measured bf16 rate; 2.05 ms in 100 calls without, and 2.35 ms
+// in a run of seconds, when the power limit has lowered the clock.
 //
 // The lane being the row, a thread holds a row's gate and up values of the same features, and the
 // SwiGLU needs no exchange: the leader's half of the columns is gate rows and the follower's the
@@ -572,6 +574,10 @@ extern "C" int lmoe_fp8_grouped_gemm(const uint8_t* xq, const float* xs, int64_t
   // the other; 8 experts of 4096 x 14336: 1 93 against 132, 64 134 against 137, 96 172 against 137; of 2 x 14336 x 4096:
   // 1 166 against 252, 64 189 against 255, 96 277 against 257; 64 of 2048 x 1408: 1 50 against 75, 64 73 against 77, 96 89
   // against 77; of 2 x 1408 x 2048: 1 80 against 128, 64 110 against 131, 96 141 against 132).  Both give the same bits.  The counts are on
-  // the device, so the rule takes all rows.
+  // the device, so the rule takes all rows.  Uneven loads do not turn it (all rows, that kernel against the other; 4096 rows, 64
+  // experts of 2 x 1408 x 2048, the most of one expert 425: 113 against 129, 2048: 107 against 129; 512 rows, 8 of 2 x 14336 x
+  // 4096, 106: 209 against 251, 256: 203 against 252; of 4096 x 14336, 106: 127 against 135, 256: 131 against 135), except
+  // where one expert has them all, which reads its weights alone and is a short call either way (4096: 78 against 44; 512:
+  // 145 against 85).
   return total_rows <= (int64_t)num_experts * kFp8DecodeRows ? run_fp8_decode(p, stream) : run_fp8_gemm(p, stream);
 }

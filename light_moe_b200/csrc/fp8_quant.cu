@@ -7,7 +7,8 @@
 // to four): the product reads a block's scales of 128 rows at a time.
 //
 // Matrices are bound by HBM (64 x 1408 x 2048 fp32 there and back 304 us, 1.85 GB: 6.1 TB/s), and so
-// are large calls of rows (32768 x 4096 bf16: 71 us, 5.7 TB/s; 8192 rows 22.5).  Back, 8192 x 4096 to bf16: 16-20 us.
+// are large calls of rows (32768 x 4096 bf16: 71 us, 5.7 TB/s; fp32 115, 5.9 TB/s; 8192 rows bf16 22).  Back, 8192 x 4096
+// to bf16: 16-20 us.  Matrices of 16-bit values, 64 x 1408 x 2048: 119 us, 4.7 TB/s: half the bytes for the same barriers and codes.
 #include <cuda_bf16.h>
 
 #include <type_traits>

@@ -20,9 +20,9 @@ from .layer import HostBufferCalls
 
 # Batches of at most FEW_TOKENS tokens, of a hidden size up to FEW_TOKENS_HIDDEN (where 8 tokens fit shared
 # memory), take the few-token kernels.  Replayed, us, those against the kernels for larger batches: 8 experts of
-# 4096 / 14336, two a token: 1 token 82 against 111, 4 173 against 196, 8 248 against 244, 12 357 against 257; 64 of 2048 /
-# 1408, six a token and two shared: 1 38 against 76, 8 97 against 124, 12 149 against 129; 8 of 1024 / 2816: 8 41 against
-# 50, 12 54 against 52.
+# 4096 / 14336, two a token: 1 token 81 against 107, 4 177 against 193, 8 245 against 238, 12 352 against 256; 64 of 2048 /
+# 1408, six a token and two shared: 1 38 against 76, 8 93 against 123, 12 144 against 131; 8 of 1024 / 2816: 8 39 against
+# 47, 12 53 against 49.
 FEW_TOKENS, FEW_TOKENS_HIDDEN = 8, 8192
 FEW_TOKENS_FFN, FEW_TOKENS_SHARED = 65536, 16   # what those kernels take
 # Experts that the router and one grouped product take.
