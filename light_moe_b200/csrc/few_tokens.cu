@@ -73,8 +73,9 @@ constexpr int kJoins = 4;        // tiles whose parts may wait to be joined
 // Hidden values in shared memory at a time: a slice's, if they fit kWholeBytes, else chunks of a multiple of
 // kChunkSteps steps in two buffers of kStageBytes (of 12 steps at least: 96 KB for 16 tokens).  What shared memory
 // takes is missing in L1, through which the weights' loads go: with 200 KB the second kernel read bf16 weights at 4.3
-// TB/s (149 us of 4 tokens, 8 experts of 4096 x 14336, two terms to a hidden value), so at 6.2 (103 us).  Three terms to a value take half as much
-// again, and chunks cost them more than L1 (7 tokens, 64 experts of 1408 x 2048 and two shared: 166 us in chunks, 160 whole).
+// TB/s (149 us of 4 tokens, 8 experts of 4096 x 14336, two terms to a hidden value), so at 6.2 (103 us).  Three terms to a
+// value take half as much again, and chunks cost them more than L1 does (7 tokens, 64 experts of 1408 x 2048 and two
+// shared: 166 us in chunks, 160 whole).
 constexpr int kChunkSteps = 12;
 constexpr uint32_t kStageBytes = 64 * 1024, kWholeBytes = 128 * 1024, kWholeBytes3 = 176 * 1024;
 constexpr uint32_t kSite = 0x800u;
